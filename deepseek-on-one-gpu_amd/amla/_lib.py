@@ -78,6 +78,27 @@ SIGNATURES = [
     ("amla_sample", c_int, [c_void_p, c_int64, c_int64, c_int64, c_float, c_float, ctypes.c_uint64, c_void_p,
                             c_void_p, c_size_t, c_void_p]),
     ("amla_sample_workspace_bytes", c_size_t, [c_int64, c_int64]),
+    ("amla_mxfp4_quantize", c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    ("amla_mxfp4_quantize_fp8", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    ("amla_mxfp4_dequantize", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    ("amla_mxfp4_linear", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                  c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
+    ("amla_mxfp4_linear_workspace_bytes", c_size_t, [
+        c_int64, c_int64, c_int64, c_int]),
+    ("amla_mxfp4_grouped_linear", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                          c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p,
+                                          c_size_t, c_void_p]),
+    ("amla_mxfp4_grouped_linear_workspace_bytes", c_size_t, [
+        c_int64, c_int64, c_int64, c_int64, c_int]),
+    ("amla_mxfp4_swiglu", c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("amla_mxfp4_swiglu_workspace_bytes", c_size_t, [
+        c_int64, c_int64, c_int64]),
+    ("amla_mxfp4_moe_experts", c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_int, c_void_p, c_size_t, c_void_p]),
+    ("amla_mxfp4_moe_experts_workspace_bytes", c_size_t, [
+        c_int64, c_int64, c_int, c_int64, c_int64]),
     ("amla_moe_combine", c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_float, c_void_p,
                                  c_void_p]),
 ]

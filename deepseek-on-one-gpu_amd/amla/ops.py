@@ -6,7 +6,8 @@ Drop-in for the MLA half of inference/ops.py: ``rms_norm`` (:10-12),
 attention half of ``transformer_layer`` (inference/forward.py:92-94) as
 ``mla_layer``; and the FFN / MoE functions on the same fp8 kernels: ``swiglu``
 (:186-192), ``dense_ffn`` / ``expert_ffn`` (:195-206), ``route`` (:209-257) and
-``moe_block`` (inference/forward.py:112-153, experts handed in).  Same argument
+``moe_block`` (inference/forward.py:112-153, experts handed in); and the same
+linears, FFN and experts for weights held in MXFP4 (``mxfp4_*``).  Same argument
 names, tensor layouts and dtypes; tensors must be
 on a ROCm device.  Every compute call goes to libamla.so; there is no CPU or
 PyTorch fallback (a missing library raises).
@@ -335,13 +336,15 @@ def swiglu(x: torch.Tensor, gate_proj: torch.Tensor, gate_scale: torch.Tensor, u
 
 
 def dense_ffn(hidden: torch.Tensor, mlp_weights: dict) -> torch.Tensor:
-    """inference/ops.py:195-199."""
-    return swiglu(hidden, *mlp_weights["gate_proj"], *mlp_weights["up_proj"], *mlp_weights["down_proj"])
+    """inference/ops.py:195-199; uint8 weights are MXFP4 pairs (``mxfp4_swiglu``)."""
+    fn = mxfp4_swiglu if _is_mxfp4(mlp_weights) else swiglu
+    return fn(hidden, *mlp_weights["gate_proj"], *mlp_weights["up_proj"], *mlp_weights["down_proj"])
 
 
 def expert_ffn(hidden: torch.Tensor, expert_weights: dict) -> torch.Tensor:
-    """inference/ops.py:202-206."""
-    return swiglu(hidden, *expert_weights["gate_proj"], *expert_weights["up_proj"], *expert_weights["down_proj"])
+    """inference/ops.py:202-206; uint8 weights are MXFP4 pairs (``mxfp4_swiglu``)."""
+    fn = mxfp4_swiglu if _is_mxfp4(expert_weights) else swiglu
+    return fn(hidden, *expert_weights["gate_proj"], *expert_weights["up_proj"], *expert_weights["down_proj"])
 
 
 def route(hidden: torch.Tensor, gate_weight: torch.Tensor, config) -> tuple[torch.Tensor, torch.Tensor]:
@@ -432,6 +435,8 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     * a mapping (or a callable) from expert index to its weight dict on the same device;
     * one dict of stacked weights ``{"gate_proj": (w (E, n, k), s (E, ceil(n/128),
       ceil(k/128))), ...}`` (all experts of the layer contiguous: no per-expert host work);
+      with uint8 tensors, stacked MXFP4 weights ``(codes (E, n, k/2), exponents (E, n, k/32))``
+      (``mxfp4_moe_experts``; the shared expert may be of either form);
     * an ``amla.experts.ExpertStreamer`` (with ``layer=``): the chosen experts are streamed
       from host memory in waves of at most the pool size, each wave computed before the
       next one is copied, so any batch runs on any pool (gpu_transfer.py:50-89 plus
@@ -471,6 +476,13 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     if m == 0:
         return out
     dev = hidden.device
+    if stacked and _is_mxfp4(experts):
+        if not device_grouping:
+            raise ValueError("moe_block: MXFP4 experts are grouped on the device only")
+        if experts["gate_proj"][0].shape[0] != E:
+            raise ValueError(f"moe_block: {experts['gate_proj'][0].shape[0]} stacked experts, config says {E}")
+        eout = mxfp4_moe_experts(h2, idx.reshape(m, top_k), experts)
+        return _moe_combine(shared_out, eout, w, m, top_k, d, config, out, hidden)
     if stacked and device_grouping and E <= MOE_DEV_MAX_EXPERTS:
         table, n_inter = _stacked_device_table(experts, E, d, dev)
         eout = torch.empty(m, top_k, d, dtype=BF16, device=dev)
@@ -577,6 +589,232 @@ def _moe_experts_streamed(h2, idx_host, streamer, layer, config) -> torch.Tensor
         _moe_experts_call(h2, idx_w, tables, n_inter, E, eout)
     streamer.release()
     return eout
+
+
+# ------------------------------------------------------------------ MXFP4
+
+MX_BLOCK = 32  # values of a row that share an exponent
+_MX_IN = {BF16: 0, torch.float16: 1, torch.float32: 2}
+_MX_OUT = (BF16, torch.float32)
+
+
+def _is_mxfp4(weights: dict) -> bool:
+    return weights["gate_proj"][0].dtype == torch.uint8
+
+
+def _mx_pair(codes: torch.Tensor, scales: torch.Tensor, name: str, dev=None) -> tuple:
+    """Checks an MXFP4 pair (codes (..., k/2), exponents (..., k/32)) and returns its shape with k."""
+    _need(codes, name, torch.uint8, dev)
+    _need(scales, name + " scale", torch.uint8, codes.device)
+    if codes.dim() == 0 or codes.shape[-1] % (MX_BLOCK // 2):
+        raise ValueError(f"{name}: rows of {tuple(codes.shape)} codes are not blocks of {MX_BLOCK} values")
+    if tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] * 2 // MX_BLOCK):
+        raise ValueError(f"{name} scale: shape {tuple(scales.shape)} does not match codes {tuple(codes.shape)}")
+    return (*codes.shape[:-1], codes.shape[-1] * 2)
+
+
+def _mx_weight(codes, scales, name, shape, dev) -> None:
+    if _mx_pair(codes, scales, name, dev) != tuple(shape):
+        raise ValueError(f"{name}: codes {tuple(codes.shape)}, expected the values of {tuple(shape)}")
+
+
+def _mx_rows(x: torch.Tensor, k: int) -> torch.Tensor:
+    """x as (rows, k) with unit column stride and row strides of whole 16 bytes."""
+    x2 = x.reshape(-1, k)
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and (x2.stride(0) < k or x2.stride(0) % (16 // x.element_size()))):
+        x2 = x2.contiguous()
+    return x2
+
+
+def _mx_x(x, what: str, k: int, dev) -> tuple:
+    """(x or codes as (rows, .), exponents or None, leading shape) of the activations of a product:
+    a bf16 tensor, or the pair that ``mxfp4_quantize`` returned for one."""
+    if isinstance(x, (tuple, list)):
+        if len(x) != 2:
+            raise ValueError(f"{what}: x must be a bfloat16 tensor or a (codes, scales) pair")
+        shape = _mx_pair(x[0], x[1], f"{what}: x", dev)
+        if shape[-1] != k:
+            raise ValueError(f"{what}: x has {shape[-1]} features, weight expects {k}")
+        return x[0].reshape(-1, k // 2), x[1].reshape(-1, k // MX_BLOCK), shape[:-1]
+    _need_cuda(x, "x")
+    if x.dtype != BF16:
+        raise TypeError(f"{what}: x must be bfloat16 (got {x.dtype})")
+    if x.device != dev:
+        raise ValueError(f"{what}: x is on {x.device}, the weight on {dev}")
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f"{what}: x of shape {tuple(x.shape)}, weight expects {k} features")
+    return _mx_rows(x, k), None, x.shape[:-1]
+
+
+def _mx_k(k: int, what: str) -> None:
+    if k == 0 or k % 128:
+        raise ValueError(f"{what}: K = {k} is not a multiple of 128")
+
+
+def _mx_out_dtype(out_dtype, what: str) -> torch.dtype:
+    """The dtype the kernel writes: bf16 rounds in its epilogue, any other is the fp32 result cast."""
+    if not isinstance(out_dtype, torch.dtype) or not (out_dtype.is_floating_point or out_dtype.is_complex):
+        raise TypeError(f"{what}: out_dtype must be a floating-point dtype (got {out_dtype})")
+    return out_dtype if out_dtype == BF16 else torch.float32
+
+
+def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """MXFP4 form of the rows of ``x`` (..., k) bf16, fp16 or fp32, k % 32 == 0: codes uint8
+    (..., k/2), two e2m1 values a byte, the first in its low half, and exponents uint8 (..., k/32),
+    one e8m0 byte per block of 32 values.
+
+    The exponent of a block is floor(log2(max |x|)) - 2 (a block of zeros: byte 0); values are
+    rounded to nearest even and saturate at 6 times the scale.  A block that holds an infinity or
+    a NaN is a block of NaN (byte 255)."""
+    _need_cuda(x, "x")
+    if x.dtype not in _MX_IN:
+        raise TypeError(f"mxfp4_quantize: x must be bfloat16, float16 or float32 (got {x.dtype})")
+    if x.dim() == 0 or x.shape[-1] % MX_BLOCK or x.shape[-1] == 0:
+        raise ValueError(f"mxfp4_quantize: the last dimension of {tuple(x.shape)} is not a multiple of {MX_BLOCK}")
+    k = x.shape[-1]
+    codes, scales = torch_ops.call("mxfp4_quantize", _mx_rows(x, k))
+    return codes.view(*x.shape[:-1], k // 2), scales.view(*x.shape[:-1], k // MX_BLOCK)
+
+
+def mxfp4_quantize_fp8(weight: torch.Tensor, scale_inv: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``mxfp4_quantize(fp8_block_dequant(weight, scale_inv))`` without the fp32 matrix between: the
+    MXFP4 form of a block-FP8 weight (n, k) of the checkpoint, k % 32 == 0."""
+    _need(weight, "weight", FP8)
+    _need(scale_inv, "scale_inv", torch.float32, weight.device)
+    if weight.dim() != 2 or weight.shape[1] % MX_BLOCK or weight.shape[1] == 0:
+        raise ValueError(f"mxfp4_quantize_fp8: weight {tuple(weight.shape)} must be (n, k) with k % {MX_BLOCK} == 0")
+    n, k = weight.shape
+    if scale_inv.shape != (math.ceil(n / 128), math.ceil(k / 128)):
+        raise ValueError(f"scale_inv shape {tuple(scale_inv.shape)} does not match weight {n}x{k}")
+    return torch_ops.call("mxfp4_quantize_fp8", weight, scale_inv)
+
+
+def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = BF16) -> torch.Tensor:
+    """The values of an MXFP4 pair, exact in bf16 and in fp32 (the two out_dtypes)."""
+    shape = _mx_pair(codes, scales, "codes")
+    if out_dtype not in _MX_OUT:
+        raise TypeError(f"mxfp4_dequantize: out_dtype must be bfloat16 or float32 (got {out_dtype})")
+    k = shape[-1]
+    if k == 0:
+        return torch.empty(shape, dtype=out_dtype, device=codes.device)
+    return torch_ops.call("mxfp4_dequantize", codes.view(-1, k // 2), scales.view(-1, k // MX_BLOCK),
+                          out_dtype == torch.float32).view(shape)
+
+
+def mxfp4_linear(x, weight: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = BF16) -> torch.Tensor:
+    """``( x @ mxfp4_dequantize(weight, scale).T ).to(out_dtype)`` on the 4-bit matrix units, the
+    linear (inference/ops.py:15-44) for MXFP4 weights: x rounded to MXFP4 like the weight, exact
+    products, fp32 sums.
+
+    ``x`` (..., k): bf16, quantised in the call, or the ``(codes, scales)`` pair of
+    ``mxfp4_quantize``, for activations that several linears share.  ``weight`` (n, k/2) and
+    ``scale`` (n, k/32) uint8, k % 128 == 0, any n."""
+    wdt = _mx_out_dtype(out_dtype, "mxfp4_linear")
+    shape = _mx_pair(weight, scale, "weight")
+    if len(shape) != 2:
+        raise ValueError("mxfp4_linear: weight must be (n, k/2)")
+    n, k = shape
+    _mx_k(k, "mxfp4_linear")
+    _mx_weight(weight, scale, "weight", shape, weight.device)
+    x2, xs, lead = _mx_x(x, "mxfp4_linear", k, weight.device)
+    y = torch_ops.call("mxfp4_linear", x2, xs, weight, scale, wdt == torch.float32).view(*lead, n)
+    return y if wdt == out_dtype else y.to(out_dtype)
+
+
+def mxfp4_grouped_linear(x, weight: torch.Tensor, scale: torch.Tensor, offsets: torch.Tensor,
+                         out_dtype: torch.dtype = BF16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``mxfp4_linear`` by expert over rows sorted by expert: rows offsets[e] .. offsets[e + 1] - 1 of
+    ``x`` (m, k) times expert e of ``weight`` (E, n, k/2), ``scale`` (E, n, k/32), E <= 1024.
+
+    ``offsets`` (E + 1,) int32 on the device, ascending; groups may be empty.  They are not checked
+    on the host: one above m counts as m, one below its predecessor as that.  Rows of no group are
+    zeros in a new output; with ``out`` ((m, n), bf16 or fp32 as out_dtype says, unit column
+    stride) they stay as they were.  ``x``: as for ``mxfp4_linear``."""
+    wdt = _mx_out_dtype(out_dtype, "mxfp4_grouped_linear")
+    shape = _mx_pair(weight, scale, "weight")
+    if len(shape) != 3:
+        raise ValueError("mxfp4_grouped_linear: weight must be (experts, n, k/2)")
+    E, n, k = shape
+    _mx_k(k, "mxfp4_grouped_linear")
+    dev = weight.device
+    _mx_weight(weight, scale, "weight", shape, dev)
+    if not 0 < E <= 1024 or n == 0:
+        raise ValueError(f"mxfp4_grouped_linear: {E} experts of {n} outputs (1 to 1024 experts)")
+    _need(offsets, "offsets", torch.int32, dev)
+    if tuple(offsets.shape) != (E + 1,):
+        raise ValueError(f"mxfp4_grouped_linear: offsets of shape {tuple(offsets.shape)}, expected ({E + 1},)")
+    x2, xs, lead = _mx_x(x, "mxfp4_grouped_linear", k, dev)
+    if len(lead) != 1:
+        raise ValueError("mxfp4_grouped_linear: x must be (m, k)")
+    if out is None:
+        y = torch_ops.call("mxfp4_grouped_linear", x2, xs, weight, scale, offsets, wdt == torch.float32)
+        return y if wdt == out_dtype else y.to(out_dtype)
+    _need_cuda(out, "out")
+    if out.dtype != out_dtype or out_dtype not in _MX_OUT:
+        raise TypeError(f"mxfp4_grouped_linear: out must be bfloat16 or float32 as out_dtype (got {out.dtype})")
+    if out.device != dev or tuple(out.shape) != (x2.shape[0], n) or (n > 1 and out.stride(1) != 1) or \
+            (out.shape[0] > 1 and out.stride(0) < n):
+        raise ValueError(f"mxfp4_grouped_linear: out must be ({x2.shape[0]}, {n}) on {dev} with rows of unit stride")
+    torch_ops.call("mxfp4_grouped_linear_out", x2, xs, weight, scale, offsets, out)
+    return out
+
+
+def mxfp4_swiglu(x: torch.Tensor, gate_proj: torch.Tensor, gate_scale: torch.Tensor, up_proj: torch.Tensor,
+                 up_scale: torch.Tensor, down_proj: torch.Tensor, down_scale: torch.Tensor) -> torch.Tensor:
+    """``swiglu`` (inference/ops.py:186-192) with MXFP4 weights: silu(gate(x)) * up(x) in fp32,
+    rounded to MXFP4 only, times down_proj.  ``x`` (..., k) bf16; gate_proj, up_proj (n, k/2), their
+    exponents (n, k/32), down_proj (k, n/2), (k, n/32); k and n multiples of 128."""
+    shape = _mx_pair(gate_proj, gate_scale, "gate_proj")
+    if len(shape) != 2:
+        raise ValueError("mxfp4_swiglu: gate_proj must be (intermediate, hidden/2)")
+    n, k = shape
+    _mx_k(k, "mxfp4_swiglu")
+    _mx_k(n, "mxfp4_swiglu")
+    dev = gate_proj.device
+    _mx_weight(gate_proj, gate_scale, "gate_proj", (n, k), dev)
+    _mx_weight(up_proj, up_scale, "up_proj", (n, k), dev)
+    _mx_weight(down_proj, down_scale, "down_proj", (k, n), dev)
+    if isinstance(x, (tuple, list)):
+        raise TypeError("mxfp4_swiglu: x must be a bfloat16 tensor")
+    x2, _, lead = _mx_x(x, "mxfp4_swiglu", k, dev)
+    return torch_ops.call("mxfp4_swiglu", x2, gate_proj, gate_scale, up_proj, up_scale, down_proj,
+                          down_scale).view(*lead, k)
+
+
+def mxfp4_moe_experts(hidden: torch.Tensor, indices: torch.Tensor, experts: dict) -> torch.Tensor:
+    """Routed experts (the loop of inference/forward.py:139-151) with stacked MXFP4 weights: row
+    (t, j) of the result (..., top_k, d) bf16 is ``mxfp4_swiglu(hidden[t], expert indices[t, j])``.
+
+    ``hidden`` (..., d) bf16, ``indices`` (..., top_k) int64 on the device (``route``), ``experts``
+    ``{"gate_proj": (codes (E, n, d/2), exponents (E, n, d/32)), "up_proj": ..., "down_proj":
+    (codes (E, d, n/2), exponents (E, d, n/32))}``, E <= 512, d and n multiples of 128.  The slots
+    are grouped by expert on the device: no host copy, no synchronisation.  A slot whose index is
+    no expert's gives a row of zeros."""
+    _need_cuda(hidden, "hidden")
+    if hidden.dtype != BF16:
+        raise TypeError(f"mxfp4_moe_experts: hidden must be bfloat16 (got {hidden.dtype})")
+    shape = _mx_pair(*experts["gate_proj"], "gate_proj", hidden.device)
+    if len(shape) != 3:
+        raise ValueError("mxfp4_moe_experts: gate_proj must be (experts, intermediate, hidden/2)")
+    E, n, d = shape
+    _mx_k(d, "mxfp4_moe_experts")
+    _mx_k(n, "mxfp4_moe_experts")
+    if not 0 < E <= MOE_DEV_MAX_EXPERTS:
+        raise ValueError(f"mxfp4_moe_experts: {E} experts (1 to {MOE_DEV_MAX_EXPERTS})")
+    for key, want in (("gate_proj", (E, n, d)), ("up_proj", (E, n, d)), ("down_proj", (E, d, n))):
+        _mx_weight(*experts[key], key, want, hidden.device)
+    if hidden.dim() == 0 or hidden.shape[-1] != d:
+        raise ValueError(f"mxfp4_moe_experts: hidden of shape {tuple(hidden.shape)}, the experts expect {d} features")
+    if not isinstance(indices, torch.Tensor) or indices.dtype != torch.int64 or indices.device != hidden.device:
+        raise ValueError("mxfp4_moe_experts: indices must be an int64 tensor on the hidden states' device")
+    if indices.dim() == 0 or indices.shape[:-1] != hidden.shape[:-1] or not 0 < indices.shape[-1] <= 64:
+        raise ValueError(f"mxfp4_moe_experts: indices {tuple(indices.shape)} do not match hidden {tuple(hidden.shape)} "
+                         "with 1 to 64 experts a token")
+    top_k = indices.shape[-1]
+    h2 = _mx_rows(hidden, d)
+    out = torch_ops.call("mxfp4_moe_experts", h2, indices.reshape(-1, top_k).contiguous(), *experts["gate_proj"],
+                         *experts["up_proj"], *experts["down_proj"])
+    return out.view(*hidden.shape[:-1], top_k, d)
 
 
 # ------------------------------------------------------------------ output head

@@ -14,6 +14,9 @@ the op, its output shape and its in-place writes:
   both mutate ``ckv_cache`` and ``kpe_cache`` in place (the cache store of
   inference/ops.py:140-141) and, when given, ``attn_out`` (the per-head output
   before o_proj).
+* ``amla::mxfp4_*``: the MXFP4 operators of amla.ops, which call their
+  implementations directly and the registered operators only under tracing
+  (the dispatch costs as much host time as the rest of a call).
 
 Tensors only, no dicts or dataclasses (the op schema cannot carry them): the
 shims in amla.ops keep the reference's signatures and unpack ``attn_weights``
@@ -231,3 +234,183 @@ def _mla_fake(hidden, *args, **kwargs):
 
 mla_decode.register_fake(_mla_fake)
 mla_prefill.register_fake(_mla_fake)
+
+
+# ------------------------------------------------------------------ MXFP4
+
+_MX_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # AMLA_BF16, AMLA_FP16, AMLA_FP32
+_mx_lib = torch.library.Library("amla", "FRAGMENT")
+_mx_impl: dict = {}
+
+
+def _mx_op(schema: str, fake):
+    """Registers amla::<schema> with its ROCm implementation and its fake one."""
+    def wrap(fn):
+        name = schema.split("(")[0]
+        _mx_lib.define(schema)
+        _mx_lib.impl(name, fn, "CUDA")
+        torch.library.register_fake(f"amla::{name}", fake, lib=_mx_lib)
+        _mx_impl[name] = fn
+        return fn
+    return wrap
+
+
+def call(name: str, *args):
+    """The implementation of amla::<name>, or the operator itself where something traces the call."""
+    if torch.compiler.is_compiling() or any(type(a) is not Tensor for a in args if isinstance(a, Tensor)):
+        return getattr(torch.ops.amla, name)(*args)
+    t = next(a for a in args if isinstance(a, Tensor))
+    if t.device.index == torch.cuda.current_device():
+        return _mx_impl[name](*args)
+    with torch.cuda.device(t.device):
+        return _mx_impl[name](*args)
+
+
+def _mx_fake_pair(x, *_):
+    rows, k = x.shape
+    return (x.new_empty(rows, k // 2, dtype=torch.uint8), x.new_empty(rows, k // 32, dtype=torch.uint8))
+
+
+def _mx_pair_out(rows: int, k: int, dev) -> tuple[Tensor, Tensor]:
+    return (torch.empty(rows, k // 2, dtype=torch.uint8, device=dev),
+            torch.empty(rows, k // 32, dtype=torch.uint8, device=dev))
+
+
+def _mx_ldx(x: Tensor, k: int) -> int:
+    return x.stride(0) if x.shape[0] > 1 else k
+
+
+def _mx_x(x, x_scales):
+    """The activations with the alignment the kernels need (copies of those that lack it)."""
+    if x_scales is not None and x_scales.data_ptr() % 4:
+        x_scales = x_scales.clone()
+    return _rows16(x), x_scales
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+@_mx_op("mxfp4_quantize(Tensor x) -> (Tensor, Tensor)", _mx_fake_pair)
+def _mxfp4_quantize(x):
+    x = _rows16(x)
+    rows, k = x.shape
+    q, s = _mx_pair_out(rows, k, x.device)
+    check(lib().amla_mxfp4_quantize(x.data_ptr(), _MX_CODES[x.dtype], rows, k, _mx_ldx(x, k), q.data_ptr(),
+                                    s.data_ptr(), _stream(x.device)) if rows else 0, "mxfp4_quantize")
+    return q, s
+
+
+@_mx_op("mxfp4_quantize_fp8(Tensor weight, Tensor scale_inv) -> (Tensor, Tensor)", _mx_fake_pair)
+def _mxfp4_quantize_fp8(weight, scale_inv):
+    weight = _rows16(weight)
+    n, k = weight.shape
+    q, s = _mx_pair_out(n, k, weight.device)
+    check(lib().amla_mxfp4_quantize_fp8(weight.data_ptr(), scale_inv.data_ptr(), n, k, q.data_ptr(), s.data_ptr(),
+                                        _stream(weight.device)) if n else 0, "mxfp4_quantize_fp8")
+    return q, s
+
+
+@_mx_op("mxfp4_dequantize(Tensor codes, Tensor scales, bool f32) -> Tensor",
+        lambda codes, scales, f32: codes.new_empty(codes.shape[0], codes.shape[1] * 2,
+                                                   dtype=torch.float32 if f32 else BF16))
+def _mxfp4_dequantize(codes, scales, f32):
+    codes = _rows16(codes)
+    rows, k = codes.shape[0], codes.shape[1] * 2
+    out = torch.empty(rows, k, dtype=torch.float32 if f32 else BF16, device=codes.device)
+    check(lib().amla_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, _MX_CODES[out.dtype],
+                                      out.data_ptr(), _stream(codes.device)) if rows else 0, "mxfp4_dequantize")
+    return out
+
+
+def _mx_linear_fake(x, x_scales, weight, scale, f32):
+    return x.new_empty(x.shape[0], weight.shape[0], dtype=torch.float32 if f32 else BF16)
+
+
+@_mx_op("mxfp4_linear(Tensor x, Tensor? x_scales, Tensor weight, Tensor scale, bool f32) -> Tensor", _mx_linear_fake)
+def _mxfp4_linear(x, x_scales, weight, scale, f32):
+    x, x_scales = _mx_x(x, x_scales)
+    m, n, k = x.shape[0], weight.shape[0], weight.shape[1] * 2
+    y = torch.empty(m, n, dtype=torch.float32 if f32 else BF16, device=x.device)
+    if m == 0 or n == 0:
+        return y
+    L = lib()
+    need = L.amla_mxfp4_linear_workspace_bytes(m, n, k, x_scales is not None)
+    ws = _scratch(x.device, need) if need else None
+    check(L.amla_mxfp4_linear(x.data_ptr(), _ptr(x_scales), m, k, _mx_ldx(x, k), weight.data_ptr(), scale.data_ptr(),
+                              n, y.data_ptr(), _MX_CODES[y.dtype], n, _ptr(ws), need, _stream(x.device)),
+          "mxfp4_linear")
+    return y
+
+
+def _mx_grouped(x, x_scales, weight, scale, offsets, y, clear) -> None:
+    x, x_scales = _mx_x(x, x_scales)
+    m, E, n, k = x.shape[0], weight.shape[0], weight.shape[1], weight.shape[2] * 2
+    if m == 0:
+        return
+    L = lib()
+    need = L.amla_mxfp4_grouped_linear_workspace_bytes(m, n, k, E, x_scales is not None)
+    ws = _scratch(x.device, need)
+    check(L.amla_mxfp4_grouped_linear(x.data_ptr(), _ptr(x_scales), m, k, _mx_ldx(x, k), weight.data_ptr(),
+                                      scale.data_ptr(), n, E, offsets.data_ptr(), y.data_ptr(), _MX_CODES[y.dtype],
+                                      y.stride(0) if m > 1 else n, clear, ws.data_ptr(), ws.numel(),
+                                      _stream(x.device)), "mxfp4_grouped_linear")
+
+
+@_mx_op("mxfp4_grouped_linear(Tensor x, Tensor? x_scales, Tensor weight, Tensor scale, Tensor offsets, bool f32) -> Tensor",
+        lambda x, x_scales, weight, scale, offsets, f32: x.new_empty(x.shape[0], weight.shape[1],
+                                                                     dtype=torch.float32 if f32 else BF16))
+def _mxfp4_grouped_linear(x, x_scales, weight, scale, offsets, f32):
+    y = torch.empty(x.shape[0], weight.shape[1], dtype=torch.float32 if f32 else BF16, device=x.device)
+    _mx_grouped(x, x_scales, weight, scale, offsets, y, 1)
+    return y
+
+
+@_mx_op("mxfp4_grouped_linear_out(Tensor x, Tensor? x_scales, Tensor weight, Tensor scale, Tensor offsets, "
+        "Tensor(a!) out) -> ()", lambda x, x_scales, weight, scale, offsets, out: None)
+def _mxfp4_grouped_linear_out(x, x_scales, weight, scale, offsets, out):
+    _mx_grouped(x, x_scales, weight, scale, offsets, out, 0)
+
+
+@_mx_op("mxfp4_swiglu(Tensor x, Tensor gate_proj, Tensor gate_scale, Tensor up_proj, Tensor up_scale, "
+        "Tensor down_proj, Tensor down_scale) -> Tensor",
+        lambda x, gate_proj, *_: x.new_empty(x.shape[0], x.shape[1]))
+def _mxfp4_swiglu(x, gate_proj, gate_scale, up_proj, up_scale, down_proj, down_scale):
+    x = _rows16(x)
+    m, k = x.shape
+    n = gate_proj.shape[0]
+    y = torch.empty(m, k, dtype=BF16, device=x.device)
+    if m == 0:
+        return y
+    L = lib()
+    need = L.amla_mxfp4_swiglu_workspace_bytes(m, k, n)
+    ws = _scratch(x.device, need)
+    check(L.amla_mxfp4_swiglu(x.data_ptr(), m, k, _mx_ldx(x, k), gate_proj.data_ptr(), gate_scale.data_ptr(),
+                              up_proj.data_ptr(), up_scale.data_ptr(), n, down_proj.data_ptr(), down_scale.data_ptr(),
+                              y.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x.device)), "mxfp4_swiglu")
+    return y
+
+
+_MX_MOE_SLOTS = 65536  # (token, k) slots of one call
+
+
+@_mx_op("mxfp4_moe_experts(Tensor hidden, Tensor indices, Tensor gate_proj, Tensor gate_scale, Tensor up_proj, "
+        "Tensor up_scale, Tensor down_proj, Tensor down_scale) -> Tensor",
+        lambda hidden, indices, *_: hidden.new_empty(hidden.shape[0], indices.shape[1], hidden.shape[1]))
+def _mxfp4_moe_experts(hidden, indices, gate_proj, gate_scale, up_proj, up_scale, down_proj, down_scale):
+    hidden = _rows16(hidden)
+    m, top_k = indices.shape
+    E, n, d = gate_proj.shape[0], gate_proj.shape[1], hidden.shape[1]
+    out = torch.empty(m, top_k, d, dtype=BF16, device=hidden.device)
+    L = lib()
+    step = _MX_MOE_SLOTS // top_k
+    for t in range(0, m, step):
+        c = min(step, m - t)
+        need = L.amla_mxfp4_moe_experts_workspace_bytes(c, d, top_k, n, E)
+        ws = _scratch(hidden.device, need)
+        check(L.amla_mxfp4_moe_experts(hidden[t:].data_ptr(), c, d, _mx_ldx(hidden, d), top_k, indices[t:].data_ptr(),
+                                       n, E, gate_proj.data_ptr(), gate_scale.data_ptr(), up_proj.data_ptr(),
+                                       up_scale.data_ptr(), down_proj.data_ptr(), down_scale.data_ptr(),
+                                       out[t:].data_ptr(), 1, ws.data_ptr(), ws.numel(), _stream(hidden.device)),
+              "mxfp4_moe_experts")
+    return out

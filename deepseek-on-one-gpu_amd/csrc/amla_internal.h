@@ -125,6 +125,11 @@ struct MoeSched {
   int down;               // 0: [gate | up] as two weight segments (n_split = gate rows), 1: down
   const int32_t *rowmap;  // gather (down = 0) or scatter (down = 1)
 };
+// Groups the (token, k) slots by expert on the device and makes such a schedule
+// (ffn_moe.hip, moe_sort_kernel): E <= 512, S <= 65536, entries of at most
+// rows_max rows.  wtab null: every expert of 0 .. E - 1 has its weights.
+int launch_moe_sort(const int64_t *idx, int S, int top_k, int E, int sb, int rows_max, const void *const *wtab,
+                    int32_t *hdr, int32_t *count, int32_t *gather, int32_t *scatter, int32_t *ent, hipStream_t st);
 AMLA_DEV void moe_sched_weights(GemvParams &p, const MoeSched &s, int e) {
   const void *const *t = s.wtab + (s.down ? 4 : 0) * s.E;
   p.w0 = static_cast<const uint8_t *>(t[e]);

@@ -974,7 +974,8 @@ AMLA_DEV int block_scan_incl(int v, int *wsum, int lane, int wave) {
 //               larger groups, skipped slots}, sb = min(tokens, 64): counts of the
 //               routing for the caller, no launch reads them.
 // Slots with a negative index are left out; an index >= E, or an expert with a
-// null or misaligned weight, is left out and counted as skipped.
+// null or misaligned weight (of wtab, when given), is left out and counted as
+// skipped.
 __global__ __launch_bounds__(1024) void moe_sort_kernel(const int64_t *__restrict__ idx, int S, int top_k, int E,
                                                         int sb, int rows_max, const void *const *__restrict__ wtab,
                                                         int32_t *__restrict__ hdr, int32_t *__restrict__ count,
@@ -989,7 +990,7 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int64_t *__restric
   for (int e = tid; e < E; e += 1024) {
     bool ok = true;
 #pragma unroll
-    for (int j = 0; j < 6; ++j) {
+    for (int j = 0; j < (wtab ? 6 : 0); ++j) {
       const uintptr_t a = reinterpret_cast<uintptr_t>(wtab[j * E + e]);
       ok = ok && a != 0 && (a & ((j & 1) ? 3 : 15)) == 0;
     }
@@ -1069,6 +1070,12 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int64_t *__restric
   }
 }
 
+int launch_moe_sort(const int64_t *idx, int S, int top_k, int E, int sb, int rows_max, const void *const *wtab,
+                    int32_t *hdr, int32_t *count, int32_t *gather, int32_t *scatter, int32_t *ent, hipStream_t st) {
+  moe_sort_kernel<<<1, 1024, 0, st>>>(idx, S, top_k, E, sb, rows_max, wtab, hdr, count, gather, scatter, ent);
+  return check_launch("expert schedule");
+}
+
 }  // namespace amla
 
 extern "C" {
@@ -1119,9 +1126,9 @@ int amla_moe_experts_dev(const void *hidden, int64_t m, int64_t d, int top_k, co
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int S = (int)(m * top_k), n = (int)n_inter, D = (int)d, E = (int)n_experts;
   int rc;
-  moe_sort_kernel<<<1, 1024, 0, st>>>(indices, S, top_k, E, (int)std::min<int64_t>(m, 64), L.rows, weight_table, hdr,
-                                      count, gather, scatter, ent);
-  if ((rc = check_launch("moe_experts_dev schedule"))) return rc;
+  if ((rc = launch_moe_sort(indices, S, top_k, E, (int)std::min<int64_t>(m, 64), L.rows, weight_table, hdr, count,
+                            gather, scatter, ent, st)))
+    return rc;
   // h rows (by position) = silu(gate) * up of hidden rows gather[], then
   // expert_out rows scatter[] = down(h)
   const MoeSched gu_s = {weight_table, ent, count, E, 0, gather}, dn_s = {weight_table, ent, count, E, 1, scatter};

@@ -9,6 +9,7 @@
 #include "amla_common.h"
 #include "amla_internal.h"
 #include "gemm_epilogue.h"
+#include "tile_order.h"
 
 namespace amla {
 
@@ -517,25 +518,6 @@ AMLA_DEV void tile_store(const TileArgs &a, const TileSums<NJ> &ts) {
 // the 64 tiles it holds at a time share 8 + 8 tile operands through its L2;
 // with up to 8 row tiles the row tiles of a column tile come together (the
 // weights are then the larger operand).
-constexpr int TL_PANEL = 8;
-
-AMLA_DEV void tile_coords(int t, int n_tiles, int m_tiles, int &nt, int &mt) {
-  if (m_tiles <= TL_PANEL) {
-    nt = t / m_tiles;
-    mt = t - nt * m_tiles;
-    return;
-  }
-  const int per = TL_PANEL * m_tiles, p = t / per, r = t - p * per;
-  const int width = min(TL_PANEL, n_tiles - p * TL_PANEL);
-  mt = r / width;
-  nt = p * TL_PANEL + r - mt * width;
-}
-// logical index of workgroup i of n (or -1): a contiguous run per XCD
-AMLA_DEV int xcd_run(int i, int n) {
-  const int run = (n + 7) >> 3, l = (i & 7) * run + (i >> 3);
-  return (i >> 3) < run && l < n ? l : -1;
-}
-
 template <int MODE, int NJ, bool WIDE>
 AMLA_DEV void tile_linear_body(const GemvParams &p, const TileArgs &a, int n0, int n1, int m0, bool staged,
                                float *partial) {

@@ -280,6 +280,88 @@ size_t amla_moe_experts_dev_workspace_bytes(int64_t m, int64_t d, int top_k, int
 int amla_moe_combine(const void *shared_out, const void *expert_out, const float *weights, int64_t m, int top_k,
                      int64_t d, float routed_scaling_factor, void *out, void *stream);
 
+/* ---- MXFP4 ----
+ *
+ * A matrix row of K values (K % 32 == 0) in MXFP4: K/2 bytes of e2m1 codes
+ * (value 2i in the low half of byte i) and K/32 bytes of e8m0 exponents, one per
+ * block of 32 values: value = e2m1(code) * 2^(byte - 127); byte 255 marks a block
+ * of NaN.  Codes are 16-byte, exponents 4-byte aligned, rows contiguous.  The
+ * reference holds its weights in block-FP8 (inference/ops.py:15-44); these entry
+ * points are the linears, the FFN and the experts for weights of half that size. */
+#define AMLA_BF16 0
+#define AMLA_FP16 1
+#define AMLA_FP32 2
+
+/* Quantises x (rows, k) of dtype AMLA_BF16 / AMLA_FP16 / AMLA_FP32, row stride
+ * ldx elements: the exponent of a block is floor(log2(max |x|)) - 2 clamped to
+ * [-127, 127] (a block of zeros: byte 0), its codes x / 2^exponent rounded to
+ * nearest even, magnitudes above 6 saturating.  A block that holds an infinity or
+ * a NaN gets byte 255 and zero codes.  codes (rows, k/2), scales (rows, k/32).
+ * k % 32 == 0, rows of x 16-byte aligned. */
+int amla_mxfp4_quantize(const void *x, int dtype, int64_t rows, int64_t k, int64_t ldx, void *codes, void *scales,
+                        void *stream);
+
+/* The same for a block-FP8 weight: quantises amla_fp8_block_dequant(weight,
+ * scale_inv) without making it.  weight (n, k) e4m3fn, scale_inv (ceil(n/128),
+ * ceil(k/128)) fp32. */
+int amla_mxfp4_quantize_fp8(const void *weight, const float *scale_inv, int64_t n, int64_t k, void *codes,
+                            void *scales, void *stream);
+
+/* out (rows, k) of dtype AMLA_BF16 or AMLA_FP32 (both hold every value exactly;
+ * magnitudes of 2^128 and above, which the quantiser does not make, become
+ * infinite). */
+int amla_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t k, int dtype, void *out,
+                          void *stream);
+
+/* y (m, n) = x (m, k) @ deq(weight)^T of dtype AMLA_BF16 or AMLA_FP32, row
+ * stride ldy: exact products of the two quantised operands summed in fp32.
+ * x: bf16 rows, stride ldx, with x_scales NULL (quantised as by
+ * amla_mxfp4_quantize), or the codes of such rows with x_scales their exponents
+ * (ldx unused).  weight (n, k/2) codes, scales (n, k/32); k % 128 == 0, any n.
+ * Workspace (16-byte aligned; 0 bytes: NULL) of
+ * amla_mxfp4_linear_workspace_bytes(m, n, k, x_scales != NULL) bytes. */
+int amla_mxfp4_linear(const void *x, const void *x_scales, int64_t m, int64_t k, int64_t ldx, const void *weight,
+                      const void *scales, int64_t n, void *y, int dtype, int64_t ldy, void *workspace,
+                      size_t workspace_bytes, void *stream);
+size_t amla_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int quantized);
+
+/* The same by expert: rows offsets[e] .. offsets[e + 1] - 1 of x times weight e
+ * of (n_experts, n, k/2) codes and (n_experts, n, k/32) exponents.  offsets:
+ * n_experts + 1 int32 in DEVICE memory, from low to high; groups may be empty.
+ * An offset above m counts as m, one below its predecessor as that (a bad list
+ * moves rows to another group or to none, it reads and writes nothing else).
+ * Rows of no group: cleared with clear_rest, else left as they were.
+ * n_experts <= 1024. */
+int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, int64_t k, int64_t ldx,
+                              const void *weight, const void *scales, int64_t n, int64_t n_experts,
+                              const int32_t *offsets, void *y, int dtype, int64_t ldy, int clear_rest,
+                              void *workspace, size_t workspace_bytes, void *stream);
+size_t amla_mxfp4_grouped_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t n_experts, int quantized);
+
+/* swiglu (inference/ops.py:186-192) with MXFP4 weights:
+ *   h = silu(x @ gate^T) * (x @ up^T) in fp32, y = bf16( mxfp4(h) @ down^T )
+ * x (m, k) bf16, row stride ldx, quantised as by amla_mxfp4_quantize; gate_w,
+ * up_w (n, k/2) with exponents (n, k/32); down_w (k, n/2) with (k, n/32); y (m,
+ * k) bf16.  k % 128 == 0, n % 128 == 0. */
+int amla_mxfp4_swiglu(const void *x, int64_t m, int64_t k, int64_t ldx, const void *gate_w, const void *gate_s,
+                      const void *up_w, const void *up_s, int64_t n, const void *down_w, const void *down_s, void *y,
+                      void *workspace, size_t workspace_bytes, void *stream);
+size_t amla_mxfp4_swiglu_workspace_bytes(int64_t m, int64_t k, int64_t n);
+
+/* amla_moe_experts_dev with stacked MXFP4 weights: expert_out[t, j] =
+ * amla_mxfp4_swiglu(hidden[t], expert indices[t, j]), the slots grouped by expert
+ * on the device.  hidden (m, d) bf16, row stride ldh; indices (m, top_k) int64 in
+ * DEVICE memory; gate_w, up_w (n_experts, n_inter, d/2), down_w (n_experts, d,
+ * n_inter/2) with their exponents.  A slot with an index outside 0 .. n_experts -
+ * 1 is skipped: its row is cleared with clear_skipped, else left as it was.
+ * m * top_k <= 65536, n_experts <= 512, top_k <= 64, d % 128 == 0, n_inter % 128
+ * == 0.  Calls that share a workspace must not overlap. */
+int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh, int top_k, const int64_t *indices,
+                           int64_t n_inter, int64_t n_experts, const void *gate_w, const void *gate_s,
+                           const void *up_w, const void *up_s, const void *down_w, const void *down_s,
+                           void *expert_out, int clear_skipped, void *workspace, size_t workspace_bytes, void *stream);
+size_t amla_mxfp4_moe_experts_workspace_bytes(int64_t m, int64_t d, int top_k, int64_t n_inter, int64_t n_experts);
+
 /* ---- output head ---- */
 
 /* The lm_head projection of forward.py:70-72 (hidden.float() @ lm_head_w.float().T):
