@@ -602,48 +602,55 @@ def _is_mxfp4(weights: dict) -> bool:
     return weights["gate_proj"][0].dtype == torch.uint8
 
 
-def _mx_pair(codes: torch.Tensor, scales: torch.Tensor, name: str, dev=None) -> tuple:
-    """Checks an MXFP4 pair (codes (..., k/2), exponents (..., k/32)) and returns its shape with k."""
+def _mx_pair(codes: torch.Tensor, scales: torch.Tensor, name: str, dev=None) -> torch.Size:
+    """Checks an MXFP4 pair (codes (..., k/2), exponents (..., k/32)) and returns the codes' shape."""
     _need(codes, name, torch.uint8, dev)
     _need(scales, name + " scale", torch.uint8, codes.device)
-    if codes.dim() == 0 or codes.shape[-1] % (MX_BLOCK // 2):
-        raise ValueError(f"{name}: rows of {tuple(codes.shape)} codes are not blocks of {MX_BLOCK} values")
-    if tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] * 2 // MX_BLOCK):
-        raise ValueError(f"{name} scale: shape {tuple(scales.shape)} does not match codes {tuple(codes.shape)}")
-    return (*codes.shape[:-1], codes.shape[-1] * 2)
+    shape = codes.shape
+    if not shape or shape[-1] % (MX_BLOCK // 2):
+        raise ValueError(f"{name}: rows of {tuple(shape)} codes are not blocks of {MX_BLOCK} values")
+    if scales.shape != shape[:-1] + (shape[-1] * 2 // MX_BLOCK,):
+        raise ValueError(f"{name} scale: shape {tuple(scales.shape)} does not match codes {tuple(shape)}")
+    return shape
 
 
-def _mx_weight(codes, scales, name, shape, dev) -> None:
-    if _mx_pair(codes, scales, name, dev) != tuple(shape):
-        raise ValueError(f"{name}: codes {tuple(codes.shape)}, expected the values of {tuple(shape)}")
+def _mx_weight(codes, scales, name, dims, dev) -> None:
+    """Checks a pair against the dimensions it has to have, the last one in values."""
+    if _mx_pair(codes, scales, name, dev) != dims[:-1] + (dims[-1] // 2,):
+        raise ValueError(f"{name}: codes {tuple(codes.shape)}, expected the values of {tuple(dims)}")
 
 
 def _mx_rows(x: torch.Tensor, k: int) -> torch.Tensor:
     """x as (rows, k) with unit column stride and row strides of whole 16 bytes."""
-    x2 = x.reshape(-1, k)
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and (x2.stride(0) < k or x2.stride(0) % (16 // x.element_size()))):
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    if x2.is_contiguous():
+        return x2
+    if x2.stride(1) != 1 or x2.stride(0) < k or x2.stride(0) % (16 // x.element_size()):
         x2 = x2.contiguous()
     return x2
 
 
 def _mx_x(x, what: str, k: int, dev) -> tuple:
-    """(x or codes as (rows, .), exponents or None, leading shape) of the activations of a product:
-    a bf16 tensor, or the pair that ``mxfp4_quantize`` returned for one."""
+    """(x or codes as (rows, .), exponents or None, x's shape but for the last) of the activations of
+    a product: a bf16 tensor, or the pair that ``mxfp4_quantize`` returned for one."""
     if isinstance(x, (tuple, list)):
         if len(x) != 2:
             raise ValueError(f"{what}: x must be a bfloat16 tensor or a (codes, scales) pair")
         shape = _mx_pair(x[0], x[1], f"{what}: x", dev)
-        if shape[-1] != k:
-            raise ValueError(f"{what}: x has {shape[-1]} features, weight expects {k}")
+        if shape[-1] * 2 != k:
+            raise ValueError(f"{what}: x has {shape[-1] * 2} features, weight expects {k}")
+        if len(shape) == 2:
+            return x[0], x[1], shape[:-1]
         return x[0].reshape(-1, k // 2), x[1].reshape(-1, k // MX_BLOCK), shape[:-1]
     _need_cuda(x, "x")
     if x.dtype != BF16:
         raise TypeError(f"{what}: x must be bfloat16 (got {x.dtype})")
     if x.device != dev:
         raise ValueError(f"{what}: x is on {x.device}, the weight on {dev}")
-    if x.dim() == 0 or x.shape[-1] != k:
-        raise ValueError(f"{what}: x of shape {tuple(x.shape)}, weight expects {k} features")
-    return _mx_rows(x, k), None, x.shape[:-1]
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"{what}: x of shape {tuple(shape)}, weight expects {k} features")
+    return _mx_rows(x, k), None, shape[:-1]
 
 
 def _mx_k(k: int, what: str) -> None:
@@ -673,6 +680,8 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"mxfp4_quantize: the last dimension of {tuple(x.shape)} is not a multiple of {MX_BLOCK}")
     k = x.shape[-1]
     codes, scales = torch_ops.call("mxfp4_quantize", _mx_rows(x, k))
+    if x.dim() == 2:
+        return codes, scales
     return codes.view(*x.shape[:-1], k // 2), scales.view(*x.shape[:-1], k // MX_BLOCK)
 
 
@@ -694,11 +703,14 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch
     shape = _mx_pair(codes, scales, "codes")
     if out_dtype not in _MX_OUT:
         raise TypeError(f"mxfp4_dequantize: out_dtype must be bfloat16 or float32 (got {out_dtype})")
-    k = shape[-1]
+    f32 = out_dtype == torch.float32
+    if len(shape) == 2:
+        return torch_ops.call("mxfp4_dequantize", codes, scales, f32)
+    k = shape[-1] * 2
     if k == 0:
-        return torch.empty(shape, dtype=out_dtype, device=codes.device)
-    return torch_ops.call("mxfp4_dequantize", codes.view(-1, k // 2), scales.view(-1, k // MX_BLOCK),
-                          out_dtype == torch.float32).view(shape)
+        return torch.empty(*shape[:-1], 0, dtype=out_dtype, device=codes.device)
+    y = torch_ops.call("mxfp4_dequantize", codes.view(-1, k // 2), scales.view(-1, k // MX_BLOCK), f32)
+    return y.view(*shape[:-1], k)
 
 
 def mxfp4_linear(x, weight: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = BF16) -> torch.Tensor:
@@ -713,11 +725,12 @@ def mxfp4_linear(x, weight: torch.Tensor, scale: torch.Tensor, out_dtype: torch.
     shape = _mx_pair(weight, scale, "weight")
     if len(shape) != 2:
         raise ValueError("mxfp4_linear: weight must be (n, k/2)")
-    n, k = shape
+    n, k = shape[0], shape[1] * 2
     _mx_k(k, "mxfp4_linear")
-    _mx_weight(weight, scale, "weight", shape, weight.device)
     x2, xs, lead = _mx_x(x, "mxfp4_linear", k, weight.device)
-    y = torch_ops.call("mxfp4_linear", x2, xs, weight, scale, wdt == torch.float32).view(*lead, n)
+    y = torch_ops.call("mxfp4_linear", x2, xs, weight, scale, wdt == torch.float32)
+    if len(lead) != 1:
+        y = y.view(*lead, n)
     return y if wdt == out_dtype else y.to(out_dtype)
 
 
@@ -734,10 +747,9 @@ def mxfp4_grouped_linear(x, weight: torch.Tensor, scale: torch.Tensor, offsets: 
     shape = _mx_pair(weight, scale, "weight")
     if len(shape) != 3:
         raise ValueError("mxfp4_grouped_linear: weight must be (experts, n, k/2)")
-    E, n, k = shape
+    E, n, k = shape[0], shape[1], shape[2] * 2
     _mx_k(k, "mxfp4_grouped_linear")
     dev = weight.device
-    _mx_weight(weight, scale, "weight", shape, dev)
     if not 0 < E <= 1024 or n == 0:
         raise ValueError(f"mxfp4_grouped_linear: {E} experts of {n} outputs (1 to 1024 experts)")
     _need(offsets, "offsets", torch.int32, dev)
@@ -767,18 +779,17 @@ def mxfp4_swiglu(x: torch.Tensor, gate_proj: torch.Tensor, gate_scale: torch.Ten
     shape = _mx_pair(gate_proj, gate_scale, "gate_proj")
     if len(shape) != 2:
         raise ValueError("mxfp4_swiglu: gate_proj must be (intermediate, hidden/2)")
-    n, k = shape
+    n, k = shape[0], shape[1] * 2
     _mx_k(k, "mxfp4_swiglu")
     _mx_k(n, "mxfp4_swiglu")
     dev = gate_proj.device
-    _mx_weight(gate_proj, gate_scale, "gate_proj", (n, k), dev)
     _mx_weight(up_proj, up_scale, "up_proj", (n, k), dev)
     _mx_weight(down_proj, down_scale, "down_proj", (k, n), dev)
     if isinstance(x, (tuple, list)):
         raise TypeError("mxfp4_swiglu: x must be a bfloat16 tensor")
     x2, _, lead = _mx_x(x, "mxfp4_swiglu", k, dev)
-    return torch_ops.call("mxfp4_swiglu", x2, gate_proj, gate_scale, up_proj, up_scale, down_proj,
-                          down_scale).view(*lead, k)
+    y = torch_ops.call("mxfp4_swiglu", x2, gate_proj, gate_scale, up_proj, up_scale, down_proj, down_scale)
+    return y if len(lead) == 1 else y.view(*lead, k)
 
 
 def mxfp4_moe_experts(hidden: torch.Tensor, indices: torch.Tensor, experts: dict) -> torch.Tensor:
@@ -796,13 +807,13 @@ def mxfp4_moe_experts(hidden: torch.Tensor, indices: torch.Tensor, experts: dict
     shape = _mx_pair(*experts["gate_proj"], "gate_proj", hidden.device)
     if len(shape) != 3:
         raise ValueError("mxfp4_moe_experts: gate_proj must be (experts, intermediate, hidden/2)")
-    E, n, d = shape
+    E, n, d = shape[0], shape[1], shape[2] * 2
     _mx_k(d, "mxfp4_moe_experts")
     _mx_k(n, "mxfp4_moe_experts")
     if not 0 < E <= MOE_DEV_MAX_EXPERTS:
         raise ValueError(f"mxfp4_moe_experts: {E} experts (1 to {MOE_DEV_MAX_EXPERTS})")
-    for key, want in (("gate_proj", (E, n, d)), ("up_proj", (E, n, d)), ("down_proj", (E, d, n))):
-        _mx_weight(*experts[key], key, want, hidden.device)
+    _mx_weight(*experts["up_proj"], "up_proj", (E, n, d), hidden.device)
+    _mx_weight(*experts["down_proj"], "down_proj", (E, d, n), hidden.device)
     if hidden.dim() == 0 or hidden.shape[-1] != d:
         raise ValueError(f"mxfp4_moe_experts: hidden of shape {tuple(hidden.shape)}, the experts expect {d} features")
     if not isinstance(indices, torch.Tensor) or indices.dtype != torch.int64 or indices.device != hidden.device:
@@ -812,9 +823,10 @@ def mxfp4_moe_experts(hidden: torch.Tensor, indices: torch.Tensor, experts: dict
                          "with 1 to 64 experts a token")
     top_k = indices.shape[-1]
     h2 = _mx_rows(hidden, d)
-    out = torch_ops.call("mxfp4_moe_experts", h2, indices.reshape(-1, top_k).contiguous(), *experts["gate_proj"],
-                         *experts["up_proj"], *experts["down_proj"])
-    return out.view(*hidden.shape[:-1], top_k, d)
+    idx = indices if indices.dim() == 2 else indices.reshape(-1, top_k)
+    out = torch_ops.call("mxfp4_moe_experts", h2, idx.contiguous(), *experts["gate_proj"], *experts["up_proj"],
+                         *experts["down_proj"])
+    return out if hidden.dim() == 2 else out.view(*hidden.shape[:-1], top_k, d)
 
 
 # ------------------------------------------------------------------ output head

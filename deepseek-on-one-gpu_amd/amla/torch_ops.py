@@ -30,6 +30,7 @@ never share scratch.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -255,15 +256,25 @@ def _mx_op(schema: str, fake):
     return wrap
 
 
-def call(name: str, *args):
+def call(name: str, t: Tensor, *args):
     """The implementation of amla::<name>, or the operator itself where something traces the call."""
-    if torch.compiler.is_compiling() or any(type(a) is not Tensor for a in args if isinstance(a, Tensor)):
-        return getattr(torch.ops.amla, name)(*args)
-    t = next(a for a in args if isinstance(a, Tensor))
+    if type(t) is not Tensor and not isinstance(t, torch.nn.Parameter) or torch.compiler.is_compiling():
+        return getattr(torch.ops.amla, name)(t, *args)
     if t.device.index == torch.cuda.current_device():
-        return _mx_impl[name](*args)
+        return _mx_impl[name](t, *args)
     with torch.cuda.device(t.device):
-        return _mx_impl[name](*args)
+        return _mx_impl[name](t, *args)
+
+
+# (the workspaces' sizes are functions of the call's sizes alone)
+_mx_linear_bytes = lru_cache(4096)(lambda *a: lib().amla_mxfp4_linear_workspace_bytes(*a))
+_mx_grouped_bytes = lru_cache(4096)(lambda *a: lib().amla_mxfp4_grouped_linear_workspace_bytes(*a))
+_mx_swiglu_bytes = lru_cache(4096)(lambda *a: lib().amla_mxfp4_swiglu_workspace_bytes(*a))
+_mx_moe_bytes = lru_cache(4096)(lambda *a: lib().amla_mxfp4_moe_experts_workspace_bytes(*a))
+
+
+def _mx_stream(t: Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _mx_fake_pair(x, *_):
@@ -297,7 +308,7 @@ def _mxfp4_quantize(x):
     rows, k = x.shape
     q, s = _mx_pair_out(rows, k, x.device)
     check(lib().amla_mxfp4_quantize(x.data_ptr(), _MX_CODES[x.dtype], rows, k, _mx_ldx(x, k), q.data_ptr(),
-                                    s.data_ptr(), _stream(x.device)) if rows else 0, "mxfp4_quantize")
+                                    s.data_ptr(), _mx_stream(x)) if rows else 0, "mxfp4_quantize")
     return q, s
 
 
@@ -307,7 +318,7 @@ def _mxfp4_quantize_fp8(weight, scale_inv):
     n, k = weight.shape
     q, s = _mx_pair_out(n, k, weight.device)
     check(lib().amla_mxfp4_quantize_fp8(weight.data_ptr(), scale_inv.data_ptr(), n, k, q.data_ptr(), s.data_ptr(),
-                                        _stream(weight.device)) if n else 0, "mxfp4_quantize_fp8")
+                                        _mx_stream(weight)) if n else 0, "mxfp4_quantize_fp8")
     return q, s
 
 
@@ -319,7 +330,7 @@ def _mxfp4_dequantize(codes, scales, f32):
     rows, k = codes.shape[0], codes.shape[1] * 2
     out = torch.empty(rows, k, dtype=torch.float32 if f32 else BF16, device=codes.device)
     check(lib().amla_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, _MX_CODES[out.dtype],
-                                      out.data_ptr(), _stream(codes.device)) if rows else 0, "mxfp4_dequantize")
+                                      out.data_ptr(), _mx_stream(codes)) if rows else 0, "mxfp4_dequantize")
     return out
 
 
@@ -335,10 +346,10 @@ def _mxfp4_linear(x, x_scales, weight, scale, f32):
     if m == 0 or n == 0:
         return y
     L = lib()
-    need = L.amla_mxfp4_linear_workspace_bytes(m, n, k, x_scales is not None)
+    need = _mx_linear_bytes(m, n, k, x_scales is not None)
     ws = _scratch(x.device, need) if need else None
     check(L.amla_mxfp4_linear(x.data_ptr(), _ptr(x_scales), m, k, _mx_ldx(x, k), weight.data_ptr(), scale.data_ptr(),
-                              n, y.data_ptr(), _MX_CODES[y.dtype], n, _ptr(ws), need, _stream(x.device)),
+                              n, y.data_ptr(), _MX_CODES[y.dtype], n, _ptr(ws), need, _mx_stream(x)),
           "mxfp4_linear")
     return y
 
@@ -349,12 +360,12 @@ def _mx_grouped(x, x_scales, weight, scale, offsets, y, clear) -> None:
     if m == 0:
         return
     L = lib()
-    need = L.amla_mxfp4_grouped_linear_workspace_bytes(m, n, k, E, x_scales is not None)
+    need = _mx_grouped_bytes(m, n, k, E, x_scales is not None)
     ws = _scratch(x.device, need)
     check(L.amla_mxfp4_grouped_linear(x.data_ptr(), _ptr(x_scales), m, k, _mx_ldx(x, k), weight.data_ptr(),
                                       scale.data_ptr(), n, E, offsets.data_ptr(), y.data_ptr(), _MX_CODES[y.dtype],
                                       y.stride(0) if m > 1 else n, clear, ws.data_ptr(), ws.numel(),
-                                      _stream(x.device)), "mxfp4_grouped_linear")
+                                      _mx_stream(x)), "mxfp4_grouped_linear")
 
 
 @_mx_op("mxfp4_grouped_linear(Tensor x, Tensor? x_scales, Tensor weight, Tensor scale, Tensor offsets, bool f32) -> Tensor",
@@ -383,11 +394,11 @@ def _mxfp4_swiglu(x, gate_proj, gate_scale, up_proj, up_scale, down_proj, down_s
     if m == 0:
         return y
     L = lib()
-    need = L.amla_mxfp4_swiglu_workspace_bytes(m, k, n)
+    need = _mx_swiglu_bytes(m, k, n)
     ws = _scratch(x.device, need)
     check(L.amla_mxfp4_swiglu(x.data_ptr(), m, k, _mx_ldx(x, k), gate_proj.data_ptr(), gate_scale.data_ptr(),
                               up_proj.data_ptr(), up_scale.data_ptr(), n, down_proj.data_ptr(), down_scale.data_ptr(),
-                              y.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x.device)), "mxfp4_swiglu")
+                              y.data_ptr(), ws.data_ptr(), ws.numel(), _mx_stream(x)), "mxfp4_swiglu")
     return y
 
 
@@ -406,11 +417,11 @@ def _mxfp4_moe_experts(hidden, indices, gate_proj, gate_scale, up_proj, up_scale
     step = _MX_MOE_SLOTS // top_k
     for t in range(0, m, step):
         c = min(step, m - t)
-        need = L.amla_mxfp4_moe_experts_workspace_bytes(c, d, top_k, n, E)
+        need = _mx_moe_bytes(c, d, top_k, n, E)
         ws = _scratch(hidden.device, need)
         check(L.amla_mxfp4_moe_experts(hidden[t:].data_ptr(), c, d, _mx_ldx(hidden, d), top_k, indices[t:].data_ptr(),
                                        n, E, gate_proj.data_ptr(), gate_scale.data_ptr(), up_proj.data_ptr(),
                                        up_scale.data_ptr(), down_proj.data_ptr(), down_scale.data_ptr(),
-                                       out[t:].data_ptr(), 1, ws.data_ptr(), ws.numel(), _stream(hidden.device)),
+                                       out[t:].data_ptr(), 1, ws.data_ptr(), ws.numel(), _mx_stream(hidden)),
               "mxfp4_moe_experts")
     return out

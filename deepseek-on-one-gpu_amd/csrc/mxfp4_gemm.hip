@@ -11,15 +11,13 @@
 
 namespace amla {
 
-constexpr int MX_ROWS = 128;         // activation rows of a tile
 constexpr int MX_MAX_GROUPS = 1024;  // experts of a grouped product
 
 // Operands of a launch.  Two weights (SILU): gate and up.  ent (with count): the
-// schedule entries (expert, first position, rows, -), expert -1 for rows to clear;
-// null: one entry of M rows.  Position p reads x row xrow[p] and writes y row
+// schedule entries (expert, first position, rows, -); null: one entry of M rows.  Position p reads x row xrow[p] and writes y row
 // yrow[p] (null: p).
 struct MxParams {
-  const void *x;       // codes, or bf16 values (xs null; skinny only)
+  const void *x;       // codes, or bf16 values (xs null; stream product only)
   const uint8_t *xs;
   int64_t ldx;         // bf16 row stride
   const int32_t *xrow, *yrow;
@@ -27,11 +25,14 @@ struct MxParams {
   int64_t wstride, sstride;  // bytes from expert to expert
   const int32_t *ent, *count;
   int M, N, K;
+  int rest;            // count[1] entries of expert -1 come behind the others
   void *y;
   int64_t ldy;
   int f32, vec;        // fp32 outputs; four outputs per store
   uint8_t *hc, *hs;    // SILU: codes and exponents by position
 };
+
+AMLA_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 AMLA_DEV void mx_store4(const MxParams &p, int64_t row, int n, f32x4 v) {
   if (p.f32) {
@@ -49,346 +50,648 @@ AMLA_DEV void mx_store4(const MxParams &p, int64_t row, int n, f32x4 v) {
 
 AMLA_DEV float mx_silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
 
-// ---------------------------------------------------------------- skinny product
+// ---------------------------------------------------------------- stream product
 
-// Up to 16 XT activation rows by 16 WT weight rows per workgroup; the waves take
-// runs of the 128-wide K steps and meet in LDS, in wave order.  Weights and
-// activations go from memory straight into the operands' registers: 16 rows x 64
-// bytes per load, four steps at a time, the exponents of four steps in one 16-byte
-// load per row (the lanes of a row share it).  FUSED: bf16 rows, quantised in the
-// registers (a lane holds whole blocks), which saves the pass and the launch
-// before it.
-template <int WT, int XT, bool FUSED, bool SILU>
-__global__ __launch_bounds__(512) void mx_skinny_kernel(MxParams p, int ntiles) {
-  extern __shared__ __align__(16) float red[];
+// Few activation rows: the weights stream once, from memory straight into the
+// operands' registers, past activations that stay in LDS.
+//
+// An item is 16 weight rows (SILU: 32 of gate and the same 32 of up) of an entry; a
+// workgroup takes a contiguous run of items.  Its waves share the K of every weight
+// row by runs of quads (512 K values) and meet in LDS, in wave order.  A wave walks
+// the quads of all its items as one sequence, with the next quad's loads in flight
+// while it multiplies one, also across items; a load is 16 rows x 64 bytes, a quad
+// 16 bytes of exponents a row more (the lanes of a row share them).
+//
+// Activations: rows of one entry (at most `mr`, a power of two, or 16 XT), bf16 ones
+// quantised on the way in, which saves the pass and the launch before it.  Codes at
+// [step][fragment][K block][row], so that the lanes of a fragment read 16 rows in a
+// row; exponents as dwords of the quad's four steps, which the MFMAs select by number.
+struct MxStream {
+  int ntiles;      // items of an entry
+  int mr;          // activation rows kept of a fragment
+  int xcodes;      // bytes of the codes, and
+  int xbytes;      // with the exponents (the partial sums come behind)
+};
+
+template <int XT, bool SILU, bool PLANES>
+__global__ __launch_bounds__(512) void mx_stream_kernel(MxParams p, MxStream sp) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  constexpr int WT = SILU ? 4 : 1;  // 16-row fragments of an item
+  constexpr int COLS = SILU ? 32 : 16;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
-  const int en = blockIdx.x / ntiles, nt = blockIdx.x - en * ntiles;
-  int e = 0, r0 = 0, rows = p.M;
-  if (p.ent) {
-    if (en >= *p.count) return;
-    e = p.ent[4 * en];
-    r0 = p.ent[4 * en + 1];
-    rows = p.ent[4 * en + 2];
-  }
-  constexpr int COLS = SILU ? 8 * WT : 16 * WT;  // outputs of the workgroup
-  if (!SILU && e < 0) {  // rows of no expert
-    for (int i = tid; i < rows * 4 * WT; i += blockDim.x) {
-      const int r = i / (4 * WT), n = nt * COLS + 4 * (i - r * 4 * WT);
-      if (n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + r] : r0 + r, n, f32x4{0.f, 0.f, 0.f, 0.f});
-    }
-    return;
-  }
+  const int steps = p.K >> 7, quads = (steps + 3) >> 2;
+  const int q0 = quads * wave / nw, q1 = quads * (wave + 1) / nw;
   const int64_t kb = p.K >> 1, ksb = p.K >> 5;
-  const uint8_t *wp[WT], *sp[WT];
-#pragma unroll
-  for (int t = 0; t < WT; ++t) {
-    const int seg = SILU && t >= WT / 2 ? 1 : 0;
-    const int n = min(nt * COLS + 16 * (SILU ? t % (WT / 2) : t) + r16, p.N - 1);  // rows past N repeat the last
-    wp[t] = p.w[seg] + e * p.wstride + n * kb + 16 * g;
-    sp[t] = p.ws[seg] + e * p.sstride + n * ksb;
-  }
-  const uint8_t *xp[XT], *xsp[XT];
-  bool act[XT];
-#pragma unroll
-  for (int j = 0; j < XT; ++j) {
-    act[j] = 16 * j + r16 < rows;
-    const int pos = r0 + min(16 * j + r16, rows - 1);
-    const int64_t xr = p.xrow ? p.xrow[pos] : pos;
-    xp[j] = static_cast<const uint8_t *>(p.x) + (FUSED ? xr * p.ldx * 2 + 64 * g : xr * kb + 16 * g);
-    xsp[j] = FUSED ? nullptr : p.xs + xr * ksb;
-  }
-  f32x4 acc[WT][XT];
-#pragma unroll
-  for (int t = 0; t < WT; ++t)
-#pragma unroll
-    for (int j = 0; j < XT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int steps = p.K >> 7, s1 = steps * (wave + 1) / nw;
-  // one run of U steps from step s
-  auto run = [&](int s, auto u_c) {
-    constexpr int U = decltype(u_c)::value;
-    u32x4 wc[U][WT], xc[U][XT], xraw[FUSED ? U : 1][FUSED ? 4 : 1];
-    uint32_t wsc[WT][U], xsc[XT][U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int t = 0; t < WT; ++t) wc[u][t] = ldg16_nt(wp[t] + (int64_t)(s + u) * 64);
-#pragma unroll
-    for (int t = 0; t < WT; ++t) {
-      if constexpr (U == 4) {
-        const u32x4_a4 v = *reinterpret_cast<const u32x4_a4 *>(sp[t] + s * 4);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) wsc[t][u] = v[u];
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) wsc[t][u] = *reinterpret_cast<const uint32_t *>(sp[t] + (s + u) * 4);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < XT; ++j) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        xc[u][j] = u32x4{0, 0, 0, 0};
-        xsc[j][u] = 0;
-      }
-      if (act[j]) {
-        if constexpr (FUSED) {
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            u16x2 am = {0, 0};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) xraw[u][q] = ldg16(xp[j] + (int64_t)(s + u) * 256 + 16 * q);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) am = mx_absmax(am, xraw[u][q]);
-            const uint32_t byte = mx_byte(mx_amax_bits(am));
-            const float sc = mx_scale(byte);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) xc[u][j][q] = mx_codes8(xraw[u][q], sc);
-            xsc[j][u] = byte << (8 * g);
-          }
-        } else {
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            xc[u][j] = ldg16(xp[j] + (int64_t)(s + u) * 64);
-            xsc[j][u] = *reinterpret_cast<const uint32_t *>(xsp[j] + (s + u) * 4);
-          }
+  // (scalar loads: a vector load among the weights' would be waited for with them)
+  typedef const __attribute__((address_space(4))) int32_t *sptr;
+  const sptr ent = (sptr)p.ent;
+  const int entries = p.ent ? *(sptr)p.count : 1;
+  const int64_t total = (int64_t)entries * sp.ntiles;
+  const int64_t i0 = total * blockIdx.x / gridDim.x, i1 = total * (blockIdx.x + 1) / gridDim.x;
+  if constexpr (!SILU)
+    if (p.rest) {  // rows of no expert
+      const int rest = p.count[1];
+      for (int en = blockIdx.x; en < rest; en += gridDim.x) {
+        const int r0 = p.ent[4 * (entries + en) + 1], rows = p.ent[4 * (entries + en) + 2], n4 = (p.N + 3) >> 2;
+        for (int i = tid; i < rows * n4; i += blockDim.x) {
+          const int r = i / n4;
+          mx_store4(p, p.yrow ? p.yrow[r0 + r] : r0 + r, 4 * (i - r * n4), f32x4{0.f, 0.f, 0.f, 0.f});
         }
       }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int t = 0; t < WT; ++t)
-#pragma unroll
-        for (int j = 0; j < XT; ++j)
-          acc[t][j] = mfma_mx<0>(wc[u][t], wsc[t][u] >> (8 * g), xc[u][j], xsc[j][u] >> (8 * g), acc[t][j]);
-  };
-  int s = steps * wave / nw;
-  for (; s + 4 <= s1; s += 4) run(s, std::integral_constant<int, 4>{});
-  for (; s < s1; ++s) run(s, std::integral_constant<int, 1>{});
+  if (i0 >= i1) return;
 
-  f32x4 *part = reinterpret_cast<f32x4 *>(red);
-#pragma unroll
-  for (int t = 0; t < WT; ++t)
-#pragma unroll
-    for (int j = 0; j < XT; ++j) part[((wave * WT + t) * XT + j) * 64 + lane] = acc[t][j];
-  __syncthreads();
-  auto total = [&](int t, int j, int l) {
-    f32x4 v = part[(t * XT + j) * 64 + l];
-    for (int w = 1; w < nw; ++w) v += part[((w * WT + t) * XT + j) * 64 + l];
-    return v;
+  // the sequence of the loads, one quad ahead of the multiplications
+  struct Loads {
+    u32x4 w[4], s;
   };
-  if constexpr (SILU) {
-    // eight lanes hold a block of 32 outputs of a row: four each
-    for (int i = tid; i < XT * 16 * 2 * WT; i += blockDim.x) {
-      const int c = i % (2 * WT), m = i / (2 * WT), t = c >> 2;
-      const int j = m >> 4, l = (c & 3) * 16 + (m & 15);
-      const f32x4 gt = total(t, j, l), up = total(t + WT / 2, j, l);
-      float h[4];
-      uint32_t am = 0;
+  int64_t ni = i0;
+  int nsub = 0, nq = q0;
+  const uint8_t *nw_p, *ns_p;
+  auto row_of = [&](int64_t item, int sub) {  // the lane's weight row
+    const int en = (int)(item / sp.ntiles), t = (int)(item - (int64_t)en * sp.ntiles);
+    const int e = p.ent ? ent[4 * uniform(en)] : 0;
+    const int seg = SILU && sub >= 2;
+    const int n = min(t * COLS + 16 * (SILU ? sub & 1 : 0) + r16, p.N - 1);  // rows past N repeat the last
+    nw_p = (seg ? p.w[1] : p.w[0]) + e * p.wstride + n * kb + 16 * g;
+    ns_p = (seg ? p.ws[1] : p.ws[0]) + e * p.sstride + n * ksb;
+  };
+  row_of(ni, 0);
+  auto load = [&](Loads &l) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        h[q] = mx_silu_mul(gt[q], up[q]);
-        am = max(am, __float_as_uint(h[q]) & 0x7fffffffu);
+    for (int u = 0; u < 4; ++u) l.w[u] = ldg16(nw_p + (int64_t)(PLANES ? min(4 * nq + u, steps - 1) : 4 * nq + u) * 64);
+    if constexpr (!PLANES) {
+      l.s = *reinterpret_cast<const u32x4_a4 *>(ns_p + nq * 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) l.s[u] = *reinterpret_cast<const uint32_t *>(ns_p + min(4 * nq + u, steps - 1) * 4);
+    }
+    if (++nq == q1) {
+      nq = q0;
+      if (++nsub == WT) {
+        nsub = 0;
+        ++ni;
       }
-      am = max(am, dpp_u32<0xB1>(am));   // quad_perm [1,0,3,2]
-      am = max(am, dpp_u32<0x4E>(am));   // quad_perm [2,3,0,1]
-      am = max(am, dpp_u32<0x141>(am));  // row_half_mirror
-      const uint32_t byte = mx_byte(am);
-      const float sc = mx_scale(byte);
-      uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, h[0], h[1], sc, 0);
-      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, h[2], h[3], sc, 1);
-      if (byte == 255) q = 0;
-      const int n = nt * COLS + 4 * c;
-      if (m < rows) {
-        *reinterpret_cast<uint16_t *>(p.hc + (int64_t)(r0 + m) * (p.N >> 1) + (n >> 1)) = (uint16_t)q;
-        if ((c & 7) == 0) p.hs[(int64_t)(r0 + m) * (p.N >> 5) + (n >> 5)] = (uint8_t)byte;
+      if (ni < i1) row_of(ni, nsub);  // (past the end: the last row again, not multiplied)
+    }
+  };
+  const int mr = sp.mr;
+  int rows = 0, r0 = 0;
+  auto fill = [&](int en) {  // the activations of an entry
+    rows = p.M;
+    if (p.ent) {
+      r0 = ent[4 * uniform(en) + 1];
+      rows = ent[4 * uniform(en) + 2];
+    }
+    const int count = (p.K >> 5) * rows, step = blockDim.x;
+    auto put = [&](int r, int blk, u32x4 c, uint32_t byte) {
+      const int j = XT > 1 ? r >> 4 : 0, st = blk >> 2, rr = XT > 1 ? r & 15 : r;
+      *reinterpret_cast<u32x4 *>(lds + 16 * (((st * XT + j) * 4 + (blk & 3)) * mr + rr)) = c;
+      lds[sp.xcodes + 4 * ((((st >> 2) * XT + j) * 4 + (blk & 3)) * mr + rr) + (st & 3)] = (uint8_t)byte;
+    };
+    auto at = [&](int i, int &r, int &blk) -> int64_t {  // (past the end: the last block again)
+      i = min(i, count - 1);
+      blk = i / rows;
+      r = i - blk * rows;
+      return p.xrow ? p.xrow[r0 + r] : r0 + r;
+    };
+    // (the loads of several blocks in flight: each trip round the loop waits for memory)
+    if (p.xs) {
+      constexpr int B = 4;
+      for (int i = tid; i < count; i += B * step) {
+        u32x4 c[B];
+        uint8_t byte[B];
+        int r[B], blk[B];
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          const int64_t xr = at(i + k * step, r[k], blk[k]);
+          c[k] = ldg16(static_cast<const uint8_t *>(p.x) + xr * kb + 16 * blk[k]);
+          byte[k] = p.xs[xr * ksb + blk[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) put(r[k], blk[k], c[k], byte[k]);
+      }
+    } else {
+      constexpr int B = 2;
+      for (int i = tid; i < count; i += B * step) {
+        u32x4 v[B][4];
+        int r[B], blk[B];
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          const int64_t xr = at(i + k * step, r[k], blk[k]);
+          const uint16_t *src = static_cast<const uint16_t *>(p.x) + xr * p.ldx + 32 * blk[k];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[k][j] = ldg16(src + 8 * j);
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          u16x2 am = {0, 0};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) am = mx_absmax(am, v[k][j]);
+          const uint32_t byte = mx_byte(mx_amax_bits(am));
+          const float sc = mx_scale(byte);
+          u32x4 c;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) c[j] = mx_codes8(v[k][j], sc);
+          put(r[k], blk[k], c, byte);
+        }
       }
     }
-  } else {
-    for (int i = tid; i < WT * XT * 64; i += blockDim.x) {
-      const int l = i & 63, t = (i >> 6) / XT, j = (i >> 6) - t * XT;
-      const int n = nt * COLS + 16 * t + 4 * (l >> 4), m = 16 * j + (l & 15);
-      if (m < rows && n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + m] : r0 + m, n, total(t, j, l));
+  };
+  auto meet = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  f32x4 acc[XT];
+#pragma unroll
+  for (int j = 0; j < XT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Loads l0, l1;
+  load(l0);
+  load(l1);
+  int64_t item = i0;
+  int en = (int)(item / sp.ntiles), tile = (int)(item - (int64_t)en * sp.ntiles);
+  fill(en);
+  meet();
+
+  const uint32_t gsel = g | (4 + g) << 8;
+  const uint8_t *xl = lds + 16 * (g * mr + (r16 & (mr - 1))), *xsl = lds + sp.xcodes + 4 * (g * mr + (r16 & (mr - 1)));
+  int sub = 0, q = q0, odd = 0;
+  auto finish = [&]() {  // an item's sums, in wave order
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds + sp.xbytes) + odd * nw * WT * XT * 64;
+    auto total_of = [&](int t, int j, int l) {
+      f32x4 v = part[(t * XT + j) * 64 + l];
+      for (int w = 1; w < nw; ++w) v += part[((w * WT + t) * XT + j) * 64 + l];
+      return v;
+    };
+    if constexpr (SILU) {
+      // eight lanes hold a block of 32 outputs of a row: four each
+      for (int i = tid; i < XT * 128; i += blockDim.x) {
+        const int c = i & 7, m = i >> 3, t = c >> 2;
+        const int j = m >> 4, l = (c & 3) * 16 + (m & 15);
+        const f32x4 gt = total_of(t, j, l), up = total_of(t + 2, j, l);
+        float h[4];
+        uint32_t am = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          h[k] = mx_silu_mul(gt[k], up[k]);
+          am = max(am, __float_as_uint(h[k]) & 0x7fffffffu);
+        }
+        am = max(am, dpp_u32<0xB1>(am));   // quad_perm [1,0,3,2]
+        am = max(am, dpp_u32<0x4E>(am));   // quad_perm [2,3,0,1]
+        am = max(am, dpp_u32<0x141>(am));  // row_half_mirror
+        const uint32_t byte = mx_byte(am);
+        const float sc = mx_scale(byte);
+        uint32_t c4 = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, h[0], h[1], sc, 0);
+        c4 = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c4, h[2], h[3], sc, 1);
+        if (byte == 255) c4 = 0;
+        if (m < rows) {
+          *reinterpret_cast<uint16_t *>(p.hc + (int64_t)(r0 + m) * (p.N >> 1) + 16 * tile + 2 * c) = (uint16_t)c4;
+          if (c == 0) p.hs[(int64_t)(r0 + m) * (p.N >> 5) + tile] = (uint8_t)byte;
+        }
+      }
+    } else {
+      for (int i = tid; i < XT * 64; i += blockDim.x) {
+        const int j = i >> 6, l = i & 63, n = tile * COLS + 4 * (l >> 4), m = 16 * j + (l & 15);
+        if (m < rows && n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + m] : r0 + m, n, total_of(0, j, l));
+      }
     }
+  };
+  // multiplies the quad in l, then refills l
+  auto body = [&](Loads &l) {
+    const uint32_t ws = __builtin_amdgcn_perm(__builtin_amdgcn_perm(l.s.w, l.s.z, gsel),
+                                              __builtin_amdgcn_perm(l.s.y, l.s.x, gsel), 0x05040100u);
+    uint32_t xs[XT];
+#pragma unroll
+    for (int j = 0; j < XT; ++j) xs[j] = *reinterpret_cast<const uint32_t *>(xsl + 16 * (q * XT + j) * mr);
+    u32x4 xc[4][XT];  // (PLANES: steps past the end read the last one's)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < XT; ++j)
+        xc[u][j] = ldg16(xl + 64 * ((PLANES ? min(4 * q + u, steps - 1) : 4 * q + u) * XT + j) * mr);
+    const int nst = PLANES ? steps - 4 * q : 4;
+#pragma unroll
+    for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<0>(l.w[0], ws, xc[0][j], xs[j], acc[j]);
+    if (!PLANES || nst > 1)
+#pragma unroll
+      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<1>(l.w[1], ws, xc[1][j], xs[j], acc[j]);
+    if (!PLANES || nst > 2)
+#pragma unroll
+      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<2>(l.w[2], ws, xc[2][j], xs[j], acc[j]);
+    if (!PLANES || nst > 3)
+#pragma unroll
+      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<3>(l.w[3], ws, xc[3][j], xs[j], acc[j]);
+    __builtin_amdgcn_sched_barrier(0);  // (the registers of l are free: no copies of them)
+    load(l);
+    __builtin_amdgcn_sched_barrier(0);
+    if (++q < q1) return;
+    q = q0;
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds + sp.xbytes) + ((odd * nw + wave) * WT + sub) * XT * 64;
+#pragma unroll
+    for (int j = 0; j < XT; ++j) {
+      part[j * 64 + lane] = acc[j];
+      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (++sub < WT) return;
+    sub = 0;
+    meet();
+    finish();
+    odd ^= 1;
+    if (++item == i1 || ++tile < sp.ntiles) return;
+    tile = 0;
+    meet();  // (every wave is past its last read of the old rows)
+    fill(++en);
+    meet();
+  };
+  const int64_t len = (i1 - i0) * WT * (q1 - q0);
+  int64_t n = 0;
+  for (; n + 2 <= len; n += 2) {
+    body(l0);
+    body(l1);
   }
+  if (n < len) body(l0);
 }
 
 // ---------------------------------------------------------------- tiles
 
-// A workgroup is four waves on two 128-row weight segments: wave w multiplies
-// rows 32 w .. +31 of both by all activation rows (2 NJ fragments of 16), so with
-// gate rows as segment 0 and up rows as segment 1 a lane holds gate and up of the
-// same outputs.  Stages of 128 K values (64 bytes a row, chunk c of row r at c ^
-// ((r >> 2) & 3): the 16 lanes of a fragment-read pass hit distinct banks) come by
-// direct copies into a ring of three, two ahead; two workgroups share a CU.
+// A workgroup is eight waves on two 128-row weight segments and up to 256 activation
+// rows: waves w and w + 4 multiply the weight rows 32 (w % 4) .. +31 of both segments
+// (fragments f of 16: segment f / 2), so with gate rows as segment 0 and up rows as
+// segment 1 a lane holds gate and up of the same outputs.  One workgroup per CU.
 //
-// Exponents: four stages at a time, 16 bytes a row; a lane picks its block's byte of
-// each of the four stages into one dword, whose bytes the MFMAs select by number.
-constexpr int MX_WST = 256 * 64;  // weight part of a stage
-template <int NJ>
-struct MxLds {
-  static constexpr int XROWS = 32 * NJ;
-  static constexpr int STAGE = MX_WST + XROWS * 64;
-  static constexpr int SCALES = 3 * STAGE;
-  static constexpr int BYTES = SCALES + (256 + XROWS) * 16;
-};
-static_assert(MxLds<4>::BYTES <= 80 * 1024, "two workgroups per CU");
+// Stages of 256 K values are whole 128-byte lines of a row, copied straight into LDS.
+// 16-byte chunk c of row r is at c ^ ((r >> 1) & 7): a pass of a 16-byte LDS read
+// takes lanes 0-3, 12-15 and 20-27 (and so on), here rows 0-3 and 12-15 of one chunk
+// and 4-11 of the next: sixteen distinct bank groups.  (Stages of 64 bytes a row: the
+// L2 delivers 20 TB/s in such pieces, 35 TB/s in lines.)
+//
+// Exponents: four K steps at a time, 16 bytes a row (PLANES: K % 512, rows without
+// that alignment: four planes of a dword a row); a lane picks its K block's bytes into
+// one dword, whose bytes the MFMAs select by number.
+constexpr int MX_WHALF = 256 * 128;       // weight part of a stage
+constexpr int MX_SCALE_LDS = 512 * 16;    // exponents of the 256 + 256 rows
 
 struct MxTile {
   const uint8_t *w[2], *ws[2];
   int wrows[2];
   const int32_t *xrow;  // of the tile's first position, or null
   int64_t x0;           // x row of the tile's first row (xrow null)
-  int rows, it0, it1;   // 128-wide K stages, it0 a multiple of 4
+  int rows, it0, it1;   // 128-wide K steps, it0 a multiple of 4
 };
 
-template <int NJ>
+// Copies of 16 bytes a lane into LDS (lane l: dst + 16 l) from `base` + lane offset +
+// scalar offset, the offsets below 4 GB.
+AMLA_DEV __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, 0xffffffffu, 0x00027000);
+}
+AMLA_DEV void mx_copy16(__amdgpu_buffer_rsrc_t r, uint8_t *dst, uint32_t lane_off, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LDS_PTR(dst), 16, lane_off, off, 0, 0);
+}
+
+template <int XF>
 struct MxSums {
-  f32x4 acc[4][2 * NJ];  // [weight fragment][activation fragment]
+  f32x4 acc[4][XF];  // [weight fragment][activation fragment]
 };
 
-template <int NJ>
-struct MxTileMain {
-  static AMLA_DEV void run(const MxParams &p, const MxTile &a, MxSums<NJ> &sums) {
+// Up to 16 XF <= 128 activation rows: the two halves of the workgroup take the two K
+// steps of a stage (and meet in LDS at the end).  Three slots, two stages on their way.
+// Bound by the weights' stream for the few rows that an expert gets.
+template <int XF>
+struct MxRowsLds {
+  static constexpr int XROWS = XF > 4 ? 128 : 16 * XF;
+  static constexpr int STAGE = MX_WHALF + XROWS * 128;
+  static constexpr int SCALES = 3 * STAGE;
+  static constexpr int BYTES = SCALES + MX_SCALE_LDS;
+};
+static_assert(MxRowsLds<8>::BYTES <= 160 * 1024, "LDS of a CU");
+
+template <int XF, bool PLANES>
+struct MxRowsMain {
+  static AMLA_DEV void run(const MxParams &p, const MxTile &a, MxSums<XF> &sums) {
   auto &acc = sums.acc;
   extern __shared__ __align__(16) uint8_t lds[];
-  using L = MxLds<NJ>;
-  constexpr int XC = NJ == 4 ? 2 : 1, C = 4 + XC;  // copies per wave and stage
+  using L = MxRowsLds<XF>;
+  constexpr int XC = XF > 4 ? 2 : 1, C = 4 + XC;  // copies per wave and stage
+  constexpr int XW = L::XROWS / 8;                // x rows a wave copies
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wk = wave >> 2;
   const int64_t kb = p.K >> 1, ksb = p.K >> 5;
   const int steps = p.K >> 7;
-  auto xrow_of = [&](int r) {  // rows past the tile repeat its last row (not stored)
+  const int seg = wave >> 2;
+  const int wrows = seg ? a.wrows[1] : a.wrows[0];
+  const auto wrsrc = mx_rsrc(seg ? a.w[1] : a.w[0]), xrsrc = mx_rsrc(static_cast<const uint8_t *>(p.x) + (a.xrow ? 0 : a.x0 * kb));
+  auto xrow_of = [&](int r) {  // (a gathered x is less than 4 GB); rows past the tile repeat its last row
     const int rc = min(r, a.rows - 1);
-    return a.xrow ? (int64_t)a.xrow[rc] : a.x0 + rc;
+    return (uint32_t)(a.xrow ? a.xrow[rc] : rc);
   };
-
-  uint32_t woff[2][2];
+  // wave w copies weight rows 32 w .. +31 (of the 256) and XW x rows, 8 rows a copy
+  uint32_t woff[4], xoff[XC];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const uint32_t r = 32 * wave + 16 * c + (lane >> 2);
-      woff[s][c] = min(r, (uint32_t)a.wrows[s] - 1) * (uint32_t)kb + 16 * ((lane & 3) ^ ((r >> 2) & 3));
-    }
-  typedef const __attribute__((address_space(1))) uint8_t *gptr;
-  gptr xptr[XC];
+  for (int c = 0; c < 4; ++c) {
+    const int r = 8 * c + (lane >> 3);
+    woff[c] = (uint32_t)min(32 * wn + r, wrows - 1) * (uint32_t)kb + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+  }
 #pragma unroll
   for (int c = 0; c < XC; ++c) {
-    const int r = 8 * NJ * wave + 16 * c + (lane >> 2);
-    xptr[c] = (gptr)(static_cast<const uint8_t *>(p.x) + xrow_of(r) * kb + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
+    const int r = XW * wave + 8 * c + (lane >> 3);
+    xoff[c] = xrow_of(r) * (uint32_t)kb + 16 * ((lane & 7) ^ ((r >> 1) & 7));
   }
-  auto opaque = [](uint32_t v) {  // (scalar base + 32-bit lane offset per copy)
-    asm volatile("" : "+v"(v));
-    return v;
-  };
-  auto copy = [&](int it, int slot) {
+  auto copy = [&](int i, int slot) {  // the stage of the K steps i, i + 1
     uint8_t *st = lds + slot * L::STAGE;
+    // (a last stage of one K step: the lanes of the other repeat it)
+    auto back = [&](int r) -> uint32_t { return PLANES && i + 1 >= steps && (((lane & 7) ^ (r >> 1)) & 4) ? 64 : 0; };
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      gptr wb = (gptr)(a.w[s] + (size_t)it * 64);
-      asm volatile("" : "+s"(wb));
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        __builtin_amdgcn_global_load_lds(wb + opaque(woff[s][c]), LDS_PTR(st + (128 * s + 32 * wave + 16 * c) * 64), 16, 0, 0);
-    }
+    for (int c = 0; c < 4; ++c)
+      mx_copy16(wrsrc, st + (32 * wave + 8 * c) * 128, woff[c] - back(8 * c + (lane >> 3)), i * 64);
 #pragma unroll
     for (int c = 0; c < XC; ++c)
-      if (NJ > 1 || lane < 32)
-        __builtin_amdgcn_global_load_lds(xptr[c] + (size_t)it * 64, LDS_PTR(st + MX_WST + (8 * NJ * wave + 16 * c) * 64), 16, 0, 0);
+      if (XF > 2 || lane < 32)
+        mx_copy16(xrsrc, st + MX_WHALF + (XW * wave + 8 * c) * 128, xoff[c] - back(XW * wave + 8 * c + (lane >> 3)), i * 64);
   };
-
-  // exponents of four stages from stage it: wave w copies those of weight rows 64 w
-  // .. +63 and of its quarter of the x rows, 16 bytes a row; where rows are not 16-byte
-  // aligned (K % 512), as four planes of one dword a row
-  const bool planes = p.K & 511;
-  const int seg = wave >> 1;
-  const uint32_t swoff = min(64 * (wave & 1) + lane, (seg ? a.wrows[1] : a.wrows[0]) - 1) * (uint32_t)ksb;
-  const gptr swp = (gptr)(seg ? a.ws[1] : a.ws[0]);
-  const gptr sxp = (gptr)(p.xs + xrow_of(8 * NJ * wave + min(lane, 8 * NJ - 1)) * ksb);
-  auto copy_scales = [&](int it) {
+  // exponent rows in LDS 64 w + lane: weight row r at 64 (r / 32) + r % 32, x row r at
+  // 64 (r / XW) + 32 + r % XW
+  typedef const __attribute__((address_space(1))) uint8_t *gptr;
+  const gptr sptr = lane < 32 ? (gptr)((seg ? a.ws[1] : a.ws[0]) + (int64_t)min(32 * wn + lane, wrows - 1) * ksb)
+                              : (gptr)(p.xs + ((a.xrow ? 0 : a.x0) + (int64_t)xrow_of(XW * wave + min(lane - 32, XW - 1))) * ksb);
+  auto copy_scales = [&](int i) {
     uint8_t *sc = lds + L::SCALES;
-    if (!planes) {
-      __builtin_amdgcn_global_load_lds(swp + it * 4 + swoff, LDS_PTR(sc + 1024 * wave), 16, 0, 0);
-      if (lane < 8 * NJ) __builtin_amdgcn_global_load_lds(sxp + it * 4, LDS_PTR(sc + 4096 + 128 * NJ * wave), 16, 0, 0);
+    if constexpr (!PLANES) {
+      __builtin_amdgcn_global_load_lds(sptr + i * 4, LDS_PTR(sc + 1024 * wave), 16, 0, 0);
     } else {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = min(it + u, steps - 1) * 4;  // stages past the end are not multiplied
-        uint8_t *pl = sc + u * (256 + L::XROWS) * 4;
-        __builtin_amdgcn_global_load_lds(swp + i + swoff, LDS_PTR(pl + 256 * wave), 4, 0, 0);
-        if (lane < 8 * NJ) __builtin_amdgcn_global_load_lds(sxp + i, LDS_PTR(pl + 1024 + 32 * NJ * wave), 4, 0, 0);
-      }
+      for (int u = 0; u < 4; ++u)
+        __builtin_amdgcn_global_load_lds(sptr + min(i + u, steps - 1) * 4, LDS_PTR(sc + 2048 * u + 256 * wave), 4, 0, 0);
     }
   };
-  // the lane's bytes of the four stages of scale row r, in stage order
+  // bytes of the wave's K step of this stage and of the next
+  const uint32_t gsel = g | (4 + g) << 8;
+  uint32_t wsc[4], xsc[XF];
+  auto read_scales = [&]() {
+    const uint8_t *sc = lds + L::SCALES + wk * (PLANES ? 2048 : 4);
+    auto row = [&](int r) {
+      const uint8_t *at = sc + r * (PLANES ? 4 : 16);
+      return __builtin_amdgcn_perm(*reinterpret_cast<const uint32_t *>(at + (PLANES ? 4096 : 8)),
+                                   *reinterpret_cast<const uint32_t *>(at), gsel);
+    };
+    const int x16 = 64 * (r16 / XW) + 32 + r16 % XW;
+#pragma unroll
+    for (int f = 0; f < 4; ++f) wsc[f] = row(64 * (4 * (f >> 1) + wn) + 16 * (f & 1) + r16);
+#pragma unroll
+    for (int j = 0; j < XF; ++j) xsc[j] = row(64 * (16 / XW) * j + x16);
+  };
+#pragma unroll
+  for (int f = 0; f < 4; ++f)
+#pragma unroll
+    for (int j = 0; j < XF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const uint32_t frag = r16 * 128 + 16 * ((4 * wk + g) ^ ((r16 >> 1) & 7));
+  copy_scales(a.it0);
+  copy(a.it0, 0);
+  if (a.it0 + 2 < a.it1) copy(a.it0 + 2, 1);
+  int slot = 0;
+  auto stage = [&](int i, auto u_c) {
+    constexpr int U = decltype(u_c)::value;
+    if (i + 2 < a.it1) wait_vmcnt<C>();  // all but the next stage's copies have landed
+    else wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if constexpr (U == 0) read_scales();
+    if constexpr (U == 1)  // (every wave has read the others before this barrier)
+      if (i + 2 < a.it1) copy_scales(i + 2);
+    if (i + 4 < a.it1) copy(i + 4, slot == 0 ? 2 : slot - 1);
+    const uint8_t *st = lds + slot * L::STAGE + frag;
+    slot = slot == 2 ? 0 : slot + 1;
+    if (PLANES && i + wk >= a.it1) return;
+    u32x4 wf[4], xf[XF];
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+      wf[f] = *reinterpret_cast<const u32x4 *>(st + ((f >> 1) * 128 + 32 * wn + 16 * (f & 1)) * 128);
+#pragma unroll
+    for (int j = 0; j < XF; ++j) xf[j] = *reinterpret_cast<const u32x4 *>(st + MX_WHALF + j * 2048);
+#pragma unroll
+    for (int j = 0; j < XF; ++j)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[f][j] = mfma_mx<U>(wf[f], wsc[f], xf[j], xsc[j], acc[f][j]);
+  };
+  for (int i = a.it0; i < a.it1; i += 4) {
+    stage(i, std::integral_constant<int, 0>{});
+    if (i + 2 < a.it1) stage(i + 2, std::integral_constant<int, 1>{});
+  }
+
+  // each half adds up half of the activation fragments (waves w and w + 4 exchange)
+  __builtin_amdgcn_s_barrier();  // every wave is past its last fragment read
+  asm volatile("" ::: "memory");
+  f32x4 *ex = reinterpret_cast<f32x4 *>(lds) + lane;
+#pragma unroll
+  for (int f = 0; f < 4; ++f)
+#pragma unroll
+    for (int j = 0; j < XF / 2; ++j)
+      ex[((wave * 4 + f) * (XF / 2) + j) * 64] = wk ? acc[f][j] : acc[f][XF / 2 + j];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  // (the K step 0 half first in every sum; the wave's own fragments end up in 0 .. XF/2 - 1)
+#pragma unroll
+  for (int f = 0; f < 4; ++f)
+#pragma unroll
+    for (int j = 0; j < XF / 2; ++j) {
+      const f32x4 o = ex[(((wave ^ 4) * 4 + f) * (XF / 2) + j) * 64];
+      acc[f][j] = wk ? o + acc[f][XF / 2 + j] : acc[f][j] + o;
+    }
+  __builtin_amdgcn_s_barrier();  // (the slots may be copied into again)
+}
+};
+
+// More rows: waves 0 .. 3 take the first 128 activation rows, the others the rest.  Two
+// slots: the second K step's fragments of a stage are read while its first is
+// multiplied, so that the slot is free for the stage after next when the second
+// begins.
+//
+// What bounds it is the power of the matrix units: 4096 x 7168 x 16384 in 272 us (3.5
+// PFLOP/s); the multiplications and barriers alone, on the same data, take 223 us.
+// Four slots of 64-byte rows, two stages on their way: 306 us (the L2 delivers 20
+// TB/s in such pieces, 35 TB/s in lines).  256 x 128 tiles, two workgroups per CU: 332.
+constexpr int MXB_STAGE = 2 * MX_WHALF;
+constexpr int MXB_SCALES = 2 * MXB_STAGE;
+constexpr int MX_TILE_LDS = MxRowsLds<8>::BYTES;
+static_assert(MXB_SCALES + MX_SCALE_LDS <= MX_TILE_LDS, "LDS of either form");
+
+template <bool PLANES>
+struct MxBigMain {
+  static AMLA_DEV void run(const MxParams &p, const MxTile &a, MxSums<8> &sums) {
+  auto &acc = sums.acc;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
+  const int64_t kb = p.K >> 1, ksb = p.K >> 5;
+  const int steps = p.K >> 7;
+  // wave w copies weight rows 32 w .. +31 (of the 256) and x rows 32 w .. +31, 8 rows a
+  // copy: lane offsets from a tile's first row, the stage as the scalar offset
+  const int seg = wave >> 2;
+  const int wrows = seg ? a.wrows[1] : a.wrows[0];
+  const auto wrsrc = mx_rsrc(seg ? a.w[1] : a.w[0]), xrsrc = mx_rsrc(static_cast<const uint8_t *>(p.x) + (a.xrow ? 0 : a.x0 * kb));
+  auto xrow_of = [&](int r) {  // (a gathered x is less than 4 GB); rows past the tile repeat its last row
+    const int rc = min(r, a.rows - 1);
+    return (uint32_t)(a.xrow ? a.xrow[rc] : rc);
+  };
+  uint32_t woff[4], xoff[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int r = 8 * c + (lane >> 3), ch = (lane & 7) ^ ((r >> 1) & 7);
+    woff[c] = (uint32_t)min(32 * wn + r, wrows - 1) * (uint32_t)kb + 16 * ch;
+    xoff[c] = xrow_of(32 * wave + r) * (uint32_t)kb + 16 * ch;
+  }
+  auto copy = [&](int i, int slot) {  // the stage of the K steps i, i + 1
+    uint8_t *st = lds + slot * MXB_STAGE + 32 * wave * 128;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      // (a last stage of one K step: the lanes of the other repeat it)
+      const uint32_t back = PLANES && i + 1 >= steps && (((lane & 7) ^ (4 * c + (lane >> 4))) & 4) ? 64 : 0;
+      mx_copy16(wrsrc, st + c * 1024, woff[c] - back, i * 64);
+      mx_copy16(xrsrc, st + MX_WHALF + c * 1024, xoff[c] - back, i * 64);
+    }
+  };
+  // exponents: wave w has 32 rows of each half, 16 bytes (or four planes of 4) a row;
+  // scale rows in LDS 64 w + lane: weight row r at 64 (r / 32) + r % 32, x row r 32 further
+  const int sl = lane & 31;
+  typedef const __attribute__((address_space(1))) uint8_t *gptr;
+  const gptr sptr = lane < 32 ? (gptr)((seg ? a.ws[1] : a.ws[0]) + (int64_t)min(32 * wn + sl, wrows - 1) * ksb)
+                              : (gptr)(p.xs + ((a.xrow ? 0 : a.x0) + (int64_t)xrow_of(32 * wave + sl)) * ksb);
+  auto copy_scales = [&](int i) {
+    uint8_t *sc = lds + MXB_SCALES;
+    if constexpr (!PLANES) {
+      __builtin_amdgcn_global_load_lds(sptr + i * 4, LDS_PTR(sc + 1024 * wave), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        __builtin_amdgcn_global_load_lds(sptr + min(i + u, steps - 1) * 4, LDS_PTR(sc + 2048 * u + 256 * wave), 4, 0, 0);
+    }
+  };
   const uint32_t gsel = g | (4 + g) << 8;
   auto pick = [&](u32x4 d) {
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d.w, d.z, gsel), __builtin_amdgcn_perm(d.y, d.x, gsel), 0x05040100u);
   };
-  uint32_t wsc[4], xsc[2 * NJ];
-  auto read_scales = [&](auto planes_c) {
-    constexpr bool PLANES = decltype(planes_c)::value;
-    const uint8_t *sc = lds + L::SCALES + r16 * (PLANES ? 4 : 16);
+  uint32_t wsc[4], xsc[8];
+  auto read_scales = [&]() {
+    const uint8_t *sc = lds + MXB_SCALES + r16 * (PLANES ? 4 : 16);
     auto row = [&](int r) {
       if constexpr (!PLANES) return *reinterpret_cast<const u32x4 *>(sc + 16 * r);
       u32x4 d;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) d[u] = *reinterpret_cast<const uint32_t *>(sc + (u * (256 + L::XROWS) + r) * 4);
+      for (int u = 0; u < 4; ++u) d[u] = *reinterpret_cast<const uint32_t *>(sc + 2048 * u + 4 * r);
       return d;
     };
 #pragma unroll
-    for (int f = 0; f < 4; ++f) wsc[f] = pick(row((f >> 1) * 128 + 32 * wave + 16 * (f & 1)));
+    for (int f = 0; f < 4; ++f) wsc[f] = pick(row(64 * (4 * (f >> 1) + wn) + 16 * (f & 1)));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < 2 * NJ; ++j) xsc[j] = pick(row(256 + 16 * j));
+    for (int j = 0; j < 8; ++j) {
+      xsc[j] = pick(row(64 * (4 * wm + (j >> 1)) + 32 + 16 * (j & 1)));
+      if (j & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    // (picked here, not in the next body: four registers a row are not there)
+#pragma unroll
+    for (int f = 0; f < 4; ++f) asm volatile("" : "+v"(wsc[f]));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(xsc[j]));
   };
-
 #pragma unroll
   for (int f = 0; f < 4; ++f)
 #pragma unroll
-    for (int j = 0; j < 2 * NJ; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 8; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  copy_scales(a.it0);
-  copy(a.it0, 0);
-  if (a.it0 + 1 < a.it1) copy(a.it0 + 1, 1);
-
-  const uint32_t frag = 16 * (g ^ ((r16 >> 2) & 3)) + r16 * 64;
-  int slot = 0;
-  auto stage = [&](int it, auto u_c) {
-    constexpr int U = decltype(u_c)::value;
-    if (it + 1 < a.it1) wait_vmcnt<C>();  // all but the next stage's copies have landed
-    else wait_vmcnt<0>();
+  const uint32_t sw = (r16 >> 1) & 7;
+  const uint32_t frag[2] = {r16 * 128 + 16 * (g ^ sw), r16 * 128 + 16 * ((4 + g) ^ sw)};
+  u32x4 wf[2][4], xf[8];
+  auto read_w = [&](int slot, int ks, int f) {
+    return *reinterpret_cast<const u32x4 *>(lds + slot * MXB_STAGE + ((f >> 1) * 128 + 32 * wn + 16 * (f & 1)) * 128 + frag[ks]);
+  };
+  auto read_x = [&](int slot, int ks, int j) {
+    return *reinterpret_cast<const u32x4 *>(lds + slot * MXB_STAGE + MX_WHALF + (128 * wm + 16 * j) * 128 + frag[ks]);
+  };
+  auto landed = [&]() {  // every copy, and every read of the slot that is free now, in all waves
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if constexpr (U == 0) {
-      if (!planes) read_scales(std::false_type{});
-      else read_scales(std::true_type{});
-    }
-    // (every wave has read the four stages' exponents before this barrier)
-    if constexpr (U == 1)
-      if (it + 3 < a.it1) copy_scales(it + 3);
-    if (it + 2 < a.it1) copy(it + 2, slot == 0 ? 2 : slot - 1);
-    const uint8_t *st = lds + slot * L::STAGE;
-    u32x4 wf[4], xf[2 * NJ];
-#pragma unroll
-    for (int f = 0; f < 4; ++f)
-      wf[f] = *reinterpret_cast<const u32x4 *>(st + ((f >> 1) * 128 + 32 * wave + 16 * (f & 1)) * 64 + frag);
-#pragma unroll
-    for (int j = 0; j < 2 * NJ; ++j) xf[j] = *reinterpret_cast<const u32x4 *>(st + MX_WST + j * 1024 + frag);
-#pragma unroll
-    for (int j = 0; j < 2 * NJ; ++j)
-#pragma unroll
-      for (int f = 0; f < 4; ++f) acc[f][j] = mfma_mx<U>(wf[f], wsc[f], xf[j], xsc[j], acc[f][j]);
-    slot = slot == 2 ? 0 : slot + 1;
   };
-  for (int it = a.it0; it < a.it1; it += 4) {
-    stage(it, std::integral_constant<int, 0>{});
-    if (it + 1 < a.it1) stage(it + 1, std::integral_constant<int, 1>{});
-    if (it + 2 < a.it1) stage(it + 2, std::integral_constant<int, 2>{});
-    if (it + 3 < a.it1) stage(it + 3, std::integral_constant<int, 3>{});
+  copy_scales(a.it0);
+  copy(a.it0, 0);
+  landed();
+  if (a.it0 + 2 < a.it1) copy(a.it0 + 2, 1);
+  read_scales();
+#pragma unroll
+  for (int f = 0; f < 4; ++f) wf[0][f] = read_w(0, 0, f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) xf[j] = read_x(0, 0, j);
+
+  // K step U of four: multiplies it, reads the next one's fragments
+  auto step = [&](auto u_c) {
+    constexpr int U = decltype(u_c)::value, SLOT = ((U + 1) >> 1) & 1, KS = (U + 1) & 1;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[f][j] = mfma_mx<U>(wf[U & 1][f], wsc[f], xf[j], xsc[j], acc[f][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      xf[j] = read_x(SLOT, KS, j);
+      if (j & 1) wf[1 - (U & 1)][j >> 1] = read_w(SLOT, KS, j >> 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  std::integral_constant<int, 0> u0;
+  std::integral_constant<int, 1> u1;
+  std::integral_constant<int, 2> u2;
+  std::integral_constant<int, 3> u3;
+  // (no branches where four steps are followed by four: the compiler would sink the
+  // multiplications behind them, and their operands into memory)
+  int i = a.it0;
+  for (; i + 8 <= a.it1; i += 4) {
+    step(u0);
+    landed();
+    copy_scales(i + 4);
+    copy(i + 4, 0);
+    step(u1);
+    step(u2);
+    landed();
+    copy(i + 6, 1);
+    step(u3);
+    read_scales();
   }
+  if constexpr (!PLANES) {  // whole fours: one is left
+    step(u0);
+    landed();
+    step(u1);
+    step(u2);
+    landed();  // (keeps the steps apart for the compiler)
+    step(u3);
+  } else {
+    for (; i < a.it1; i += 4) {
+      const int left = a.it1 - i;
+      step(u0);
+      landed();
+      if (left > 4) {
+        copy_scales(i + 4);
+        copy(i + 4, 0);
+      }
+      if (left > 1) step(u1);
+      if (left > 2) step(u2);
+      landed();
+      if (left > 6) copy(i + 6, 1);
+      if (left > 3) step(u3);
+      if (left > 4) read_scales();
+    }
+  }
+  // (nor sink the last of them into the branches of the stores)
+#pragma unroll
+  for (int f = 0; f < 4; ++f)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[f][j]));
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();  // (the slots may be copied into again)
 }
 };
 
@@ -429,21 +732,16 @@ AMLA_DEV void mx_tile_store(const MxParams &p, const f32x4 (&v)[4], int wave, in
 }
 
 struct MxSplit {
-  int n_tiles, m_tiles;  // one weight: tiles of 256 outputs (SILU: 128) x 128 rows
-  int parts;             // K parts of every tile, whole runs of four stages
-  float *partial;        // [tile][part][fragment][wave][lane] f32x4
+  int n_tiles, m_tiles;  // one weight: tiles of 256 outputs (SILU: 128) x 256 rows
+  int parts;             // K parts of every tile, whole runs of four steps
+  float *partial;        // [tile][part][activation fragment][weight fragment][wave % 4][lane] f32x4
 };
+constexpr int MX_ROWS = 256;  // activation rows of a tile
 constexpr int MX_PART_F32 = 256 * MX_ROWS;
 
-AMLA_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// Column tile nt of `rows` positions from r0 of expert e.
-template <int NJ, bool SILU>
-AMLA_DEV void mx_tile(const MxParams &p, int e, int r0, int rows, int nt, int it0, int it1, f32x4 *partial) {
-  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+template <bool SILU>
+AMLA_DEV MxTile mx_tile_of(const MxParams &p, int e, int r0, int rows, int n0, int it0, int it1) {
   MxTile a;
-  const int n0 = nt * (SILU ? 128 : 256);
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     int n = SILU ? n0 : n0 + 128 * s;
@@ -457,34 +755,54 @@ AMLA_DEV void mx_tile(const MxParams &p, int e, int r0, int rows, int nt, int it
   a.rows = rows;
   a.it0 = it0;
   a.it1 = it1;
-  MxSums<NJ> sums;
-  MxTileMain<NJ>::run(p, a, sums);
-  auto &acc = sums.acc;
+  return a;
+}
+
+// Stores fragments j0 .. j0 + XF - 1 of a tile, held as acc[.][0 .. XF - 1].
+template <int XF, int HELD, bool SILU>
+AMLA_DEV void mx_tile_out(const MxParams &p, const MxSums<HELD> &sums, int j0, int r0, int rows, int n0, f32x4 *partial) {
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15;
+  const int wn = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
 #pragma unroll
-  for (int j = 0; j < 2 * NJ; ++j) {
-    f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+  for (int j = 0; j < XF; ++j) {
+    const f32x4 v[4] = {sums.acc[0][j], sums.acc[1][j], sums.acc[2][j], sums.acc[3][j]};
     if (partial) {
 #pragma unroll
-      for (int f = 0; f < 4; ++f) partial[((f * 8 + j) * 4 + wave) * 64 + lane] = v[f];
+      for (int f = 0; f < 4; ++f) partial[(((j0 + j) * 4 + f) * 4 + wn) * 64 + lane] = v[f];
       continue;
     }
-    const int m = 16 * j + r16;
-    const bool live = m < rows;
+    const int m = 16 * (j0 + j) + r16;
     const int pos = r0 + min(m, rows - 1);
-    mx_tile_store<SILU>(p, v, wave, lane, live, pos, p.yrow ? p.yrow[pos] : pos, n0);
+    mx_tile_store<SILU>(p, v, wn, lane, m < rows, pos, p.yrow ? p.yrow[pos] : pos, n0);
   }
 }
 
-template <bool SILU>
-AMLA_DEV void mx_tile_rows(const MxParams &p, int e, int r0, int rows, int nt, int it0, int it1, f32x4 *partial) {
-  if (rows <= 32) mx_tile<1, SILU>(p, e, r0, rows, nt, it0, it1, partial);
-  else if (rows <= 64) mx_tile<2, SILU>(p, e, r0, rows, nt, it0, it1, partial);
-  else mx_tile<4, SILU>(p, e, r0, rows, nt, it0, it1, partial);
+template <int XF, bool SILU, bool PLANES>
+AMLA_DEV void mx_rows_tile(const MxParams &p, const MxTile &a, int r0, int n0, f32x4 *partial) {
+  MxSums<XF> sums;
+  MxRowsMain<XF, PLANES>::run(p, a, sums);
+  mx_tile_out<XF / 2, XF, SILU>(p, sums, __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) * (XF / 2), r0, a.rows, n0, partial);
+}
+
+// Column tile nt of `rows` <= 256 positions from r0 of expert e, K steps it0 .. it1 - 1.
+template <bool SILU, bool PLANES>
+AMLA_DEV void mx_tile(const MxParams &p, int e, int r0, int rows, int nt, int it0, int it1, f32x4 *partial) {
+  const int n0 = nt * (SILU ? 128 : 256);
+  const MxTile a = mx_tile_of<SILU>(p, e, r0, rows, n0, it0, it1);
+  if (rows <= 32) mx_rows_tile<2, SILU, PLANES>(p, a, r0, n0, partial);
+  else if (rows <= 64) mx_rows_tile<4, SILU, PLANES>(p, a, r0, n0, partial);
+  else if (rows <= 96) mx_rows_tile<6, SILU, PLANES>(p, a, r0, n0, partial);
+  else if (rows <= 128) mx_rows_tile<8, SILU, PLANES>(p, a, r0, n0, partial);
+  else {
+    MxSums<8> sums;
+    MxBigMain<PLANES>::run(p, a, sums);
+    mx_tile_out<8, 8, SILU>(p, sums, __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) * 8, r0, rows, n0, partial);
+  }
 }
 
 // One weight: tile t, K part q.
-template <bool SILU>
-__global__ __launch_bounds__(256, 2) void mx_linear_kernel(MxParams p, MxSplit sp) {
+template <bool SILU, bool PLANES>
+__global__ __launch_bounds__(512, 1) void mx_linear_kernel(MxParams p, MxSplit sp) {
   const int tiles = sp.n_tiles * sp.m_tiles;
   const int l = xcd_run(blockIdx.x, tiles * sp.parts);
   if (l < 0) return;
@@ -496,54 +814,55 @@ __global__ __launch_bounds__(256, 2) void mx_linear_kernel(MxParams p, MxSplit s
   f32x4 *partial = sp.parts > 1 ? reinterpret_cast<f32x4 *>(sp.partial) + (size_t)(t * sp.parts + q) * (MX_PART_F32 / 4)
                                 : nullptr;
   mt = uniform(mt);
-  mx_tile_rows<SILU>(p, 0, mt * MX_ROWS, min(MX_ROWS, p.M - mt * MX_ROWS), uniform(nt), uniform(it0), uniform(it1), partial);
+  mx_tile<SILU, PLANES>(p, 0, mt * MX_ROWS, min(MX_ROWS, p.M - mt * MX_ROWS), uniform(nt), uniform(it0), uniform(it1), partial);
 }
 
-// Sums the K parts of row fragment j of a tile in part order.
+// Sums the K parts of activation fragment j of a tile in part order.
 template <bool SILU>
 __global__ __launch_bounds__(256) void mx_finish_kernel(MxParams p, MxSplit sp) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = blockIdx.x >> 3, j = blockIdx.x & 7;
+  const int t = blockIdx.x >> 4, j = blockIdx.x & 15;
   int nt, mt;
   tile_coords(t, sp.n_tiles, sp.m_tiles, nt, mt);
   if (mt * MX_ROWS + 16 * j >= p.M) return;
   const f32x4 *src = reinterpret_cast<const f32x4 *>(sp.partial) + (size_t)t * sp.parts * (MX_PART_F32 / 4) +
-                     (j * 4 + wave) * 64 + lane;
+                     j * 1024 + wave * 64 + lane;
   f32x4 v[4];
 #pragma unroll
-  for (int f = 0; f < 4; ++f) v[f] = src[f * 2048];
+  for (int f = 0; f < 4; ++f) v[f] = src[f * 256];
+#pragma unroll 4
   for (int q = 1; q < sp.parts; ++q)
 #pragma unroll
-    for (int f = 0; f < 4; ++f) v[f] += src[(size_t)q * (MX_PART_F32 / 4) + f * 2048];
+    for (int f = 0; f < 4; ++f) v[f] += src[(size_t)q * (MX_PART_F32 / 4) + f * 256];
   const int m = mt * MX_ROWS + 16 * j + (lane & 15);
   mx_tile_store<SILU>(p, v, wave, lane, m < p.M, m, m, nt * (SILU ? 128 : 256));
 }
 
-// The scheduled entries of up to 128 rows: a contiguous run of (entry, column
+// The scheduled entries of up to 256 rows: a contiguous run of (entry, column
 // tile) per XCD, so that the activation rows of an entry are read from one L2.
-template <bool SILU>
-__global__ __launch_bounds__(256, 2) void mx_sched_kernel(MxParams p, int ntiles) {
-  const int l = xcd_run(blockIdx.x, *p.count * ntiles);
+template <bool SILU, bool PLANES>
+__global__ __launch_bounds__(512, 1) void mx_sched_kernel(MxParams p, int ntiles) {
+  const int l = xcd_run(blockIdx.x, (p.count[0] + (p.rest ? p.count[1] : 0)) * ntiles);
   if (l < 0) return;
   const int t = uniform(l / ntiles), nt = uniform(l) - t * ntiles;
   const int32_t *en = p.ent + 4 * t;
   const int e = uniform(en[0]), r0 = uniform(en[1]), rows = uniform(en[2]);
   if (!SILU && e < 0) {  // rows of no expert
-    for (int i = threadIdx.x; i < rows * 64; i += 256) {
+    for (int i = threadIdx.x; i < rows * 64; i += 512) {
       const int r = i >> 6, n = nt * 256 + 4 * (i & 63);
       if (n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + r] : r0 + r, n, f32x4{0.f, 0.f, 0.f, 0.f});
     }
     return;
   }
-  mx_tile_rows<SILU>(p, e, r0, rows, nt, 0, p.K >> 7, nullptr);
+  mx_tile<SILU, PLANES>(p, e, r0, rows, nt, 0, p.K >> 7, nullptr);
 }
 
 // ---------------------------------------------------------------- schedules
 
 // Entries of the groups [offsets[e], offsets[e + 1]) of m rows, at most rows_max
 // rows each.  Offsets are taken as they come but never past m and never
-// backwards: bad ones lose rows, not bounds.  rest: the rows of no group as
-// entries of expert -1.
+// backwards: bad ones lose rows, not bounds.  count: the entries; with rest, the
+// rows of no group as count[1] more, of expert -1.
 __global__ __launch_bounds__(1024) void mx_group_kernel(const int32_t *__restrict__ offsets, int E, int m, int rows_max,
                                                         int rest, int32_t *__restrict__ count,
                                                         int32_t *__restrict__ ent) {
@@ -585,6 +904,7 @@ __global__ __launch_bounds__(1024) void mx_group_kernel(const int32_t *__restric
   }
   if (tid == 1023) {
     int c = n;
+    count[0] = n;
     if (rest) {
       const int lo[2] = {0, start[E]}, hi[2] = {start[0], m};
       for (int k = 0; k < 2; ++k)
@@ -593,7 +913,7 @@ __global__ __launch_bounds__(1024) void mx_group_kernel(const int32_t *__restric
           en[0] = -1; en[1] = r; en[2] = min(rows_max, hi[k] - r); en[3] = 0;
         }
     }
-    *count = c;
+    count[1] = c - n;
   }
 }
 
@@ -607,39 +927,77 @@ __global__ __launch_bounds__(256) void mx_clear_skipped_kernel(const int64_t *__
 
 // ---------------------------------------------------------------- launches
 
-// Waves of a skinny workgroup: K steps to share
-static int mx_waves(int K) { return K / 128 >= 16 ? 8 : 4; }
-
-template <int WT, int XT, bool FUSED, bool SILU>
-static int launch_skinny(const MxParams &p, int entries, hipStream_t st) {
-  const int cols = SILU ? 8 * WT : 16 * WT, ntiles = (p.N + cols - 1) / cols, nw = mx_waves(p.K);
-  const int64_t blocks = (int64_t)entries * ntiles;
-  if (blocks > INT32_MAX) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d entries", entries);
-  mx_skinny_kernel<WT, XT, FUSED, SILU><<<dim3((unsigned)blocks), 64 * nw, nw * WT * XT * 1024, st>>>(p, ntiles);
-  return check_launch("mxfp4 skinny product");
-}
-
-constexpr int MX_SKINNY_FUSED = 16;  // bf16 rows the skinny kernel quantises itself
-constexpr int MX_SKINNY = 64;        // most rows of an entry on it
-
-// entries of at most `rows` rows; p.xs null: bf16 rows (rows <= MX_SKINNY_FUSED)
-static int launch_mx_skinny(const MxParams &p, int rows, int entries, hipStream_t st) {
-  const bool wide = (int64_t)entries * (p.N / 32) >= 400;  // 32 weight rows a workgroup still fill the machine
-  if (!p.xs) return wide ? launch_skinny<2, 1, true, false>(p, entries, st) : launch_skinny<1, 1, true, false>(p, entries, st);
-  if (rows <= 16) return wide ? launch_skinny<2, 1, false, false>(p, entries, st) : launch_skinny<1, 1, false, false>(p, entries, st);
-  if (rows <= 32) return launch_skinny<2, 2, false, false>(p, entries, st);
-  return launch_skinny<2, 4, false, false>(p, entries, st);
-}
-static int launch_mx_skinny_silu(const MxParams &p, int rows, int entries, hipStream_t st) {
-  if (!p.xs) return launch_skinny<4, 1, true, true>(p, entries, st);
-  return launch_skinny<4, 1, false, true>(p, entries, st);
-}
-
 template <typename F>
-static int mx_lds(F *fn) {  // dynamic LDS above 64 KB
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           MxLds<4>::BYTES);
-  return e == hipSuccess ? AMLA_OK : fail((int)e, "mxfp4 tiles: LDS size: %s", hipGetErrorString(e));
+static int mx_lds(F *fn, int bytes) {  // dynamic LDS above 64 KB
+  if (bytes <= 64 * 1024) return AMLA_OK;
+  const hipError_t e =
+      hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == hipSuccess ? AMLA_OK : fail((int)e, "mxfp4 product: LDS size: %s", hipGetErrorString(e));
+}
+
+// Activation rows kept of a fragment, and fragments, for entries of at most `rows` rows
+static int mx_keep(int rows) {
+  int mr = 1;
+  while (mr < rows && mr < 16) mr *= 2;
+  return mr;
+}
+static int mx_fragments(int rows) { return (rows + 15) / 16; }
+static int64_t mx_stream_bytes(int rows, int64_t K) { return (int64_t)mx_keep(rows) * mx_fragments(rows) * (K / 2 + (K + 511) / 512 * 16); }
+// waves of a workgroup: equal runs of quads where there are any
+static int mx_waves(int64_t K) {
+  const int quads = (int)((K + 511) / 512);
+  int best = 1;
+  double cost = 1e9;
+  for (int w = 1; w <= std::min(8, quads); ++w) {
+    const double c = (double)((quads + w - 1) / w) * w / quads + 0.25 / w;
+    if (c < cost) {
+      cost = c;
+      best = w;
+    }
+  }
+  return best;
+}
+
+static int64_t mx_stream_lds(int rows, int64_t K, bool silu) {  // with two items' partial sums
+  return mx_stream_bytes(rows, K) + 2048 * mx_waves(K) * mx_fragments(rows) * (silu ? 4 : 1);
+}
+static bool mx_stream_fits(int rows, int64_t K, bool silu) {
+  return rows <= (silu ? 16 : 64) && mx_stream_lds(rows, K, silu) <= 160 * 1024;
+}
+
+template <int XT, bool SILU>
+static int launch_stream(const MxParams &p, int rows, int entries, hipStream_t st) {
+  MxStream sp;
+  sp.ntiles = (p.N + (SILU ? 31 : 15)) / (SILU ? 32 : 16);
+  sp.mr = mx_keep(rows);
+  sp.xcodes = sp.mr * XT * (p.K >> 1);
+  sp.xbytes = (int)mx_stream_bytes(rows, p.K);
+  const int nw = mx_waves(p.K);
+  const int lds = (int)mx_stream_lds(rows, p.K, SILU);
+  // three items or more a workgroup (each takes in the activations for itself), up to
+  // 16 waves a CU.  18432 x 7168, one row: 256 workgroups 19.6 us, 512 22.0; 24576 x
+  // 1536, 8 rows: 512 9.0, 1280 9.8; 57 experts of 7168 x 2048: 256 110, 1024 75.
+  const int64_t items = (int64_t)entries * sp.ntiles;
+  const int per_cu = std::max<int>(1, (int)std::min<int64_t>({16 / nw, 160 * 1024 / lds, items / (3 * 256)}));
+  const unsigned blocks = (unsigned)std::min<int64_t>(items, 256 * per_cu);
+  const auto kernel = p.K % 512 ? mx_stream_kernel<XT, SILU, true> : mx_stream_kernel<XT, SILU, false>;
+  const int rc = mx_lds(kernel, lds);
+  if (rc) return rc;
+  kernel<<<dim3(blocks), 64 * nw, lds, st>>>(p, sp);
+  return check_launch("mxfp4 stream product");
+}
+
+// Entries of at most `rows` <= 64 rows, bf16 rows where p.xs is null.
+static int launch_mx_stream(const MxParams &p, int rows, int entries, hipStream_t st) {
+  switch (mx_fragments(rows)) {
+    case 1: return launch_stream<1, false>(p, rows, entries, st);
+    case 2: return launch_stream<2, false>(p, rows, entries, st);
+    case 3: return launch_stream<3, false>(p, rows, entries, st);
+    default: return launch_stream<4, false>(p, rows, entries, st);
+  }
+}
+static int launch_mx_stream_silu(const MxParams &p, int rows, int entries, hipStream_t st) {
+  return launch_stream<1, true>(p, rows, entries, st);
 }
 
 static MxSplit plan_mx_split(int64_t M, int N, int K, bool silu) {
@@ -657,14 +1015,15 @@ static size_t mx_split_bytes(const MxSplit &sp) {
 }
 
 template <bool SILU>
-static int launch_mx_linear(const MxParams &p, MxSplit sp, hipStream_t st) {
+static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st) {
   const int64_t blocks = ((int64_t)sp.n_tiles * sp.m_tiles * sp.parts + 7) / 8 * 8;
-  if (blocks > INT32_MAX) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
-  int rc = mx_lds(mx_linear_kernel<SILU>);
+  if (blocks > INT32_MAX / 16) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
+  const auto kernel = p.K % 512 ? mx_linear_kernel<SILU, true> : mx_linear_kernel<SILU, false>;
+  int rc = mx_lds(kernel, MX_TILE_LDS);
   if (rc) return rc;
-  mx_linear_kernel<SILU><<<dim3((unsigned)blocks), 256, MxLds<4>::BYTES, st>>>(p, sp);
+  kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, sp);
   if ((rc = check_launch("mxfp4 product")) || sp.parts == 1) return rc;
-  mx_finish_kernel<SILU><<<dim3((unsigned)(sp.n_tiles * sp.m_tiles * 8)), 256, 0, st>>>(p, sp);
+  mx_finish_kernel<SILU><<<dim3((unsigned)(sp.n_tiles * sp.m_tiles * 16)), 256, 0, st>>>(p, sp);
   return check_launch("mxfp4 K-part finish");
 }
 
@@ -673,9 +1032,10 @@ static int launch_mx_sched(const MxParams &p, int max_entries, hipStream_t st) {
   const int cols = SILU ? 128 : 256, ntiles = (p.N + cols - 1) / cols;
   const int64_t blocks = ((int64_t)max_entries * ntiles + 7) / 8 * 8;
   if (blocks > INT32_MAX) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d entries", max_entries);
-  int rc = mx_lds(mx_sched_kernel<SILU>);
+  const auto kernel = p.K % 512 ? mx_sched_kernel<SILU, true> : mx_sched_kernel<SILU, false>;
+  const int rc = mx_lds(kernel, MX_TILE_LDS);
   if (rc) return rc;
-  mx_sched_kernel<SILU><<<dim3((unsigned)blocks), 256, MxLds<4>::BYTES, st>>>(p, ntiles);
+  kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, ntiles);
   return check_launch("mxfp4 grouped product");
 }
 
@@ -694,19 +1054,21 @@ static size_t mx_scale_bytes(int64_t rows, int64_t k) { return (size_t)rows * (k
 
 struct MxLinearLayout {
   size_t xc, xs, part, total;
-  bool skinny;
+  bool stream, fused;  // fused: the stream product quantises
   MxSplit sp;
 };
+constexpr int64_t MX_FUSED = 32 * 1024;  // values of x that each workgroup may quantise for itself
 // held: x comes quantised
 static MxLinearLayout mx_linear_layout(int64_t m, int64_t k, int64_t n, bool held) {
   MxLinearLayout L = {};
   MxTake take;
-  L.skinny = m <= MX_SKINNY;
-  if (!held && m > MX_SKINNY_FUSED) {
+  L.stream = m <= 64 && mx_stream_fits((int)m, k, false);
+  L.fused = L.stream && m * k <= MX_FUSED;
+  if (!held && !L.fused) {
     L.xc = take(mx_codes_bytes(m, k));
     L.xs = take(mx_scale_bytes(m, k));
   }
-  if (!L.skinny) {
+  if (!L.stream) {
     L.sp = plan_mx_split(m, (int)n, (int)k, false);
     L.part = take(mx_split_bytes(L.sp));
   }
@@ -717,17 +1079,17 @@ static MxLinearLayout mx_linear_layout(int64_t m, int64_t k, int64_t n, bool hel
 struct MxGroupedLayout {
   size_t count, ent, xc, xs, total;
   int rows, max_entries;  // of an entry; entries at most
-  bool skinny;
+  bool stream;
 };
 static MxGroupedLayout mx_grouped_layout(int64_t m, int64_t k, int64_t E, bool held) {
   MxGroupedLayout L = {};
   MxTake take;
-  L.skinny = m <= 16;
-  L.rows = L.skinny ? 16 : MX_ROWS;
+  L.stream = m <= 16 && mx_stream_fits((int)m, k, false);
+  L.rows = L.stream ? 16 : MX_ROWS;
   L.max_entries = (int)(std::min(E, m) + m / L.rows + 2);
-  L.count = take(4);
+  L.count = take(8);
   L.ent = take((size_t)L.max_entries * 16);
-  if (!held && !L.skinny) {
+  if (!held && !L.stream) {
     L.xc = take(mx_codes_bytes(m, k));
     L.xs = take(mx_scale_bytes(m, k));
   }
@@ -737,23 +1099,23 @@ static MxGroupedLayout mx_grouped_layout(int64_t m, int64_t k, int64_t E, bool h
 
 struct MxSwigluLayout {
   size_t xc, xs, hc, hs, lin, total;
-  bool skinny;
+  bool stream;
   MxSplit sp;
   MxLinearLayout down;
 };
 static MxSwigluLayout mx_swiglu_layout(int64_t m, int64_t k, int64_t n) {
   MxSwigluLayout L = {};
   MxTake take;
-  L.skinny = m <= MX_SKINNY_FUSED;
+  L.stream = m <= 16 && mx_stream_fits((int)m, k, true);
   L.hc = take(mx_codes_bytes(m, n));
   L.hs = take(mx_scale_bytes(m, n));
-  if (!L.skinny) {
+  if (!L.stream) {
     L.xc = take(mx_codes_bytes(m, k));
     L.xs = take(mx_scale_bytes(m, k));
     L.sp = plan_mx_split(m, (int)n, (int)k, true);
   }
   L.down = mx_linear_layout(m, n, k, true);
-  L.lin = take(std::max(L.skinny ? 0 : mx_split_bytes(L.sp), L.down.total));
+  L.lin = take(std::max(L.stream ? 0 : mx_split_bytes(L.sp), L.down.total));
   L.total = take.off;
   return L;
 }
@@ -761,14 +1123,14 @@ static MxSwigluLayout mx_swiglu_layout(int64_t m, int64_t k, int64_t n) {
 struct MxMoeLayout {
   size_t hdr, count, gather, scatter, ent, xc, xs, hc, hs, total;
   int rows, max_entries;
-  bool skinny;
+  bool stream;
 };
 static MxMoeLayout mx_moe_layout(int64_t m, int64_t d, int top_k, int64_t n, int64_t E) {
   MxMoeLayout L = {};
   MxTake take;
   const int64_t S = m * top_k;
-  L.skinny = m <= 16;
-  L.rows = L.skinny ? 16 : MX_ROWS;
+  L.stream = m <= 16 && mx_stream_fits((int)m, d, true) && mx_stream_fits((int)m, n, false);
+  L.rows = L.stream ? 16 : MX_ROWS;
   L.max_entries = (int)std::min<int64_t>(S, std::min<int64_t>(E, S) + S / L.rows);
   L.hdr = take(16);
   L.count = take(4);
@@ -777,7 +1139,7 @@ static MxMoeLayout mx_moe_layout(int64_t m, int64_t d, int top_k, int64_t n, int
   L.ent = take((size_t)L.max_entries * 16);
   L.hc = take(mx_codes_bytes(S, n));
   L.hs = take(mx_scale_bytes(S, n));
-  if (!L.skinny) {
+  if (!L.stream) {
     L.xc = take(mx_codes_bytes(m, d));
     L.xs = take(mx_scale_bytes(m, d));
   }
@@ -835,13 +1197,13 @@ int amla_mxfp4_linear(const void *x, const void *x_scales, int64_t m, int64_t k,
   p.ws[0] = p.ws[1] = static_cast<const uint8_t *>(scales);
   p.M = (int)m; p.N = (int)n; p.K = (int)k;
   mx_outputs(p, y, ldy, dtype);
-  if (!x_scales && m > MX_SKINNY_FUSED) {
+  if (!x_scales && !L.fused) {
     const int rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(x), m, k, ldx, ws + L.xc, ws + L.xs, st);
     if (rc) return rc;
     p.x = ws + L.xc;
     p.xs = ws + L.xs;
   }
-  if (L.skinny) return launch_mx_skinny(p, (int)m, 1, st);
+  if (L.stream) return launch_mx_stream(p, (int)m, 1, st);
   MxSplit sp = L.sp;
   sp.partial = reinterpret_cast<float *>(ws + L.part);
   return launch_mx_linear<false>(p, sp, st);
@@ -888,9 +1250,10 @@ int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, in
   p.sstride = n * (k / 32);
   p.ent = ent;
   p.count = count;
+  p.rest = clear_rest != 0;
   p.M = (int)m; p.N = (int)n; p.K = (int)k;
   mx_outputs(p, y, ldy, dtype);
-  if (L.skinny) return launch_mx_skinny(p, L.rows, L.max_entries, st);
+  if (L.stream) return launch_mx_stream(p, (int)m, (int)std::min<int64_t>(n_experts, m), st);
   if (!x_scales) {
     if ((rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(x), m, k, ldx, ws + L.xc, ws + L.xs, st))) return rc;
     p.x = ws + L.xc;
@@ -937,8 +1300,8 @@ int amla_mxfp4_swiglu(const void *x, int64_t m, int64_t k, int64_t ldx, const vo
   p.hc = ws + L.hc;
   p.hs = ws + L.hs;
   int rc;
-  if (L.skinny) {
-    rc = launch_mx_skinny_silu(p, (int)m, 1, st);
+  if (L.stream) {
+    rc = launch_mx_stream_silu(p, (int)m, 1, st);
   } else {
     if ((rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(x), m, k, ldx, ws + L.xc, ws + L.xs, st))) return rc;
     p.x = ws + L.xc;
@@ -1017,9 +1380,9 @@ int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh
   q.ws[0] = q.ws[1] = static_cast<const uint8_t *>(down_s);
   q.N = (int)d; q.K = (int)n_inter;
   mx_outputs(q, expert_out, d, AMLA_BF16);
-  if (L.skinny) {
-    if ((rc = launch_mx_skinny_silu(p, L.rows, L.max_entries, st))) return rc;
-    return launch_mx_skinny(q, L.rows, L.max_entries, st);
+  if (L.stream) {
+    if ((rc = launch_mx_stream_silu(p, (int)m, L.max_entries, st))) return rc;
+    return launch_mx_stream(q, (int)m, L.max_entries, st);
   }
   if ((rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(hidden), m, d, ldh, ws + L.xc, ws + L.xs, st)))
     return rc;
