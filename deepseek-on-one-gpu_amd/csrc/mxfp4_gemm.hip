@@ -28,7 +28,7 @@ struct MxParams {
   int rest;            // count[1] entries of expert -1 come behind the others
   void *y;
   int64_t ldy;
-  int f32, vec;        // fp32 outputs; four outputs per store
+  int f32, vec, vec16; // fp32 outputs; four outputs, 16 bytes of them per store
   uint8_t *hc, *hs;    // SILU: codes and exponents by position
 };
 
@@ -502,7 +502,8 @@ struct MxRowsMain {
       const f32x4 o = ex[(((wave ^ 4) * 4 + f) * (XF / 2) + j) * 64];
       acc[f][j] = wk ? o + acc[f][XF / 2 + j] : acc[f][j] + o;
     }
-  __builtin_amdgcn_s_barrier();  // (the slots may be copied into again)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();  // (LDS is free)
 }
 };
 
@@ -691,42 +692,95 @@ struct MxBigMain {
 #pragma unroll
     for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[f][j]));
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();  // (the slots may be copied into again)
+  __builtin_amdgcn_s_barrier();  // (LDS is free)
 }
 };
 
-// Outputs of activation row m (from the tile's position r0; n0 first output, ncols
-// of them): v[f] as the lane holds them, fragment f of segment f / 2, outputs
-// 32 wave + 16 (f % 2) + 4 g .. +3.
-template <bool SILU>
-AMLA_DEV void mx_tile_store(const MxParams &p, const f32x4 (&v)[4], int wave, int lane, bool live, int pos, int64_t yrow,
-                            int n0) {
-  const int g = lane >> 4;
+// Stores a tile of `rows` positions from r0, outputs from n0.  The threads hold it as
+// v(j)[f], activation fragment j of j0 .. j0 + XF - 1, weight fragment f: row 16 j +
+// lane % 16, outputs 128 (f / 2) + 32 wn + 16 (f % 2) + 4 (lane / 16) .. +3.  Rows go
+// through LDS, so that every store is 16 bytes of a run of 512 in one row: stores from
+// where the sums are held, 32 bytes in each of 16 rows, reach 1.7 TB/s (down
+// projection of 16000 routed rows 505 us, 370 without its stores).
+constexpr int MX_PITCH_Y = 512 + 16, MX_PITCH_H = 64 + 16;
+template <int XF, bool SILU, typename V>
+AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, int r0, int n0) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  auto meet = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
   if constexpr (SILU) {
     // the four lanes of a row hold its block of 32: eight values each
-    float h[8];
-    uint32_t am = 0;
+    uint8_t *hs = lds + MX_PITCH_H * 256;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[i] = mx_silu_mul(v[i >> 2][i & 3], v[2 + (i >> 2)][i & 3]);
-      am = max(am, __float_as_uint(h[i]) & 0x7fffffffu);
+    for (int j = 0; j < XF; ++j) {
+      const auto t = v(j);
+      float h[8];
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        h[i] = mx_silu_mul(t.f[i >> 2][i & 3], t.f[2 + (i >> 2)][i & 3]);
+        am = max(am, __float_as_uint(h[i]) & 0x7fffffffu);
+      }
+      am = max(am, (uint32_t)__shfl_xor((int)am, 16, 64));
+      am = max(am, (uint32_t)__shfl_xor((int)am, 32, 64));
+      const uint32_t byte = mx_byte(am);
+      uint32_t q = mx_codes8(h, mx_scale(byte));
+      if (byte == 255) q = 0;
+      const int m = 16 * (j0 + j) + r16;
+      *reinterpret_cast<uint16_t *>(lds + MX_PITCH_H * m + 16 * wn + 2 * g) = (uint16_t)q;
+      *reinterpret_cast<uint16_t *>(lds + MX_PITCH_H * m + 16 * wn + 2 * g + 8) = (uint16_t)(q >> 16);
+      if (g == 0) hs[4 * m + wn] = (uint8_t)byte;
     }
-    am = max(am, (uint32_t)__shfl_xor((int)am, 16, 64));
-    am = max(am, (uint32_t)__shfl_xor((int)am, 32, 64));
-    const uint32_t byte = mx_byte(am);
-    uint32_t q = mx_codes8(h, mx_scale(byte));
-    if (byte == 255) q = 0;
-    if (!live) return;
-    uint8_t *hc = p.hc + (int64_t)pos * (p.N >> 1) + ((n0 + 32 * wave) >> 1) + 2 * g;
-    *reinterpret_cast<uint16_t *>(hc) = (uint16_t)q;
-    *reinterpret_cast<uint16_t *>(hc + 8) = (uint16_t)(q >> 16);
-    if (g == 0) p.hs[(int64_t)pos * (p.N >> 5) + (n0 >> 5) + wave] = (uint8_t)byte;
-  } else {
-    if (!live) return;
+    meet();
+    for (int i = tid; i < rows * 4; i += threads)
+      *reinterpret_cast<u32x4 *>(p.hc + (int64_t)(r0 + (i >> 2)) * (p.N >> 1) + (n0 >> 1) + 16 * (i & 3)) =
+          ldg16(lds + MX_PITCH_H * (i >> 2) + 16 * (i & 3));
+    for (int i = tid; i < rows; i += threads)
+      *reinterpret_cast<uint32_t *>(p.hs + (int64_t)(r0 + i) * (p.N >> 5) + (n0 >> 5)) =
+          *reinterpret_cast<const uint32_t *>(hs + 4 * i);
+  } else if (!p.vec16) {  // any stride and alignment
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      const int n = n0 + (f >> 1) * 128 + 32 * wave + 16 * (f & 1) + 4 * g;
-      if (n < p.N) mx_store4(p, yrow, n, v[f]);
+    for (int j = 0; j < XF; ++j) {
+      const auto t = v(j);
+      const int m = 16 * (j0 + j) + r16;
+      if (m >= rows) continue;
+      const int64_t yr = p.yrow ? p.yrow[r0 + m] : r0 + m;
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const int n = n0 + (f >> 1) * 128 + 32 * wn + 16 * (f & 1) + 4 * g;
+        if (n < p.N) mx_store4(p, yr, n, t.f[f]);
+      }
+    }
+  } else {
+    // bf16: both segments of a row; fp32: one after the other
+    for (int s = 0; s < (p.f32 ? 2 : 1); ++s) {
+      if (s) meet();
+#pragma unroll
+      for (int j = 0; j < XF; ++j) {
+        const auto t = v(j);
+        uint8_t *row = lds + MX_PITCH_Y * (16 * (j0 + j) + r16);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const int c = 32 * wn + 16 * (f & 1) + 4 * g;
+          if (!p.f32)
+            *reinterpret_cast<u32x2 *>(row + 2 * (128 * (f >> 1) + c)) =
+                u32x2{pack_bf16(t.f[f].x, t.f[f].y), pack_bf16(t.f[f].z, t.f[f].w)};
+          else if (f >> 1 == s)
+            *reinterpret_cast<f32x4 *>(row + 4 * c) = t.f[f];
+        }
+      }
+      meet();
+      const int per = p.f32 ? 4 : 8, n = n0 + 128 * s + per * (tid & 31);
+      if (n < p.N)
+        for (int r = tid >> 5; r < rows; r += threads >> 5) {
+          const int64_t yr = p.yrow ? p.yrow[r0 + r] : r0 + r;
+          *reinterpret_cast<u32x4 *>(static_cast<uint8_t *>(p.y) + (yr * p.ldy + n) * (p.f32 ? 4 : 2)) =
+              ldg16(lds + MX_PITCH_Y * r + 16 * (tid & 31));
+        }
     }
   }
 }
@@ -738,6 +792,8 @@ struct MxSplit {
 };
 constexpr int MX_ROWS = 256;  // activation rows of a tile
 constexpr int MX_PART_F32 = 256 * MX_ROWS;
+constexpr int MX_FINISH_LDS = MX_PITCH_H * 256 + 4 * 16;  // exponents behind the most rows' codes
+static_assert(MX_FINISH_LDS >= 16 * MX_PITCH_Y && 256 * MX_PITCH_Y <= MX_TILE_LDS, "staged rows");
 
 template <bool SILU>
 AMLA_DEV MxTile mx_tile_of(const MxParams &p, int e, int r0, int rows, int n0, int it0, int it1) {
@@ -758,23 +814,22 @@ AMLA_DEV MxTile mx_tile_of(const MxParams &p, int e, int r0, int rows, int n0, i
   return a;
 }
 
-// Stores fragments j0 .. j0 + XF - 1 of a tile, held as acc[.][0 .. XF - 1].
+// The fragments j0 .. j0 + XF - 1 of a tile, held as acc[.][0 .. XF - 1].
+struct MxFrag {
+  f32x4 f[4];
+};
 template <int XF, int HELD, bool SILU>
 AMLA_DEV void mx_tile_out(const MxParams &p, const MxSums<HELD> &sums, int j0, int r0, int rows, int n0, f32x4 *partial) {
-  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15;
-  const int wn = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const int lane = threadIdx.x & 63, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  if (partial) {
 #pragma unroll
-  for (int j = 0; j < XF; ++j) {
-    const f32x4 v[4] = {sums.acc[0][j], sums.acc[1][j], sums.acc[2][j], sums.acc[3][j]};
-    if (partial) {
+    for (int j = 0; j < XF; ++j)
 #pragma unroll
-      for (int f = 0; f < 4; ++f) partial[(((j0 + j) * 4 + f) * 4 + wn) * 64 + lane] = v[f];
-      continue;
-    }
-    const int m = 16 * (j0 + j) + r16;
-    const int pos = r0 + min(m, rows - 1);
-    mx_tile_store<SILU>(p, v, wn, lane, m < rows, pos, p.yrow ? p.yrow[pos] : pos, n0);
+      for (int f = 0; f < 4; ++f) partial[(((j0 + j) * 4 + f) * 4 + wn) * 64 + lane] = sums.acc[f][j];
+    return;
   }
+  mx_tile_store<XF, SILU>(
+      p, [&](int j) { return MxFrag{{sums.acc[0][j], sums.acc[1][j], sums.acc[2][j], sums.acc[3][j]}}; }, j0, wn, rows, r0, n0);
 }
 
 template <int XF, bool SILU, bool PLANES>
@@ -834,8 +889,9 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(MxParams p, MxSplit sp) 
   for (int q = 1; q < sp.parts; ++q)
 #pragma unroll
     for (int f = 0; f < 4; ++f) v[f] += src[(size_t)q * (MX_PART_F32 / 4) + f * 256];
-  const int m = mt * MX_ROWS + 16 * j + (lane & 15);
-  mx_tile_store<SILU>(p, v, wave, lane, m < p.M, m, m, nt * (SILU ? 128 : 256));
+  const int m0 = mt * MX_ROWS + 16 * j;
+  mx_tile_store<1, SILU>(p, [&](int) { return MxFrag{{v[0], v[1], v[2], v[3]}}; }, 0, wave, min(16, p.M - m0), m0,
+                         nt * (SILU ? 128 : 256));
 }
 
 // The scheduled entries of up to 256 rows: a contiguous run of (entry, column
@@ -1023,7 +1079,7 @@ static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st
   if (rc) return rc;
   kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, sp);
   if ((rc = check_launch("mxfp4 product")) || sp.parts == 1) return rc;
-  mx_finish_kernel<SILU><<<dim3((unsigned)(sp.n_tiles * sp.m_tiles * 16)), 256, 0, st>>>(p, sp);
+  mx_finish_kernel<SILU><<<dim3((unsigned)(sp.n_tiles * sp.m_tiles * 16)), 256, MX_FINISH_LDS, st>>>(p, sp);
   return check_launch("mxfp4 K-part finish");
 }
 
@@ -1155,6 +1211,7 @@ static void mx_outputs(MxParams &p, void *y, int64_t ldy, int dtype) {
   p.y = y;
   p.ldy = ldy;
   p.f32 = dtype == AMLA_FP32;
+  p.vec16 = p.N % (p.f32 ? 4 : 8) == 0 && ldy % (p.f32 ? 4 : 8) == 0 && aligned16(y);
   p.vec = p.N % 4 == 0 && ldy % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (p.f32 ? 16 : 8) == 0;
 }
 
