@@ -1186,7 +1186,7 @@ static MxMoeLayout mx_moe_layout(int64_t m, int64_t d, int top_k, int64_t n, int
   MxTake take;
   const int64_t S = m * top_k;
   L.stream = m <= 16 && mx_stream_fits((int)m, d, true) && mx_stream_fits((int)m, n, false);
-  L.rows = L.stream ? 16 : MX_ROWS;
+  L.rows = L.stream ? (int)m : MX_ROWS;  // (a token may name an expert several times: more entries)
   L.max_entries = (int)std::min<int64_t>(S, std::min<int64_t>(E, S) + S / L.rows);
   L.hdr = take(16);
   L.count = take(4);

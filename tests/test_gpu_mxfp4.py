@@ -157,6 +157,20 @@ def test_linear_shapes_strides_and_types():
     _check(ops.mxfp4_linear(odd, *w), y[:4], slack[:4], "base off the 16-byte grid")
 
 
+@pytest.mark.parametrize("m", [1, 70, 130])
+@pytest.mark.parametrize("k", [1024, 1152])
+def test_linear_with_exponents_off_the_16_byte_grid(m, k):
+    g = _gen(m + k)
+    x, (c, s) = _x(g, m, k).to(DEV), _weight(g, 300, k)
+    moved = torch.empty(s.numel() + 4, dtype=torch.uint8, device=DEV)[4:].view(s.shape).copy_(s)
+    assert moved.data_ptr() % 16 == 4 and moved.is_contiguous()
+    assert torch.equal(ops.mxfp4_linear(x, c, moved), ops.mxfp4_linear(x, c, s))
+    xc, xs = ops.mxfp4_quantize(x)
+    for off in (4, 1):
+        held = torch.empty(xs.numel() + off, dtype=torch.uint8, device=DEV)[off:].view(xs.shape).copy_(xs)
+        assert torch.equal(ops.mxfp4_linear((xc, held), c, moved), ops.mxfp4_linear((xc, xs), c, s))
+
+
 @pytest.mark.parametrize("m", [1, 40, 200])
 def test_linear_nan_blocks_stay_in_their_row_and_column(m):
     g = _gen(m)
@@ -220,6 +234,24 @@ def test_grouped_offsets_past_the_end_or_backwards_stay_in_bounds(m):
         assert (got[lo:hi] - full[e][lo:hi]).abs().max() <= 2.0 ** -7 * full[e][lo:hi].abs().max()
 
 
+@pytest.mark.parametrize("E", [1023, 1024])
+@pytest.mark.parametrize("m", [9, 600])
+def test_grouped_linear_of_the_most_groups(E, m):
+    g = _gen(E + m)
+    w = _weight(g, E, 16, 128)
+    cuts = torch.sort(torch.randint(0, m + 1, (E + 1,), generator=g)).values
+    cuts[0], cuts[-1] = 0, m
+    cuts[-2] = min(int(cuts[-2]), m - 1)  # (the last group has rows)
+    cuts = torch.cummax(torch.minimum(cuts, torch.tensor([m - 1] * E + [m])), 0).values
+    x = _x(g, m, 128)
+    group = torch.bucketize(torch.arange(m), cuts, right=True) - 1
+    wv, xq = _vals(w), M.rounded(x)
+    y = (xq[:, None, :] * wv[group]).sum(-1)
+    mag = (xq[:, None, :].abs() * wv[group].abs()).sum(-1)
+    _check(ops.mxfp4_grouped_linear(x.to(DEV), *w, cuts.int().to(DEV)), y, M.linear_slack(mag, 128, HALF_STEP[BF16], y),
+           f"{m} rows in {E} groups")
+
+
 # ------------------------------------------------------------------ swiglu and experts
 
 def _ffn(g, d, n, E=None):
@@ -258,6 +290,19 @@ def test_moe_experts(m, d, n, E, top_k):
     got = ops.mxfp4_moe_experts(x.to(DEV), idx.to(DEV), w)
     _check(got, want, slack + HALF_STEP[BF16] * want.abs() + 2.0 ** -8 * slack, f"experts {m} {d} {n} {E} {top_k}")
     assert torch.equal(got, ops.mxfp4_moe_experts(x.to(DEV), idx.to(DEV), w))
+
+
+@pytest.mark.parametrize("m,top_k", [(1, 8), (2, 20), (3, 8), (5, 64), (16, 5)])
+def test_moe_experts_with_one_expert_for_every_slot(m, top_k):
+    """More rows for an expert than there are tokens: the slots of a token are equal rows."""
+    g = _gen(m * top_k)
+    x, w = _x(g, m, 640).to(DEV), _ffn(g, 640, 256, 3)
+    once = ops.mxfp4_moe_experts(x, torch.ones(m, 1, dtype=torch.int64, device=DEV), w)
+    vals = {key: _vals((w[key][0][1], w[key][1][1])) for key in w}
+    y, slack = M.swiglu(M.rounded(x.cpu()), vals["gate_proj"], vals["up_proj"], vals["down_proj"])
+    _check(once[:, 0], y, slack + HALF_STEP[BF16] * y.abs() + 2.0 ** -8 * slack, "one slot a token")
+    got = ops.mxfp4_moe_experts(x, torch.ones(m, top_k, dtype=torch.int64, device=DEV), w)
+    assert torch.equal(got, once.expand(m, top_k, 640))
 
 
 @pytest.mark.parametrize("tokens", [3, 40])
