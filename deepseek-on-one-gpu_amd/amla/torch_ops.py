@@ -244,12 +244,19 @@ _mx_lib = torch.library.Library("amla", "FRAGMENT")
 _mx_impl: dict = {}
 
 
+def _on_device(fn, t: Tensor, *args):
+    if t.device.index == torch.cuda.current_device():
+        return fn(t, *args)
+    with torch.cuda.device(t.device):
+        return fn(t, *args)
+
+
 def _mx_op(schema: str, fake):
     """Registers amla::<schema> with its ROCm implementation and its fake one."""
     def wrap(fn):
         name = schema.split("(")[0]
         _mx_lib.define(schema)
-        _mx_lib.impl(name, fn, "CUDA")
+        _mx_lib.impl(name, lambda t, *args: _on_device(fn, t, *args), "CUDA")
         torch.library.register_fake(f"amla::{name}", fake, lib=_mx_lib)
         _mx_impl[name] = fn
         return fn
@@ -260,10 +267,7 @@ def call(name: str, t: Tensor, *args):
     """The implementation of amla::<name>, or the operator itself where something traces the call."""
     if type(t) is not Tensor and not isinstance(t, torch.nn.Parameter) or torch.compiler.is_compiling():
         return getattr(torch.ops.amla, name)(t, *args)
-    if t.device.index == torch.cuda.current_device():
-        return _mx_impl[name](t, *args)
-    with torch.cuda.device(t.device):
-        return _mx_impl[name](t, *args)
+    return _on_device(_mx_impl[name], t, *args)
 
 
 # (the workspaces' sizes are functions of the call's sizes alone)
@@ -402,7 +406,7 @@ def _mxfp4_swiglu(x, gate_proj, gate_scale, up_proj, up_scale, down_proj, down_s
     return y
 
 
-_MX_MOE_SLOTS = 65536  # (token, k) slots of one call
+_MX_MOE_SLOTS, _MX_MOE_CODES = 65536, 2 ** 32 - 1  # (token, k) slots and bytes of codes of one call
 
 
 @_mx_op("mxfp4_moe_experts(Tensor hidden, Tensor indices, Tensor gate_proj, Tensor gate_scale, Tensor up_proj, "
@@ -414,7 +418,7 @@ def _mxfp4_moe_experts(hidden, indices, gate_proj, gate_scale, up_proj, up_scale
     E, n, d = gate_proj.shape[0], gate_proj.shape[1], hidden.shape[1]
     out = torch.empty(m, top_k, d, dtype=BF16, device=hidden.device)
     L = lib()
-    step = _MX_MOE_SLOTS // top_k
+    step = min(_MX_MOE_SLOTS // top_k, _MX_MOE_CODES // (d // 2))
     for t in range(0, m, step):
         c = min(step, m - t)
         need = _mx_moe_bytes(c, d, top_k, n, E)

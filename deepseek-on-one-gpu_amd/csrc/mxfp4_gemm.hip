@@ -983,6 +983,8 @@ __global__ __launch_bounds__(256) void mx_clear_skipped_kernel(const int64_t *__
 
 // ---------------------------------------------------------------- launches
 
+constexpr int64_t MX_MAX_BLOCKS = (1 << 23) - 8;  // of 512 threads, fewer than 2^32 a launch
+
 template <typename F>
 static int mx_lds(F *fn, int bytes) {  // dynamic LDS above 64 KB
   if (bytes <= 64 * 1024) return AMLA_OK;
@@ -1073,7 +1075,7 @@ static size_t mx_split_bytes(const MxSplit &sp) {
 template <bool SILU>
 static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st) {
   const int64_t blocks = ((int64_t)sp.n_tiles * sp.m_tiles * sp.parts + 7) / 8 * 8;
-  if (blocks > INT32_MAX / 16) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
+  if (blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
   const auto kernel = p.K % 512 ? mx_linear_kernel<SILU, true> : mx_linear_kernel<SILU, false>;
   int rc = mx_lds(kernel, MX_TILE_LDS);
   if (rc) return rc;
@@ -1087,7 +1089,7 @@ template <bool SILU>
 static int launch_mx_sched(const MxParams &p, int max_entries, hipStream_t st) {
   const int cols = SILU ? 128 : 256, ntiles = (p.N + cols - 1) / cols;
   const int64_t blocks = ((int64_t)max_entries * ntiles + 7) / 8 * 8;
-  if (blocks > INT32_MAX) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d entries", max_entries);
+  if (blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d entries", max_entries);
   const auto kernel = p.K % 512 ? mx_sched_kernel<SILU, true> : mx_sched_kernel<SILU, false>;
   const int rc = mx_lds(kernel, MX_TILE_LDS);
   if (rc) return rc;
@@ -1207,6 +1209,13 @@ static bool mx_sizes_ok(int64_t m, int64_t n, int64_t k) {
   return m > 0 && n > 0 && k > 0 && m <= INT32_MAX && n <= INT32_MAX / 4 && k <= (1 << 24) && k % 128 == 0;
 }
 
+// (both products of an FFN: k to n and n to k)
+static bool mx_ffn_sizes_ok(int64_t m, int64_t n, int64_t k) { return mx_sizes_ok(m, n, k) && mx_sizes_ok(m, k, n); }
+static bool mx_moe_sizes_ok(int64_t m, int64_t d, int64_t top_k, int64_t n, int64_t E) {
+  return top_k > 0 && top_k <= 64 && E > 0 && E <= 512 && m <= 65536 && m * top_k <= 65536 && mx_ffn_sizes_ok(m, n, d) &&
+         m * (d / 2) <= UINT32_MAX;  // gathered rows: 32-bit offsets
+}
+
 static void mx_outputs(MxParams &p, void *y, int64_t ldy, int dtype) {
   p.y = y;
   p.ldy = ldy;
@@ -1320,7 +1329,7 @@ int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, in
 }
 
 size_t amla_mxfp4_swiglu_workspace_bytes(int64_t m, int64_t k, int64_t n) {
-  if (!mx_sizes_ok(m, n, k) || n % 128) return 0;
+  if (!mx_ffn_sizes_ok(m, n, k)) return 0;
   return mx_swiglu_layout(m, k, n).total;
 }
 
@@ -1333,7 +1342,7 @@ int amla_mxfp4_swiglu(const void *x, int64_t m, int64_t k, int64_t ldx, const vo
                                              (long long)k, (long long)n);
   if (ldx < k) return fail(AMLA_EINVAL, "mxfp4_swiglu: row stride smaller than the row");
   if (m == 0) return AMLA_OK;
-  bool ok = mx_sizes_ok(m, n, k) && n % 128 == 0 && ldx % 8 == 0 && aligned16(x) && aligned16(y);
+  bool ok = mx_ffn_sizes_ok(m, n, k) && ldx % 8 == 0 && aligned16(x) && aligned16(y);
   for (const void *w : {gate_w, up_w, down_w}) ok = ok && aligned16(w);
   for (const void *s : {gate_s, up_s, down_s}) ok = ok && reinterpret_cast<uintptr_t>(s) % 4 == 0;
   if (!ok)
@@ -1373,8 +1382,7 @@ int amla_mxfp4_swiglu(const void *x, int64_t m, int64_t k, int64_t ldx, const vo
 }
 
 size_t amla_mxfp4_moe_experts_workspace_bytes(int64_t m, int64_t d, int top_k, int64_t n_inter, int64_t n_experts) {
-  if (!mx_sizes_ok(m, n_inter, d) || n_inter % 128 || top_k <= 0 || top_k > 64 || n_experts <= 0 || n_experts > 512 ||
-      m * top_k > 65536)
+  if (!mx_moe_sizes_ok(m, d, top_k, n_inter, n_experts))
     return 0;
   return mx_moe_layout(m, d, top_k, n_inter, n_experts).total;
 }
@@ -1388,15 +1396,13 @@ int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh
   if (m < 0 || d <= 0 || top_k <= 0 || n_inter <= 0 || n_experts <= 0 || ldh < d)
     return fail(AMLA_EINVAL, "mxfp4_moe_experts: bad sizes");
   if (m == 0) return AMLA_OK;
-  if (top_k > 64 || n_experts > 512 || m > 65536 || m * top_k > 65536)
-    return fail(AMLA_EUNSUPPORTED, "mxfp4_moe_experts: needs top_k <= 64, at most 512 experts and 65536 slots per call");
-  bool ok = mx_sizes_ok(m, n_inter, d) && n_inter % 128 == 0 && ldh % 8 == 0 && aligned16(hidden) && aligned16(expert_out);
+  bool ok = mx_moe_sizes_ok(m, d, top_k, n_inter, n_experts) && ldh % 8 == 0 && aligned16(hidden) && aligned16(expert_out);
   for (const void *w : {gate_w, up_w, down_w}) ok = ok && aligned16(w);
   for (const void *s : {gate_s, up_s, down_s}) ok = ok && reinterpret_cast<uintptr_t>(s) % 4 == 0;
   if (!ok)
     return fail(AMLA_EUNSUPPORTED,
-                "mxfp4_moe_experts: needs hidden %% 128 == 0, intermediate %% 128 == 0, 16-byte aligned rows and "
-                "weights and 4-byte aligned scales");
+                "mxfp4_moe_experts: needs top_k <= 64, at most 512 experts, 65536 slots and 4 GB of codes per call, "
+                "hidden and intermediate sizes %% 128 == 0, 16-byte aligned rows and weights and 4-byte aligned scales");
   const MxMoeLayout L = mx_moe_layout(m, d, top_k, n_inter, n_experts);
   if (!workspace || workspace_bytes < L.total || !aligned16(workspace))
     return fail(AMLA_EWORKSPACE, "mxfp4_moe_experts: needs %zu bytes of 16-byte aligned workspace (got %zu)", L.total,

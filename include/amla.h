@@ -317,7 +317,8 @@ int amla_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, i
  * stride ldy: exact products of the two quantised operands summed in fp32.
  * x: bf16 rows, stride ldx, with x_scales NULL (quantised as by
  * amla_mxfp4_quantize), or the codes of such rows with x_scales their exponents
- * (ldx unused).  weight (n, k/2) codes, scales (n, k/32); k % 128 == 0, any n.
+ * (ldx unused).  weight (n, k/2) codes, scales (n, k/32); k % 128 == 0, k <= 2^24
+ * (as every K of a product below), any n.
  * Workspace (16-byte aligned; 0 bytes: NULL) of
  * amla_mxfp4_linear_workspace_bytes(m, n, k, x_scales != NULL) bytes. */
 int amla_mxfp4_linear(const void *x, const void *x_scales, int64_t m, int64_t k, int64_t ldx, const void *weight,
@@ -354,8 +355,8 @@ size_t amla_mxfp4_swiglu_workspace_bytes(int64_t m, int64_t k, int64_t n);
  * DEVICE memory; gate_w, up_w (n_experts, n_inter, d/2), down_w (n_experts, d,
  * n_inter/2) with their exponents.  A slot with an index outside 0 .. n_experts -
  * 1 is skipped: its row is cleared with clear_skipped, else left as it was.
- * m * top_k <= 65536, n_experts <= 512, top_k <= 64, d % 128 == 0, n_inter % 128
- * == 0.  Calls that share a workspace must not overlap. */
+ * m * top_k <= 65536, m * d / 2 < 2^32, n_experts <= 512, top_k <= 64, d % 128 ==
+ * 0, n_inter % 128 == 0.  Calls that share a workspace must not overlap. */
 int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh, int top_k, const int64_t *indices,
                            int64_t n_inter, int64_t n_experts, const void *gate_w, const void *gate_s,
                            const void *up_w, const void *up_s, const void *down_w, const void *down_s,
