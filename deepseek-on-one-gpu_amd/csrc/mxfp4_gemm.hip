@@ -785,13 +785,14 @@ AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, in
   }
 }
 
+// One weight: tiles of 256 outputs (SILU: 128) x `rows` activation rows.  The first
+// `whole` tiles (rounds of 256) take all of K, the others a K part a workgroup.
 struct MxSplit {
-  int n_tiles, m_tiles;  // one weight: tiles of 256 outputs (SILU: 128) x 256 rows
-  int parts;             // K parts of every tile, whole runs of four steps
-  float *partial;        // [tile][part][activation fragment][weight fragment][wave % 4][lane] f32x4
+  int n_tiles, m_tiles, rows, whole;
+  int parts;       // K parts of the other tiles, whole runs of four steps
+  float *partial;  // [tile][part][activation fragment][weight fragment][wave % 4][lane] f32x4
 };
-constexpr int MX_ROWS = 256;  // activation rows of a tile
-constexpr int MX_PART_F32 = 256 * MX_ROWS;
+constexpr int MX_ROWS = 256;  // most activation rows of a tile
 constexpr int MX_FINISH_LDS = MX_PITCH_H * 256 + 4 * 16;  // exponents behind the most rows' codes
 static_assert(MX_FINISH_LDS >= 16 * MX_PITCH_Y && 256 * MX_PITCH_Y <= MX_TILE_LDS, "staged rows");
 
@@ -855,41 +856,55 @@ AMLA_DEV void mx_tile(const MxParams &p, int e, int r0, int rows, int nt, int it
   }
 }
 
-// One weight: tile t, K part q.
+// Column tiles of a panel: an XCD's run of tiles has about as many weight rows as
+// activation rows, and reads the fewest.
+AMLA_DEV int mx_panel(int rows) { return max(1, TL_PANEL * rows / MX_ROWS); }
+
+// One weight: the whole tiles, then the K parts of the others, each as contiguous runs
+// per XCD.
 template <bool SILU, bool PLANES>
 __global__ __launch_bounds__(512, 1) void mx_linear_kernel(MxParams p, MxSplit sp) {
-  const int tiles = sp.n_tiles * sp.m_tiles;
-  const int l = xcd_run(blockIdx.x, tiles * sp.parts);
-  if (l < 0) return;
-  const int q = l / tiles, t = l - q * tiles;
+  const int split = sp.n_tiles * sp.m_tiles - sp.whole, steps = p.K >> 7;
+  int t, it0 = 0, it1 = steps;
+  f32x4 *partial = nullptr;
+  if ((int)blockIdx.x < sp.whole) {
+    t = xcd_run(blockIdx.x, sp.whole);
+  } else {
+    const int l = xcd_run(blockIdx.x - sp.whole, split * sp.parts);
+    if (l < 0) return;
+    const int q = l / split, quads = (steps + 3) >> 2;
+    t = l - q * split;
+    if (sp.parts > 1) {
+      it0 = 4 * (quads * q / sp.parts);
+      it1 = min(steps, 4 * (quads * (q + 1) / sp.parts));
+      partial = reinterpret_cast<f32x4 *>(sp.partial) + (size_t)(t * sp.parts + q) * (64 * sp.rows);
+    }
+    t += sp.whole;
+  }
   int nt, mt;
-  tile_coords(t, sp.n_tiles, sp.m_tiles, nt, mt);
-  const int steps = p.K >> 7, quads = (steps + 3) >> 2;
-  const int it0 = 4 * (quads * q / sp.parts), it1 = min(steps, 4 * (quads * (q + 1) / sp.parts));
-  f32x4 *partial = sp.parts > 1 ? reinterpret_cast<f32x4 *>(sp.partial) + (size_t)(t * sp.parts + q) * (MX_PART_F32 / 4)
-                                : nullptr;
-  mt = uniform(mt);
-  mx_tile<SILU, PLANES>(p, 0, mt * MX_ROWS, min(MX_ROWS, p.M - mt * MX_ROWS), uniform(nt), uniform(it0), uniform(it1), partial);
+  tile_coords(t, sp.n_tiles, sp.m_tiles, nt, mt, mx_panel(sp.rows));
+  const int r0 = uniform(mt) * sp.rows;
+  mx_tile<SILU, PLANES>(p, 0, r0, min(sp.rows, p.M - r0), uniform(nt), uniform(it0), uniform(it1), partial);
 }
 
 // Sums the K parts of activation fragment j of a tile in part order.
 template <bool SILU>
 __global__ __launch_bounds__(256) void mx_finish_kernel(MxParams p, MxSplit sp) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = blockIdx.x >> 4, j = blockIdx.x & 15;
+  const int t = blockIdx.x / (sp.rows >> 4), j = blockIdx.x - t * (sp.rows >> 4);
   int nt, mt;
-  tile_coords(t, sp.n_tiles, sp.m_tiles, nt, mt);
-  if (mt * MX_ROWS + 16 * j >= p.M) return;
-  const f32x4 *src = reinterpret_cast<const f32x4 *>(sp.partial) + (size_t)t * sp.parts * (MX_PART_F32 / 4) +
-                     j * 1024 + wave * 64 + lane;
+  tile_coords(t + sp.whole, sp.n_tiles, sp.m_tiles, nt, mt, mx_panel(sp.rows));
+  const int m0 = mt * sp.rows + 16 * j;
+  if (m0 >= p.M) return;
+  const size_t part = 64 * sp.rows;
+  const f32x4 *src = reinterpret_cast<const f32x4 *>(sp.partial) + t * sp.parts * part + j * 1024 + wave * 64 + lane;
   f32x4 v[4];
 #pragma unroll
   for (int f = 0; f < 4; ++f) v[f] = src[f * 256];
 #pragma unroll 4
   for (int q = 1; q < sp.parts; ++q)
 #pragma unroll
-    for (int f = 0; f < 4; ++f) v[f] += src[(size_t)q * (MX_PART_F32 / 4) + f * 256];
-  const int m0 = mt * MX_ROWS + 16 * j;
+    for (int f = 0; f < 4; ++f) v[f] += src[q * part + f * 256];
   mx_tile_store<1, SILU>(p, [&](int) { return MxFrag{{v[0], v[1], v[2], v[3]}}; }, 0, wave, min(16, p.M - m0), m0,
                          nt * (SILU ? 128 : 256));
 }
@@ -1058,30 +1073,57 @@ static int launch_mx_stream_silu(const MxParams &p, int rows, int entries, hipSt
   return launch_stream<1, true>(p, rows, entries, st);
 }
 
+// Rows and K parts of the tiles by what they cost: a stage of 256 K values and the rest
+// of a tile (us, 32 to 256 rows), rounds of 256 workgroups, and the sums of the K parts
+// through memory.  Few tiles stay on small rows (777 x 2112 x 7168: 32 rows 21.6 us, 64
+// in two parts 22.8, 128 in four 25.9, 256 in five 29.3; 300 x 7168 x 16384: 128 in
+// three 42.2, 256 in four 43.8), long K on parts (200 x 7168 x 18432: 128 rows in four
+// parts 38, in one 95), and a last round that is far from full is split alone (1000 x
+// 36864 x 7168: 64 of 576 tiles in two to four parts 170 - 174 us, in one 183).
 static MxSplit plan_mx_split(int64_t M, int N, int K, bool silu) {
-  MxSplit sp = {};
-  const int cols = silu ? 128 : 256;
-  sp.n_tiles = (N + cols - 1) / cols;
-  sp.m_tiles = (int)((M + MX_ROWS - 1) / MX_ROWS);
-  const int64_t tiles = (int64_t)sp.n_tiles * sp.m_tiles;
-  const int quads = (K / 128 + 3) / 4;
-  sp.parts = (int)std::max<int64_t>(1, std::min<int64_t>(quads, 256 / tiles));
-  return sp;
+  const double stage_us[4] = {0.65, 0.8, 1.3, 1.9}, tile_us[4] = {3.5, 4.5, 5, 10}, finish_us = 5, part_us = 0.23;
+  const int cols = silu ? 128 : 256, quads = (K / 128 + 3) / 4;
+  MxSplit best = {};
+  double least = 1e30;
+  for (int i = 0; i < 4; ++i) {
+    MxSplit sp = {};
+    sp.rows = 32 << i;
+    sp.n_tiles = (N + cols - 1) / cols;
+    sp.m_tiles = (int)((M + sp.rows - 1) / sp.rows);
+    const int64_t tiles = (int64_t)sp.n_tiles * sp.m_tiles;
+    if (tiles > 1 << 30) continue;
+    sp.whole = (int)(tiles / 256 * 256);
+    const int rest = (int)tiles - sp.whole;
+    const double whole = sp.whole / 256 * (quads * 2 * stage_us[i] + tile_us[i]);
+    for (sp.parts = 1; sp.parts == 1 || (sp.parts <= quads && sp.parts * rest <= 256); ++sp.parts) {
+      double us = whole;
+      if (rest) us += (quads + sp.parts - 1) / sp.parts * 2 * stage_us[i] + tile_us[i];
+      if (sp.parts > 1) us += finish_us + part_us * sp.parts * rest * sp.rows / 1024;
+      if (us < least) {
+        least = us;
+        best = sp;
+      }
+      if (!rest) break;
+    }
+    if (sp.rows >= M) break;
+  }
+  if (best.parts == 1) best.whole = 0;  // one run per XCD for all
+  return best;
 }
 static size_t mx_split_bytes(const MxSplit &sp) {
-  return sp.parts > 1 ? (size_t)sp.n_tiles * sp.m_tiles * sp.parts * MX_PART_F32 * 4 : 0;
+  return sp.parts > 1 ? ((size_t)sp.n_tiles * sp.m_tiles - sp.whole) * sp.parts * 1024 * sp.rows : 0;
 }
 
 template <bool SILU>
 static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st) {
-  const int64_t blocks = ((int64_t)sp.n_tiles * sp.m_tiles * sp.parts + 7) / 8 * 8;
-  if (blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
+  const int64_t split = (int64_t)sp.n_tiles * sp.m_tiles - sp.whole, blocks = sp.whole + (split * sp.parts + 7) / 8 * 8;
+  if (!sp.rows || blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
   const auto kernel = p.K % 512 ? mx_linear_kernel<SILU, true> : mx_linear_kernel<SILU, false>;
   int rc = mx_lds(kernel, MX_TILE_LDS);
   if (rc) return rc;
   kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, sp);
   if ((rc = check_launch("mxfp4 product")) || sp.parts == 1) return rc;
-  mx_finish_kernel<SILU><<<dim3((unsigned)(sp.n_tiles * sp.m_tiles * 16)), 256, MX_FINISH_LDS, st>>>(p, sp);
+  mx_finish_kernel<SILU><<<dim3((unsigned)(split * (sp.rows / 16))), 256, MX_FINISH_LDS, st>>>(p, sp);
   return check_launch("mxfp4 K-part finish");
 }
 

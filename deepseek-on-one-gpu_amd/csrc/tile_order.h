@@ -8,16 +8,16 @@ namespace amla {
 // Column tiles a panel holds (the row tiles of a panel come one after another).
 constexpr int TL_PANEL = 8;
 
-AMLA_DEV void tile_coords(int t, int n_tiles, int m_tiles, int &nt, int &mt) {
-  if (m_tiles <= TL_PANEL) {
+AMLA_DEV void tile_coords(int t, int n_tiles, int m_tiles, int &nt, int &mt, int panel = TL_PANEL) {
+  if (m_tiles <= panel) {
     nt = t / m_tiles;
     mt = t - nt * m_tiles;
     return;
   }
-  const int per = TL_PANEL * m_tiles, p = t / per, r = t - p * per;
-  const int width = min(TL_PANEL, n_tiles - p * TL_PANEL);
+  const int per = panel * m_tiles, p = t / per, r = t - p * per;
+  const int width = min(panel, n_tiles - p * panel);
   mt = r / width;
-  nt = p * TL_PANEL + r - mt * width;
+  nt = p * panel + r - mt * width;
 }
 // logical index of workgroup i of n (or -1): a contiguous run per XCD
 AMLA_DEV int xcd_run(int i, int n) {
