@@ -696,6 +696,10 @@ struct MxBigMain {
 }
 };
 
+struct MxFrag {
+  f32x4 f[4];
+};
+
 // Stores a tile of `rows` positions from r0, outputs from n0.  The threads hold it as
 // v(j)[f], activation fragment j of j0 .. j0 + XF - 1, weight fragment f: row 16 j +
 // lane % 16, outputs 128 (f / 2) + 32 wn + 16 (f % 2) + 4 (lane / 16) .. +3.  Rows go
@@ -703,7 +707,7 @@ struct MxBigMain {
 // where the sums are held, 32 bytes in each of 16 rows, reach 1.7 TB/s (down
 // projection of 16000 routed rows 505 us, 370 without its stores).
 constexpr int MX_PITCH_Y = 512 + 16, MX_PITCH_H = 64 + 16;
-template <int XF, bool SILU, typename V>
+template <int XF, bool SILU, int SEGS = 2, typename V>
 AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, int r0, int n0) {
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -750,21 +754,21 @@ AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, in
       if (m >= rows) continue;
       const int64_t yr = p.yrow ? p.yrow[r0 + m] : r0 + m;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
+      for (int f = 0; f < 2 * SEGS; ++f) {
         const int n = n0 + (f >> 1) * 128 + 32 * wn + 16 * (f & 1) + 4 * g;
         if (n < p.N) mx_store4(p, yr, n, t.f[f]);
       }
     }
   } else {
-    // bf16: both segments of a row; fp32: one after the other
-    for (int s = 0; s < (p.f32 ? 2 : 1); ++s) {
+    // bf16: all segments of a row; fp32: one after the other
+    for (int s = 0; s < (p.f32 ? SEGS : 1); ++s) {
       if (s) meet();
 #pragma unroll
       for (int j = 0; j < XF; ++j) {
         const auto t = v(j);
         uint8_t *row = lds + MX_PITCH_Y * (16 * (j0 + j) + r16);
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
+        for (int f = 0; f < 2 * SEGS; ++f) {
           const int c = 32 * wn + 16 * (f & 1) + 4 * g;
           if (!p.f32)
             *reinterpret_cast<u32x2 *>(row + 2 * (128 * (f >> 1) + c)) =
@@ -774,21 +778,153 @@ AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, in
         }
       }
       meet();
-      const int per = p.f32 ? 4 : 8, n = n0 + 128 * s + per * (tid & 31);
+      const int log = p.f32 || SEGS == 2 ? 5 : 4, c = tid & ((1 << log) - 1);  // a row's 16-byte pieces
+      const int n = n0 + 128 * s + (p.f32 ? 4 : 8) * c;
       if (n < p.N)
-        for (int r = tid >> 5; r < rows; r += threads >> 5) {
+        for (int r = tid >> log; r < rows; r += threads >> log) {
           const int64_t yr = p.yrow ? p.yrow[r0 + r] : r0 + r;
           *reinterpret_cast<u32x4 *>(static_cast<uint8_t *>(p.y) + (yr * p.ldy + n) * (p.f32 ? 4 : 2)) =
-              ldg16(lds + MX_PITCH_Y * r + 16 * (tid & 31));
+              ldg16(lds + MX_PITCH_Y * r + 16 * c);
         }
     }
   }
+}
+
+// Few tiles of one weight: 128 weight rows x up to 64 activation rows for sixteen waves,
+// wave w on weight rows 32 (w % 4) .. +31 and K step w / 4 of a stage of 512 K values;
+// the four sums of an output meet in LDS.  Nothing but waits bounds such a call (a
+// barrier, the reads and eight multiplications one after the other in every wave), so
+// its stages are long and four waves of a SIMD stand in for each other: 777 x 2112 x
+// 7168 in 17.3 us, 21.8 with tiles of 256 x 32; eight waves with stages of 256 and five
+// of them on their way 19.1, which 24 workgroups alone take 0.44 us a stage for.
+//
+// A stage: two halves of 128-byte lines as above, rows of exponents behind them (wave w
+// copies those of weight rows 8 w .. +7 and x rows 4 w .. +3).  Three slots.
+constexpr int MXS_ROWS = 64;
+constexpr int MXS_X = 2 * 128 * 128, MXS_SCALES = MXS_X + 2 * MXS_ROWS * 128, MXS_STAGE = MXS_SCALES + 16 * 12 * 16;
+constexpr int MXS_LDS = 3 * MXS_STAGE;
+static_assert(MXS_LDS <= 160 * 1024 && 16 * 8 * 1024 <= MXS_LDS, "LDS of a CU, the sums");
+
+template <bool PLANES>
+AMLA_DEV void mx_small_tile(const MxParams &p, int r0, int rows, int n0) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  constexpr int C = 3 + (PLANES ? 4 : 1);  // copies of a wave and stage
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wk = wave >> 2;
+  const int64_t kb = p.K >> 1, ksb = p.K >> 5;
+  const int steps = p.K >> 7, quads = (steps + 3) >> 2, wrows = min(128, p.N - n0);
+  const auto wrsrc = mx_rsrc(p.w[0] + n0 * kb), xrsrc = mx_rsrc(static_cast<const uint8_t *>(p.x) + r0 * kb);
+  // wave w copies half w / 8 of weight rows 16 (w % 8) .. +15 and x rows 8 (w % 8) .. +7
+  // (rows past the tile repeat its last)
+  const int half = wave >> 3, w8 = wave & 7, ch = lane & 7;
+  const int wr = 16 * w8 + (lane >> 3), xr = 8 * w8 + (lane >> 3);  // (the second weight copy: row + 8, the same chunk ^ 4)
+  const int wch = ch ^ ((wr >> 1) & 7), xch = ch ^ ((xr >> 1) & 7);
+  const uint32_t woff[2] = {(uint32_t)min(wr, wrows - 1) * (uint32_t)kb + 16 * wch,
+                            (uint32_t)min(wr + 8, wrows - 1) * (uint32_t)kb + 16 * (wch ^ 4)};
+  const uint32_t xoff = (uint32_t)min(xr, rows - 1) * (uint32_t)kb + 16 * xch;
+  typedef const __attribute__((address_space(1))) uint8_t *gptr;
+  const gptr sptr = lane < 8 ? (gptr)(p.ws[0] + (n0 + (int64_t)min(8 * wave + lane, wrows - 1)) * ksb)
+                             : (gptr)(p.xs + (r0 + (int64_t)min(4 * wave + (lane & 3), rows - 1)) * ksb);
+  auto issue = [&](int q, int slot) {
+    uint8_t *st = lds + slot * MXS_STAGE;
+    const uint32_t off = q * 256 + 128 * half;
+    auto copy = [&](__amdgpu_buffer_rsrc_t r, uint8_t *dst, uint32_t lane_off, int c) {
+      if constexpr (!PLANES) mx_copy16(r, dst, lane_off, off);
+      else  // steps past the end: the lanes repeat the last one
+        mx_copy16(r, dst, lane_off + off - 64 * max(0, 4 * q + 2 * half + (c >> 2) - (steps - 1)), 0);
+    };
+    copy(wrsrc, st + half * 16384 + 16 * w8 * 128, woff[0], wch);
+    copy(wrsrc, st + half * 16384 + (16 * w8 + 8) * 128, woff[1], wch ^ 4);
+    copy(xrsrc, st + MXS_X + half * 8192 + 8 * w8 * 128, xoff, xch);
+    if (lane < 12) {
+      if constexpr (!PLANES) {
+        __builtin_amdgcn_global_load_lds(sptr + q * 16, LDS_PTR(st + MXS_SCALES + 192 * wave), 16, 0, 0);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          __builtin_amdgcn_global_load_lds(sptr + min(4 * q + u, steps - 1) * 4,
+                                           LDS_PTR(st + MXS_SCALES + 768 * u + 48 * wave), 4, 0, 0);
+      }
+    }
+  };
+  f32x4 acc[2][4];
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  issue(0, 0);
+  if (quads > 1) issue(1, 1);
+
+  const uint32_t frag = r16 * 128 + 16 * ((4 * (wk & 1) + g) ^ ((r16 >> 1) & 7));
+  int slot = 0;
+  for (int q = 0; q < quads; ++q) {
+    if (q + 1 < quads) wait_vmcnt<C>();  // all but the next stage's copies have landed
+    else wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (q + 2 < quads) issue(q + 2, slot == 0 ? 2 : slot - 1);
+    const uint8_t *st = lds + slot * MXS_STAGE;
+    slot = slot == 2 ? 0 : slot + 1;
+    if (PLANES && 4 * q + wk >= steps) continue;
+    uint32_t wsc[2], xsc[4];
+    const uint8_t *sc = st + MXS_SCALES + wk * (PLANES ? 768 : 4) + g;
+    auto scale = [&](int r) { return (uint32_t)sc[r * (PLANES ? 4 : 16)]; };
+#pragma unroll
+    for (int f = 0; f < 2; ++f) wsc[f] = scale(12 * (4 * wn + 2 * f + (r16 >> 3)) + (r16 & 7));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xsc[j] = scale(12 * (4 * j + (r16 >> 2)) + 8 + (r16 & 3));
+    const uint8_t *wp = st + (wk >> 1) * 16384 + 32 * wn * 128 + frag, *xp = st + MXS_X + (wk >> 1) * 8192 + frag;
+    u32x4 wf[2], xf[4];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) wf[f] = *reinterpret_cast<const u32x4 *>(wp + f * 2048);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xf[j] = *reinterpret_cast<const u32x4 *>(xp + j * 2048);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) acc[f][j] = mfma_mx<0>(wf[f], wsc[f], xf[j], xsc[j], acc[f][j]);
+  }
+
+  auto meet = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  meet();  // every wave is past its last fragment read
+  f32x4 *ex = reinterpret_cast<f32x4 *>(lds) + lane;
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ex[((wave * 2 + f) * 4 + j) * 64] = acc[f][j];
+  meet();
+  // wave w sums activation fragment w / 4, in the order of the K steps
+  MxFrag sum = {};
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    sum.f[f] = ex[((wn * 2 + f) * 4 + wk) * 64];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) sum.f[f] += ex[(((wn + 4 * k) * 2 + f) * 4 + wk) * 64];
+  }
+  meet();  // (LDS is free)
+  mx_tile_store<1, false, 1>(p, [&](int) { return sum; }, wk, wn, rows, r0, n0);
+}
+
+template <bool PLANES>
+__global__ __launch_bounds__(1024, 1) void mx_small_kernel(MxParams p, int n_tiles, int m_tiles) {
+  const int t = xcd_run(blockIdx.x, n_tiles * m_tiles);
+  if (t < 0) return;
+  int nt, mt;
+  tile_coords(t, n_tiles, m_tiles, nt, mt, TL_PANEL / 2);
+  const int r0 = uniform(mt) * MXS_ROWS;
+  mx_small_tile<PLANES>(p, r0, min(MXS_ROWS, p.M - r0), uniform(nt) * 128);
 }
 
 // One weight: tiles of 256 outputs (SILU: 128) x `rows` activation rows.  The first
 // `whole` tiles (rounds of 256) take all of K, the others a K part a workgroup.
 struct MxSplit {
   int n_tiles, m_tiles, rows, whole;
+  bool small;      // tiles of 128 outputs x 64 rows (parts 1)
   int parts;       // K parts of the other tiles, whole runs of four steps
   float *partial;  // [tile][part][activation fragment][weight fragment][wave % 4][lane] f32x4
 };
@@ -816,9 +952,6 @@ AMLA_DEV MxTile mx_tile_of(const MxParams &p, int e, int r0, int rows, int n0, i
 }
 
 // The fragments j0 .. j0 + XF - 1 of a tile, held as acc[.][0 .. XF - 1].
-struct MxFrag {
-  f32x4 f[4];
-};
 template <int XF, int HELD, bool SILU>
 AMLA_DEV void mx_tile_out(const MxParams &p, const MxSums<HELD> &sums, int j0, int r0, int rows, int n0, f32x4 *partial) {
   const int lane = threadIdx.x & 63, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
@@ -1075,15 +1208,16 @@ static int launch_mx_stream_silu(const MxParams &p, int rows, int entries, hipSt
   return launch_stream<1, true>(p, rows, entries, st);
 }
 
-// Rows and K parts of the tiles by what they cost: a stage of 256 K values and the rest
-// of a tile (us, 32 to 256 rows), rounds of 256 workgroups, and the sums of the K parts
-// through memory.  Few tiles stay on small rows (777 x 2112 x 7168: 32 rows 21.6 us, 64
-// in two parts 22.8, 128 in four 25.9, 256 in five 29.3; 300 x 7168 x 16384: 128 in
-// three 42.2, 256 in four 43.8), long K on parts (200 x 7168 x 18432: 128 rows in four
-// parts 38, in one 95), and a last round that is far from full is split alone (1000 x
+// The tiles of one weight by what they cost: a stage of 256 K values and the rest of a
+// tile (us, 32 to 256 rows), rounds of 256 workgroups, the sums of K parts through
+// memory.  Few tiles stay small (777 x 2112 x 7168: 128 x 64 17.3 us, 256 x 32 21.6, 256 x
+// 64 in two parts 22.8, x 128 in four 25.9, x 256 in five 29.3; 300 x 7168 x 16384: x 128
+// in three 42.2, x 256 in four 43.8), long K goes in parts (200 x 7168 x 18432: x 128 in
+// four 39, in one 95), and a last round that is far from full is split alone (1000 x
 // 36864 x 7168: 64 of 576 tiles in two to four parts 170 - 174 us, in one 183).
 static MxSplit plan_mx_split(int64_t M, int N, int K, bool silu) {
   const double stage_us[4] = {0.65, 0.8, 1.3, 1.9}, tile_us[4] = {3.5, 4.5, 5, 10}, finish_us = 5, part_us = 0.23;
+  const double small_quad_us = 0.9, small_tile_us = 4.6;
   const int cols = silu ? 128 : 256, quads = (K / 128 + 3) / 4;
   MxSplit best = {};
   double least = 1e30;
@@ -1109,6 +1243,16 @@ static MxSplit plan_mx_split(int64_t M, int N, int K, bool silu) {
     }
     if (sp.rows >= M) break;
   }
+  if (!silu && M > 32) {
+    MxSplit sp = {};
+    sp.small = true;
+    sp.parts = 1;
+    sp.rows = MXS_ROWS;
+    sp.n_tiles = (N + 127) / 128;
+    sp.m_tiles = (int)((M + MXS_ROWS - 1) / MXS_ROWS);
+    const double rounds = (double)(((int64_t)sp.n_tiles * sp.m_tiles + 255) / 256);
+    if (rounds * (quads * small_quad_us + small_tile_us) < least) best = sp;
+  }
   if (best.parts == 1) best.whole = 0;  // one run per XCD for all
   return best;
 }
@@ -1121,8 +1265,15 @@ static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st
   const int64_t split = (int64_t)sp.n_tiles * sp.m_tiles - sp.whole, blocks = sp.whole + (split * sp.parts + 7) / 8 * 8;
   if (!sp.rows || blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
   const auto kernel = p.K % 512 ? mx_linear_kernel<SILU, true> : mx_linear_kernel<SILU, false>;
-  int rc = mx_lds(kernel, MX_TILE_LDS);
-  if (rc) return rc;
+  int rc;
+  if constexpr (!SILU)
+    if (sp.small) {
+      const auto small = p.K % 512 ? mx_small_kernel<true> : mx_small_kernel<false>;
+      if ((rc = mx_lds(small, MXS_LDS))) return rc;
+      small<<<dim3((unsigned)blocks), 1024, MXS_LDS, st>>>(p, sp.n_tiles, sp.m_tiles);
+      return check_launch("mxfp4 product of few tiles");
+    }
+  if ((rc = mx_lds(kernel, MX_TILE_LDS))) return rc;
   kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, sp);
   if ((rc = check_launch("mxfp4 product")) || sp.parts == 1) return rc;
   mx_finish_kernel<SILU><<<dim3((unsigned)(split * (sp.rows / 16))), 256, MX_FINISH_LDS, st>>>(p, sp);

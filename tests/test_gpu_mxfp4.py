@@ -157,6 +157,21 @@ def test_linear_shapes_strides_and_types():
     _check(ops.mxfp4_linear(odd, *w), y[:4], slack[:4], "base off the 16-byte grid")
 
 
+@pytest.mark.parametrize("m,n,k", [(4097, 4096, 8192), (200, 1000, 18432), (70, 576, 7168), (1000, 2112, 3712)])
+def test_linear_in_k_parts_and_rounds(m, n, k):
+    """Sizes whose last round of tiles, or all of them, run in K parts: some rows of each tile."""
+    g = _gen(m + k)
+    x, w = _x(g, m, k).to(DEV), _weight(g, n, k)
+    rows = torch.tensor(sorted({r for r in (0, 15, 16, 31, 32, 63, 64, 65, 127, 128, 255, 256, 900, 4000, m - 2, m - 1) if r < m}))
+    xq = ops.mxfp4_dequantize(*ops.mxfp4_quantize(x[rows.to(DEV)]), F32).double()
+    wv = ops.mxfp4_dequantize(*w, F32).double()
+    y, mag = xq @ wv.T, xq.abs() @ wv.abs().T
+    for out in (BF16, F32):
+        got = ops.mxfp4_linear(x, *w, out_dtype=out)
+        _check(got[rows.to(DEV)], y.cpu(), M.linear_slack(mag.cpu(), k, HALF_STEP[out], y.cpu()), f"{m}x{n}x{k} {out}")
+        assert torch.equal(got, ops.mxfp4_linear(x, *w, out_dtype=out))
+
+
 @pytest.mark.parametrize("m", [1, 70, 130])
 @pytest.mark.parametrize("k", [1024, 1152])
 def test_linear_with_exponents_off_the_16_byte_grid(m, k):
