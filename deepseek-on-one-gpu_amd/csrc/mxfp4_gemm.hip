@@ -59,8 +59,15 @@ AMLA_DEV float mx_silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; 
 // workgroup takes a contiguous run of items.  Its waves share the K of every weight
 // row by runs of quads (512 K values) and meet in LDS, in wave order.  A wave walks
 // the quads of all its items as one sequence, with the next quad's loads in flight
-// while it multiplies one, also across items; a load is 16 rows x 64 bytes, a quad
-// 16 bytes of exponents a row more (the lanes of a row share them).
+// while it multiplies one, also across items; a quad is 16 rows x 256 bytes, and 16
+// bytes of exponents a row more (the lanes of a row share them).
+//
+// The matrix units want 16 rows x 64 bytes in a register.  Up to 16 activation rows a
+// load takes 4 rows x 256 bytes all the same, and the wave turns the quad over in 4 KB
+// of LDS of its own (no barrier: its LDS operations stay in order): memory delivers
+// whole lines faster (8 x 65536 x 7168 58 -> 54 us, 8 x 7168 x 18432 22.8 -> 21.5, 4 x 2112
+// x 7168 7.0 -> 6.3).  Four waves a SIMD have to fit: with 129 registers instead of 128
+// the down projections of 57 experts took 87 us, 73 so.
 //
 // Activations: rows of one entry (at most `mr`, a power of two, or 16 XT), bf16 ones
 // quantised on the way in, which saves the pass and the launch before it.  Codes at
@@ -71,13 +78,17 @@ struct MxStream {
   int mr;          // activation rows kept of a fragment
   int xcodes;      // bytes of the codes, and
   int xbytes;      // with the exponents (the partial sums come behind)
+  int turn;        // of the waves' 4 KB, behind the partial sums
 };
+// turned over in LDS
+constexpr bool mx_turns(int fragments, bool planes) { return fragments == 1 && !planes; }
 
 template <int XT, bool SILU, bool PLANES>
-__global__ __launch_bounds__(512) void mx_stream_kernel(MxParams p, MxStream sp) {
+__global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParams p, MxStream sp) {
   extern __shared__ __align__(16) uint8_t lds[];
   constexpr int WT = SILU ? 4 : 1;  // 16-row fragments of an item
   constexpr int COLS = SILU ? 32 : 16;
+  constexpr bool TURN = mx_turns(XT, PLANES);
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
   const int steps = p.K >> 7, quads = (steps + 3) >> 2;
@@ -109,18 +120,28 @@ __global__ __launch_bounds__(512) void mx_stream_kernel(MxParams p, MxStream sp)
   int64_t ni = i0;
   int nsub = 0, nq = q0;
   const uint8_t *nw_p, *ns_p;
+  uint32_t noff[4];  // TURN: of the lane's four rows
   auto row_of = [&](int64_t item, int sub) {  // the lane's weight row
     const int en = (int)(item / sp.ntiles), t = (int)(item - (int64_t)en * sp.ntiles);
     const int e = p.ent ? ent[4 * uniform(en)] : 0;
     const int seg = SILU && sub >= 2;
     const int n = min(t * COLS + 16 * (SILU ? sub & 1 : 0) + r16, p.N - 1);  // rows past N repeat the last
-    nw_p = (seg ? p.w[1] : p.w[0]) + e * p.wstride + n * kb + 16 * g;
+    if constexpr (!TURN) {
+      nw_p = (seg ? p.w[1] : p.w[0]) + e * p.wstride + n * kb + 16 * g;
+    } else {
+      const int n0 = t * COLS + 16 * (SILU ? sub & 1 : 0);
+      nw_p = (seg ? p.w[1] : p.w[0]) + e * p.wstride + n0 * kb + 16 * r16;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) noff[u] = (uint32_t)min(4 * u + g, p.N - 1 - n0) * (uint32_t)kb;
+    }
     ns_p = (seg ? p.ws[1] : p.ws[0]) + e * p.sstride + n * ksb;
   };
   row_of(ni, 0);
   auto load = [&](Loads &l) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) l.w[u] = ldg16(nw_p + (int64_t)(PLANES ? min(4 * nq + u, steps - 1) : 4 * nq + u) * 64);
+    for (int u = 0; u < 4; ++u)
+      l.w[u] = ldg16(TURN ? nw_p + noff[u] + nq * 256
+                          : nw_p + (int64_t)(PLANES ? min(4 * nq + u, steps - 1) : 4 * nq + u) * 64);
     if constexpr (!PLANES) {
       l.s = *reinterpret_cast<const u32x4_a4 *>(ns_p + nq * 16);
     } else {
@@ -273,19 +294,36 @@ __global__ __launch_bounds__(512) void mx_stream_kernel(MxParams p, MxStream sp)
       for (int j = 0; j < XT; ++j)
         xc[u][j] = ldg16(xl + 64 * ((PLANES ? min(4 * q + u, steps - 1) : 4 * q + u) * XT + j) * mr);
     const int nst = PLANES ? steps - 4 * q : 4;
+    auto multiply = [&](const u32x4 *w) {
 #pragma unroll
-    for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<0>(l.w[0], ws, xc[0][j], xs[j], acc[j]);
-    if (!PLANES || nst > 1)
+      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<0>(w[0], ws, xc[0][j], xs[j], acc[j]);
+      if (!PLANES || nst > 1)
 #pragma unroll
-      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<1>(l.w[1], ws, xc[1][j], xs[j], acc[j]);
-    if (!PLANES || nst > 2)
+        for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<1>(w[1], ws, xc[1][j], xs[j], acc[j]);
+      if (!PLANES || nst > 2)
 #pragma unroll
-      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<2>(l.w[2], ws, xc[2][j], xs[j], acc[j]);
-    if (!PLANES || nst > 3)
+        for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<2>(w[2], ws, xc[2][j], xs[j], acc[j]);
+      if (!PLANES || nst > 3)
 #pragma unroll
-      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<3>(l.w[3], ws, xc[3][j], xs[j], acc[j]);
-    __builtin_amdgcn_sched_barrier(0);  // (the registers of l are free: no copies of them)
-    load(l);
+        for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<3>(w[3], ws, xc[3][j], xs[j], acc[j]);
+    };
+    if constexpr (TURN) {
+      // 16-byte chunk c of row r at c ^ r: sixteen bank groups both ways
+      uint8_t *turn = lds + sp.turn + 4096 * wave;
+      u32x4 w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4 *>(turn + 256 * (4 * u + g) + 16 * (r16 ^ (4 * u + g))) = l.w[u];
+      __builtin_amdgcn_sched_barrier(0);  // (the registers of l are free: no copies of them)
+      load(l);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[u] = ldg16(turn + 256 * r16 + 16 * ((4 * u + g) ^ r16));
+      multiply(w);
+    } else {
+      multiply(l.w);
+      __builtin_amdgcn_sched_barrier(0);
+      load(l);
+    }
     __builtin_amdgcn_sched_barrier(0);
     if (++q < q1) return;
     q = q0;
@@ -1165,8 +1203,11 @@ static int mx_waves(int64_t K) {
   return best;
 }
 
-static int64_t mx_stream_lds(int rows, int64_t K, bool silu) {  // with two items' partial sums
+static int64_t mx_stream_sums(int rows, int64_t K, bool silu) {  // with two items' partial sums
   return mx_stream_bytes(rows, K) + 2048 * mx_waves(K) * mx_fragments(rows) * (silu ? 4 : 1);
+}
+static int64_t mx_stream_lds(int rows, int64_t K, bool silu) {
+  return mx_stream_sums(rows, K, silu) + (mx_turns(mx_fragments(rows), K % 512) ? 4096 * mx_waves(K) : 0);
 }
 static bool mx_stream_fits(int rows, int64_t K, bool silu) {
   return rows <= (silu ? 16 : 64) && mx_stream_lds(rows, K, silu) <= 160 * 1024;
@@ -1179,6 +1220,7 @@ static int launch_stream(const MxParams &p, int rows, int entries, hipStream_t s
   sp.mr = mx_keep(rows);
   sp.xcodes = sp.mr * XT * (p.K >> 1);
   sp.xbytes = (int)mx_stream_bytes(rows, p.K);
+  sp.turn = (int)mx_stream_sums(rows, p.K, SILU);
   const int nw = mx_waves(p.K);
   const int lds = (int)mx_stream_lds(rows, p.K, SILU);
   // three items or more a workgroup (each takes in the activations for itself), up to
