@@ -1,8 +1,9 @@
 // MXFP4 products for gfx950: y = deq(x) deq(w)^T with both operands in 4 bits on
-// the scaled MFMA (16x16x128, exact products, fp32 sums).  A skinny kernel for up
-// to 64 activation rows, tiles of 256 weight rows x up to 128 activation rows for
-// more, each for one weight or for a device schedule of experts, with the output
-// rows or silu(gate) * up quantised again as epilogue.
+// the scaled MFMA (16x16x128, exact products, fp32 sums).  A stream kernel for up
+// to 16 activation rows, bound by the weights' bytes; tiles of 256 weight rows x up
+// to 256 activation rows for more, and of 128 x 64 where there are few; each for one
+// weight or (but the last) for a device schedule of experts, with the output rows or
+// silu(gate) * up quantised again as epilogue.
 #include <algorithm>
 #include <type_traits>
 
@@ -52,7 +53,7 @@ AMLA_DEV float mx_silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; 
 
 // ---------------------------------------------------------------- stream product
 
-// Few activation rows: the weights stream once, from memory straight into the
+// Up to 16 activation rows: the weights stream once, from memory straight into the
 // operands' registers, past activations that stay in LDS.
 //
 // An item is 16 weight rows (SILU: 32 of gate and the same 32 of up) of an entry; a
@@ -62,33 +63,30 @@ AMLA_DEV float mx_silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; 
 // while it multiplies one, also across items; a quad is 16 rows x 256 bytes, and 16
 // bytes of exponents a row more (the lanes of a row share them).
 //
-// The matrix units want 16 rows x 64 bytes in a register.  Up to 16 activation rows a
-// load takes 4 rows x 256 bytes all the same, and the wave turns the quad over in 4 KB
-// of LDS of its own (no barrier: its LDS operations stay in order): memory delivers
-// whole lines faster (8 x 65536 x 7168 58 -> 54 us, 8 x 7168 x 18432 22.8 -> 21.5, 4 x 2112
+// The matrix units want 16 rows x 64 bytes in a register.  A load takes 4 rows x 256
+// bytes all the same, and the wave turns the quad over in 4 KB of LDS of its own (no
+// barrier: its LDS operations stay in order): memory delivers whole lines faster (8 x 65536 x 7168 58 -> 54 us, 8 x 7168 x 18432 22.8 -> 21.5, 4 x 2112
 // x 7168 7.0 -> 6.3).  Four waves a SIMD have to fit: with 129 registers instead of 128
 // the down projections of 57 experts took 87 us, 73 so.
 //
-// Activations: rows of one entry (at most `mr`, a power of two, or 16 XT), bf16 ones
-// quantised on the way in, which saves the pass and the launch before it.  Codes at
-// [step][fragment][K block][row], so that the lanes of a fragment read 16 rows in a
-// row; exponents as dwords of the quad's four steps, which the MFMAs select by number.
+// Activations: rows of one entry (at most `mr`, a power of two), bf16 ones quantised on
+// the way in, which saves the pass and the launch before it.  Codes at [step][K
+// block][row], so that the lanes read 16 rows in a row; exponents as dwords of the
+// quad's four steps, which the MFMAs select by number.
 struct MxStream {
   int ntiles;      // items of an entry
-  int mr;          // activation rows kept of a fragment
+  int mr;          // activation rows kept
   int xcodes;      // bytes of the codes, and
   int xbytes;      // with the exponents (the partial sums come behind)
   int turn;        // of the waves' 4 KB, behind the partial sums
 };
-// turned over in LDS
-constexpr bool mx_turns(int fragments, bool planes) { return fragments == 1 && !planes; }
 
-template <int XT, bool SILU, bool PLANES>
-__global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParams p, MxStream sp) {
+template <bool SILU, bool PLANES>
+__global__ __launch_bounds__(512, 4) void mx_stream_kernel(MxParams p, MxStream sp) {
   extern __shared__ __align__(16) uint8_t lds[];
   constexpr int WT = SILU ? 4 : 1;  // 16-row fragments of an item
   constexpr int COLS = SILU ? 32 : 16;
-  constexpr bool TURN = mx_turns(XT, PLANES);
+  constexpr bool TURN = !PLANES;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
   const int steps = p.K >> 7, quads = (steps + 3) >> 2;
@@ -167,9 +165,9 @@ __global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParam
     }
     const int count = (p.K >> 5) * rows, step = blockDim.x;
     auto put = [&](int r, int blk, u32x4 c, uint32_t byte) {
-      const int j = XT > 1 ? r >> 4 : 0, st = blk >> 2, rr = XT > 1 ? r & 15 : r;
-      *reinterpret_cast<u32x4 *>(lds + 16 * (((st * XT + j) * 4 + (blk & 3)) * mr + rr)) = c;
-      lds[sp.xcodes + 4 * ((((st >> 2) * XT + j) * 4 + (blk & 3)) * mr + rr) + (st & 3)] = (uint8_t)byte;
+      const int st = blk >> 2;
+      *reinterpret_cast<u32x4 *>(lds + 16 * (blk * mr + r)) = c;
+      lds[sp.xcodes + 4 * (((st >> 2) * 4 + (blk & 3)) * mr + r) + (st & 3)] = (uint8_t)byte;
     };
     auto at = [&](int i, int &r, int &blk) -> int64_t {  // (past the end: the last block again)
       i = min(i, count - 1);
@@ -226,9 +224,7 @@ __global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParam
     asm volatile("" ::: "memory");
   };
 
-  f32x4 acc[XT];
-#pragma unroll
-  for (int j = 0; j < XT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   Loads l0, l1;
   load(l0);
   load(l1);
@@ -241,18 +237,18 @@ __global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParam
   const uint8_t *xl = lds + 16 * (g * mr + (r16 & (mr - 1))), *xsl = lds + sp.xcodes + 4 * (g * mr + (r16 & (mr - 1)));
   int sub = 0, q = q0, odd = 0;
   auto finish = [&]() {  // an item's sums, in wave order
-    f32x4 *part = reinterpret_cast<f32x4 *>(lds + sp.xbytes) + odd * nw * WT * XT * 64;
-    auto total_of = [&](int t, int j, int l) {
-      f32x4 v = part[(t * XT + j) * 64 + l];
-      for (int w = 1; w < nw; ++w) v += part[((w * WT + t) * XT + j) * 64 + l];
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds + sp.xbytes) + odd * nw * WT * 64;
+    auto total_of = [&](int t, int l) {
+      f32x4 v = part[t * 64 + l];
+      for (int w = 1; w < nw; ++w) v += part[(w * WT + t) * 64 + l];
       return v;
     };
     if constexpr (SILU) {
       // eight lanes hold a block of 32 outputs of a row: four each
-      for (int i = tid; i < XT * 128; i += blockDim.x) {
+      for (int i = tid; i < 128; i += blockDim.x) {
         const int c = i & 7, m = i >> 3, t = c >> 2;
-        const int j = m >> 4, l = (c & 3) * 16 + (m & 15);
-        const f32x4 gt = total_of(t, j, l), up = total_of(t + 2, j, l);
+        const int l = (c & 3) * 16 + m;
+        const f32x4 gt = total_of(t, l), up = total_of(t + 2, l);
         float h[4];
         uint32_t am = 0;
 #pragma unroll
@@ -274,9 +270,9 @@ __global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParam
         }
       }
     } else {
-      for (int i = tid; i < XT * 64; i += blockDim.x) {
-        const int j = i >> 6, l = i & 63, n = tile * COLS + 4 * (l >> 4), m = 16 * j + (l & 15);
-        if (m < rows && n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + m] : r0 + m, n, total_of(0, j, l));
+      if (tid < 64) {
+        const int n = tile * COLS + 4 * (tid >> 4), m = tid & 15;
+        if (m < rows && n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + m] : r0 + m, n, total_of(0, tid));
       }
     }
   };
@@ -284,28 +280,16 @@ __global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParam
   auto body = [&](Loads &l) {
     const uint32_t ws = __builtin_amdgcn_perm(__builtin_amdgcn_perm(l.s.w, l.s.z, gsel),
                                               __builtin_amdgcn_perm(l.s.y, l.s.x, gsel), 0x05040100u);
-    uint32_t xs[XT];
+    const uint32_t xs = *reinterpret_cast<const uint32_t *>(xsl + 16 * q * mr);
+    u32x4 xc[4];  // (PLANES: steps past the end read the last one's)
 #pragma unroll
-    for (int j = 0; j < XT; ++j) xs[j] = *reinterpret_cast<const uint32_t *>(xsl + 16 * (q * XT + j) * mr);
-    u32x4 xc[4][XT];  // (PLANES: steps past the end read the last one's)
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int j = 0; j < XT; ++j)
-        xc[u][j] = ldg16(xl + 64 * ((PLANES ? min(4 * q + u, steps - 1) : 4 * q + u) * XT + j) * mr);
+    for (int u = 0; u < 4; ++u) xc[u] = ldg16(xl + 64 * (PLANES ? min(4 * q + u, steps - 1) : 4 * q + u) * mr);
     const int nst = PLANES ? steps - 4 * q : 4;
     auto multiply = [&](const u32x4 *w) {
-#pragma unroll
-      for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<0>(w[0], ws, xc[0][j], xs[j], acc[j]);
-      if (!PLANES || nst > 1)
-#pragma unroll
-        for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<1>(w[1], ws, xc[1][j], xs[j], acc[j]);
-      if (!PLANES || nst > 2)
-#pragma unroll
-        for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<2>(w[2], ws, xc[2][j], xs[j], acc[j]);
-      if (!PLANES || nst > 3)
-#pragma unroll
-        for (int j = 0; j < XT; ++j) acc[j] = mfma_mx<3>(w[3], ws, xc[3][j], xs[j], acc[j]);
+      acc = mfma_mx<0>(w[0], ws, xc[0], xs, acc);
+      if (!PLANES || nst > 1) acc = mfma_mx<1>(w[1], ws, xc[1], xs, acc);
+      if (!PLANES || nst > 2) acc = mfma_mx<2>(w[2], ws, xc[2], xs, acc);
+      if (!PLANES || nst > 3) acc = mfma_mx<3>(w[3], ws, xc[3], xs, acc);
     };
     if constexpr (TURN) {
       // 16-byte chunk c of row r at c ^ r: sixteen bank groups both ways
@@ -327,12 +311,9 @@ __global__ __launch_bounds__(512, XT == 1 ? 4 : 1) void mx_stream_kernel(MxParam
     __builtin_amdgcn_sched_barrier(0);
     if (++q < q1) return;
     q = q0;
-    f32x4 *part = reinterpret_cast<f32x4 *>(lds + sp.xbytes) + ((odd * nw + wave) * WT + sub) * XT * 64;
-#pragma unroll
-    for (int j = 0; j < XT; ++j) {
-      part[j * 64 + lane] = acc[j];
-      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds + sp.xbytes) + ((odd * nw + wave) * WT + sub) * 64;
+    part[lane] = acc;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
     if (++sub < WT) return;
     sub = 0;
     meet();
@@ -1179,14 +1160,13 @@ static int mx_lds(F *fn, int bytes) {  // dynamic LDS above 64 KB
   return e == hipSuccess ? AMLA_OK : fail((int)e, "mxfp4 product: LDS size: %s", hipGetErrorString(e));
 }
 
-// Activation rows kept of a fragment, and fragments, for entries of at most `rows` rows
+// Activation rows kept for entries of at most `rows` <= 16 rows
 static int mx_keep(int rows) {
   int mr = 1;
-  while (mr < rows && mr < 16) mr *= 2;
+  while (mr < rows) mr *= 2;
   return mr;
 }
-static int mx_fragments(int rows) { return (rows + 15) / 16; }
-static int64_t mx_stream_bytes(int rows, int64_t K) { return (int64_t)mx_keep(rows) * mx_fragments(rows) * (K / 2 + (K + 511) / 512 * 16); }
+static int64_t mx_stream_bytes(int rows, int64_t K) { return (int64_t)mx_keep(rows) * (K / 2 + (K + 511) / 512 * 16); }
 // waves of a workgroup: equal runs of quads where there are any, rather four to seven
 // (7168 x 16384, one row: four 17.9 us, eight 19.3)
 static int mx_waves(int64_t K) {
@@ -1204,21 +1184,26 @@ static int mx_waves(int64_t K) {
 }
 
 static int64_t mx_stream_sums(int rows, int64_t K, bool silu) {  // with two items' partial sums
-  return mx_stream_bytes(rows, K) + 2048 * mx_waves(K) * mx_fragments(rows) * (silu ? 4 : 1);
+  return mx_stream_bytes(rows, K) + 2048 * mx_waves(K) * (silu ? 4 : 1);
 }
 static int64_t mx_stream_lds(int rows, int64_t K, bool silu) {
-  return mx_stream_sums(rows, K, silu) + (mx_turns(mx_fragments(rows), K % 512) ? 4096 * mx_waves(K) : 0);
+  return mx_stream_sums(rows, K, silu) + (K % 512 ? 0 : 4096 * mx_waves(K));
 }
-static bool mx_stream_fits(int rows, int64_t K, bool silu) {
-  return rows <= (silu ? 16 : 64) && mx_stream_lds(rows, K, silu) <= 160 * 1024;
+// Up to 16 rows, as long as it does not take longer to take them in (each workgroup for
+// itself) than a tile's pipeline to start: 16 x 7168 x 12288 19.0 us, tiles 20.0; 12 x 7168
+// x 16384 24.3 and 22.6; 5 x 7168 x 32768 40 and 35.  Above, tiles: 32 x 18432 x 7168 24.0
+// us, with two fragments of activation rows here 26; 64 x 24576 x 1536 8.6, with four 13.7
+// (few outputs lose by it: 20 x 2112 x 7168 12.5, here 10.4).
+static bool mx_stream_fits(int64_t rows, int64_t K, bool silu) {
+  return rows <= 16 && mx_stream_bytes((int)rows, K) <= 112 * 1024 && mx_stream_lds((int)rows, K, silu) <= 160 * 1024;
 }
 
-template <int XT, bool SILU>
-static int launch_stream(const MxParams &p, int rows, int entries, hipStream_t st) {
+template <bool SILU>
+static int launch_mx_stream(const MxParams &p, int rows, int entries, hipStream_t st) {
   MxStream sp;
   sp.ntiles = (p.N + (SILU ? 31 : 15)) / (SILU ? 32 : 16);
   sp.mr = mx_keep(rows);
-  sp.xcodes = sp.mr * XT * (p.K >> 1);
+  sp.xcodes = sp.mr * (p.K >> 1);
   sp.xbytes = (int)mx_stream_bytes(rows, p.K);
   sp.turn = (int)mx_stream_sums(rows, p.K, SILU);
   const int nw = mx_waves(p.K);
@@ -1230,24 +1215,11 @@ static int launch_stream(const MxParams &p, int rows, int entries, hipStream_t s
   const int per_cu = std::max<int>(1, (int)std::min<int64_t>({16 / nw, 160 * 1024 / lds, items / (3 * 256)}));
   const int64_t run = (items + 256 * per_cu - 1) / (256 * per_cu);  // items of the longest run
   const unsigned blocks = (unsigned)((items + run - 1) / run);
-  const auto kernel = p.K % 512 ? mx_stream_kernel<XT, SILU, true> : mx_stream_kernel<XT, SILU, false>;
+  const auto kernel = p.K % 512 ? mx_stream_kernel<SILU, true> : mx_stream_kernel<SILU, false>;
   const int rc = mx_lds(kernel, lds);
   if (rc) return rc;
   kernel<<<dim3(blocks), 64 * nw, lds, st>>>(p, sp);
   return check_launch("mxfp4 stream product");
-}
-
-// Entries of at most `rows` <= 64 rows, bf16 rows where p.xs is null.
-static int launch_mx_stream(const MxParams &p, int rows, int entries, hipStream_t st) {
-  switch (mx_fragments(rows)) {
-    case 1: return launch_stream<1, false>(p, rows, entries, st);
-    case 2: return launch_stream<2, false>(p, rows, entries, st);
-    case 3: return launch_stream<3, false>(p, rows, entries, st);
-    default: return launch_stream<4, false>(p, rows, entries, st);
-  }
-}
-static int launch_mx_stream_silu(const MxParams &p, int rows, int entries, hipStream_t st) {
-  return launch_stream<1, true>(p, rows, entries, st);
 }
 
 // The tiles of one weight by what they cost: a stage of 256 K values and the rest of a
@@ -1352,12 +1324,14 @@ struct MxLinearLayout {
   bool stream, fused;  // fused: the stream product quantises
   MxSplit sp;
 };
-constexpr int64_t MX_FUSED = 32 * 1024;  // values of x that each workgroup may quantise for itself
+// Values of x that each workgroup may quantise for itself: 1 x 7168 x 16384 16.8 us, with a
+// pass before it 19.0; 8 x 18432 x 7168 20.7 and 21.3; 16 x 2112 x 7168 11.8 and 11.0.
+constexpr int64_t MX_FUSED = 72 * 1024;
 // held: x comes quantised
 static MxLinearLayout mx_linear_layout(int64_t m, int64_t k, int64_t n, bool held) {
   MxLinearLayout L = {};
   MxTake take;
-  L.stream = m <= 64 && mx_stream_fits((int)m, k, false);
+  L.stream = mx_stream_fits(m, k, false);
   L.fused = L.stream && m * k <= MX_FUSED;
   if (!held && !L.fused) {
     L.xc = take(mx_codes_bytes(m, k));
@@ -1379,7 +1353,7 @@ struct MxGroupedLayout {
 static MxGroupedLayout mx_grouped_layout(int64_t m, int64_t k, int64_t E, bool held) {
   MxGroupedLayout L = {};
   MxTake take;
-  L.stream = m <= 16 && mx_stream_fits((int)m, k, false);
+  L.stream = mx_stream_fits(m, k, false);
   L.rows = L.stream ? 16 : MX_ROWS;
   L.max_entries = (int)(std::min(E, m) + m / L.rows + 2);
   L.count = take(8);
@@ -1401,7 +1375,7 @@ struct MxSwigluLayout {
 static MxSwigluLayout mx_swiglu_layout(int64_t m, int64_t k, int64_t n) {
   MxSwigluLayout L = {};
   MxTake take;
-  L.stream = m <= 16 && mx_stream_fits((int)m, k, true);
+  L.stream = mx_stream_fits(m, k, true);
   L.hc = take(mx_codes_bytes(m, n));
   L.hs = take(mx_scale_bytes(m, n));
   if (!L.stream) {
@@ -1424,7 +1398,7 @@ static MxMoeLayout mx_moe_layout(int64_t m, int64_t d, int top_k, int64_t n, int
   MxMoeLayout L = {};
   MxTake take;
   const int64_t S = m * top_k;
-  L.stream = m <= 16 && mx_stream_fits((int)m, d, true) && mx_stream_fits((int)m, n, false);
+  L.stream = mx_stream_fits(m, d, true) && mx_stream_fits(m, n, false);
   L.rows = L.stream ? (int)m : MX_ROWS;  // (a token may name an expert several times: more entries)
   L.max_entries = (int)std::min<int64_t>(S, std::min<int64_t>(E, S) + S / L.rows);
   L.hdr = take(16);
@@ -1506,7 +1480,7 @@ int amla_mxfp4_linear(const void *x, const void *x_scales, int64_t m, int64_t k,
     p.x = ws + L.xc;
     p.xs = ws + L.xs;
   }
-  if (L.stream) return launch_mx_stream(p, (int)m, 1, st);
+  if (L.stream) return launch_mx_stream<false>(p, (int)m, 1, st);
   MxSplit sp = L.sp;
   sp.partial = reinterpret_cast<float *>(ws + L.part);
   return launch_mx_linear<false>(p, sp, st);
@@ -1556,7 +1530,7 @@ int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, in
   p.rest = clear_rest != 0;
   p.M = (int)m; p.N = (int)n; p.K = (int)k;
   mx_outputs(p, y, ldy, dtype);
-  if (L.stream) return launch_mx_stream(p, (int)m, (int)std::min<int64_t>(n_experts, m), st);
+  if (L.stream) return launch_mx_stream<false>(p, (int)m, (int)std::min<int64_t>(n_experts, m), st);
   if (!x_scales) {
     if ((rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(x), m, k, ldx, ws + L.xc, ws + L.xs, st))) return rc;
     p.x = ws + L.xc;
@@ -1604,7 +1578,7 @@ int amla_mxfp4_swiglu(const void *x, int64_t m, int64_t k, int64_t ldx, const vo
   p.hs = ws + L.hs;
   int rc;
   if (L.stream) {
-    rc = launch_mx_stream_silu(p, (int)m, 1, st);
+    rc = launch_mx_stream<true>(p, (int)m, 1, st);
   } else {
     if ((rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(x), m, k, ldx, ws + L.xc, ws + L.xs, st))) return rc;
     p.x = ws + L.xc;
@@ -1681,8 +1655,8 @@ int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh
   q.N = (int)d; q.K = (int)n_inter;
   mx_outputs(q, expert_out, d, AMLA_BF16);
   if (L.stream) {
-    if ((rc = launch_mx_stream_silu(p, (int)m, L.max_entries, st))) return rc;
-    return launch_mx_stream(q, (int)m, L.max_entries, st);
+    if ((rc = launch_mx_stream<true>(p, (int)m, L.max_entries, st))) return rc;
+    return launch_mx_stream<false>(q, (int)m, L.max_entries, st);
   }
   if ((rc = launch_mx_quantize_bf16(static_cast<const uint16_t *>(hidden), m, d, ldh, ws + L.xc, ws + L.xs, st)))
     return rc;
