@@ -65,9 +65,14 @@ AMLA_DEV float mx_silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; 
 //
 // The matrix units want 16 rows x 64 bytes in a register.  A load takes 4 rows x 256
 // bytes all the same, and the wave turns the quad over in 4 KB of LDS of its own (no
-// barrier: its LDS operations stay in order): memory delivers whole lines faster (8 x 65536 x 7168 58 -> 54 us, 8 x 7168 x 18432 22.8 -> 21.5, 4 x 2112
-// x 7168 7.0 -> 6.3).  Four waves a SIMD have to fit: with 129 registers instead of 128
-// the down projections of 57 experts took 87 us, 73 so.
+// barrier: its LDS operations stay in order): memory delivers whole lines faster (8 x
+// 65536 x 7168 58 -> 54 us, 8 x 7168 x 18432 22.8 -> 21.5, 4 x 2112 x 7168 7.0 -> 6.3).
+// Four waves a SIMD have to fit: with 129 registers instead of 128 the down projections
+// of 57 experts took 87 us, 73 so.
+//
+// Bound by the weights' stream: 1 x 262144 x 7168 in 177 us, 5.6 TB/s, and 4 us for the
+// start and the end of a call.  Three quads in flight instead of two, two or four 16-row
+// fragments an item and other numbers of workgroups changed that by 2 % at most.
 //
 // Activations: rows of one entry (at most `mr`, a power of two), bf16 ones quantised on
 // the way in, which saves the pass and the launch before it.  Codes at [step][K
@@ -1208,11 +1213,13 @@ static int launch_mx_stream(const MxParams &p, int rows, int entries, hipStream_
   sp.turn = (int)mx_stream_sums(rows, p.K, SILU);
   const int nw = mx_waves(p.K);
   const int lds = (int)mx_stream_lds(rows, p.K, SILU);
-  // three items or more a workgroup (each takes in the activations for itself), up to
-  // 16 waves a CU.  18432 x 7168, one row: 256 workgroups 19.6 us, 512 22.0; 24576 x
-  // 1536, 8 rows: 512 9.0, 1280 9.8; 57 experts of 7168 x 2048: 256 110, 1024 75.
-  const int64_t items = (int64_t)entries * sp.ntiles;
-  const int per_cu = std::max<int>(1, (int)std::min<int64_t>({16 / nw, 160 * 1024 / lds, items / (3 * 256)}));
+  // Three items or more a workgroup (each takes in the activations for itself), up to 16
+  // waves a CU, but more than one workgroup of few waves for few rows.  8 x 24576 x 1536:
+  // 512 workgroups 8.6 us, 1280 9.3; 1 x 7168 x 16384, four waves each: 448 of one item
+  // 15.9, 224 of two 16.8; 8 x 7168 x 8192: 16.6 and 15.0; 1 x 7168 x 18432, six waves: 19.8
+  // and 18.3; down projections of 57 experts of 7168 x 2048: 256 108, 1024 73.
+  const int64_t items = (int64_t)entries * sp.ntiles, most = std::min(16 / nw, 160 * 1024 / lds);
+  const int per_cu = (int)std::max<int64_t>(1, std::min(most, std::max<int64_t>(items / (3 * 256), nw <= 4 && sp.mr <= 4 ? 2 : 1)));
   const int64_t run = (items + 256 * per_cu - 1) / (256 * per_cu);  // items of the longest run
   const unsigned blocks = (unsigned)((items + run - 1) / run);
   const auto kernel = p.K % 512 ? mx_stream_kernel<SILU, true> : mx_stream_kernel<SILU, false>;
