@@ -382,7 +382,10 @@ struct MxSums {
 
 // Up to 16 XF <= 128 activation rows: the two halves of the workgroup take the two K
 // steps of a stage (and meet in LDS at the end).  Three slots, two stages on their way.
-// Bound by the weights' stream for the few rows that an expert gets.
+// Bound by the weights' stream for the few rows that an expert gets: gate and up of 256
+// experts of 7168 x 2048 for 2000 tokens in 840 us, 4.8 TB/s.  Copies of the weights alone
+// take 612; those of the activations add 55, of the exponents (16 of a line's 128 bytes at
+// a time) 45, the stores 35, entries of more than 128 rows 55.
 template <int XF>
 struct MxRowsLds {
   static constexpr int XROWS = XF > 4 ? 128 : 16 * XF;
@@ -536,8 +539,8 @@ struct MxRowsMain {
 // multiplied, so that the slot is free for the stage after next when the second
 // begins.
 //
-// What bounds it is the power of the matrix units: 4096 x 7168 x 16384 in 272 us (3.5
-// PFLOP/s); the multiplications and barriers alone, on the same data, take 223 us.
+// What bounds it is the power of the matrix units: 4096 x 7168 x 16384 in 241 - 255 us (3.8
+// - 4.0 PFLOP/s); the multiplications and barriers alone, on the same data, take 223 us.
 // Four slots of 64-byte rows, two stages on their way: 306 us (the L2 delivers 20
 // TB/s in such pieces, 35 TB/s in lines).  256 x 128 tiles, two workgroups per CU: 332.
 constexpr int MXB_STAGE = 2 * MX_WHALF;
@@ -1068,6 +1071,8 @@ __global__ __launch_bounds__(256) void mx_finish_kernel(MxParams p, MxSplit sp) 
 
 // The scheduled entries of up to 256 rows: a contiguous run of (entry, column
 // tile) per XCD, so that the activation rows of an entry are read from one L2.
+// A workgroup a tile: persistent ones that take the next tile's first stages during
+// the stores were slower (gate and up of 2000 tokens 930 us against 900, in turn).
 template <bool SILU, bool PLANES>
 __global__ __launch_bounds__(512, 1) void mx_sched_kernel(MxParams p, int ntiles) {
   const int l = xcd_run(blockIdx.x, (p.count[0] + (p.rest ? p.count[1] : 0)) * ntiles);

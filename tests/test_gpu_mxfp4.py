@@ -320,6 +320,25 @@ def test_moe_experts_with_one_expert_for_every_slot(m, top_k):
     assert torch.equal(got, once.expand(m, top_k, 640))
 
 
+def test_moe_experts_of_more_slots_than_a_call_takes():
+    """9000 x 8 slots run as two calls (65536 slots each at most): tokens on both sides of the cut."""
+    g = _gen(5)
+    x, w = _x(g, 9000, 128), _ffn(g, 128, 128, 16)
+    idx = torch.rand(9000, 16, generator=g).argsort(1)[:, :8].contiguous()
+    idx[8191, 3], idx[8192, 0] = -1, 16
+    got = ops.mxfp4_moe_experts(x.to(DEV), idx.to(DEV), w).cpu()
+    t = torch.tensor([0, 1, 4095, 8190, 8191, 8192, 8193, 8999])
+    vals = {key: _vals(w[key]) for key in w}
+    xq = M.rounded(x[t])
+    want, slack = torch.zeros(len(t), 8, 128, dtype=torch.float64), torch.zeros(len(t), 8, 128, dtype=torch.float64)
+    for i, tok in enumerate(t.tolist()):
+        for j, e in enumerate(idx[tok].tolist()):
+            if 0 <= e < 16:
+                y, s = M.swiglu(xq[i:i + 1], vals["gate_proj"][e], vals["up_proj"][e], vals["down_proj"][e])
+                want[i, j], slack[i, j] = y[0], s[0]
+    _check(got[t], want, slack + HALF_STEP[BF16] * want.abs() + 2.0 ** -8 * slack, "9000 tokens")
+
+
 @pytest.mark.parametrize("tokens", [3, 40])
 def test_moe_block_on_mxfp4_experts(tokens):
     """route, the shared expert (fp8), the MXFP4 experts and the combine as an engine runs them, also
@@ -417,6 +436,29 @@ def test_side_stream_and_capture():
         eager = step(fresh)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), i
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call has scratch of its own: what runs beside it leaves its result alone."""
+    g = _gen(7)
+    w, ff = _weight(g, 2048, 1024), _ffn(g, 512, 256, 8)
+    xs = [(_x(g, 200, 1024).to(DEV), _x(g, 100, 512).to(DEV), torch.randint(0, 8, (100, 4), generator=g).to(DEV))
+          for _ in range(2)]
+
+    def step(a, b, idx):
+        return ops.mxfp4_linear(a, *w), ops.mxfp4_linear(a[:5], *w), ops.mxfp4_moe_experts(b, idx, ff)
+
+    want = [step(*x) for x in xs]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(step(*xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for res in got[i] for a, b in zip(res, want[i]))
 
 
 def test_compiled_calls_equal_eager_ones():
