@@ -36,7 +36,7 @@ def _stream_ptr(t: torch.Tensor) -> int:
 
 
 def _need_cuda(t: torch.Tensor, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a tensor on a ROCm device")
 
 

@@ -817,9 +817,9 @@ AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, in
   }
 }
 
-// Few tiles of one weight: 128 weight rows x up to 64 activation rows for sixteen waves,
-// wave w on weight rows 32 (w % 4) .. +31 and K step w / 4 of a stage of 512 K values;
-// the four sums of an output meet in LDS.  Nothing but waits bounds such a call (a
+// Few tiles: 128 weight rows (gate and up: 64 + 64) x up to 64 activation rows for sixteen
+// waves, wave w on weight rows 32 (w % 4) .. +31 (16 (w % 4) .. +15 of each) and K step
+// w / 4 of a stage of 512 K values; the four sums of an output meet in LDS.  Nothing but waits bounds such a call (a
 // barrier, the reads and eight multiplications one after the other in every wave), so
 // its stages are long and four waves of a SIMD stand in for each other: 777 x 2112 x
 // 7168 in 17.3 us, 21.8 with tiles of 256 x 32; eight waves with stages of 256 and five
@@ -832,26 +832,33 @@ constexpr int MXS_X = 2 * 128 * 128, MXS_SCALES = MXS_X + 2 * MXS_ROWS * 128, MX
 constexpr int MXS_LDS = 3 * MXS_STAGE;
 static_assert(MXS_LDS <= 160 * 1024 && 16 * 8 * 1024 <= MXS_LDS, "LDS of a CU, the sums");
 
-template <bool PLANES>
-AMLA_DEV void mx_small_tile(const MxParams &p, int r0, int rows, int n0) {
+template <bool SILU, bool PLANES>
+AMLA_DEV void mx_small_tile(const MxParams &p, int e, int r0, int rows, int n0) {
   extern __shared__ __align__(16) uint8_t lds[];
   constexpr int C = 3 + (PLANES ? 4 : 1);  // copies of a wave and stage
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wk = wave >> 2;
   const int64_t kb = p.K >> 1, ksb = p.K >> 5;
-  const int steps = p.K >> 7, quads = (steps + 3) >> 2, wrows = min(128, p.N - n0);
-  const auto wrsrc = mx_rsrc(p.w[0] + n0 * kb), xrsrc = mx_rsrc(static_cast<const uint8_t *>(p.x) + r0 * kb);
+  const int steps = p.K >> 7, quads = (steps + 3) >> 2, wrows = min(SILU ? 64 : 128, p.N - n0);
   // wave w copies half w / 8 of weight rows 16 (w % 8) .. +15 and x rows 8 (w % 8) .. +7
   // (rows past the tile repeat its last)
-  const int half = wave >> 3, w8 = wave & 7, ch = lane & 7;
+  const int half = wave >> 3, w8 = wave & 7, seg = SILU ? w8 >> 2 : 0, ch = lane & 7;
+  const auto wrsrc = mx_rsrc((seg ? p.w[1] : p.w[0]) + e * p.wstride + n0 * kb);
+  const auto xrsrc = mx_rsrc(static_cast<const uint8_t *>(p.x) + (p.xrow ? 0 : r0 * kb));
+  auto xrow_of = [&](int r) {  // (a gathered x is less than 4 GB)
+    const int rc = min(r, rows - 1);
+    return (uint32_t)(p.xrow ? p.xrow[r0 + rc] : rc);
+  };
   const int wr = 16 * w8 + (lane >> 3), xr = 8 * w8 + (lane >> 3);  // (the second weight copy: row + 8, the same chunk ^ 4)
-  const int wch = ch ^ ((wr >> 1) & 7), xch = ch ^ ((xr >> 1) & 7);
-  const uint32_t woff[2] = {(uint32_t)min(wr, wrows - 1) * (uint32_t)kb + 16 * wch,
-                            (uint32_t)min(wr + 8, wrows - 1) * (uint32_t)kb + 16 * (wch ^ 4)};
-  const uint32_t xoff = (uint32_t)min(xr, rows - 1) * (uint32_t)kb + 16 * xch;
+  const int wch = ch ^ ((wr >> 1) & 7), xch = ch ^ ((xr >> 1) & 7), wl = wr - 64 * seg;
+  const uint32_t woff[2] = {(uint32_t)min(wl, wrows - 1) * (uint32_t)kb + 16 * wch,
+                            (uint32_t)min(wl + 8, wrows - 1) * (uint32_t)kb + 16 * (wch ^ 4)};
+  const uint32_t xoff = xrow_of(xr) * (uint32_t)kb + 16 * xch;
   typedef const __attribute__((address_space(1))) uint8_t *gptr;
-  const gptr sptr = lane < 8 ? (gptr)(p.ws[0] + (n0 + (int64_t)min(8 * wave + lane, wrows - 1)) * ksb)
-                             : (gptr)(p.xs + (r0 + (int64_t)min(4 * wave + (lane & 3), rows - 1)) * ksb);
+  const int sseg = SILU ? wave >> 3 : 0;
+  const gptr sptr = lane < 8 ? (gptr)((sseg ? p.ws[1] : p.ws[0]) + e * p.sstride +
+                                      (n0 + (int64_t)min(8 * wave - 64 * sseg + lane, wrows - 1)) * ksb)
+                             : (gptr)(p.xs + ((p.xrow ? 0 : r0) + (int64_t)xrow_of(4 * wave + (lane & 3))) * ksb);
   auto issue = [&](int q, int slot) {
     uint8_t *st = lds + slot * MXS_STAGE;
     const uint32_t off = q * 256 + 128 * half;
@@ -883,6 +890,7 @@ AMLA_DEV void mx_small_tile(const MxParams &p, int r0, int rows, int n0) {
   if (quads > 1) issue(1, 1);
 
   const uint32_t frag = r16 * 128 + 16 * ((4 * (wk & 1) + g) ^ ((r16 >> 1) & 7));
+  auto wfrag = [&](int f) { return SILU ? 64 * f + 16 * wn : 32 * wn + 16 * f; };  // its first row
   int slot = 0;
   for (int q = 0; q < quads; ++q) {
     if (q + 1 < quads) wait_vmcnt<C>();  // all but the next stage's copies have landed
@@ -898,13 +906,13 @@ AMLA_DEV void mx_small_tile(const MxParams &p, int r0, int rows, int n0) {
     const uint8_t *sc = st + MXS_SCALES + wk * (PLANES ? 768 : 4) + g;
     auto scale = [&](int r) { return (uint32_t)sc[r * (PLANES ? 4 : 16)]; };
 #pragma unroll
-    for (int f = 0; f < 2; ++f) wsc[f] = scale(12 * (4 * wn + 2 * f + (r16 >> 3)) + (r16 & 7));
+    for (int f = 0; f < 2; ++f) wsc[f] = scale(12 * (wfrag(f) / 8 + (r16 >> 3)) + (r16 & 7));
 #pragma unroll
     for (int j = 0; j < 4; ++j) xsc[j] = scale(12 * (4 * j + (r16 >> 2)) + 8 + (r16 & 3));
-    const uint8_t *wp = st + (wk >> 1) * 16384 + 32 * wn * 128 + frag, *xp = st + MXS_X + (wk >> 1) * 8192 + frag;
+    const uint8_t *wp = st + (wk >> 1) * 16384 + frag, *xp = st + MXS_X + (wk >> 1) * 8192 + frag;
     u32x4 wf[2], xf[4];
 #pragma unroll
-    for (int f = 0; f < 2; ++f) wf[f] = *reinterpret_cast<const u32x4 *>(wp + f * 2048);
+    for (int f = 0; f < 2; ++f) wf[f] = *reinterpret_cast<const u32x4 *>(wp + wfrag(f) * 128);
 #pragma unroll
     for (int j = 0; j < 4; ++j) xf[j] = *reinterpret_cast<const u32x4 *>(xp + j * 2048);
 #pragma unroll
@@ -934,24 +942,69 @@ AMLA_DEV void mx_small_tile(const MxParams &p, int r0, int rows, int n0) {
     for (int k = 1; k < 4; ++k) sum.f[f] += ex[(((wn + 4 * k) * 2 + f) * 4 + wk) * 64];
   }
   meet();  // (LDS is free)
-  mx_tile_store<1, false, 1>(p, [&](int) { return sum; }, wk, wn, rows, r0, n0);
+  if constexpr (!SILU) {
+    mx_tile_store<1, false, 1>(p, [&](int) { return sum; }, wk, wn, rows, r0, n0);
+  } else {
+    // sum: gate and up of outputs 16 wn + 4 g .. +3 of row 16 wk + r16; then four lanes
+    // hold a block of 32 outputs of a row: eight each
+    constexpr int PITCH = 64 + 4;
+    float *h = reinterpret_cast<float *>(lds);
+    f32x4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = mx_silu_mul(sum.f[0][k], sum.f[1][k]);
+    *reinterpret_cast<f32x4 *>(h + PITCH * (16 * wk + r16) + 16 * wn + 4 * g) = v;
+    meet();
+    const int m = tid >> 3, c = tid & 7;
+    if (m < rows) {  // (tid < 512; the lanes of a row together)
+      float o[8];
+      uint32_t am = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        o[k] = h[PITCH * m + 8 * c + k];
+        am = max(am, __float_as_uint(o[k]) & 0x7fffffffu);
+      }
+      am = max(am, dpp_u32<0xB1>(am));  // quad_perm [1,0,3,2]
+      am = max(am, dpp_u32<0x4E>(am));  // quad_perm [2,3,0,1]
+      const uint32_t byte = mx_byte(am), codes = mx_codes8(o, mx_scale(byte));
+      *reinterpret_cast<uint32_t *>(p.hc + (int64_t)(r0 + m) * (p.N >> 1) + (n0 >> 1) + 4 * c) = byte == 255 ? 0u : codes;
+      if ((c & 3) == 0) p.hs[(int64_t)(r0 + m) * (p.N >> 5) + (n0 >> 5) + (c >> 2)] = (uint8_t)byte;
+    }
+  }
 }
 
-template <bool PLANES>
+template <bool SILU, bool PLANES>
 __global__ __launch_bounds__(1024, 1) void mx_small_kernel(MxParams p, int n_tiles, int m_tiles) {
   const int t = xcd_run(blockIdx.x, n_tiles * m_tiles);
   if (t < 0) return;
   int nt, mt;
   tile_coords(t, n_tiles, m_tiles, nt, mt, TL_PANEL / 2);
   const int r0 = uniform(mt) * MXS_ROWS;
-  mx_small_tile<PLANES>(p, r0, min(MXS_ROWS, p.M - r0), uniform(nt) * 128);
+  mx_small_tile<SILU, PLANES>(p, 0, r0, min(MXS_ROWS, p.M - r0), uniform(nt) * (SILU ? 64 : 128));
+}
+
+// The same for the scheduled entries of up to 64 rows.
+template <bool SILU, bool PLANES>
+__global__ __launch_bounds__(1024, 1) void mx_small_sched_kernel(MxParams p, int ntiles) {
+  const int l = xcd_run(blockIdx.x, (p.count[0] + (p.rest ? p.count[1] : 0)) * ntiles);
+  if (l < 0) return;
+  const int t = uniform(l / ntiles), n0 = (uniform(l) - t * ntiles) * (SILU ? 64 : 128);
+  const int32_t *en = p.ent + 4 * t;
+  const int e = uniform(en[0]), r0 = uniform(en[1]), rows = uniform(en[2]);
+  if (!SILU && e < 0) {  // rows of no expert
+    for (int i = threadIdx.x; i < rows * 32; i += 1024) {
+      const int r = i >> 5, n = n0 + 4 * (i & 31);
+      if (n < p.N) mx_store4(p, p.yrow ? p.yrow[r0 + r] : r0 + r, n, f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    return;
+  }
+  mx_small_tile<SILU, PLANES>(p, e, r0, rows, n0);
 }
 
 // One weight: tiles of 256 outputs (SILU: 128) x `rows` activation rows.  The first
 // `whole` tiles (rounds of 256) take all of K, the others a K part a workgroup.
 struct MxSplit {
   int n_tiles, m_tiles, rows, whole;
-  bool small;      // tiles of 128 outputs x 64 rows (parts 1)
+  bool small;      // tiles of 128 outputs (SILU: 64) x 64 rows (parts 1)
   int parts;       // K parts of the other tiles, whole runs of four steps
   float *partial;  // [tile][part][activation fragment][weight fragment][wave % 4][lane] f32x4
 };
@@ -1160,7 +1213,7 @@ __global__ __launch_bounds__(256) void mx_clear_skipped_kernel(const int64_t *__
 
 // ---------------------------------------------------------------- launches
 
-constexpr int64_t MX_MAX_BLOCKS = (1 << 23) - 8;  // of 512 threads, fewer than 2^32 a launch
+constexpr int64_t MX_MAX_BLOCKS = (1 << 22) - 8;  // of 1024 threads, fewer than 2^32 a launch
 
 template <typename F>
 static int mx_lds(F *fn, int bytes) {  // dynamic LDS above 64 KB
@@ -1269,12 +1322,12 @@ static MxSplit plan_mx_split(int64_t M, int N, int K, bool silu) {
     }
     if (sp.rows >= M) break;
   }
-  if (!silu && M > 32) {
+  if (M > 32) {
     MxSplit sp = {};
     sp.small = true;
     sp.parts = 1;
     sp.rows = MXS_ROWS;
-    sp.n_tiles = (N + 127) / 128;
+    sp.n_tiles = silu ? (N + 63) / 64 : (N + 127) / 128;
     sp.m_tiles = (int)((M + MXS_ROWS - 1) / MXS_ROWS);
     const double rounds = (double)(((int64_t)sp.n_tiles * sp.m_tiles + 255) / 256);
     if (rounds * (quads * small_quad_us + small_tile_us) < least) best = sp;
@@ -1292,13 +1345,12 @@ static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st
   if (!sp.rows || blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
   const auto kernel = p.K % 512 ? mx_linear_kernel<SILU, true> : mx_linear_kernel<SILU, false>;
   int rc;
-  if constexpr (!SILU)
-    if (sp.small) {
-      const auto small = p.K % 512 ? mx_small_kernel<true> : mx_small_kernel<false>;
-      if ((rc = mx_lds(small, MXS_LDS))) return rc;
-      small<<<dim3((unsigned)blocks), 1024, MXS_LDS, st>>>(p, sp.n_tiles, sp.m_tiles);
-      return check_launch("mxfp4 product of few tiles");
-    }
+  if (sp.small) {
+    const auto small = p.K % 512 ? mx_small_kernel<SILU, true> : mx_small_kernel<SILU, false>;
+    if ((rc = mx_lds(small, MXS_LDS))) return rc;
+    small<<<dim3((unsigned)blocks), 1024, MXS_LDS, st>>>(p, sp.n_tiles, sp.m_tiles);
+    return check_launch("mxfp4 product of few tiles");
+  }
   if ((rc = mx_lds(kernel, MX_TILE_LDS))) return rc;
   kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, sp);
   if ((rc = check_launch("mxfp4 product")) || sp.parts == 1) return rc;
@@ -1306,14 +1358,31 @@ static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st
   return check_launch("mxfp4 K-part finish");
 }
 
+// Whether `slots` rows in groups of E make at most a round of small tiles (of a product
+// of `tiles` of them side by side).  The estimate takes the groups as equal: the sizes
+// are known to the device alone, and the grid is made for the worst case.  K = 7168 to 2048
+// outputs with schedule and quantising: 300 rows in 2 groups 23 us, large tiles 52; 1000 in
+// 4 32 and 68; 40 in 16 (256 tiles) 33 and 43.  Two rounds: 150 rows in 32 groups 36.6 and
+// 32.4 (the product alone), 40 rows in 8 groups, 2048 to 7168, 24.8 and 20.8.
+static bool mx_small_round(int64_t slots, int64_t E, int64_t tiles) {
+  const int64_t groups = std::min(E, slots), each = (slots + groups - 1) / groups;
+  return groups * ((each + MXS_ROWS - 1) / MXS_ROWS) * tiles <= 256;
+}
+
 template <bool SILU>
-static int launch_mx_sched(const MxParams &p, int max_entries, hipStream_t st) {
-  const int cols = SILU ? 128 : 256, ntiles = (p.N + cols - 1) / cols;
+static int launch_mx_sched(const MxParams &p, int max_entries, bool small, hipStream_t st) {
+  const int cols = (SILU ? 128 : 256) / (small ? 2 : 1), ntiles = (p.N + cols - 1) / cols;
   const int64_t blocks = ((int64_t)max_entries * ntiles + 7) / 8 * 8;
   if (blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d entries", max_entries);
+  int rc;
+  if (small) {
+    const auto kernel = p.K % 512 ? mx_small_sched_kernel<SILU, true> : mx_small_sched_kernel<SILU, false>;
+    if ((rc = mx_lds(kernel, MXS_LDS))) return rc;
+    kernel<<<dim3((unsigned)blocks), 1024, MXS_LDS, st>>>(p, ntiles);
+    return check_launch("mxfp4 grouped product of few tiles");
+  }
   const auto kernel = p.K % 512 ? mx_sched_kernel<SILU, true> : mx_sched_kernel<SILU, false>;
-  const int rc = mx_lds(kernel, MX_TILE_LDS);
-  if (rc) return rc;
+  if ((rc = mx_lds(kernel, MX_TILE_LDS))) return rc;
   kernel<<<dim3((unsigned)blocks), 512, MX_TILE_LDS, st>>>(p, ntiles);
   return check_launch("mxfp4 grouped product");
 }
@@ -1360,13 +1429,14 @@ static MxLinearLayout mx_linear_layout(int64_t m, int64_t k, int64_t n, bool hel
 struct MxGroupedLayout {
   size_t count, ent, xc, xs, total;
   int rows, max_entries;  // of an entry; entries at most
-  bool stream;
+  bool stream, small;
 };
-static MxGroupedLayout mx_grouped_layout(int64_t m, int64_t k, int64_t E, bool held) {
+static MxGroupedLayout mx_grouped_layout(int64_t m, int64_t k, int64_t n, int64_t E, bool held) {
   MxGroupedLayout L = {};
   MxTake take;
   L.stream = mx_stream_fits(m, k, false);
-  L.rows = L.stream ? 16 : MX_ROWS;
+  L.small = !L.stream && mx_small_round(m, E, (n + 127) / 128);
+  L.rows = L.stream ? 16 : L.small ? MXS_ROWS : MX_ROWS;
   L.max_entries = (int)(std::min(E, m) + m / L.rows + 2);
   L.count = take(8);
   L.ent = take((size_t)L.max_entries * 16);
@@ -1404,14 +1474,16 @@ static MxSwigluLayout mx_swiglu_layout(int64_t m, int64_t k, int64_t n) {
 struct MxMoeLayout {
   size_t hdr, count, gather, scatter, ent, xc, xs, hc, hs, total;
   int rows, max_entries;
-  bool stream;
+  bool stream, small_up, small_down;
 };
 static MxMoeLayout mx_moe_layout(int64_t m, int64_t d, int top_k, int64_t n, int64_t E) {
   MxMoeLayout L = {};
   MxTake take;
   const int64_t S = m * top_k;
   L.stream = mx_stream_fits(m, d, true) && mx_stream_fits(m, n, false);
-  L.rows = L.stream ? (int)m : MX_ROWS;  // (a token may name an expert several times: more entries)
+  L.small_up = !L.stream && mx_small_round(S, E, (n + 63) / 64);
+  L.small_down = !L.stream && mx_small_round(S, E, (d + 127) / 128);
+  L.rows = L.stream ? (int)m : L.small_up || L.small_down ? MXS_ROWS : MX_ROWS;  // (a token may name an expert several times: more entries)
   L.max_entries = (int)std::min<int64_t>(S, std::min<int64_t>(E, S) + S / L.rows);
   L.hdr = take(16);
   L.count = take(4);
@@ -1500,7 +1572,7 @@ int amla_mxfp4_linear(const void *x, const void *x_scales, int64_t m, int64_t k,
 
 size_t amla_mxfp4_grouped_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t n_experts, int quantized) {
   if (!mx_sizes_ok(m, n, k) || n_experts <= 0 || n_experts > MX_MAX_GROUPS) return 0;
-  return mx_grouped_layout(m, k, n_experts, quantized != 0).total;
+  return mx_grouped_layout(m, k, n, n_experts, quantized != 0).total;
 }
 
 int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, int64_t k, int64_t ldx,
@@ -1519,7 +1591,7 @@ int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, in
     return fail(AMLA_EUNSUPPORTED,
                 "mxfp4_grouped_linear: needs k %% 128 == 0, at most %d experts, 16-byte aligned x rows and weight and "
                 "4-byte aligned scales (n=%lld k=%lld)", MX_MAX_GROUPS, (long long)n, (long long)k);
-  const MxGroupedLayout L = mx_grouped_layout(m, k, n_experts, x_scales != nullptr);
+  const MxGroupedLayout L = mx_grouped_layout(m, k, n, n_experts, x_scales != nullptr);
   if (!workspace || workspace_bytes < L.total || !aligned16(workspace))
     return fail(AMLA_EWORKSPACE, "mxfp4_grouped_linear: needs %zu bytes of 16-byte aligned workspace (got %zu)", L.total,
                 workspace ? workspace_bytes : (size_t)0);
@@ -1548,7 +1620,7 @@ int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, in
     p.x = ws + L.xc;
     p.xs = ws + L.xs;
   }
-  return launch_mx_sched<false>(p, L.max_entries, st);
+  return launch_mx_sched<false>(p, L.max_entries, L.small, st);
 }
 
 size_t amla_mxfp4_swiglu_workspace_bytes(int64_t m, int64_t k, int64_t n) {
@@ -1674,8 +1746,8 @@ int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh
     return rc;
   p.x = ws + L.xc;
   p.xs = ws + L.xs;
-  if ((rc = launch_mx_sched<true>(p, L.max_entries, st))) return rc;
-  return launch_mx_sched<false>(q, L.max_entries, st);
+  if ((rc = launch_mx_sched<true>(p, L.max_entries, L.small_up, st))) return rc;
+  return launch_mx_sched<false>(q, L.max_entries, L.small_down, st);
 }
 
 }  // extern "C"

@@ -209,7 +209,8 @@ def _offsets(sizes):
 
 
 GROUPS = [([1], 64, 128), ([0, 3, 0, 1], 100, 256), ([5, 0, 11], 257, 640), ([40, 0, 1, 130, 17], 300, 384),
-          ([128, 129, 0, 64, 33, 32], 512, 1664), ([0, 0, 0], 64, 128), ([2] * 70, 48, 256)]
+          ([128, 129, 0, 64, 33, 32], 512, 1664), ([0, 0, 0], 64, 128), ([2] * 70, 48, 256),
+          ([128, 129, 0, 64, 33, 32, 300], 8194, 384), ([97, 17, 257, 1, 0, 160], 8192, 512), ([64, 65, 0, 200], 1030, 1024)]
 
 
 @pytest.mark.parametrize("sizes,n,k", GROUPS)
@@ -275,7 +276,8 @@ def _ffn(g, d, n, E=None):
 
 
 @pytest.mark.parametrize("m,d,n", [(1, 128, 128), (3, 1152, 640), (16, 256, 384), (17, 512, 256), (70, 384, 128),
-                                   (150, 1024, 640), (8, 2048, 1536)])
+                                   (150, 1024, 640), (8, 2048, 1536), (300, 512, 4096),
+                                   (1000, 640, 8192), (1000, 512, 8192), (200, 1536, 512)])
 def test_swiglu(m, d, n):
     g = _gen(m * d)
     x, w = _x(g, m, d), _ffn(g, d, n)
@@ -286,7 +288,8 @@ def test_swiglu(m, d, n):
 
 
 @pytest.mark.parametrize("m,d,n,E,top_k", [(1, 128, 128, 4, 2), (5, 256, 384, 6, 3), (16, 1152, 640, 8, 2),
-                                           (17, 256, 128, 3, 3), (60, 512, 256, 8, 2), (300, 256, 128, 2, 2)])
+                                           (17, 256, 128, 3, 3), (60, 512, 256, 8, 2), (300, 256, 128, 2, 2),
+                                           (300, 4096, 2048, 4, 2), (90, 4224, 2176, 4, 4), (200, 640, 4096, 8, 3)])
 def test_moe_experts(m, d, n, E, top_k):
     g = _gen(m * E)
     x, w = _x(g, m, d), _ffn(g, d, n, E)
