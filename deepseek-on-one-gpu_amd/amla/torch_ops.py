@@ -251,6 +251,10 @@ def _on_device(fn, t: Tensor, *args):
         return fn(t, *args)
 
 
+def _mx_no_backward(ctx, *grads):
+    raise RuntimeError("the MXFP4 operators have no backward pass")
+
+
 def _mx_op(schema: str, fake):
     """Registers amla::<schema> with its ROCm implementation and its fake one."""
     def wrap(fn):
@@ -258,6 +262,8 @@ def _mx_op(schema: str, fake):
         _mx_lib.define(schema)
         _mx_lib.impl(name, lambda t, *args: _on_device(fn, t, *args), "CUDA")
         torch.library.register_fake(f"amla::{name}", fake, lib=_mx_lib)
+        if "!" not in schema:
+            torch.library.register_autograd(f"amla::{name}", _mx_no_backward, lib=_mx_lib)
         _mx_impl[name] = fn
         return fn
     return wrap
@@ -265,7 +271,8 @@ def _mx_op(schema: str, fake):
 
 def call(name: str, t: Tensor, *args):
     """The implementation of amla::<name>, or the operator itself where something traces the call."""
-    if type(t) is not Tensor and not isinstance(t, torch.nn.Parameter) or torch.compiler.is_compiling():
+    if t.requires_grad or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter) or \
+            torch.compiler.is_compiling():
         return getattr(torch.ops.amla, name)(t, *args)
     return _on_device(_mx_impl[name], t, *args)
 

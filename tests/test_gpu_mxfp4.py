@@ -464,6 +464,21 @@ def test_calls_on_two_streams_at_once():
         assert all(torch.equal(a, b) for res in got[i] for a, b in zip(res, want[i]))
 
 
+def test_no_backward_is_said_not_passed_over():
+    g = _gen(12)
+    w, ff = _weight(g, 64, 256), _ffn(g, 256, 128)
+    x = _x(g, 5, 256).to(DEV)
+    leaf = x.clone().requires_grad_()
+    for f in (lambda t: ops.mxfp4_linear(t, *w), lambda t: ops.dense_ffn(t, ff), lambda t: ops.mxfp4_linear(2 * t, *w)):
+        y = f(leaf)
+        with pytest.raises(RuntimeError, match="no backward"):
+            y.float().sum().backward()
+        with torch.no_grad():
+            assert torch.equal(f(leaf), y) and not f(leaf).requires_grad
+    assert torch.equal(ops.mxfp4_linear(leaf, *w), ops.mxfp4_linear(x, *w))
+    assert all(torch.equal(a, b) for a, b in zip(ops.mxfp4_quantize(leaf), ops.mxfp4_quantize(x)))
+
+
 def test_compiled_calls_equal_eager_ones():
     g = _gen(6)
     w = _weight(g, 256, 512)
