@@ -118,7 +118,7 @@ def test_dequantize_ends_of_the_range():
 
 LINEARS = [(1, 16, 128), (1, 1001, 1152), (2, 7168, 2048), (5, 130, 640), (16, 2112, 7168), (17, 576, 1536), (32, 256, 512),
            (33, 999, 768), (64, 1536, 7168), (65, 257, 384), (100, 1536, 7168), (128, 256, 256), (129, 512, 1664),
-           (300, 2050, 2048), (1000, 640, 1280)]
+           (300, 2050, 2048), (1000, 640, 1280), (5, 272, 32768), (16, 144, 13056), (2, 7, 12288)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEARS)
