@@ -15,8 +15,8 @@ namespace amla {
 constexpr int MX_MAX_GROUPS = 1024;  // experts of a grouped product
 
 // Operands of a launch.  Two weights (SILU): gate and up.  ent (with count): the
-// schedule entries (expert, first position, rows, -); null: one entry of M rows.  Position p reads x row xrow[p] and writes y row
-// yrow[p] (null: p).
+// schedule entries (expert, first position, rows, -); null: one entry of M rows.
+// Position p reads x row xrow[p] and writes y row yrow[p] (null: p).
 struct MxParams {
   const void *x;       // codes, or bf16 values (xs null; stream product only)
   const uint8_t *xs;
@@ -819,9 +819,9 @@ AMLA_DEV void mx_tile_store(const MxParams &p, V v, int j0, int wn, int rows, in
 
 // Few tiles: 128 weight rows (gate and up: 64 + 64) x up to 64 activation rows for sixteen
 // waves, wave w on weight rows 32 (w % 4) .. +31 (16 (w % 4) .. +15 of each) and K step
-// w / 4 of a stage of 512 K values; the four sums of an output meet in LDS.  Nothing but waits bounds such a call (a
-// barrier, the reads and eight multiplications one after the other in every wave), so
-// its stages are long and four waves of a SIMD stand in for each other: 777 x 2112 x
+// w / 4 of a stage of 512 K values; the four sums of an output meet in LDS.  Nothing but
+// waits bounds such a call (a barrier, the reads and eight multiplications one after the
+// other in every wave), so its stages are long and four waves of a SIMD stand in for each other: 777 x 2112 x
 // 7168 in 17.3 us, 21.8 with tiles of 256 x 32; eight waves with stages of 256 and five
 // of them on their way 19.1, which 24 workgroups alone take 0.44 us a stage for.
 //
