@@ -15,7 +15,8 @@ the op, its output shape and its in-place writes:
   inference/ops.py:140-141) and, when given, ``attn_out`` (the per-head output
   before o_proj).
 * ``amla::mxfp4_*``: the MXFP4 operators of amla.ops, which call their
-  implementations directly and the registered operators only under tracing
+  implementations directly, and the registered operators where something could
+  tell the difference: a tracer, a transform, a mode, a subclass, a gradient
   (the dispatch costs as much host time as the rest of a call).
 
 Tensors only, no dicts or dataclasses (the op schema cannot carry them): the
@@ -35,6 +36,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.overrides import has_torch_function
 
 from ._lib import MlaArgs, check, lib
 
@@ -245,7 +247,7 @@ _mx_impl: dict = {}
 
 
 def _on_device(fn, t: Tensor, *args):
-    if t.device.index == torch.cuda.current_device():
+    if t.device.index == torch._C._cuda_getDevice():
         return fn(t, *args)
     with torch.cuda.device(t.device):
         return fn(t, *args)
@@ -269,10 +271,20 @@ def _mx_op(schema: str, fake):
     return wrap
 
 
+# Bits of the thread's dispatch keys that are off while nothing watches torch's operators: tracers,
+# transforms (vmap, grad, jvp, functionalize), torch.jit.trace and dispatch modes set some of them.
+_WATCHED = ~torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect).add(
+    torch._C.DispatchKey.ADInplaceOrView).raw_repr()
+_thread_keys = torch._C._dispatch_tls_local_include_set
+_dynamo = torch.compiler.is_dynamo_compiling
+
+
 def call(name: str, t: Tensor, *args):
-    """The implementation of amla::<name>, or the operator itself where something traces the call."""
-    if t.requires_grad or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter) or \
-            torch.compiler.is_compiling():
+    """The implementation of amla::<name>, or the operator itself where the difference shows: something
+    traces, transforms or intercepts torch's operators, an argument is a tensor subclass, or a gradient
+    is asked for."""
+    if _dynamo() or _thread_keys().raw_repr() & _WATCHED or has_torch_function((t, *args)) or t.requires_grad or \
+            type(t) is not Tensor and not isinstance(t, torch.nn.Parameter):
         return getattr(torch.ops.amla, name)(t, *args)
     return _on_device(_mx_impl[name], t, *args)
 

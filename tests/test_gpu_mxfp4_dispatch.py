@@ -1,0 +1,97 @@
+"""The public MXFP4 functions on the GPU under tracers, transforms and dispatch modes."""
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from amla import ops
+from oracle import ref_mxfp4 as M
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _weight(g, *shape):
+    return tuple(t.to(DEV) for t in M.quantize(torch.randn(*shape, generator=g) * 0.05))
+
+
+def _calls():
+    """name: (function of x (m, 256), operator it has to show)."""
+    g = torch.Generator().manual_seed(1)
+    w, w3 = _weight(g, 96, 256), _weight(g, 3, 96, 256)
+    ff = {"gate_proj": _weight(g, 128, 256), "up_proj": _weight(g, 128, 256), "down_proj": _weight(g, 256, 128)}
+    ex = {"gate_proj": _weight(g, 3, 128, 256), "up_proj": _weight(g, 3, 128, 256), "down_proj": _weight(g, 3, 256, 128)}
+    off = torch.tensor([0, 2, 2, 5], dtype=torch.int32, device=DEV)
+    idx = torch.randint(0, 3, (5, 2), generator=g).to(DEV)
+    return {
+        "quantize": (lambda x: ops.mxfp4_quantize(x), "mxfp4_quantize"),
+        "round trip": (lambda x: ops.mxfp4_dequantize(*ops.mxfp4_quantize(x), F32), "mxfp4_dequantize"),
+        "linear": (lambda x: ops.mxfp4_linear(x, *w), "mxfp4_linear"),
+        "held": (lambda x: ops.mxfp4_linear(ops.mxfp4_quantize(x), *w, out_dtype=F32), "mxfp4_linear"),
+        "grouped": (lambda x: ops.mxfp4_grouped_linear(x, *w3, off), "mxfp4_grouped_linear"),
+        "dense_ffn": (lambda x: ops.dense_ffn(x, ff), "mxfp4_swiglu"),
+        "expert_ffn": (lambda x: ops.expert_ffn(x, ff), "mxfp4_swiglu"),
+        "experts": (lambda x: ops.mxfp4_moe_experts(x, idx, ex), "mxfp4_moe_experts"),
+    }
+
+
+def _x(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(BF16).to(DEV)
+
+
+def _equal(a, b):
+    if isinstance(a, (tuple, list)):
+        return len(a) == len(b) and all(_equal(u, v) for u, v in zip(a, b))
+    return a.dtype == b.dtype and torch.equal(a, b)
+
+
+NAMES = ["quantize", "round trip", "linear", "held", "grouped", "dense_ffn", "expert_ffn", "experts"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_traces_replay_on_new_inputs(name):
+    f, op = _calls()[name]
+    a, b = _x(1, 5, 256), _x(2, 5, 256)
+    want = f(b)
+    gm = make_fx(f)(a)
+    assert any(f"amla.{op}." in str(n.target) for n in gm.graph.nodes)
+    assert _equal(gm(b), want)
+    traced = torch.jit.trace(f, a, check_trace=False)
+    assert f"amla::{op}" in str(traced.graph)
+    assert _equal(traced(b), want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_modes_see_the_operator(name):
+    f, op = _calls()[name]
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    x = _x(3, 5, 256)
+    want = f(x)
+    with Mode():
+        got = f(x)
+    assert any(f"amla.{op}." in s for s in seen) and _equal(got, want)
+
+
+@pytest.mark.parametrize("name", [n for n in NAMES if n not in ("grouped", "experts")])
+def test_vmap_equals_the_calls_one_by_one(name):
+    f, _ = _calls()[name]
+    x = _x(4, 3, 5, 256)
+    got = torch.func.vmap(f)(x)
+    for i in range(3):
+        assert _equal(tuple(t[i] for t in got) if isinstance(got, tuple) else got[i], f(x[i]))
+
+
+def test_vmap_over_experts_of_a_stack():
+    g = torch.Generator().manual_seed(5)
+    c, s = _weight(g, 4, 96, 256)
+    x = _x(6, 5, 256)
+    got = torch.func.vmap(lambda a, b: ops.mxfp4_linear(x, a, b))(c, s)
+    for e in range(4):
+        assert torch.equal(got[e], ops.mxfp4_linear(x, c[e], s[e]))

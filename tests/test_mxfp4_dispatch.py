@@ -1,0 +1,215 @@
+"""The MXFP4 operators under what watches torch's operators: tracers, transforms, dispatch modes.
+
+On the CPU, with stand-ins for the kernels: a stand-in writes its output behind torch's back, as a
+kernel does, so that a trace which misses the operator replays uninitialised memory."""
+import ctypes
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.overrides import TorchFunctionMode
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from amla import torch_ops
+
+BF16, U8 = torch.bfloat16, torch.uint8
+
+
+def _write(out, value):
+    """The bytes of ``value`` into ``out`` by its address."""
+    value = value.to(out.dtype).contiguous()
+    if out.numel():
+        ctypes.memmove(out.data_ptr(), value.data_ptr(), out.numel() * out.element_size())
+    return out
+
+
+def _linear(x, x_scales, weight, scale, f32):
+    y = torch.empty(x.shape[0], weight.shape[0], dtype=torch.float32 if f32 else BF16)
+    return _write(y, x.float().sum(1, keepdim=True) + weight.float().sum(1))
+
+
+def _grouped(x, x_scales, weight, scale, offsets, f32):
+    y = torch.empty(x.shape[0], weight.shape[1], dtype=torch.float32 if f32 else BF16)
+    return _write(y, x.float().sum(1, keepdim=True) + weight.float().sum((0, 2)))
+
+
+def _grouped_out(x, x_scales, weight, scale, offsets, out):
+    _write(out, x.float().sum(1, keepdim=True) + weight.float().sum((0, 2)))
+
+
+def _swiglu(x, *w):
+    return _write(torch.empty(x.shape, dtype=BF16), x.float() * 3)
+
+
+def _moe(hidden, indices, *w):
+    y = torch.empty(hidden.shape[0], indices.shape[1], hidden.shape[1], dtype=BF16)
+    return _write(y, hidden.float()[:, None] + indices[..., None])
+
+
+def _pair(x, *_):
+    rows, k = x.shape
+    s = x.float().abs().sum(1, keepdim=True)
+    return (_write(torch.empty(rows, k // 2, dtype=U8), (s % 200).expand(rows, k // 2)),
+            _write(torch.empty(rows, k // 32, dtype=U8), (s % 100).expand(rows, k // 32)))
+
+
+def _dequantize(codes, scales, f32):
+    y = torch.empty(codes.shape[0], codes.shape[1] * 2, dtype=torch.float32 if f32 else BF16)
+    return _write(y, codes.float().repeat_interleave(2, 1))
+
+
+STAND_INS = {"mxfp4_quantize": _pair, "mxfp4_quantize_fp8": _pair, "mxfp4_dequantize": _dequantize,
+             "mxfp4_linear": _linear, "mxfp4_grouped_linear": _grouped, "mxfp4_grouped_linear_out": _grouped_out,
+             "mxfp4_swiglu": _swiglu, "mxfp4_moe_experts": _moe}
+
+
+@pytest.fixture(autouse=True)
+def stand_ins(monkeypatch):
+    lib = torch.library.Library("amla", "IMPL")
+    for name, fn in STAND_INS.items():
+        lib.impl(name, fn, "CPU")
+        monkeypatch.setitem(torch_ops._mx_impl, name, fn)
+    monkeypatch.setattr(torch_ops, "_on_device", lambda fn, t, *args: fn(t, *args))
+    yield
+    lib._destroy()
+
+
+def _u8(*shape):
+    return torch.randint(0, 200, shape, dtype=U8)
+
+
+def _x(m=4, k=128):
+    return torch.randint(-8, 9, (m, k)).to(BF16)
+
+
+# name: (the call as a function of its first tensor, that tensor)
+def _calls():
+    w, s = _u8(6, 64), _u8(6, 4)
+    w3, s3 = _u8(2, 6, 64), _u8(2, 6, 4)
+    ff = [_u8(128, 64), _u8(128, 4)] * 3
+    off = torch.tensor([0, 1, 4], dtype=torch.int32)
+    idx = torch.randint(0, 2, (4, 2))
+    c = torch_ops.call
+    return {
+        "mxfp4_quantize": (lambda t: c("mxfp4_quantize", t), _x),
+        "mxfp4_quantize_fp8": (lambda t: c("mxfp4_quantize_fp8", t, torch.ones(1, 1)), lambda: _x().to(torch.float8_e4m3fn)),
+        "mxfp4_dequantize": (lambda t: c("mxfp4_dequantize", t, s, False), lambda: _u8(6, 64)),
+        "mxfp4_linear": (lambda t: c("mxfp4_linear", t, None, w, s, True), _x),
+        "mxfp4_grouped_linear": (lambda t: c("mxfp4_grouped_linear", t, None, w3, s3, off, False), _x),
+        "mxfp4_swiglu": (lambda t: c("mxfp4_swiglu", t, *ff), _x),
+        "mxfp4_moe_experts": (lambda t: c("mxfp4_moe_experts", t, idx, w3, s3, w3, s3, w3, s3), _x),
+    }
+
+
+NAMES = sorted(set(STAND_INS) - {"mxfp4_grouped_linear_out"})
+
+
+def _equal(a, b):
+    if isinstance(a, (tuple, list)):
+        return len(a) == len(b) and all(_equal(u, v) for u, v in zip(a, b))
+    return a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("how", ["real", "fake", "symbolic", "pre_dispatch"])
+@pytest.mark.parametrize("name", NAMES)
+def test_make_fx_records_the_operator(name, how):
+    f, make = _calls()[name]
+    kw = {"pre_dispatch": True} if how == "pre_dispatch" else {"tracing_mode": how, "_allow_non_fake_inputs": True}
+    gm = make_fx(f, **kw)(make())
+    targets = [str(n.target) for n in gm.graph.nodes if n.op == "call_function"]
+    assert f"amla.{name}.default" in targets and not any("empty" in t for t in targets)
+    fresh = make()
+    assert _equal(gm(fresh), f(fresh))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_jit_trace_records_the_operator(name):
+    f, make = _calls()[name]
+    traced = torch.jit.trace(f, make(), check_trace=False)
+    assert f"amla::{name}" in str(traced.graph)
+    fresh = make()
+    assert _equal(traced(fresh), f(fresh))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_dispatch_and_function_modes_see_the_operator(name):
+    f, make = _calls()[name]
+    seen = []
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    t = make()
+    want = f(t)
+    for mode in (Dispatch, Function):
+        seen.clear()
+        with mode():
+            got = f(t)
+        assert any(f"amla.{name}" in s for s in seen), (mode, seen)
+        assert _equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["mxfp4_linear", "mxfp4_swiglu", "mxfp4_quantize"])
+def test_vmap_runs_the_operator_by_item(name):
+    f, make = _calls()[name]
+    t = torch.stack([make() for _ in range(3)])
+    got = torch.func.vmap(f)(t)
+    assert _equal(got, torch.func.vmap(f)(t))
+    for i in range(3):
+        item = tuple(g[i] for g in got) if isinstance(got, tuple) else got[i]
+        assert _equal(item, f(t[i]))
+
+
+def test_vmap_over_the_weights():
+    x, w, s = _x(), _u8(3, 6, 64), _u8(3, 6, 4)
+    got = torch.func.vmap(lambda a, b: torch_ops.call("mxfp4_linear", x, None, a, b, True))(w, s)
+    assert _equal(got, torch.stack([_linear(x, None, w[i], s[i], True) for i in range(3)]))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_compiled_calls_hold_the_operator(name):
+    f, make = _calls()[name]
+    graphs = []
+
+    def backend(gm, inputs):
+        graphs.append(str(gm.graph))
+        return gm.forward
+
+    torch._dynamo.reset()
+    t = make()
+    assert _equal(torch.compile(f, fullgraph=True, backend=backend)(t), f(t))
+    assert len(graphs) == 1 and f"amla.{name}" in graphs[0]
+
+
+def test_a_subclass_behind_the_first_argument_is_seen():
+    seen = []
+
+    class Marked(torch.Tensor):
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return super().__torch_function__(func, types, args, kwargs or {})
+
+    w = _u8(6, 64).as_subclass(Marked)
+    torch_ops.call("mxfp4_linear", _x(), None, w, _u8(6, 4), True)
+    assert any("amla.mxfp4_linear" in s for s in seen)
+
+
+def test_eager_calls_do_not_pass_the_dispatcher(monkeypatch):
+    """The ordinary call (with and without grad mode, in inference mode) runs its implementation."""
+    f, make = _calls()["mxfp4_linear"]
+    t = make()
+    ran = []
+    monkeypatch.setattr(torch_ops, "_on_device", lambda fn, t, *args: ran.append(1) or fn(t, *args))
+    for ctx in (torch.enable_grad, torch.no_grad, torch.inference_mode):
+        with ctx():
+            f(t)
+    f(torch.nn.Parameter(t, requires_grad=False))
+    assert len(ran) == 4
