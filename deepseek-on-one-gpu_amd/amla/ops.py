@@ -742,7 +742,8 @@ def mxfp4_grouped_linear(x, weight: torch.Tensor, scale: torch.Tensor, offsets: 
     ``offsets`` (E + 1,) int32 on the device, ascending; groups may be empty.  They are not checked
     on the host: one above m counts as m, one below its predecessor as that.  Rows of no group are
     zeros in a new output; with ``out`` ((m, n), bf16 or fp32 as out_dtype says, unit column
-    stride) they stay as they were.  ``x``: as for ``mxfp4_linear``."""
+    stride) they stay as they were.  ``x``: as for ``mxfp4_linear``.  With ``out``, an x or out that
+    requires a gradient is refused while grad mode is on."""
     wdt = _mx_out_dtype(out_dtype, "mxfp4_grouped_linear")
     shape = _mx_pair(weight, scale, "weight")
     if len(shape) != 3:

@@ -403,7 +403,23 @@ def _mxfp4_grouped_linear(x, x_scales, weight, scale, offsets, f32):
 @_mx_op("mxfp4_grouped_linear_out(Tensor x, Tensor? x_scales, Tensor weight, Tensor scale, Tensor offsets, "
         "Tensor(a!) out) -> ()", lambda x, x_scales, weight, scale, offsets, out: None)
 def _mxfp4_grouped_linear_out(x, x_scales, weight, scale, offsets, out):
+    _mx_out_gradient(x, out)
     _mx_grouped(x, x_scales, weight, scale, offsets, out, 0)
+    torch.autograd.graph.increment_version(out)
+
+
+def _mx_out_gradient(x, out) -> None:
+    if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+        raise RuntimeError("mxfp4_grouped_linear: out= has no gradient, but x or out requires one")
+
+
+def _mxfp4_grouped_linear_out_autograd(x, x_scales, weight, scale, offsets, out):
+    _mx_out_gradient(x, out)
+    with torch._C._AutoDispatchBelowAutograd():
+        torch.ops.amla.mxfp4_grouped_linear_out(x, x_scales, weight, scale, offsets, out)
+
+
+_mx_lib.impl("mxfp4_grouped_linear_out", _mxfp4_grouped_linear_out_autograd, "Autograd")
 
 
 @_mx_op("mxfp4_swiglu(Tensor x, Tensor gate_proj, Tensor gate_scale, Tensor up_proj, Tensor up_scale, "

@@ -95,3 +95,26 @@ def test_vmap_over_experts_of_a_stack():
     got = torch.func.vmap(lambda a, b: ops.mxfp4_linear(x, a, b))(c, s)
     for e in range(4):
         assert torch.equal(got[e], ops.mxfp4_linear(x, c[e], s[e]))
+
+
+# ------------------------------------------------------------------ gradients
+
+def test_grouped_out_refuses_gradients_and_counts_as_written():
+    g = torch.Generator().manual_seed(7)
+    w = _weight(g, 3, 96, 256)
+    off = torch.tensor([0, 2, 2, 5], dtype=torch.int32, device=DEV)
+    leaf = _x(8, 5, 256).requires_grad_()
+    out = torch.ones(5, 96, dtype=BF16, device=DEV)
+    for x in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError, match="out= .* gradient"):
+            ops.mxfp4_grouped_linear(x, *w, off, out=out)
+    with pytest.raises(RuntimeError, match="out= .* gradient"):
+        ops.mxfp4_grouped_linear(leaf.detach(), *w, off, out=out.clone().requires_grad_())
+    assert (out == 1).all()
+    saved = torch.ones(5, 96, dtype=BF16, device=DEV, requires_grad=True)
+    y = (saved * out).sum()
+    with torch.no_grad():
+        ops.mxfp4_grouped_linear(leaf, *w, off, out=out)
+    assert torch.equal(out, ops.mxfp4_grouped_linear(leaf.detach(), *w, off))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

@@ -213,3 +213,73 @@ def test_eager_calls_do_not_pass_the_dispatcher(monkeypatch):
             f(t)
     f(torch.nn.Parameter(t, requires_grad=False))
     assert len(ran) == 4
+
+
+# ------------------------------------------------------------------ gradients
+
+def _out_call(x, out):
+    w, s = _u8(2, 6, 64), _u8(2, 6, 4)
+    torch_ops.call("mxfp4_grouped_linear_out", x, None, w, s, torch.tensor([0, 1, 4], dtype=torch.int32), out)
+    return out
+
+
+@pytest.fixture
+def real_out(monkeypatch):
+    """The package's own implementation of the operator with an ``out``, but for its launch."""
+    monkeypatch.undo()
+    monkeypatch.setattr(torch_ops, "_on_device", lambda fn, t, *args: fn(t, *args))
+    monkeypatch.setattr(torch_ops, "_mx_grouped", lambda x, xs, w, s, off, y, clear: _grouped_out(x, xs, w, s, off, y))
+
+
+def test_out_has_no_gradient_to_give(real_out):
+    """Like torch's own out= variants: an error while a gradient is asked for, not a lost term."""
+    leaf = _x().requires_grad_()
+    out = torch.zeros(4, 6, dtype=BF16)
+    for x in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError, match="out= .* gradient"):
+            _out_call(x, out)
+    with pytest.raises(RuntimeError, match="out= .* gradient"):
+        _out_call(_x(), torch.zeros(4, 6, dtype=BF16, requires_grad=True))
+    assert not out.any()
+    with pytest.raises(RuntimeError, match="out= .* gradient"):
+        torch.ops.amla.mxfp4_grouped_linear_out(leaf, None, _u8(2, 6, 64), _u8(2, 6, 4),
+                                                torch.tensor([0, 1, 4], dtype=torch.int32), out)
+    with torch.no_grad():
+        assert _out_call(leaf, out).any()
+    with torch.inference_mode():
+        assert _out_call(leaf, torch.zeros(4, 6, dtype=BF16)).any()
+
+
+@pytest.mark.parametrize("through", ["call", "operator"])
+def test_out_counts_as_written(real_out, through):
+    """Autograd sees that a tensor it saved was overwritten."""
+    out = torch.ones(4, 6, dtype=BF16)
+    a = torch.ones(4, 6, dtype=BF16, requires_grad=True)
+    y = (a * out).sum()
+    before = out._version
+    if through == "call":
+        _out_call(_x(), out)
+    else:
+        lib = torch.library.Library("amla", "IMPL")
+        try:
+            lib.impl("mxfp4_grouped_linear_out", torch_ops._mx_impl["mxfp4_grouped_linear_out"], "CPU", allow_override=True)
+            torch.ops.amla.mxfp4_grouped_linear_out(_x(), None, _u8(2, 6, 64), _u8(2, 6, 4),
+                                                    torch.tensor([0, 1, 4], dtype=torch.int32), out)
+        finally:
+            lib._destroy()
+    assert out._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_compiled_out():
+    def f(x, out):
+        w = torch.ones(2, 6, 64, dtype=U8)
+        torch_ops.call("mxfp4_grouped_linear_out", x, None, w, w[:, :, :4], torch.tensor([0, 1, 4], dtype=torch.int32), out)
+        return out + 1
+
+    x = _x()
+    a, b = torch.zeros(4, 6, dtype=BF16), torch.zeros(4, 6, dtype=BF16)
+    torch._dynamo.reset()
+    got = torch.compile(f, fullgraph=True, backend="aot_eager")(x, a)
+    assert _equal(got, f(x, b)) and _equal(a, b) and a.any()
