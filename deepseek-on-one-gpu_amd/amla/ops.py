@@ -482,7 +482,8 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
         if experts["gate_proj"][0].shape[0] != E:
             raise ValueError(f"moe_block: {experts['gate_proj'][0].shape[0]} stacked experts, config says {E}")
         eout = mxfp4_moe_experts(h2, idx.reshape(m, top_k), experts)
-        return _moe_combine(shared_out, eout, w, m, top_k, d, config, out, hidden)
+        return torch_ops.without_backward(
+            lambda: _moe_combine(shared_out, eout, w, m, top_k, d, config, out, hidden), hidden, gate_weight, w, shared_out)
     if stacked and device_grouping and E <= MOE_DEV_MAX_EXPERTS:
         table, n_inter = _stacked_device_table(experts, E, d, dev)
         eout = torch.empty(m, top_k, d, dtype=BF16, device=dev)
@@ -672,7 +673,8 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
     The exponent of a block is floor(log2(max |x|)) - 2 (a block of zeros: byte 0); values are
     rounded to nearest even and saturate at 6 times the scale.  A block that holds an infinity or
-    a NaN is a block of NaN (byte 255)."""
+    a NaN is a block of NaN (byte 255).  Codes and exponents are whole numbers: no gradient passes
+    through a pair, while a backward through a product of the values themselves raises."""
     _need_cuda(x, "x")
     if x.dtype not in _MX_IN:
         raise TypeError(f"mxfp4_quantize: x must be bfloat16, float16 or float32 (got {x.dtype})")

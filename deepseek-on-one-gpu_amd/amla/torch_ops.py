@@ -257,6 +257,23 @@ def _mx_no_backward(ctx, *grads):
     raise RuntimeError("the MXFP4 operators have no backward pass")
 
 
+class _NoBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, fn, *sources):
+        return fn()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _mx_no_backward(ctx, *grads)
+
+
+def without_backward(fn, *sources: Tensor) -> Tensor:
+    """``fn()``, a tensor made of ``sources`` behind autograd's back: a backward through it raises."""
+    if torch.is_grad_enabled() and any(s.requires_grad for s in sources):
+        return _NoBackward.apply(fn, *sources)
+    return fn()
+
+
 def _mx_op(schema: str, fake):
     """Registers amla::<schema> with its ROCm implementation and its fake one."""
     def wrap(fn):

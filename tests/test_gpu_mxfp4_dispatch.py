@@ -5,6 +5,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from amla import ops
+from amla.config import DeepSeekConfig
 from oracle import ref_mxfp4 as M
 
 pytestmark = pytest.mark.gpu
@@ -118,3 +119,23 @@ def test_grouped_out_refuses_gradients_and_counts_as_written():
     assert torch.equal(out, ops.mxfp4_grouped_linear(leaf.detach(), *w, off))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_moe_block_backward_raises_beside_a_residual():
+    g = torch.Generator().manual_seed(9)
+    cfg = DeepSeekConfig(hidden_size=512, n_routed_experts=16, num_experts_per_tok=4, n_group=4, topk_group=2,
+                         moe_intermediate_size=256)
+    experts = {"gate_proj": _weight(g, 16, 256, 512), "up_proj": _weight(g, 16, 256, 512),
+               "down_proj": _weight(g, 16, 512, 256)}
+    shared = {"gate_proj": _weight(g, 256, 512), "up_proj": _weight(g, 256, 512), "down_proj": _weight(g, 512, 256)}
+    h, gate = _x(10, 1, 6, 512), _x(11, 16, 512)
+    want = ops.moe_block(h, gate, shared, experts, cfg)
+    idx, wt = ops.route(h, gate, cfg)
+    for hidden, gt, routing in ((h.clone().requires_grad_(), gate, None), (h, gate.clone().requires_grad_(), None),
+                                (h, gate, (idx, wt.clone().requires_grad_()))):
+        y = ops.moe_block(hidden, gt, shared, experts, cfg, routing=routing)
+        assert torch.equal(y, want)
+        with pytest.raises(RuntimeError, match="no backward"):
+            (torch.zeros_like(h, requires_grad=True) + y).float().sum().backward()
+        with torch.no_grad():
+            assert not ops.moe_block(hidden, gt, shared, experts, cfg, routing=routing).requires_grad

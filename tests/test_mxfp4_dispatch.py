@@ -10,7 +10,8 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.overrides import TorchFunctionMode
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from amla import torch_ops
+from amla import ops, torch_ops
+from amla.config import DeepSeekConfig
 
 BF16, U8 = torch.bfloat16, torch.uint8
 
@@ -283,3 +284,48 @@ def test_compiled_out():
     torch._dynamo.reset()
     got = torch.compile(f, fullgraph=True, backend="aot_eager")(x, a)
     assert _equal(got, f(x, b)) and _equal(a, b) and a.any()
+
+
+def _moe_parts(monkeypatch):
+    """moe_block's parts but for the launches."""
+    monkeypatch.setattr(ops, "route", lambda h, gate, cfg: (torch.zeros(*h.shape[:-1], 2, dtype=torch.int64),
+                                                            torch.ones(*h.shape[:-1], 2)))
+    monkeypatch.setattr(ops, "expert_ffn", lambda h, w: _write(torch.empty(h.shape, dtype=BF16), h * 2))
+    monkeypatch.setattr(ops, "mxfp4_moe_experts", lambda h, i, w: _write(torch.empty(*i.shape, h.shape[-1], dtype=BF16), h[:, None].expand(*i.shape, -1)))
+
+    def combine(shared, eout, w, m, top_k, d, config, out, hidden):
+        return _write(out, (shared.reshape(m, d) + eout.sum(1)).view(out.shape))
+
+    monkeypatch.setattr(ops, "_moe_combine", combine)
+    cfg = DeepSeekConfig(hidden_size=128, n_routed_experts=2, num_experts_per_tok=2, n_group=1, topk_group=1,
+                         moe_intermediate_size=128)
+    w = _u8(2, 128, 64)
+    return cfg, {"gate_proj": (w, w), "up_proj": (w, w), "down_proj": (w, w)}
+
+
+def test_moe_block_on_mxfp4_experts_has_no_backward(monkeypatch):
+    """With a residual beside it, a lost gradient would pass unseen."""
+    cfg, experts = _moe_parts(monkeypatch)
+    h, gate = _x(), _x(2)
+    want = ops.moe_block(h, gate, {}, experts, cfg)
+    assert not want.requires_grad
+    weights = torch.ones(4, 2, requires_grad=True)
+    idx = torch.zeros(4, 2, dtype=torch.int64)
+    for hidden, gt, routing in ((h.clone().requires_grad_(), gate, None), (h, gate.clone().requires_grad_(), None),
+                                (h, gate, (idx, weights))):
+        residual = torch.zeros_like(h, requires_grad=True)
+        y = ops.moe_block(hidden, gt, {}, experts, cfg, routing=routing)
+        assert torch.equal(y, want)
+        y += 0  # (an ordinary tensor: in-place residuals work)
+        with pytest.raises(RuntimeError, match="no backward"):
+            (residual + y).float().sum().backward()
+        with torch.no_grad():
+            assert not ops.moe_block(hidden, gt, {}, experts, cfg, routing=routing).requires_grad
+
+
+def test_a_quantised_pair_carries_no_gradient():
+    """Its tensors are whole numbers, as after torch's own casts to them."""
+    leaf = _x().requires_grad_()
+    pair = torch_ops.call("mxfp4_quantize", leaf)
+    assert not any(t.requires_grad for t in pair)
+    assert not torch_ops.call("mxfp4_linear", *pair, _u8(6, 64), _u8(6, 4), True).requires_grad
