@@ -36,6 +36,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.overrides import has_torch_function
 
 from ._lib import MlaArgs, check, lib
@@ -298,12 +299,22 @@ _dynamo = torch.compiler.is_dynamo_compiling
 
 def call(name: str, t: Tensor, *args):
     """The implementation of amla::<name>, or the operator itself where the difference shows: something
-    traces, transforms or intercepts torch's operators, an argument is a tensor subclass, or a gradient
+    traces, transforms or intercepts torch's operators, an argument is a tensor subclass, or a derivative
     is asked for."""
     if _dynamo() or _thread_keys().raw_repr() & _WATCHED or has_torch_function((t, *args)) or t.requires_grad or \
-            type(t) is not Tensor and not isinstance(t, torch.nn.Parameter):
+            forward_ad._current_level >= 0 or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter):
+        if name not in _MX_WHOLE:
+            _no_tangent(t)
         return getattr(torch.ops.amla, name)(t, *args)
     return _on_device(_mx_impl[name], t, *args)
+
+
+_MX_WHOLE = ("mxfp4_quantize", "mxfp4_quantize_fp8")  # outputs are whole numbers: no derivative passes through
+
+
+def _no_tangent(t: Tensor) -> None:
+    if not _dynamo() and forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError("the MXFP4 operators have no derivative in forward mode")
 
 
 # (the workspaces' sizes are functions of the call's sizes alone)

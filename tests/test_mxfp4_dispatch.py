@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.overrides import TorchFunctionMode
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -329,3 +330,19 @@ def test_a_quantised_pair_carries_no_gradient():
     pair = torch_ops.call("mxfp4_quantize", leaf)
     assert not any(t.requires_grad for t in pair)
     assert not torch_ops.call("mxfp4_linear", *pair, _u8(6, 64), _u8(6, 4), True).requires_grad
+
+
+@pytest.mark.parametrize("name", ["mxfp4_linear", "mxfp4_grouped_linear", "mxfp4_swiglu", "mxfp4_moe_experts"])
+def test_forward_mode_is_refused_not_passed_over(name):
+    f, make = _calls()[name]
+    x, t = make(), make()
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.func.jvp(f, (x,), (t,))
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no derivative"):
+            f(forward_ad.make_dual(x, t))
+        assert _equal(f(x), f(x.clone()))  # a plain tensor beside dual ones
+    out = torch.zeros(4, 6, dtype=BF16)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no derivative"):
+            _out_call(forward_ad.make_dual(_x(), _x()), out)
