@@ -1215,11 +1215,13 @@ __global__ __launch_bounds__(256) void mx_clear_skipped_kernel(const int64_t *__
 
 constexpr int64_t MX_MAX_BLOCKS = (1 << 22) - 8;  // of 1024 threads, fewer than 2^32 a launch
 
+// Dynamic LDS above 64 KB.  The limit is the process's: it is always the CU's, so that no call
+// lowers it between another thread's setting and launch.
 template <typename F>
-static int mx_lds(F *fn, int bytes) {  // dynamic LDS above 64 KB
+static int mx_lds(F *fn, int bytes) {
   if (bytes <= 64 * 1024) return AMLA_OK;
   const hipError_t e =
-      hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   return e == hipSuccess ? AMLA_OK : fail((int)e, "mxfp4 product: LDS size: %s", hipGetErrorString(e));
 }
 

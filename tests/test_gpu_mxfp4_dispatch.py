@@ -1,4 +1,6 @@
 """The public MXFP4 functions on the GPU under tracers, transforms and dispatch modes."""
+import threading
+
 import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
@@ -139,3 +141,27 @@ def test_moe_block_backward_raises_beside_a_residual():
             (torch.zeros_like(h, requires_grad=True) + y).float().sum().backward()
         with torch.no_grad():
             assert not ops.moe_block(hidden, gt, shared, experts, cfg, routing=routing).requires_grad
+
+
+def test_calls_of_two_host_threads():
+    """Calls of different LDS sizes of one kernel from two threads: each gives what it gives alone."""
+    g = torch.Generator().manual_seed(12)
+    parts = [(_x(13, 8, 16384), _weight(g, 512, 16384)), (_x(14, 8, 12288), _weight(g, 512, 12288))]
+    want = [ops.mxfp4_linear(x, *w) for x, w in parts]
+    torch.cuda.synchronize()
+    results = [[], []]
+
+    def work(i):
+        x, w = parts[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(40):
+                results[i].append(ops.mxfp4_linear(x, *w))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for i in range(2):
+        assert len(results[i]) == 40 and all(torch.equal(y, want[i]) for y in results[i])
