@@ -1341,10 +1341,15 @@ static size_t mx_split_bytes(const MxSplit &sp) {
   return sp.parts > 1 ? ((size_t)sp.n_tiles * sp.m_tiles - sp.whole) * sp.parts * 1024 * sp.rows : 0;
 }
 
+static int64_t mx_linear_blocks(const MxSplit &sp) {
+  return sp.whole + (((int64_t)sp.n_tiles * sp.m_tiles - sp.whole) * sp.parts + 7) / 8 * 8;
+}
+// (checked by the entries before the first launch)
+static bool mx_linear_grid_ok(const MxSplit &sp) { return sp.rows && mx_linear_blocks(sp) <= MX_MAX_BLOCKS; }
+
 template <bool SILU>
 static int launch_mx_linear(const MxParams &p, const MxSplit &sp, hipStream_t st) {
-  const int64_t split = (int64_t)sp.n_tiles * sp.m_tiles - sp.whole, blocks = sp.whole + (split * sp.parts + 7) / 8 * 8;
-  if (!sp.rows || blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d x %d outputs", p.M, p.N);
+  const int64_t split = (int64_t)sp.n_tiles * sp.m_tiles - sp.whole, blocks = mx_linear_blocks(sp);
   const auto kernel = p.K % 512 ? mx_linear_kernel<SILU, true> : mx_linear_kernel<SILU, false>;
   int rc;
   if (sp.small) {
@@ -1371,11 +1376,19 @@ static bool mx_small_round(int64_t slots, int64_t E, int64_t tiles) {
   return groups * ((each + MXS_ROWS - 1) / MXS_ROWS) * tiles <= 256;
 }
 
+static int mx_sched_tiles(int64_t n, bool silu, bool small) {  // of an entry
+  const int cols = (silu ? 128 : 256) / (small ? 2 : 1);
+  return (int)((n + cols - 1) / cols);
+}
+static int64_t mx_sched_blocks(int max_entries, int ntiles) { return ((int64_t)max_entries * ntiles + 7) / 8 * 8; }
+static bool mx_sched_grid_ok(int max_entries, int64_t n, bool silu, bool small) {
+  return mx_sched_blocks(max_entries, mx_sched_tiles(n, silu, small)) <= MX_MAX_BLOCKS;
+}
+
 template <bool SILU>
 static int launch_mx_sched(const MxParams &p, int max_entries, bool small, hipStream_t st) {
-  const int cols = (SILU ? 128 : 256) / (small ? 2 : 1), ntiles = (p.N + cols - 1) / cols;
-  const int64_t blocks = ((int64_t)max_entries * ntiles + 7) / 8 * 8;
-  if (blocks > MX_MAX_BLOCKS) return fail(AMLA_EUNSUPPORTED, "mxfp4 product: %d entries", max_entries);
+  const int ntiles = mx_sched_tiles(p.N, SILU, small);
+  const int64_t blocks = mx_sched_blocks(max_entries, ntiles);
   int rc;
   if (small) {
     const auto kernel = p.K % 512 ? mx_small_sched_kernel<SILU, true> : mx_small_sched_kernel<SILU, false>;
@@ -1547,6 +1560,8 @@ int amla_mxfp4_linear(const void *x, const void *x_scales, int64_t m, int64_t k,
                 "mxfp4_linear: needs k %% 128 == 0, 16-byte aligned x rows and weight and 4-byte aligned scales "
                 "(n=%lld k=%lld)", (long long)n, (long long)k);
   const MxLinearLayout L = mx_linear_layout(m, k, n, x_scales != nullptr);
+  if (!L.stream && !mx_linear_grid_ok(L.sp))
+    return fail(AMLA_EUNSUPPORTED, "mxfp4_linear: %lld x %lld outputs", (long long)m, (long long)n);
   if (L.total && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
     return fail(AMLA_EWORKSPACE, "mxfp4_linear: needs %zu bytes of 16-byte aligned workspace (got %zu)", L.total,
                 workspace ? workspace_bytes : (size_t)0);
@@ -1594,6 +1609,8 @@ int amla_mxfp4_grouped_linear(const void *x, const void *x_scales, int64_t m, in
                 "mxfp4_grouped_linear: needs k %% 128 == 0, at most %d experts, 16-byte aligned x rows and weight and "
                 "4-byte aligned scales (n=%lld k=%lld)", MX_MAX_GROUPS, (long long)n, (long long)k);
   const MxGroupedLayout L = mx_grouped_layout(m, k, n, n_experts, x_scales != nullptr);
+  if (!L.stream && !mx_sched_grid_ok(L.max_entries, n, false, L.small))
+    return fail(AMLA_EUNSUPPORTED, "mxfp4_grouped_linear: %lld x %lld outputs", (long long)m, (long long)n);
   if (!workspace || workspace_bytes < L.total || !aligned16(workspace))
     return fail(AMLA_EWORKSPACE, "mxfp4_grouped_linear: needs %zu bytes of 16-byte aligned workspace (got %zu)", L.total,
                 workspace ? workspace_bytes : (size_t)0);
@@ -1647,6 +1664,8 @@ int amla_mxfp4_swiglu(const void *x, int64_t m, int64_t k, int64_t ldx, const vo
                 "mxfp4_swiglu: needs k %% 128 == 0, n %% 128 == 0, 16-byte aligned rows and weights and 4-byte aligned "
                 "scales (n=%lld k=%lld)", (long long)n, (long long)k);
   const MxSwigluLayout L = mx_swiglu_layout(m, k, n);
+  if ((!L.stream && !mx_linear_grid_ok(L.sp)) || (!L.down.stream && !mx_linear_grid_ok(L.down.sp)))
+    return fail(AMLA_EUNSUPPORTED, "mxfp4_swiglu: %lld x %lld outputs", (long long)m, (long long)std::max(n, k));
   if (!workspace || workspace_bytes < L.total || !aligned16(workspace))
     return fail(AMLA_EWORKSPACE, "mxfp4_swiglu: needs %zu bytes of 16-byte aligned workspace (got %zu)", L.total,
                 workspace ? workspace_bytes : (size_t)0);
@@ -1701,6 +1720,10 @@ int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh
                 "mxfp4_moe_experts: needs top_k <= 64, at most 512 experts, 65536 slots and 4 GB of codes per call, "
                 "hidden and intermediate sizes %% 128 == 0, 16-byte aligned rows and weights and 4-byte aligned scales");
   const MxMoeLayout L = mx_moe_layout(m, d, top_k, n_inter, n_experts);
+  if (!L.stream && !(mx_sched_grid_ok(L.max_entries, n_inter, true, L.small_up) &&
+                     mx_sched_grid_ok(L.max_entries, d, false, L.small_down)))
+    return fail(AMLA_EUNSUPPORTED, "mxfp4_moe_experts: %lld tokens of hidden size %lld and intermediate size %lld",
+                (long long)m, (long long)d, (long long)n_inter);
   if (!workspace || workspace_bytes < L.total || !aligned16(workspace))
     return fail(AMLA_EWORKSPACE, "mxfp4_moe_experts: needs %zu bytes of 16-byte aligned workspace (got %zu)", L.total,
                 workspace ? workspace_bytes : (size_t)0);

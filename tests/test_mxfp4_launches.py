@@ -40,3 +40,23 @@ def test_lds_limits_are_never_lowered(tmp_path):
                 launches += 1
                 assert rest[2] <= limit.get(f, 64 * 1024) and rest[2] <= 160 * 1024
     assert launches >= len(calls) and len(limit) >= 6
+
+
+def test_outputs_beyond_a_grid_are_refused_before_anything_runs(tmp_path):
+    """Neither x is quantised nor a schedule made for a call that is refused."""
+    n = 2 ** 29 - 1
+    calls = [_linear(600, 128, n), _linear(2 ** 31 - 1, 128, 128), _linear(600, 128, n, held=True), _grouped(33, 128, n, 2),
+             _grouped(40, 256, n, 1, held=True), _swiglu(2 ** 31 - 1, 128, 128), _moe(4000, 128, 16, 2 ** 24, 512),
+             _moe(300, 2 ** 24, 1, 128, 512)]
+    for (name, args), (rc, log) in zip(calls, hip_calls(tmp_path, calls)):
+        assert rc == -3 and not log, (name, args, rc, log)
+
+
+def test_largest_grids_hold_fewer_than_2_to_32_threads(tmp_path):
+    calls = [_linear(40, 128, 2 ** 29 - 400), _linear(2 ** 30, 128, 100), _grouped(256, 128, 2 ** 27, 2),
+             _swiglu(2 ** 27, 128, 128), _moe(65536, 128, 1, 2 ** 18, 512)]
+    for (name, args), (rc, log) in zip(calls, hip_calls(tmp_path, calls)):
+        assert rc in (0, -3) and (rc == 0) == bool(log), (name, args, rc, log)
+        for what, f, *rest in log:
+            if what == "launch":
+                assert 0 < rest[0] * rest[1] < 2 ** 32, (name, args, rest)
