@@ -381,7 +381,7 @@ def _mxfp4_dequantize(codes, scales, f32):
     rows, k = codes.shape[0], codes.shape[1] * 2
     out = torch.empty(rows, k, dtype=torch.float32 if f32 else BF16, device=codes.device)
     check(lib().amla_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, _MX_CODES[out.dtype],
-                                      out.data_ptr(), _mx_stream(codes)) if rows else 0, "mxfp4_dequantize")
+                                      out.data_ptr(), _mx_stream(codes)) if out.numel() else 0, "mxfp4_dequantize")
     return out
 
 

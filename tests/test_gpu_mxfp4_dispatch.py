@@ -165,3 +165,12 @@ def test_calls_of_two_host_threads():
         t.join(60)
     for i in range(2):
         assert len(results[i]) == 40 and all(torch.equal(y, want[i]) for y in results[i])
+
+
+@pytest.mark.parametrize("lead", [(5,), (2, 3), (0,)])
+def test_dequantise_of_empty_pairs(lead):
+    for k in (0, 64) if 0 in lead else (0,):
+        c = torch.empty(*lead, k // 2, dtype=torch.uint8, device=DEV)
+        s = torch.empty(*lead, k // 32, dtype=torch.uint8, device=DEV)
+        assert ops.mxfp4_dequantize(c, s).shape == (*lead, k)
+        assert ops.mxfp4_dequantize(c, s, F32).dtype == F32

@@ -346,3 +346,15 @@ def test_forward_mode_is_refused_not_passed_over(name):
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="no derivative"):
             _out_call(forward_ad.make_dual(_x(), _x()), out)
+
+
+# ------------------------------------------------------------------ empty pairs
+
+@pytest.mark.parametrize("shape", [(5, 0), (0, 64), (0, 0)])
+def test_dequantise_of_no_values(monkeypatch, shape):
+    monkeypatch.undo()
+    codes = torch.empty(shape, dtype=U8)
+    scales = torch.empty(shape[0], shape[1] // 16, dtype=U8)
+    for f32 in (False, True):
+        y = torch_ops._mx_impl["mxfp4_dequantize"](codes, scales, f32)
+        assert y.shape == (shape[0], 2 * shape[1]) and y.dtype == (torch.float32 if f32 else BF16)
