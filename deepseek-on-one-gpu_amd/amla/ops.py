@@ -472,7 +472,7 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     if not h2.is_contiguous() or h2.data_ptr() % 16:
         h2 = h2.contiguous()
     m = h2.shape[0]
-    out = torch.empty_like(hidden)
+    out = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device)  # rows in order, whatever hidden's strides
     if m == 0:
         return out
     dev = hidden.device

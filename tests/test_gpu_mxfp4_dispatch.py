@@ -174,3 +174,27 @@ def test_dequantise_of_empty_pairs(lead):
         s = torch.empty(*lead, k // 32, dtype=torch.uint8, device=DEV)
         assert ops.mxfp4_dequantize(c, s).shape == (*lead, k)
         assert ops.mxfp4_dequantize(c, s, F32).dtype == F32
+
+
+def _moe(g, experts_of):
+    cfg = DeepSeekConfig(hidden_size=512, n_routed_experts=16, num_experts_per_tok=4, n_group=4, topk_group=2,
+                         moe_intermediate_size=256)
+    shared = {"gate_proj": _weight(g, 256, 512), "up_proj": _weight(g, 256, 512), "down_proj": _weight(g, 512, 256)}
+    return cfg, shared, {k: experts_of(*s) for k, s in {"gate_proj": (16, 256, 512), "up_proj": (16, 256, 512),
+                                                        "down_proj": (16, 512, 256)}.items()}
+
+
+def _fp8_stack(g, E, n, k):
+    return ((torch.randn(E, n, k, generator=g) * 60).clamp(-448, 448).to(torch.float8_e4m3fn).to(DEV),
+            torch.full((E, -(-n // 128), -(-k // 128)), 1e-3, device=DEV))
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "fp8"])
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_moe_block_of_a_permuted_batch(kind, tokens):
+    g = torch.Generator().manual_seed(15)
+    cfg, shared, experts = _moe(g, (lambda *s: _weight(g, *s)) if kind == "mxfp4" else (lambda *s: _fp8_stack(g, *s)))
+    h = _x(16, tokens, 2, 512).transpose(0, 1)
+    gate = _x(17, 16, 512)
+    got = ops.moe_block(h, gate, shared, experts, cfg)
+    assert torch.equal(got, ops.moe_block(h.contiguous(), gate, shared, experts, cfg))

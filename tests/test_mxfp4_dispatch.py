@@ -358,3 +358,14 @@ def test_dequantise_of_no_values(monkeypatch, shape):
     for f32 in (False, True):
         y = torch_ops._mx_impl["mxfp4_dequantize"](codes, scales, f32)
         assert y.shape == (shape[0], 2 * shape[1]) and y.dtype == (torch.float32 if f32 else BF16)
+
+
+# ------------------------------------------------------------------ moe_block's arguments
+
+def test_moe_block_of_a_permuted_batch(monkeypatch):
+    """Hidden states with permuted strides (a batch kept time first): the result is written row by row."""
+    cfg, experts = _moe_parts(monkeypatch)
+    h = _x(6).view(3, 2, 128).transpose(0, 1)
+    assert not h.is_contiguous()
+    got = ops.moe_block(h, _x(2), {}, experts, cfg)
+    assert got.shape == h.shape and torch.equal(got, ops.moe_block(h.contiguous(), _x(2), {}, experts, cfg))
