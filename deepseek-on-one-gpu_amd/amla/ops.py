@@ -462,6 +462,7 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     get = None if stacked or streamed else (experts if callable(experts) else experts.__getitem__)
     if routing is not None:
         idx, w = routing
+        _check_routing(idx, w, hidden, config.num_experts_per_tok, stacked and device_grouping)
     else:
         idx, w = route(hidden, gate_weight, config)
     shared_out = expert_ffn(hidden, shared_weights)
@@ -525,6 +526,18 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     _moe_experts_call(h2, idx_host, tables, n_inter, E, eout)
     del keep
     return _moe_combine(shared_out, eout, w, m, top_k, d, config, out, hidden)
+
+
+def _check_routing(idx, w, hidden, top_k: int, on_device: bool) -> None:
+    """A routing as ``route`` gives it; the indices may be on the host where the slots are grouped there."""
+    for t, name, dtype in ((idx, "indices", torch.int64), (w, "weights", torch.float32)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+            raise TypeError(f"moe_block: the routing's {name} must be a {dtype} tensor")
+        if t.numel() != hidden.shape[:-1].numel() * top_k:
+            raise ValueError(f"moe_block: routing {name} {tuple(t.shape)} for hidden {tuple(hidden.shape)}, {top_k} "
+                             "experts a token")
+    if w.device != hidden.device or idx.device != hidden.device and (on_device or idx.device.type != "cpu"):
+        raise ValueError(f"moe_block: the routing is on {idx.device} and {w.device}, hidden on {hidden.device}")
 
 
 def _moe_experts_call(h2, idx_host, tables, n_inter, E, eout) -> None:

@@ -369,3 +369,16 @@ def test_moe_block_of_a_permuted_batch(monkeypatch):
     assert not h.is_contiguous()
     got = ops.moe_block(h, _x(2), {}, experts, cfg)
     assert got.shape == h.shape and torch.equal(got, ops.moe_block(h.contiguous(), _x(2), {}, experts, cfg))
+
+
+def test_moe_block_refuses_a_routing_of_other_types(monkeypatch):
+    """The combine reads the weights as fp32 and the grouping the indices as int64, by address."""
+    cfg, experts = _moe_parts(monkeypatch)
+    h, gate = _x(), _x(2)
+    idx, w = torch.zeros(4, 2, dtype=torch.int64), torch.ones(4, 2)
+    assert ops.moe_block(h, gate, {}, experts, cfg, routing=(idx, w)).shape == h.shape
+    for routing in ((idx.int(), w), (idx, w.to(BF16)), (idx, w.double()), (idx, w.to("meta")), (idx[:3], w), (idx, w[:3]),
+                    (idx[:, :1], w), (idx, torch.ones(4, 3)), (idx.tolist(), w)):
+        for ex in (experts, {0: {}, 1: {}}):
+            with pytest.raises((TypeError, ValueError), match="routing"):
+                ops.moe_block(h, gate, {}, ex, cfg, routing=routing)
