@@ -436,7 +436,8 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     * one dict of stacked weights ``{"gate_proj": (w (E, n, k), s (E, ceil(n/128),
       ceil(k/128))), ...}`` (all experts of the layer contiguous: no per-expert host work);
       with uint8 tensors, stacked MXFP4 weights ``(codes (E, n, k/2), exponents (E, n, k/32))``
-      (``mxfp4_moe_experts``; the shared expert may be of either form);
+      (``mxfp4_moe_experts``; the shared expert may be of either form; MXFP4 experts are taken in
+      this form only);
     * an ``amla.experts.ExpertStreamer`` (with ``layer=``): the chosen experts are streamed
       from host memory in waves of at most the pool size, each wave computed before the
       next one is copied, so any batch runs on any pool (gpu_transfer.py:50-89 plus
@@ -507,6 +508,8 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
         ew = get(int(e))
         for j, key in enumerate(("gate_proj", "up_proj", "down_proj")):
             wt, sc = ew[key]
+            if wt.dtype == torch.uint8:
+                raise ValueError("moe_block: MXFP4 experts are given as one dict of stacked weights")
             if wt.dtype != FP8 or sc.dtype != torch.float32 or wt.device != dev or sc.device != dev or \
                     not (wt.is_contiguous() and sc.is_contiguous()):
                 raise ValueError(f"moe_block: expert {e} {key} must be contiguous e4m3fn weights with fp32 "

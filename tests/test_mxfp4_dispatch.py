@@ -382,3 +382,12 @@ def test_moe_block_refuses_a_routing_of_other_types(monkeypatch):
         for ex in (experts, {0: {}, 1: {}}):
             with pytest.raises((TypeError, ValueError), match="routing"):
                 ops.moe_block(h, gate, {}, ex, cfg, routing=routing)
+
+
+def test_moe_block_says_how_mxfp4_experts_are_held(monkeypatch):
+    """A mapping or a callable of per-expert pairs: refused by what it is, not as bad fp8 weights."""
+    cfg, experts = _moe_parts(monkeypatch)
+    by_expert = {e: {k: (c[e], s[e]) for k, (c, s) in experts.items()} for e in range(2)}
+    for given in (by_expert, by_expert.__getitem__):
+        with pytest.raises(ValueError, match="MXFP4 experts .* stacked"):
+            ops.moe_block(_x(), _x(2), {}, given, cfg)
