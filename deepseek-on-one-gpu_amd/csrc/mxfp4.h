@@ -26,7 +26,7 @@ AMLA_DEV uint32_t mx_byte(uint32_t amax) {
 // 2^(byte - 127) for byte <= 254
 AMLA_DEV float mx_scale(uint32_t byte) { return __uint_as_float(byte ? byte << 23 : 1u << 22); }
 
-// Eight fp32 values -> eight codes; `keep` 0 clears them (NaN block)
+// Eight fp32 values -> eight codes (the callers clear those of a NaN block)
 AMLA_DEV uint32_t mx_codes8(const float *v, float scale) {
   uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], scale, 0);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], scale, 1);

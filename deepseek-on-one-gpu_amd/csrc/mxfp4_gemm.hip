@@ -539,8 +539,12 @@ struct MxRowsMain {
 // multiplied, so that the slot is free for the stage after next when the second
 // begins.
 //
-// What bounds it is the power of the matrix units: 4096 x 7168 x 16384 in 241 - 255 us (3.8
-// - 4.0 PFLOP/s); the multiplications and barriers alone, on the same data, take 223 us.
+// Bound by the power of the matrix units and by whole rounds of tiles.  16384 K values to 7168
+// outputs: 4096 rows (448 tiles, two rounds of the 256 CUs with the second three quarters
+// full) in 226 - 243 us (4.0 - 4.3 PFLOP/s), on zeros in 195; 4608 rows (504 tiles) in 244 -
+// 259, on zeros in 196: idle CUs in the second round cost all of their time on zeros, where
+// power does not bound, and half of it on data.
+// The multiplications and barriers of 4096 rows alone, on the same data, take 223 us.
 // Four slots of 64-byte rows, two stages on their way: 306 us (the L2 delivers 20
 // TB/s in such pieces, 35 TB/s in lines).  256 x 128 tiles, two workgroups per CU: 332.
 constexpr int MXB_STAGE = 2 * MX_WHALF;
@@ -1420,8 +1424,11 @@ struct MxLinearLayout {
   bool stream, fused;  // fused: the stream product quantises
   MxSplit sp;
 };
-// Values of x that each workgroup may quantise for itself: 1 x 7168 x 16384 16.8 us, with a
-// pass before it 19.0; 8 x 18432 x 7168 20.7 and 21.3; 16 x 2112 x 7168 11.8 and 11.0.
+// Values of x that each workgroup of a linear may quantise for itself: 1 x 7168 x 16384 16.8
+// us, with a pass before it 19.0; 8 x 18432 x 7168 20.7 and 21.3; 16 x 2112 x 7168 11.8 and
+// 11.0.  SwiGLU, groups and experts always do on the stream product, which has more weight rows
+// there: SwiGLU of 7168 to 18432, 1 row 38.6 and 40.7, 8 rows 44.8 and 45.4, 16 rows 49.7 and
+// 49.1; 16 rows of 32 groups, 7168 to 2048, 24.9 and 26.8; 8 tokens on 64 experts 209 and 211.5.
 constexpr int64_t MX_FUSED = 72 * 1024;
 // held: x comes quantised
 static MxLinearLayout mx_linear_layout(int64_t m, int64_t k, int64_t n, bool held) {
@@ -1498,7 +1505,12 @@ static MxMoeLayout mx_moe_layout(int64_t m, int64_t d, int top_k, int64_t n, int
   L.stream = mx_stream_fits(m, d, true) && mx_stream_fits(m, n, false);
   L.small_up = !L.stream && mx_small_round(S, E, (n + 63) / 64);
   L.small_down = !L.stream && mx_small_round(S, E, (d + 127) / 128);
-  L.rows = L.stream ? (int)m : L.small_up || L.small_down ? MXS_ROWS : MX_ROWS;  // (a token may name an expert several times: more entries)
+  // One schedule for both products: where only one of them has small tiles, the other runs large ones
+  // on entries of 64 rows.  Hidden size 7168, intermediate 2048: 400 rows in 8 ragged groups 69 us, with
+  // large tiles for both 82; in 2 groups 45 and 81.  2048 and 7168: 700 in 4 groups 67 and 80 - 104, 900
+  // in 16 even ones 126 and 121.  (An entry of the stream product holds m rows at most, also where tokens
+  // name an expert several times: more entries then.)
+  L.rows = L.stream ? (int)m : L.small_up || L.small_down ? MXS_ROWS : MX_ROWS;
   L.max_entries = (int)std::min<int64_t>(S, std::min<int64_t>(E, S) + S / L.rows);
   L.hdr = take(16);
   L.count = take(4);

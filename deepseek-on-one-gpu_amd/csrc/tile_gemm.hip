@@ -513,11 +513,7 @@ AMLA_DEV void tile_store(const TileArgs &a, const TileSums<NJ> &ts) {
 // ---------------------------------------------------------------- linears of many rows
 
 // The GEMM of launch_gemm (GemvMode epilogues): tiles of 256 weight rows x 128
-// activation rows.  Workgroup i runs on XCD i % 8: each XCD takes a contiguous
-// run of the tiles in panels of 8 column tiles, row tiles within a panel, so
-// the 64 tiles it holds at a time share 8 + 8 tile operands through its L2;
-// with up to 8 row tiles the row tiles of a column tile come together (the
-// weights are then the larger operand).
+// activation rows, in the order of tile_order.h.
 template <int MODE, int NJ, bool WIDE>
 AMLA_DEV void tile_linear_body(const GemvParams &p, const TileArgs &a, int n0, int n1, int m0, bool staged,
                                float *partial) {

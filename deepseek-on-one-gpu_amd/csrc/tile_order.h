@@ -1,4 +1,12 @@
 // Order of the GEMM tiles over workgroups and XCDs.
+//
+// Workgroup i runs on XCD i % 8.  xcd_run gives each XCD a contiguous run of the tiles;
+// tile_coords orders them in panels of `panel` column tiles, row tiles within a panel, so
+// that the tiles an XCD holds at a time share their operands through its L2: of 64 tiles
+// panels of 8 read 8 + 8 operands.  Where the row tiles are fewer than a panel's columns
+// they come together for each column tile (the weights are then the larger operand).
+// `panel` is 8 for the largest tiles; callers with smaller row tiles pass fewer, so that the
+// weight rows of a panel stay about as many as the activation rows read beside them.
 #pragma once
 
 #include "amla_common.h"
