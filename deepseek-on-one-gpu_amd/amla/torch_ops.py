@@ -38,6 +38,7 @@ import torch
 from torch import Tensor
 from torch.autograd import forward_ad
 from torch.overrides import has_torch_function
+from torch.utils._device import DeviceContext
 
 from ._lib import MlaArgs, check, lib
 
@@ -301,12 +302,24 @@ def call(name: str, t: Tensor, *args):
     """The implementation of amla::<name>, or the operator itself where the difference shows: something
     traces, transforms or intercepts torch's operators, an argument is a tensor subclass, or a derivative
     is asked for."""
-    if _dynamo() or _thread_keys().raw_repr() & _WATCHED or has_torch_function((t, *args)) or t.requires_grad or \
-            forward_ad._current_level >= 0 or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter):
+    if _dynamo() or _thread_keys().raw_repr() & _WATCHED or has_torch_function((t, *args)) and _intercepted(t, *args) or \
+            t.requires_grad or forward_ad._current_level >= 0 or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter):
         if name not in _MX_WHOLE:
             _no_tangent(t)
         return getattr(torch.ops.amla, name)(t, *args)
     return _on_device(_mx_impl[name], t, *args)
+
+
+_PLAIN_TYPES = frozenset((Tensor, torch.nn.Parameter, type(None), bool))  # of an operator's arguments
+
+
+def _intercepted(*args) -> bool:
+    """Whether a function mode other than a default device is on, or an argument is a subclass."""
+    modes = torch._C._len_torch_function_stack()
+    for i in range(modes):
+        if type(torch._C._get_function_stack_at(i)) is not DeviceContext:
+            return True
+    return not modes or not _PLAIN_TYPES.issuperset(map(type, args))
 
 
 _MX_WHOLE = ("mxfp4_quantize", "mxfp4_quantize_fp8")  # outputs are whole numbers: no derivative passes through

@@ -391,3 +391,23 @@ def test_moe_block_says_how_mxfp4_experts_are_held(monkeypatch):
     for given in (by_expert, by_expert.__getitem__):
         with pytest.raises(ValueError, match="MXFP4 experts .* stacked"):
             ops.moe_block(_x(), _x(2), {}, given, cfg)
+
+
+def test_a_default_device_does_not_count_as_a_mode(monkeypatch):
+    """torch.set_default_device and ``with device`` are function modes that change factories only."""
+    f, make = _calls()["mxfp4_linear"]
+    t = make()
+    ran = []
+    monkeypatch.setattr(torch_ops, "_on_device", lambda fn, t, *args: ran.append(1) or fn(t, *args))
+    with torch.device("cpu"):
+        f(t)
+        assert len(ran) == 1
+
+        class Watch(TorchFunctionMode):
+            def __torch_function__(self, func, types, args=(), kwargs=None):
+                return func(*args, **(kwargs or {}))
+
+        with Watch():
+            f(t)
+        f(t.as_subclass(type("Sub", (torch.Tensor,), {})))
+        assert len(ran) == 1
