@@ -463,7 +463,8 @@ def moe_block(hidden: torch.Tensor, gate_weight: torch.Tensor, shared_weights: d
     get = None if stacked or streamed else (experts if callable(experts) else experts.__getitem__)
     if routing is not None:
         idx, w = routing
-        _check_routing(idx, w, hidden, config.num_experts_per_tok, stacked and device_grouping)
+        on_device = stacked and device_grouping and (config.n_routed_experts <= MOE_DEV_MAX_EXPERTS or _is_mxfp4(experts))
+        _check_routing(idx, w, hidden, config.num_experts_per_tok, on_device)
     else:
         idx, w = route(hidden, gate_weight, config)
     shared_out = expert_ffn(hidden, shared_weights)

@@ -3,6 +3,7 @@
 On the CPU, with stand-ins for the kernels: a stand-in writes its output behind torch's back, as a
 kernel does, so that a trace which misses the operator replays uninitialised memory."""
 import ctypes
+import dataclasses
 
 import pytest
 import torch
@@ -411,3 +412,22 @@ def test_a_default_device_does_not_count_as_a_mode(monkeypatch):
             f(t)
         f(t.as_subclass(type("Sub", (torch.Tensor,), {})))
         assert len(ran) == 1
+
+
+@pytest.mark.parametrize("experts,on_device", [(2, True), (512, True), (513, False)])
+def test_moe_block_takes_indices_on_the_host_where_it_groups_there(monkeypatch, experts, on_device):
+    """fp8 experts past what the device groups: the indices come to the host, or are there already."""
+    cfg, _ = _moe_parts(monkeypatch)
+    cfg = dataclasses.replace(cfg, n_routed_experts=experts)
+    seen = []
+
+    def check(idx, w, hidden, top_k, where):
+        seen.append(where)
+        raise StopIteration
+
+    monkeypatch.setattr(ops, "_check_routing", check)
+    w8 = torch.zeros(experts, 1, 1, dtype=torch.float8_e4m3fn)
+    with pytest.raises(StopIteration):
+        ops.moe_block(_x(), _x(2), {}, {k: (w8, w8) for k in ("gate_proj", "up_proj", "down_proj")}, cfg,
+                      routing=(torch.zeros(4, 2, dtype=torch.int64), torch.ones(4, 2)))
+    assert seen == [on_device]
