@@ -38,6 +38,22 @@ class MlaArgs(ctypes.Structure):
     ]
 
 
+class LatentCache(ctypes.Structure):
+    """Mirror of ``amla_latent_cache`` in include/amla.h (same field order)."""
+    _fields_ = [("latent", c_void_p), ("k_pe", c_void_p), ("scales", c_void_p), ("block_table", c_void_p),
+                ("ld_table", c_int64), ("cols", c_int64), ("pages", c_int64), ("page_size", ctypes.c_int32)]
+
+
+class PackedArgs(ctypes.Structure):
+    """Mirror of ``amla_packed_args`` in include/amla.h (same field order)."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("k_pe", c_void_p), ("out", c_void_p),
+                ("lse", c_void_p), ("offsets", c_void_p), ("k_offsets", c_void_p), ("q_rows", c_int64),
+                ("k_rows", c_int64), ("seqs", c_int64), ("ldq", c_int64), ("ldq_head", c_int64), ("ldk", c_int64),
+                ("ldk_head", c_int64), ("ldv", c_int64), ("ldv_head", c_int64), ("ld_pe", c_int64),
+                ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("dn", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("scale", c_float)]
+
+
 # (name, restype, argtypes) of every exported entry point
 SIGNATURES = [
     ("amla_abi_version", c_int, []),
@@ -99,6 +115,15 @@ SIGNATURES = [
                                        c_int, c_void_p, c_size_t, c_void_p]),
     ("amla_mxfp4_moe_experts_workspace_bytes", c_size_t, [
         c_int64, c_int64, c_int, c_int64, c_int64]),
+    ("amla_latent_cache_write", c_int, [ctypes.POINTER(LatentCache), c_void_p, c_int64, c_int64, c_void_p, c_float,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    ("amla_latent_cache_read", c_int, [ctypes.POINTER(LatentCache), c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                       c_void_p, c_int, c_void_p]),
+    ("amla_latent_attention", c_int, [ctypes.POINTER(LatentCache), c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                      c_int64, c_int64, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
+                                      c_void_p]),
+    ("amla_latent_attention_workspace_bytes", c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    ("amla_packed_attention", c_int, [ctypes.POINTER(PackedArgs), c_void_p]),
     ("amla_moe_combine", c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_float, c_void_p,
                                  c_void_p]),
 ]

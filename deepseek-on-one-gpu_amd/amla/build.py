@@ -16,7 +16,7 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 LIB = os.path.join(PKG, "libamla.so")
 SOURCES = ["fp8_linear.hip", "mla_decode.hip", "mla_prefill.hip", "ffn_moe.hip", "lm_head.hip", "tile_gemm.hip",
-           "mxfp4_quant.hip", "mxfp4_gemm.hip"]
+           "mxfp4_quant.hip", "mxfp4_gemm.hip", "latent_cache.hip", "latent_attn.hip", "packed_attn.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

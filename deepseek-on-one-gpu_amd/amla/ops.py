@@ -7,8 +7,9 @@ attention half of ``transformer_layer`` (inference/forward.py:92-94) as
 ``mla_layer``; and the FFN / MoE functions on the same fp8 kernels: ``swiglu``
 (:186-192), ``dense_ffn`` / ``expert_ffn`` (:195-206), ``route`` (:209-257) and
 ``moe_block`` (inference/forward.py:112-153, experts handed in); and the same
-linears, FFN and experts for weights held in MXFP4 (``mxfp4_*``).  Same argument
-names, tensor layouts and dtypes; tensors must be
+linears, FFN and experts for weights held in MXFP4 (``mxfp4_*``); and, for a
+server of many sequences, a paged latent cache (``latent_cache_*``), the attention
+over it and that of packed prompts.  Same argument names, tensor layouts and dtypes; tensors must be
 on a ROCm device.  Every compute call goes to libamla.so; there is no CPU or
 PyTorch fallback (a missing library raises).
 
@@ -847,6 +848,201 @@ def mxfp4_moe_experts(hidden: torch.Tensor, indices: torch.Tensor, experts: dict
     out = torch_ops.call("mxfp4_moe_experts", h2, idx.contiguous(), *experts["gate_proj"], *experts["up_proj"],
                          *experts["down_proj"])
     return out if hidden.dim() == 2 else out.view(*hidden.shape[:-1], top_k, d)
+
+
+# ------------------------------------------------------------------ paged latent cache
+
+def latent_cache(pages: int, page_size: int, config, device, dtype: torch.dtype = FP8) -> tuple:
+    """An empty pool of rows for ``latent_cache_write``: ``(latent (pages, page_size, kv_lora_rank),
+    k_pe (pages, page_size, qk_rope_head_dim) bf16)`` with bf16 latents, and for e4m3 latents (``dtype``
+    float8_e4m3fn, the default) also ``scales (pages, page_size)`` uint8, the exponent byte of each row:
+    value = code * 2^(byte - 127).  641 bytes a row instead of 1152.  page_size: a power of two."""
+    if dtype not in (FP8, BF16):
+        raise TypeError(f"latent_cache: dtype must be float8_e4m3fn or bfloat16 (got {dtype})")
+    if pages <= 0 or page_size <= 0 or page_size > 65536 or page_size & (page_size - 1):
+        raise ValueError(f"latent_cache: {pages} pages of {page_size} rows (a power of two up to 65536)")
+    latent = torch.zeros(pages, page_size, config.kv_lora_rank, dtype=torch.uint8 if dtype == FP8 else BF16, device=device)
+    k_pe = torch.zeros(pages, page_size, config.qk_rope_head_dim, dtype=BF16, device=device)
+    if dtype == BF16:
+        return latent, k_pe
+    return latent.view(FP8), k_pe, torch.full((pages, page_size), 127, dtype=torch.uint8, device=device)
+
+
+LATENT, LATENT_ROPE = 512, 64  # values of a row
+
+
+def _latent_parts(cache, what: str) -> tuple:
+    """(latent, k_pe, scales or None) of a checked cache."""
+    if not isinstance(cache, (tuple, list)) or len(cache) not in (2, 3):
+        raise ValueError(f"{what}: the cache is (latent, k_pe) or (latent, k_pe, scales)")
+    latent, k_pe = cache[0], cache[1]
+    scales = cache[2] if len(cache) == 3 else None
+    _need(latent, "latent", BF16 if scales is None else FP8)
+    _need(k_pe, "k_pe", BF16, latent.device)
+    if latent.dim() != 3 or latent.shape[2] != LATENT or k_pe.shape != latent.shape[:2] + (LATENT_ROPE,) or not latent.numel():
+        raise ValueError(f"{what}: cache of {tuple(latent.shape)} and {tuple(k_pe.shape)}, expected (pages, page_size, "
+                         f"{LATENT}) and (pages, page_size, {LATENT_ROPE})")
+    if scales is not None:
+        _need(scales, "scales", torch.uint8, latent.device)
+        if scales.shape != latent.shape[:2]:
+            raise ValueError(f"{what}: scales {tuple(scales.shape)} of a cache of {tuple(latent.shape)}")
+    return latent, k_pe, scales
+
+
+def _need_i32(t, name: str, what: str, dev, shape: tuple) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != dev or t.shape != shape or \
+            not t.is_contiguous():
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{what}: {name} must be a contiguous int32 tensor {shape} on {dev} (got {got})")
+
+
+def _need_table(t, what: str, dev) -> int:
+    """Checks a block table (sequences, pages of a sequence) and returns its sequences."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != dev or t.dim() != 2 or \
+            (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        raise ValueError(f"{what}: block_table must be an int32 tensor (sequences, pages) with rows of unit stride on {dev}")
+    return t.shape[0]
+
+
+def latent_cache_write(kv: torch.Tensor, kv_a_layernorm: torch.Tensor, rope_freqs: torch.Tensor, cache: tuple,
+                       block_table: torch.Tensor, position, *, offsets: torch.Tensor | None = None,
+                       eps: float = 1e-6) -> None:
+    """Stores new rows of the cache: the norm of inference/ops.py:148 and the rotation of :158-159,
+    done once as a row is written, where the reference stores it raw (:140-141) and repeats them.
+
+    ``kv`` bf16, the output of kv_a_proj_with_mqa: (B, S, 576), S new rows of every sequence, or with
+    ``offsets`` ((B + 1,) int32 on the device, ascending) the packed rows (T, 576), offsets[b] ..
+    offsets[b + 1] - 1 of sequence b.  ``position``: as for ``mla_attention``, the first new row of each
+    sequence.  ``rope_freqs``: ``precompute_rope_freqs``.  ``cache``: ``latent_cache``; row i of
+    sequence b is row i % page_size of page ``block_table[b, i // page_size]`` ((B, n) int32 on the
+    device).  All in fp32 with one rounding, to bf16 or to e4m3 with the smallest power of two that
+    keeps the row within 448 times it (2^-32 .. 2^32); a row with an infinity or a NaN becomes one of
+    NaN.  Rows of no sequence, of a page outside the pool or past the rope table are not written;
+    nothing of that is checked on the host.  Two rows of a call must not share a place."""
+    what = "latent_cache_write"
+    latent, k_pe, scales = _latent_parts(cache, what)
+    dev = latent.device
+    _need_cuda(kv, "kv")
+    if kv.dtype != BF16 or kv.device != dev:
+        raise TypeError(f"{what}: kv must be bfloat16 on {dev} (got {kv.dtype} on {kv.device})")
+    if kv.dim() != (3 if offsets is None else 2) or kv.shape[-1] != LATENT + LATENT_ROPE:
+        raise ValueError(f"{what}: kv of shape {tuple(kv.shape)}, expected (B, S, 576), or (T, 576) with offsets")
+    _need(kv_a_layernorm, "kv_a_layernorm", BF16, dev)
+    if kv_a_layernorm.shape != (LATENT,):
+        raise ValueError(f"{what}: kv_a_layernorm of shape {tuple(kv_a_layernorm.shape)}")
+    if rope_freqs.dtype != torch.complex64 or rope_freqs.device != dev or not rope_freqs.is_contiguous() or \
+            rope_freqs.dim() != 2 or rope_freqs.shape[1] != LATENT_ROPE // 2:
+        raise TypeError(f"{what}: rope_freqs must be a contiguous complex64 tensor (positions, {LATENT_ROPE // 2}) on {dev}")
+    B = _need_table(block_table, what, dev)
+    if offsets is None:
+        if kv.shape[0] != B:
+            raise ValueError(f"{what}: kv of {kv.shape[0]} sequences, block_table of {B}")
+        kv = kv.reshape(-1, LATENT + LATENT_ROPE)
+    else:
+        _need_i32(offsets, "offsets", what, dev, (B + 1,))
+    pos = _positions(position, B, 1, dev, None)[0] if B else torch.empty(0, dtype=torch.int32, device=dev)
+    _need_i32(pos, "position", what, dev, (B,))
+    torch_ops.call_latent("latent_cache_write", kv, kv_a_layernorm, rope_freqs, latent, k_pe, scales, block_table, pos,
+                          offsets, float(eps))
+
+
+def latent_cache_read(cache: tuple, block_table: torch.Tensor, offsets: torch.Tensor, rows: int, *,
+                      position: torch.Tensor | None = None, out: tuple | None = None) -> tuple:
+    """Rows of the cache as (latent (rows, 512), k_pe (rows, 64)) bf16, packed: rows offsets[b] ..
+    offsets[b + 1] - 1 ((B + 1,) int32 on the device, ascending) are rows position[b] .. of sequence b
+    ((B,) int32 on the device; None: from row 0).  The values are the cache's own, exactly.  What kv_b
+    takes for a prompt that continues a cached one (inference/ops.py:144-151).
+
+    Rows of no sequence or of no page are zeros, and with ``out`` ((latent, k_pe) to write to) stay as
+    they were."""
+    what = "latent_cache_read"
+    latent, k_pe, scales = _latent_parts(cache, what)
+    dev = latent.device
+    B = _need_table(block_table, what, dev)
+    _need_i32(offsets, "offsets", what, dev, (B + 1,))
+    if position is not None:
+        _need_i32(position, "position", what, dev, (B,))
+    rows = int(rows)
+    if rows < 0:
+        raise ValueError(f"{what}: {rows} rows")
+    if out is None:
+        return torch_ops.call_latent("latent_cache_read", latent, k_pe, scales, block_table, offsets, position, rows)
+    for t, n in zip(out, (LATENT, LATENT_ROPE), strict=True):
+        _need(t, "out", BF16, dev)
+        if t.shape != (rows, n):
+            raise ValueError(f"{what}: out of shape {tuple(t.shape)}, expected ({rows}, {n})")
+    torch_ops.call_latent("latent_cache_read_out", latent, k_pe, scales, block_table, offsets, position, *out)
+    return tuple(out)
+
+
+def latent_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, lengths: torch.Tensor, scale: float, *,
+                     return_lse: bool = False):
+    """Attention of the newest tokens over the paged cache, in latent space: the scores and the weighted
+    sum of ``mla_attention``'s decode (inference/ops.py:162-182, with kv_b absorbed into the query).
+
+    ``q`` (B, S, H, 576) bf16: per head the query times W_UK (512) and the rotated rope query (64), any H,
+    any strides.  ``lengths`` (B,) int32 on the device: the rows of each sequence, the S new ones
+    included; token s sees rows 0 .. lengths[b] - S + s.  ``scale``: ``softmax_scale(config)``.  Returns
+    (B, S, H, 512) bf16, the softmax-weighted sums of latents (times W_UV: the heads' outputs), and with
+    ``return_lse`` the log of the sum of exp(scores), (B, S, H) fp32.  A token that sees no row gives
+    zeros and -inf; pages outside the pool hold no rows.  A length past the table counts as its end."""
+    what = "latent_attention"
+    latent, k_pe, scales = _latent_parts(cache, what)
+    dev = latent.device
+    _need_cuda(q, "q")
+    if q.dtype != BF16 or q.device != dev:
+        raise TypeError(f"{what}: q must be bfloat16 on {dev} (got {q.dtype} on {q.device})")
+    B = _need_table(block_table, what, dev)
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != LATENT + LATENT_ROPE:
+        raise ValueError(f"{what}: q of shape {tuple(q.shape)}, expected ({B}, S, H, {LATENT + LATENT_ROPE})")
+    _need_i32(lengths, "lengths", what, dev, (B,))
+    o, lse = torch_ops.call_latent("latent_attention", q, latent, k_pe, scales, block_table, lengths, float(scale),
+                                   bool(return_lse))
+    return (o, lse) if return_lse else o
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, scale: float, *,
+                     k_offsets: torch.Tensor | None = None, k_pe: torch.Tensor | None = None, causal: bool = True,
+                     return_lse: bool = False):
+    """Attention of whole prompts packed one after another (inference/ops.py:162-182 for sequences of
+    different lengths): rows offsets[b] .. offsets[b + 1] - 1 of ``q`` over rows k_offsets[b] .. of ``k``
+    and ``v`` (int32 (B + 1,) on the device, ascending; ``k_offsets`` None: the same).
+
+    ``q`` (T, H, d), ``k`` (N, G, d), ``v`` (N, G, 128) bf16, H a multiple of G, each H / G heads sharing
+    keys and values, d 128 or 192; or with ``k_pe`` (N, 64), a rope key shared by all heads, d = 192 and
+    ``k`` (N, G, 128): kv_b's output (N, G, 256) goes in as two views.  Queries are the last tokens of
+    their sequence: with ``causal`` row i of n sees key j of m where j <= i + m - n.  Returns (T, H, 128)
+    bf16, with ``return_lse`` also the log of the sum of exp(scores) (T, H) fp32.  A row that sees no
+    key gives zeros and -inf.  Offsets are not checked on the host; they are clamped to the rows, and
+    the output of rows in no sequence is left unset."""
+    what = "packed_attention"
+    _need_cuda(q, "q")
+    dev = q.device
+    for t, name in ((q, "q"), (k, "k"), (v, "v")) + (((k_pe, "k_pe"),) if k_pe is not None else ()):
+        _need_cuda(t, name)
+        if t.dtype != BF16 or t.device != dev:
+            raise TypeError(f"{what}: {name} must be bfloat16 on {dev} (got {t.dtype} on {t.device})")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"{what}: q, k and v must be (rows, heads, values)")
+    dk = k.shape[2] + (0 if k_pe is None else LATENT_ROPE)
+    if dk not in (128, 192) or q.shape[2] != dk or v.shape[2] != 128:
+        raise ValueError(f"{what}: heads of {q.shape[2]} query, {dk} key and {v.shape[2]} value columns (128 or 192 of the "
+                         "first two, 128 of the last)")
+    if v.shape[:2] != k.shape[:2] or (k_pe is not None and k_pe.shape != (k.shape[0], LATENT_ROPE)):
+        raise ValueError(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)}, k_pe "
+                         f"{None if k_pe is None else tuple(k_pe.shape)} do not match")
+    if not k.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{what}: {q.shape[1]} heads over {k.shape[1]} key heads")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{what}: scale must be positive (got {scale})")
+    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or not offsets.numel():
+        raise ValueError(f"{what}: offsets must be an int32 tensor (sequences + 1,)")
+    _need_i32(offsets, "offsets", what, dev, offsets.shape)
+    if k_offsets is not None:
+        _need_i32(k_offsets, "k_offsets", what, dev, offsets.shape)
+    o, lse = torch_ops.call_latent("packed_attention", q, k, v, k_pe, offsets, k_offsets, float(scale), bool(causal),
+                                   bool(return_lse))
+    return (o, lse) if return_lse else o
 
 
 # ------------------------------------------------------------------ output head

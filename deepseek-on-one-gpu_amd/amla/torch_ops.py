@@ -18,6 +18,9 @@ the op, its output shape and its in-place writes:
   implementations directly, and the registered operators where something could
   tell the difference: a tracer, a transform, a mode, a subclass, a gradient
   (the dispatch costs as much host time as the rest of a call).
+* ``amla::latent_*`` / ``amla::packed_attention``: the paged latent cache and the
+  attention of packed prompts, in the same way; ``latent_cache_write`` and
+  ``latent_cache_read_out`` mutate what they write.
 
 Tensors only, no dicts or dataclasses (the op schema cannot carry them): the
 shims in amla.ops keep the reference's signatures and unpack ``attn_weights``
@@ -40,7 +43,7 @@ from torch.autograd import forward_ad
 from torch.overrides import has_torch_function
 from torch.utils._device import DeviceContext
 
-from ._lib import MlaArgs, check, lib
+from ._lib import LatentCache, MlaArgs, PackedArgs, check, lib
 
 BF16 = torch.bfloat16
 
@@ -505,3 +508,147 @@ def _mxfp4_moe_experts(hidden, indices, gate_proj, gate_scale, up_proj, up_scale
                                        out[t:].data_ptr(), 1, ws.data_ptr(), ws.numel(), _mx_stream(hidden)),
               "mxfp4_moe_experts")
     return out
+
+
+# ------------------------------------------------------------------ paged latent cache, packed prompts
+
+def _lc_no_backward(ctx, *grads):
+    raise RuntimeError("the latent cache's operators have no backward pass")
+
+
+def _lc_op(schema: str, fake):
+    """Registers amla::<schema> like ``_mx_op``."""
+    def wrap(fn):
+        name = schema.split("(")[0]
+        _mx_lib.define(schema)
+        _mx_lib.impl(name, lambda t, *args: _on_device(fn, t, *args), "CUDA")
+        torch.library.register_fake(f"amla::{name}", fake, lib=_mx_lib)
+        if "!" in schema:
+            def refuse(*args):
+                _lc_out_gradient(*args)
+                with torch._C._AutoDispatchBelowAutograd():
+                    getattr(torch.ops.amla, name)(*args)
+            _mx_lib.impl(name, refuse, "Autograd")
+        else:
+            torch.library.register_autograd(f"amla::{name}", _lc_no_backward, lib=_mx_lib)
+        _mx_impl[name] = fn
+        return fn
+    return wrap
+
+
+def _lc_out_gradient(*args) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in args):
+        raise RuntimeError("the latent cache has no gradient, but a tensor of the call requires one")
+
+
+def call_latent(name: str, *args):
+    """``call`` for operators with several differentiable inputs: their tensors all decide."""
+    if _dynamo() or _thread_keys().raw_repr() & _WATCHED or has_torch_function(args) and _intercepted(*args) or \
+            forward_ad._current_level >= 0 or any(_needs_operator(t) for t in args if isinstance(t, Tensor)):
+        if not _dynamo() and forward_ad._current_level >= 0 and \
+                any(isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
+            raise RuntimeError("the latent cache's operators have no derivative in forward mode")
+        return getattr(torch.ops.amla, name)(*args)
+    return _on_device(_mx_impl[name], *args)
+
+
+def _needs_operator(t: Tensor) -> bool:
+    return t.requires_grad or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter)
+
+
+def _lc_cache(latent, k_pe, scales, block_table) -> LatentCache:
+    return LatentCache(latent.data_ptr(), k_pe.data_ptr(), _ptr(scales), block_table.data_ptr(), block_table.stride(0),
+                       block_table.shape[1], latent.shape[0], latent.shape[1])
+
+
+def _lc_rows(x: Tensor) -> Tensor:
+    """x itself when its rows are 16-byte aligned with unit stride, else a copy of such."""
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not any(s % 8 for s in x.stride()[:-1]):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+@_lc_op("latent_cache_write(Tensor kv, Tensor weight, Tensor freqs, Tensor(a!) latent, Tensor(b!) k_pe, Tensor(c!)? scales, "
+        "Tensor block_table, Tensor position, Tensor? offsets, float eps) -> ()", lambda *args: None)
+def _latent_cache_write(kv, weight, freqs, latent, k_pe, scales, block_table, position, offsets, eps):
+    kv, weight = _lc_rows(kv), _rows16(weight)
+    rows = kv.shape[0]
+    check(lib().amla_latent_cache_write(_lc_cache(latent, k_pe, scales, block_table), kv.data_ptr(), rows,
+                                        kv.stride(0) if rows > 1 else kv.shape[1], weight.data_ptr(), eps,
+                                        freqs.data_ptr(), freqs.shape[0], _ptr(offsets), block_table.shape[0],
+                                        position.data_ptr(), _mx_stream(kv)), "latent_cache_write")
+    for t in (latent, k_pe, scales):
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
+def _lc_read(latent, k_pe, scales, block_table, offsets, position, out, out_pe, clear) -> None:
+    check(lib().amla_latent_cache_read(_lc_cache(latent, k_pe, scales, block_table), out.shape[0], offsets.data_ptr(),
+                                       block_table.shape[0], _ptr(position), out.data_ptr(), out_pe.data_ptr(), clear,
+                                       _mx_stream(latent)), "latent_cache_read")
+
+
+def _lc_read_fake(latent, k_pe, scales, block_table, offsets, position, rows):
+    return (k_pe.new_empty(rows, latent.shape[2]), k_pe.new_empty(rows, k_pe.shape[2]))
+
+
+@_lc_op("latent_cache_read(Tensor latent, Tensor k_pe, Tensor? scales, Tensor block_table, Tensor offsets, "
+        "Tensor? position, int rows) -> (Tensor, Tensor)", _lc_read_fake)
+def _latent_cache_read(latent, k_pe, scales, block_table, offsets, position, rows):
+    out, out_pe = _lc_read_fake(latent, k_pe, scales, block_table, offsets, position, rows)
+    _lc_read(latent, k_pe, scales, block_table, offsets, position, out, out_pe, 1)
+    return out, out_pe
+
+
+@_lc_op("latent_cache_read_out(Tensor latent, Tensor k_pe, Tensor? scales, Tensor block_table, Tensor offsets, "
+        "Tensor? position, Tensor(a!) out, Tensor(b!) out_pe) -> ()", lambda *args: None)
+def _latent_cache_read_out(latent, k_pe, scales, block_table, offsets, position, out, out_pe):
+    _lc_read(latent, k_pe, scales, block_table, offsets, position, out, out_pe, 0)
+    torch.autograd.graph.increment_version(out)
+    torch.autograd.graph.increment_version(out_pe)
+
+
+_lc_attention_bytes = lru_cache(4096)(lambda *a: lib().amla_latent_attention_workspace_bytes(*a))
+
+
+def _latent_attention_fake(q, latent, k_pe, scales, block_table, lengths, scale, lse):
+    B, S, H, _ = q.shape
+    return q.new_empty(B, S, H, latent.shape[2]), q.new_empty((B, S, H) if lse else (0,), dtype=torch.float32)
+
+
+@_lc_op("latent_attention(Tensor q, Tensor latent, Tensor k_pe, Tensor? scales, Tensor block_table, Tensor lengths, "
+        "float scale, bool lse) -> (Tensor, Tensor)", _latent_attention_fake)
+def _latent_attention(q, latent, k_pe, scales, block_table, lengths, scale, lse):
+    q = _lc_rows(q)
+    B, S, H, _ = q.shape
+    out, lse_out = _latent_attention_fake(q, latent, k_pe, scales, block_table, lengths, scale, lse)
+    if not out.numel():
+        return out, lse_out
+    need = _lc_attention_bytes(B, S, H, block_table.shape[1] * latent.shape[1])
+    ws = _scratch(q.device, need)
+    check(lib().amla_latent_attention(_lc_cache(latent, k_pe, scales, block_table), q.data_ptr(), B, S, H, q.stride(0),
+                                      q.stride(1), q.stride(2), lengths.data_ptr(), scale, out.data_ptr(),
+                                      lse_out.data_ptr() if lse else None, ws.data_ptr(), ws.numel(), _mx_stream(q)),
+          "latent_attention")
+    return out, lse_out
+
+
+def _packed_attention_fake(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse):
+    rows, H, _ = q.shape
+    return q.new_empty(rows, H, v.shape[2]), q.new_empty((rows, H) if lse else (0,), dtype=torch.float32)
+
+
+@_lc_op("packed_attention(Tensor q, Tensor k, Tensor v, Tensor? k_pe, Tensor offsets, Tensor? k_offsets, float scale, "
+        "bool causal, bool lse) -> (Tensor, Tensor)", _packed_attention_fake)
+def _packed_attention(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse):
+    q, k, v = _lc_rows(q), _lc_rows(k), _lc_rows(v)
+    k_pe = None if k_pe is None else _lc_rows(k_pe)
+    out, lse_out = _packed_attention_fake(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse)
+    if not out.numel():
+        return out, lse_out
+    check(lib().amla_packed_attention(PackedArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(k_pe), out.data_ptr(), lse_out.data_ptr() if lse else None,
+        offsets.data_ptr(), _ptr(k_offsets), q.shape[0], k.shape[0], offsets.shape[0] - 1, q.stride(0), q.stride(1),
+        k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0 if k_pe is None else k_pe.stride(0), q.shape[1], k.shape[1],
+        k.shape[2], causal, scale), _mx_stream(q)), "packed_attention")
+    return out, lse_out

@@ -363,6 +363,93 @@ int amla_mxfp4_moe_experts(const void *hidden, int64_t m, int64_t d, int64_t ldh
                            void *expert_out, int clear_skipped, void *workspace, size_t workspace_bytes, void *stream);
 size_t amla_mxfp4_moe_experts_workspace_bytes(int64_t m, int64_t d, int top_k, int64_t n_inter, int64_t n_experts);
 
+/* ---- paged latent cache ----
+ *
+ * What attention needs of a token, kept as one row: the latent normed with
+ * kv_a_layernorm (512 values) and the rope key rotated at the token's position
+ * (64, bf16).  The reference keeps raw rows, one contiguous cache per sequence
+ * (inference/engine.py:72-87), and norms and rotates all of them on every step
+ * (inference/ops.py:144-159); here that happens once, as the row is written.
+ * Rows live in pages of one pool: row i of sequence b is row i % page_size of
+ * page block_table[b * ld_table + i / page_size].  A table entry outside
+ * 0 .. pages - 1 is no page: its rows are not written, read as zeros and not
+ * attended to.  Latents are bf16 or, with scales, e4m3 codes with one exponent
+ * byte a row: value = code * 2^(byte - 127), the smallest power of two in
+ * 2^-32 .. 2^32 that keeps the row's largest magnitude at or below 448 times it
+ * (a row with an infinity or a NaN: byte 255 and codes of NaN). */
+typedef struct amla_latent_cache {
+  void *latent;                /* (pages, page_size, 512) bf16, or e4m3fn with scales */
+  void *k_pe;                  /* (pages, page_size, 64) bf16 */
+  void *scales;                /* (pages, page_size) exponent bytes, or NULL: bf16 latents */
+  const int32_t *block_table;  /* (sequences, cols), row stride ld_table */
+  int64_t ld_table;
+  int64_t cols;
+  int64_t pages;
+  int32_t page_size;           /* a power of two up to 65536 */
+} amla_latent_cache;
+
+/* Most sequences of a call of the entry points below. */
+#define AMLA_MAX_SEQS 65535
+
+/* Writes `rows` new rows: kv (rows, 576) bf16, row stride ldkv, the outputs of
+ * kv_a_proj_with_mqa (inference/ops.py:136-141), as
+ *   latent = x rsqrt(mean(x^2) + eps) gamma, k_pe = rope(x_pe, position)
+ * in fp32 with one rounding.  Row i of kv is row positions[b] + i - offsets[b]
+ * of the sequence b with offsets[b] <= i < offsets[b + 1] (offsets: seqs + 1
+ * ascending int32 in DEVICE memory, or NULL for rows / seqs rows each).  Rows of
+ * no sequence, of no page or at positions outside 0 .. rope_rows - 1 are not
+ * written.  Two rows of a call must not share a place in the pool. */
+int amla_latent_cache_write(const amla_latent_cache *cache, const void *kv, int64_t rows, int64_t ldkv,
+                            const void *gamma, float eps, const float *rope_table, int64_t rope_rows,
+                            const int32_t *offsets, int64_t seqs, const int32_t *positions, void *stream);
+
+/* Reads packed rows back: latent (rows, 512) and k_pe (rows, 64) bf16 (exact for
+ * either form of cache).  offsets and positions as above, positions NULL: from
+ * row 0.  Rows of no sequence or page: zeros with clear_rest, else left as they
+ * were. */
+int amla_latent_cache_read(const amla_latent_cache *cache, int64_t rows, const int32_t *offsets, int64_t seqs,
+                           const int32_t *positions, void *latent, void *k_pe, int clear_rest, void *stream);
+
+/* Attention of the newest tokens in latent space (the scores and the weighted sum
+ * of amla_mla_decode, without its projections) over the paged cache:
+ *   s_t = scale * q . (latent_t | k_pe_t),  out = sum_t softmax(s)_t latent_t,
+ *   lse = log(sum_t exp(s_t))
+ * q (seqs, seq_len, heads, 576) bf16, strides in elements, unit stride within a
+ * head; token s of sequence b sees rows 0 .. lengths[b] - seq_len + s (lengths:
+ * DEVICE int32, the rows held with the new tokens').  A token that sees no row
+ * gives zeros and lse = -inf.  out (seqs, seq_len, heads, 512) bf16, lse (seqs,
+ * seq_len, heads) fp32 or NULL.  Any heads; the rows of one sequence are split
+ * over workgroups whose sums meet in the workspace (16-byte aligned, scratch
+ * only).  The size depends on cols and page_size of the cache, on nothing else of it. */
+int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t seqs, int64_t seq_len, int64_t heads,
+                          int64_t ldq_seq, int64_t ldq_token, int64_t ldq_head, const int32_t *lengths, float scale,
+                          void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+size_t amla_latent_attention_workspace_bytes(int64_t seqs, int64_t seq_len, int64_t heads, int64_t max_rows);
+
+/* Attention of whole prompts, packed one after another (the causal attention of
+ * amla_mla_prefill, inference/ops.py:162-182, for sequences of different lengths):
+ * rows offsets[b] .. offsets[b + 1] - 1 of q are the last of the rows
+ * k_offsets[b] .. k_offsets[b + 1] - 1 of k and v; with causal, row i of n sees
+ * key j of m where j <= i + m - n, else all m.
+ * q (q_rows, heads, dk) with dk = dn + (k_pe ? 64 : 0), dn 128 or 192 (k_pe: 128
+ * only), k (k_rows, kv_heads, dn), v (k_rows, kv_heads, 128), k_pe (k_rows, 64)
+ * shared by all heads, all bf16 with strides in elements (multiples of 8) and
+ * unit stride within a head; heads / kv_heads heads share keys and values.
+ * out (q_rows, heads, 128) bf16 and lse (q_rows, heads) fp32 or NULL, contiguous;
+ * a row that sees no key gives zeros and -inf, rows of no sequence are not
+ * written. */
+typedef struct amla_packed_args {
+  const void *q, *k, *v, *k_pe;
+  void *out;
+  float *lse;
+  const int32_t *offsets, *k_offsets;  /* DEVICE, seqs + 1 ascending; k_offsets NULL: offsets */
+  int64_t q_rows, k_rows, seqs;
+  int64_t ldq, ldq_head, ldk, ldk_head, ldv, ldv_head, ld_pe;
+  int32_t heads, kv_heads, dn, causal;
+  float scale;
+} amla_packed_args;
+int amla_packed_attention(const amla_packed_args *args, void *stream);
+
 /* ---- output head ---- */
 
 /* The lm_head projection of forward.py:70-72 (hidden.float() @ lm_head_w.float().T):
