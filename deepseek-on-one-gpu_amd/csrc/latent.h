@@ -34,6 +34,11 @@ struct LatentPages {
   }
 };
 
+// 64 lanes x 16 bytes from per-lane addresses to 1 KB of LDS.  Functions of their own, not templates: inside
+// one the host pass of the compiler drops the enclosing kernel without a word.
+AMLA_DEV void copy_lds(const void *src, void *dst) { __builtin_amdgcn_global_load_lds(src, LDS_PTR(dst), 16, 0, 0); }
+AMLA_DEV void copy_lds_nt(const void *src, void *dst) { __builtin_amdgcn_global_load_lds(src, LDS_PTR(dst), 16, 0, 2); }
+
 // Host checks of a cache shared by its entry points: 0 or the code of fail().
 int latent_pages(const amla_latent_cache *c, const char *what, LatentPages *p);
 

@@ -105,129 +105,515 @@ struct SplitPlan {
 // 128), 16-byte chunks permuted within a row so that every fragment read is free of bank
 // conflicts (16 consecutive lanes of a 16-byte read, and the 32 lanes of one pass of a
 // transpose read, differ in address bits 4 - 7), then per row: the exponent as a float
-// (-inf where there is no row), 2^-exponent and the exponent byte.
+// (-inf where there is no row), 2^-exponent and 2^exponent.
 template <bool F8> struct Tile;
 template <> struct Tile<true> {
   static constexpr int ROWS = 64, RB = 512, STAGES = 3;
-  static AMLA_DEV int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8); }
+  static AMLA_DEV constexpr int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8); }
 };
 template <> struct Tile<false> {
   static constexpr int ROWS = 32, RB = 1024, STAGES = 4;
-  static AMLA_DEV int swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+  static AMLA_DEV constexpr int swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
 };
 template <bool F8> struct Stage {
   static constexpr int ROWS = Tile<F8>::ROWS;
-  static constexpr int PE = ROWS * Tile<F8>::RB, EXP = PE + ROWS * 128, INV = EXP + ROWS * 4, BYTE = INV + ROWS * 4;
-  static constexpr int SIZE = BYTE + ROWS * 4;
-  static constexpr int LDS = SIZE * Tile<F8>::STAGES;
+  static constexpr int PE = ROWS * Tile<F8>::RB, EXP = PE + ROWS * 128, INV = EXP + ROWS * 4, MUL = INV + ROWS * 4;
+  static constexpr int SIZE = (MUL + ROWS * 4 + 1023) / 1024 * 1024;  // chunks enter addresses by xor
+  static constexpr int QR = SIZE * Tile<F8>::STAGES;  // e4m3: the rope queries, 4 KB a wave
+  static constexpr int LDS = QR + (F8 ? 4 * 4096 : 0);
 };
 
 // The reference m of a query row's sums moves (a multiplication of all of them) only when a score passes
 // it by 2^40: fp32 and bf16 have the range, and e4m3 has a scale for each block.  m is a whole number.
 constexpr float LAG = 40.f;
+constexpr float M_NONE = -1e30f;  // no row seen yet (finite: 2^(-inf - M_NONE) is 0)
 
-template <int OFS>
-AMLA_DEV u32x4 lds_read16(uint32_t addr) {
+template <int OFS> AMLA_DEV u32x4 lds_read16(uint32_t addr) {
   u32x4 v;
   asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFS) : "memory");
   return v;
 }
-AMLA_DEV u32x4 lds_read16(uint32_t addr) { return lds_read16<0>(addr); }
-AMLA_DEV uint32_t lds_read4(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ds_read_b32 %0, %1" : "=v"(v) : "v"(addr) : "memory");
-  return v;
-}
-AMLA_DEV u32x2 lds_read_tr8(uint32_t addr) {
+template <bool F8, int OFS> AMLA_DEV u32x2 lds_read_tr(uint32_t addr) {
   u32x2 v;
-  asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(v) : "v"(addr) : "memory");
+  if constexpr (F8) asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFS) : "memory");
+  else asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFS) : "memory");
   return v;
 }
-AMLA_DEV u32x2 lds_read_tr16(uint32_t addr) {
-  u32x2 v;
-  asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(v) : "v"(addr) : "memory");
-  return v;
-}
-// Waits until at most N LDS operations are in flight and ties the registers that the wait guards to it.
-template <int N> AMLA_DEV void lds_wait() { asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(N) : "memory"); }
+// Waits until at most N LDS operations are in flight; lds_tie ties registers that a wait guards to it.
+template <int N> AMLA_DEV void lds_wait() { asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(N < 15 ? N : 15) : "memory"); }
 template <typename T, typename... R> AMLA_DEV void lds_tie(T &v, R &...rest) {
   asm volatile("" : "+v"(v)::"memory");
   if constexpr (sizeof...(rest) > 0) lds_tie(rest...);
 }
-template <int N, typename... T> AMLA_DEV void lds_wait(T &...v) {
-  lds_wait<N>();
-  lds_tie(v...);
-}
 
-AMLA_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-AMLA_DEV i32x8 join(u32x4 a, u32x4 b) {
-  return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+// Scores accumulate in vector registers (inline asm): the accumulator registers hold the outputs.  The
+// wait states cover a conversion that wrote the A operand just before.
+AMLA_DEV void mfma_score(f32x16 &c, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
-// A (32 x 64) B (64 x 32) of e4m3 codes, lane l holding 32 codes of row (column) l % 32,
-// each operand times 2^(byte - 127) of the low byte of its scale: codes 0 - 15 of both lanes of a row are
-// one block, scaled by the byte of lane l % 32, codes 16 - 31 the other, by that of lane l % 32 + 32
-AMLA_DEV f32x16 mfma32_f8(i32x8 a, int as, i32x8 b, int bs, f32x16 c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, as, 0, bs);
+AMLA_DEV void mfma_score0(f32x16 &c, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+}
+// Outputs accumulate in accumulator registers that nothing else reads inside the loop.  The wait states
+// cover moves of the operands just before; settle() covers what follows outside the loop.
+AMLA_DEV void mfma_value(f32x16 &c, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+AMLA_DEV i32x8 join(u32x2 a, u32x2 b, u32x2 c, u32x2 d) {
+  return i32x8{(int)a.x, (int)a.y, (int)b.x, (int)b.y, (int)c.x, (int)c.y, (int)d.x, (int)d.y};
+}
+// A (32 x 64) B (64 x 32) of e4m3 codes, lane l holding 32 codes of row (column) l % 32, B times
+// 2^(byte - 127) of the low byte of its scale: codes 0 - 15 of both lanes of a column are one block, scaled
+// by the byte of lane l % 32, codes 16 - 31 the other, by that of lane l % 32 + 32.  one: 127.
+AMLA_DEV void mfma_value(f32x16 &c, i32x8 a, int one, i32x8 b, int bs) {
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+               : "+a"(c) : "v"(a), "v"(b), "v"(one), "v"(bs));
+}
+// Before vector code reads what the asm MFMAs above wrote, and before they read what it wrote.
+template <int N> AMLA_DEV void settle(f32x16 (&o)[N]) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < N; ++c) asm volatile("" : "+a"(o[c]));
 }
 
 AMLA_DEV int pk_fp8x4(float a, float b, float c, float d) {
-  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  // (the first conversion's other half is written by the second: any register will do for it)
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, __float_as_int(a), false);
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
-// x = hi + lo / 16 in e4m3: four values, magnitudes up to 448.  hi keeps the four leading
-// bits, lo the next four, so a bf16 value comes through whole.
+// x = hi + lo / 16 in e4m3, magnitudes up to 256: hi keeps four leading bits, lo the next four
 AMLA_DEV void split_fp8x4(const float *x, int &hi, int &lo) {
   hi = pk_fp8x4(x[0], x[1], x[2], x[3]);
   const f32x2 a = fp8x2_to_f32<false>(hi), b = fp8x2_to_f32<true>(hi);
   lo = pk_fp8x4((x[0] - a.x) * 16.f, (x[1] - a.y) * 16.f, (x[2] - b.x) * 16.f, (x[3] - b.y) * 16.f);
 }
+// Eight codes times a power of two, exact in bf16
+AMLA_DEV bf16x8 codes_to_bf16(uint32_t w0, uint32_t w1, float scale) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+  const bf16x2_t c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+  const bf16x2_t c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+  const bf16x2_t c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+  return bf16x8{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+}
 
-// Copies a wave's rows of a tile, ROWS / 4 from row r0 on, straight into LDS: lane L holds the
-// pool row of row r0 + L % (ROWS / 4) (below 0: row 0 of the pool).
-template <bool F8>
-AMLA_DEV void copy_rows(const LatentPages &pg, uint8_t *st, int r0, int slot) {
-  using T = Tile<F8>;
-  constexpr int WR = T::ROWS / 4;
-  const int lane = threadIdx.x & 63;
-  if constexpr (F8) {
+// ---------------------------------------------------------------- copies
+//
+// A wave copies ROWS / 4 rows of each tile straight into LDS.  `slot` holds the pool row of
+// row L % (ROWS / 4) in lane L, `pe` those of rows 8 i + L / 8 (below 0: row 0 of the pool is
+// copied, its place cleared before use).
+template <bool F8> struct Rows {
+  static constexpr int WR = Tile<F8>::ROWS / 4, NPE = WR / 8, NLAT = F8 ? WR / 2 : WR, COPIES = NLAT + NPE;
+  int slot, pe[NPE];
+  AMLA_DEV void lookup(const LatentPages &pg, int b, int t0, int last) {
+    const int lane = threadIdx.x & 63;
+    slot = pg.slot(b, min(t0 + lane % WR, last));
 #pragma unroll
-    for (int i = 0; i < WR / 2; ++i) {  // two rows of 512 bytes each
-      const int r = 2 * i + (lane >> 5);
-      const size_t s = max(__shfl(slot, r, 64), 0);
-      __builtin_amdgcn_global_load_lds(pg.latent + s * 512 + 16 * ((lane & 31) ^ T::swz(r0 + r)),
-                                       LDS_PTR(st + (r0 + 2 * i) * 512), 16, 0, 2);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < WR; ++i) {
-      const size_t s = max(__shfl(slot, i, 64), 0);
-      __builtin_amdgcn_global_load_lds(pg.latent + s * 1024 + 16 * (lane ^ T::swz(r0 + i)), LDS_PTR(st + (r0 + i) * 1024),
-                                       16, 0, 2);
+    for (int i = 0; i < NPE; ++i) pe[i] = pg.slot(b, min(t0 + 8 * i + (lane >> 3), last));
+  }
+  // The lane's part of the source addresses.  Opaque, so that the compiler forms each copy's address from
+  // it instead of holding ten of them in registers throughout the loop.
+  static AMLA_DEV uint2 lanes(int r0) {
+    const int lane = threadIdx.x & 63;
+    uint32_t lat = F8 ? 16 * ((lane & 31) ^ Tile<F8>::swz(lane >> 5)) : 16 * (lane ^ Tile<F8>::swz(r0 & 15));
+    uint32_t pe = 16 * ((lane & 7) ^ ((r0 >> 1) & 7) ^ (lane >> 4));
+    asm volatile("" : "+v"(lat), "+v"(pe));
+    return uint2{lat, pe};
+  }
+  // copy I (0 .. COPIES - 1) into the stage at st, r0 = first row of the wave in it (a multiple of 8; the swizzles
+  // are xors of bits of the row)
+  template <int I> AMLA_DEV void copy(const LatentPages &pg, uint8_t *st, int r0, uint2 lanes) const {
+    using T = Tile<F8>;
+    const int lane = threadIdx.x & 63;
+    if constexpr (I >= NLAT) {
+      constexpr int k = I - NLAT;
+      copy_lds_nt(reinterpret_cast<const uint8_t *>(pg.k_pe) + (size_t)max(pe[k], 0) * 128 + (lanes.y ^ (64 * k)),
+                  st + Stage<F8>::PE + (r0 + 8 * k) * 128);
+    } else if constexpr (F8) {  // two rows of 512 bytes
+      const int s0 = __builtin_amdgcn_readlane(slot, 2 * I), s1 = __builtin_amdgcn_readlane(slot, 2 * I + 1);
+      const int s = max(lane < 32 ? s0 : s1, 0);
+      copy_lds_nt(pg.latent + (size_t)s * 512 + (lanes.x ^ (16 * T::swz(2 * I))), st + (r0 + 2 * I) * 512);
+    } else {
+      const size_t s = max(__builtin_amdgcn_readlane(slot, I), 0);
+      copy_lds_nt(pg.latent + s * 1024 + (lanes.x ^ (16 * T::swz(I))), st + (r0 + I) * 1024);
     }
   }
-#pragma unroll
-  for (int i = 0; i < WR / 8; ++i) {
-    const int r = 8 * i + (lane >> 3);
-    const size_t s = max(__shfl(slot, r, 64), 0);
-    __builtin_amdgcn_global_load_lds(pg.k_pe + s * 64 + 8 * ((lane & 7) ^ (((r0 + r) >> 1) & 7)),
-                                     LDS_PTR(st + Stage<F8>::PE + (r0 + 8 * i) * 128), 16, 0, 2);
+};
+template <bool F8, int I = 0> AMLA_DEV void copy_all(const Rows<F8> &rows, const LatentPages &pg, uint8_t *st, int r0) {
+  if constexpr (I < Rows<F8>::COPIES) {
+    rows.template copy<I>(pg, st, r0, Rows<F8>::lanes(r0));
+    copy_all<F8, I + 1>(rows, pg, st, r0);
   }
 }
+
+// ---------------------------------------------------------------- the two phases of a tile
+
+template <bool F8, int HG> struct Wave {
+  static constexpr int KB = Tile<F8>::ROWS / 32;  // 32-row blocks of a tile
+  static constexpr int CG = 4 / HG, NCB = 16 / CG;
+  bf16x8 q[32], qr[F8 ? 1 : 4];  // e4m3: the rope queries lie in LDS at qra, 1 KB a fragment
+  uint32_t qra;
+  f32x16 o[NCB];  // O^T: columns x queries
+  f32x16 s[2];    // S^T of the tile in work: rows x queries (bf16: two chains of the one block)
+  i32x8 phi, plo; // P of the tile before it: e4m3 halves and their scale,
+  int ps, ps_lo, one;
+  u32x4 pb[2];    // or bf16
+  float m, l;
+};
+
+// Reads of score step I: two fragments, one of each chain of MFMAs.
+template <bool F8, int I> AMLA_DEV void score_read(u32x4 (&d)[3], uint32_t kl, uint32_t kr, uint32_t qra) {
+  constexpr int RB = Tile<F8>::RB;
+  if constexpr (I >= 16) {  // the rope key, 16 columns a step: of rows j32, 32 + j32, or two steps of one row
+    constexpr int ks = I - 16;
+    d[0] = lds_read16<0>(kr ^ (F8 ? 32 * ks : 64 * ks));
+    d[1] = F8 ? lds_read16<32 * 128>(kr ^ (32 * ks)) : lds_read16<0>(kr ^ (64 * ks + 32));
+    if constexpr (F8) d[2] = lds_read16<1024 * ks>(qra);
+  } else if constexpr (F8) {  // codes 32 I + 16 hh .. + 15 of rows j32, 32 + j32
+    d[0] = lds_read16<256 * (I >> 3)>(kl ^ (32 * (I & 7)));
+    d[1] = lds_read16<256 * (I >> 3) + 32 * RB>(kl ^ (32 * (I & 7)));
+  } else {  // values 32 I + 8 hh .. + 7, and those 16 on
+    d[0] = lds_read16<256 * (I >> 2)>(kl ^ (32 * ((2 * I) & 7)));
+    d[1] = lds_read16<256 * (I >> 2)>(kl ^ (32 * ((2 * I + 1) & 7)));
+  }
+}
+
+template <bool F8> constexpr int score_reads(int i) { return i >= 16 + (F8 ? 4 : 2) ? 0 : F8 && i >= 16 ? 3 : 2; }
+constexpr int SCORE_AHEAD = 2;  // steps that reads go out ahead
+
+template <bool F8, int HG, int I>
+AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint32_t kl, uint32_t kr, float &f0, float &f1,
+                         uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
+  constexpr int N = 16 + (F8 ? 4 : 2);  // steps over the latent and the rope key
+  if constexpr (I < N) {
+    constexpr int c = I % (SCORE_AHEAD + 1);
+    if constexpr (I + SCORE_AHEAD < N) score_read<F8, I + SCORE_AHEAD>(ka[(I + SCORE_AHEAD) % (SCORE_AHEAD + 1)], kl, kr, w.qra);
+    lds_wait<score_reads<F8>(I + 1) + score_reads<F8>(I + 2)>();
+    lds_tie(ka[c][0], ka[c][1]);
+    if constexpr (F8 && I >= 16) lds_tie(ka[c][2]);
+    if constexpr (I == 0) lds_tie(f0, f1);
+    if constexpr (I >= 16) {
+      constexpr int k0 = F8 ? I - 16 : 2 * (I - 16), k1 = F8 ? k0 : k0 + 1;
+      mfma_score(w.s[0], as_bf16x8(ka[c][0]), F8 ? as_bf16x8(ka[c][2]) : w.qr[F8 ? 0 : k0]);
+      mfma_score(w.s[1], as_bf16x8(ka[c][1]), F8 ? as_bf16x8(ka[c][2]) : w.qr[F8 ? 0 : k1]);
+    } else if constexpr (F8) {
+      const u32x4 x = ka[c][0], y = ka[c][1];
+      const bf16x8 x0 = codes_to_bf16(x.x, x.y, f0), y0 = codes_to_bf16(y.x, y.y, f1);
+      const bf16x8 x1 = codes_to_bf16(x.z, x.w, f0), y1 = codes_to_bf16(y.z, y.w, f1);
+      if constexpr (I == 0) {
+        mfma_score0(w.s[0], x0, w.q[0]);
+        mfma_score0(w.s[1], y0, w.q[0]);
+      } else {
+        mfma_score(w.s[0], x0, w.q[2 * I]);
+        mfma_score(w.s[1], y0, w.q[2 * I]);
+      }
+      mfma_score(w.s[0], x1, w.q[2 * I + 1]);
+      mfma_score(w.s[1], y1, w.q[2 * I + 1]);
+    } else if constexpr (I == 0) {
+      mfma_score0(w.s[0], as_bf16x8(ka[c][0]), w.q[0]);
+      mfma_score0(w.s[1], as_bf16x8(ka[c][1]), w.q[1]);
+    } else {
+      mfma_score(w.s[0], as_bf16x8(ka[c][0]), w.q[2 * I]);
+      mfma_score(w.s[1], as_bf16x8(ka[c][1]), w.q[2 * I + 1]);
+    }
+    if constexpr (I > 0 && I <= Rows<F8>::COPIES) next.template copy<I - 1>(pg, st_next, r0, lanes);
+    __builtin_amdgcn_sched_barrier(0);
+    score_step<F8, HG, I + 1>(w, ka, kl, kr, f0, f1, lanes, next, pg, st_next, r0);
+  }
+}
+
+// S^T of the tile whose stage is at LDS address base, with the copies of a later tile spread between.
+// Two chains of MFMAs: one alone runs at two thirds of the rate.
+template <bool F8, int HG>
+AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next,
+                          int r0) {
+  using T = Tile<F8>;
+  using G = Stage<F8>;
+  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
+  // the lane's row and first chunk; chunk c sits at c ^ swz(row): bits 1 .. 3 of c enter by xor, higher ones by offset
+  const uint32_t kl = base + j32 * T::RB + 16 * (hh ^ T::swz(j32));
+  const uint32_t kr = base + G::PE + j32 * 128 + 16 * (hh ^ ((j32 >> 1) & 7));
+  float f0 = 1.f, f1 = 1.f;
+  if constexpr (F8) {  // 2^exponent of rows j32 and 32 + j32
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f0) : "v"(base + 4 * j32), "i"(G::MUL) : "memory");
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f1) : "v"(base + 4 * j32), "i"(G::MUL + 128) : "memory");
+  }
+  u32x4 ka[SCORE_AHEAD + 1][3];
+  score_read<F8, 0>(ka[0], kl, kr, w.qra);
+  score_read<F8, 1>(ka[1], kl, kr, w.qra);
+  score_step<F8, HG, 0>(w, ka, kl, kr, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
+  // the results are read by vector code that the compiler schedules: cover the asm's write-to-read wait states
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  asm volatile("" : "+v"(w.s[0]), "+v"(w.s[1]));
+}
+
+// The second phase of a tile goes in steps of one 32-column block of the values; each carries some of the
+// slices (four rows) of the softmax: first all scaled scores and their maxima, then the probabilities.
+template <bool F8, int HG> struct Slices {
+  static constexpr int KB = Wave<F8, HG>::KB, NCB = Wave<F8, HG>::NCB, NZ = 4 * KB, NS = 8 * KB;
+  static constexpr int PER = (NS + NCB - 1) / NCB;
+  static constexpr int first(int c) { return (c * NS + NCB - 1) / NCB; }
+  static constexpr int reads(int c) {  // row factors read for step c: bf16's probabilities need none
+    if (c >= NCB) return 0;
+    int n = 0;
+    for (int s = first(c); s < first(c + 1); ++s) n += s < NZ || F8;
+    return n;
+  }
+};
+template <bool F8, int HG> struct StepReads {
+  u32x2 v[4];
+  u32x4 ex[Slices<F8, HG>::PER];
+};
+template <bool F8, int HG> struct ValueState {
+  static constexpr int KB = Wave<F8, HG>::KB;
+  uint32_t v0, v1, eb;
+  float scale_log2;
+  int lim;  // MASK: rows of the tile below lim are seen by the lane's query
+  float mx[KB], ref[KB], sum[KB], mn, f;
+  bool moved;
+  i32x8 phi, plo;
+  u32x4 pb[2];
+  StepReads<F8, HG> rd[3];
+};
+
+template <bool F8, int HG, int S, int END> AMLA_DEV void slice_read(ValueState<F8, HG> &x, u32x4 *ex) {
+  using G = Stage<F8>;
+  using L = Slices<F8, HG>;
+  if constexpr (S < END) {
+    constexpr int t = S % L::NZ;
+    if constexpr (S < L::NZ || F8) ex[0] = lds_read16<(S < L::NZ ? G::EXP : G::INV) + 4 * (32 * (t >> 2) + 8 * (t & 3))>(x.eb);
+    slice_read<F8, HG, S + 1, END>(x, ex + 1);
+  }
+}
+template <bool F8, int HG, bool PV, bool ZP, int C> AMLA_DEV void value_read(ValueState<F8, HG> &x) {
+  using L = Slices<F8, HG>;
+  if constexpr (C < L::NCB) {
+    StepReads<F8, HG> &r = x.rd[C % 3];
+    if constexpr (PV && F8) {
+      const uint32_t a = x.v0 ^ (32 * (C & 7));
+      r.v[0] = lds_read_tr<F8, 256 * (C >> 3)>(a);
+      r.v[1] = lds_read_tr<F8, 256 * (C >> 3) + 8192>(a);
+      r.v[2] = lds_read_tr<F8, 256 * (C >> 3) + 16384>(a);
+      r.v[3] = lds_read_tr<F8, 256 * (C >> 3) + 24576>(a);
+    } else if constexpr (PV) {
+      const uint32_t a = x.v0 ^ (64 * (C & 3)), b = x.v1 ^ (64 * (C & 3));
+      r.v[0] = lds_read_tr<F8, 256 * (C >> 2)>(a);
+      r.v[1] = lds_read_tr<F8, 256 * (C >> 2)>(b);
+      r.v[2] = lds_read_tr<F8, 256 * (C >> 2) + 16384>(a);
+      r.v[3] = lds_read_tr<F8, 256 * (C >> 2) + 16384>(b);
+    }
+    if constexpr (ZP) slice_read<F8, HG, L::first(C), L::first(C + 1)>(x, r.ex);
+  }
+}
+
+// Slice S of the softmax, its row factors in ex:
+//   z = s log2(e) scale + exponent of the row, P = 2^(z - ref), l sums 2^(s - m) = P 2^(ref - m - exponent)
+// e4m3: 32 rows are one block of the matrix unit with a scale of its own, 2^(ref - m), so that rows far
+// below the sequence's maximum keep their bits: a reference for all would drop those below 2^-22 of it,
+// and thousands of them can outweigh it.
+template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 ex) {
+  using L = Slices<F8, HG>;
+  constexpr int KB = L::KB, t = S % L::NZ, kb = t >> 2, q4 = t & 3;
+  f32x16 &z = w.s[kb];
+  if constexpr (S < L::NZ) {
+    if constexpr (q4 == 0) x.mx[kb] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float sc = F8 ? z[4 * q4 + i] : z[4 * q4 + i] + w.s[1][4 * q4 + i];
+      z[4 * q4 + i] = __builtin_fmaf(sc, x.scale_log2, __uint_as_float(ex[i]));
+    }
+    if constexpr (MASK) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[4 * q4 + i] = 32 * kb + 8 * q4 + i < x.lim ? z[4 * q4 + i] : -INFINITY;
+    }
+    x.mx[kb] = __builtin_fmaxf(__builtin_fmaxf(x.mx[kb], z[4 * q4]), z[4 * q4 + 1]);
+    x.mx[kb] = __builtin_fmaxf(__builtin_fmaxf(x.mx[kb], z[4 * q4 + 2]), z[4 * q4 + 3]);
+    if constexpr (S == L::NZ - 1) {
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x.mx[k]), __float_as_uint(x.mx[k]), false, false);
+        x.mx[k] = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+      }
+      const float top = __builtin_fmaxf(x.mx[0], x.mx[KB - 1]);
+      x.moved = top > w.m + LAG;
+      x.mn = x.moved ? ceilf(top) : w.m;
+      x.f = __builtin_amdgcn_exp2f(w.m - x.mn);
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        x.ref[k] = F8 ? floorf(__builtin_fmaxf(x.mx[k], M_NONE)) - 7.f : x.mn;
+        x.sum[k] = 0.f;
+      }
+    }
+  } else {
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(z[4 * q4 + i] - x.ref[kb]);
+    if constexpr (F8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.sum[kb] = __builtin_fmaf(e[i], __uint_as_float(ex[i]), x.sum[kb]);
+      int hi, lo;
+      split_fp8x4(e, hi, lo);
+      x.phi[4 * kb + q4] = hi;
+      x.plo[4 * kb + q4] = lo;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.sum[kb] += e[i];
+      x.pb[q4 >> 1][2 * (q4 & 1)] = pack_bf16(e[0], e[1]);
+      x.pb[q4 >> 1][2 * (q4 & 1) + 1] = pack_bf16(e[2], e[3]);
+    }
+  }
+}
+template <bool F8, int HG, bool MASK, int S, int END>
+AMLA_DEV void softmax_slices(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 *ex) {
+  if constexpr (S < END) {
+    if constexpr (S < Slices<F8, HG>::NZ || F8) lds_tie(ex[0]);
+    softmax_slice<F8, HG, MASK, S>(w, x, ex[0]);
+    softmax_slices<F8, HG, MASK, S + 1, END>(w, x, ex + 1);
+  }
+}
+
+template <bool F8, int HG, bool MASK, bool PV, bool ZP, int C>
+AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
+  using L = Slices<F8, HG>;
+  if constexpr (C < L::NCB) {
+    StepReads<F8, HG> &r = x.rd[C % 3];
+    value_read<F8, HG, PV, ZP, C + 2>(x);
+    // this step's reads have landed: those of the next two steps may be in flight
+    lds_wait<(PV ? 4 * ((C + 1 < L::NCB) + (C + 2 < L::NCB)) : 0) + (ZP ? L::reads(C + 1) + L::reads(C + 2) : 0)>();
+    if constexpr (PV) {
+      lds_tie(r.v[0], r.v[1], r.v[2], r.v[3]);
+      if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.phi, w.ps);
+      else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[0].x, r.v[0].y, r.v[1].x, r.v[1].y}), as_bf16x8(w.pb[0]));
+    }
+    if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r.ex);
+    if constexpr (PV) {
+      if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.plo, w.ps_lo);
+      else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[2].x, r.v[2].y, r.v[3].x, r.v[3].y}), as_bf16x8(w.pb[1]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    value_step<F8, HG, MASK, PV, ZP, C + 1>(w, x);
+  }
+}
+
+// O^T += C^T P^T of the tile before (its stage at pv) while the scores of this tile (stage at zb) become
+// probabilities.  Returns the factor that O has to be multiplied by before the next tile's turn, and
+// whether any lane's is not 1.
+template <bool F8, int HG, bool MASK, bool PV, bool ZP>
+AMLA_DEV bool value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, float scale_log2, int lim, float &f) {
+  using T = Tile<F8>;
+  using L = Slices<F8, HG>;
+  constexpr int KB = L::KB, NCB = L::NCB;
+  const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+  ValueState<F8, HG> x;
+  if constexpr (F8) {  // rows 16 i + 4 hh + {0..3, 8..11} of 16 columns
+    const int r = 8 * (L16 >> 3) + 4 * hh + ((L16 >> 1) & 3);
+    x.v0 = pv + r * T::RB + 16 * ((g16 & 1) ^ T::swz(r)) + 8 * (L16 & 1);
+    x.v0 = (x.v0 ^ (32 * ((NCB * cg) & 7))) + 256 * ((NCB * cg) >> 3);
+  } else {   // rows 16 kk + 8 i + 4 hh + 0..3
+    const int r = 4 * hh + (L16 >> 2), ch = 2 * (g16 & 1) + ((L16 >> 1) & 1);
+    x.v0 = pv + r * T::RB + 16 * (ch ^ T::swz(r)) + 8 * (L16 & 1) + 256 * ((NCB * cg) >> 2);
+    x.v1 = pv + (r + 8) * T::RB + 16 * (ch ^ T::swz(r + 8)) + 8 * (L16 & 1) + 256 * ((NCB * cg) >> 2);
+  }
+  x.eb = zb + 16 * hh;
+  x.scale_log2 = scale_log2;
+  x.lim = lim;
+  value_read<F8, HG, PV, ZP, 0>(x);
+  value_read<F8, HG, PV, ZP, 1>(x);
+  value_step<F8, HG, MASK, PV, ZP, 0>(w, x);
+  if constexpr (ZP) {
+    f = x.f;
+    w.m = x.mn;
+    w.l *= f;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) w.l += F8 ? x.sum[k] * __builtin_amdgcn_exp2f(x.ref[k] - w.m) : x.sum[k];
+    // the scale of block k comes from the lanes of half k; 4 .. 160, the low halves' 4 less
+    if constexpr (F8) {
+      w.ps = (int)__builtin_fmaxf((hh ? x.ref[KB - 1] : x.ref[0]) - w.m, -123.f) + 127;
+      w.ps_lo = w.ps - 4;
+    }
+    w.phi = x.phi;
+    w.plo = x.plo;
+    w.pb[0] = x.pb[0];
+    w.pb[1] = x.pb[1];
+    return __ballot(x.moved) != 0;
+  }
+  return false;
+}
+
+// The copies of a split: which rows of the pool a wave brings, and what is known of those under way.
+template <bool F8> struct Feed {
+  static constexpr int TILE = Tile<F8>::ROWS, NST = Tile<F8>::STAGES, PD = NST - 2;  // a tile, the one before it, PD to come
+  static constexpr int WR = Rows<F8>::WR, COPIES = Rows<F8>::COPIES;
+  const LatentPages &pg;
+  uint8_t *sm;
+  int b, wave, held, last, cur;  // last: rows past it are copied from it (and have no part in anything)
+  Rows<F8> rows[PD + 1];         // [0]: the tile in work, [PD]: the next to go out
+  int byte[PD + 1];
+
+  AMLA_DEV void start(int t_first) {
+    cur = 0;
+#pragma unroll
+    for (int d = 0; d <= PD; ++d) {
+      rows[d].lookup(pg, b, (t_first + d) * TILE + WR * wave, last);
+      byte[d] = 127;
+      if (d < PD) {
+        if constexpr (F8) byte[d] = pg.scales[max(rows[d].slot, 0)];
+        copy_all<F8>(rows[d], pg, sm + d * Stage<F8>::SIZE, WR * wave);
+      }
+    }
+  }
+  // The rows of tile `tile` have landed in every wave, their factors beside them.
+  AMLA_DEV void arrive(int tile) {
+    using G = Stage<F8>;
+    constexpr int RB = Tile<F8>::RB;
+    const int lane = threadIdx.x & 63;
+    wait_vmcnt<(PD - 1) * COPIES>();
+    uint8_t *st = sm + cur * G::SIZE;
+    // rows of no page: zeros in place of what was copied (a NaN there would come through 0 * NaN)
+    const bool none = lane < WR && rows[0].slot < 0;
+    for (uint64_t bad = __ballot(none); bad; bad &= bad - 1) {
+      const int r = WR * wave + __builtin_ctzll(bad);
+      for (int i = lane; i < RB / 16; i += 64) *reinterpret_cast<u32x4 *>(st + r * RB + 16 * i) = u32x4{0, 0, 0, 0};
+      if (lane < 8) *reinterpret_cast<u32x4 *>(st + G::PE + r * 128 + 16 * lane) = u32x4{0, 0, 0, 0};
+    }
+    if (lane < WR) {
+      const int r = WR * wave + lane, by = none ? 127 : byte[0];
+      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = none || tile * TILE + r >= held ? -INFINITY : (float)(by - 127);
+      if constexpr (F8) {
+        *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = (uint32_t)(254 - by) << 23;
+        *reinterpret_cast<uint32_t *>(st + G::MUL + 4 * r) = by == 255 ? 0x7fc00000u : (uint32_t)by << 23;
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if constexpr (F8) byte[PD] = pg.scales[max(rows[PD].slot, 0)];
+  }
+  AMLA_DEV uint8_t *next_stage() const { return sm + (cur + PD) % NST * Stage<F8>::SIZE; }
+  // After the copies of tile + PD went out
+  AMLA_DEV void advance(int tile) {
+#pragma unroll
+    for (int d = 0; d < PD; ++d) {
+      rows[d] = rows[d + 1];
+      byte[d] = byte[d + 1];
+    }
+    rows[PD].lookup(pg, b, (tile + PD + 1) * TILE + WR * wave, last);
+    cur = cur + 1 == NST ? 0 : cur + 1;
+  }
+};
 
 // One workgroup of four waves per (sequence, chunk of 32 HG rows, split).  HG waves hold 32
 // query rows each; the 4 / HG waves of the same rows compute the same scores and
 // accumulate 512 HG / 4 columns each.
-template <bool F8, int HG>
+template <bool F8, int HG, bool MASK>
 __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p) {
-  extern __shared__ __align__(16) uint8_t sm[];
+  extern __shared__ __align__(1024) uint8_t sm[];
   using T = Tile<F8>;
   using G = Stage<F8>;
-  constexpr int TILE = T::ROWS, NST = T::STAGES, PD = NST - 1;
-  constexpr int CG = 4 / HG, NCB = 16 / CG;  // 32-column blocks of a wave
-  constexpr int KB = TILE / 32;              // 32-row blocks of a tile
-  constexpr int WR = TILE / 4;               // rows that a wave copies
+  using W = Wave<F8, HG>;
+  constexpr int TILE = T::ROWS, CG = W::CG, NCB = W::NCB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j32 = lane & 31, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+  const int j32 = lane & 31, hh = lane >> 5;
   const int hg = wave / CG, cg = wave % CG;
 
   const SplitPlan<TILE> plan(p);
@@ -235,250 +621,76 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   if (at.x < 0) return;
   const int b = at.x, splits = at.z;
   const int chunk = ((int)blockIdx.x - at.y) / splits, split = ((int)blockIdx.x - at.y) % splits;
-  const int rows_held = min(max(p.lengths[b], 0), p.cap);
+  const int rows_held = __builtin_amdgcn_readfirstlane(min(max(p.lengths[b], 0), p.cap));
   const int n_tiles = lc_ceil_div(rows_held, TILE);
   const int t_first = (int)((int64_t)split * n_tiles / splits), t_end = (int)((int64_t)(split + 1) * n_tiles / splits);
-
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
 
-  const int my_row = WR * wave + lane % WR;
-  int slot_of[PD], byte_of[PD];
-#pragma unroll
-  for (int d = 0; d < PD; ++d) {
-    slot_of[d] = -1;
-    byte_of[d] = 127;
-    if (t_first + d < t_end) {
-      slot_of[d] = p.pg.slot(b, min((t_first + d) * TILE + my_row, rows_held - 1));
-      if (F8) byte_of[d] = p.pg.scales[max(slot_of[d], 0)];
-      copy_rows<F8>(p.pg, sm + d * G::SIZE, WR * wave, slot_of[d]);
-    }
-  }
+  Feed<F8> feed{p.pg, sm, b, wave, rows_held, min(rows_held, t_end * TILE) - 1};
+  feed.start(t_first);
 
-  // ---- queries: B fragments, lane = row of the chunk
+  // queries: B fragments, lane = row of the chunk, in the order of the score steps' reads
+  W w;
   const int row = (chunk * HG + hg) * 32 + j32;
   const int rq = min(row, p.rows - 1), tok = rq / p.heads;
-  const int limit = rows_held - (p.seq_len - 1 - tok);  // rows [0, limit) are seen
+  const int limit = rows_held - (p.seq_len - 1 - tok) - 4 * hh;  // rows [0, limit + 4 hh) are seen
   const uint16_t *qp = p.q + b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
-  constexpr int QN = F8 ? 8 : 32;
-  i32x8 qhi[F8 ? QN : 1], qlo[F8 ? QN : 1];
-  bf16x8 qb[F8 ? 1 : QN], qr[4];
-  int qs = 127;
-  if constexpr (F8) {
-    u32x4 raw[QN][4];
-    uint32_t amax = 0;
 #pragma unroll
-    for (int ks = 0; ks < QN; ++ks)
+  for (int i = 0; i < 32; ++i)
+    w.q[i] = as_bf16x8(ldg16(qp + (F8 ? 32 * (i >> 1) + 16 * hh + 8 * (i & 1) : 16 * i + 8 * hh)));
+  w.qra = lds0 + G::QR + 4096 * wave + 16 * lane;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        raw[ks][c] = ldg16(qp + 64 * ks + 32 * hh + 8 * c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          amax = max(amax, max((raw[ks][c][e] << 16) & 0x7fffffffu, raw[ks][c][e] & 0x7fff0000u));
-      }
-    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
-    // the exponent that brings the row's largest magnitude into [128, 256)
-    const int e = min(max((int)(amax >> 23) - 127 - 7, -100), 100);
-    qs = 127 + e;
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int ks = 0; ks < QN; ++ks)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = raw[ks][c][2 * h], w1 = raw[ks][c][2 * h + 1];
-          const float x[4] = {lo_bf(w0) * inv, hi_bf(w0) * inv, lo_bf(w1) * inv, hi_bf(w1) * inv};
-          int hi, lo;
-          split_fp8x4(x, hi, lo);
-          qhi[ks][2 * c + h] = hi;
-          qlo[ks][2 * c + h] = lo;
-        }
-  } else {
-#pragma unroll
-    for (int ks = 0; ks < QN; ++ks) qb[ks] = as_bf16x8(ldg16(qp + 16 * ks + 8 * hh));
+  for (int i = 0; i < 4; ++i) {
+    const u32x4 v = ldg16(qp + LC_LORA + 16 * i + 8 * hh);
+    if constexpr (F8) *reinterpret_cast<u32x4 *>(sm + G::QR + 4096 * wave + 1024 * i + 16 * lane) = v;  // (the wave's own)
+    else w.qr[i] = as_bf16x8(v);
   }
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) qr[ks] = as_bf16x8(ldg16(qp + LC_LORA + 16 * ks + 8 * hh));
-
-  f32x16 o[NCB];
 #pragma unroll
   for (int c = 0; c < NCB; ++c)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
-  float m = -1e30f, l = 0.f;  // finite: exp2(-inf - m) is 0 while no row has been seen
+    for (int i = 0; i < 16; ++i) w.o[c][i] = 0.f;
+  settle(w.o);
+  w.m = M_NONE;
+  w.l = 0.f;
+  w.one = 127;
 
-  int cur = 0;
-  for (int tile = t_first; tile < t_end; ++tile, cur = cur + 1 == NST ? 0 : cur + 1) {
-    // ---- this tile's rows have landed in every wave
-    if (tile + PD - 1 < t_end) wait_vmcnt<(PD - 1) * (F8 ? WR / 2 + WR / 8 : WR + WR / 8)>();
-    else wait_vmcnt<0>();
-    uint8_t *st = sm + cur * G::SIZE;
-    {
-      // rows of no page: zeros in place of what the copy clamped to (a masked NaN would come through 0 * NaN)
-      const int sl = slot_of[0], t = tile * TILE + WR * wave + lane;
-      const bool none = lane < WR && sl < 0;
-      for (uint64_t bad = __ballot(none); bad; bad &= bad - 1) {
-        const int r = WR * wave + __builtin_ctzll(bad);
-        for (int i = lane; i < T::RB / 16; i += 64) *reinterpret_cast<u32x4 *>(st + r * T::RB + 16 * i) = u32x4{0, 0, 0, 0};
-        if (lane < 8) *reinterpret_cast<u32x4 *>(st + G::PE + r * 128 + 16 * lane) = u32x4{0, 0, 0, 0};
-      }
-      if (lane < WR) {
-        const int r = WR * wave + lane, by = none ? 127 : byte_of[0];
-        *reinterpret_cast<float *>(st + G::EXP + 4 * r) = none || t >= rows_held ? -INFINITY : (float)(by - 127);
-        *reinterpret_cast<float *>(st + G::INV + 4 * r) = __uint_as_float((uint32_t)(254 - by) << 23);
-        *reinterpret_cast<int *>(st + G::BYTE + 4 * r) = by;
-      }
+  float f;
+  int tile = t_first;
+  uint32_t base = lds0;
+  feed.arrive(tile);
+  score_phase<F8, HG>(w, base, feed.rows[Feed<F8>::PD], p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+  feed.advance(tile);
+  value_phase<F8, HG, MASK, false, true>(w, base, base, cg, p.scale_log2, limit - tile * TILE, f);  // O is still 0
+  for (++tile;;) {
+    bool moved = false;
+    while (tile < t_end && !moved) {
+      const uint32_t before = base;
+      feed.arrive(tile);
+      base = lds0 + feed.cur * G::SIZE;
+      score_phase<F8, HG>(w, base, feed.rows[Feed<F8>::PD], p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+      feed.advance(tile);
+      moved = value_phase<F8, HG, MASK, true, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE, f);
+      ++tile;
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int d = 0; d + 1 < PD; ++d) {
-      slot_of[d] = slot_of[d + 1];
-      byte_of[d] = byte_of[d + 1];
-    }
-    if (tile + PD < t_end) {
-      slot_of[PD - 1] = p.pg.slot(b, min((tile + PD) * TILE + my_row, rows_held - 1));
-      if (F8) byte_of[PD - 1] = p.pg.scales[max(slot_of[PD - 1], 0)];
-      copy_rows<F8>(p.pg, sm + (cur + PD) % NST * G::SIZE, WR * wave, slot_of[PD - 1]);
-    }
-
-    // ---- scores: S^T (rows x 32 queries)
-    const uint32_t base = lds0 + cur * G::SIZE;
-    f32x16 s[KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const int r = 32 * kb + j32, sw = T::swz(r);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-      if constexpr (F8) {
-        uint32_t ab = lds_read4(base + G::BYTE + 4 * r);
-        lds_wait<0>(ab);
-#pragma unroll
-        for (int ks = 0; ks < QN; ++ks) {
-          u32x4 a0 = lds_read16(base + r * 512 + 16 * ((4 * ks + 2 * hh) ^ sw));
-          u32x4 a1 = lds_read16(base + r * 512 + 16 * ((4 * ks + 2 * hh + 1) ^ sw));
-          lds_wait<0>(a0, a1);
-          const i32x8 a = join(a0, a1);
-          s[kb] = mfma32_f8(a, (int)ab, qhi[ks], qs, s[kb]);
-          s[kb] = mfma32_f8(a, (int)ab, qlo[ks], qs - 4, s[kb]);
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < QN; ++ks) {
-          u32x4 a = lds_read16(base + r * 1024 + 16 * ((2 * ks + hh) ^ sw));
-          lds_wait<0>(a);
-          s[kb] = mfma32(as_bf16x8(a), qb[ks], s[kb]);
-        }
-      }
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        u32x4 a = lds_read16(base + G::PE + r * 128 + 16 * ((2 * ks + hh) ^ ((r >> 1) & 7)));
-        lds_wait<0>(a);
-        s[kb] = mfma32(as_bf16x8(a), qr[ks], s[kb]);
-      }
-    }
-    // ---- z = s log2(e) scale + exponent
-    float mx[KB];  // of 32 rows
-    const bool tail = (tile + 1) * TILE > rows_held - (p.seq_len - 1);
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      mx[kb] = -INFINITY;
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        u32x4 ex = lds_read16(base + G::EXP + 4 * (32 * kb + 8 * q4 + 4 * hh));
-        lds_wait<0>(ex);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float z = __builtin_fmaf(s[kb][4 * q4 + i], p.scale_log2, __uint_as_float(ex[i]));
-          if (tail && tile * TILE + 32 * kb + 8 * q4 + 4 * hh + i >= limit) z = -INFINITY;
-          s[kb][4 * q4 + i] = z;
-          mx[kb] = __builtin_fmaxf(mx[kb], z);
-        }
-      }
-      mx[kb] = __builtin_fmaxf(mx[kb], __shfl_xor(mx[kb], 32, 64));
-    }
-    const float top = __builtin_fmaxf(mx[0], mx[KB - 1]);
-    if (__ballot(top > m + LAG)) {
-      const float mn = top > m + LAG ? ceilf(top) : m;
-      const float f = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int c = 0; c < NCB; ++c) o[c] *= f;
-    }
-    // ---- P = 2^(z - ref); l sums 2^(s - m) = P 2^(ref - m) 2^-exponent
-    // e4m3: 32 rows are one block of the matrix unit with a scale of its own, 2^(ref - m), so that rows far
-    // below the sequence's maximum keep their bits: a reference for all would drop those below 2^-22 of
-    // it, and thousands of them can outweigh it.
-    float ref[KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) ref[kb] = F8 ? floorf(__builtin_fmaxf(mx[kb], -1e30f)) - 7.f : m;
-    i32x8 phi, plo;
-    u32x4 pb[2];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      float sum = 0.f;
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(s[kb][4 * q4 + i] - ref[kb]);
-        if constexpr (F8) {
-          u32x4 iv = lds_read16(base + G::INV + 4 * (32 * kb + 8 * q4 + 4 * hh));
-          lds_wait<0>(iv);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(e[i], __uint_as_float(iv[i]), sum);
-          int hi, lo;
-          split_fp8x4(e, hi, lo);
-          phi[4 * kb + q4] = hi;
-          plo[4 * kb + q4] = lo;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum += e[i];
-          pb[q4 >> 1][2 * (q4 & 1)] = pack_bf16(e[0], e[1]);
-          pb[q4 >> 1][2 * (q4 & 1) + 1] = pack_bf16(e[2], e[3]);
-        }
-      }
-      l += F8 ? sum * __builtin_amdgcn_exp2f(ref[kb] - m) : sum;
-    }
-    // the scale of block kb comes from the lanes of half kb; 4 .. 160, the low halves' 4 less
-    const int ps = (int)__builtin_fmaxf((hh ? ref[KB - 1] : ref[0]) - m, -123.f) + 127;
-    // ---- O^T (columns x queries) += C^T P^T
+    if (!moved) break;
+    // the multiplication of O stays outside the loop that holds O in accumulator registers
+    settle(w.o);
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
-      const int cb = cg * NCB + c;
-      if constexpr (F8) {
-        u32x2 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // rows 16 i + 4 hh + {0..3, 8..11}
-          const int r = 16 * i + 8 * (L16 >> 3) + 4 * hh + ((L16 >> 1) & 3);
-          v[i] = lds_read_tr8(base + r * 512 + 16 * ((2 * cb + (g16 & 1)) ^ T::swz(r)) + 8 * (L16 & 1));
-        }
-        lds_wait<0>(v[0], v[1], v[2], v[3]);
-        const i32x8 a = join(u32x4{v[0].x, v[0].y, v[1].x, v[1].y}, u32x4{v[2].x, v[2].y, v[3].x, v[3].y});
-        o[c] = mfma32_f8(a, 127, phi, ps, o[c]);
-        o[c] = mfma32_f8(a, 127, plo, ps - 4, o[c]);
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          u32x2 v[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = 16 * kk + 8 * i + 4 * hh + (L16 >> 2);
-            v[i] = lds_read_tr16(base + r * 1024 + 16 * ((4 * cb + 2 * (g16 & 1) + ((L16 >> 1) & 1)) ^ T::swz(r)) + 8 * (L16 & 1));
-          }
-          lds_wait<0>(v[0], v[1]);
-          o[c] = mfma32(as_bf16x8(u32x4{v[0].x, v[0].y, v[1].x, v[1].y}), as_bf16x8(pb[kk]), o[c]);
-        }
-      }
+      w.o[c] *= f;
+      asm volatile("" : "+a"(w.o[c]));
     }
+    settle(w.o);
   }
+  value_phase<F8, HG, MASK, true, false>(w, base, base, cg, p.scale_log2, 0, f);
+  settle(w.o);
+  wait_vmcnt<0>();
 
   // ---- the split's sums, normalised: the output itself, or a partial one
+  float l = w.l;
   l += __shfl_xor(l, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse2 = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  const float lse2 = l == 0.f ? -INFINITY : w.m + __builtin_amdgcn_logf(l);
   if (row >= p.rows) return;
   const size_t dst = splits == 1 ? (size_t)b * p.rows + row : (size_t)blockIdx.x * (32 * HG) + 32 * hg + j32;
   uint16_t *od = (splits == 1 ? p.out : p.part_o) + dst * LC_LORA;
@@ -486,9 +698,9 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   for (int c = 0; c < NCB; ++c)
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
-      const u32x2 w = {pack_bf16(o[c][4 * q4] * inv, o[c][4 * q4 + 1] * inv),
-                       pack_bf16(o[c][4 * q4 + 2] * inv, o[c][4 * q4 + 3] * inv)};
-      *reinterpret_cast<u32x2 *>(od + 32 * (cg * NCB + c) + 8 * q4 + 4 * hh) = w;
+      const u32x2 x = {pack_bf16(w.o[c][4 * q4] * inv, w.o[c][4 * q4 + 1] * inv),
+                       pack_bf16(w.o[c][4 * q4 + 2] * inv, w.o[c][4 * q4 + 3] * inv)};
+      *reinterpret_cast<u32x2 *>(od + 32 * (cg * NCB + c) + 8 * q4 + 4 * hh) = x;
     }
   if (cg == 0 && hh == 0) {
     if (splits > 1) p.part_lse[dst] = lse2;
@@ -541,7 +753,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
 constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 
 // 32-row groups of a workgroup: as many as the rows of a sequence fill
-static int attn_groups(int64_t) { return 1; }
+static int attn_groups(int64_t rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 struct AttnSizes {
   int hg;
   int64_t chunks, slots;
@@ -558,10 +770,12 @@ static AttnSizes attn_sizes(int64_t seqs, int64_t rows, int64_t max_rows) {
 
 template <bool F8, int HG>
 static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
-  static const hipError_t attr = hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  const auto kernel = p.seq_len > 1 ? latent_attn_kernel<F8, HG, true> : latent_attn_kernel<F8, HG, false>;
+  static const hipError_t attr[2] = {
+      hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
+      hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
   (void)attr;
-  latent_attn_kernel<F8, HG><<<dim3((unsigned)p.slots), 256, Stage<F8>::LDS, st>>>(p);
+  kernel<<<dim3((unsigned)p.slots), 256, Stage<F8>::LDS, st>>>(p);
   int rc = check_launch("latent_attention");
   if (rc) return rc;
   latent_join_kernel<F8, HG><<<dim3((unsigned)((p.rows + 3) / 4), (unsigned)p.seqs), 256, 0, st>>>(p);
@@ -615,11 +829,11 @@ int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t
   p.part_lse = reinterpret_cast<float *>(p.part_o + (size_t)s.slots * 32 * s.hg * LC_LORA);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (p.pg.scales) {
-
-    return launch_attn<true, 1>(p, st);
+    if (s.hg == 4) return launch_attn<true, 4>(p, st);
+    return s.hg == 2 ? launch_attn<true, 2>(p, st) : launch_attn<true, 1>(p, st);
   }
-
-  return launch_attn<false, 1>(p, st);
+  if (s.hg == 4) return launch_attn<false, 4>(p, st);
+  return s.hg == 2 ? launch_attn<false, 2>(p, st) : launch_attn<false, 1>(p, st);
 }
 
 }  // extern "C"

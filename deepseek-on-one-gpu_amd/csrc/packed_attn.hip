@@ -97,11 +97,11 @@ __global__ __launch_bounds__(64 * PA_NW, 1) void packed_attn_kernel(PackedParams
     uint8_t *d = st + 8 * wave * 128;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      __builtin_amdgcn_global_load_lds(kr + 64 * half, LDS_PTR(d + half * PA_HALF), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vr + 64 * half, LDS_PTR(d + VAL + half * PA_HALF), 16, 0, 0);
+      copy_lds(kr + 64 * half, d + half * PA_HALF);
+      copy_lds(vr + 64 * half, d + VAL + half * PA_HALF);
     }
     if constexpr (ROPE)
-      __builtin_amdgcn_global_load_lds(p.k_pe ? p.k_pe + t * p.ld_pe + 8 * kc : kr + 128, LDS_PTR(d + 2 * PA_HALF), 16, 0, 0);
+      copy_lds(p.k_pe ? p.k_pe + t * p.ld_pe + 8 * kc : kr + 128, d + 2 * PA_HALF);
   };
 
   if (ntiles > 0) copy(0, sm);
