@@ -25,13 +25,15 @@ struct LatentPages {
   int64_t ld_table;
   int32_t pages, cols;
   int page_shift;    // page_size = 1 << page_shift
-  // Pool row of row t >= 0 of sequence b, -1 where the table has no valid page for it.
-  AMLA_DEV int slot(int b, int t) const {
+  // The table's entry for row t >= 0 of sequence b (-1 past the table), and the pool row it means: -1 for none.
+  AMLA_DEV int page(int b, int t) const {
     const int c = t >> page_shift;
-    if (c >= cols) return -1;
-    const int page = table[b * ld_table + c];
+    return c < cols ? table[b * ld_table + c] : -1;
+  }
+  AMLA_DEV int row(int page, int t) const {
     return (uint32_t)page < (uint32_t)pages ? (page << page_shift) + (t & ((1 << page_shift) - 1)) : -1;
   }
+  AMLA_DEV int slot(int b, int t) const { return row(page(b, t), t); }
 };
 
 // 64 lanes x 16 bytes from per-lane addresses to 1 KB of LDS.  Functions of their own, not templates: inside

@@ -119,13 +119,16 @@ template <bool F8> struct Stage {
   static constexpr int ROWS = Tile<F8>::ROWS;
   static constexpr int PE = ROWS * Tile<F8>::RB, EXP = PE + ROWS * 128, INV = EXP + ROWS * 4, MUL = INV + ROWS * 4;
   static constexpr int SIZE = (MUL + ROWS * 4 + 1023) / 1024 * 1024;  // chunks enter addresses by xor
-  static constexpr int QR = SIZE * Tile<F8>::STAGES;  // e4m3: the rope queries, 4 KB a wave
-  static constexpr int LDS = QR + (F8 ? 4 * 4096 : 0);
+  // query fragments that the registers have no room for: QL of the latent ones, e4m3: and the four of the rope key
+  static constexpr int Q = SIZE * Tile<F8>::STAGES, QL = F8 ? 5 : 3, QF = QL + (F8 ? 4 : 0);
+  static constexpr int LDS = Q + 4 * QF * 1024;
 };
 
-// The reference m of a query row's sums moves (a multiplication of all of them) only when a score passes
-// it by 2^40: fp32 and bf16 have the range, and e4m3 has a scale for each block.  m is a whole number.
-constexpr float LAG = 40.f;
+// The reference m of a query row's sums is its maximum over the split's first tile, so that the output
+// accumulators are never multiplied: fp32 and bf16 have the range, and e4m3 has a scale for each block.  A
+// row whose scores pass m by 2^LAG later on (or that saw nothing in the first tile) has the workgroup do
+// its split once more, with m from all of it.
+constexpr float LAG = 60.f;
 constexpr float M_NONE = -1e30f;  // no row seen yet (finite: 2^(-inf - M_NONE) is 0)
 
 template <int OFS> AMLA_DEV u32x4 lds_read16(uint32_t addr) {
@@ -205,11 +208,18 @@ AMLA_DEV bf16x8 codes_to_bf16(uint32_t w0, uint32_t w1, float scale) {
 template <bool F8> struct Rows {
   static constexpr int WR = Tile<F8>::ROWS / 4, NPE = WR / 8, NLAT = F8 ? WR / 2 : WR, COPIES = NLAT + NPE;
   int slot, pe[NPE];
-  AMLA_DEV void lookup(const LatentPages &pg, int b, int t0, int last) {
+  // The table's pages of the rows from t0 on: loaded here, used a tile later (a load waits for every copy before it).
+  AMLA_DEV void load(const LatentPages &pg, int b, int t0, int last) {
     const int lane = threadIdx.x & 63;
-    slot = pg.slot(b, min(t0 + lane % WR, last));
+    slot = pg.page(b, min(t0 + lane % WR, last));
 #pragma unroll
-    for (int i = 0; i < NPE; ++i) pe[i] = pg.slot(b, min(t0 + 8 * i + (lane >> 3), last));
+    for (int i = 0; i < NPE; ++i) pe[i] = pg.page(b, min(t0 + 8 * i + (lane >> 3), last));
+  }
+  AMLA_DEV void resolve(const LatentPages &pg, int t0, int last) {
+    const int lane = threadIdx.x & 63;
+    slot = pg.row(slot, min(t0 + lane % WR, last));
+#pragma unroll
+    for (int i = 0; i < NPE; ++i) pe[i] = pg.row(pe[i], min(t0 + 8 * i + (lane >> 3), last));
   }
   // The lane's part of the source addresses.  Opaque, so that the compiler forms each copy's address from
   // it instead of holding ten of them in registers throughout the loop.
@@ -248,17 +258,29 @@ template <bool F8, int I = 0> AMLA_DEV void copy_all(const Rows<F8> &rows, const
 
 // ---------------------------------------------------------------- the two phases of a tile
 
+// Latent query fragment f: its place in LDS (one every third, or fifth, score step), -1: in registers.
+template <bool F8> constexpr int q_place(int f) {
+  const int every = F8 ? 6 : 10;
+  return f % every == 1 && f / every < Stage<F8>::QL ? f / every : -1;
+}
+template <bool F8> constexpr int q_reg(int f) {
+  int n = 0;
+  for (int i = 0; i < f; ++i) n += q_place<F8>(i) < 0;
+  return n;
+}
+static_assert(Stage<true>::LDS <= 160 * 1024 && Stage<false>::LDS <= 160 * 1024);
+
 template <bool F8, int HG> struct Wave {
   static constexpr int KB = Tile<F8>::ROWS / 32;  // 32-row blocks of a tile
   static constexpr int CG = 4 / HG, NCB = 16 / CG;
-  bf16x8 q[32], qr[F8 ? 1 : 4];  // e4m3: the rope queries lie in LDS at qra, 1 KB a fragment
+  bf16x8 q[32 - Stage<F8>::QL], qr[F8 ? 1 : 4];  // the rest at qra in LDS, 1 KB a fragment
   uint32_t qra;
   f32x16 o[NCB];  // O^T: columns x queries
   f32x16 s[2];    // S^T of the tile in work: rows x queries (bf16: two chains of the one block)
   i32x8 phi, plo; // P of the tile before it: e4m3 halves and their scale,
   int ps, ps_lo, one;
   u32x4 pb[2];    // or bf16
-  float m, l;
+  float m, l, top;  // reference, sum of 2^(s - m), maximum so far
 };
 
 // Reads of score step I: two fragments, one of each chain of MFMAs.
@@ -268,7 +290,7 @@ template <bool F8, int I> AMLA_DEV void score_read(u32x4 (&d)[3], uint32_t kl, u
     constexpr int ks = I - 16;
     d[0] = lds_read16<0>(kr ^ (F8 ? 32 * ks : 64 * ks));
     d[1] = F8 ? lds_read16<32 * 128>(kr ^ (32 * ks)) : lds_read16<0>(kr ^ (64 * ks + 32));
-    if constexpr (F8) d[2] = lds_read16<1024 * ks>(qra);
+    if constexpr (F8) d[2] = lds_read16<1024 * (Stage<F8>::QL + ks)>(qra);
   } else if constexpr (F8) {  // codes 32 I + 16 hh .. + 15 of rows j32, 32 + j32
     d[0] = lds_read16<256 * (I >> 3)>(kl ^ (32 * (I & 7)));
     d[1] = lds_read16<256 * (I >> 3) + 32 * RB>(kl ^ (32 * (I & 7)));
@@ -276,9 +298,12 @@ template <bool F8, int I> AMLA_DEV void score_read(u32x4 (&d)[3], uint32_t kl, u
     d[0] = lds_read16<256 * (I >> 2)>(kl ^ (32 * ((2 * I) & 7)));
     d[1] = lds_read16<256 * (I >> 2)>(kl ^ (32 * ((2 * I + 1) & 7)));
   }
+  if constexpr (I < 16 && q_place<F8>(2 * I + 1) >= 0) d[2] = lds_read16<1024 * q_place<F8>(2 * I + 1)>(qra);
 }
 
-template <bool F8> constexpr int score_reads(int i) { return i >= 16 + (F8 ? 4 : 2) ? 0 : F8 && i >= 16 ? 3 : 2; }
+template <bool F8> constexpr int score_reads(int i) {
+  return i >= 16 + (F8 ? 4 : 2) ? 0 : (i >= 16 ? F8 : q_place<F8>(2 * i + 1) >= 0) ? 3 : 2;
+}
 constexpr int SCORE_AHEAD = 2;  // steps that reads go out ahead
 
 template <bool F8, int HG, int I>
@@ -290,31 +315,33 @@ AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint3
     if constexpr (I + SCORE_AHEAD < N) score_read<F8, I + SCORE_AHEAD>(ka[(I + SCORE_AHEAD) % (SCORE_AHEAD + 1)], kl, kr, w.qra);
     lds_wait<score_reads<F8>(I + 1) + score_reads<F8>(I + 2)>();
     lds_tie(ka[c][0], ka[c][1]);
-    if constexpr (F8 && I >= 16) lds_tie(ka[c][2]);
+    if constexpr (score_reads<F8>(I) == 3) lds_tie(ka[c][2]);
+    constexpr int r0q = q_reg<F8>(I < 16 ? 2 * I : 0), r1q = q_reg<F8>(I < 16 ? 2 * I + 1 : 0);
+    const bf16x8 qa = w.q[r0q], qb = score_reads<F8>(I) == 3 ? as_bf16x8(ka[c][2]) : w.q[r1q];
     if constexpr (I == 0) lds_tie(f0, f1);
     if constexpr (I >= 16) {
       constexpr int k0 = F8 ? I - 16 : 2 * (I - 16), k1 = F8 ? k0 : k0 + 1;
-      mfma_score(w.s[0], as_bf16x8(ka[c][0]), F8 ? as_bf16x8(ka[c][2]) : w.qr[F8 ? 0 : k0]);
-      mfma_score(w.s[1], as_bf16x8(ka[c][1]), F8 ? as_bf16x8(ka[c][2]) : w.qr[F8 ? 0 : k1]);
+      mfma_score(w.s[0], as_bf16x8(ka[c][0]), F8 ? qb : w.qr[F8 ? 0 : k0]);
+      mfma_score(w.s[1], as_bf16x8(ka[c][1]), F8 ? qb : w.qr[F8 ? 0 : k1]);
     } else if constexpr (F8) {
       const u32x4 x = ka[c][0], y = ka[c][1];
       const bf16x8 x0 = codes_to_bf16(x.x, x.y, f0), y0 = codes_to_bf16(y.x, y.y, f1);
       const bf16x8 x1 = codes_to_bf16(x.z, x.w, f0), y1 = codes_to_bf16(y.z, y.w, f1);
       if constexpr (I == 0) {
-        mfma_score0(w.s[0], x0, w.q[0]);
-        mfma_score0(w.s[1], y0, w.q[0]);
+        mfma_score0(w.s[0], x0, qa);
+        mfma_score0(w.s[1], y0, qa);
       } else {
-        mfma_score(w.s[0], x0, w.q[2 * I]);
-        mfma_score(w.s[1], y0, w.q[2 * I]);
+        mfma_score(w.s[0], x0, qa);
+        mfma_score(w.s[1], y0, qa);
       }
-      mfma_score(w.s[0], x1, w.q[2 * I + 1]);
-      mfma_score(w.s[1], y1, w.q[2 * I + 1]);
+      mfma_score(w.s[0], x1, qb);
+      mfma_score(w.s[1], y1, qb);
     } else if constexpr (I == 0) {
-      mfma_score0(w.s[0], as_bf16x8(ka[c][0]), w.q[0]);
-      mfma_score0(w.s[1], as_bf16x8(ka[c][1]), w.q[1]);
+      mfma_score0(w.s[0], as_bf16x8(ka[c][0]), qa);
+      mfma_score0(w.s[1], as_bf16x8(ka[c][1]), qb);
     } else {
-      mfma_score(w.s[0], as_bf16x8(ka[c][0]), w.q[2 * I]);
-      mfma_score(w.s[1], as_bf16x8(ka[c][1]), w.q[2 * I + 1]);
+      mfma_score(w.s[0], as_bf16x8(ka[c][0]), qa);
+      mfma_score(w.s[1], as_bf16x8(ka[c][1]), qb);
     }
     if constexpr (I > 0 && I <= Rows<F8>::COPIES) next.template copy<I - 1>(pg, st_next, r0, lanes);
     __builtin_amdgcn_sched_barrier(0);
@@ -369,8 +396,7 @@ template <bool F8, int HG> struct ValueState {
   uint32_t v0, v1, eb;
   float scale_log2;
   int lim;  // MASK: rows of the tile below lim are seen by the lane's query
-  float mx[KB], ref[KB], sum[KB], mn, f;
-  bool moved;
+  float mx[KB], ref[KB], sum[KB];
   i32x8 phi, plo;
   u32x4 pb[2];
   StepReads<F8, HG> rd[3];
@@ -411,7 +437,7 @@ template <bool F8, int HG, bool PV, bool ZP, int C> AMLA_DEV void value_read(Val
 // e4m3: 32 rows are one block of the matrix unit with a scale of its own, 2^(ref - m), so that rows far
 // below the sequence's maximum keep their bits: a reference for all would drop those below 2^-22 of it,
 // and thousands of them can outweigh it.
-template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 ex) {
+template <bool F8, int HG, bool MASK, bool FIRST, int S> AMLA_DEV void softmax_slice(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 ex) {
   using L = Slices<F8, HG>;
   constexpr int KB = L::KB, t = S % L::NZ, kb = t >> 2, q4 = t & 3;
   f32x16 &z = w.s[kb];
@@ -435,12 +461,11 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
         x.mx[k] = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       }
       const float top = __builtin_fmaxf(x.mx[0], x.mx[KB - 1]);
-      x.moved = top > w.m + LAG;
-      x.mn = x.moved ? ceilf(top) : w.m;
-      x.f = __builtin_amdgcn_exp2f(w.m - x.mn);
+      w.top = __builtin_fmaxf(w.top, top);
+      if constexpr (FIRST) w.m = w.m == M_NONE ? __builtin_fmaxf(ceilf(top), M_NONE) : w.m;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        x.ref[k] = F8 ? floorf(__builtin_fmaxf(x.mx[k], M_NONE)) - 7.f : x.mn;
+        x.ref[k] = F8 ? floorf(__builtin_fmaxf(x.mx[k], M_NONE)) - 7.f : w.m;
         x.sum[k] = 0.f;
       }
     }
@@ -463,12 +488,12 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
     }
   }
 }
-template <bool F8, int HG, bool MASK, int S, int END>
+template <bool F8, int HG, bool MASK, bool FIRST, int S, int END>
 AMLA_DEV void softmax_slices(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 *ex) {
   if constexpr (S < END) {
     if constexpr (S < Slices<F8, HG>::NZ || F8) lds_tie(ex[0]);
-    softmax_slice<F8, HG, MASK, S>(w, x, ex[0]);
-    softmax_slices<F8, HG, MASK, S + 1, END>(w, x, ex + 1);
+    softmax_slice<F8, HG, MASK, FIRST, S>(w, x, ex[0]);
+    softmax_slices<F8, HG, MASK, FIRST, S + 1, END>(w, x, ex + 1);
   }
 }
 
@@ -485,7 +510,7 @@ AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
       if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.phi, w.ps);
       else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[0].x, r.v[0].y, r.v[1].x, r.v[1].y}), as_bf16x8(w.pb[0]));
     }
-    if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r.ex);
+    if constexpr (ZP) softmax_slices<F8, HG, MASK, !PV, L::first(C), L::first(C + 1)>(w, x, r.ex);
     if constexpr (PV) {
       if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.plo, w.ps_lo);
       else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[2].x, r.v[2].y, r.v[3].x, r.v[3].y}), as_bf16x8(w.pb[1]));
@@ -495,11 +520,10 @@ AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
   }
 }
 
-// O^T += C^T P^T of the tile before (its stage at pv) while the scores of this tile (stage at zb) become
-// probabilities.  Returns the factor that O has to be multiplied by before the next tile's turn, and
-// whether any lane's is not 1.
+// O^T += C^T P^T of the tile before (its stage at pv; PV) while the scores of this tile (stage at zb; ZP)
+// become probabilities.  Without PV the tile is the split's first.
 template <bool F8, int HG, bool MASK, bool PV, bool ZP>
-AMLA_DEV bool value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, float scale_log2, int lim, float &f) {
+AMLA_DEV void value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, float scale_log2, int lim) {
   using T = Tile<F8>;
   using L = Slices<F8, HG>;
   constexpr int KB = L::KB, NCB = L::NCB;
@@ -521,9 +545,6 @@ AMLA_DEV bool value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, flo
   value_read<F8, HG, PV, ZP, 1>(x);
   value_step<F8, HG, MASK, PV, ZP, 0>(w, x);
   if constexpr (ZP) {
-    f = x.f;
-    w.m = x.mn;
-    w.l *= f;
 #pragma unroll
     for (int k = 0; k < KB; ++k) w.l += F8 ? x.sum[k] * __builtin_amdgcn_exp2f(x.ref[k] - w.m) : x.sum[k];
     // the scale of block k comes from the lanes of half k; 4 .. 160, the low halves' 4 less
@@ -535,9 +556,7 @@ AMLA_DEV bool value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, flo
     w.plo = x.plo;
     w.pb[0] = x.pb[0];
     w.pb[1] = x.pb[1];
-    return __ballot(x.moved) != 0;
   }
-  return false;
 }
 
 // The copies of a split: which rows of the pool a wave brings, and what is known of those under way.
@@ -547,20 +566,25 @@ template <bool F8> struct Feed {
   const LatentPages &pg;
   uint8_t *sm;
   int b, wave, held, last, cur;  // last: rows past it are copied from it (and have no part in anything)
-  Rows<F8> rows[PD + 1];         // [0]: the tile in work, [PD]: the next to go out
-  int byte[PD + 1];
+  Rows<F8> after; // the one after it
+  Rows<F8> next;  // the tile to go out next: pages of the table until arrive(), then pool rows
+  int none[PD + 1], byte[PD + 1];  // [0]: the tile in work, [PD]: the one going out; whether the lane's row has no page, its byte
 
   AMLA_DEV void start(int t_first) {
     cur = 0;
+    Rows<F8> r[PD];
 #pragma unroll
-    for (int d = 0; d <= PD; ++d) {
-      rows[d].lookup(pg, b, (t_first + d) * TILE + WR * wave, last);
+    for (int d = 0; d < PD; ++d) r[d].load(pg, b, (t_first + d) * TILE + WR * wave, last);
+#pragma unroll
+    for (int d = 0; d < PD; ++d) {
+      r[d].resolve(pg, (t_first + d) * TILE + WR * wave, last);
+      none[d] = r[d].slot < 0;
       byte[d] = 127;
-      if (d < PD) {
-        if constexpr (F8) byte[d] = pg.scales[max(rows[d].slot, 0)];
-        copy_all<F8>(rows[d], pg, sm + d * Stage<F8>::SIZE, WR * wave);
-      }
+      if constexpr (F8) byte[d] = pg.scales[max(r[d].slot, 0)];
     }
+    next.load(pg, b, (t_first + PD) * TILE + WR * wave, last);
+#pragma unroll
+    for (int d = 0; d < PD; ++d) copy_all<F8>(r[d], pg, sm + d * Stage<F8>::SIZE, WR * wave);
   }
   // The rows of tile `tile` have landed in every wave, their factors beside them.
   AMLA_DEV void arrive(int tile) {
@@ -570,15 +594,15 @@ template <bool F8> struct Feed {
     wait_vmcnt<(PD - 1) * COPIES>();
     uint8_t *st = sm + cur * G::SIZE;
     // rows of no page: zeros in place of what was copied (a NaN there would come through 0 * NaN)
-    const bool none = lane < WR && rows[0].slot < 0;
-    for (uint64_t bad = __ballot(none); bad; bad &= bad - 1) {
+    const bool gone = lane < WR && none[0];
+    for (uint64_t bad = __ballot(gone); bad; bad &= bad - 1) {
       const int r = WR * wave + __builtin_ctzll(bad);
       for (int i = lane; i < RB / 16; i += 64) *reinterpret_cast<u32x4 *>(st + r * RB + 16 * i) = u32x4{0, 0, 0, 0};
       if (lane < 8) *reinterpret_cast<u32x4 *>(st + G::PE + r * 128 + 16 * lane) = u32x4{0, 0, 0, 0};
     }
     if (lane < WR) {
-      const int r = WR * wave + lane, by = none ? 127 : byte[0];
-      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = none || tile * TILE + r >= held ? -INFINITY : (float)(by - 127);
+      const int r = WR * wave + lane, by = gone ? 127 : byte[0];
+      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = gone || tile * TILE + r >= held ? -INFINITY : (float)(by - 127);
       if constexpr (F8) {
         *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = (uint32_t)(254 - by) << 23;
         *reinterpret_cast<uint32_t *>(st + G::MUL + 4 * r) = by == 255 ? 0x7fc00000u : (uint32_t)by << 23;
@@ -587,17 +611,21 @@ template <bool F8> struct Feed {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if constexpr (F8) byte[PD] = pg.scales[max(rows[PD].slot, 0)];
+    next.resolve(pg, (tile + PD) * TILE + WR * wave, last);
+    none[PD] = next.slot < 0;
+    byte[PD] = 127;
+    if constexpr (F8) byte[PD] = pg.scales[max(next.slot, 0)];
+    after.load(pg, b, (tile + PD + 1) * TILE + WR * wave, last);
   }
   AMLA_DEV uint8_t *next_stage() const { return sm + (cur + PD) % NST * Stage<F8>::SIZE; }
-  // After the copies of tile + PD went out
-  AMLA_DEV void advance(int tile) {
+  // After the copies of `next` went out
+  AMLA_DEV void advance() {
 #pragma unroll
     for (int d = 0; d < PD; ++d) {
-      rows[d] = rows[d + 1];
+      none[d] = none[d + 1];
       byte[d] = byte[d + 1];
     }
-    rows[PD].lookup(pg, b, (tile + PD + 1) * TILE + WR * wave, last);
+    next = after;
     cur = cur + 1 == NST ? 0 : cur + 1;
   }
 };
@@ -635,56 +663,58 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   const int rq = min(row, p.rows - 1), tok = rq / p.heads;
   const int limit = rows_held - (p.seq_len - 1 - tok) - 4 * hh;  // rows [0, limit + 4 hh) are seen
   const uint16_t *qp = p.q + b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
+  uint8_t *const ql = sm + G::Q + 1024 * G::QF * wave + 16 * lane;
+  w.qra = lds0 + G::Q + 1024 * G::QF * wave + 16 * lane;
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    w.q[i] = as_bf16x8(ldg16(qp + (F8 ? 32 * (i >> 1) + 16 * hh + 8 * (i & 1) : 16 * i + 8 * hh)));
-  w.qra = lds0 + G::QR + 4096 * wave + 16 * lane;
+  for (int i = 0; i < 32; ++i) {
+    const u32x4 v = ldg16(qp + (F8 ? 32 * (i >> 1) + 16 * hh + 8 * (i & 1) : 16 * i + 8 * hh));
+    if (q_place<F8>(i) >= 0) *reinterpret_cast<u32x4 *>(ql + 1024 * q_place<F8>(i)) = v;  // (the wave's own place)
+    else w.q[q_reg<F8>(i)] = as_bf16x8(v);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const u32x4 v = ldg16(qp + LC_LORA + 16 * i + 8 * hh);
-    if constexpr (F8) *reinterpret_cast<u32x4 *>(sm + G::QR + 4096 * wave + 1024 * i + 16 * lane) = v;  // (the wave's own)
+    if constexpr (F8) *reinterpret_cast<u32x4 *>(ql + 1024 * (G::QL + i)) = v;
     else w.qr[i] = as_bf16x8(v);
   }
-#pragma unroll
-  for (int c = 0; c < NCB; ++c)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w.o[c][i] = 0.f;
-  settle(w.o);
   w.m = M_NONE;
-  w.l = 0.f;
   w.one = 127;
-
-  float f;
-  int tile = t_first;
-  uint32_t base = lds0;
-  feed.arrive(tile);
-  score_phase<F8, HG>(w, base, feed.rows[Feed<F8>::PD], p.pg, feed.next_stage(), Rows<F8>::WR * wave);
-  feed.advance(tile);
-  value_phase<F8, HG, MASK, false, true>(w, base, base, cg, p.scale_log2, limit - tile * TILE, f);  // O is still 0
-  for (++tile;;) {
-    bool moved = false;
-    while (tile < t_end && !moved) {
+  for (;;) {  // once, or twice where m turned out too low
+#pragma unroll
+    for (int c = 0; c < NCB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w.o[c][i] = 0.f;
+    settle(w.o);
+    w.l = 0.f;
+    w.top = -INFINITY;
+    uint32_t base = lds0;
+    feed.arrive(t_first);
+    score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+    feed.advance();
+    value_phase<F8, HG, MASK, false, true>(w, base, base, cg, p.scale_log2, limit - t_first * TILE);
+    for (int tile = t_first + 1; tile < t_end; ++tile) {
       const uint32_t before = base;
       feed.arrive(tile);
       base = lds0 + feed.cur * G::SIZE;
-      score_phase<F8, HG>(w, base, feed.rows[Feed<F8>::PD], p.pg, feed.next_stage(), Rows<F8>::WR * wave);
-      feed.advance(tile);
-      moved = value_phase<F8, HG, MASK, true, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE, f);
-      ++tile;
+      score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+      feed.advance();
+      value_phase<F8, HG, MASK, true, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE);
     }
-    if (!moved) break;
-    // the multiplication of O stays outside the loop that holds O in accumulator registers
+    value_phase<F8, HG, MASK, true, false>(w, base, base, cg, p.scale_log2, 0);
     settle(w.o);
-#pragma unroll
-    for (int c = 0; c < NCB; ++c) {
-      w.o[c] *= f;
-      asm volatile("" : "+a"(w.o[c]));
-    }
-    settle(w.o);
+    wait_vmcnt<0>();  // (copies past the last tile)
+    const bool low = w.top > w.m + LAG;
+    // the waves agree: their copies and barriers are common
+    __syncthreads();
+    uint32_t *vote = reinterpret_cast<uint32_t *>(sm);
+    if (lane == 0) vote[wave] = __ballot(low) != 0;
+    __syncthreads();
+    const bool again = (vote[0] | vote[1] | vote[2] | vote[3]) != 0;
+    __syncthreads();
+    if (!again) break;
+    w.m = low ? ceilf(w.top) : w.m;
+    feed.start(t_first);
   }
-  value_phase<F8, HG, MASK, true, false>(w, base, base, cg, p.scale_log2, 0, f);
-  settle(w.o);
-  wait_vmcnt<0>();
 
   // ---- the split's sums, normalised: the output itself, or a partial one
   float l = w.l;
