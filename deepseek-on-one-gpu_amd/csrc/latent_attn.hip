@@ -26,14 +26,22 @@ struct LatentAttnParams {
 };
 
 AMLA_DEV int lc_ceil_div(int a, int b) { return (a + b - 1) / b; }
+// Sum, maximum and inclusive prefix sum over the wave by lane moves inside the vector unit (a shuffle goes
+// through LDS, about ten times the latency).
 AMLA_DEV int wave_isum(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return (int)wave_reduce_u32((uint32_t)v, [] __device__(uint32_t x, uint32_t y) { return x + y; });
 }
-AMLA_DEV int wave_imax(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+AMLA_DEV int wave_imax(int v) { return (int)wave_max_u32((uint32_t)v); }  // of values >= 0
+template <int CTRL, int ROWS> AMLA_DEV int dpp_or_zero(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true);
+}
+AMLA_DEV int wave_iscan(int v) {
+  v += dpp_or_zero<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8 within 16 lanes
+  v += dpp_or_zero<0x112, 0xf>(v);
+  v += dpp_or_zero<0x114, 0xf>(v);
+  v += dpp_or_zero<0x118, 0xf>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);  // lane 15 of each row to the next (rows 1 and 3)
+  v += dpp_or_zero<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
   return v;
 }
 
@@ -75,12 +83,7 @@ struct SplitPlan {
     int base = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += 64) {
       const int s = lc_ceil_div(tiles(b0 + lane), len);
-      int incl = s * p.chunks;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += v;
-      }
+      const int incl = wave_iscan(s * p.chunks);
       const uint64_t past = __ballot(base + incl > slot);
       if (past) {
         const int l = __builtin_ctzll(past);
@@ -130,6 +133,14 @@ template <bool F8> struct Stage {
 // its split once more, with m from all of it.
 constexpr float LAG = 60.f;
 constexpr float M_NONE = -1e30f;  // no row seen yet (finite: 2^(-inf - M_NONE) is 0)
+
+// The lane, opaque to the compiler: what is derived from it is formed anew instead of held in a register
+// throughout the loop (there are none to spare).
+AMLA_DEV int fresh_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 
 template <int OFS> AMLA_DEV u32x4 lds_read16(uint32_t addr) {
   u32x4 v;
@@ -202,32 +213,24 @@ AMLA_DEV bf16x8 codes_to_bf16(uint32_t w0, uint32_t w1, float scale) {
 
 // ---------------------------------------------------------------- copies
 //
-// A wave copies ROWS / 4 rows of each tile straight into LDS.  `slot` holds the pool row of
-// row L % (ROWS / 4) in lane L, `pe` those of rows 8 i + L / 8 (below 0: row 0 of the pool is
+// A wave copies ROWS / 4 rows of each tile straight into LDS.  Lane L holds the pool row of row
+// L % (ROWS / 4) in `slot` and those of rows 8 i + L / 8 in `pe` (below 0: row 0 of the pool is
 // copied, its place cleared before use).
 template <bool F8> struct Rows {
   static constexpr int WR = Tile<F8>::ROWS / 4, NPE = WR / 8, NLAT = F8 ? WR / 2 : WR, COPIES = NLAT + NPE;
   int slot, pe[NPE];
-  // The table's pages of the rows from t0 on: loaded here, used a tile later (a load waits for every copy before it).
-  AMLA_DEV void load(const LatentPages &pg, int b, int t0, int last) {
+  AMLA_DEV void spread() {
     const int lane = threadIdx.x & 63;
-    slot = pg.page(b, min(t0 + lane % WR, last));
 #pragma unroll
-    for (int i = 0; i < NPE; ++i) pe[i] = pg.page(b, min(t0 + 8 * i + (lane >> 3), last));
-  }
-  AMLA_DEV void resolve(const LatentPages &pg, int t0, int last) {
-    const int lane = threadIdx.x & 63;
-    slot = pg.row(slot, min(t0 + lane % WR, last));
+    for (int i = 0; i < NPE; ++i) pe[i] = __shfl(slot, 8 * i + (lane >> 3), 64);
 #pragma unroll
-    for (int i = 0; i < NPE; ++i) pe[i] = pg.row(pe[i], min(t0 + 8 * i + (lane >> 3), last));
+    for (int i = 0; i < NPE; ++i) asm volatile("" : "+v"(pe[i]));  // the shuffle ends before LDS operations are counted by hand
   }
-  // The lane's part of the source addresses.  Opaque, so that the compiler forms each copy's address from
-  // it instead of holding ten of them in registers throughout the loop.
+  // The lane's part of the source addresses.
   static AMLA_DEV uint2 lanes(int r0) {
-    const int lane = threadIdx.x & 63;
-    uint32_t lat = F8 ? 16 * ((lane & 31) ^ Tile<F8>::swz(lane >> 5)) : 16 * (lane ^ Tile<F8>::swz(r0 & 15));
-    uint32_t pe = 16 * ((lane & 7) ^ ((r0 >> 1) & 7) ^ (lane >> 4));
-    asm volatile("" : "+v"(lat), "+v"(pe));
+    const int lane = fresh_lane();
+    const uint32_t lat = F8 ? 16 * ((lane & 31) ^ Tile<F8>::swz(lane >> 5)) : 16 * (lane ^ Tile<F8>::swz(r0 & 15));
+    const uint32_t pe = 16 * ((lane & 7) ^ ((r0 >> 1) & 7) ^ (lane >> 4));
     return uint2{lat, pe};
   }
   // copy I (0 .. COPIES - 1) into the stage at st, r0 = first row of the wave in it (a multiple of 8; the swizzles
@@ -306,35 +309,35 @@ template <bool F8> constexpr int score_reads(int i) {
 }
 constexpr int SCORE_AHEAD = 2;  // steps that reads go out ahead
 
+// x0: e4m3: the step's first fragment, converted in the step before (a conversion of four instructions fits
+// under each MFMA; all sixteen of a step in front of its four MFMAs cost 5900 cycles a tile, not 3900)
 template <bool F8, int HG, int I>
-AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint32_t kl, uint32_t kr, float &f0, float &f1,
-                         uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
+AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, float f0,
+                         float f1, uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
   constexpr int N = 16 + (F8 ? 4 : 2);  // steps over the latent and the rope key
   if constexpr (I < N) {
     constexpr int c = I % (SCORE_AHEAD + 1);
     if constexpr (I + SCORE_AHEAD < N) score_read<F8, I + SCORE_AHEAD>(ka[(I + SCORE_AHEAD) % (SCORE_AHEAD + 1)], kl, kr, w.qra);
-    lds_wait<score_reads<F8>(I + 1) + score_reads<F8>(I + 2)>();
-    lds_tie(ka[c][0], ka[c][1]);
-    if constexpr (score_reads<F8>(I) == 3) lds_tie(ka[c][2]);
     constexpr int r0q = q_reg<F8>(I < 16 ? 2 * I : 0), r1q = q_reg<F8>(I < 16 ? 2 * I + 1 : 0);
     const bf16x8 qa = w.q[r0q], qb = score_reads<F8>(I) == 3 ? as_bf16x8(ka[c][2]) : w.q[r1q];
-    if constexpr (I == 0) lds_tie(f0, f1);
+    bf16x8 xn = x0;
     if constexpr (I >= 16) {
       constexpr int k0 = F8 ? I - 16 : 2 * (I - 16), k1 = F8 ? k0 : k0 + 1;
       mfma_score(w.s[0], as_bf16x8(ka[c][0]), F8 ? qb : w.qr[F8 ? 0 : k0]);
       mfma_score(w.s[1], as_bf16x8(ka[c][1]), F8 ? qb : w.qr[F8 ? 0 : k1]);
     } else if constexpr (F8) {
       const u32x4 x = ka[c][0], y = ka[c][1];
-      const bf16x8 x0 = codes_to_bf16(x.x, x.y, f0), y0 = codes_to_bf16(y.x, y.y, f1);
-      const bf16x8 x1 = codes_to_bf16(x.z, x.w, f0), y1 = codes_to_bf16(y.z, y.w, f1);
-      if constexpr (I == 0) {
-        mfma_score0(w.s[0], x0, qa);
-        mfma_score0(w.s[1], y0, qa);
-      } else {
-        mfma_score(w.s[0], x0, qa);
-        mfma_score(w.s[1], y0, qa);
-      }
+      if constexpr (I == 0) mfma_score0(w.s[0], x0, qa);
+      else mfma_score(w.s[0], x0, qa);
+      const bf16x8 y0 = codes_to_bf16(y.x, y.y, f1);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (I == 0) mfma_score0(w.s[1], y0, qa);
+      else mfma_score(w.s[1], y0, qa);
+      const bf16x8 x1 = codes_to_bf16(x.z, x.w, f0);
+      __builtin_amdgcn_sched_barrier(0);
       mfma_score(w.s[0], x1, qb);
+      const bf16x8 y1 = codes_to_bf16(y.z, y.w, f1);
+      __builtin_amdgcn_sched_barrier(0);
       mfma_score(w.s[1], y1, qb);
     } else if constexpr (I == 0) {
       mfma_score0(w.s[0], as_bf16x8(ka[c][0]), qa);
@@ -344,8 +347,15 @@ AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint3
       mfma_score(w.s[1], as_bf16x8(ka[c][1]), qb);
     }
     if constexpr (I > 0 && I <= Rows<F8>::COPIES) next.template copy<I - 1>(pg, st_next, r0, lanes);
+    if constexpr (I + 1 < N) {
+      constexpr int n = (I + 1) % (SCORE_AHEAD + 1);
+      lds_wait<score_reads<F8>(I + 2)>();
+      lds_tie(ka[n][0], ka[n][1]);
+      if constexpr (score_reads<F8>(I + 1) == 3) lds_tie(ka[n][2]);
+      if constexpr (F8 && I + 1 < 16) xn = codes_to_bf16(ka[n][0].x, ka[n][0].y, f0);
+    }
     __builtin_amdgcn_sched_barrier(0);
-    score_step<F8, HG, I + 1>(w, ka, kl, kr, f0, f1, lanes, next, pg, st_next, r0);
+    score_step<F8, HG, I + 1>(w, ka, kl, kr, xn, f0, f1, lanes, next, pg, st_next, r0);
   }
 }
 
@@ -356,7 +366,7 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
                           int r0) {
   using T = Tile<F8>;
   using G = Stage<F8>;
-  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
+  const int lane = fresh_lane(), j32 = lane & 31, hh = lane >> 5;
   // the lane's row and first chunk; chunk c sits at c ^ swz(row): bits 1 .. 3 of c enter by xor, higher ones by offset
   const uint32_t kl = base + j32 * T::RB + 16 * (hh ^ T::swz(j32));
   const uint32_t kr = base + G::PE + j32 * 128 + 16 * (hh ^ ((j32 >> 1) & 7));
@@ -368,7 +378,13 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
   u32x4 ka[SCORE_AHEAD + 1][3];
   score_read<F8, 0>(ka[0], kl, kr, w.qra);
   score_read<F8, 1>(ka[1], kl, kr, w.qra);
-  score_step<F8, HG, 0>(w, ka, kl, kr, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
+  lds_wait<score_reads<F8>(1)>();
+  lds_tie(f0, f1, ka[0][0], ka[0][1]);
+  if constexpr (score_reads<F8>(0) == 3) lds_tie(ka[0][2]);
+  bf16x8 x0;
+  if constexpr (F8) x0 = codes_to_bf16(ka[0][0].x, ka[0][0].y, f0);
+  else x0 = as_bf16x8(ka[0][0]);
+  score_step<F8, HG, 0>(w, ka, kl, kr, x0, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
   // the results are read by vector code that the compiler schedules: cover the asm's write-to-read wait states
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   asm volatile("" : "+v"(w.s[0]), "+v"(w.s[1]));
@@ -378,8 +394,10 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
 // slices (four rows) of the softmax: first all scaled scores and their maxima, then the probabilities.
 template <bool F8, int HG> struct Slices {
   static constexpr int KB = Wave<F8, HG>::KB, NCB = Wave<F8, HG>::NCB, NZ = 4 * KB, NS = 8 * KB;
-  static constexpr int PER = (NS + NCB - 1) / NCB;
-  static constexpr int first(int c) { return (c * NS + NCB - 1) / NCB; }
+  static constexpr int PER = NZ / (NCB / 4);  // slices of a step, at most
+  static constexpr int first(int c) {         // scores in the first quarter of the steps, the longer rest behind
+    return c <= NCB / 4 ? c * PER : NZ + ((c - NCB / 4) * NZ + 3 * NCB / 4 - 1) / (3 * NCB / 4);
+  }
   static constexpr int reads(int c) {  // row factors read for step c: bf16's probabilities need none
     if (c >= NCB) return 0;
     int n = 0;
@@ -411,17 +429,17 @@ template <bool F8, int HG, int S, int END> AMLA_DEV void slice_read(ValueState<F
     slice_read<F8, HG, S + 1, END>(x, ex + 1);
   }
 }
-template <bool F8, int HG, bool PV, bool ZP, int C> AMLA_DEV void value_read(ValueState<F8, HG> &x) {
+template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F8, HG> &x) {
   using L = Slices<F8, HG>;
   if constexpr (C < L::NCB) {
     StepReads<F8, HG> &r = x.rd[C % 3];
-    if constexpr (PV && F8) {
+    if constexpr (F8) {
       const uint32_t a = x.v0 ^ (32 * (C & 7));
       r.v[0] = lds_read_tr<F8, 256 * (C >> 3)>(a);
       r.v[1] = lds_read_tr<F8, 256 * (C >> 3) + 8192>(a);
       r.v[2] = lds_read_tr<F8, 256 * (C >> 3) + 16384>(a);
       r.v[3] = lds_read_tr<F8, 256 * (C >> 3) + 24576>(a);
-    } else if constexpr (PV) {
+    } else {
       const uint32_t a = x.v0 ^ (64 * (C & 3)), b = x.v1 ^ (64 * (C & 3));
       r.v[0] = lds_read_tr<F8, 256 * (C >> 2)>(a);
       r.v[1] = lds_read_tr<F8, 256 * (C >> 2)>(b);
@@ -437,7 +455,7 @@ template <bool F8, int HG, bool PV, bool ZP, int C> AMLA_DEV void value_read(Val
 // e4m3: 32 rows are one block of the matrix unit with a scale of its own, 2^(ref - m), so that rows far
 // below the sequence's maximum keep their bits: a reference for all would drop those below 2^-22 of it,
 // and thousands of them can outweigh it.
-template <bool F8, int HG, bool MASK, bool FIRST, int S> AMLA_DEV void softmax_slice(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 ex) {
+template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 ex) {
   using L = Slices<F8, HG>;
   constexpr int KB = L::KB, t = S % L::NZ, kb = t >> 2, q4 = t & 3;
   f32x16 &z = w.s[kb];
@@ -462,7 +480,7 @@ template <bool F8, int HG, bool MASK, bool FIRST, int S> AMLA_DEV void softmax_s
       }
       const float top = __builtin_fmaxf(x.mx[0], x.mx[KB - 1]);
       w.top = __builtin_fmaxf(w.top, top);
-      if constexpr (FIRST) w.m = w.m == M_NONE ? __builtin_fmaxf(ceilf(top), M_NONE) : w.m;
+      w.m = w.m == M_NONE ? __builtin_fmaxf(ceilf(top), M_NONE) : w.m;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
         x.ref[k] = F8 ? floorf(__builtin_fmaxf(x.mx[k], M_NONE)) - 7.f : w.m;
@@ -488,46 +506,42 @@ template <bool F8, int HG, bool MASK, bool FIRST, int S> AMLA_DEV void softmax_s
     }
   }
 }
-template <bool F8, int HG, bool MASK, bool FIRST, int S, int END>
+template <bool F8, int HG, bool MASK, int S, int END>
 AMLA_DEV void softmax_slices(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 *ex) {
   if constexpr (S < END) {
     if constexpr (S < Slices<F8, HG>::NZ || F8) lds_tie(ex[0]);
-    softmax_slice<F8, HG, MASK, FIRST, S>(w, x, ex[0]);
-    softmax_slices<F8, HG, MASK, FIRST, S + 1, END>(w, x, ex + 1);
+    softmax_slice<F8, HG, MASK, S>(w, x, ex[0]);
+    softmax_slices<F8, HG, MASK, S + 1, END>(w, x, ex + 1);
   }
 }
 
-template <bool F8, int HG, bool MASK, bool PV, bool ZP, int C>
+template <bool F8, int HG, bool MASK, bool ZP, int C>
 AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
   using L = Slices<F8, HG>;
   if constexpr (C < L::NCB) {
     StepReads<F8, HG> &r = x.rd[C % 3];
-    value_read<F8, HG, PV, ZP, C + 2>(x);
+    value_read<F8, HG, ZP, C + 2>(x);
     // this step's reads have landed: those of the next two steps may be in flight
-    lds_wait<(PV ? 4 * ((C + 1 < L::NCB) + (C + 2 < L::NCB)) : 0) + (ZP ? L::reads(C + 1) + L::reads(C + 2) : 0)>();
-    if constexpr (PV) {
-      lds_tie(r.v[0], r.v[1], r.v[2], r.v[3]);
-      if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.phi, w.ps);
-      else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[0].x, r.v[0].y, r.v[1].x, r.v[1].y}), as_bf16x8(w.pb[0]));
-    }
-    if constexpr (ZP) softmax_slices<F8, HG, MASK, !PV, L::first(C), L::first(C + 1)>(w, x, r.ex);
-    if constexpr (PV) {
-      if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.plo, w.ps_lo);
-      else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[2].x, r.v[2].y, r.v[3].x, r.v[3].y}), as_bf16x8(w.pb[1]));
-    }
+    lds_wait<4 * ((C + 1 < L::NCB) + (C + 2 < L::NCB)) + (ZP ? L::reads(C + 1) + L::reads(C + 2) : 0)>();
+    lds_tie(r.v[0], r.v[1], r.v[2], r.v[3]);
+    if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.phi, w.ps);
+    else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[0].x, r.v[0].y, r.v[1].x, r.v[1].y}), as_bf16x8(w.pb[0]));
+    if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r.ex);
+    if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.plo, w.ps_lo);
+    else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[2].x, r.v[2].y, r.v[3].x, r.v[3].y}), as_bf16x8(w.pb[1]));
     __builtin_amdgcn_sched_barrier(0);
-    value_step<F8, HG, MASK, PV, ZP, C + 1>(w, x);
+    value_step<F8, HG, MASK, ZP, C + 1>(w, x);
   }
 }
 
-// O^T += C^T P^T of the tile before (its stage at pv; PV) while the scores of this tile (stage at zb; ZP)
-// become probabilities.  Without PV the tile is the split's first.
-template <bool F8, int HG, bool MASK, bool PV, bool ZP>
+// O^T += C^T P^T of the tile before (its stage at pv) while the scores of this tile (stage at zb; ZP) become
+// probabilities.
+template <bool F8, int HG, bool MASK, bool ZP>
 AMLA_DEV void value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, float scale_log2, int lim) {
   using T = Tile<F8>;
   using L = Slices<F8, HG>;
   constexpr int KB = L::KB, NCB = L::NCB;
-  const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+  const int lane = fresh_lane(), hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
   ValueState<F8, HG> x;
   if constexpr (F8) {  // rows 16 i + 4 hh + {0..3, 8..11} of 16 columns
     const int r = 8 * (L16 >> 3) + 4 * hh + ((L16 >> 1) & 3);
@@ -541,9 +555,9 @@ AMLA_DEV void value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, flo
   x.eb = zb + 16 * hh;
   x.scale_log2 = scale_log2;
   x.lim = lim;
-  value_read<F8, HG, PV, ZP, 0>(x);
-  value_read<F8, HG, PV, ZP, 1>(x);
-  value_step<F8, HG, MASK, PV, ZP, 0>(w, x);
+  value_read<F8, HG, ZP, 0>(x);
+  value_read<F8, HG, ZP, 1>(x);
+  value_step<F8, HG, MASK, ZP, 0>(w, x);
   if constexpr (ZP) {
 #pragma unroll
     for (int k = 0; k < KB; ++k) w.l += F8 ? x.sum[k] * __builtin_amdgcn_exp2f(x.ref[k] - w.m) : x.sum[k];
@@ -566,23 +580,29 @@ template <bool F8> struct Feed {
   const LatentPages &pg;
   uint8_t *sm;
   int b, wave, held, last, cur;  // last: rows past it are copied from it (and have no part in anything)
-  Rows<F8> after; // the one after it
-  Rows<F8> next;  // the tile to go out next: pages of the table until arrive(), then pool rows
-  int none[PD + 1], byte[PD + 1];  // [0]: the tile in work, [PD]: the one going out; whether the lane's row has no page, its byte
+  Rows<F8> next;     // the tile that goes out next
+  int page;          // the table's entry for the lane's row of the tile after it
+  int byte[PD + 1];  // the row's exponent, -1 where it has no page; [0]: the tile in work, [PD]: the one going out
 
+  AMLA_DEV int row_of(int tile) const { return min(tile * TILE + WR * wave + (int)(threadIdx.x & 63) % WR, last); }
+  AMLA_DEV int byte_of(int slot) const {
+    int v = 127;
+    if constexpr (F8) v = pg.scales[max(slot, 0)];
+    return slot < 0 ? -1 : v;
+  }
   AMLA_DEV void start(int t_first) {
     cur = 0;
     Rows<F8> r[PD];
 #pragma unroll
-    for (int d = 0; d < PD; ++d) r[d].load(pg, b, (t_first + d) * TILE + WR * wave, last);
+    for (int d = 0; d < PD; ++d) r[d].slot = pg.page(b, row_of(t_first + d));
+    page = pg.page(b, row_of(t_first + PD));
 #pragma unroll
     for (int d = 0; d < PD; ++d) {
-      r[d].resolve(pg, (t_first + d) * TILE + WR * wave, last);
-      none[d] = r[d].slot < 0;
-      byte[d] = 127;
-      if constexpr (F8) byte[d] = pg.scales[max(r[d].slot, 0)];
+      r[d].slot = pg.row(r[d].slot, row_of(t_first + d));
+      r[d].spread();
     }
-    next.load(pg, b, (t_first + PD) * TILE + WR * wave, last);
+#pragma unroll
+    for (int d = 0; d < PD; ++d) byte[d] = byte_of(r[d].slot);
 #pragma unroll
     for (int d = 0; d < PD; ++d) copy_all<F8>(r[d], pg, sm + d * Stage<F8>::SIZE, WR * wave);
   }
@@ -593,8 +613,8 @@ template <bool F8> struct Feed {
     const int lane = threadIdx.x & 63;
     wait_vmcnt<(PD - 1) * COPIES>();
     uint8_t *st = sm + cur * G::SIZE;
-    // rows of no page: zeros in place of what was copied (a NaN there would come through 0 * NaN)
-    const bool gone = lane < WR && none[0];
+    // rows of no page or past the end: zeros in place of what was copied (a NaN there would come through 0 * NaN)
+    const bool gone = lane < WR && (byte[0] < 0 || tile * TILE + WR * wave + lane >= held);
     for (uint64_t bad = __ballot(gone); bad; bad &= bad - 1) {
       const int r = WR * wave + __builtin_ctzll(bad);
       for (int i = lane; i < RB / 16; i += 64) *reinterpret_cast<u32x4 *>(st + r * RB + 16 * i) = u32x4{0, 0, 0, 0};
@@ -602,7 +622,7 @@ template <bool F8> struct Feed {
     }
     if (lane < WR) {
       const int r = WR * wave + lane, by = gone ? 127 : byte[0];
-      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = gone || tile * TILE + r >= held ? -INFINITY : (float)(by - 127);
+      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = gone ? -INFINITY : (float)(by - 127);
       if constexpr (F8) {
         *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = (uint32_t)(254 - by) << 23;
         *reinterpret_cast<uint32_t *>(st + G::MUL + 4 * r) = by == 255 ? 0x7fc00000u : (uint32_t)by << 23;
@@ -611,21 +631,16 @@ template <bool F8> struct Feed {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    next.resolve(pg, (tile + PD) * TILE + WR * wave, last);
-    none[PD] = next.slot < 0;
-    byte[PD] = 127;
-    if constexpr (F8) byte[PD] = pg.scales[max(next.slot, 0)];
-    after.load(pg, b, (tile + PD + 1) * TILE + WR * wave, last);
+    next.slot = pg.row(page, row_of(tile + PD));
+    next.spread();
+    page = pg.page(b, row_of(tile + PD + 1));  // (loaded a tile ahead: a load waits for every copy before it)
+    byte[PD] = byte_of(next.slot);
   }
   AMLA_DEV uint8_t *next_stage() const { return sm + (cur + PD) % NST * Stage<F8>::SIZE; }
   // After the copies of `next` went out
   AMLA_DEV void advance() {
 #pragma unroll
-    for (int d = 0; d < PD; ++d) {
-      none[d] = none[d + 1];
-      byte[d] = byte[d + 1];
-    }
-    next = after;
+    for (int d = 0; d < PD; ++d) byte[d] = byte[d + 1];
     cur = cur + 1 == NST ? 0 : cur + 1;
   }
 };
@@ -645,10 +660,13 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   const int hg = wave / CG, cg = wave % CG;
 
   const SplitPlan<TILE> plan(p);
-  const int3 at = plan.find(blockIdx.x);
+  // workgroup i runs on XCD i % 8: each takes a run of slots, so that a sequence's queries come from its L2
+  const int per_xcd = lc_ceil_div(plan.used(plan.len), 8), slot = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd) return;
+  const int3 at = plan.find(slot);
   if (at.x < 0) return;
   const int b = at.x, splits = at.z;
-  const int chunk = ((int)blockIdx.x - at.y) / splits, split = ((int)blockIdx.x - at.y) % splits;
+  const int chunk = (slot - at.y) / splits, split = (slot - at.y) % splits;
   const int rows_held = __builtin_amdgcn_readfirstlane(min(max(p.lengths[b], 0), p.cap));
   const int n_tiles = lc_ceil_div(rows_held, TILE);
   const int t_first = (int)((int64_t)split * n_tiles / splits), t_end = (int)((int64_t)(split + 1) * n_tiles / splits);
@@ -687,20 +705,21 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
     settle(w.o);
     w.l = 0.f;
     w.top = -INFINITY;
+    // nothing before the first tile: probabilities of 0 times its own values, which saves a second copy of the loop's code
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.phi[i] = w.plo[i] = 0;
+    w.pb[0] = w.pb[1] = u32x4{0, 0, 0, 0};
+    w.ps = w.ps_lo = 127;
     uint32_t base = lds0;
-    feed.arrive(t_first);
-    score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
-    feed.advance();
-    value_phase<F8, HG, MASK, false, true>(w, base, base, cg, p.scale_log2, limit - t_first * TILE);
-    for (int tile = t_first + 1; tile < t_end; ++tile) {
+    for (int tile = t_first; tile < t_end; ++tile) {
       const uint32_t before = base;
       feed.arrive(tile);
       base = lds0 + feed.cur * G::SIZE;
       score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
       feed.advance();
-      value_phase<F8, HG, MASK, true, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE);
+      value_phase<F8, HG, MASK, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE);
     }
-    value_phase<F8, HG, MASK, true, false>(w, base, base, cg, p.scale_log2, 0);
+    value_phase<F8, HG, MASK, false>(w, base, base, cg, p.scale_log2, 0);
     settle(w.o);
     wait_vmcnt<0>();  // (copies past the last tile)
     const bool low = w.top > w.m + LAG;
@@ -721,58 +740,91 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   l += __shfl_xor(l, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse2 = l == 0.f ? -INFINITY : w.m + __builtin_amdgcn_logf(l);
-  if (row >= p.rows) return;
-  const size_t dst = splits == 1 ? (size_t)b * p.rows + row : (size_t)blockIdx.x * (32 * HG) + 32 * hg + j32;
-  uint16_t *od = (splits == 1 ? p.out : p.part_o) + dst * LC_LORA;
+  // rows of 1 KB / CG through LDS (chunk c of a wave's row at c ^ row), so that a store is whole lines
+  constexpr int RBYTES = 1024 / CG;
+  uint8_t *turn = sm + wave * 32 * RBYTES;
 #pragma unroll
   for (int c = 0; c < NCB; ++c)
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const u32x2 x = {pack_bf16(w.o[c][4 * q4] * inv, w.o[c][4 * q4 + 1] * inv),
-                       pack_bf16(w.o[c][4 * q4 + 2] * inv, w.o[c][4 * q4 + 3] * inv)};
-      *reinterpret_cast<u32x2 *>(od + 32 * (cg * NCB + c) + 8 * q4 + 4 * hh) = x;
-    }
-  if (cg == 0 && hh == 0) {
-    if (splits > 1) p.part_lse[dst] = lse2;
-    else if (p.lse) p.lse[dst] = lse2 * 0.6931471805599453f;
+    for (int q4 = 0; q4 < 4; ++q4)
+      *reinterpret_cast<u32x2 *>(turn + j32 * RBYTES + 16 * ((4 * c + q4) ^ (j32 % (4 * NCB))) + 8 * hh) =
+          u32x2{pack_bf16(w.o[c][4 * q4] * inv, w.o[c][4 * q4 + 1] * inv),
+                pack_bf16(w.o[c][4 * q4 + 2] * inv, w.o[c][4 * q4 + 3] * inv)};
+  const int row0 = (chunk * HG + hg) * 32, held = min(32, p.rows - row0);
+  const size_t dst0 = splits == 1 ? (size_t)b * p.rows + row0 : (size_t)slot * (32 * HG) + 32 * hg;
+  uint8_t *od = reinterpret_cast<uint8_t *>((splits == 1 ? p.out : p.part_o) + dst0 * LC_LORA) + cg * RBYTES;
+  constexpr int LPR = RBYTES / 16;  // lanes of a row
+#pragma unroll 4
+  for (int r0 = 0; r0 < held; r0 += CG) {
+    const int r = r0 + lane / LPR, c = lane % LPR;
+    if (r < held)
+      *reinterpret_cast<u32x4 *>(od + (size_t)r * (LC_LORA * 2) + 16 * c) =
+          *reinterpret_cast<const u32x4 *>(turn + r * RBYTES + 16 * (c ^ (r % (4 * NCB))));
+  }
+  if (cg == 0 && hh == 0 && row < p.rows) {
+    if (splits > 1) p.part_lse[dst0 + j32] = lse2;
+    else if (p.lse) p.lse[dst0 + j32] = lse2 * 0.6931471805599453f;
   }
 }
 
-// Joins the splits of a query row, one wave per row: sum_j 2^(lse_j - max) O_j / sum_j 2^(lse_j - max).
+// Joins the splits of a query row: sum_j 2^(lse_j - max) O_j / sum_j 2^(lse_j - max).  One workgroup a row, wave k
+// taking splits k, k + 4, .., eight rows of 1 KB in flight; the waves' sums meet in LDS in wave order.
 template <bool F8, int HG>
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
-  const int lane = threadIdx.x & 63;
-  const int b = blockIdx.y, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float part[3][64][9];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y, row = blockIdx.x;
   const SplitPlan<Tile<F8>::ROWS> plan(p);
   const int2 at = plan.of(b);
-  if (at.y == 1 || row >= p.rows) return;
+  const int n = __builtin_amdgcn_readfirstlane(at.y);
+  if (n == 1) return;
   const size_t dst = (size_t)b * p.rows + row;
   u32x4 *od = reinterpret_cast<u32x4 *>(p.out + dst * LC_LORA) + lane;
-  if (at.y == 0) {
-    *od = u32x4{0, 0, 0, 0};
-    if (lane == 0 && p.lse) p.lse[dst] = -INFINITY;
+  if (n == 0) {
+    if (wave == 0) *od = u32x4{0, 0, 0, 0};
+    if (threadIdx.x == 0 && p.lse) p.lse[dst] = -INFINITY;
     return;
   }
-  const int chunk = row / (32 * HG);
-  const size_t src = (size_t)(at.x + chunk * at.y) * (32 * HG) + row % (32 * HG);
+  const size_t src = (size_t)(at.x + row / (32 * HG) * n) * (32 * HG) + row % (32 * HG);
+  const float *lse = p.part_lse + src;
   float top = -INFINITY;
-  for (int j = lane; j < at.y; j += 64) top = __builtin_fmaxf(top, p.part_lse[src + (size_t)j * (32 * HG)]);
+  for (int j = lane; j < n; j += 64) top = __builtin_fmaxf(top, lse[(size_t)j * (32 * HG)]);
   top = wave_max(top);
   const float ref = top == -INFINITY ? 0.f : top;
   float total = 0.f, a[8] = {};
-  for (int j0 = 0; j0 < at.y; j0 += 64) {
-    const float w = j0 + lane < at.y ? __builtin_amdgcn_exp2f(p.part_lse[src + (size_t)(j0 + lane) * (32 * HG)] - ref) : 0.f;
-    total += wave_sum(w);
-    for (int j = 0; j < min(64, at.y - j0); ++j) {
-      const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
-      if (wj == 0.f) continue;
-      const u32x4 v = ldg16(p.part_o + (src + (size_t)(j0 + j) * (32 * HG)) * LC_LORA + 8 * lane);
+  const uint16_t *po = p.part_o + src * LC_LORA + 8 * lane;
+  for (int j0 = wave; j0 < n; j0 += 32) {
+    float w[8];
+    u32x4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int j = min(j0 + 4 * k, n - 1);
+      v[k] = ldg16(po + (size_t)j * (32 * HG * LC_LORA));
+      w[k] = j0 + 4 * k < n ? lse[(size_t)j * (32 * HG)] - ref : -INFINITY;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = __builtin_amdgcn_exp2f(w[k]);
+      total += f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        a[2 * e] += wj * lo_bf(v[e]);
-        a[2 * e + 1] += wj * hi_bf(v[e]);
+        a[2 * e] = __builtin_fmaf(f, lo_bf(v[k][e]), a[2 * e]);
+        a[2 * e + 1] = __builtin_fmaf(f, hi_bf(v[k][e]), a[2 * e + 1]);
       }
     }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[wave - 1][lane][e] = a[e];
+    part[wave - 1][lane][8] = total;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] += part[k][lane][e];
+    total += part[k][lane][8];
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
   *od = u32x4{pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv), pack_bf16(a[4] * inv, a[5] * inv),
@@ -805,10 +857,10 @@ static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
       hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
       hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
   (void)attr;
-  kernel<<<dim3((unsigned)p.slots), 256, Stage<F8>::LDS, st>>>(p);
+  kernel<<<dim3((unsigned)(p.slots + 7) / 8 * 8), 256, Stage<F8>::LDS, st>>>(p);  // whole runs of every XCD
   int rc = check_launch("latent_attention");
   if (rc) return rc;
-  latent_join_kernel<F8, HG><<<dim3((unsigned)((p.rows + 3) / 4), (unsigned)p.seqs), 256, 0, st>>>(p);
+  latent_join_kernel<F8, HG><<<dim3((unsigned)p.rows, (unsigned)p.seqs), 256, 0, st>>>(p);
   return check_launch("latent_attention join");
 }
 
@@ -841,7 +893,7 @@ int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t
     return fail(AMLA_EUNSUPPORTED, "%s: q rows and out must be 16-byte aligned", what);
   const int64_t cap = cache->cols * cache->page_size;
   const AttnSizes s = attn_sizes(seqs, seq_len * heads, cap);
-  if (s.slots > (1 << 24) || (seq_len * heads + 3) / 4 > (1 << 24))
+  if (s.slots > (1 << 24) || seq_len * heads > (1 << 24))
     return fail(AMLA_EUNSUPPORTED, "%s: too many query rows", what);
   if (workspace_bytes < amla_latent_attention_workspace_bytes(seqs, seq_len, heads, cap) || !workspace)
     return fail(AMLA_EWORKSPACE, "%s: workspace too small", what);
