@@ -59,7 +59,7 @@ struct SplitPlan {
   AMLA_DEV int used(int L) const {
     int n = 0;
     for (int b = threadIdx.x & 63; b < p.seqs; b += 64) n += lc_ceil_div(tiles(b), L);
-    return wave_isum(n) * p.chunks;
+    return __builtin_amdgcn_readfirstlane(wave_isum(n)) * p.chunks;  // (scalar: what follows from it is uniform)
   }
   AMLA_DEV explicit SplitPlan(const LatentAttnParams &p_) : p(p_) {
     int sum = 0, most = 0;
@@ -68,14 +68,14 @@ struct SplitPlan {
       sum += n;
       most = max(most, n);
     }
-    const int64_t total = (int64_t)wave_isum(sum) * p.chunks;
+    const int64_t total = (int64_t)__builtin_amdgcn_readfirstlane(wave_isum(sum)) * p.chunks;
     int lo = max(1, (int)((total + p.slots - 1) / p.slots));
-    int hi = max(lo, min(wave_imax(most), (int)(total / max(1, p.slots - p.chunks * p.seqs)) + 1));
+    int hi = max(lo, min(__builtin_amdgcn_readfirstlane(wave_imax(most)), (int)(total / max(1, p.slots - p.chunks * p.seqs)) + 1));
     for (int probe = lo; lo < hi; probe = (lo + hi) >> 1) {
       if (used(probe) <= p.slots) hi = probe;
       else lo = probe + 1;
     }
-    len = __builtin_amdgcn_readfirstlane(lo);
+    len = lo;
   }
   // (sequence, first slot of it, its splits) of a slot; sequence -1 past the plan
   AMLA_DEV int3 find(int slot) const {
@@ -98,7 +98,8 @@ struct SplitPlan {
   AMLA_DEV int2 of(int b) const {
     int before = 0;
     for (int i = threadIdx.x & 63; i < b; i += 64) before += lc_ceil_div(tiles(i), len);
-    return int2{wave_isum(before) * p.chunks, lc_ceil_div(tiles(b), len)};
+    return int2{__builtin_amdgcn_readfirstlane(wave_isum(before)) * p.chunks,
+                __builtin_amdgcn_readfirstlane(lc_ceil_div(tiles(b), len))};
   }
 };
 
@@ -195,11 +196,17 @@ AMLA_DEV int pk_fp8x4(float a, float b, float c, float d) {
   const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, __float_as_int(a), false);
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
+AMLA_DEV int pk_fp8x4_16(float a, float b, float c, float d, float sixteenth) {  // of 16 times the values
+  int w;  // (the builtin's vector of shorts made the compiler take unrelated registers apart, before they were loaded)
+  asm("v_cvt_scalef32_pk_fp8_f32 %0, %1, %2, %3" : "=v"(w) : "v"(a), "v"(b), "v"(sixteenth));
+  asm("v_cvt_scalef32_pk_fp8_f32 %0, %1, %2, %3 op_sel:[0,0,0,1]" : "+v"(w) : "v"(c), "v"(d), "v"(sixteenth));
+  return w;
+}
 // x = hi + lo / 16 in e4m3, magnitudes up to 256: hi keeps four leading bits, lo the next four
-AMLA_DEV void split_fp8x4(const float *x, int &hi, int &lo) {
+AMLA_DEV void split_fp8x4(const float *x, float sixteenth, int &hi, int &lo) {
   hi = pk_fp8x4(x[0], x[1], x[2], x[3]);
   const f32x2 a = fp8x2_to_f32<false>(hi), b = fp8x2_to_f32<true>(hi);
-  lo = pk_fp8x4((x[0] - a.x) * 16.f, (x[1] - a.y) * 16.f, (x[2] - b.x) * 16.f, (x[3] - b.y) * 16.f);
+  lo = pk_fp8x4_16(x[0] - a.x, x[1] - a.y, x[2] - b.x, x[3] - b.y, sixteenth);
 }
 // Eight codes times a power of two, exact in bf16
 AMLA_DEV bf16x8 codes_to_bf16(uint32_t w0, uint32_t w1, float scale) {
@@ -223,8 +230,11 @@ template <bool F8> struct Rows {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < NPE; ++i) pe[i] = __shfl(slot, 8 * i + (lane >> 3), 64);
+  }
+  // The shuffle ends before LDS operations are counted by hand.
+  AMLA_DEV void landed() {
 #pragma unroll
-    for (int i = 0; i < NPE; ++i) asm volatile("" : "+v"(pe[i]));  // the shuffle ends before LDS operations are counted by hand
+    for (int i = 0; i < NPE; ++i) asm volatile("" : "+v"(pe[i]));
   }
   // The lane's part of the source addresses.
   static AMLA_DEV uint2 lanes(int r0) {
@@ -307,17 +317,30 @@ template <bool F8, int I> AMLA_DEV void score_read(u32x4 (&d)[3], uint32_t kl, u
 template <bool F8> constexpr int score_reads(int i) {
   return i >= 16 + (F8 ? 4 : 2) ? 0 : (i >= 16 ? F8 : q_place<F8>(2 * i + 1) >= 0) ? 3 : 2;
 }
-constexpr int SCORE_AHEAD = 2;  // steps that reads go out ahead
+// Steps that reads go out ahead: as many as the registers allow (an LDS read returns after 300 - 400 cycles with
+// four waves reading; two steps of bf16 are 128 cycles of products)
+template <bool F8, int HG> constexpr int score_ahead() { return F8 ? (HG == 4 ? 2 : 4) : (HG == 4 ? 3 : 6); }
+template <bool F8> constexpr int score_reads(int first, int last) {
+  int n = 0;
+  for (int i = first; i <= last; ++i) n += score_reads<F8>(i);
+  return n;
+}
+template <bool F8, int N, int I = 0> AMLA_DEV void score_reads_first(u32x4 (*ka)[3], uint32_t kl, uint32_t kr, uint32_t qra) {
+  if constexpr (I < N) {
+    score_read<F8, I>(ka[I], kl, kr, qra);
+    score_reads_first<F8, N, I + 1>(ka, kl, kr, qra);
+  }
+}
 
 // x0: e4m3: the step's first fragment, converted in the step before (a conversion of four instructions fits
 // under each MFMA; all sixteen of a step in front of its four MFMAs cost 5900 cycles a tile, not 3900)
 template <bool F8, int HG, int I>
-AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, float f0,
+AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, float f0,
                          float f1, uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
   constexpr int N = 16 + (F8 ? 4 : 2);  // steps over the latent and the rope key
   if constexpr (I < N) {
-    constexpr int c = I % (SCORE_AHEAD + 1);
-    if constexpr (I + SCORE_AHEAD < N) score_read<F8, I + SCORE_AHEAD>(ka[(I + SCORE_AHEAD) % (SCORE_AHEAD + 1)], kl, kr, w.qra);
+    constexpr int AHEAD = score_ahead<F8, HG>(), c = I % (AHEAD + 1);
+    if constexpr (I + AHEAD < N) score_read<F8, I + AHEAD>(ka[(I + AHEAD) % (AHEAD + 1)], kl, kr, w.qra);
     constexpr int r0q = q_reg<F8>(I < 16 ? 2 * I : 0), r1q = q_reg<F8>(I < 16 ? 2 * I + 1 : 0);
     const bf16x8 qa = w.q[r0q], qb = score_reads<F8>(I) == 3 ? as_bf16x8(ka[c][2]) : w.q[r1q];
     bf16x8 xn = x0;
@@ -348,8 +371,8 @@ AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[SCORE_AHEAD + 1][3], uint3
     }
     if constexpr (I > 0 && I <= Rows<F8>::COPIES) next.template copy<I - 1>(pg, st_next, r0, lanes);
     if constexpr (I + 1 < N) {
-      constexpr int n = (I + 1) % (SCORE_AHEAD + 1);
-      lds_wait<score_reads<F8>(I + 2)>();
+      constexpr int n = (I + 1) % (AHEAD + 1);
+      lds_wait<score_reads<F8>(I + 2, I + AHEAD)>();
       lds_tie(ka[n][0], ka[n][1]);
       if constexpr (score_reads<F8>(I + 1) == 3) lds_tie(ka[n][2]);
       if constexpr (F8 && I + 1 < 16) xn = codes_to_bf16(ka[n][0].x, ka[n][0].y, f0);
@@ -375,10 +398,10 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f0) : "v"(base + 4 * j32), "i"(G::MUL) : "memory");
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f1) : "v"(base + 4 * j32), "i"(G::MUL + 128) : "memory");
   }
-  u32x4 ka[SCORE_AHEAD + 1][3];
-  score_read<F8, 0>(ka[0], kl, kr, w.qra);
-  score_read<F8, 1>(ka[1], kl, kr, w.qra);
-  lds_wait<score_reads<F8>(1)>();
+  constexpr int AHEAD = score_ahead<F8, HG>();
+  u32x4 ka[AHEAD + 1][3];
+  score_reads_first<F8, AHEAD>(ka, kl, kr, w.qra);
+  lds_wait<score_reads<F8>(1, AHEAD - 1)>();
   lds_tie(f0, f1, ka[0][0], ka[0][1]);
   if constexpr (score_reads<F8>(0) == 3) lds_tie(ka[0][2]);
   bf16x8 x0;
@@ -394,10 +417,8 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
 // slices (four rows) of the softmax: first all scaled scores and their maxima, then the probabilities.
 template <bool F8, int HG> struct Slices {
   static constexpr int KB = Wave<F8, HG>::KB, NCB = Wave<F8, HG>::NCB, NZ = 4 * KB, NS = 8 * KB;
-  static constexpr int PER = NZ / (NCB / 4);  // slices of a step, at most
-  static constexpr int first(int c) {         // scores in the first quarter of the steps, the longer rest behind
-    return c <= NCB / 4 ? c * PER : NZ + ((c - NCB / 4) * NZ + 3 * NCB / 4 - 1) / (3 * NCB / 4);
-  }
+  static constexpr int PER = (NS + NCB - 1) / NCB;  // slices of a step, at most
+  static constexpr int first(int c) { return (c * NS + NCB - 1) / NCB; }
   static constexpr int reads(int c) {  // row factors read for step c: bf16's probabilities need none
     if (c >= NCB) return 0;
     int n = 0;
@@ -409,6 +430,7 @@ template <bool F8, int HG> struct StepReads {
   u32x2 v[4];
   u32x4 ex[Slices<F8, HG>::PER];
 };
+constexpr int VALUE_AHEAD = 2;
 template <bool F8, int HG> struct ValueState {
   static constexpr int KB = Wave<F8, HG>::KB;
   uint32_t v0, v1, eb;
@@ -417,22 +439,22 @@ template <bool F8, int HG> struct ValueState {
   float mx[KB], ref[KB], sum[KB];
   i32x8 phi, plo;
   u32x4 pb[2];
-  StepReads<F8, HG> rd[3];
+  StepReads<F8, HG> rd[VALUE_AHEAD + 1];
 };
 
-template <bool F8, int HG, int S, int END> AMLA_DEV void slice_read(ValueState<F8, HG> &x, u32x4 *ex) {
+template <bool F8, int HG, int S, int END, int K = 0> AMLA_DEV void slice_read(ValueState<F8, HG> &x, StepReads<F8, HG> &r) {
   using G = Stage<F8>;
   using L = Slices<F8, HG>;
   if constexpr (S < END) {
     constexpr int t = S % L::NZ;
-    if constexpr (S < L::NZ || F8) ex[0] = lds_read16<(S < L::NZ ? G::EXP : G::INV) + 4 * (32 * (t >> 2) + 8 * (t & 3))>(x.eb);
-    slice_read<F8, HG, S + 1, END>(x, ex + 1);
+    if constexpr (S < L::NZ || F8) r.ex[K] = lds_read16<(S < L::NZ ? G::EXP : G::INV) + 4 * (32 * (t >> 2) + 8 * (t & 3))>(x.eb);
+    slice_read<F8, HG, S + 1, END, K + 1>(x, r);
   }
 }
 template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F8, HG> &x) {
   using L = Slices<F8, HG>;
   if constexpr (C < L::NCB) {
-    StepReads<F8, HG> &r = x.rd[C % 3];
+    StepReads<F8, HG> &r = x.rd[C % (VALUE_AHEAD + 1)];
     if constexpr (F8) {
       const uint32_t a = x.v0 ^ (32 * (C & 7));
       r.v[0] = lds_read_tr<F8, 256 * (C >> 3)>(a);
@@ -446,7 +468,7 @@ template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F
       r.v[2] = lds_read_tr<F8, 256 * (C >> 2) + 16384>(a);
       r.v[3] = lds_read_tr<F8, 256 * (C >> 2) + 16384>(b);
     }
-    if constexpr (ZP) slice_read<F8, HG, L::first(C), L::first(C + 1)>(x, r.ex);
+    if constexpr (ZP) slice_read<F8, HG, L::first(C), L::first(C + 1)>(x, r);
   }
 }
 
@@ -495,7 +517,7 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.sum[kb] = __builtin_fmaf(e[i], __uint_as_float(ex[i]), x.sum[kb]);
       int hi, lo;
-      split_fp8x4(e, hi, lo);
+      split_fp8x4(e, 0.0625f, hi, lo);
       x.phi[4 * kb + q4] = hi;
       x.plo[4 * kb + q4] = lo;
     } else {
@@ -506,12 +528,16 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
     }
   }
 }
-template <bool F8, int HG, bool MASK, int S, int END>
-AMLA_DEV void softmax_slices(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 *ex) {
+template <bool F8, int HG, bool MASK, int S, int END, int K = 0>
+AMLA_DEV void softmax_slices(Wave<F8, HG> &w, ValueState<F8, HG> &x, StepReads<F8, HG> &r) {
   if constexpr (S < END) {
-    if constexpr (S < Slices<F8, HG>::NZ || F8) lds_tie(ex[0]);
-    softmax_slice<F8, HG, MASK, S>(w, x, ex[0]);
-    softmax_slices<F8, HG, MASK, S + 1, END>(w, x, ex + 1);
+    u32x4 ex = {0, 0, 0, 0};
+    if constexpr (S < Slices<F8, HG>::NZ || F8) {
+      ex = r.ex[K];
+      lds_tie(ex);
+    }
+    softmax_slice<F8, HG, MASK, S>(w, x, ex);
+    softmax_slices<F8, HG, MASK, S + 1, END, K + 1>(w, x, r);
   }
 }
 
@@ -519,16 +545,19 @@ template <bool F8, int HG, bool MASK, bool ZP, int C>
 AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
   using L = Slices<F8, HG>;
   if constexpr (C < L::NCB) {
-    StepReads<F8, HG> &r = x.rd[C % 3];
-    value_read<F8, HG, ZP, C + 2>(x);
+    StepReads<F8, HG> &r = x.rd[C % (VALUE_AHEAD + 1)];
+    value_read<F8, HG, ZP, C + VALUE_AHEAD>(x);
     // this step's reads have landed: those of the next two steps may be in flight
     lds_wait<4 * ((C + 1 < L::NCB) + (C + 2 < L::NCB)) + (ZP ? L::reads(C + 1) + L::reads(C + 2) : 0)>();
-    lds_tie(r.v[0], r.v[1], r.v[2], r.v[3]);
-    if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.phi, w.ps);
-    else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[0].x, r.v[0].y, r.v[1].x, r.v[1].y}), as_bf16x8(w.pb[0]));
-    if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r.ex);
-    if constexpr (F8) mfma_value(w.o[C], join(r.v[0], r.v[1], r.v[2], r.v[3]), w.one, w.plo, w.ps_lo);
-    else mfma_value(w.o[C], as_bf16x8(u32x4{r.v[2].x, r.v[2].y, r.v[3].x, r.v[3].y}), as_bf16x8(w.pb[1]));
+    // (locals, not members: a pass that sees the members in memory loads several at once, and then takes registers
+    // apart that are still being loaded)
+    u32x2 v0 = r.v[0], v1 = r.v[1], v2 = r.v[2], v3 = r.v[3];
+    lds_tie(v0, v1, v2, v3);
+    if constexpr (F8) mfma_value(w.o[C], join(v0, v1, v2, v3), w.one, w.phi, w.ps);
+    else mfma_value(w.o[C], as_bf16x8(u32x4{v0.x, v0.y, v1.x, v1.y}), as_bf16x8(w.pb[0]));
+    if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r);
+    if constexpr (F8) mfma_value(w.o[C], join(v0, v1, v2, v3), w.one, w.plo, w.ps_lo);
+    else mfma_value(w.o[C], as_bf16x8(u32x4{v2.x, v2.y, v3.x, v3.y}), as_bf16x8(w.pb[1]));
     __builtin_amdgcn_sched_barrier(0);
     value_step<F8, HG, MASK, ZP, C + 1>(w, x);
   }
@@ -590,6 +619,30 @@ template <bool F8> struct Feed {
     if constexpr (F8) v = pg.scales[max(slot, 0)];
     return slot < 0 ? -1 : v;
   }
+  // Rows of the pool for the tile that goes out after `tile`, from the page loaded before; the page of the one behind it.
+  // (Each is loaded a tile ahead of its use: a load waits for every copy before it.)
+  AMLA_DEV void prepare(int tile) {
+    next.slot = pg.row(page, row_of(tile + 1));
+    next.spread();
+    byte[PD] = byte_of(next.slot);
+    page = pg.page(b, row_of(tile + 2));
+  }
+  // Factors of the rows of tile `tile`, the next in work, beside where they are landing
+  AMLA_DEV void factors(int tile) {
+    using G = Stage<F8>;
+    uint8_t *st = sm + cur * G::SIZE;
+    const int lane = threadIdx.x & 63;
+    if (lane < WR) {
+      const int r = WR * wave + lane;
+      const bool gone = byte[0] < 0 || tile * TILE + r >= held;
+      const int by = gone ? 127 : byte[0];
+      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = gone ? -INFINITY : (float)(by - 127);
+      if constexpr (F8) {
+        *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = (uint32_t)(254 - by) << 23;
+        *reinterpret_cast<uint32_t *>(st + G::MUL + 4 * r) = by == 255 ? 0x7fc00000u : (uint32_t)by << 23;
+      }
+    }
+  }
   AMLA_DEV void start(int t_first) {
     cur = 0;
     Rows<F8> r[PD];
@@ -605,13 +658,17 @@ template <bool F8> struct Feed {
     for (int d = 0; d < PD; ++d) byte[d] = byte_of(r[d].slot);
 #pragma unroll
     for (int d = 0; d < PD; ++d) copy_all<F8>(r[d], pg, sm + d * Stage<F8>::SIZE, WR * wave);
+    asm volatile("" ::: "memory");
+    prepare(t_first + PD - 1);
+    factors(t_first);
   }
-  // The rows of tile `tile` have landed in every wave, their factors beside them.
+  // The rows of tile `tile` have landed in every wave
   AMLA_DEV void arrive(int tile) {
     using G = Stage<F8>;
-    constexpr int RB = Tile<F8>::RB;
+    constexpr int RB = Tile<F8>::RB, LOADS = F8 ? 2 : 1;
     const int lane = threadIdx.x & 63;
-    wait_vmcnt<(PD - 1) * COPIES>();
+    // behind its copies: those of PD - 1 tiles, and prepare()'s loads
+    wait_vmcnt<(PD - 1) * COPIES + LOADS>();
     uint8_t *st = sm + cur * G::SIZE;
     // rows of no page or past the end: zeros in place of what was copied (a NaN there would come through 0 * NaN)
     const bool gone = lane < WR && (byte[0] < 0 || tile * TILE + WR * wave + lane >= held);
@@ -620,28 +677,19 @@ template <bool F8> struct Feed {
       for (int i = lane; i < RB / 16; i += 64) *reinterpret_cast<u32x4 *>(st + r * RB + 16 * i) = u32x4{0, 0, 0, 0};
       if (lane < 8) *reinterpret_cast<u32x4 *>(st + G::PE + r * 128 + 16 * lane) = u32x4{0, 0, 0, 0};
     }
-    if (lane < WR) {
-      const int r = WR * wave + lane, by = gone ? 127 : byte[0];
-      *reinterpret_cast<float *>(st + G::EXP + 4 * r) = gone ? -INFINITY : (float)(by - 127);
-      if constexpr (F8) {
-        *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = (uint32_t)(254 - by) << 23;
-        *reinterpret_cast<uint32_t *>(st + G::MUL + 4 * r) = by == 255 ? 0x7fc00000u : (uint32_t)by << 23;
-      }
-    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
+    next.landed();
     asm volatile("" ::: "memory");
-    next.slot = pg.row(page, row_of(tile + PD));
-    next.spread();
-    page = pg.page(b, row_of(tile + PD + 1));  // (loaded a tile ahead: a load waits for every copy before it)
-    byte[PD] = byte_of(next.slot);
   }
   AMLA_DEV uint8_t *next_stage() const { return sm + (cur + PD) % NST * Stage<F8>::SIZE; }
-  // After the copies of `next` went out
-  AMLA_DEV void advance() {
+  // After tile `tile`: `next` went out during it
+  AMLA_DEV void advance(int tile) {
 #pragma unroll
     for (int d = 0; d < PD; ++d) byte[d] = byte[d + 1];
     cur = cur + 1 == NST ? 0 : cur + 1;
+    prepare(tile + PD);
+    factors(tile + 1);
   }
 };
 
@@ -716,8 +764,8 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
       feed.arrive(tile);
       base = lds0 + feed.cur * G::SIZE;
       score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
-      feed.advance();
       value_phase<F8, HG, MASK, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE);
+      feed.advance(tile);
     }
     value_phase<F8, HG, MASK, false>(w, base, base, cg, p.scale_log2, 0);
     settle(w.o);
@@ -776,7 +824,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
   const int b = blockIdx.y, row = blockIdx.x;
   const SplitPlan<Tile<F8>::ROWS> plan(p);
   const int2 at = plan.of(b);
-  const int n = __builtin_amdgcn_readfirstlane(at.y);
+  const int n = at.y;
   if (n == 1) return;
   const size_t dst = (size_t)b * p.rows + row;
   u32x4 *od = reinterpret_cast<u32x4 *>(p.out + dst * LC_LORA) + lane;
