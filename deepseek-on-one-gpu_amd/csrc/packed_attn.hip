@@ -11,11 +11,9 @@
 namespace amla {
 
 constexpr int PA_KT = 64;                 // keys per tile
-constexpr int PA_NW = 8;                  // waves per workgroup, 32 queries each
-constexpr int PA_QB = 32 * PA_NW;         // queries per workgroup
-constexpr int PA_NST = 3;                 // LDS stages: copies run up to two tiles ahead
+constexpr int PA_QB = 256;                // queries per workgroup: four waves, two groups of 32 each
+constexpr int PA_NST = 3;                 // LDS stages: a tile, the one before it (values), the one to come
 constexpr int PA_VD = 128;
-constexpr float PA_LAG = 40.f;            // the running maximum moves when a score passes it by 2^40: fp32 and bf16 have the range
 constexpr int PA_HALF = PA_KT * 128;      // 64 rows of 128 bytes: 64 key or value columns of a tile
 
 struct PackedParams {
@@ -30,12 +28,7 @@ struct PackedParams {
 };
 
 // Offsets are not checked on the host: clamped to the rows there are, and none below its predecessor's.
-struct PackedSpan {
-  int q0, nq, k0, nk;
-};
 AMLA_DEV int span_start(const int32_t *off, int b, int rows) { return min(max(off[b], 0), rows); }
-
-AMLA_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // Query block `tile` of the batch: (sequence, block of it), wave-uniform; the sequence is -1 past the end.
 AMLA_DEV int2 find_block(const PackedParams &p, int tile) {
@@ -64,144 +57,434 @@ AMLA_DEV int2 find_block(const PackedParams &p, int tile) {
   return int2{-1, 0};
 }
 
-// ROPE: 64 more key columns beside the first 128
-template <bool ROPE>
-__global__ __launch_bounds__(64 * PA_NW, 1) void packed_attn_kernel(PackedParams p) {
-  extern __shared__ __align__(16) uint8_t sm[];
-  constexpr int KS = ROPE ? 12 : 8;        // 16-wide K steps
-  constexpr int NK = ROPE ? 3 : 2;         // half-row arrays of keys
-  constexpr int VAL = NK * PA_HALF, STAGE = (NK + 2) * PA_HALF;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j32 = lane & 31, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+// ---------------------------------------------------------------- one wave's part of a tile
+//
+// Scores S^T (keys x queries) = K Q^T and outputs O^T (columns x queries) += V^T P^T, 32x32x16
+// products; lane l holds column l % 32, so a query's statistics stay in its two lanes and P
+// goes from the score registers into the product as it is.  64 queries a wave: each fragment
+// read from LDS feeds two products (with 32 the reads alone take as long as the matrix units).
 
-  const int h = blockIdx.x % p.heads;
+template <bool ROPE> struct PackedWave {
+  static constexpr int KS = ROPE ? 12 : 8, NK = ROPE ? 3 : 2;  // 16-wide steps and 64-wide arrays of a key
+  static constexpr int VAL = NK * PA_HALF, STAGE = (NK + 2) * PA_HALF, COPIES = 2 * (NK + 2);
+  bf16x8 q[2][KS];
+  f32x16 o[2][4];  // [group][32 columns]
+  f32x16 s[2][2];  // scores of the tile in work: [group][32 keys]
+  f32x16 t[2];     // second 32 keys of the tile before, not yet exponentiated
+  u32x4 p[2][4];   // P of the tile before, 16 keys each
+  float m[2], l[2], top[2];  // reference (log2 units), sum of 2^(z - m), largest score so far
+};
+// The reference m is the maximum of the first tile that shows a row any key: fp32 and bf16 have the range for
+// sums up to 2^PA_LAG above it.  A row that passes it has the workgroup start over with m from all keys.
+constexpr float PA_LAG = 60.f, PA_NONE = -1e30f;
+
+template <int OFS> AMLA_DEV u32x4 pa_read16(uint32_t addr) {
+  u32x4 v;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFS) : "memory");
+  return v;
+}
+template <int OFS> AMLA_DEV u32x2 pa_read_tr(uint32_t addr) {
+  u32x2 v;
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFS) : "memory");
+  return v;
+}
+template <int N> AMLA_DEV void pa_wait() { asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(N) : "memory"); }
+template <typename T> AMLA_DEV void pa_tie(T &v) { asm volatile("" : "+v"(v)::"memory"); }
+// Scores in vector registers, queries and outputs in accumulator registers (inline asm: left to itself the compiler moves
+// accumulators between the two every tile).  The wait states cover moves of the operands just before.
+AMLA_DEV void pa_score(f32x16 &c, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+}
+AMLA_DEV void pa_score0(f32x16 &c, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b));
+}
+AMLA_DEV void pa_value(f32x16 &c, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+AMLA_DEV void pa_settle() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
+
+// Where a wave's copies come from: rows 16 w .. + 15 of a tile, as 8-row pieces of 128-byte half-rows.  Bases are
+// uniform, each lane adds a fixed offset; chunk c of row r of a key array sits at c ^ ((r >> 1) & 7), the 64-byte
+// half g of a value row at g ^ ((r >> 2) & 1), both free of bank conflicts.
+struct PackedFeed {
+  const char *k, *v, *pe;       // the head's first key, value and rope key of the sequence
+  int64_t ldk, ldv, ldpe;       // bytes of a row
+  int klim, row0;               // keys in use, the wave's first row of a tile
+  uint32_t ok[2], ov, op[2];    // lane offsets
+  AMLA_DEV void init(int lane) {
+    const int r8 = lane >> 3;
+    const uint32_t rr = klim < PA_KT ? 0 : r8;  // fewer keys than a tile: any row in bounds, nothing of it is used
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const uint32_t kc = 16 * ((lane & 7) ^ ((r8 >> 1) + 4 * g));
+      ok[g] = rr * (uint32_t)ldk + kc;
+      op[g] = rr * (uint32_t)ldpe + kc;
+    }
+    ov = rr * (uint32_t)ldv + 16 * ((lane & 7) ^ (4 * ((r8 >> 2) & 1)));
+  }
+  // First key of the tile that is loaded as tile j: the last one ends with the last key (what it repeats is masked).
+  AMLA_DEV int first(int j) const { return max(min(j * PA_KT, klim - PA_KT), 0); }
+  // copy I of tile j
+  template <bool ROPE, int I> AMLA_DEV void copy(int j, uint8_t *st) const {
+    constexpr int NK = ROPE ? 3 : 2, arr = I >> 1, g = I & 1;
+    const int64_t row = klim < PA_KT ? 0 : first(j) + row0 + 8 * g;
+    uint8_t *dst = st + arr * PA_HALF + (row0 + 8 * g) * 128;
+    if constexpr (arr >= NK) copy_lds(v + row * ldv + 128 * (arr - NK) + ov, dst);
+    else if constexpr (arr == 2) copy_lds(pe + row * ldpe + op[g], dst);
+    else copy_lds(k + row * ldk + 128 * arr + ok[g], dst);
+  }
+  // Tile 0 with every row clamped to the keys there are
+  template <bool ROPE> AMLA_DEV void copy_first(uint8_t *st, int lane) const {
+    constexpr int NK = ROPE ? 3 : 2;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int r8 = lane >> 3;
+      const int64_t row = min(row0 + 8 * g + r8, klim - 1);
+      const int kc = 16 * ((lane & 7) ^ ((r8 >> 1) + 4 * g)), vc = 16 * ((lane & 7) ^ (4 * ((r8 >> 2) & 1)));
+      uint8_t *dst = st + (row0 + 8 * g) * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        copy_lds(k + row * ldk + 128 * h + kc, dst + h * PA_HALF);
+        copy_lds(v + row * ldv + 128 * h + vc, dst + (NK + h) * PA_HALF);
+      }
+      if constexpr (ROPE) copy_lds(pe + row * ldpe + kc, dst + 2 * PA_HALF);
+    }
+  }
+  template <bool ROPE, int I = 0> AMLA_DEV void copy_all(int j, uint8_t *st) const {
+    if constexpr (I < 2 * ((ROPE ? 3 : 2) + 2)) {
+      copy<ROPE, I>(j, st);
+      copy_all<ROPE, I + 1>(j, st);
+    }
+  }
+};
+
+// Four probabilities of group G: keys 4 Q4 .. of 32, from score registers
+template <bool ROPE, int G, int Q4> AMLA_DEV void pa_exp(PackedWave<ROPE> &w, u32x4 &p, const f32x16 &z, float c) {
+  float e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * Q4 + i], c, -w.m[G]));
+  w.l[G] += (e[0] + e[1]) + (e[2] + e[3]);
+  p[2 * (Q4 & 1)] = pack_bf16(e[0], e[1]);
+  p[2 * (Q4 & 1) + 1] = pack_bf16(e[2], e[3]);
+}
+
+constexpr int PA_KEY_AHEAD = 3, PA_VAL_AHEAD = 2;  // steps that LDS reads go out ahead
+
+template <bool ROPE, int I> AMLA_DEV void pa_key_read(u32x4 (&ka)[2], uint32_t kr) {
+  const uint32_t a = kr ^ (32 * (I & 3));
+  ka[0] = pa_read16<(I >> 2) * PA_HALF>(a);
+  ka[1] = pa_read16<(I >> 2) * PA_HALF + 32 * 128>(a);
+}
+// Step I of the scores; between its products the copies of tile j and, one slice of four a step, what is left of the
+// softmax of the tile before
+template <bool ROPE, int I>
+AMLA_DEV void pa_score_step(PackedWave<ROPE> &w, u32x4 (&ka)[PA_KEY_AHEAD + 1][2], uint32_t kr, float c, const PackedFeed &f,
+                            int j, uint8_t *st) {
+  constexpr int KS = PackedWave<ROPE>::KS, COPIES = PackedWave<ROPE>::COPIES, A = PA_KEY_AHEAD;
+  if constexpr (I < KS) {
+    if constexpr (I + A < KS) pa_key_read<ROPE, I + A>(ka[(I + A) % (A + 1)], kr);
+    pa_wait<2 * (KS - 1 - I < A ? KS - 1 - I : A)>();
+    u32x4 x = ka[I % (A + 1)][0], y = ka[I % (A + 1)][1];
+    pa_tie(x);
+    pa_tie(y);
+    if constexpr (I == 0) pa_score0(w.s[0][0], as_bf16x8(x), w.q[0][0]);
+    else pa_score(w.s[0][0], as_bf16x8(x), w.q[0][I]);
+    if constexpr (I < 8) pa_exp<ROPE, I & 1, (I >> 1)>(w, w.p[I & 1][2 + (I >> 2)], w.t[I & 1], c);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (I == 0) pa_score0(w.s[0][1], as_bf16x8(y), w.q[0][0]);
+    else pa_score(w.s[0][1], as_bf16x8(y), w.q[0][I]);
+    if constexpr (KS == 12 ? I >= 1 && I <= COPIES : true) f.copy<ROPE, KS == 12 ? I - 1 : I>(j, st);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (I == 0) pa_score0(w.s[1][0], as_bf16x8(x), w.q[1][0]);
+    else pa_score(w.s[1][0], as_bf16x8(x), w.q[1][I]);
+    if constexpr (I == 0) pa_score0(w.s[1][1], as_bf16x8(y), w.q[1][0]);
+    else pa_score(w.s[1][1], as_bf16x8(y), w.q[1][I]);
+    __builtin_amdgcn_sched_barrier(0);
+    pa_score_step<ROPE, I + 1>(w, ka, kr, c, f, j, st);
+  }
+}
+template <bool ROPE>
+AMLA_DEV void pa_score_phase(PackedWave<ROPE> &w, uint32_t base, float c, const PackedFeed &f, int j, uint8_t *st) {
+  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
+  const uint32_t kr = base + j32 * 128 + 16 * (hh ^ ((j32 >> 1) & 7));
+  u32x4 ka[PA_KEY_AHEAD + 1][2];
+  pa_key_read<ROPE, 0>(ka[0], kr);
+  pa_key_read<ROPE, 1>(ka[1], kr);
+  pa_key_read<ROPE, 2>(ka[2], kr);
+  pa_score_step<ROPE, 0>(w, ka, kr, c, f, j, st);
+  pa_settle();
+#pragma unroll
+  for (int g = 0; g < 2; ++g) asm volatile("" : "+v"(w.s[g][0]), "+v"(w.s[g][1]));
+}
+
+template <int C> AMLA_DEV void pa_val_read(u32x2 (&v)[4], uint32_t v0) {
+  if constexpr (C < 8) {
+    const uint32_t a = v0 ^ (64 * ((C >> 1) & 1));
+    constexpr int ofs = (C >> 2) * PA_HALF + (C & 1) * 4096;
+    v[0] = pa_read_tr<ofs>(a);
+    v[1] = pa_read_tr<ofs + 1024>(a);
+    v[2] = pa_read_tr<ofs + 2048>(a);
+    v[3] = pa_read_tr<ofs + 3072>(a);
+  }
+}
+// MASK: keys lo .. lim - 1 of the tile are seen by the lane's query of group G
+template <bool ROPE, bool MASK, int G, int KEYS> AMLA_DEV void pa_max(PackedWave<ROPE> &w, int lo, int lim) {
+  f32x16 &z = w.s[G][KEYS];
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    if constexpr (MASK) {
+#pragma unroll
+      for (int k = i; k < i + 2; ++k) {
+        const int key = 32 * KEYS + 8 * (k >> 2) + (k & 3);
+        z[k] = key < lim && key >= lo ? z[k] : -INFINITY;
+      }
+    }
+    w.top[G] = __builtin_fmaxf(__builtin_fmaxf(w.top[G], z[i]), z[i + 1]);
+  }
+}
+// Step C of the outputs: 32 columns C / 2, keys 32 (C % 2) .. + 31; between its products the mask and maximum of the
+// scores (steps 0, 1), then the probabilities of their first 32 keys
+template <bool ROPE, bool MASK, bool SOFT, int C>
+AMLA_DEV void pa_value_step(PackedWave<ROPE> &w, u32x2 (&vv)[PA_VAL_AHEAD + 1][4], u32x4 (&pn)[2][2], uint32_t v0, float c, int lo,
+                            int lim0, int lim1) {
+  if constexpr (C < 8) {
+    constexpr int A = PA_VAL_AHEAD, cb = C >> 1, kk = 2 * (C & 1);
+    pa_val_read<C + A>(vv[(C + A) % (A + 1)], v0);
+    pa_wait<4 * (7 - C < A ? 7 - C : A)>();
+    u32x2 a = vv[C % (A + 1)][0], b = vv[C % (A + 1)][1], d = vv[C % (A + 1)][2], e = vv[C % (A + 1)][3];
+    pa_tie(a);
+    pa_tie(b);
+    pa_tie(d);
+    pa_tie(e);
+    const bf16x8 x = as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), y = as_bf16x8(u32x4{d.x, d.y, e.x, e.y});
+    if constexpr (SOFT && C == 2) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(w.top[g]), __float_as_uint(w.top[g]), false, false);
+        w.top[g] = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        w.m[g] = w.m[g] == PA_NONE ? __builtin_fmaxf(ceilf(w.top[g] * c), PA_NONE) : w.m[g];
+      }
+    }
+    pa_value(w.o[0][cb], x, as_bf16x8(w.p[0][kk]));
+    if constexpr (SOFT && C == 0) pa_max<ROPE, MASK, 0, 0>(w, lo, lim0);
+    if constexpr (SOFT && C == 1) pa_max<ROPE, MASK, 1, 0>(w, lo, lim1);
+    __builtin_amdgcn_sched_barrier(0);
+    pa_value(w.o[1][cb], x, as_bf16x8(w.p[1][kk]));
+    if constexpr (SOFT && C == 0) pa_max<ROPE, MASK, 0, 1>(w, lo, lim0);
+    if constexpr (SOFT && C == 1) pa_max<ROPE, MASK, 1, 1>(w, lo, lim1);
+    __builtin_amdgcn_sched_barrier(0);
+    pa_value(w.o[0][cb], y, as_bf16x8(w.p[0][kk + 1]));
+    if constexpr (SOFT && C >= 2 && C < 6) pa_exp<ROPE, 0, C - 2>(w, pn[0][(C - 2) >> 1], w.s[0][0], c);
+    __builtin_amdgcn_sched_barrier(0);
+    pa_value(w.o[1][cb], y, as_bf16x8(w.p[1][kk + 1]));
+    if constexpr (SOFT && C >= 2 && C < 6) pa_exp<ROPE, 1, C - 2>(w, pn[1][(C - 2) >> 1], w.s[1][0], c);
+    __builtin_amdgcn_sched_barrier(0);
+    pa_value_step<ROPE, MASK, SOFT, C + 1>(w, vv, pn, v0, c, lo, lim0, lim1);
+  }
+}
+// O^T += V^T P^T of the tile before (its stage at pv) while the scores of this tile are masked and half of them become
+// probabilities (SOFT)
+template <bool ROPE, bool MASK, bool SOFT>
+AMLA_DEV void pa_value_phase(PackedWave<ROPE> &w, uint32_t pv, float c, int lo, int lim0, int lim1) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+  const uint32_t v0 = pv + PackedWave<ROPE>::VAL + (4 * hh + (L16 >> 2)) * 128 + 64 * hh + 32 * (g16 & 1) + 8 * (L16 & 3);
+  u32x2 vv[PA_VAL_AHEAD + 1][4];
+  u32x4 pn[2][2];
+  pa_val_read<0>(vv[0], v0);
+  pa_val_read<1>(vv[1], v0);
+  pa_value_step<ROPE, MASK, SOFT, 0>(w, vv, pn, v0, c, lo, lim0, lim1);
+  if constexpr (SOFT) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      w.p[g][0] = pn[g][0];
+      w.p[g][1] = pn[g][1];
+      w.t[g] = w.s[g][1];
+    }
+  }
+}
+// The second half of the last tile's probabilities, and its part of the outputs
+template <bool ROPE, int Q4 = 0> AMLA_DEV void pa_last(PackedWave<ROPE> &w, uint32_t pv, float c) {
+  if constexpr (Q4 < 4) {
+    pa_exp<ROPE, 0, Q4>(w, w.p[0][2 + (Q4 >> 1)], w.t[0], c);
+    pa_exp<ROPE, 1, Q4>(w, w.p[1][2 + (Q4 >> 1)], w.t[1], c);
+    pa_last<ROPE, Q4 + 1>(w, pv, c);
+  } else {
+    pa_value_phase<ROPE, false, false>(w, pv, c, 0, 0, 0);
+  }
+}
+
+// The LDS stages in turn: the tile in work, the one before it, the one on its way
+template <bool ROPE> struct PackedStages {
+  uint32_t first, now, before;
+  AMLA_DEV void arrive() const {  // this tile landed in every wave, and no wave reads the stage two tiles back any more
+    wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  AMLA_DEV uint32_t next() const {
+    const uint32_t n = now + PackedWave<ROPE>::STAGE;
+    return n == first + PA_NST * PackedWave<ROPE>::STAGE ? first : n;
+  }
+  AMLA_DEV void advance() {
+    before = now;
+    now = next();
+  }
+};
+
+// ROPE: 64 more key columns beside the first 128.  One workgroup of four waves per head and block of 256 queries.
+template <bool ROPE>
+__global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
+  extern __shared__ __align__(1024) uint8_t sm[];
+  using W = PackedWave<ROPE>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j32 = lane & 31, hh = lane >> 5;
+
+  // workgroup i runs on XCD i % 8: a head's blocks, and heads that share keys, come from the same L2 where heads divide
+  const int i = blockIdx.x % p.heads;
+  const int h = p.heads % 8 ? i : (i & 7) * (p.heads >> 3) + (i >> 3);
   const int2 blk = find_block(p, blockIdx.x / p.heads);
   if (blk.x < 0) return;
-  PackedSpan sp;
-  sp.q0 = span_start(p.offsets, blk.x, p.q_rows);
-  sp.nq = span_start(p.offsets, blk.x + 1, p.q_rows) - sp.q0;
-  sp.k0 = span_start(p.k_offsets, blk.x, p.k_rows);
-  sp.nk = max(span_start(p.k_offsets, blk.x + 1, p.k_rows) - sp.k0, 0);
-  const int s_begin = blk.y * PA_QB, s_wave = s_begin + 32 * wave;
-  const int past = sp.nk - sp.nq;  // keys before the first query's own (causal)
-  const int klim = p.causal ? min(sp.nk, max(past + min(s_begin + PA_QB, sp.nq), 0)) : sp.nk;  // keys the block needs
+  const int q0 = span_start(p.offsets, blk.x, p.q_rows), nq = span_start(p.offsets, blk.x + 1, p.q_rows) - q0;
+  const int k0 = span_start(p.k_offsets, blk.x, p.k_rows);
+  const int nk = max(span_start(p.k_offsets, blk.x + 1, p.k_rows) - k0, 0);
+  const int s_begin = blk.y * PA_QB, s_wave = s_begin + 64 * wave;
+  const int past = nk - nq;  // keys before the first query's own (causal)
+  const int klim = p.causal ? min(nk, max(past + min(s_begin + PA_QB, nq), 0)) : nk;  // keys that the block needs
   const int ntiles = (klim + PA_KT - 1) / PA_KT;
+  // keys that the wave's first query sees, and its last one
+  const int seen_all = s_wave >= nq ? 0 : p.causal ? min(max(past + s_wave + 1, 0), nk) : nk;
+  const int seen_any = s_wave >= nq ? 0 : p.causal ? min(max(past + min(s_wave + 64, nq), 0), nk) : nk;
+  const int n_any = (seen_any + PA_KT - 1) / PA_KT;
+  // tiles wholly seen by all of the wave's queries; the last one may be loaded from further ahead
+  const int n_all = min(seen_all / PA_KT, klim / PA_KT);
+
   const int kvh = h / p.group;
+  PackedFeed f;
+  f.k = reinterpret_cast<const char *>(p.k + k0 * p.ldk + kvh * p.ldk_head);
+  f.v = reinterpret_cast<const char *>(p.v + k0 * p.ldv + kvh * p.ldv_head);
+  f.pe = p.k_pe ? reinterpret_cast<const char *>(p.k_pe + k0 * p.ld_pe) : f.k + 256;
+  f.ldk = 2 * p.ldk;
+  f.ldv = 2 * p.ldv;
+  f.ldpe = p.k_pe ? 2 * p.ld_pe : f.ldk;
+  f.klim = klim;
+  f.row0 = 16 * wave;
+  f.init(lane);
+  if (ntiles > 0) f.copy_first<ROPE>(sm, lane);
 
-  auto copy = [&] __device__(int t0, uint8_t *st) {  // wave w: rows 8w .. 8w+7 of the tile
-    const int r8 = lane >> 3, r = 8 * wave + r8;
-    const size_t t = sp.k0 + min(t0 + r, klim - 1);
-    const int kc = (lane & 7) ^ ((r >> 1) & 7), vc = (lane & 7) ^ (4 * ((r >> 2) & 1));
-    const uint16_t *kr = p.k + t * p.ldk + kvh * p.ldk_head + 8 * kc;
-    const uint16_t *vr = p.v + t * p.ldv + kvh * p.ldv_head + 8 * vc;
-    uint8_t *d = st + 8 * wave * 128;
+  W w;
+  int lim[2];  // keys [0, lim) are seen by the lane's query of each group
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      copy_lds(kr + 64 * half, d + half * PA_HALF);
-      copy_lds(vr + 64 * half, d + VAL + half * PA_HALF);
+  for (int g = 0; g < 2; ++g) {
+    const int iq = min(s_wave + 32 * g + j32, nq - 1);
+    const uint16_t *qp = p.q + (size_t)(q0 + iq) * p.ldq + h * p.ldq_head + 8 * hh;
+#pragma unroll
+    for (int ks = 0; ks < W::KS; ++ks) w.q[g][ks] = as_bf16x8(ldg16(qp + 16 * ks));
+    lim[g] = (p.causal ? min(past + iq + 1, nk) : nk) - 4 * hh;
+    w.m[g] = PA_NONE;
+  }
+  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
+  const float c = p.scale_log2;
+
+  for (;;) {  // once, or twice where m turned out too low
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int cb = 0; cb < 4; ++cb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w.o[g][cb][r] = 0.f;
+        asm volatile("" : "+a"(w.o[g][cb]));
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w.t[g][r] = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w.p[g][k] = u32x4{0, 0, 0, 0};
+      w.l[g] = 0.f;
+      w.top[g] = -INFINITY;
     }
-    if constexpr (ROPE)
-      copy_lds(p.k_pe ? p.k_pe + t * p.ld_pe + 8 * kc : kr + 128, d + 2 * PA_HALF);
-  };
-
-  if (ntiles > 0) copy(0, sm);
-  const int iq = min(s_wave + j32, sp.nq - 1);
-  const uint16_t *qp = p.q + (size_t)(sp.q0 + iq) * p.ldq + h * p.ldq_head + 8 * hh;
-  bf16x8 qf[KS];
+    pa_settle();
+    // nothing before the first tile: probabilities and values of 0
+    PackedStages<ROPE> at{lds0, lds0, lds0 + (PA_NST - 1) * W::STAGE};
+    for (int o = threadIdx.x * 16; o < 2 * PA_HALF; o += 4096)
+      *reinterpret_cast<u32x4 *>(sm + (PA_NST - 1) * W::STAGE + W::VAL + o) = u32x4{0, 0, 0, 0};
+    int j = 0;
+    for (; j < n_all; ++j) {
+      at.arrive();
+      pa_score_phase<ROPE>(w, at.now, c, f, j + 1, sm + (at.next() - lds0));
+      pa_value_phase<ROPE, false, true>(w, at.before, c, 0, 0, 0);
+      at.advance();
+    }
+    for (; j < n_any; ++j) {
+      at.arrive();
+      pa_score_phase<ROPE>(w, at.now, c, f, j + 1, sm + (at.next() - lds0));
+      const int first = f.first(j);
+      pa_value_phase<ROPE, true, true>(w, at.before, c, j * PA_KT - first - 4 * hh, lim[0] - first, lim[1] - first);
+      at.advance();
+    }
+    pa_last<ROPE>(w, at.before, c);
+    for (; j < ntiles; ++j) {  // the wave's queries see no more: it goes on copying for the others
+      at.arrive();
+      f.copy_all<ROPE>(j + 1, sm + (at.next() - lds0));
+      at.advance();
+    }
+    pa_settle();
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qf[ks] = as_bf16x8(ldg16(qp + 16 * ks));
-  f32x16 o[4];
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
-  float m = -1e30f, l = 0.f;  // finite: exp2(-inf - m) is 0 while no key has been seen
-  const int limit = p.causal ? min(past + iq + 1, sp.nk) : sp.nk;  // keys [0, limit) are seen
-  const int seen_by_all = p.causal ? min(past + s_wave + 1, sp.nk) : sp.nk;
-
-  for (int j = 0; j < ntiles; ++j) {
-    uint8_t *st = sm + (j % PA_NST) * STAGE;
-    if (j + 1 < ntiles) copy((j + 1) * PA_KT, sm + ((j + 1) % PA_NST) * STAGE);
-    if (j + 1 < ntiles) wait_vmcnt<ROPE ? 5 : 4>();
-    else wait_vmcnt<0>();
+      for (int cb = 0; cb < 4; ++cb) asm volatile("" : "+a"(w.o[g][cb]));
+    wait_vmcnt<0>();  // (copies past the last tile)
+    const bool low0 = w.top[0] * c > w.m[0] + PA_LAG, low1 = w.top[1] * c > w.m[1] + PA_LAG;
+    // the waves agree: their copies and barriers are common
     __syncthreads();
-    f32x16 s[2];
-#pragma unroll
-    for (int kg = 0; kg < 2; ++kg) {
-      const int r = 32 * kg + j32;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kg][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 a = *reinterpret_cast<const u32x4 *>(st + (ks >> 2) * PA_HALF + r * 128 +
-                                                         16 * ((2 * (ks & 3) + hh) ^ ((r >> 1) & 7)));
-        s[kg] = mfma32(as_bf16x8(a), qf[ks], s[kg]);
-      }
-    }
-    float mx = -INFINITY;
-    const bool masked = (j + 1) * PA_KT > seen_by_all;
-#pragma unroll
-    for (int kg = 0; kg < 2; ++kg)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float z = s[kg][i] * p.scale_log2;
-        if (masked && j * PA_KT + 32 * kg + 8 * (i >> 2) + 4 * hh + (i & 3) >= limit) z = -INFINITY;
-        s[kg][i] = z;
-        mx = __builtin_fmaxf(mx, z);
-      }
-    mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__ballot(mx > m + PA_LAG)) {
-      const float mn = mx > m + PA_LAG ? mx : m, f = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] *= f;
-    }
-    u32x4 pb[4];
-#pragma unroll
-    for (int kg = 0; kg < 2; ++kg)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(s[kg][i] - m), e1 = __builtin_amdgcn_exp2f(s[kg][i + 1] - m);
-        l += e0 + e1;
-        pb[2 * kg + (i >> 3)][(i >> 1) & 3] = pack_bf16(e0, e1);
-      }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        u32x2 t[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = 16 * kk + 8 * i + 4 * hh + (L16 >> 2);
-          const uint8_t *a = st + VAL + (c >> 1) * PA_HALF + r * 128 + 64 * ((c & 1) ^ hh) + 32 * (g16 & 1) + 8 * (L16 & 3);
-          typedef short v4s __attribute__((ext_vector_type(4)));
-          t[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)a));
-        }
-        o[c] = mfma32(as_bf16x8(u32x4{t[0].x, t[0].y, t[1].x, t[1].y}), as_bf16x8(pb[kk]), o[c]);
-      }
+    uint32_t *vote = reinterpret_cast<uint32_t *>(sm);
+    if (lane == 0) vote[wave] = __ballot(low0 || low1) != 0;
+    __syncthreads();
+    const bool again = (vote[0] | vote[1] | vote[2] | vote[3]) != 0;
+    __syncthreads();
+    if (!again) break;
+    w.m[0] = low0 ? ceilf(w.top[0] * c) : w.m[0];
+    w.m[1] = low1 ? ceilf(w.top[1] * c) : w.m[1];
+    f.copy_first<ROPE>(sm, lane);
   }
 
-  l += __shfl_xor(l, 32, 64);
-  if (s_wave + j32 >= sp.nq) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const size_t dst = (size_t)(sp.q0 + s_wave + j32) * p.heads + h;
-  if (p.lse && hh == 0) p.lse[dst] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  // outputs: rows of 256 bytes through LDS (chunk ch of a row at ch ^ (row & 15)), so that a store is whole rows
+  uint8_t *turn = sm + wave * 64 * 256;
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int g = 0; g < 2; ++g) {
+    float l = w.l[g];
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int r = 32 * g + j32;
+    if (p.lse && hh == 0 && s_wave + r < nq)
+      p.lse[(size_t)(q0 + s_wave + r) * p.heads + h] =
+          l == 0.f ? -INFINITY : (w.m[g] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-      *reinterpret_cast<u32x2 *>(p.out + dst * PA_VD + 32 * c + 8 * q4 + 4 * hh) =
-          u32x2{pack_bf16(o[c][4 * q4] * inv, o[c][4 * q4 + 1] * inv), pack_bf16(o[c][4 * q4 + 2] * inv, o[c][4 * q4 + 3] * inv)};
+    for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<u32x2 *>(turn + r * 256 + 16 * ((4 * cb + q4) ^ (j32 & 15)) + 8 * hh) =
+            l == 0.f ? u32x2{0, 0}  // (no key seen: what the products left does not count)
+                     : u32x2{pack_bf16(w.o[g][cb][4 * q4] * inv, w.o[g][cb][4 * q4 + 1] * inv),
+                             pack_bf16(w.o[g][cb][4 * q4 + 2] * inv, w.o[g][cb][4 * q4 + 3] * inv)};
+  }
+  const int held = min(64, nq - s_wave);
+#pragma unroll 4
+  for (int r0 = 0; r0 < 64; r0 += 4) {
+    const int r = r0 + (lane >> 4), ch = lane & 15;
+    if (r < held)
+      *reinterpret_cast<u32x4 *>(p.out + ((size_t)(q0 + s_wave + r) * p.heads + h) * PA_VD + 8 * ch) =
+          *reinterpret_cast<const u32x4 *>(turn + r * 256 + 16 * (ch ^ (r & 15)));
+  }
 }
 
 template <bool ROPE>
 static int launch_packed(const PackedParams &p, int64_t blocks, hipStream_t st) {
-  constexpr int lds = (ROPE ? 5 : 4) * PA_HALF * PA_NST;
+  constexpr int lds = PackedWave<ROPE>::STAGE * PA_NST;
   static const hipError_t attr =
       hipFuncSetAttribute((const void *)packed_attn_kernel<ROPE>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   (void)attr;
-  packed_attn_kernel<ROPE><<<dim3((unsigned)blocks), 64 * PA_NW, lds, st>>>(p);
+  packed_attn_kernel<ROPE><<<dim3((unsigned)blocks), 256, lds, st>>>(p);
   return check_launch("packed_attention");
 }
 
@@ -225,7 +508,7 @@ extern "C" int amla_packed_attention(const amla_packed_args *a, void *stream) {
     return fail(AMLA_EUNSUPPORTED, "%s: at most 2^31 - 1 rows and %d sequences", what, AMLA_MAX_SEQS);
   const int64_t lds[] = {a->ldq, a->ldq_head, a->ldk, a->ldk_head, a->ldv, a->ldv_head, a->k_pe ? a->ld_pe : 0};
   for (int64_t ld : lds)
-    if (ld % 8) return fail(AMLA_EUNSUPPORTED, "%s: strides must be multiples of 8 values", what);
+    if (ld % 8 || ld < 0 || ld > (1 << 27)) return fail(AMLA_EUNSUPPORTED, "%s: strides must be multiples of 8 values up to 2^27", what);
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_pe) || !aligned16(a->out))
     return fail(AMLA_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", what);
   const int64_t tiles = a->q_rows / PA_QB + std::min(a->seqs, a->q_rows);  // at least the blocks there are
