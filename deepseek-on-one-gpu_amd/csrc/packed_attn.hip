@@ -71,7 +71,9 @@ template <bool ROPE> struct PackedWave {
   f32x16 o[2][4];  // [group][32 columns]
   f32x16 s[2][2];  // scores of the tile in work: [group][32 keys]
   f32x16 t[2];     // second 32 keys of the tile before, not yet exponentiated
+  f32x4 u[2];      // nor the last four of its first 32
   u32x4 p[2][4];   // P of the tile before, 16 keys each
+  float e[2];      // a probability that waits for the other half of its register
   float m[2], l[2], top[2];  // reference (log2 units), sum of 2^(z - m), largest score so far
 };
 // The reference m is the maximum of the first tile that shows a row any key: fp32 and bf16 have the range for
@@ -91,15 +93,18 @@ template <int OFS> AMLA_DEV u32x2 pa_read_tr(uint32_t addr) {
 template <int N> AMLA_DEV void pa_wait() { asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(N) : "memory"); }
 template <typename T> AMLA_DEV void pa_tie(T &v) { asm volatile("" : "+v"(v)::"memory"); }
 // Scores in vector registers, queries and outputs in accumulator registers (inline asm: left to itself the compiler moves
-// accumulators between the two every tile).  The wait states cover moves of the operands just before.
-AMLA_DEV void pa_score(f32x16 &c, bf16x8 a, bf16x8 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+// accumulators between the two every tile).
+// WAIT: the step's first product, whose operands the compiler may have moved just before (two wait states); the other
+// products of a step read the same registers.
+template <bool ZERO, bool WAIT> AMLA_DEV void pa_score(f32x16 &c, bf16x8 a, bf16x8 b) {
+  if constexpr (ZERO && WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b));
+  else if constexpr (ZERO) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b));
+  else if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
 }
-AMLA_DEV void pa_score0(f32x16 &c, bf16x8 a, bf16x8 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b));
-}
-AMLA_DEV void pa_value(f32x16 &c, bf16x8 a, bf16x8 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+template <bool WAIT> AMLA_DEV void pa_value(f32x16 &c, bf16x8 a, bf16x8 b) {
+  if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 AMLA_DEV void pa_settle() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
 
@@ -111,6 +116,7 @@ struct PackedFeed {
   int64_t ldk, ldv, ldpe;       // bytes of a row
   int klim, row0;               // keys in use, the wave's first row of a tile
   uint32_t ok[2], ov, op[2];    // lane offsets
+  const char *tk[2], *tv[2], *tp[2];  // rows row0, row0 + 8 of the tile that is copied next
   AMLA_DEV void init(int lane) {
     const int r8 = lane >> 3;
     const uint32_t rr = klim < PA_KT ? 0 : r8;  // fewer keys than a tile: any row in bounds, nothing of it is used
@@ -124,14 +130,22 @@ struct PackedFeed {
   }
   // First key of the tile that is loaded as tile j: the last one ends with the last key (what it repeats is masked).
   AMLA_DEV int first(int j) const { return max(min(j * PA_KT, klim - PA_KT), 0); }
-  // copy I of tile j
-  template <bool ROPE, int I> AMLA_DEV void copy(int j, uint8_t *st) const {
+  AMLA_DEV void aim(int j) {
+    const int64_t row = klim < PA_KT ? 0 : first(j) + row0, more = klim < PA_KT ? 0 : 8;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      tk[g] = k + (row + more * g) * ldk;
+      tv[g] = v + (row + more * g) * ldv;
+      tp[g] = pe + (row + more * g) * ldpe;
+    }
+  }
+  // copy I of the tile aimed at
+  template <bool ROPE, int I> AMLA_DEV void copy(uint8_t *st) const {
     constexpr int NK = ROPE ? 3 : 2, arr = I >> 1, g = I & 1;
-    const int64_t row = klim < PA_KT ? 0 : first(j) + row0 + 8 * g;
     uint8_t *dst = st + arr * PA_HALF + (row0 + 8 * g) * 128;
-    if constexpr (arr >= NK) copy_lds(v + row * ldv + 128 * (arr - NK) + ov, dst);
-    else if constexpr (arr == 2) copy_lds(pe + row * ldpe + op[g], dst);
-    else copy_lds(k + row * ldk + 128 * arr + ok[g], dst);
+    if constexpr (arr >= NK) copy_lds(tv[g] + 128 * (arr - NK) + ov, dst);
+    else if constexpr (arr == 2) copy_lds(tp[g] + op[g], dst);
+    else copy_lds(tk[g] + 128 * arr + ok[g], dst);
   }
   // Tile 0 with every row clamped to the keys there are
   template <bool ROPE> AMLA_DEV void copy_first(uint8_t *st, int lane) const {
@@ -150,22 +164,49 @@ struct PackedFeed {
       if constexpr (ROPE) copy_lds(pe + row * ldpe + kc, dst + 2 * PA_HALF);
     }
   }
-  template <bool ROPE, int I = 0> AMLA_DEV void copy_all(int j, uint8_t *st) const {
+  template <bool ROPE, int I = 0> AMLA_DEV void copy_all(uint8_t *st) const {
     if constexpr (I < 2 * ((ROPE ? 3 : 2) + 2)) {
-      copy<ROPE, I>(j, st);
-      copy_all<ROPE, I + 1>(j, st);
+      copy<ROPE, I>(st);
+      copy_all<ROPE, I + 1>(st);
     }
   }
 };
 
-// Four probabilities of group G: keys 4 Q4 .. of 32, from score registers
-template <bool ROPE, int G, int Q4> AMLA_DEV void pa_exp(PackedWave<ROPE> &w, u32x4 &p, const f32x16 &z, float c) {
-  float e[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * Q4 + i], c, -w.m[G]));
-  w.l[G] += (e[0] + e[1]) + (e[2] + e[3]);
-  p[2 * (Q4 & 1)] = pack_bf16(e[0], e[1]);
-  p[2 * (Q4 & 1) + 1] = pack_bf16(e[2], e[3]);
+// Probability N of the 32 that follow each other in a group's registers (first 32 keys: 0 .. 15, second: 16 .. 31), by two
+// groups: one exponential is what hides behind one product
+template <int N> AMLA_DEV void pa_exp(float z, float c, float m, float &l, float &e, uint32_t &p) {
+  const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -m));
+  if constexpr (N & 1) {
+    p = pack_bf16(e, x);
+    l += e + x;
+  } else {
+    e = x;
+  }
+}
+constexpr int PA_EARLY = 12;  // of the 32, those that the value products take; the next scores' products the others
+// I: 0 .. 2 PA_EARLY - 1, the early ones
+template <bool ROPE, int I> AMLA_DEV void pa_soft_early(PackedWave<ROPE> &w, u32x4 (&pn)[2][2], float c) {
+  constexpr int g = I & 1, n = I >> 1;
+  float l = w.l[g], e = w.e[g];
+  uint32_t p = 0;
+  pa_exp<n>(w.s[g][0][n], c, w.m[g], l, e, p);
+  w.l[g] = l;
+  w.e[g] = e;
+  if constexpr (n & 1) pn[g][n >> 3][(n >> 1) & 3] = p;
+}
+// I: 0 .. 2 (32 - PA_EARLY) - 1, the late ones
+template <bool ROPE, int I> AMLA_DEV void pa_soft_late(PackedWave<ROPE> &w, float c) {
+  constexpr int g = I & 1, n = PA_EARLY + (I >> 1);
+  if constexpr (n < 32) {
+    float l = w.l[g], e = w.e[g], z;
+    uint32_t p = 0;
+    if constexpr (n < 16) z = w.u[g][n - PA_EARLY];
+    else z = w.t[g][n - 16];
+    pa_exp<n>(z, c, w.m[g], l, e, p);
+    w.l[g] = l;
+    w.e[g] = e;
+    if constexpr (n & 1) w.p[g][n >> 3][(n >> 1) & 3] = p;
+  }
 }
 
 constexpr int PA_KEY_AHEAD = 3, PA_VAL_AHEAD = 2;  // steps that LDS reads go out ahead
@@ -175,43 +216,52 @@ template <bool ROPE, int I> AMLA_DEV void pa_key_read(u32x4 (&ka)[2], uint32_t k
   ka[0] = pa_read16<(I >> 2) * PA_HALF>(a);
   ka[1] = pa_read16<(I >> 2) * PA_HALF + 32 * 128>(a);
 }
-// Step I of the scores; between its products the copies of tile j and, one slice of four a step, what is left of the
-// softmax of the tile before
+// What goes behind product K of score step I: a copy of the tile to come (one a step) or late probabilities
+template <bool ROPE, int I, int K> AMLA_DEV void pa_score_slot(PackedWave<ROPE> &w, float c, const PackedFeed &f, uint8_t *st) {
+  if constexpr (!ROPE) {  // 40 probabilities and 8 copies behind 32 products
+    if constexpr (K == 0) f.copy<ROPE, I>(st);
+    if constexpr (K == 1 || K == 2) pa_soft_late<ROPE, 5 * I + 2 * K - 2>(w, c);
+    if constexpr (K > 0) pa_soft_late<ROPE, 5 * I + (K == 3 ? 4 : 2 * K - 1)>(w, c);
+  } else if constexpr (I == 0 || I == 11) {  // 40 and 10 behind 48: 5 probabilities in the outer steps, 3 in the others
+    constexpr int L = I == 0 ? 0 : 35;
+    if constexpr (K == 0) pa_soft_late<ROPE, L>(w, c);
+    pa_soft_late<ROPE, L + 1 + K>(w, c);
+  } else {
+    if constexpr (K == 0) f.copy<ROPE, I - 1>(st);
+    else pa_soft_late<ROPE, 5 + 3 * (I - 1) + K - 1>(w, c);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
 template <bool ROPE, int I>
 AMLA_DEV void pa_score_step(PackedWave<ROPE> &w, u32x4 (&ka)[PA_KEY_AHEAD + 1][2], uint32_t kr, float c, const PackedFeed &f,
-                            int j, uint8_t *st) {
-  constexpr int KS = PackedWave<ROPE>::KS, COPIES = PackedWave<ROPE>::COPIES, A = PA_KEY_AHEAD;
+                            uint8_t *st) {
+  constexpr int KS = PackedWave<ROPE>::KS, A = PA_KEY_AHEAD;
   if constexpr (I < KS) {
     if constexpr (I + A < KS) pa_key_read<ROPE, I + A>(ka[(I + A) % (A + 1)], kr);
     pa_wait<2 * (KS - 1 - I < A ? KS - 1 - I : A)>();
     u32x4 x = ka[I % (A + 1)][0], y = ka[I % (A + 1)][1];
     pa_tie(x);
     pa_tie(y);
-    if constexpr (I == 0) pa_score0(w.s[0][0], as_bf16x8(x), w.q[0][0]);
-    else pa_score(w.s[0][0], as_bf16x8(x), w.q[0][I]);
-    if constexpr (I < 8) pa_exp<ROPE, I & 1, (I >> 1)>(w, w.p[I & 1][2 + (I >> 2)], w.t[I & 1], c);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (I == 0) pa_score0(w.s[0][1], as_bf16x8(y), w.q[0][0]);
-    else pa_score(w.s[0][1], as_bf16x8(y), w.q[0][I]);
-    if constexpr (KS == 12 ? I >= 1 && I <= COPIES : true) f.copy<ROPE, KS == 12 ? I - 1 : I>(j, st);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (I == 0) pa_score0(w.s[1][0], as_bf16x8(x), w.q[1][0]);
-    else pa_score(w.s[1][0], as_bf16x8(x), w.q[1][I]);
-    if constexpr (I == 0) pa_score0(w.s[1][1], as_bf16x8(y), w.q[1][0]);
-    else pa_score(w.s[1][1], as_bf16x8(y), w.q[1][I]);
-    __builtin_amdgcn_sched_barrier(0);
-    pa_score_step<ROPE, I + 1>(w, ka, kr, c, f, j, st);
+    pa_score<I == 0, true>(w.s[0][0], as_bf16x8(x), w.q[0][I]);
+    pa_score_slot<ROPE, I, 0>(w, c, f, st);
+    pa_score<I == 0, false>(w.s[0][1], as_bf16x8(y), w.q[0][I]);
+    pa_score_slot<ROPE, I, 1>(w, c, f, st);
+    pa_score<I == 0, false>(w.s[1][0], as_bf16x8(x), w.q[1][I]);
+    pa_score_slot<ROPE, I, 2>(w, c, f, st);
+    pa_score<I == 0, false>(w.s[1][1], as_bf16x8(y), w.q[1][I]);
+    pa_score_slot<ROPE, I, 3>(w, c, f, st);
+    pa_score_step<ROPE, I + 1>(w, ka, kr, c, f, st);
   }
 }
 template <bool ROPE>
-AMLA_DEV void pa_score_phase(PackedWave<ROPE> &w, uint32_t base, float c, const PackedFeed &f, int j, uint8_t *st) {
+AMLA_DEV void pa_score_phase(PackedWave<ROPE> &w, uint32_t base, float c, const PackedFeed &f, uint8_t *st) {
   const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
   const uint32_t kr = base + j32 * 128 + 16 * (hh ^ ((j32 >> 1) & 7));
   u32x4 ka[PA_KEY_AHEAD + 1][2];
   pa_key_read<ROPE, 0>(ka[0], kr);
   pa_key_read<ROPE, 1>(ka[1], kr);
   pa_key_read<ROPE, 2>(ka[2], kr);
-  pa_score_step<ROPE, 0>(w, ka, kr, c, f, j, st);
+  pa_score_step<ROPE, 0>(w, ka, kr, c, f, st);
   pa_settle();
 #pragma unroll
   for (int g = 0; g < 2; ++g) asm volatile("" : "+v"(w.s[g][0]), "+v"(w.s[g][1]));
@@ -228,10 +278,10 @@ template <int C> AMLA_DEV void pa_val_read(u32x2 (&v)[4], uint32_t v0) {
   }
 }
 // MASK: keys lo .. lim - 1 of the tile are seen by the lane's query of group G
-template <bool ROPE, bool MASK, int G, int KEYS> AMLA_DEV void pa_max(PackedWave<ROPE> &w, int lo, int lim) {
+template <bool ROPE, bool MASK, int G, int KEYS, int HALF> AMLA_DEV void pa_max(PackedWave<ROPE> &w, int lo, int lim) {
   f32x16 &z = w.s[G][KEYS];
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
+  for (int i = 8 * HALF; i < 8 * HALF + 8; i += 2) {
     if constexpr (MASK) {
 #pragma unroll
       for (int k = i; k < i + 2; ++k) {
@@ -242,8 +292,30 @@ template <bool ROPE, bool MASK, int G, int KEYS> AMLA_DEV void pa_max(PackedWave
     w.top[G] = __builtin_fmaxf(__builtin_fmaxf(w.top[G], z[i]), z[i + 1]);
   }
 }
-// Step C of the outputs: 32 columns C / 2, keys 32 (C % 2) .. + 31; between its products the mask and maximum of the
-// scores (steps 0, 1), then the probabilities of their first 32 keys
+// Both lanes of a query agree on its largest score so far; the first one sets its reference
+AMLA_DEV void pa_refer(float &top, float &m, float c) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+  top = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+  m = m == PA_NONE ? __builtin_fmaxf(ceilf(top * c), PA_NONE) : m;
+}
+// What goes behind value product N: a part of the mask and the maximum of the scores (0 .. 7), the reference, then an early
+// probability each
+template <bool ROPE, bool MASK, bool SOFT, int N>
+AMLA_DEV void pa_value_slot(PackedWave<ROPE> &w, u32x4 (&pn)[2][2], float c, int lo, int lim0, int lim1) {
+  if constexpr (SOFT) {
+    if constexpr (N < 8) {
+      pa_max<ROPE, MASK, (N & 1), ((N >> 2) & 1), ((N >> 1) & 1)>(w, lo, N & 1 ? lim1 : lim0);
+    } else {
+      if constexpr (N == 8) {
+        pa_refer(w.top[0], w.m[0], c);
+        pa_refer(w.top[1], w.m[1], c);
+      }
+      pa_soft_early<ROPE, N - 8>(w, pn, c);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Step C of the outputs: 32 columns C / 2, keys 32 (C % 2) .. + 31
 template <bool ROPE, bool MASK, bool SOFT, int C>
 AMLA_DEV void pa_value_step(PackedWave<ROPE> &w, u32x2 (&vv)[PA_VAL_AHEAD + 1][4], u32x4 (&pn)[2][2], uint32_t v0, float c, int lo,
                             int lim0, int lim1) {
@@ -257,28 +329,14 @@ AMLA_DEV void pa_value_step(PackedWave<ROPE> &w, u32x2 (&vv)[PA_VAL_AHEAD + 1][4
     pa_tie(d);
     pa_tie(e);
     const bf16x8 x = as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), y = as_bf16x8(u32x4{d.x, d.y, e.x, e.y});
-    if constexpr (SOFT && C == 2) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(w.top[g]), __float_as_uint(w.top[g]), false, false);
-        w.top[g] = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        w.m[g] = w.m[g] == PA_NONE ? __builtin_fmaxf(ceilf(w.top[g] * c), PA_NONE) : w.m[g];
-      }
-    }
-    pa_value(w.o[0][cb], x, as_bf16x8(w.p[0][kk]));
-    if constexpr (SOFT && C == 0) pa_max<ROPE, MASK, 0, 0>(w, lo, lim0);
-    if constexpr (SOFT && C == 1) pa_max<ROPE, MASK, 1, 0>(w, lo, lim1);
-    __builtin_amdgcn_sched_barrier(0);
-    pa_value(w.o[1][cb], x, as_bf16x8(w.p[1][kk]));
-    if constexpr (SOFT && C == 0) pa_max<ROPE, MASK, 0, 1>(w, lo, lim0);
-    if constexpr (SOFT && C == 1) pa_max<ROPE, MASK, 1, 1>(w, lo, lim1);
-    __builtin_amdgcn_sched_barrier(0);
-    pa_value(w.o[0][cb], y, as_bf16x8(w.p[0][kk + 1]));
-    if constexpr (SOFT && C >= 2 && C < 6) pa_exp<ROPE, 0, C - 2>(w, pn[0][(C - 2) >> 1], w.s[0][0], c);
-    __builtin_amdgcn_sched_barrier(0);
-    pa_value(w.o[1][cb], y, as_bf16x8(w.p[1][kk + 1]));
-    if constexpr (SOFT && C >= 2 && C < 6) pa_exp<ROPE, 1, C - 2>(w, pn[1][(C - 2) >> 1], w.s[1][0], c);
-    __builtin_amdgcn_sched_barrier(0);
+    pa_value<true>(w.o[0][cb], x, as_bf16x8(w.p[0][kk]));
+    pa_value_slot<ROPE, MASK, SOFT, 4 * C>(w, pn, c, lo, lim0, lim1);
+    pa_value<false>(w.o[1][cb], x, as_bf16x8(w.p[1][kk]));
+    pa_value_slot<ROPE, MASK, SOFT, 4 * C + 1>(w, pn, c, lo, lim0, lim1);
+    pa_value<true>(w.o[0][cb], y, as_bf16x8(w.p[0][kk + 1]));
+    pa_value_slot<ROPE, MASK, SOFT, 4 * C + 2>(w, pn, c, lo, lim0, lim1);
+    pa_value<false>(w.o[1][cb], y, as_bf16x8(w.p[1][kk + 1]));
+    pa_value_slot<ROPE, MASK, SOFT, 4 * C + 3>(w, pn, c, lo, lim0, lim1);
     pa_value_step<ROPE, MASK, SOFT, C + 1>(w, vv, pn, v0, c, lo, lim0, lim1);
   }
 }
@@ -297,17 +355,18 @@ AMLA_DEV void pa_value_phase(PackedWave<ROPE> &w, uint32_t pv, float c, int lo, 
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       w.p[g][0] = pn[g][0];
-      w.p[g][1] = pn[g][1];
+      w.p[g][1].x = pn[g][1].x;
+      w.p[g][1].y = pn[g][1].y;
+      w.u[g] = __builtin_shufflevector(w.s[g][0], w.s[g][0], 12, 13, 14, 15);
       w.t[g] = w.s[g][1];
     }
   }
 }
-// The second half of the last tile's probabilities, and its part of the outputs
-template <bool ROPE, int Q4 = 0> AMLA_DEV void pa_last(PackedWave<ROPE> &w, uint32_t pv, float c) {
-  if constexpr (Q4 < 4) {
-    pa_exp<ROPE, 0, Q4>(w, w.p[0][2 + (Q4 >> 1)], w.t[0], c);
-    pa_exp<ROPE, 1, Q4>(w, w.p[1][2 + (Q4 >> 1)], w.t[1], c);
-    pa_last<ROPE, Q4 + 1>(w, pv, c);
+// What is left of the last tile's probabilities, and its part of the outputs
+template <bool ROPE, int I = 0> AMLA_DEV void pa_last(PackedWave<ROPE> &w, uint32_t pv, float c) {
+  if constexpr (I < 2 * (32 - PA_EARLY)) {
+    pa_soft_late<ROPE, I>(w, c);
+    pa_last<ROPE, I + 1>(w, pv, c);
   } else {
     pa_value_phase<ROPE, false, false>(w, pv, c, 0, 0, 0);
   }
@@ -397,6 +456,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) w.t[g][r] = -INFINITY;
+      w.u[g] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int k = 0; k < 4; ++k) w.p[g][k] = u32x4{0, 0, 0, 0};
       w.l[g] = 0.f;
@@ -410,13 +470,15 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     int j = 0;
     for (; j < n_all; ++j) {
       at.arrive();
-      pa_score_phase<ROPE>(w, at.now, c, f, j + 1, sm + (at.next() - lds0));
+      f.aim(j + 1);
+      pa_score_phase<ROPE>(w, at.now, c, f, sm + (at.next() - lds0));
       pa_value_phase<ROPE, false, true>(w, at.before, c, 0, 0, 0);
       at.advance();
     }
     for (; j < n_any; ++j) {
       at.arrive();
-      pa_score_phase<ROPE>(w, at.now, c, f, j + 1, sm + (at.next() - lds0));
+      f.aim(j + 1);
+      pa_score_phase<ROPE>(w, at.now, c, f, sm + (at.next() - lds0));
       const int first = f.first(j);
       pa_value_phase<ROPE, true, true>(w, at.before, c, j * PA_KT - first - 4 * hh, lim[0] - first, lim[1] - first);
       at.advance();
@@ -424,7 +486,8 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     pa_last<ROPE>(w, at.before, c);
     for (; j < ntiles; ++j) {  // the wave's queries see no more: it goes on copying for the others
       at.arrive();
-      f.copy_all<ROPE>(j + 1, sm + (at.next() - lds0));
+      f.aim(j + 1);
+      f.copy_all<ROPE>(sm + (at.next() - lds0));
       at.advance();
     }
     pa_settle();
