@@ -73,7 +73,7 @@ template <bool ROPE> struct PackedWave {
   f32x16 t[2];     // second 32 keys of the tile before, not yet exponentiated
   f32x4 u[2];      // nor the last four of its first 32
   u32x4 p[2][4];   // P of the tile before, 16 keys each
-  float e[2];      // a probability that waits for the other half of its register
+  float x[2][2];   // the last two probabilities, not yet summed and packed
   float m[2], l[2], top[2];  // reference (log2 units), sum of 2^(z - m), largest score so far
 };
 // The reference m is the maximum of the first tile that shows a row any key: fp32 and bf16 have the range for
@@ -172,49 +172,48 @@ struct PackedFeed {
   }
 };
 
-// Probability N of the 32 that follow each other in a group's registers (first 32 keys: 0 .. 15, second: 16 .. 31), by two
-// groups: one exponential is what hides behind one product
-template <int N> AMLA_DEV void pa_exp(float z, float c, float m, float &l, float &e, uint32_t &p) {
-  const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -m));
-  if constexpr (N & 1) {
-    p = pack_bf16(e, x);
-    l += e + x;
-  } else {
-    e = x;
-  }
+// Softmax, one exponential behind each product.  A group's 32 probabilities a tile are numbered as they follow each other
+// in its registers (first 32 keys: 0 .. 15, second: 16 .. 31); the value products take the first PA_EARLY, the next
+// scores' products the others, both groups in turn.  A result is summed and packed one turn later: it is not waited for.
+constexpr int PA_EARLY = 12;
+template <bool ROPE, int G, int N> AMLA_DEV void pa_turn(PackedWave<ROPE> &w, u32x4 (&p)[4], float z, float c) {
+  const float y = __builtin_fmaf(z, c, -w.m[G]);
+  if constexpr (N > 0 && N % 2 == 0) p[(N - 2) >> 3][((N - 2) >> 1) & 3] = pack_bf16(w.x[G][0], w.x[G][1]);
+  w.l[G] += w.x[G][N & 1];
+  w.x[G][N & 1] = __builtin_amdgcn_exp2f(y);
 }
-constexpr int PA_EARLY = 12;  // of the 32, those that the value products take; the next scores' products the others
-// I: 0 .. 2 PA_EARLY - 1, the early ones
-template <bool ROPE, int I> AMLA_DEV void pa_soft_early(PackedWave<ROPE> &w, u32x4 (&pn)[2][2], float c) {
+// I: 0 .. 2 PA_EARLY - 1
+template <bool ROPE, int I> AMLA_DEV void pa_soft_early(PackedWave<ROPE> &w, u32x4 (&pn)[2][4], float c) {
   constexpr int g = I & 1, n = I >> 1;
-  float l = w.l[g], e = w.e[g];
-  uint32_t p = 0;
-  pa_exp<n>(w.s[g][0][n], c, w.m[g], l, e, p);
-  w.l[g] = l;
-  w.e[g] = e;
-  if constexpr (n & 1) pn[g][n >> 3][(n >> 1) & 3] = p;
+  pa_turn<ROPE, g, n>(w, pn[g], w.s[g][0][n], c);
 }
-// I: 0 .. 2 (32 - PA_EARLY) - 1, the late ones
+// I: 0 .. 2 (32 - PA_EARLY) - 1
 template <bool ROPE, int I> AMLA_DEV void pa_soft_late(PackedWave<ROPE> &w, float c) {
   constexpr int g = I & 1, n = PA_EARLY + (I >> 1);
-  if constexpr (n < 32) {
-    float l = w.l[g], e = w.e[g], z;
-    uint32_t p = 0;
-    if constexpr (n < 16) z = w.u[g][n - PA_EARLY];
-    else z = w.t[g][n - 16];
-    pa_exp<n>(z, c, w.m[g], l, e, p);
-    w.l[g] = l;
-    w.e[g] = e;
-    if constexpr (n & 1) w.p[g][n >> 3][(n >> 1) & 3] = p;
-  }
+  if constexpr (n < 16) pa_turn<ROPE, g, n>(w, w.p[g], w.u[g][n - PA_EARLY], c);
+  else if constexpr (n < 32) pa_turn<ROPE, g, n>(w, w.p[g], w.t[g][n - 16], c);
+}
+template <bool ROPE> AMLA_DEV void pa_soft_end(PackedWave<ROPE> &w) {
+  w.p[0][3].w = pack_bf16(w.x[0][0], w.x[0][1]);
+  w.p[1][3].w = pack_bf16(w.x[1][0], w.x[1][1]);
 }
 
-constexpr int PA_KEY_AHEAD = 3, PA_VAL_AHEAD = 2;  // steps that LDS reads go out ahead
+constexpr int PA_AHEAD = 3;  // steps that LDS reads go out ahead, across the phases too: 300 to 400 cycles
 
 template <bool ROPE, int I> AMLA_DEV void pa_key_read(u32x4 (&ka)[2], uint32_t kr) {
   const uint32_t a = kr ^ (32 * (I & 3));
   ka[0] = pa_read16<(I >> 2) * PA_HALF>(a);
   ka[1] = pa_read16<(I >> 2) * PA_HALF + 32 * 128>(a);
+}
+template <int C> AMLA_DEV void pa_val_read(u32x2 (&v)[4], uint32_t v0) {
+  if constexpr (C < 8) {
+    const uint32_t a = v0 ^ (64 * ((C >> 1) & 1));
+    constexpr int ofs = (C >> 2) * PA_HALF + (C & 1) * 4096;
+    v[0] = pa_read_tr<ofs>(a);
+    v[1] = pa_read_tr<ofs + 1024>(a);
+    v[2] = pa_read_tr<ofs + 2048>(a);
+    v[3] = pa_read_tr<ofs + 3072>(a);
+  }
 }
 // What goes behind product K of score step I: a copy of the tile to come (one a step) or late probabilities
 template <bool ROPE, int I, int K> AMLA_DEV void pa_score_slot(PackedWave<ROPE> &w, float c, const PackedFeed &f, uint8_t *st) {
@@ -233,12 +232,13 @@ template <bool ROPE, int I, int K> AMLA_DEV void pa_score_slot(PackedWave<ROPE> 
   __builtin_amdgcn_sched_barrier(0);
 }
 template <bool ROPE, int I>
-AMLA_DEV void pa_score_step(PackedWave<ROPE> &w, u32x4 (&ka)[PA_KEY_AHEAD + 1][2], uint32_t kr, float c, const PackedFeed &f,
-                            uint8_t *st) {
-  constexpr int KS = PackedWave<ROPE>::KS, A = PA_KEY_AHEAD;
+AMLA_DEV void pa_score_step(PackedWave<ROPE> &w, u32x4 (&ka)[PA_AHEAD + 1][2], u32x2 (&vv)[PA_AHEAD + 1][4], uint32_t kr,
+                            uint32_t v0, float c, const PackedFeed &f, uint8_t *st) {
+  constexpr int KS = PackedWave<ROPE>::KS, A = PA_AHEAD;
   if constexpr (I < KS) {
     if constexpr (I + A < KS) pa_key_read<ROPE, I + A>(ka[(I + A) % (A + 1)], kr);
-    pa_wait<2 * (KS - 1 - I < A ? KS - 1 - I : A)>();
+    else pa_val_read<I + A - KS>(vv[I + A - KS], v0);
+    if constexpr (I >= A) pa_wait<I + A < KS ? 2 * A : 2 * (KS - 1 - I) + 4 * (I + A + 1 - KS)>();  // (the first A are there)
     u32x4 x = ka[I % (A + 1)][0], y = ka[I % (A + 1)][1];
     pa_tie(x);
     pa_tie(y);
@@ -250,33 +250,38 @@ AMLA_DEV void pa_score_step(PackedWave<ROPE> &w, u32x4 (&ka)[PA_KEY_AHEAD + 1][2
     pa_score_slot<ROPE, I, 2>(w, c, f, st);
     pa_score<I == 0, false>(w.s[1][1], as_bf16x8(y), w.q[1][I]);
     pa_score_slot<ROPE, I, 3>(w, c, f, st);
-    pa_score_step<ROPE, I + 1>(w, ka, kr, c, f, st);
+    pa_score_step<ROPE, I + 1>(w, ka, vv, kr, v0, c, f, st);
   }
 }
-template <bool ROPE>
-AMLA_DEV void pa_score_phase(PackedWave<ROPE> &w, uint32_t base, float c, const PackedFeed &f, uint8_t *st) {
+template <bool ROPE> AMLA_DEV uint32_t pa_key_addr(uint32_t stage) {
   const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
-  const uint32_t kr = base + j32 * 128 + 16 * (hh ^ ((j32 >> 1) & 7));
-  u32x4 ka[PA_KEY_AHEAD + 1][2];
+  return stage + j32 * 128 + 16 * (hh ^ ((j32 >> 1) & 7));
+}
+template <bool ROPE> AMLA_DEV uint32_t pa_val_addr(uint32_t stage) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+  return stage + PackedWave<ROPE>::VAL + (4 * hh + (L16 >> 2)) * 128 + 64 * hh + 32 * (g16 & 1) + 8 * (L16 & 3);
+}
+// The next tile landed in every wave, and no wave reads the stage two tiles back any more
+AMLA_DEV void pa_arrive() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// The first reads of a tile's keys; complete when the loop turns (a register whose read is on its way must not be moved)
+template <bool ROPE> AMLA_DEV void pa_first_keys(u32x4 (&ka)[PA_AHEAD + 1][2], uint32_t kr) {
   pa_key_read<ROPE, 0>(ka[0], kr);
   pa_key_read<ROPE, 1>(ka[1], kr);
   pa_key_read<ROPE, 2>(ka[2], kr);
-  pa_score_step<ROPE, 0>(w, ka, kr, c, f, st);
-  pa_settle();
-#pragma unroll
-  for (int g = 0; g < 2; ++g) asm volatile("" : "+v"(w.s[g][0]), "+v"(w.s[g][1]));
+}
+AMLA_DEV void pa_have_keys(u32x4 (&ka)[PA_AHEAD + 1][2]) {
+  u32x4 a = ka[0][0], b = ka[0][1], d = ka[1][0], e = ka[1][1], g = ka[2][0], h = ka[2][1];
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a), "+v"(b), "+v"(d), "+v"(e), "+v"(g), "+v"(h)::"memory");
+  ka[0][0] = a;
+  ka[0][1] = b;
+  ka[1][0] = d;
+  ka[1][1] = e;
+  ka[2][0] = g;
+  ka[2][1] = h;
 }
 
-template <int C> AMLA_DEV void pa_val_read(u32x2 (&v)[4], uint32_t v0) {
-  if constexpr (C < 8) {
-    const uint32_t a = v0 ^ (64 * ((C >> 1) & 1));
-    constexpr int ofs = (C >> 2) * PA_HALF + (C & 1) * 4096;
-    v[0] = pa_read_tr<ofs>(a);
-    v[1] = pa_read_tr<ofs + 1024>(a);
-    v[2] = pa_read_tr<ofs + 2048>(a);
-    v[3] = pa_read_tr<ofs + 3072>(a);
-  }
-}
 // MASK: keys lo .. lim - 1 of the tile are seen by the lane's query of group G
 template <bool ROPE, bool MASK, int G, int KEYS, int HALF> AMLA_DEV void pa_max(PackedWave<ROPE> &w, int lo, int lim) {
   f32x16 &z = w.s[G][KEYS];
@@ -301,7 +306,7 @@ AMLA_DEV void pa_refer(float &top, float &m, float c) {
 // What goes behind value product N: a part of the mask and the maximum of the scores (0 .. 7), the reference, then an early
 // probability each
 template <bool ROPE, bool MASK, bool SOFT, int N>
-AMLA_DEV void pa_value_slot(PackedWave<ROPE> &w, u32x4 (&pn)[2][2], float c, int lo, int lim0, int lim1) {
+AMLA_DEV void pa_value_slot(PackedWave<ROPE> &w, u32x4 (&pn)[2][4], float c, int lo, int lim0, int lim1) {
   if constexpr (SOFT) {
     if constexpr (N < 8) {
       pa_max<ROPE, MASK, (N & 1), ((N >> 2) & 1), ((N >> 1) & 1)>(w, lo, N & 1 ? lim1 : lim0);
@@ -315,19 +320,22 @@ AMLA_DEV void pa_value_slot(PackedWave<ROPE> &w, u32x4 (&pn)[2][2], float c, int
   }
   __builtin_amdgcn_sched_barrier(0);
 }
-// Step C of the outputs: 32 columns C / 2, keys 32 (C % 2) .. + 31
+// Step C of the outputs: 32 columns C / 2, keys 32 (C % 2) .. + 31.  SOFT: the tile to come is met before step 6, and
+// its first keys are read.
 template <bool ROPE, bool MASK, bool SOFT, int C>
-AMLA_DEV void pa_value_step(PackedWave<ROPE> &w, u32x2 (&vv)[PA_VAL_AHEAD + 1][4], u32x4 (&pn)[2][2], uint32_t v0, float c, int lo,
-                            int lim0, int lim1) {
+AMLA_DEV void pa_value_step(PackedWave<ROPE> &w, u32x4 (&ka)[PA_AHEAD + 1][2], u32x2 (&vv)[PA_AHEAD + 1][4], u32x4 (&pn)[2][4],
+                            uint32_t v0, uint32_t next, float c, int lo, int lim0, int lim1) {
   if constexpr (C < 8) {
-    constexpr int A = PA_VAL_AHEAD, cb = C >> 1, kk = 2 * (C & 1);
+    constexpr int A = PA_AHEAD, cb = C >> 1, kk = 2 * (C & 1);
     pa_val_read<C + A>(vv[(C + A) % (A + 1)], v0);
-    pa_wait<4 * (7 - C < A ? 7 - C : A)>();
+    if constexpr (SOFT && C == 6) pa_arrive();
+    else if constexpr (!SOFT || C < 6) pa_wait<4 * (7 - C < A ? 7 - C : A)>();
     u32x2 a = vv[C % (A + 1)][0], b = vv[C % (A + 1)][1], d = vv[C % (A + 1)][2], e = vv[C % (A + 1)][3];
     pa_tie(a);
     pa_tie(b);
     pa_tie(d);
     pa_tie(e);
+    if constexpr (SOFT && C == 6) pa_first_keys<ROPE>(ka, pa_key_addr<ROPE>(next));
     const bf16x8 x = as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), y = as_bf16x8(u32x4{d.x, d.y, e.x, e.y});
     pa_value<true>(w.o[0][cb], x, as_bf16x8(w.p[0][kk]));
     pa_value_slot<ROPE, MASK, SOFT, 4 * C>(w, pn, c, lo, lim0, lim1);
@@ -337,50 +345,54 @@ AMLA_DEV void pa_value_step(PackedWave<ROPE> &w, u32x2 (&vv)[PA_VAL_AHEAD + 1][4
     pa_value_slot<ROPE, MASK, SOFT, 4 * C + 2>(w, pn, c, lo, lim0, lim1);
     pa_value<false>(w.o[1][cb], y, as_bf16x8(w.p[1][kk + 1]));
     pa_value_slot<ROPE, MASK, SOFT, 4 * C + 3>(w, pn, c, lo, lim0, lim1);
-    pa_value_step<ROPE, MASK, SOFT, C + 1>(w, vv, pn, v0, c, lo, lim0, lim1);
+    pa_value_step<ROPE, MASK, SOFT, C + 1>(w, ka, vv, pn, v0, next, c, lo, lim0, lim1);
   }
 }
-// O^T += V^T P^T of the tile before (its stage at pv) while the scores of this tile are masked and half of them become
-// probabilities (SOFT)
-template <bool ROPE, bool MASK, bool SOFT>
-AMLA_DEV void pa_value_phase(PackedWave<ROPE> &w, uint32_t pv, float c, int lo, int lim0, int lim1) {
-  const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
-  const uint32_t v0 = pv + PackedWave<ROPE>::VAL + (4 * hh + (L16 >> 2)) * 128 + 64 * hh + 32 * (g16 & 1) + 8 * (L16 & 3);
-  u32x2 vv[PA_VAL_AHEAD + 1][4];
-  u32x4 pn[2][2];
-  pa_val_read<0>(vv[0], v0);
-  pa_val_read<1>(vv[1], v0);
-  pa_value_step<ROPE, MASK, SOFT, 0>(w, vv, pn, v0, c, lo, lim0, lim1);
-  if constexpr (SOFT) {
+// A tile (its keys at now): scores, while what is left of the tile before becomes probabilities and the tile to come (next)
+// is copied; then O^T += V^T P^T of the tile before while the scores are masked and the first of them become probabilities
+template <bool ROPE, bool MASK>
+AMLA_DEV void pa_tile(PackedWave<ROPE> &w, u32x4 (&ka)[PA_AHEAD + 1][2], uint32_t now, uint32_t before, uint32_t next, uint8_t *st,
+                      float c, const PackedFeed &f, int lo, int lim0, int lim1) {
+  const uint32_t v0 = pa_val_addr<ROPE>(before);
+  u32x2 vv[PA_AHEAD + 1][4];
+  u32x4 pn[2][4];
+  pa_score_step<ROPE, 0>(w, ka, vv, pa_key_addr<ROPE>(now), v0, c, f, st);
+  pa_soft_end<ROPE>(w);
+  pa_settle();
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      w.p[g][0] = pn[g][0];
-      w.p[g][1].x = pn[g][1].x;
-      w.p[g][1].y = pn[g][1].y;
-      w.u[g] = __builtin_shufflevector(w.s[g][0], w.s[g][0], 12, 13, 14, 15);
-      w.t[g] = w.s[g][1];
-    }
+  for (int g = 0; g < 2; ++g) asm volatile("" : "+v"(w.s[g][0]), "+v"(w.s[g][1]));
+  pa_value_step<ROPE, MASK, true, 0>(w, ka, vv, pn, v0, next, c, lo, lim0, lim1);
+  pa_have_keys(ka);
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    w.p[g][0] = pn[g][0];
+    w.p[g][1].x = pn[g][1].x;
+    w.u[g] = __builtin_shufflevector(w.s[g][0], w.s[g][0], 12, 13, 14, 15);
+    w.t[g] = w.s[g][1];
   }
 }
 // What is left of the last tile's probabilities, and its part of the outputs
-template <bool ROPE, int I = 0> AMLA_DEV void pa_last(PackedWave<ROPE> &w, uint32_t pv, float c) {
+template <bool ROPE, int I = 0> AMLA_DEV void pa_last(PackedWave<ROPE> &w, uint32_t before, float c) {
   if constexpr (I < 2 * (32 - PA_EARLY)) {
     pa_soft_late<ROPE, I>(w, c);
-    pa_last<ROPE, I + 1>(w, pv, c);
+    pa_last<ROPE, I + 1>(w, before, c);
   } else {
-    pa_value_phase<ROPE, false, false>(w, pv, c, 0, 0, 0);
+    pa_soft_end<ROPE>(w);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) w.l[g] += w.x[g][0] + w.x[g][1];
+    const uint32_t v0 = pa_val_addr<ROPE>(before);
+    u32x4 ka[PA_AHEAD + 1][2], pn[2][4];
+    u32x2 vv[PA_AHEAD + 1][4];
+    pa_val_read<0>(vv[0], v0);
+    pa_val_read<1>(vv[1], v0);
+    pa_val_read<2>(vv[2], v0);
+    pa_value_step<ROPE, false, false, 0>(w, ka, vv, pn, v0, 0, c, 0, 0, 0);
   }
 }
 
 // The LDS stages in turn: the tile in work, the one before it, the one on its way
 template <bool ROPE> struct PackedStages {
   uint32_t first, now, before;
-  AMLA_DEV void arrive() const {  // this tile landed in every wave, and no wave reads the stage two tiles back any more
-    wait_vmcnt<0>();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  }
   AMLA_DEV uint32_t next() const {
     const uint32_t n = now + PackedWave<ROPE>::STAGE;
     return n == first + PA_NST * PackedWave<ROPE>::STAGE ? first : n;
@@ -459,7 +471,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
       w.u[g] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int k = 0; k < 4; ++k) w.p[g][k] = u32x4{0, 0, 0, 0};
-      w.l[g] = 0.f;
+      w.l[g] = w.x[g][0] = w.x[g][1] = 0.f;
       w.top[g] = -INFINITY;
     }
     pa_settle();
@@ -467,27 +479,28 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     PackedStages<ROPE> at{lds0, lds0, lds0 + (PA_NST - 1) * W::STAGE};
     for (int o = threadIdx.x * 16; o < 2 * PA_HALF; o += 4096)
       *reinterpret_cast<u32x4 *>(sm + (PA_NST - 1) * W::STAGE + W::VAL + o) = u32x4{0, 0, 0, 0};
+    u32x4 ka[PA_AHEAD + 1][2];
+    pa_arrive();
+    pa_first_keys<ROPE>(ka, pa_key_addr<ROPE>(lds0));
+    pa_have_keys(ka);
     int j = 0;
     for (; j < n_all; ++j) {
-      at.arrive();
       f.aim(j + 1);
-      pa_score_phase<ROPE>(w, at.now, c, f, sm + (at.next() - lds0));
-      pa_value_phase<ROPE, false, true>(w, at.before, c, 0, 0, 0);
+      pa_tile<ROPE, false>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, 0, 0, 0);
       at.advance();
     }
     for (; j < n_any; ++j) {
-      at.arrive();
       f.aim(j + 1);
-      pa_score_phase<ROPE>(w, at.now, c, f, sm + (at.next() - lds0));
       const int first = f.first(j);
-      pa_value_phase<ROPE, true, true>(w, at.before, c, j * PA_KT - first - 4 * hh, lim[0] - first, lim[1] - first);
+      pa_tile<ROPE, true>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, j * PA_KT - first - 4 * hh,
+                          lim[0] - first, lim[1] - first);
       at.advance();
     }
     pa_last<ROPE>(w, at.before, c);
     for (; j < ntiles; ++j) {  // the wave's queries see no more: it goes on copying for the others
-      at.arrive();
       f.aim(j + 1);
       f.copy_all<ROPE>(sm + (at.next() - lds0));
+      pa_arrive();
       at.advance();
     }
     pa_settle();
