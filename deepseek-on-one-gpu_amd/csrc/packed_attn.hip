@@ -30,15 +30,21 @@ struct PackedParams {
 // Offsets are not checked on the host: clamped to the rows there are, and none below its predecessor's.
 AMLA_DEV int span_start(const int32_t *off, int b, int rows) { return min(max(off[b], 0), rows); }
 
-// Query block `tile` of the batch: (sequence, block of it), wave-uniform; the sequence is -1 past the end.
-AMLA_DEV int2 find_block(const PackedParams &p, int tile) {
+// A query block: its number within the sequence (-1: past the end), the sequence's first query and key and their counts.
+struct PackedBlock {
+  int block, q0, nq, k0, nk;
+};
+// Query block `tile` of the batch, wave-uniform.  Lane l looks at sequence b0 + l, queries and keys at once: one trip to
+// memory for up to 64 sequences.
+AMLA_DEV PackedBlock find_block(const PackedParams &p, int tile) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-    const int b = b0 + lane;
-    int n = 0;
-    if (b < p.seqs) n = max(span_start(p.offsets, b + 1, p.q_rows) - span_start(p.offsets, b, p.q_rows), 0);
-    const int blocks = (n + PA_QB - 1) / PA_QB;
+    const int b = min(b0 + lane, p.seqs - 1);
+    const int q0 = span_start(p.offsets, b, p.q_rows), k0 = span_start(p.k_offsets, b, p.k_rows);
+    const int nq = max(span_start(p.offsets, b + 1, p.q_rows) - q0, 0);
+    const int nk = max(span_start(p.k_offsets, b + 1, p.k_rows) - k0, 0);
+    const int blocks = b0 + lane < p.seqs ? (nq + PA_QB - 1) / PA_QB : 0;
     int incl = blocks;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -48,13 +54,14 @@ AMLA_DEV int2 find_block(const PackedParams &p, int tile) {
     const uint64_t past = __ballot(base + incl > tile);
     if (past) {
       const int l = __builtin_ctzll(past);
-      const int before = base + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(blocks, l);
+      const int n = __builtin_amdgcn_readlane(blocks, l), before = base + __builtin_amdgcn_readlane(incl, l) - n;
       // a sequence's last blocks see the most keys: they go first
-      return int2{b0 + l, __builtin_amdgcn_readlane(blocks, l) - 1 - (tile - before)};
+      return PackedBlock{n - 1 - (tile - before), __builtin_amdgcn_readlane(q0, l), __builtin_amdgcn_readlane(nq, l),
+                         __builtin_amdgcn_readlane(k0, l), __builtin_amdgcn_readlane(nk, l)};
     }
     base += __builtin_amdgcn_readlane(incl, 63);
   }
-  return int2{-1, 0};
+  return PackedBlock{-1, 0, 0, 0, 0};
 }
 
 // ---------------------------------------------------------------- one wave's part of a tile
@@ -414,12 +421,11 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
   // workgroup i runs on XCD i % 8: a head's blocks, and heads that share keys, come from the same L2 where heads divide
   const int i = blockIdx.x % p.heads;
   const int h = p.heads % 8 ? i : (i & 7) * (p.heads >> 3) + (i >> 3);
-  const int2 blk = find_block(p, blockIdx.x / p.heads);
-  if (blk.x < 0) return;
-  const int q0 = span_start(p.offsets, blk.x, p.q_rows), nq = span_start(p.offsets, blk.x + 1, p.q_rows) - q0;
-  const int k0 = span_start(p.k_offsets, blk.x, p.k_rows);
-  const int nk = max(span_start(p.k_offsets, blk.x + 1, p.k_rows) - k0, 0);
-  const int s_begin = blk.y * PA_QB, s_wave = s_begin + 64 * wave;
+  const PackedBlock blk = find_block(p, blockIdx.x / p.heads);
+  if (blk.block < 0) return;
+  const int q0 = blk.q0, nq = blk.nq, nk = blk.nk;
+  const int64_t k0 = blk.k0;
+  const int s_begin = blk.block * PA_QB, s_wave = s_begin + 64 * wave;
   const int past = nk - nq;  // keys before the first query's own (causal)
   const int klim = p.causal ? min(nk, max(past + min(s_begin + PA_QB, nq), 0)) : nk;  // keys that the block needs
   const int ntiles = (klim + PA_KT - 1) / PA_KT;
