@@ -878,14 +878,15 @@ def _latent_parts(cache, what: str) -> tuple:
     latent, k_pe = cache[0], cache[1]
     scales = cache[2] if len(cache) == 3 else None
     _need(latent, "latent", BF16 if scales is None else FP8)
-    _need(k_pe, "k_pe", BF16, latent.device)
-    if latent.dim() != 3 or latent.shape[2] != LATENT or k_pe.shape != latent.shape[:2] + (LATENT_ROPE,) or not latent.numel():
-        raise ValueError(f"{what}: cache of {tuple(latent.shape)} and {tuple(k_pe.shape)}, expected (pages, page_size, "
+    dev, shape = latent.device, latent.shape
+    _need(k_pe, "k_pe", BF16, dev)
+    if len(shape) != 3 or shape[2] != LATENT or k_pe.shape != (shape[0], shape[1], LATENT_ROPE) or not latent.numel():
+        raise ValueError(f"{what}: cache of {tuple(shape)} and {tuple(k_pe.shape)}, expected (pages, page_size, "
                          f"{LATENT}) and (pages, page_size, {LATENT_ROPE})")
     if scales is not None:
-        _need(scales, "scales", torch.uint8, latent.device)
-        if scales.shape != latent.shape[:2]:
-            raise ValueError(f"{what}: scales {tuple(scales.shape)} of a cache of {tuple(latent.shape)}")
+        _need(scales, "scales", torch.uint8, dev)
+        if scales.shape != shape[:2]:
+            raise ValueError(f"{what}: scales {tuple(scales.shape)} of a cache of {tuple(shape)}")
     return latent, k_pe, scales
 
 

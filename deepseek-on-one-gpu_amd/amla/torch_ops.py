@@ -544,7 +544,7 @@ def _lc_out_gradient(*args) -> None:
 def call_latent(name: str, *args):
     """``call`` for operators with several differentiable inputs: their tensors all decide."""
     if _dynamo() or _thread_keys().raw_repr() & _WATCHED or has_torch_function(args) and _intercepted(*args) or \
-            forward_ad._current_level >= 0 or any(_needs_operator(t) for t in args if isinstance(t, Tensor)):
+            forward_ad._current_level >= 0 or _need_operator(args):
         if not _dynamo() and forward_ad._current_level >= 0 and \
                 any(isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
             raise RuntimeError("the latent cache's operators have no derivative in forward mode")
@@ -552,8 +552,14 @@ def call_latent(name: str, *args):
     return _on_device(_mx_impl[name], *args)
 
 
-def _needs_operator(t: Tensor) -> bool:
-    return t.requires_grad or type(t) is not Tensor and not isinstance(t, torch.nn.Parameter)
+def _need_operator(args) -> bool:
+    for t in args:  # (a loop: a generator costs a microsecond of a call's ten)
+        if type(t) is Tensor:
+            if t.requires_grad:
+                return True
+        elif isinstance(t, Tensor) and (t.requires_grad or not isinstance(t, torch.nn.Parameter)):
+            return True
+    return False
 
 
 def _lc_cache(latent, k_pe, scales, block_table) -> LatentCache:
@@ -563,8 +569,12 @@ def _lc_cache(latent, k_pe, scales, block_table) -> LatentCache:
 
 def _lc_rows(x: Tensor) -> Tensor:
     """x itself when its rows are 16-byte aligned with unit stride, else a copy of such."""
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not any(s % 8 for s in x.stride()[:-1]):
-        return x
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0:
+        for s in x.stride()[:-1]:
+            if s % 8:
+                break
+        else:
+            return x
     return x.clone(memory_format=torch.contiguous_format)
 
 

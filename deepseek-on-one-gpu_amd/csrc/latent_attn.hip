@@ -882,15 +882,22 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
 
 constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 
-// 32-row groups of a workgroup: as many as the rows of a sequence fill
-static int attn_groups(int64_t rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
+// 32-row groups of a workgroup: as many as the rows of a sequence fill, since they share each tile's way through LDS, but
+// fewer while the cached rows do not keep all CUs at work for long: then more, shorter workgroups win.  Measured with 128
+// heads, one new token and fp8 rows (1 / 2 / 4 groups): 1 x 257 rows 17.2 / 18.9 / 21.5 us, 64 x 200 35.6 / 46.7 / 51.7,
+// 1 x 16384 33.8 / 34.8 / 43.1, 4 x 8192 42.0 / 37.5 / 39.2, 8 x 8192 65.5 / 49.4 / 45.6, 8 x 32768 205 / 126 / 90.
+static int attn_groups(int64_t seqs, int64_t rows, int64_t max_rows) {
+  const int fill = rows > 64 ? 4 : rows > 32 ? 2 : 1;
+  const double pairs = (double)seqs * rows * max_rows / LA_UNITS;  // query rows x cached rows of a CU
+  return std::min(fill, pairs <= 32 * 256 ? 1 : pairs <= 32 * 512 ? 2 : 4);
+}
 struct AttnSizes {
   int hg;
   int64_t chunks, slots;
 };
 static AttnSizes attn_sizes(int64_t seqs, int64_t rows, int64_t max_rows) {
   AttnSizes s;
-  s.hg = attn_groups(rows);
+  s.hg = attn_groups(seqs, rows, max_rows);
   s.chunks = (rows + 32 * s.hg - 1) / (32 * s.hg);
   s.slots = std::max<int64_t>(LA_UNITS, s.chunks * seqs + LA_UNITS / 2);
   const int64_t tiles = std::max<int64_t>(1, (max_rows + 31) / 32);  // no split is shorter than a tile
