@@ -409,8 +409,7 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
   else x0 = as_bf16x8(ka[0][0]);
   score_step<F8, HG, 0>(w, ka, kl, kr, x0, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
   // the results are read by vector code that the compiler schedules: cover the asm's write-to-read wait states
-  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
-  asm volatile("" : "+v"(w.s[0]), "+v"(w.s[1]));
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(w.s[0]), "+v"(w.s[1])::"memory");
 }
 
 // The second phase of a tile goes in steps of one 32-column block of the values; each carries some of the
@@ -611,6 +610,8 @@ template <bool F8> struct Feed {
   int b, wave, held, last, cur;  // last: rows past it are copied from it (and have no part in anything)
   Rows<F8> next;     // the tile that goes out next
   int page;          // the table's entry for the lane's row of the tile after it
+  int tail = 0;      // the newest rows that some token does not see
+  int odd = INT32_MAX;  // the first of them with a value that is no number
   int byte[PD + 1];  // the row's exponent, -1 where it has no page; [0]: the tile in work, [PD]: the one going out
 
   AMLA_DEV int row_of(int tile) const { return min(tile * TILE + WR * wave + (int)(threadIdx.x & 63) % WR, last); }
@@ -638,7 +639,7 @@ template <bool F8> struct Feed {
       const int by = gone ? 127 : byte[0];
       *reinterpret_cast<float *>(st + G::EXP + 4 * r) = gone ? -INFINITY : (float)(by - 127);
       if constexpr (F8) {
-        *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = (uint32_t)(254 - by) << 23;
+        *reinterpret_cast<uint32_t *>(st + G::INV + 4 * r) = by == 255 ? 0x00200000u : (uint32_t)(254 - by) << 23;
         *reinterpret_cast<uint32_t *>(st + G::MUL + 4 * r) = by == 255 ? 0x7fc00000u : (uint32_t)by << 23;
       }
     }
@@ -663,7 +664,7 @@ template <bool F8> struct Feed {
     factors(t_first);
   }
   // The rows of tile `tile` have landed in every wave
-  AMLA_DEV void arrive(int tile) {
+  template <bool MASK> AMLA_DEV void arrive(int tile) {
     using G = Stage<F8>;
     constexpr int RB = Tile<F8>::RB, LOADS = F8 ? 2 : 1;
     const int lane = threadIdx.x & 63;
@@ -676,6 +677,23 @@ template <bool F8> struct Feed {
       const int r = WR * wave + __builtin_ctzll(bad);
       for (int i = lane; i < RB / 16; i += 64) *reinterpret_cast<u32x4 *>(st + r * RB + 16 * i) = u32x4{0, 0, 0, 0};
       if (lane < 8) *reinterpret_cast<u32x4 *>(st + G::PE + r * 128 + 16 * lane) = u32x4{0, 0, 0, 0};
+    }
+    if constexpr (MASK) {
+      // rows that some token does not see: one with an infinity or a NaN becomes zeros too, and the tokens that do see it
+      // get their NaN at the end
+      const int end = min(held - tile * TILE - WR * wave, WR);
+      for (int r = max(held - tail - tile * TILE - WR * wave, 0); r < end; ++r) {
+        u32x4 *at = reinterpret_cast<u32x4 *>(st + (WR * wave + r) * RB + 16 * (lane % (RB / 16)));
+        const u32x4 v = *at;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          bad |= F8 ? (((v[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0
+                    : (((v[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+        if (!__ballot(bad) && __builtin_amdgcn_readlane(byte[0], r) != 255) continue;
+        *at = u32x4{0, 0, 0, 0};
+        odd = min(odd, tile * TILE + WR * wave + r);
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -721,6 +739,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
 
   Feed<F8> feed{p.pg, sm, b, wave, rows_held, min(rows_held, t_end * TILE) - 1};
+  if constexpr (MASK) feed.tail = p.seq_len - 1;
   feed.start(t_first);
 
   // queries: B fragments, lane = row of the chunk, in the order of the score steps' reads
@@ -761,7 +780,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
     uint32_t base = lds0;
     for (int tile = t_first; tile < t_end; ++tile) {
       const uint32_t before = base;
-      feed.arrive(tile);
+      feed.template arrive<MASK>(tile);
       base = lds0 + feed.cur * G::SIZE;
       score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
       value_phase<F8, HG, MASK, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE);
@@ -774,9 +793,14 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
     // the waves agree: their copies and barriers are common
     __syncthreads();
     uint32_t *vote = reinterpret_cast<uint32_t *>(sm);
-    if (lane == 0) vote[wave] = __ballot(low) != 0;
+    const bool any_low = __ballot(low) != 0;
+    if (lane == 0) {
+      vote[wave] = any_low;
+      if constexpr (MASK) vote[4 + wave] = (uint32_t)feed.odd;
+    }
     __syncthreads();
     const bool again = (vote[0] | vote[1] | vote[2] | vote[3]) != 0;
+    if constexpr (MASK) feed.odd = (int)min(min(vote[4], vote[5]), min(vote[6], vote[7]));
     __syncthreads();
     if (!again) break;
     w.m = low ? ceilf(w.top) : w.m;
@@ -786,6 +810,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   // ---- the split's sums, normalised: the output itself, or a partial one
   float l = w.l;
   l += __shfl_xor(l, 32, 64);
+  if constexpr (MASK) l = feed.odd < limit + 4 * hh ? __uint_as_float(0x7fc00000u) : l;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse2 = l == 0.f ? -INFINITY : w.m + __builtin_amdgcn_logf(l);
   // rows of 1 KB / CG through LDS (chunk c of a wave's row at c ^ row), so that a store is whole lines

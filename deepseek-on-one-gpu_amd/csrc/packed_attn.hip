@@ -113,7 +113,12 @@ template <bool WAIT> AMLA_DEV void pa_value(f32x16 &c, bf16x8 a, bf16x8 b) {
   if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-AMLA_DEV void pa_settle() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
+// Before vector code reads what the products above wrote, and before they read what it wrote.
+AMLA_DEV void pa_settle(f32x16 (&o)[2][4]) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
+               : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[0][2]), "+a"(o[0][3]), "+a"(o[1][0]), "+a"(o[1][1]), "+a"(o[1][2]),
+                 "+a"(o[1][3])::"memory");
+}
 
 // Where a wave's copies come from: rows 16 w .. + 15 of a tile, as 8-row pieces of 128-byte half-rows.  Bases are
 // uniform, each lane adds a fixed offset; chunk c of row r of a key array sits at c ^ ((r >> 1) & 7), the 64-byte
@@ -170,6 +175,26 @@ struct PackedFeed {
       }
       if constexpr (ROPE) copy_lds(pe + row * ldpe + kc, dst + 2 * PA_HALF);
     }
+  }
+  // Values of the tile at st that are no numbers become 0 in LDS: a masked probability of 0 would make them NaN.  Each lane
+  // looks at what it copied; true if any lane found one.
+  template <bool ROPE> AMLA_DEV bool clean(uint8_t *st, int lane) const {
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 *at = reinterpret_cast<u32x4 *>(st + PackedWave<ROPE>::VAL + (i >> 1) * PA_HALF + (row0 + 8 * (i & 1)) * 128 + 16 * lane);
+      const u32x4 x = *at;
+      u32x4 y = x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if ((x[k] & 0x7f80u) == 0x7f80u) y[k] &= 0xffff0000u;
+        if ((x[k] & 0x7f800000u) == 0x7f800000u) y[k] &= 0xffffu;
+      }
+      const bool bad = y.x != x.x || y.y != x.y || y.z != x.z || y.w != x.w;
+      if (bad) *at = y;
+      found |= bad;
+    }
+    return __ballot(found) != 0;
   }
   template <bool ROPE, int I = 0> AMLA_DEV void copy_all(uint8_t *st) const {
     if constexpr (I < 2 * ((ROPE ? 3 : 2) + 2)) {
@@ -289,19 +314,39 @@ AMLA_DEV void pa_have_keys(u32x4 (&ka)[PA_AHEAD + 1][2]) {
   ka[2][1] = h;
 }
 
-// MASK: keys lo .. lim - 1 of the tile are seen by the lane's query of group G
-template <bool ROPE, bool MASK, int G, int KEYS, int HALF> AMLA_DEV void pa_max(PackedWave<ROPE> &w, int lo, int lim) {
-  f32x16 &z = w.s[G][KEYS];
+// A copy that the compiler does not see through: a score that outlives its tile by another name would be moved right behind
+// the product that makes it, before it is there.
+AMLA_DEV float pa_copy(float x) {
+  float y;
+  asm("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+  return y;
+}
+// Eight scores of group G in value slot N = 0 .. 7: their mask (keys lo .. lim - 1 of the tile are seen by the lane's query)
+// and maximum; the second 32 keys go to t
+template <bool ROPE, bool MASK, int N> AMLA_DEV void pa_max(PackedWave<ROPE> &w, int lo, int lim) {
+  constexpr int G = N & 1, KEYS = N >> 2, HALF = (N >> 1) & 1;
 #pragma unroll
   for (int i = 8 * HALF; i < 8 * HALF + 8; i += 2) {
+    float z[2] = {w.s[G][KEYS][i], w.s[G][KEYS][i + 1]};
     if constexpr (MASK) {
 #pragma unroll
-      for (int k = i; k < i + 2; ++k) {
-        const int key = 32 * KEYS + 8 * (k >> 2) + (k & 3);
+      for (int k = 0; k < 2; ++k) {
+        const int key = 32 * KEYS + 8 * (i >> 2) + (i & 3) + k;
         z[k] = key < lim && key >= lo ? z[k] : -INFINITY;
       }
+      if constexpr (KEYS == 0) {
+        w.s[G][0][i] = z[0];
+        w.s[G][0][i + 1] = z[1];
+      } else {
+        w.t[G][i] = z[0];
+        w.t[G][i + 1] = z[1];
+      }
     }
-    w.top[G] = __builtin_fmaxf(__builtin_fmaxf(w.top[G], z[i]), z[i + 1]);
+    w.top[G] = __builtin_fmaxf(__builtin_fmaxf(w.top[G], z[0]), z[1]);
+  }
+  if constexpr (!MASK) {
+#pragma unroll
+    for (int i = 4 * (N >> 1); i < 4 * (N >> 1) + 4; ++i) w.t[G][i] = pa_copy(w.s[G][1][i]);
   }
 }
 // Both lanes of a query agree on its largest score so far; the first one sets its reference
@@ -316,7 +361,7 @@ template <bool ROPE, bool MASK, bool SOFT, int N>
 AMLA_DEV void pa_value_slot(PackedWave<ROPE> &w, u32x4 (&pn)[2][4], float c, int lo, int lim0, int lim1) {
   if constexpr (SOFT) {
     if constexpr (N < 8) {
-      pa_max<ROPE, MASK, (N & 1), ((N >> 2) & 1), ((N >> 1) & 1)>(w, lo, N & 1 ? lim1 : lim0);
+      pa_max<ROPE, MASK, N>(w, lo, N & 1 ? lim1 : lim0);
     } else {
       if constexpr (N == 8) {
         pa_refer(w.top[0], w.m[0], c);
@@ -365,17 +410,15 @@ AMLA_DEV void pa_tile(PackedWave<ROPE> &w, u32x4 (&ka)[PA_AHEAD + 1][2], uint32_
   u32x4 pn[2][4];
   pa_score_step<ROPE, 0>(w, ka, vv, pa_key_addr<ROPE>(now), v0, c, f, st);
   pa_soft_end<ROPE>(w);
-  pa_settle();
-#pragma unroll
-  for (int g = 0; g < 2; ++g) asm volatile("" : "+v"(w.s[g][0]), "+v"(w.s[g][1]));
+  // (one statement: a move of the scores between the wait and them would read them too early)
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(w.s[0][0]), "+v"(w.s[0][1]), "+v"(w.s[1][0]), "+v"(w.s[1][1])::"memory");
   pa_value_step<ROPE, MASK, true, 0>(w, ka, vv, pn, v0, next, c, lo, lim0, lim1);
   pa_have_keys(ka);
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     w.p[g][0] = pn[g][0];
     w.p[g][1].x = pn[g][1].x;
-    w.u[g] = __builtin_shufflevector(w.s[g][0], w.s[g][0], 12, 13, 14, 15);
-    w.t[g] = w.s[g][1];
+    w.u[g] = f32x4{pa_copy(w.s[g][0][12]), pa_copy(w.s[g][0][13]), pa_copy(w.s[g][0][14]), pa_copy(w.s[g][0][15])};
   }
 }
 // What is left of the last tile's probabilities, and its part of the outputs
@@ -433,8 +476,9 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
   const int seen_all = s_wave >= nq ? 0 : p.causal ? min(max(past + s_wave + 1, 0), nk) : nk;
   const int seen_any = s_wave >= nq ? 0 : p.causal ? min(max(past + min(s_wave + 64, nq), 0), nk) : nk;
   const int n_any = (seen_any + PA_KT - 1) / PA_KT;
-  // tiles wholly seen by all of the wave's queries; the last one may be loaded from further ahead
+  // tiles wholly seen by all of the wave's queries, and by all of the block's; the last one may be loaded from further ahead
   const int n_all = min(seen_all / PA_KT, klim / PA_KT);
+  const int n_block = min((p.causal ? min(max(past + s_begin + 1, 0), nk) : nk) / PA_KT, klim / PA_KT);
 
   const int kvh = h / p.group;
   PackedFeed f;
@@ -463,6 +507,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
   const float c = p.scale_log2;
 
+  bool odd = false;  // values that clean() took out
   for (;;) {  // once, or twice where m turned out too low
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -470,7 +515,6 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
       for (int cb = 0; cb < 4; ++cb) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) w.o[g][cb][r] = 0.f;
-        asm volatile("" : "+a"(w.o[g][cb]));
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) w.t[g][r] = -INFINITY;
@@ -480,7 +524,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
       w.l[g] = w.x[g][0] = w.x[g][1] = 0.f;
       w.top[g] = -INFINITY;
     }
-    pa_settle();
+    pa_settle(w.o);
     // nothing before the first tile: probabilities and values of 0
     PackedStages<ROPE> at{lds0, lds0, lds0 + (PA_NST - 1) * W::STAGE};
     for (int o = threadIdx.x * 16; o < 2 * PA_HALF; o += 4096)
@@ -490,13 +534,21 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     pa_first_keys<ROPE>(ka, pa_key_addr<ROPE>(lds0));
     pa_have_keys(ka);
     int j = 0;
+    for (; j < min(n_block, n_all); ++j) {
+      f.aim(j + 1);
+      pa_tile<ROPE, false>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, 0, 0, 0);
+      at.advance();
+    }
+    // from here on some query does not see all of a tile
     for (; j < n_all; ++j) {
       f.aim(j + 1);
+      odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
       pa_tile<ROPE, false>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, 0, 0, 0);
       at.advance();
     }
     for (; j < n_any; ++j) {
       f.aim(j + 1);
+      odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
       const int first = f.first(j);
       pa_tile<ROPE, true>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, j * PA_KT - first - 4 * hh,
                           lim[0] - first, lim[1] - first);
@@ -505,25 +557,24 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     pa_last<ROPE>(w, at.before, c);
     for (; j < ntiles; ++j) {  // the wave's queries see no more: it goes on copying for the others
       f.aim(j + 1);
+      if (j >= n_block) odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
       f.copy_all<ROPE>(sm + (at.next() - lds0));
       pa_arrive();
       at.advance();
     }
-    pa_settle();
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int cb = 0; cb < 4; ++cb) asm volatile("" : "+a"(w.o[g][cb]));
+    pa_settle(w.o);
     wait_vmcnt<0>();  // (copies past the last tile)
     const bool low0 = w.top[0] * c > w.m[0] + PA_LAG, low1 = w.top[1] * c > w.m[1] + PA_LAG;
     // the waves agree: their copies and barriers are common
     __syncthreads();
     uint32_t *vote = reinterpret_cast<uint32_t *>(sm);
-    if (lane == 0) vote[wave] = __ballot(low0 || low1) != 0;
+    const bool low = __ballot(low0 || low1) != 0;
+    if (lane == 0) vote[wave] = (low ? 1 : 0) | (odd ? 2 : 0);
     __syncthreads();
-    const bool again = (vote[0] | vote[1] | vote[2] | vote[3]) != 0;
+    const uint32_t votes = vote[0] | vote[1] | vote[2] | vote[3];
     __syncthreads();
-    if (!again) break;
+    odd = votes & 2;
+    if (!(votes & 1)) break;
     w.m[0] = low0 ? ceilf(w.top[0] * c) : w.m[0];
     w.m[1] = low1 ? ceilf(w.top[1] * c) : w.m[1];
     f.copy_first<ROPE>(sm, lane);
@@ -551,6 +602,18 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
                              pack_bf16(w.o[g][cb][4 * q4 + 2] * inv, w.o[g][cb][4 * q4 + 3] * inv)};
   }
   const int held = min(64, nq - s_wave);
+  if (__builtin_amdgcn_readfirstlane((int)odd)) {  // infinities and NaN enter the outputs of the queries that see them
+    for (int key = n_block * PA_KT; key < seen_any; ++key) {
+      const uint32_t x = reinterpret_cast<const uint32_t *>(f.v + key * f.ldv)[lane];
+      const bool lo = (x & 0x7f80u) == 0x7f80u, hi = (x & 0x7f800000u) == 0x7f800000u;
+      if (!__ballot(lo || hi)) continue;
+      for (int r = p.causal ? max(key - past - s_wave, 0) : 0; r < held; ++r) {
+        uint32_t *at = reinterpret_cast<uint32_t *>(turn + r * 256 + 16 * ((lane >> 2) ^ (r & 15)) + 4 * (lane & 3));
+        const float a = lo_bf(*at), b = hi_bf(*at);
+        *at = pack_bf16(lo ? a + lo_bf(x) : a, hi ? b + hi_bf(x) : b);
+      }
+    }
+  }
 #pragma unroll 4
   for (int r0 = 0; r0 < 64; r0 += 4) {
     const int r = r0 + (lane >> 4), ch = lane & 15;

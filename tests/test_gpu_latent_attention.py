@@ -125,6 +125,48 @@ def test_pages_outside_the_pool_hold_no_rows(fp8):
     _run(q, cache, table, lengths, what=f"fp8={fp8} bad lengths")
 
 
+def _wider(table, cols):
+    """The table with more columns, of no pages: more rows than there are count for the choice of a workgroup's size."""
+    return torch.cat([table, torch.full((table.shape[0], cols - table.shape[1]), -1, dtype=torch.int32)], 1)
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", [(1, 128, 200), (1, 128, 300), (3, 40, 200), (3, 40, 300), (2, 17, 1100)])
+def test_workgroups_of_more_query_rows(fp8, S, H, cols):
+    """Two and four groups of 32 query rows: taken where seqs rows max_rows passes 256 CUs times 8192 and 16384."""
+    lens = [700, 65]
+    q, cache, table, lengths = _case(S + H, lens, S, H, fp8, 64)
+    _run(q, cache, _wider(table, cols), lengths, what=f"fp8={fp8} S={S} H={H} {cols} columns")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", [(3, 5, 0), (2, 64, 0), (3, 128, 0), (3, 128, 100), (3, 128, 200), (70, 4, 0)])
+def test_what_a_token_does_not_see_does_not_reach_it(fp8, S, H, cols):
+    """An infinity or a NaN in one of the newest rows: the tokens before it keep their bits, the others get NaN."""
+    q, cache, table, lengths = _case(71, [200, 129], S, H, fp8, 16)
+    table = _wider(table, cols * 4) if cols else table
+    run = lambda c: ops.latent_attention(to_dev(q), c, to_dev(table), to_dev(lengths), SCALE, return_lse=True)  # noqa: E731
+    print(f"[case] fp8={fp8} S={S} H={H}", flush=True)
+    want, want_lse = run(to_dev(cache))
+    assert torch.isfinite(want).all()
+    for back, kind in ((1, "row"), (1, "one"), (S - 1, "one"), (1, "rope"), (S // 2, "row")):
+        dc = to_dev(tuple(t.clone() for t in cache))
+        for b, n in ((0, 200), (1, 129)):
+            page, at = table[b, (n - back) // 16], (n - back) % 16
+            if kind == "rope":
+                dc[1][page, at, 7] = float("nan")
+            elif fp8 and kind == "row":
+                dc[0].view(torch.uint8)[page, at], dc[2][page, at] = 0x7F, 255
+            elif fp8:
+                dc[0].view(torch.uint8)[page, at, 300] = 0xFF
+            else:
+                dc[0][page, at, 300 if kind == "one" else slice(None)] = float("inf") if kind == "one" else float("nan")
+        got, lse = run(dc)
+        sees = S - back  # the first token that sees the row
+        assert torch.equal(got[:, :sees], want[:, :sees]) and torch.equal(lse[:, :sees], want_lse[:, :sees]), (back, kind)
+        assert torch.isnan(got[:, sees:]).all(), (back, kind)
+
+
 def test_strides_and_no_lse():
     q, cache, table, lengths = _case(6, [100, 37], 2, 24, True, 16)
     want, _ = _run(q, cache, table, lengths, what="contiguous")

@@ -71,6 +71,35 @@ def test_scores_that_keep_rising():
     _run(q, k.flip(0), v, pe, off, koff, scale, causal=False, what="falling")
 
 
+@pytest.mark.parametrize("new,past,H,G,form", [([40], [0], 2, 1, "plain"), ([300, 70], [0, 90], 4, 4, "mla"), ([513], [100], 2, 2, "whole")])
+def test_what_a_query_does_not_see_does_not_reach_it(new, past, H, G, form):
+    """Infinities and NaN in a later key and in its values: the queries before it keep their bits, and the others the bits
+    of every column without one."""
+    lens = [a + b for a, b in zip(new, past)]
+    q, k, v, pe, off, koff, scale = _case(21, new, lens, H, G, form)
+    run = lambda k, v: ops.packed_attention(to_dev(q), to_dev(k), to_dev(v), to_dev(off), scale, k_offsets=to_dev(koff),  # noqa: E731
+                                            k_pe=to_dev(pe))
+    print(f"[case] {form} {new} {past}", flush=True)
+    want = run(k, v)
+    assert torch.isfinite(want).all()
+    for b in range(len(new)):
+        for first in sorted({1, new[b] // 3, new[b] - 1}):  # the first query that sees the key
+            key, row = int(koff[b]) + past[b] + first, int(off[b]) + first
+            sees = torch.zeros(sum(new), dtype=torch.bool, device=DEV)
+            sees[row:int(off[b + 1])] = True
+            v2, k2 = v.clone(), k.clone()
+            v2[key, :, 3], v2[key, :, 77], v2[key, :, 78] = float("inf"), float("nan"), float("-inf")
+            got = run(k, v2)
+            assert torch.equal(got[~sees], want[~sees]), (b, first)
+            rest = [c for c in range(128) if c not in (3, 77, 78)]
+            assert torch.equal(got[sees][..., rest], want[sees][..., rest]), (b, first)
+            assert (got[sees][..., 3] == float("inf")).all() and torch.isnan(got[sees][..., 77]).all(), (b, first)
+            assert (got[sees][..., 78] == float("-inf")).all(), (b, first)
+            k2[key] = float("nan")
+            got = run(k2, v)
+            assert torch.equal(got[~sees], want[~sees]) and torch.isnan(got[sees]).all(), (b, first)
+
+
 def test_strides_alignment_and_no_lse():
     q, k, v, pe, off, koff, scale = _case(9, [50, 20], [50, 20], 4, 4, "mla")
     want, _ = _run(q, k, v, pe, off, koff, scale, what="views of kv_b")
