@@ -507,8 +507,11 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
   const float c = p.scale_log2;
 
-  bool odd = false;  // values that clean() took out
-  for (;;) {  // once, or twice where m turned out too low
+  // Once; again where m turned out too low, or where an output is no number: then without the values that are none in
+  // tiles that some query does not see all of (they would come through a probability of 0), which enter at the end.  (Looking
+  // at each such tile first cost 5 in 100 of five prompts' time.)
+  bool careful = false, odd = false;  // odd: clean() took something out
+  for (;;) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
 #pragma unroll
@@ -534,21 +537,14 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     pa_first_keys<ROPE>(ka, pa_key_addr<ROPE>(lds0));
     pa_have_keys(ka);
     int j = 0;
-    for (; j < min(n_block, n_all); ++j) {
+    for (; j < (careful ? min(n_block, n_all) : n_all); ++j) {
       f.aim(j + 1);
-      pa_tile<ROPE, false>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, 0, 0, 0);
-      at.advance();
-    }
-    // from here on some query does not see all of a tile
-    for (; j < n_all; ++j) {
-      f.aim(j + 1);
-      odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
       pa_tile<ROPE, false>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, 0, 0, 0);
       at.advance();
     }
     for (; j < n_any; ++j) {
       f.aim(j + 1);
-      odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
+      if (careful) odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
       const int first = f.first(j);
       pa_tile<ROPE, true>(w, ka, at.now, at.before, at.next(), sm + (at.next() - lds0), c, f, j * PA_KT - first - 4 * hh,
                           lim[0] - first, lim[1] - first);
@@ -557,7 +553,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     pa_last<ROPE>(w, at.before, c);
     for (; j < ntiles; ++j) {  // the wave's queries see no more: it goes on copying for the others
       f.aim(j + 1);
-      if (j >= n_block) odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
+      if (careful && j >= n_block) odd |= f.clean<ROPE>(sm + (at.now - lds0), lane);
       f.copy_all<ROPE>(sm + (at.next() - lds0));
       pa_arrive();
       at.advance();
@@ -565,16 +561,25 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     pa_settle(w.o);
     wait_vmcnt<0>();  // (copies past the last tile)
     const bool low0 = w.top[0] * c > w.m[0] + PA_LAG, low1 = w.top[1] * c > w.m[1] + PA_LAG;
+    float none[2] = {0.f, 0.f};  // 0, or NaN where an output is infinite or NaN
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) none[g] = __builtin_fmaf(w.o[g][cb][r], 0.f, none[g]);
     // the waves agree: their copies and barriers are common
+    const bool low = __ballot(low0 || low1) != 0;
+    const bool strange = __ballot((w.l[0] != 0.f && none[0] != 0.f) || (w.l[1] != 0.f && none[1] != 0.f)) != 0;
     __syncthreads();
     uint32_t *vote = reinterpret_cast<uint32_t *>(sm);
-    const bool low = __ballot(low0 || low1) != 0;
-    if (lane == 0) vote[wave] = (low ? 1 : 0) | (odd ? 2 : 0);
+    if (lane == 0) vote[wave] = (low ? 1 : 0) | (odd ? 2 : 0) | (strange ? 4 : 0);
     __syncthreads();
     const uint32_t votes = vote[0] | vote[1] | vote[2] | vote[3];
     __syncthreads();
     odd = votes & 2;
-    if (!(votes & 1)) break;
+    if (!(votes & 1) && (careful || !(votes & 4))) break;
+    careful |= (votes & 4) != 0;
     w.m[0] = low0 ? ceilf(w.top[0] * c) : w.m[0];
     w.m[1] = low1 ? ceilf(w.top[1] * c) : w.m[1];
     f.copy_first<ROPE>(sm, lane);
