@@ -859,6 +859,9 @@ def latent_cache(pages: int, page_size: int, config, device, dtype: torch.dtype 
     value = code * 2^(byte - 127).  641 bytes a row instead of 1152.  page_size: a power of two."""
     if dtype not in (FP8, BF16):
         raise TypeError(f"latent_cache: dtype must be float8_e4m3fn or bfloat16 (got {dtype})")
+    if config.kv_lora_rank != LATENT or config.qk_rope_head_dim != LATENT_ROPE:
+        raise ValueError(f"latent_cache: rows are {LATENT} + {LATENT_ROPE} values (the configuration's: {config.kv_lora_rank} + "
+                         f"{config.qk_rope_head_dim})")
     if pages <= 0 or page_size <= 0 or page_size > 65536 or page_size & (page_size - 1):
         raise ValueError(f"latent_cache: {pages} pages of {page_size} rows (a power of two up to 65536)")
     latent = torch.zeros(pages, page_size, config.kv_lora_rank, dtype=torch.uint8 if dtype == FP8 else BF16, device=device)

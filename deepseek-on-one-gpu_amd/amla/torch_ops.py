@@ -563,8 +563,11 @@ def _need_operator(args) -> bool:
 
 
 def _lc_cache(latent, k_pe, scales, block_table) -> LatentCache:
-    return LatentCache(latent.data_ptr(), k_pe.data_ptr(), _ptr(scales), block_table.data_ptr(), block_table.stride(0),
-                       block_table.shape[1], latent.shape[0], latent.shape[1])
+    seqs, cols = block_table.shape
+    if not seqs:
+        cols = 0  # (an empty table has no address)
+    return LatentCache(latent.data_ptr(), k_pe.data_ptr(), _ptr(scales), block_table.data_ptr(), max(block_table.stride(0), cols),
+                       cols, latent.shape[0], latent.shape[1])
 
 
 def _lc_rows(x: Tensor) -> Tensor:

@@ -973,7 +973,7 @@ int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t
     return fail(AMLA_EUNSUPPORTED, "%s: q rows and out must be 16-byte aligned", what);
   const int64_t cap = cache->cols * cache->page_size;
   const AttnSizes s = attn_sizes(seqs, seq_len * heads, cap);
-  if (s.slots > (1 << 24) || seq_len * heads > (1 << 24))
+  if (s.slots >= (1 << 24) - 8 || seq_len * heads >= 1 << 24)  // grids of fewer than 2^32 threads
     return fail(AMLA_EUNSUPPORTED, "%s: too many query rows", what);
   if (workspace_bytes < amla_latent_attention_workspace_bytes(seqs, seq_len, heads, cap) || !workspace)
     return fail(AMLA_EWORKSPACE, "%s: workspace too small", what);

@@ -16,7 +16,7 @@
 namespace amla {
 
 int latent_pages(const amla_latent_cache *c, const char *what, LatentPages *p) {
-  if (!c || !c->latent || !c->k_pe || !c->block_table) return fail(AMLA_EINVAL, "%s: null pointer", what);
+  if (!c || !c->latent || !c->k_pe || (!c->block_table && c->cols)) return fail(AMLA_EINVAL, "%s: null pointer", what);
   if (c->page_size <= 0 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
     return fail(AMLA_EUNSUPPORTED, "%s: page_size %d is no power of two up to 65536", what, c->page_size);
   if (c->pages <= 0 || c->cols < 0 || c->ld_table < c->cols) return fail(AMLA_EINVAL, "%s: bad shape", what);
@@ -174,6 +174,7 @@ int amla_latent_cache_write(const amla_latent_cache *cache, const void *kv, int6
   if (rope_rows < 0) return fail(AMLA_EINVAL, "%s: bad shape", what);
   if (ldkv < LC_LORA + LC_ROPE || ldkv % 8 || !aligned16(kv) || !aligned16(gamma))
     return fail(AMLA_EUNSUPPORTED, "%s: rows of 576 values, rows and gamma 16-byte aligned", what);
+  if (rows >= 1 << 26) return fail(AMLA_EUNSUPPORTED, "%s: at most 2^26 - 1 rows a call", what);  // 2^32 threads
   const dim3 grid((unsigned)((rows + LC_WAVES - 1) / LC_WAVES));
   const auto fn = pg.scales ? latent_write_kernel<true> : latent_write_kernel<false>;
   fn<<<grid, 64 * LC_WAVES, 0, reinterpret_cast<hipStream_t>(stream)>>>(
@@ -192,6 +193,7 @@ int amla_latent_cache_read(const amla_latent_cache *cache, int64_t rows, const i
   if (rc || rows == 0) return rc;
   if (!latent || !k_pe) return fail(AMLA_EINVAL, "%s: null pointer", what);
   if (!aligned16(latent) || !aligned16(k_pe)) return fail(AMLA_EUNSUPPORTED, "%s: outputs must be 16-byte aligned", what);
+  if (rows >= 1 << 28) return fail(AMLA_EUNSUPPORTED, "%s: at most 2^28 - 1 rows a call", what);
   const dim3 grid((unsigned)((rows + LC_WAVES * LC_ROWS - 1) / (LC_WAVES * LC_ROWS)));
   const auto fn = pg.scales ? latent_read_kernel<true> : latent_read_kernel<false>;
   fn<<<grid, 64 * LC_WAVES, 0, reinterpret_cast<hipStream_t>(stream)>>>(pg, map, (int)rows, static_cast<u32x4 *>(latent),
