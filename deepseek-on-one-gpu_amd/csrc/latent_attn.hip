@@ -711,6 +711,60 @@ template <bool F8> struct Feed {
   }
 };
 
+// A split's sums, normalised: the output itself, or a partial one.  l, m: of the lane's query row.
+template <int HG, int NCB>
+AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB], float l, float m, int b, int chunk, int slot,
+                          int splits, int wave) {
+  constexpr int CG = 4 / HG;
+  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5, hg = wave / CG, cg = wave % CG;
+  const int row = (chunk * HG + hg) * 32 + j32;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float lse2 = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  // rows of 1 KB / CG through LDS (chunk c of a wave's row at c ^ row), so that a store is whole lines
+  constexpr int RBYTES = 1024 / CG;
+  uint8_t *turn = sm + wave * 32 * RBYTES;
+#pragma unroll
+  for (int c = 0; c < NCB; ++c)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *reinterpret_cast<u32x2 *>(turn + j32 * RBYTES + 16 * ((4 * c + q4) ^ (j32 % (4 * NCB))) + 8 * hh) =
+          u32x2{pack_bf16(o[c][4 * q4] * inv, o[c][4 * q4 + 1] * inv), pack_bf16(o[c][4 * q4 + 2] * inv, o[c][4 * q4 + 3] * inv)};
+  const int row0 = (chunk * HG + hg) * 32, held = min(32, p.rows - row0);
+  const size_t dst0 = splits == 1 ? (size_t)b * p.rows + row0 : (size_t)slot * (32 * HG) + 32 * hg;
+  uint16_t *to[2] = {p.part_o, p.out};
+  asm volatile("" : "+s"(to[0]), "+s"(to[1]));  // (a choice between the two arguments' places would be made in scratch memory)
+  uint8_t *od = reinterpret_cast<uint8_t *>((splits == 1 ? to[1] : to[0]) + dst0 * LC_LORA) + cg * RBYTES;
+  constexpr int LPR = RBYTES / 16;  // lanes of a row
+#pragma unroll 4
+  for (int r0 = 0; r0 < held; r0 += CG) {
+    const int r = r0 + lane / LPR, c = lane % LPR;
+    if (r < held)
+      *reinterpret_cast<u32x4 *>(od + (size_t)r * (LC_LORA * 2) + 16 * c) =
+          *reinterpret_cast<const u32x4 *>(turn + r * RBYTES + 16 * (c ^ (r % (4 * NCB))));
+  }
+  if (cg == 0 && hh == 0 && row < p.rows) {
+    if (splits > 1) p.part_lse[dst0 + j32] = lse2;
+    else if (p.lse) p.lse[dst0 + j32] = lse2 * 0.6931471805599453f;
+  }
+}
+
+// The work of a workgroup: its split of a sequence.
+struct SplitWork {
+  int b, chunk, slot, splits, held, t_first, t_end;  // b < 0: none
+};
+template <bool F8> AMLA_DEV SplitWork split_work(const LatentAttnParams &p) {
+  constexpr int TILE = Tile<F8>::ROWS;
+  const SplitPlan<TILE> plan(p);
+  // workgroup i runs on XCD i % 8: each takes a run of slots, so that a sequence's queries come from its L2
+  const int per_xcd = lc_ceil_div(plan.used(plan.len), 8), slot = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+  const int3 at = plan.find(slot);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || at.x < 0) return SplitWork{-1, 0, 0, 0, 0, 0, 0};
+  const int split = (slot - at.y) % at.z, held = __builtin_amdgcn_readfirstlane(min(max(p.lengths[at.x], 0), p.cap));
+  const int n_tiles = lc_ceil_div(held, TILE);
+  return SplitWork{at.x, (slot - at.y) / at.z, slot, at.z, held, (int)((int64_t)split * n_tiles / at.z),
+                   (int)((int64_t)(split + 1) * n_tiles / at.z)};
+}
+
 // One workgroup of four waves per (sequence, chunk of 32 HG rows, split).  HG waves hold 32
 // query rows each; the 4 / HG waves of the same rows compute the same scores and
 // accumulate 512 HG / 4 columns each.
@@ -725,17 +779,10 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   const int j32 = lane & 31, hh = lane >> 5;
   const int hg = wave / CG, cg = wave % CG;
 
-  const SplitPlan<TILE> plan(p);
-  // workgroup i runs on XCD i % 8: each takes a run of slots, so that a sequence's queries come from its L2
-  const int per_xcd = lc_ceil_div(plan.used(plan.len), 8), slot = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_xcd) return;
-  const int3 at = plan.find(slot);
-  if (at.x < 0) return;
-  const int b = at.x, splits = at.z;
-  const int chunk = (slot - at.y) / splits, split = (slot - at.y) % splits;
-  const int rows_held = __builtin_amdgcn_readfirstlane(min(max(p.lengths[b], 0), p.cap));
-  const int n_tiles = lc_ceil_div(rows_held, TILE);
-  const int t_first = (int)((int64_t)split * n_tiles / splits), t_end = (int)((int64_t)(split + 1) * n_tiles / splits);
+  const SplitWork at = split_work<F8>(p);
+  if (at.b < 0) return;
+  const int b = at.b, chunk = at.chunk, slot = at.slot, splits = at.splits, rows_held = at.held;
+  const int t_first = at.t_first, t_end = at.t_end;
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
 
   Feed<F8> feed{p.pg, sm, b, wave, rows_held, min(rows_held, t_end * TILE) - 1};
@@ -807,37 +854,355 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
     feed.start(t_first);
   }
 
-  // ---- the split's sums, normalised: the output itself, or a partial one
   float l = w.l;
   l += __shfl_xor(l, 32, 64);
   if constexpr (MASK) l = feed.odd < limit + 4 * hh ? __uint_as_float(0x7fc00000u) : l;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse2 = l == 0.f ? -INFINITY : w.m + __builtin_amdgcn_logf(l);
-  // rows of 1 KB / CG through LDS (chunk c of a wave's row at c ^ row), so that a store is whole lines
-  constexpr int RBYTES = 1024 / CG;
-  uint8_t *turn = sm + wave * 32 * RBYTES;
-#pragma unroll
-  for (int c = 0; c < NCB; ++c)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-      *reinterpret_cast<u32x2 *>(turn + j32 * RBYTES + 16 * ((4 * c + q4) ^ (j32 % (4 * NCB))) + 8 * hh) =
-          u32x2{pack_bf16(w.o[c][4 * q4] * inv, w.o[c][4 * q4 + 1] * inv),
-                pack_bf16(w.o[c][4 * q4 + 2] * inv, w.o[c][4 * q4 + 3] * inv)};
-  const int row0 = (chunk * HG + hg) * 32, held = min(32, p.rows - row0);
-  const size_t dst0 = splits == 1 ? (size_t)b * p.rows + row0 : (size_t)slot * (32 * HG) + 32 * hg;
-  uint8_t *od = reinterpret_cast<uint8_t *>((splits == 1 ? p.out : p.part_o) + dst0 * LC_LORA) + cg * RBYTES;
-  constexpr int LPR = RBYTES / 16;  // lanes of a row
-#pragma unroll 4
-  for (int r0 = 0; r0 < held; r0 += CG) {
-    const int r = r0 + lane / LPR, c = lane % LPR;
-    if (r < held)
-      *reinterpret_cast<u32x4 *>(od + (size_t)r * (LC_LORA * 2) + 16 * c) =
-          *reinterpret_cast<const u32x4 *>(turn + r * RBYTES + 16 * (c ^ (r % (4 * NCB))));
+  store_split<HG>(p, sm, w.o, l, w.m, b, chunk, slot, splits, wave);
+}
+
+// ---------------------------------------------------------------- few query rows
+//
+// One workgroup per (sequence, 32 query rows, split).  Wave (r, q) scores one half of a tile's rows for 16 of the queries
+// with 16x16x32 products and writes its probabilities to LDS; a tile later, behind the barrier that the tiles have anyway,
+// each wave takes all of them for its 128 columns.  So a tile's keys are read, and e4m3 converted, twice and not once a
+// wave, which is what bounds the kernel above with one group of queries (LDS: 1700 of its cycles a bf16 tile).
+template <bool F8> struct FewStage {
+  using G = Stage<F8>;
+  // probabilities as the value products take them, 16 bytes a lane: bf16: rows 16 k ..; e4m3: high halves, low halves, the
+  // scales of both blocks.  Two buffers: a tile's are read while the next one's are written.
+  static constexpr int LO = 2048, PS = 4096, PBUF = F8 ? 4352 : 2048, P = G::Q;
+  static constexpr int TOP = P + 2 * PBUF, M = TOP + 256, SUM = M + 128, ODD = SUM + 256, LIM = ODD + 16, LDS = LIM + 128;
+};
+static_assert(FewStage<true>::LDS <= 160 * 1024 && FewStage<false>::LDS <= 160 * 1024);
+
+template <bool F8> struct FewWave {
+  static constexpr int N = F8 ? 10 : 18, READS = F8 ? 2 : 1, AHEAD = F8 ? 4 : 8;  // score steps, reads of one, steps ahead
+  bf16x8 q[18];   // the wave's 16 queries, in the order of the score steps
+  f32x16 o[4];    // O^T: the wave's 128 columns x 32 queries
+  f32x4 s[2];     // S^T: e4m3: rows 16 u .. of the wave's 32; bf16: two chains of its 16
+  float m, l, top;
+};
+// What a wave reads of a tile besides the keys: factors of the rows of its scores (4 (lane / 16) .. and, e4m3, 16 on)
+template <bool F8> struct FewFactors {
+  u32x4 ex[2], inv[2];
+  float mul[2];
+};
+// What it needs for the values of the tile before: probabilities and the first columns
+template <bool F8> struct FewValues {
+  u32x4 p[4];
+  int ps;
+  u32x2 v[3][4];
+};
+
+template <bool F8, int I> AMLA_DEV void few_read(u32x4 (&d)[2], uint32_t kl, uint32_t kr) {
+  if constexpr (F8) {
+    if constexpr (I < 8) {  // codes 64 I + 16 (lane / 16) ..
+      d[0] = lds_read16<256 * (I >> 2)>(kl ^ (64 * (I & 3)));
+      d[1] = lds_read16<256 * (I >> 2) + 16 * 512>(kl ^ (64 * (I & 3)));
+    } else {
+      d[0] = lds_read16<0>(kr ^ (64 * (I - 8)));
+      d[1] = lds_read16<16 * 128>(kr ^ (64 * (I - 8)));
+    }
+  } else {  // values 32 I + 8 (lane / 16) ..
+    if constexpr (I < 16) d[0] = lds_read16<256 * (I >> 2)>(kl ^ (64 * (I & 3)));
+    else d[0] = lds_read16<0>(kr ^ (64 * (I - 16)));
   }
-  if (cg == 0 && hh == 0 && row < p.rows) {
-    if (splits > 1) p.part_lse[dst0 + j32] = lse2;
-    else if (p.lse) p.lse[dst0 + j32] = lse2 * 0.6931471805599453f;
+}
+template <bool F8, int I> AMLA_DEV void few_reads_first(u32x4 (*ka)[2], uint32_t kl, uint32_t kr) {
+  if constexpr (I < FewWave<F8>::AHEAD) {
+    few_read<F8, I>(ka[I], kl, kr);
+    few_reads_first<F8, I + 1>(ka, kl, kr);
   }
+}
+AMLA_DEV f32x4 mfma_few(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+template <bool F8, bool COPY, int I>
+AMLA_DEV void few_step(FewWave<F8> &w, u32x4 (&ka)[FewWave<F8>::AHEAD + 1][2], const float (&mul)[2], uint32_t kl, uint32_t kr,
+                       uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
+  using W = FewWave<F8>;
+  if constexpr (I < W::N) {
+    constexpr int A = W::AHEAD, c = I % (A + 1);
+    if constexpr (I + A < W::N) few_read<F8, I + A>(ka[(I + A) % (A + 1)], kl, kr);
+    lds_wait<W::READS * (W::N - 1 - I < A ? W::N - 1 - I : A)>();
+    u32x4 x = ka[c][0], y = x;
+    if constexpr (F8) {
+      y = ka[c][1];
+      lds_tie(x, y);
+    } else {
+      lds_tie(x);
+    }
+    if constexpr (!F8) {
+      w.s[I & 1] = mfma_few(as_bf16x8(x), w.q[I], w.s[I & 1]);
+    } else if constexpr (I < 8) {
+      w.s[0] = mfma_few(codes_to_bf16(x.x, x.y, mul[0]), w.q[2 * I], w.s[0]);
+      w.s[1] = mfma_few(codes_to_bf16(y.x, y.y, mul[1]), w.q[2 * I], w.s[1]);
+      w.s[0] = mfma_few(codes_to_bf16(x.z, x.w, mul[0]), w.q[2 * I + 1], w.s[0]);
+      w.s[1] = mfma_few(codes_to_bf16(y.z, y.w, mul[1]), w.q[2 * I + 1], w.s[1]);
+    } else {
+      w.s[0] = mfma_few(as_bf16x8(x), w.q[16 + I - 8], w.s[0]);
+      w.s[1] = mfma_few(as_bf16x8(y), w.q[16 + I - 8], w.s[1]);
+    }
+    if constexpr (COPY && I < Rows<F8>::COPIES) next.template copy<I>(pg, st_next, r0, lanes);
+    few_step<F8, COPY, I + 1>(w, ka, mul, kl, kr, lanes, next, pg, st_next, r0);
+  }
+}
+// Scores of the tile at LDS address base; COPY: with the copies of a later one between
+template <bool F8, bool COPY>
+AMLA_DEV void few_scores(FewWave<F8> &w, FewFactors<F8> &f, uint32_t base, int half, const Rows<F8> &next, const LatentPages &pg,
+                         uint8_t *st_next, int r0) {
+  using G = Stage<F8>;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, row = half * (G::ROWS / 2) + l16;
+  const uint32_t fr = base + 4 * (half * (G::ROWS / 2) + 4 * g), fm = base + 4 * row;
+  f.ex[0] = lds_read16<G::EXP>(fr);
+  if constexpr (F8) {
+    f.ex[1] = lds_read16<G::EXP + 64>(fr);
+    f.inv[0] = lds_read16<G::INV>(fr);
+    f.inv[1] = lds_read16<G::INV + 64>(fr);
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f.mul[0]) : "v"(fm), "i"(G::MUL) : "memory");
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f.mul[1]) : "v"(fm), "i"(G::MUL + 64) : "memory");
+  }
+  const uint32_t kl = base + row * Tile<F8>::RB + 16 * (g ^ Tile<F8>::swz(row));
+  const uint32_t kr = base + G::PE + row * 128 + 16 * (g ^ ((row >> 1) & 7));
+  u32x4 ka[FewWave<F8>::AHEAD + 1][2];
+  few_reads_first<F8, 0>(ka, kl, kr);
+  lds_wait<FewWave<F8>::READS * FewWave<F8>::AHEAD>();
+  lds_tie(f.ex[0]);
+  if constexpr (F8) lds_tie(f.ex[1], f.inv[0], f.inv[1], f.mul[0], f.mul[1]);
+  else f.mul[0] = f.mul[1] = 1.f;
+  w.s[0] = w.s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  few_step<F8, COPY, 0>(w, ka, f.mul, kl, kr, Rows<F8>::lanes(r0), next, pg, st_next, r0);
+}
+// z = s log2(e) scale + exponent of the row, in place; rows past lim are not seen
+template <bool F8, bool MASK> AMLA_DEV float few_scaled(FewWave<F8> &w, const FewFactors<F8> &f, float scale_log2, int lim) {
+  float top = -INFINITY;
+  if constexpr (!F8) w.s[0] += w.s[1];
+#pragma unroll
+  for (int u = 0; u < (F8 ? 2 : 1); ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float z = __builtin_fmaf(w.s[u][i], scale_log2, __uint_as_float(f.ex[u][i]));
+      if constexpr (MASK) z = 16 * u + i < lim ? z : -INFINITY;
+      w.s[u][i] = z;
+      top = __builtin_fmaxf(top, z);
+    }
+  return top;
+}
+// The largest of the four lanes of a query
+AMLA_DEV float few_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __builtin_fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+AMLA_DEV void few_write(uint32_t addr, uint32_t v) { asm volatile("ds_write_b32 %0, %1" ::"v"(addr), "v"(v) : "memory"); }
+// Probabilities of the wave's scores, to LDS: rows 4 (g / 2 + 2 u) .. of query lane / 16 belong to lane query + 32 (g % 2)
+// of the value products
+template <bool F8> AMLA_DEV void few_probabilities(FewWave<F8> &w, const FewFactors<F8> &f, float top, uint32_t pbuf, int half, int qh) {
+  const int lane = threadIdx.x & 63, query = 16 * qh + (lane & 15), g = lane >> 4;
+  const uint32_t to = pbuf + 1024 * half + 16 * (query + 32 * (g & 1));
+  w.top = __builtin_fmaxf(w.top, top);
+  if constexpr (F8) {
+    const float ref = floorf(__builtin_fmaxf(few_max(top), M_NONE)) - 7.f;  // of the 32 rows: a block of the matrix unit
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(w.s[u][i] - ref);
+        sum = __builtin_fmaf(e[i], __uint_as_float(f.inv[u][i]), sum);
+      }
+      int hi, lo;
+      split_fp8x4(e, 0.0625f, hi, lo);
+      few_write(to + 4 * (g >> 1) + 8 * u, hi);
+      few_write(to + FewStage<F8>::LO + 4 * (g >> 1) + 8 * u, lo);
+    }
+    w.l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(ref - w.m), w.l);
+    few_write(pbuf + FewStage<F8>::PS + 4 * (32 * half + query), (int)__builtin_fmaxf(ref - w.m, -123.f) + 127);
+  } else {
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(w.s[0][i] - w.m);
+    w.l += (e[0] + e[1]) + (e[2] + e[3]);
+    const u32x2 v = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
+    asm volatile("ds_write_b64 %0, %1" ::"v"(to + 8 * (g >> 1)), "v"(v) : "memory");
+  }
+}
+template <bool F8, int C> AMLA_DEV void few_value_read(FewValues<F8> &x, uint32_t v0, uint32_t v1) {
+  if constexpr (C < 4) {
+    u32x2(&v)[4] = x.v[C % 3];
+    const uint32_t a = v0 ^ (F8 ? 32 * C : 64 * C), b = v1 ^ (64 * C);
+    if constexpr (F8) {
+      v[0] = lds_read_tr<F8, 0>(a);
+      v[1] = lds_read_tr<F8, 8192>(a);
+      v[2] = lds_read_tr<F8, 16384>(a);
+      v[3] = lds_read_tr<F8, 24576>(a);
+    } else {
+      v[0] = lds_read_tr<F8, 0>(a);
+      v[1] = lds_read_tr<F8, 0>(b);
+      v[2] = lds_read_tr<F8, 16384>(a);
+      v[3] = lds_read_tr<F8, 16384>(b);
+    }
+  }
+}
+// Where the wave's columns 128 c .. of the values at pv begin: like value_phase of four column groups
+template <bool F8> AMLA_DEV uint2 few_value_addr(uint32_t pv, int cg) {
+  using T = Tile<F8>;
+  const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
+  if constexpr (F8) {
+    const int r = 8 * (L16 >> 3) + 4 * hh + ((L16 >> 1) & 3);
+    const uint32_t v = pv + r * T::RB + 16 * ((g16 & 1) ^ T::swz(r)) + 8 * (L16 & 1);
+    return uint2{(v ^ (32 * ((4 * cg) & 7))) + 256 * ((4 * cg) >> 3), 0};
+  } else {
+    const int r = 4 * hh + (L16 >> 2), ch = 2 * (g16 & 1) + ((L16 >> 1) & 1);
+    const uint32_t v = pv + 8 * (L16 & 1) + 256 * cg;
+    return uint2{v + r * T::RB + 16 * (ch ^ T::swz(r)), v + (r + 8) * T::RB + 16 * (ch ^ T::swz(r + 8))};
+  }
+}
+// The probabilities at pbuf and the first values
+template <bool F8> AMLA_DEV void few_values_first(FewValues<F8> &x, uint32_t pbuf, uint2 v) {
+  const int lane = threadIdx.x & 63;
+  x.p[0] = lds_read16<0>(pbuf + 16 * lane);
+  x.p[1] = lds_read16<1024>(pbuf + 16 * lane);
+  if constexpr (F8) {
+    x.p[2] = lds_read16<2048>(pbuf + 16 * lane);
+    x.p[3] = lds_read16<3072>(pbuf + 16 * lane);
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(x.ps) : "v"(pbuf + 4 * lane), "i"(FewStage<F8>::PS) : "memory");
+  }
+  few_value_read<F8, 0>(x, v.x, v.y);
+  few_value_read<F8, 1>(x, v.x, v.y);
+}
+template <bool F8, int C> AMLA_DEV void few_value_step(FewWave<F8> &w, FewValues<F8> &x, uint2 v) {
+  if constexpr (C < 4) {
+    few_value_read<F8, C + 2>(x, v.x, v.y);
+    lds_wait<4 * ((C + 1 < 4) + (C + 2 < 4))>();
+    if constexpr (C == 0) {
+      u32x4 a = x.p[0], b = x.p[1];
+      lds_tie(a, b);
+      x.p[0] = a;
+      x.p[1] = b;
+      if constexpr (F8) {
+        u32x4 d = x.p[2], e = x.p[3];
+        int ps = x.ps;
+        lds_tie(d, e, ps);
+        x.p[2] = d;
+        x.p[3] = e;
+        x.ps = ps;
+      }
+    }
+    u32x2 a = x.v[C % 3][0], b = x.v[C % 3][1], d = x.v[C % 3][2], e = x.v[C % 3][3];
+    lds_tie(a, b, d, e);
+    if constexpr (F8) {
+      const i32x8 hi = {(int)x.p[0].x, (int)x.p[0].y, (int)x.p[0].z, (int)x.p[0].w, (int)x.p[1].x, (int)x.p[1].y, (int)x.p[1].z, (int)x.p[1].w};
+      const i32x8 lo = {(int)x.p[2].x, (int)x.p[2].y, (int)x.p[2].z, (int)x.p[2].w, (int)x.p[3].x, (int)x.p[3].y, (int)x.p[3].z, (int)x.p[3].w};
+      mfma_value(w.o[C], join(a, b, d, e), 127, hi, x.ps);
+      mfma_value(w.o[C], join(a, b, d, e), 127, lo, x.ps - 4);
+    } else {
+      mfma_value(w.o[C], as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), as_bf16x8(x.p[0]));
+      mfma_value(w.o[C], as_bf16x8(u32x4{d.x, d.y, e.x, e.y}), as_bf16x8(x.p[1]));
+    }
+    few_value_step<F8, C + 1>(w, x, v);
+  }
+}
+
+template <bool F8, bool MASK>
+__global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParams p) {
+  extern __shared__ __align__(1024) uint8_t sm[];
+  using G = Stage<F8>;
+  using F = FewStage<F8>;
+  constexpr int TILE = Tile<F8>::ROWS;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = wave & 1, qh = wave >> 1, l16 = lane & 15, g = lane >> 4;
+  const SplitWork at = split_work<F8>(p);
+  if (at.b < 0) return;
+  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)sm);
+
+  Feed<F8> feed{p.pg, sm, at.b, wave, at.held, min(at.held, at.t_end * TILE) - 1};
+  if constexpr (MASK) feed.tail = p.seq_len - 1;
+  feed.start(at.t_first);
+
+  FewWave<F8> w;
+  const int query = 16 * qh + l16, rq = min(at.chunk * 32 + query, p.rows - 1), tok = rq / p.heads;
+  // rows of a tile below lim - TILE tile are seen: of the lane's first, row TILE / 2 half + 4 g
+  const int limit = at.held - (p.seq_len - 1 - tok), lim = limit - TILE / 2 * half - 4 * g;
+  const uint16_t *qp = p.q + at.b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w.q[i] = as_bf16x8(ldg16(qp + (F8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) w.q[16 + i] = as_bf16x8(ldg16(qp + LC_LORA + 32 * i + 8 * g));
+  w.m = M_NONE;
+  float *const x_top = reinterpret_cast<float *>(sm + F::TOP), *const x_m = reinterpret_cast<float *>(sm + F::M);
+  FewFactors<F8> f;
+  for (int pass = 0;; ++pass) {  // once, or twice where m turned out too low
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w.o[c][i] = 0.f;
+    settle(w.o);
+    w.l = 0.f;
+    w.top = -INFINITY;
+    // nothing before the first tile: probabilities of 0 times its own values
+    for (int o = threadIdx.x * 4; o < F::PBUF; o += 1024)
+      *reinterpret_cast<uint32_t *>(sm + F::P + F::PBUF + o) = o < F::PS ? 0u : 127u;
+    if (pass == 0) {  // the waves agree on m: the first tile's maxima, its scores made twice
+      feed.template arrive<MASK>(at.t_first);
+      few_scores<F8, false>(w, f, lds0, half, feed.next, p.pg, sm, 0);
+      const float top = few_max(few_scaled<F8, MASK>(w, f, p.scale_log2, lim - at.t_first * TILE));
+      x_top[32 * half + query] = top;
+      __syncthreads();
+      w.m = __builtin_fmaxf(ceilf(__builtin_fmaxf(x_top[query], x_top[32 + query])), M_NONE);
+    }
+    uint32_t base = lds0, pbuf = lds0 + F::P;
+    for (int tile = at.t_first; tile < at.t_end; ++tile) {
+      const uint32_t before = base, p_before = 2 * lds0 + 2 * F::P + F::PBUF - pbuf;
+      feed.template arrive<MASK>(tile);
+      base = lds0 + feed.cur * G::SIZE;
+      FewValues<F8> x;
+      const uint2 v = few_value_addr<F8>(before, wave);
+      few_values_first<F8>(x, p_before, v);
+      few_scores<F8, true>(w, f, base, half, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+      few_value_step<F8, 0>(w, x, v);
+      const float top = few_scaled<F8, MASK>(w, f, p.scale_log2, lim - tile * TILE);
+      few_probabilities<F8>(w, f, top, pbuf, half, qh);
+      pbuf = p_before;
+      feed.advance(tile);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    {
+      FewValues<F8> x;
+      const uint2 v = few_value_addr<F8>(base, wave);
+      few_values_first<F8>(x, 2 * lds0 + 2 * F::P + F::PBUF - pbuf, v);
+      few_value_step<F8, 0>(w, x, v);
+    }
+    settle(w.o);
+    wait_vmcnt<0>();  // (copies past the last tile)
+    const float top = few_max(w.top);
+    x_top[32 * half + query] = top;
+    x_m[query] = w.m;
+    if constexpr (MASK) reinterpret_cast<int *>(sm + F::ODD)[wave] = feed.odd;
+    __syncthreads();
+    const float high = __builtin_fmaxf(x_top[query], x_top[32 + query]);
+    const bool again = __ballot(__builtin_fmaxf(x_top[lane & 31], x_top[32 + (lane & 31)]) > x_m[lane & 31] + LAG) != 0;
+    __syncthreads();
+    if (!again) break;
+    w.m = high > w.m + LAG ? ceilf(high) : w.m;
+    feed.start(at.t_first);
+  }
+  // sums over the four lanes and both halves of a query, handed to the lanes that hold its outputs
+  float *const x_sum = reinterpret_cast<float *>(sm + F::SUM);
+  w.l += __shfl_xor(w.l, 16, 64);
+  w.l += __shfl_xor(w.l, 32, 64);
+  x_sum[32 * half + query] = w.l;
+  x_m[query] = w.m;
+  if constexpr (MASK) reinterpret_cast<int *>(sm + F::LIM)[query] = limit;
+  __syncthreads();
+  float l = x_sum[lane & 31] + x_sum[32 + (lane & 31)];
+  const float m = x_m[lane & 31];
+  if constexpr (MASK) {
+    const int *odd = reinterpret_cast<const int *>(sm + F::ODD);
+    const int first = min(min(odd[0], odd[1]), min(odd[2], odd[3]));
+    l = first < reinterpret_cast<const int *>(sm + F::LIM)[lane & 31] ? __uint_as_float(0x7fc00000u) : l;
+  }
+  store_split<1>(p, sm, w.o, l, m, at.b, at.chunk, at.slot, at.splits, wave);
 }
 
 // Joins the splits of a query row: sum_j 2^(lse_j - max) O_j / sum_j 2^(lse_j - max).  One workgroup a row, wave k
@@ -908,13 +1273,13 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
 constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 
 // 32-row groups of a workgroup: as many as the rows of a sequence fill, since they share each tile's way through LDS, but
-// fewer while the cached rows do not keep all CUs at work for long: then more, shorter workgroups win.  Measured with 128
-// heads, one new token and fp8 rows (1 / 2 / 4 groups): 1 x 257 rows 17.2 / 18.9 / 21.5 us, 64 x 200 35.6 / 46.7 / 51.7,
-// 1 x 16384 33.8 / 34.8 / 43.1, 4 x 8192 42.0 / 37.5 / 39.2, 8 x 8192 65.5 / 49.4 / 45.6, 8 x 32768 205 / 126 / 90.
+// one (the kernel for few query rows) while the cached rows do not keep all CUs at work for long: then more, shorter
+// workgroups win.  Measured with 128 heads and one new token (1 / 2 / 4 groups, us), fp8: 1 x 257 rows 15.9 / 18.9 / 23.0,
+// 64 x 200 30 / 47 / 53, 8 x 4096 34 / 37 / 41, 8 x 8192 50 / 49 / 48, 32 x 4096 88 / 81 / 68, 8 x 32768 145 / 126 / 95;
+// bf16: 8 x 4096 34 / 40 / 42, 8 x 8192 49 / 54 / 50, 8 x 32768 148 / 146 / 105; 64 heads, 40 x 4096, fp8 70 / 63.
 static int attn_groups(int64_t seqs, int64_t rows, int64_t max_rows) {
-  const int fill = rows > 64 ? 4 : rows > 32 ? 2 : 1;
   const double pairs = (double)seqs * rows * max_rows / LA_UNITS;  // query rows x cached rows of a CU
-  return std::min(fill, pairs <= 32 * 256 ? 1 : pairs <= 32 * 512 ? 2 : 4);
+  return pairs <= 32 * 1024 || rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
 }
 struct AttnSizes {
   int hg;
@@ -932,12 +1297,24 @@ static AttnSizes attn_sizes(int64_t seqs, int64_t rows, int64_t max_rows) {
 
 template <bool F8, int HG>
 static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
-  const auto kernel = p.seq_len > 1 ? latent_attn_kernel<F8, HG, true> : latent_attn_kernel<F8, HG, false>;
+  typedef void (*Kernel)(LatentAttnParams);
+  Kernel one, many;  // one new token, or some
+  int lds;
+  if constexpr (HG == 1) {
+    one = latent_attn_few_kernel<F8, false>;
+    many = latent_attn_few_kernel<F8, true>;
+    lds = FewStage<F8>::LDS;
+  } else {
+    one = latent_attn_kernel<F8, HG, false>;
+    many = latent_attn_kernel<F8, HG, true>;
+    lds = Stage<F8>::LDS;
+  }
   static const hipError_t attr[2] = {
-      hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
-      hipFuncSetAttribute((const void *)latent_attn_kernel<F8, HG, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
+      hipFuncSetAttribute((const void *)one, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
+      hipFuncSetAttribute((const void *)many, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
   (void)attr;
-  kernel<<<dim3((unsigned)(p.slots + 7) / 8 * 8), 256, Stage<F8>::LDS, st>>>(p);  // whole runs of every XCD
+  const Kernel kernel = p.seq_len > 1 ? many : one;
+  kernel<<<dim3((unsigned)(p.slots + 7) / 8 * 8), 256, lds, st>>>(p);  // whole runs of every XCD
   int rc = check_launch("latent_attention");
   if (rc) return rc;
   latent_join_kernel<F8, HG><<<dim3((unsigned)p.rows, (unsigned)p.seqs), 256, 0, st>>>(p);

@@ -17,13 +17,13 @@ def _regs(text: str) -> set:
 
 
 def mfma_hazards(instrs: list) -> list:
-    """``instrs``: (instruction, from inline asm) pairs of one kernel."""
+    """``instrs``: (instruction, from inline asm) pairs of one kernel; the compiler's own matrix instructions are its care."""
     issues, written, live = [], [], []  # live: [registers, wait states since, text]
-    for s, _ in instrs:
+    for s, ours in instrs:
         op, _, rest = s.partition(" ")
         args = rest.split(",")
         mfma = op.startswith("v_mfma")
-        if mfma:
+        if mfma and ours:
             sources, states = _regs(",".join(args[1:])), 0
             for count, regs, text in reversed(written):
                 if states >= 2:
@@ -37,7 +37,7 @@ def mfma_hazards(instrs: list) -> list:
                     issues.append(f"{s}  touches the result of [{text}] after {since}")
         count = int(args[0]) + 1 if op == "s_nop" else 8 if mfma else 1
         live = [[r, n + count, t] for r, n, t in live if n + count < 18]
-        if mfma:
+        if mfma and ours:
             live.append([_regs(args[0]), 0, s])
         plain = op.startswith("v_") and not mfma and not op.startswith("v_cmp")
         written = (written + [(count, _regs(args[0]) if plain else set(), s)])[-4:]

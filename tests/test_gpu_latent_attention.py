@@ -131,16 +131,16 @@ def _wider(table, cols):
 
 
 @pytest.mark.parametrize("fp8", [True, False])
-@pytest.mark.parametrize("S,H,cols", [(1, 128, 200), (1, 128, 300), (3, 40, 200), (3, 40, 300), (2, 17, 1100)])
+@pytest.mark.parametrize("S,H,cols", [(1, 128, 530), (3, 40, 560), (2, 17, 2000), (1, 64, 1100)])
 def test_workgroups_of_more_query_rows(fp8, S, H, cols):
-    """Two and four groups of 32 query rows: taken where seqs rows max_rows passes 256 CUs times 8192 and 16384."""
+    """Two and four groups of 32 query rows: taken where sequences x rows x columns' rows pass 256 CUs times 32768."""
     lens = [700, 65]
     q, cache, table, lengths = _case(S + H, lens, S, H, fp8, 64)
     _run(q, cache, _wider(table, cols), lengths, what=f"fp8={fp8} S={S} H={H} {cols} columns")
 
 
 @pytest.mark.parametrize("fp8", [True, False])
-@pytest.mark.parametrize("S,H,cols", [(3, 5, 0), (2, 64, 0), (3, 128, 0), (3, 128, 100), (3, 128, 200), (70, 4, 0)])
+@pytest.mark.parametrize("S,H,cols", [(3, 5, 0), (2, 64, 0), (3, 128, 0), (2, 30, 1100), (3, 128, 200), (70, 4, 0)])
 def test_what_a_token_does_not_see_does_not_reach_it(fp8, S, H, cols):
     """An infinity or a NaN in one of the newest rows: the tokens before it keep their bits, the others get NaN."""
     q, cache, table, lengths = _case(71, [200, 129], S, H, fp8, 16)
