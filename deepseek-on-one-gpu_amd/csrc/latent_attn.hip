@@ -227,9 +227,9 @@ template <bool F8> struct Rows {
   static constexpr int WR = Tile<F8>::ROWS / 4, NPE = WR / 8, NLAT = F8 ? WR / 2 : WR, COPIES = NLAT + NPE;
   int slot, pe[NPE];
   AMLA_DEV void spread() {
-    const int lane = threadIdx.x & 63;
+    const int lane = fresh_lane();
 #pragma unroll
-    for (int i = 0; i < NPE; ++i) pe[i] = __shfl(slot, 8 * i + (lane >> 3), 64);
+    for (int i = 0; i < NPE; ++i) pe[i] = __builtin_amdgcn_ds_bpermute(4 * (8 * i + (lane >> 3)), slot);
   }
   // The shuffle ends before LDS operations are counted by hand.
   AMLA_DEV void landed() {
@@ -515,6 +515,7 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
     if constexpr (F8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.sum[kb] = __builtin_fmaf(e[i], __uint_as_float(ex[i]), x.sum[kb]);
+      asm volatile("" : "+v"(x.sum[kb]));  // (here: left to itself the compiler sums up at the end, and keeps all terms until then)
       int hi, lo;
       split_fp8x4(e, 0.0625f, hi, lo);
       x.phi[4 * kb + q4] = hi;
@@ -522,6 +523,7 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.sum[kb] += e[i];
+      asm volatile("" : "+v"(x.sum[kb]));
       x.pb[q4 >> 1][2 * (q4 & 1)] = pack_bf16(e[0], e[1]);
       x.pb[q4 >> 1][2 * (q4 & 1) + 1] = pack_bf16(e[2], e[3]);
     }
@@ -614,7 +616,7 @@ template <bool F8> struct Feed {
   int odd = INT32_MAX;  // the first of them with a value that is no number
   int byte[PD + 1];  // the row's exponent, -1 where it has no page; [0]: the tile in work, [PD]: the one going out
 
-  AMLA_DEV int row_of(int tile) const { return min(tile * TILE + WR * wave + (int)(threadIdx.x & 63) % WR, last); }
+  AMLA_DEV int row_of(int tile) const { return min(tile * TILE + WR * wave + fresh_lane() % WR, last); }
   AMLA_DEV int byte_of(int slot) const {
     int v = 127;
     if constexpr (F8) v = pg.scales[max(slot, 0)];
@@ -632,7 +634,7 @@ template <bool F8> struct Feed {
   AMLA_DEV void factors(int tile) {
     using G = Stage<F8>;
     uint8_t *st = sm + cur * G::SIZE;
-    const int lane = threadIdx.x & 63;
+    const int lane = fresh_lane();
     if (lane < WR) {
       const int r = WR * wave + lane;
       const bool gone = byte[0] < 0 || tile * TILE + r >= held;
