@@ -1276,12 +1276,13 @@ constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 
 // 32-row groups of a workgroup: as many as the rows of a sequence fill, since they share each tile's way through LDS, but
 // one (the kernel for few query rows) while the cached rows do not keep all CUs at work for long: then more, shorter
-// workgroups win.  Measured with 128 heads and one new token (1 / 2 / 4 groups, us), fp8: 1 x 257 rows 15.9 / 18.9 / 23.0,
-// 64 x 200 30 / 47 / 53, 8 x 4096 34 / 37 / 41, 8 x 8192 50 / 49 / 48, 32 x 4096 88 / 81 / 68, 8 x 32768 145 / 126 / 95;
-// bf16: 8 x 4096 34 / 40 / 42, 8 x 8192 49 / 54 / 50, 8 x 32768 148 / 146 / 105; 64 heads, 40 x 4096, fp8 70 / 63.
+// workgroups win.  Measured with 128 heads and one new token (1 / 2 / 4 groups, us), fp8: 1 x 257 rows 16 / 19 / 22,
+// 64 x 200 31 / 48 / 53, 8 x 4096 34 / 38 / 41, 8 x 6144 43 / 44 / 44, 32 x 2048 57 / 56 / 53, 32 x 4096 90 / 83 / 68,
+// 8 x 32768 149 / 128 / 92; bf16: 8 x 4096 34 / 40 / 41, 8 x 8192 50 / 54 / 49, 8 x 32768 148 / 145 / 104; 64 heads, 40 x
+// 4096: fp8 71 / 65, bf16 74 / 73.
 static int attn_groups(int64_t seqs, int64_t rows, int64_t max_rows) {
   const double pairs = (double)seqs * rows * max_rows / LA_UNITS;  // query rows x cached rows of a CU
-  return pairs <= 32 * 1024 || rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  return pairs < 32 * 1024 || rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
 }
 struct AttnSizes {
   int hg;
