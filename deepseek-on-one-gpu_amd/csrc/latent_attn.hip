@@ -896,16 +896,19 @@ template <bool F8> struct FewValues {
   u32x2 v[3][4];
 };
 
+// Chunk of 64 (e4m3) or 32 values that lanes 16 g .. read: an order in which the 16 lanes that LDS serves at a time, 0 - 3,
+// 12 - 15 and 20 - 27 of each half wave, find their rows' chunks in 16 different places of 256 bytes
+template <bool F8> AMLA_DEV constexpr int few_chunk(int g) { return F8 ? (g & 1) << 1 | g >> 1 : (g >> 1) ^ (3 * (g & 1)); }
 template <bool F8, int I> AMLA_DEV void few_read(u32x4 (&d)[2], uint32_t kl, uint32_t kr) {
   if constexpr (F8) {
-    if constexpr (I < 8) {  // codes 64 I + 16 (lane / 16) ..
+    if constexpr (I < 8) {  // codes 64 I + 16 few_chunk ..
       d[0] = lds_read16<256 * (I >> 2)>(kl ^ (64 * (I & 3)));
       d[1] = lds_read16<256 * (I >> 2) + 16 * 512>(kl ^ (64 * (I & 3)));
     } else {
       d[0] = lds_read16<0>(kr ^ (64 * (I - 8)));
       d[1] = lds_read16<16 * 128>(kr ^ (64 * (I - 8)));
     }
-  } else {  // values 32 I + 8 (lane / 16) ..
+  } else {  // values 32 I + 8 few_chunk ..
     if constexpr (I < 16) d[0] = lds_read16<256 * (I >> 2)>(kl ^ (64 * (I & 3)));
     else d[0] = lds_read16<0>(kr ^ (64 * (I - 16)));
   }
@@ -962,7 +965,7 @@ AMLA_DEV void few_scores(FewWave<F8> &w, FewFactors<F8> &f, uint32_t base, int h
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f.mul[0]) : "v"(fm), "i"(G::MUL) : "memory");
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f.mul[1]) : "v"(fm), "i"(G::MUL + 64) : "memory");
   }
-  const uint32_t kl = base + row * Tile<F8>::RB + 16 * (g ^ Tile<F8>::swz(row));
+  const uint32_t kl = base + row * Tile<F8>::RB + 16 * (few_chunk<F8>(g) ^ Tile<F8>::swz(row));
   const uint32_t kr = base + G::PE + row * 128 + 16 * (g ^ ((row >> 1) & 7));
   u32x4 ka[FewWave<F8>::AHEAD + 1][2];
   few_reads_first<F8, 0>(ka, kl, kr);
@@ -1128,7 +1131,8 @@ __global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParam
   const int limit = at.held - (p.seq_len - 1 - tok), lim = limit - TILE / 2 * half - 4 * g;
   const uint16_t *qp = p.q + at.b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w.q[i] = as_bf16x8(ldg16(qp + (F8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g)));
+  for (int i = 0; i < 16; ++i)
+    w.q[i] = as_bf16x8(ldg16(qp + (F8 ? 64 * (i >> 1) + 16 * few_chunk<F8>(g) + 8 * (i & 1) : 32 * i + 8 * few_chunk<F8>(g))));
 #pragma unroll
   for (int i = 0; i < 2; ++i) w.q[16 + i] = as_bf16x8(ldg16(qp + LC_LORA + 32 * i + 8 * g));
   w.m = M_NONE;

@@ -122,7 +122,7 @@ AMLA_DEV void pa_settle(f32x16 (&o)[2][4]) {
 
 // Where a wave's copies come from: rows 16 w .. + 15 of a tile, as 8-row pieces of 128-byte half-rows.  Bases are
 // uniform, each lane adds a fixed offset; chunk c of row r of a key array sits at c ^ ((r >> 1) & 7), the 64-byte
-// half g of a value row at g ^ ((r >> 2) & 1), both free of bank conflicts.
+// half g of a value row at g ^ ((r >> 1) & 1), both free of bank conflicts.
 struct PackedFeed {
   const char *k, *v, *pe;       // the head's first key, value and rope key of the sequence
   int64_t ldk, ldv, ldpe;       // bytes of a row
@@ -138,7 +138,7 @@ struct PackedFeed {
       ok[g] = rr * (uint32_t)ldk + kc;
       op[g] = rr * (uint32_t)ldpe + kc;
     }
-    ov = rr * (uint32_t)ldv + 16 * ((lane & 7) ^ (4 * ((r8 >> 2) & 1)));
+    ov = rr * (uint32_t)ldv + 16 * ((lane & 7) ^ (4 * ((r8 >> 1) & 1)));
   }
   // First key of the tile that is loaded as tile j: the last one ends with the last key (what it repeats is masked).
   AMLA_DEV int first(int j) const { return max(min(j * PA_KT, klim - PA_KT), 0); }
@@ -166,7 +166,7 @@ struct PackedFeed {
     for (int g = 0; g < 2; ++g) {
       const int r8 = lane >> 3;
       const int64_t row = min(row0 + 8 * g + r8, klim - 1);
-      const int kc = 16 * ((lane & 7) ^ ((r8 >> 1) + 4 * g)), vc = 16 * ((lane & 7) ^ (4 * ((r8 >> 2) & 1)));
+      const int kc = 16 * ((lane & 7) ^ ((r8 >> 1) + 4 * g)), vc = 16 * ((lane & 7) ^ (4 * ((r8 >> 1) & 1)));
       uint8_t *dst = st + (row0 + 8 * g) * 128;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -291,7 +291,7 @@ template <bool ROPE> AMLA_DEV uint32_t pa_key_addr(uint32_t stage) {
 }
 template <bool ROPE> AMLA_DEV uint32_t pa_val_addr(uint32_t stage) {
   const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
-  return stage + PackedWave<ROPE>::VAL + (4 * hh + (L16 >> 2)) * 128 + 64 * hh + 32 * (g16 & 1) + 8 * (L16 & 3);
+  return stage + PackedWave<ROPE>::VAL + (4 * hh + (L16 >> 2)) * 128 + 64 * (L16 >> 3) + 32 * (g16 & 1) + 8 * (L16 & 3);
 }
 // The next tile landed in every wave, and no wave reads the stage two tiles back any more
 AMLA_DEV void pa_arrive() {
