@@ -1,5 +1,12 @@
 // Attention of the newest tokens over the paged latent cache (latent.h), in latent space:
 //   s_t = scale q . (c_t | r_t),  out = sum_t softmax(s)_t c_t
+// One pass over the cached rows with a running sum per query row, all in fp32; scores are products of bf16 (e4m3 codes are
+// exact in it), probabilities are rounded once for the matrix units: to bf16, or to two e4m3 halves that hold eight bits
+// of them (inference/ops.py:179 rounds them to bf16).  Every row of the cache serves all heads, so it is read once from
+// memory per 128 query rows and split of the sequence.  Many query rows: latent_attn_kernel, bound by the matrix units
+// (8 x 32768 rows, 128 heads, e4m3: 91 us where 73 GFLOP at a large product's rate take 61; the units are busy 42 % of
+// the cycles, conversions, softmax and barriers take the others).  Few: latent_attn_few_kernel, bound by the copies (40
+// ragged sequences, 16 heads, bf16: 64 us for 342 MB, the copies alone 58).  Then latent_join_kernel.
 #include <algorithm>
 #include <math.h>
 
@@ -767,9 +774,12 @@ template <bool F8> AMLA_DEV SplitWork split_work(const LatentAttnParams &p) {
                    (int)((int64_t)(split + 1) * n_tiles / at.z)};
 }
 
-// One workgroup of four waves per (sequence, chunk of 32 HG rows, split).  HG waves hold 32
+// One workgroup of four waves per (sequence, chunk of 32 HG rows, split).  HG (2 or 4) waves hold 32
 // query rows each; the 4 / HG waves of the same rows compute the same scores and
-// accumulate 512 HG / 4 columns each.
+// accumulate 512 HG / 4 columns each.  O^T fills half of a wave's 512 registers, the queries
+// most of the others: one wave a SIMD, whose own products hide its conversions, copies, LDS
+// reads and softmax, each placed between two of them (one phase after the other took twice
+// as long).  What spills in the loop costs most: a reload waits behind all copies under way.
 template <bool F8, int HG, bool MASK>
 __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p) {
   extern __shared__ __align__(1024) uint8_t sm[];

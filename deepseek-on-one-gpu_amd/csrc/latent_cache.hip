@@ -37,7 +37,8 @@ int latent_pages(const amla_latent_cache *c, const char *what, LatentPages *p) {
 
 constexpr int LC_WAVES = 4;
 
-// One wave per row: lane l holds latents 8l .. 8l+7 and, for l < 32, the rope pair l.
+// One wave per row: lane l holds latents 8l .. 8l+7 and, for l < 32, the rope pair l.  Bound by latency (offsets, table,
+// row, table of angles): 4.0 us for 32 rows, 7.1 for 8111 (14.5 MB; 3.1 at a copy's rate).
 template <bool F8>
 __global__ __launch_bounds__(64 * LC_WAVES) void latent_write_kernel(LatentPages pg, PackedRows map,
                                                                      const uint16_t *__restrict__ kv, int rows,
@@ -100,7 +101,8 @@ __global__ __launch_bounds__(64 * LC_WAVES) void latent_write_kernel(LatentPages
   }
 }
 
-// LC_ROWS rows a wave, each found by the lane of its number, then moved by the whole wave.
+// LC_ROWS rows a wave: their places are looked up first, so that the loads of all of them are under way together.  e4m3 to
+// bf16 is exact.  40001 rows, 72 MB: 15.2 us, 4.7 TB/s, the rate of a large copy; 8111 rows 6.9 us, 1501 of bf16 4.6.
 constexpr int LC_ROWS = 4;
 
 template <bool F8>
