@@ -44,6 +44,12 @@ AMLA_DEV void copy_lds_nt(const void *src, void *dst) { __builtin_amdgcn_global_
 // Host checks of a cache shared by its entry points: 0 or the code of fail().
 int latent_pages(const amla_latent_cache *c, const char *what, LatentPages *p);
 
+// Lets a kernel have all of a CU's LDS; per call, since it holds for the current device.
+template <typename F> inline int latent_lds(F *fn, const char *what) {
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  return e == hipSuccess ? AMLA_OK : fail((int)e, "%s: LDS size: %s", what, hipGetErrorString(e));
+}
+
 // The sequence of packed row i (the same in every lane): the number of b with
 // offsets[b + 1] <= i, for ascending offsets; seqs if none holds it.  All loads of 64
 // offsets each are independent, so it takes one round trip, not one per halving.

@@ -6,7 +6,7 @@
 // memory per 128 query rows and split of the sequence.  Many query rows: latent_attn_kernel, bound by the matrix units
 // (8 x 32768 rows, 128 heads, e4m3: 91 us where 73 GFLOP at a large product's rate take 61; the units are busy 42 % of
 // the cycles, conversions, softmax and barriers take the others).  Few: latent_attn_few_kernel, bound by the copies (40
-// ragged sequences, 16 heads, bf16: 64 us for 342 MB, the copies alone 58).  Then latent_join_kernel.
+// ragged sequences, 16 heads, bf16: 64 us for 342 MB; the copies alone take nine tenths).  Then latent_join_kernel.
 #include <algorithm>
 #include <math.h>
 
@@ -1080,7 +1080,7 @@ template <bool F8> AMLA_DEV void few_values_first(FewValues<F8> &x, uint32_t pbu
   x.p[1] = lds_read16<1024>(pbuf + 16 * lane);
   if constexpr (F8) {
     x.p[2] = lds_read16<2048>(pbuf + 16 * lane);
-    x.p[3] = lds_read16<3072>(pbuf + 16 * lane);
+    x.p[3] = lds_read16<3 * 1024>(pbuf + 16 * lane);
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(x.ps) : "v"(pbuf + 4 * lane), "i"(FewStage<F8>::PS) : "memory");
   }
   few_value_read<F8, 0>(x, v.x, v.y);
@@ -1314,26 +1314,19 @@ static AttnSizes attn_sizes(int64_t seqs, int64_t rows, int64_t max_rows) {
 
 template <bool F8, int HG>
 static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
-  typedef void (*Kernel)(LatentAttnParams);
-  Kernel one, many;  // one new token, or some
+  void (*kernel)(LatentAttnParams);
   int lds;
   if constexpr (HG == 1) {
-    one = latent_attn_few_kernel<F8, false>;
-    many = latent_attn_few_kernel<F8, true>;
+    kernel = p.seq_len > 1 ? latent_attn_few_kernel<F8, true> : latent_attn_few_kernel<F8, false>;
     lds = FewStage<F8>::LDS;
   } else {
-    one = latent_attn_kernel<F8, HG, false>;
-    many = latent_attn_kernel<F8, HG, true>;
+    kernel = p.seq_len > 1 ? latent_attn_kernel<F8, HG, true> : latent_attn_kernel<F8, HG, false>;
     lds = Stage<F8>::LDS;
   }
-  static const hipError_t attr[2] = {
-      hipFuncSetAttribute((const void *)one, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
-      hipFuncSetAttribute((const void *)many, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
-  (void)attr;
-  const Kernel kernel = p.seq_len > 1 ? many : one;
-  kernel<<<dim3((unsigned)(p.slots + 7) / 8 * 8), 256, lds, st>>>(p);  // whole runs of every XCD
-  int rc = check_launch("latent_attention");
+  int rc = latent_lds(kernel, "latent_attention");
   if (rc) return rc;
+  kernel<<<dim3((unsigned)(p.slots + 7) / 8 * 8), 256, lds, st>>>(p);  // whole runs of every XCD
+  if ((rc = check_launch("latent_attention"))) return rc;
   latent_join_kernel<F8, HG><<<dim3((unsigned)p.rows, (unsigned)p.seqs), 256, 0, st>>>(p);
   return check_launch("latent_attention join");
 }

@@ -252,7 +252,7 @@ template <int C> AMLA_DEV void pa_val_read(u32x2 (&v)[4], uint32_t v0) {
     v[0] = pa_read_tr<ofs>(a);
     v[1] = pa_read_tr<ofs + 1024>(a);
     v[2] = pa_read_tr<ofs + 2048>(a);
-    v[3] = pa_read_tr<ofs + 3072>(a);
+    v[3] = pa_read_tr<ofs + 3 * 1024>(a);
   }
 }
 // What goes behind product K of score step I: a copy of the tile to come (one a step) or late probabilities
@@ -639,9 +639,8 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
 template <bool ROPE>
 static int launch_packed(const PackedParams &p, int64_t blocks, hipStream_t st) {
   constexpr int lds = PackedWave<ROPE>::STAGE * PA_NST;
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void *)packed_attn_kernel<ROPE>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-  (void)attr;
+  const int rc = latent_lds(packed_attn_kernel<ROPE>, "packed_attention");
+  if (rc) return rc;
   packed_attn_kernel<ROPE><<<dim3((unsigned)blocks), 256, lds, st>>>(p);
   return check_launch("packed_attention");
 }
