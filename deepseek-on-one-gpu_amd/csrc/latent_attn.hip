@@ -28,8 +28,11 @@ struct LatentAttnParams {
   float scale_log2;
   uint16_t *out;
   float *lse;
-  uint16_t *part_o;                // (slots, rows of a chunk, 512) bf16, each split normalised
-  float *part_lse;                 // (slots, rows of a chunk) log2 of the split's sum of 2^s
+  // Of each split: its sums, normalised, (slots, rows of a chunk, 512) in fp16 times part_scale, a power of two for each of
+  // the up to four waves that hold a row's columns; log2 of its sum of 2^s.  fp16 and not bf16, whose rounding would add as
+  // much error as the output's own; fp32 would be twice the bytes, a tenth of a long batch's time.
+  uint16_t *part_o;
+  float *part_lse, *part_scale;    // (slots, rows of a chunk), (slots, rows of a chunk, 4)
 };
 
 AMLA_DEV int lc_ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -136,7 +139,8 @@ template <bool F8> struct Stage {
 };
 
 // The reference m of a query row's sums is its maximum over the split's first tile, so that the output
-// accumulators are never multiplied: fp32 and bf16 have the range, and e4m3 has a scale for each block.  A
+// accumulators are never multiplied: fp32 and bf16 have the range, and e4m3 has a scale for each block.  It is the maximum
+// itself, not a whole number above it: the probability of the loudest row, all there is of a short sequence, is not rounded.  A
 // row whose scores pass m by 2^LAG later on (or that saw nothing in the first tile) has the workgroup do
 // its split once more, with m from all of it.
 constexpr float LAG = 60.f;
@@ -478,6 +482,11 @@ template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F
   }
 }
 
+// The reference of a block of e4m3 probabilities, whose largest score is mx: m plus a whole number, so that the block's scale
+// is a power of two, and 2^(mx - ref) in 128 .. 256 (m's own row: 128, without rounding)
+AMLA_DEV float block_ref(float mx, float m) { return m + (floorf(__builtin_fmaxf(mx, M_NONE) - m) - 7.f); }
+// Its scale for the matrix unit: 2^(ref - m), whole but for the rounding of ref
+AMLA_DEV int block_scale(float ref, float m) { return (int)__builtin_rintf(__builtin_fmaxf(ref - m, -123.f)) + 127; }
 // Slice S of the softmax, its row factors in ex:
 //   z = s log2(e) scale + exponent of the row, P = 2^(z - ref), l sums 2^(s - m) = P 2^(ref - m - exponent)
 // e4m3: 32 rows are one block of the matrix unit with a scale of its own, 2^(ref - m), so that rows far
@@ -508,10 +517,10 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
       }
       const float top = __builtin_fmaxf(x.mx[0], x.mx[KB - 1]);
       w.top = __builtin_fmaxf(w.top, top);
-      w.m = w.m == M_NONE ? __builtin_fmaxf(ceilf(top), M_NONE) : w.m;
+      w.m = w.m == M_NONE ? __builtin_fmaxf(top, M_NONE) : w.m;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        x.ref[k] = F8 ? floorf(__builtin_fmaxf(x.mx[k], M_NONE)) - 7.f : w.m;
+        x.ref[k] = F8 ? block_ref(x.mx[k], w.m) : w.m;
         x.sum[k] = 0.f;
       }
     }
@@ -600,7 +609,7 @@ AMLA_DEV void value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, flo
     for (int k = 0; k < KB; ++k) w.l += F8 ? x.sum[k] * __builtin_amdgcn_exp2f(x.ref[k] - w.m) : x.sum[k];
     // the scale of block k comes from the lanes of half k; 4 .. 160, the low halves' 4 less
     if constexpr (F8) {
-      w.ps = (int)__builtin_fmaxf((hh ? x.ref[KB - 1] : x.ref[0]) - w.m, -123.f) + 127;
+      w.ps = block_scale(hh ? x.ref[KB - 1] : x.ref[0], w.m);
       w.ps_lo = w.ps - 4;
     }
     w.phi = x.phi;
@@ -720,6 +729,24 @@ template <bool F8> struct Feed {
   }
 };
 
+AMLA_DEV uint32_t pack_f16(float a, float b) {  // to nearest even
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+}
+// A wave's sums times inv as rows in LDS: of 16 NCB values in each lane's row, chunk c of 16 bytes at c ^ row
+template <bool F16, int NCB> AMLA_DEV void turn_rows(uint8_t *turn, const f32x16 (&o)[NCB], float inv) {
+  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int c = 0; c < NCB; ++c)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = o[c][4 * q4 + i] * inv;
+      *reinterpret_cast<u32x2 *>(turn + j32 * 64 * NCB + 16 * ((4 * c + q4) ^ (j32 % (4 * NCB))) + 8 * hh) =
+          F16 ? u32x2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])} : u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    }
+}
 // A split's sums, normalised: the output itself, or a partial one.  l, m: of the lane's query row.
 template <int HG, int NCB>
 AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB], float l, float m, int b, int chunk, int slot,
@@ -727,17 +754,26 @@ AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB
   constexpr int CG = 4 / HG;
   const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5, hg = wave / CG, cg = wave % CG;
   const int row = (chunk * HG + hg) * 32 + j32;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse2 = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
-  // rows of 1 KB / CG through LDS (chunk c of a wave's row at c ^ row), so that a store is whole lines
+  float scale = 1.f;
+  if (splits > 1) {  // the largest of the row's values in this wave to 2^14 .. 2^15
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < NCB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(o[c][i]));
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    top = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * inv;
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 240);  // biased; below 15: zeros nearly
+    scale = __uint_as_float((uint32_t)(e - 14) << 23);                   // 2^(e - 127 - 14)
+    inv *= __uint_as_float((uint32_t)(254 - (e - 14)) << 23);
+  }
+  // rows of 1 KB / CG through LDS, so that a store is whole lines
   constexpr int RBYTES = 1024 / CG;
   uint8_t *turn = sm + wave * 32 * RBYTES;
-#pragma unroll
-  for (int c = 0; c < NCB; ++c)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-      *reinterpret_cast<u32x2 *>(turn + j32 * RBYTES + 16 * ((4 * c + q4) ^ (j32 % (4 * NCB))) + 8 * hh) =
-          u32x2{pack_bf16(o[c][4 * q4] * inv, o[c][4 * q4 + 1] * inv), pack_bf16(o[c][4 * q4 + 2] * inv, o[c][4 * q4 + 3] * inv)};
+  if (splits > 1) turn_rows<true>(turn, o, inv);
+  else turn_rows<false>(turn, o, inv);
   const int row0 = (chunk * HG + hg) * 32, held = min(32, p.rows - row0);
   const size_t dst0 = splits == 1 ? (size_t)b * p.rows + row0 : (size_t)slot * (32 * HG) + 32 * hg;
   uint16_t *to[2] = {p.part_o, p.out};
@@ -751,6 +787,7 @@ AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB
       *reinterpret_cast<u32x4 *>(od + (size_t)r * (LC_LORA * 2) + 16 * c) =
           *reinterpret_cast<const u32x4 *>(turn + r * RBYTES + 16 * (c ^ (r % (4 * NCB))));
   }
+  if (splits > 1 && hh == 0 && row < p.rows) p.part_scale[(dst0 + j32) * 4 + cg] = scale;
   if (cg == 0 && hh == 0 && row < p.rows) {
     if (splits > 1) p.part_lse[dst0 + j32] = lse2;
     else if (p.lse) p.lse[dst0 + j32] = lse2 * 0.6931471805599453f;
@@ -862,7 +899,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
     if constexpr (MASK) feed.odd = (int)min(min(vote[4], vote[5]), min(vote[6], vote[7]));
     __syncthreads();
     if (!again) break;
-    w.m = low ? ceilf(w.top) : w.m;
+    w.m = low ? w.top : w.m;
     feed.start(t_first);
   }
 
@@ -1016,7 +1053,7 @@ template <bool F8> AMLA_DEV void few_probabilities(FewWave<F8> &w, const FewFact
   const uint32_t to = pbuf + 1024 * half + 16 * (query + 32 * (g & 1));
   w.top = __builtin_fmaxf(w.top, top);
   if constexpr (F8) {
-    const float ref = floorf(__builtin_fmaxf(few_max(top), M_NONE)) - 7.f;  // of the 32 rows: a block of the matrix unit
+    const float ref = block_ref(few_max(top), w.m);  // of the 32 rows: a block of the matrix unit
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -1032,7 +1069,7 @@ template <bool F8> AMLA_DEV void few_probabilities(FewWave<F8> &w, const FewFact
       few_write(to + FewStage<F8>::LO + 4 * (g >> 1) + 8 * u, lo);
     }
     w.l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(ref - w.m), w.l);
-    few_write(pbuf + FewStage<F8>::PS + 4 * (32 * half + query), (int)__builtin_fmaxf(ref - w.m, -123.f) + 127);
+    few_write(pbuf + FewStage<F8>::PS + 4 * (32 * half + query), block_scale(ref, w.m));
   } else {
     float e[4];
 #pragma unroll
@@ -1165,7 +1202,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParam
       const float top = few_max(few_scaled<F8, MASK>(w, f, p.scale_log2, lim - at.t_first * TILE));
       x_top[32 * half + query] = top;
       __syncthreads();
-      w.m = __builtin_fmaxf(ceilf(__builtin_fmaxf(x_top[query], x_top[32 + query])), M_NONE);
+      w.m = __builtin_fmaxf(__builtin_fmaxf(x_top[query], x_top[32 + query]), M_NONE);
     }
     uint32_t base = lds0, pbuf = lds0 + F::P;
     for (int tile = at.t_first; tile < at.t_end; ++tile) {
@@ -1200,7 +1237,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParam
     const bool again = __ballot(__builtin_fmaxf(x_top[lane & 31], x_top[32 + (lane & 31)]) > x_m[lane & 31] + LAG) != 0;
     __syncthreads();
     if (!again) break;
-    w.m = high > w.m + LAG ? ceilf(high) : w.m;
+    w.m = high > w.m + LAG ? high : w.m;
     feed.start(at.t_first);
   }
   // sums over the four lanes and both halves of a query, handed to the lanes that hold its outputs
@@ -1247,23 +1284,28 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
   const float ref = top == -INFINITY ? 0.f : top;
   float total = 0.f, a[8] = {};
   const uint16_t *po = p.part_o + src * LC_LORA + 8 * lane;
+  const float *ps = p.part_scale + src * 4 + lane / (64 * HG / 4);
   for (int j0 = wave; j0 < n; j0 += 32) {
-    float w[8];
+    float w[8], s[8];
     u32x4 v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int j = min(j0 + 4 * k, n - 1);
       v[k] = ldg16(po + (size_t)j * (32 * HG * LC_LORA));
+      s[k] = ps[(size_t)j * (32 * HG * 4)];
       w[k] = j0 + 4 * k < n ? lse[(size_t)j * (32 * HG)] - ref : -INFINITY;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float f = __builtin_amdgcn_exp2f(w[k]);
       total += f;
+      typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        a[2 * e] = __builtin_fmaf(f, lo_bf(v[k][e]), a[2 * e]);
-        a[2 * e + 1] = __builtin_fmaf(f, hi_bf(v[k][e]), a[2 * e + 1]);
+        const uint32_t word = v[k][e];  // (a cast of the element itself takes element 0)
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, word);
+        a[2 * e] = __builtin_fmaf(f, (float)h[0] * s[k], a[2 * e]);
+        a[2 * e + 1] = __builtin_fmaf(f, (float)h[1] * s[k], a[2 * e + 1]);
       }
     }
   }
@@ -1341,7 +1383,7 @@ size_t amla_latent_attention_workspace_bytes(int64_t seqs, int64_t seq_len, int6
   if (seqs <= 0 || seq_len <= 0 || heads <= 0 || seqs > AMLA_MAX_SEQS || seq_len > INT32_MAX || heads > INT32_MAX / seq_len)
     return 0;
   const AttnSizes s = attn_sizes(seqs, seq_len * heads, max_rows);
-  return (size_t)s.slots * 32 * s.hg * (LC_LORA * 2 + 4);
+  return (size_t)s.slots * 32 * s.hg * (LC_LORA * 2 + 4 + 16);
 }
 
 int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t seqs, int64_t seq_len, int64_t heads,
@@ -1376,6 +1418,7 @@ int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t
   p.lse = lse;
   p.part_o = static_cast<uint16_t *>(workspace);
   p.part_lse = reinterpret_cast<float *>(p.part_o + (size_t)s.slots * 32 * s.hg * LC_LORA);
+  p.part_scale = p.part_lse + (size_t)s.slots * 32 * s.hg;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (p.pg.scales) {
     if (s.hg == 4) return launch_attn<true, 4>(p, st);

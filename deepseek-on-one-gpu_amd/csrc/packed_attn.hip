@@ -91,7 +91,8 @@ template <bool ROPE> struct PackedWave {
   float x[2][2];   // the last two probabilities, not yet summed and packed
   float m[2], l[2], top[2];  // reference (log2 units), sum of 2^(z - m), largest score so far
 };
-// The reference m is the maximum of the first tile that shows a row any key: fp32 and bf16 have the range for
+// The reference m is the maximum of the first tile that shows a row any key (itself, not a whole number above it: the
+// probability of the largest score, all there is where few keys are seen, is not rounded): fp32 and bf16 have the range for
 // sums up to 2^PA_LAG above it.  A row that passes it has the workgroup start over with m from all keys.
 constexpr float PA_LAG = 60.f, PA_NONE = -1e30f;
 
@@ -361,7 +362,7 @@ template <bool ROPE, bool MASK, int N> AMLA_DEV void pa_max(PackedWave<ROPE> &w,
 AMLA_DEV void pa_refer(float &top, float &m, float c) {
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
   top = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-  m = m == PA_NONE ? __builtin_fmaxf(ceilf(top * c), PA_NONE) : m;
+  m = m == PA_NONE ? __builtin_fmaxf(top * c, PA_NONE) : m;
 }
 // What goes behind value product N: a part of the mask and the maximum of the scores (0 .. 7), the reference, then an early
 // probability each
@@ -588,8 +589,8 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     odd = votes & 2;
     if (!(votes & 1) && (careful || !(votes & 4))) break;
     careful |= (votes & 4) != 0;
-    w.m[0] = low0 ? ceilf(w.top[0] * c) : w.m[0];
-    w.m[1] = low1 ? ceilf(w.top[1] * c) : w.m[1];
+    w.m[0] = low0 ? w.top[0] * c : w.m[0];
+    w.m[1] = low1 ? w.top[1] * c : w.m[1];
     f.copy_first<ROPE>(sm, lane);
   }
 

@@ -63,7 +63,8 @@ def check_attention(got, want, lse, want_lse, weight, size, what):
     the row's largest), so it is off by at most ds = (576 2^-24 + 2^-21) size, the last part for the
     products with log2 e and the scale.  A probability is off by expm1(2 ds) at most, then rounded to
     bf16 or to two e4m3 halves: 2^-8 at most.  l is the fp32 sum of unrounded probabilities.  A split's
-    sums are rounded to bf16 (2^-8 of them, at most of the weight), the joined ones again.  So
+    sums are rounded too (to fp16 times a power of two: far less than the 2^-8 of the weight counted
+    here), the joined ones to bf16.  So
     |d out| <= weight (expm1(2 ds) + 2^-7) + 2^-8 |out| + 2^-24, and |d lse| <= ds + 2^-20 (1 + |lse|)."""
     got, lse = got.double().cpu(), lse.double().cpu()
     empty = want_lse == float("-inf")
