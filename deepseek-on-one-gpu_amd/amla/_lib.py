@@ -51,7 +51,7 @@ class PackedArgs(ctypes.Structure):
                 ("k_rows", c_int64), ("seqs", c_int64), ("ldq", c_int64), ("ldq_head", c_int64), ("ldk", c_int64),
                 ("ldk_head", c_int64), ("ldv", c_int64), ("ldv_head", c_int64), ("ld_pe", c_int64),
                 ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("dn", ctypes.c_int32),
-                ("causal", ctypes.c_int32), ("scale", c_float)]
+                ("causal", ctypes.c_int32), ("scale", c_float), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 # (name, restype, argtypes) of every exported entry point
@@ -124,6 +124,7 @@ SIGNATURES = [
                                       c_void_p]),
     ("amla_latent_attention_workspace_bytes", c_size_t, [c_int64, c_int64, c_int64, c_int64]),
     ("amla_packed_attention", c_int, [ctypes.POINTER(PackedArgs), c_void_p]),
+    ("amla_packed_attention_workspace_bytes", ctypes.c_size_t, [c_int64, c_int64, c_int64, c_int64]),
     ("amla_moe_combine", c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_float, c_void_p,
                                  c_void_p]),
 ]

@@ -621,6 +621,7 @@ def _latent_cache_read_out(latent, k_pe, scales, block_table, offsets, position,
     torch.autograd.graph.increment_version(out_pe)
 
 
+_packed_bytes = lru_cache(4096)(lambda *a: lib().amla_packed_attention_workspace_bytes(*a))
 _lc_attention_bytes = lru_cache(4096)(lambda *a: lib().amla_latent_attention_workspace_bytes(*a))
 
 
@@ -659,9 +660,11 @@ def _packed_attention(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse):
     out, lse_out = _packed_attention_fake(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse)
     if not out.numel():
         return out, lse_out
+    need = _packed_bytes(q.shape[0], k.shape[0], offsets.shape[0] - 1, q.shape[1])
+    ws = _scratch(q.device, need) if need else None
     check(lib().amla_packed_attention(PackedArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(k_pe), out.data_ptr(), lse_out.data_ptr() if lse else None,
         offsets.data_ptr(), _ptr(k_offsets), q.shape[0], k.shape[0], offsets.shape[0] - 1, q.stride(0), q.stride(1),
         k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0 if k_pe is None else k_pe.stride(0), q.shape[1], k.shape[1],
-        k.shape[2], causal, scale), _mx_stream(q)), "packed_attention")
+        k.shape[2], causal, scale, _ptr(ws), need), _mx_stream(q)), "packed_attention")
     return out, lse_out

@@ -41,6 +41,12 @@ struct LatentPages {
 AMLA_DEV void copy_lds(const void *src, void *dst) { __builtin_amdgcn_global_load_lds(src, LDS_PTR(dst), 16, 0, 0); }
 AMLA_DEV void copy_lds_nt(const void *src, void *dst) { __builtin_amdgcn_global_load_lds(src, LDS_PTR(dst), 16, 0, 2); }
 
+// Two values in fp16, to nearest even
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+AMLA_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b}); }
+AMLA_DEV float lo_f16(uint32_t x) { return (float)__builtin_bit_cast(f16x2, x)[0]; }
+AMLA_DEV float hi_f16(uint32_t x) { return (float)__builtin_bit_cast(f16x2, x)[1]; }
+
 // Host checks of a cache shared by its entry points: 0 or the code of fail().
 int latent_pages(const amla_latent_cache *c, const char *what, LatentPages *p);
 

@@ -729,10 +729,6 @@ template <bool F8> struct Feed {
   }
 };
 
-AMLA_DEV uint32_t pack_f16(float a, float b) {  // to nearest even
-  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
-}
 // A wave's sums times inv as rows in LDS: of 16 NCB values in each lane's row, chunk c of 16 bytes at c ^ row
 template <bool F16, int NCB> AMLA_DEV void turn_rows(uint8_t *turn, const f32x16 (&o)[NCB], float inv) {
   const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
@@ -1299,13 +1295,11 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
     for (int k = 0; k < 8; ++k) {
       const float f = __builtin_amdgcn_exp2f(w[k]);
       total += f;
-      typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t word = v[k][e];  // (a cast of the element itself takes element 0)
-        const f16x2_t h = __builtin_bit_cast(f16x2_t, word);
-        a[2 * e] = __builtin_fmaf(f, (float)h[0] * s[k], a[2 * e]);
-        a[2 * e + 1] = __builtin_fmaf(f, (float)h[1] * s[k], a[2 * e + 1]);
+        const uint32_t x = v[k][e];
+        a[2 * e] = __builtin_fmaf(f, lo_f16(x) * s[k], a[2 * e]);
+        a[2 * e + 1] = __builtin_fmaf(f, hi_f16(x) * s[k], a[2 * e + 1]);
       }
     }
   }

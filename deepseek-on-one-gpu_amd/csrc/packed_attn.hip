@@ -31,8 +31,13 @@ struct PackedParams {
   const int32_t *offsets, *k_offsets;
   int q_rows, k_rows, seqs, heads, group, causal;
   int tiles;                         // query blocks of all sequences, at most
+  int splits;                        // workgroups of a block, at most
   int64_t ldq, ldq_head, ldk, ldk_head, ldv, ldv_head, ld_pe;
   float scale_log2;
+  // With splits: of each (block, head, split) 256 rows of 128 sums, normalised, in fp16 times a power of two a row (bf16 would
+  // add as much error as the output's rounding), and (log2 of the sum of 2^s, the power) of each row
+  uint16_t *part_o;
+  float *part_ls;
 };
 
 // Offsets are not checked on the host: clamped to the rows there are, and none below its predecessor's.
@@ -70,6 +75,32 @@ AMLA_DEV PackedBlock find_block(const PackedParams &p, int tile) {
     base += __builtin_amdgcn_readlane(incl, 63);
   }
   return PackedBlock{-1, 0, 0, 0, 0};
+}
+
+// Tiles of 64 keys that one workgroup takes of a block: with few blocks their keys are split, so that all CUs have work and
+// no block is much longer than the others: total / 256, but not below PA_LEAST (2 us each; starting and joining take 10).
+constexpr int PA_LEAST = 6;
+AMLA_DEV int split_tiles(const PackedParams &p) {
+  const int lane = threadIdx.x & 63;
+  float total = 0.f;
+  for (int b0 = 0; b0 < p.seqs; b0 += 64) {
+    const int b = min(b0 + lane, p.seqs - 1);
+    const int nq = max(span_start(p.offsets, b + 1, p.q_rows) - span_start(p.offsets, b, p.q_rows), 0);
+    const int nk = max(span_start(p.k_offsets, b + 1, p.k_rows) - span_start(p.k_offsets, b, p.k_rows), 0);
+    const float blocks = b0 + lane < p.seqs ? (float)((nq + PA_QB - 1) / PA_QB) : 0.f;
+    total += blocks * (p.causal ? max(nk - nq, 0) / (float)PA_KT + 2.f * (blocks + 1.f) : nk / (float)PA_KT);
+  }
+  const float each = wave_sum(total) * p.heads / 256.f;
+  return __builtin_amdgcn_readfirstlane(max(PA_LEAST, (int)__builtin_fminf(each, 1e9f) + 1));
+}
+// Keys that a block needs, and its splits
+AMLA_DEV int block_keys(const PackedParams &p, const PackedBlock &b) {
+  return p.causal ? min(b.nk, max(b.nk - b.nq + min((b.block + 1) * PA_QB, b.nq), 0)) : b.nk;
+}
+AMLA_DEV int block_splits(const PackedParams &p, int keys) {
+  if (p.splits == 1) return 1;
+  const int tiles = (keys + PA_KT - 1) / PA_KT, each = split_tiles(p);
+  return max(1, min(p.splits, (tiles + each - 1) / each));
 }
 
 // ---------------------------------------------------------------- one wave's part of a tile
@@ -462,8 +493,24 @@ template <bool ROPE> struct PackedStages {
   }
 };
 
-// ROPE: 64 more key columns beside the first 128.  One workgroup of four waves per head and block of 256 queries.
-template <bool ROPE>
+// A group's sums times inv as rows of 256 bytes in LDS (the lane's at turn): chunk ch of a row at ch ^ (row & 15)
+template <bool F16> AMLA_DEV void pa_turn_rows(uint8_t *turn, const f32x16 (&o)[4], float inv, bool none) {
+  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = none ? 0.f : o[cb][4 * q4 + i] * inv;  // (no key seen: what the products left does not count)
+      *reinterpret_cast<u32x2 *>(turn + 16 * ((4 * cb + q4) ^ (j32 & 15)) + 8 * hh) =
+          F16 ? u32x2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])} : u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    }
+}
+
+// ROPE: 64 more key columns beside the first 128.  One workgroup of four waves per head, block of 256 queries and split.
+// SPLIT: calls of one split a block keep a shorter kernel (1 % of five prompts of 4099 rows, 352 us after 355 on one card).
+template <bool ROPE, bool SPLIT>
 __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
   extern __shared__ __align__(1024) uint8_t sm[];
   using W = PackedWave<ROPE>;
@@ -471,14 +518,23 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
   const int j32 = lane & 31, hh = lane >> 5;
 
   // workgroup i runs on XCD i % 8: a head's blocks, and heads that share keys, come from the same L2 where heads divide
-  const int i = blockIdx.x % p.heads;
+  const int i = blockIdx.x % p.heads, unit = blockIdx.x / p.heads;
   const int h = p.heads % 8 ? i : (i & 7) * (p.heads >> 3) + (i >> 3);
-  const PackedBlock blk = find_block(p, blockIdx.x / p.heads);
+  const int tile0 = SPLIT ? unit / p.splits : unit, split = SPLIT ? unit % p.splits : 0;
+  const PackedBlock blk = find_block(p, tile0);
   if (blk.block < 0) return;
-  const int q0 = blk.q0, nq = blk.nq, nk = blk.nk;
-  const int64_t k0 = blk.k0;
+  int splits = 1, first_key = 0, last_key = blk.nk;
+  if constexpr (SPLIT) {  // the split's keys: as a sequence that begins and ends with them
+    const int keys = block_keys(p, blk), all = (keys + PA_KT - 1) / PA_KT;
+    splits = block_splits(p, keys);
+    if (split >= splits) return;
+    first_key = (int)((int64_t)split * all / splits) * PA_KT;
+    if (splits > 1) last_key = min(blk.nk, (int)((int64_t)(split + 1) * all / splits) * PA_KT);
+  }
+  const int q0 = blk.q0, nq = blk.nq, nk = last_key - first_key;
+  const int64_t k0 = blk.k0 + first_key;
   const int s_begin = blk.block * PA_QB, s_wave = s_begin + 64 * wave;
-  const int past = nk - nq;  // keys before the first query's own (causal)
+  const int past = blk.nk - nq - first_key;  // keys before the first query's own (causal)
   const int klim = p.causal ? min(nk, max(past + min(s_begin + PA_QB, nq), 0)) : nk;  // keys that the block needs
   const int ntiles = (klim + PA_KT - 1) / PA_KT;
   // keys that the wave's first query sees, and its last one
@@ -596,24 +652,46 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
 
   // outputs: rows of 256 bytes through LDS (chunk ch of a row at ch ^ (row & 15)), so that a store is whole rows
   uint8_t *turn = sm + wave * 64 * 256;
+  const size_t slot = ((size_t)tile0 * p.heads + h) * p.splits + split;
+  const bool part = SPLIT && splits > 1;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     float l = w.l[g];
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float inv = l == 0.f ? 0.f : 1.f / l;
     const int r = 32 * g + j32;
-    if (p.lse && hh == 0 && s_wave + r < nq)
-      p.lse[(size_t)(q0 + s_wave + r) * p.heads + h] =
-          l == 0.f ? -INFINITY : (w.m[g] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    const float lse2 = l == 0.f ? -INFINITY : w.m[g] + __builtin_amdgcn_logf(l);
+    if (part) {  // the row's largest value to 2^14 .. 2^15
+      float top = 0.f;
 #pragma unroll
-    for (int cb = 0; cb < 4; ++cb)
+      for (int cb = 0; cb < 4; ++cb)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<u32x2 *>(turn + r * 256 + 16 * ((4 * cb + q4) ^ (j32 & 15)) + 8 * hh) =
-            l == 0.f ? u32x2{0, 0}  // (no key seen: what the products left does not count)
-                     : u32x2{pack_bf16(w.o[g][cb][4 * q4] * inv, w.o[g][cb][4 * q4 + 1] * inv),
-                             pack_bf16(w.o[g][cb][4 * q4 + 2] * inv, w.o[g][cb][4 * q4 + 3] * inv)};
+        for (int k = 0; k < 16; ++k) top = __builtin_fmaxf(top, __builtin_fabsf(w.o[g][cb][k]));
+      if (__ballot(top == INFINITY)) {  // of the finite ones
+        top = 0.f;
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float x = __builtin_fabsf(w.o[g][cb][k]);
+            top = x < INFINITY ? __builtin_fmaxf(top, x) : top;
+          }
+      }
+      const auto sx = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = __builtin_fmaxf(__uint_as_float(sx[0]), __uint_as_float(sx[1])) * inv;
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 240) - 14;
+      inv *= __uint_as_float((uint32_t)(254 - e) << 23);
+      if (hh == 0) {
+        float *ls = p.part_ls + 2 * (slot * PA_QB + 64 * wave + r);
+        ls[0] = lse2;
+        ls[1] = __uint_as_float((uint32_t)e << 23);
+      }
+      pa_turn_rows<true>(turn + r * 256, w.o[g], inv, l == 0.f);
+    } else {
+      if (p.lse && hh == 0 && s_wave + r < nq) p.lse[(size_t)(q0 + s_wave + r) * p.heads + h] = lse2 * 0.6931471805599453f;
+      pa_turn_rows<false>(turn + r * 256, w.o[g], inv, l == 0.f);
+    }
   }
   const int held = min(64, nq - s_wave);
   if (__builtin_amdgcn_readfirstlane((int)odd)) {  // infinities and NaN enter the outputs of the queries that see them
@@ -623,32 +701,99 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
       if (!__ballot(lo || hi)) continue;
       for (int r = p.causal ? max(key - past - s_wave, 0) : 0; r < held; ++r) {
         uint32_t *at = reinterpret_cast<uint32_t *>(turn + r * 256 + 16 * ((lane >> 2) ^ (r & 15)) + 4 * (lane & 3));
-        const float a = lo_bf(*at), b = hi_bf(*at);
-        *at = pack_bf16(lo ? a + lo_bf(x) : a, hi ? b + hi_bf(x) : b);
+        const uint32_t y = *at;
+        const float a = part ? lo_f16(y) : lo_bf(y), b = part ? hi_f16(y) : hi_bf(y);
+        const float c0 = lo ? a + lo_bf(x) : a, c1 = hi ? b + hi_bf(x) : b;
+        *at = part ? pack_f16(c0, c1) : pack_bf16(c0, c1);
       }
     }
+  }
+  uint16_t *od = p.out + ((size_t)(q0 + s_wave) * p.heads + h) * PA_VD;
+  size_t ld = (size_t)p.heads * PA_VD;
+  if (part) {
+    od = p.part_o + (slot * PA_QB + 64 * wave) * PA_VD;
+    ld = PA_VD;
   }
 #pragma unroll 4
   for (int r0 = 0; r0 < 64; r0 += 4) {
     const int r = r0 + (lane >> 4), ch = lane & 15;
     if (r < held)
-      *reinterpret_cast<u32x4 *>(p.out + ((size_t)(q0 + s_wave + r) * p.heads + h) * PA_VD + 8 * ch) =
-          *reinterpret_cast<const u32x4 *>(turn + r * 256 + 16 * (ch ^ (r & 15)));
+      *reinterpret_cast<u32x4 *>(od + r * ld + 8 * ch) = *reinterpret_cast<const u32x4 *>(turn + r * 256 + 16 * (ch ^ (r & 15)));
   }
 }
 
-template <bool ROPE>
+// Joins the splits of 32 rows of a block: sum_j 2^(lse_j - max) O_j / sum_j 2^(lse_j - max), 16 lanes a row, in split order.
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
+  const int h = blockIdx.x % p.heads, tile0 = blockIdx.x / p.heads;
+  const PackedBlock blk = find_block(p, tile0);
+  if (blk.block < 0) return;
+  const int splits = block_splits(p, block_keys(p, blk));
+  if (splits == 1) return;
+  const size_t slot = ((size_t)tile0 * p.heads + h) * p.splits;
+  const int ch = threadIdx.x & 15;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = 32 * blockIdx.y + 16 * k + (threadIdx.x >> 4), row = blk.block * PA_QB + r;
+    if (row >= blk.nq) continue;
+    const float *ls = p.part_ls + 2 * (slot * PA_QB + r);
+    const uint16_t *po = p.part_o + (slot * PA_QB + r) * PA_VD + 8 * ch;
+    float top = -INFINITY;
+    for (int j = 0; j < splits; ++j) top = __builtin_fmaxf(top, ls[(size_t)j * 2 * PA_QB]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float total = 0.f, a[8] = {};
+#pragma unroll 4
+    for (int j = 0; j < splits; ++j) {
+      const f32x2 l = *reinterpret_cast<const f32x2 *>(ls + (size_t)j * 2 * PA_QB);
+      const u32x4 v = ldg16(po + (size_t)j * PA_QB * PA_VD);
+      const float f = __builtin_amdgcn_exp2f(l.x - ref);
+      total += f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = v[e];
+        a[2 * e] = __builtin_fmaf(f, lo_f16(x) * l.y, a[2 * e]);
+        a[2 * e + 1] = __builtin_fmaf(f, hi_f16(x) * l.y, a[2 * e + 1]);
+      }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const size_t at = (size_t)(blk.q0 + row) * p.heads + h;
+    *reinterpret_cast<u32x4 *>(p.out + at * PA_VD + 8 * ch) =
+        u32x4{pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv), pack_bf16(a[4] * inv, a[5] * inv),
+              pack_bf16(a[6] * inv, a[7] * inv)};
+    if (ch == 0 && p.lse) p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+  }
+}
+
+template <bool ROPE, bool SPLIT>
 static int launch_packed(const PackedParams &p, int64_t blocks, hipStream_t st) {
   constexpr int lds = PackedWave<ROPE>::STAGE * PA_NST;
-  const int rc = latent_lds(packed_attn_kernel<ROPE>, "packed_attention");
+  const int rc = latent_lds(packed_attn_kernel<ROPE, SPLIT>, "packed_attention");
   if (rc) return rc;
-  packed_attn_kernel<ROPE><<<dim3((unsigned)blocks), 256, lds, st>>>(p);
-  return check_launch("packed_attention");
+  packed_attn_kernel<ROPE, SPLIT><<<dim3((unsigned)blocks * p.splits), 256, lds, st>>>(p);
+  const int err = check_launch("packed_attention");
+  if (err || !SPLIT) return err;
+  packed_join_kernel<<<dim3((unsigned)blocks, PA_QB / 32), 256, 0, st>>>(p);
+  return check_launch("packed_attention join");
+}
+
+// Query blocks of a call, at least those there are
+static int64_t packed_blocks(int64_t q_rows, int64_t seqs) { return q_rows / PA_QB + std::min(seqs, q_rows); }
+// Splits of a block, at most: where blocks times heads leave half of the CUs idle.  One or 64 rows of 16 heads behind 4000
+// keys: 111 -> 28 and 114 -> 36 us, 1000 rows 150 -> 94, 16 rows of 128 heads 113 -> 69, 4000 rows of 8 heads 105 -> 78.
+// With 256 blocks and heads nothing was won (4000 rows of 16 heads: 121, 124 split), few keys only pay for the join.
+static int packed_splits(int64_t units, int64_t k_rows) {
+  return units > 128 || k_rows <= PA_LEAST * PA_KT ? 1 : (int)std::min<int64_t>(32, 512 / units);
 }
 
 }  // namespace amla
 
 using namespace amla;
+
+extern "C" size_t amla_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t seqs, int64_t heads) {
+  if (q_rows <= 0 || k_rows < 0 || seqs <= 0 || heads <= 0 || q_rows > INT32_MAX || seqs > AMLA_MAX_SEQS || heads > INT32_MAX) return 0;
+  const int64_t units = packed_blocks(q_rows, seqs) * heads;
+  const int splits = packed_splits(units, k_rows);
+  return splits == 1 ? 0 : (size_t)units * splits * PA_QB * (PA_VD * 2 + 8);
+}
 
 extern "C" int amla_packed_attention(const amla_packed_args *a, void *stream) {
   const char *what = "packed_attention";
@@ -669,9 +814,15 @@ extern "C" int amla_packed_attention(const amla_packed_args *a, void *stream) {
     if (ld % 8 || ld < 0 || ld > (1 << 27)) return fail(AMLA_EUNSUPPORTED, "%s: strides must be multiples of 8 values up to 2^27", what);
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_pe) || !aligned16(a->out))
     return fail(AMLA_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", what);
-  const int64_t tiles = a->q_rows / PA_QB + std::min(a->seqs, a->q_rows);  // at least the blocks there are
+  const int64_t tiles = packed_blocks(a->q_rows, a->seqs);
   if (tiles * a->heads > (1 << 23)) return fail(AMLA_EUNSUPPORTED, "%s: too many query blocks", what);
+  const size_t need = amla_packed_attention_workspace_bytes(a->q_rows, a->k_rows, a->seqs, a->heads);
+  if (need && (!a->workspace || a->workspace_bytes < need)) return fail(AMLA_EWORKSPACE, "%s: workspace too small", what);
+  if (need && !aligned16(a->workspace)) return fail(AMLA_EUNSUPPORTED, "%s: workspace must be 16-byte aligned", what);
   PackedParams p = {};
+  p.splits = packed_splits(tiles * a->heads, a->k_rows);
+  p.part_o = static_cast<uint16_t *>(a->workspace);
+  p.part_ls = reinterpret_cast<float *>(p.part_o + (size_t)tiles * a->heads * p.splits * PA_QB * PA_VD);
   p.q = static_cast<const uint16_t *>(a->q); p.k = static_cast<const uint16_t *>(a->k);
   p.v = static_cast<const uint16_t *>(a->v); p.k_pe = static_cast<const uint16_t *>(a->k_pe);
   p.out = static_cast<uint16_t *>(a->out); p.lse = a->lse;
@@ -682,5 +833,7 @@ extern "C" int amla_packed_attention(const amla_packed_args *a, void *stream) {
   p.ldv = a->ldv; p.ldv_head = a->ldv_head; p.ld_pe = a->ld_pe;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return a->dn == 192 || a->k_pe ? launch_packed<true>(p, tiles * a->heads, st) : launch_packed<false>(p, tiles * a->heads, st);
+  const int64_t blocks = tiles * a->heads;
+  if (a->dn == 192 || a->k_pe) return p.splits > 1 ? launch_packed<true, true>(p, blocks, st) : launch_packed<true, false>(p, blocks, st);
+  return p.splits > 1 ? launch_packed<false, true>(p, blocks, st) : launch_packed<false, false>(p, blocks, st);
 }

@@ -447,7 +447,11 @@ typedef struct amla_packed_args {
   int64_t ldq, ldq_head, ldk, ldk_head, ldv, ldv_head, ld_pe;
   int32_t heads, kv_heads, dn, causal;
   float scale;
+  void *workspace;                     /* 16-byte aligned scratch of the size below; NULL where that is 0 */
+  size_t workspace_bytes;
 } amla_packed_args;
+/* 0 where nothing is split: few blocks of queries have their keys split over workgroups, whose sums meet in the workspace. */
+size_t amla_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t seqs, int64_t heads);
 int amla_packed_attention(const amla_packed_args *args, void *stream);
 
 /* ---- output head ---- */

@@ -55,6 +55,44 @@ def test_not_causal_and_unlike_lengths(form):
     _run(*_case(5, [9, 4], [0, 3], 4, 2, form), causal=False, what=f"{form} no keys")
 
 
+@pytest.mark.parametrize("new,past,H,G,form", [([1], [3001], 3, 1, "plain"), ([40, 3], [2500, 700], 16, 16, "mla"), ([300], [1500], 6, 3, "whole"),
+                                              ([1, 0, 7], [255, 900, 4096], 8, 2, "mla"), ([1100], [0], 2, 2, "plain")])
+def test_few_blocks_split_their_keys(new, past, H, G, form):
+    lens = [a + b for a, b in zip(new, past)]
+    _run(*_case(41 + H, new, lens, H, G, form), what=f"{form} split {new} behind {past}")
+    _run(*_case(42 + H, new, lens, H, G, form), causal=False, what=f"{form} split, not causal")
+
+
+def test_split_keys_that_keep_rising_and_a_captured_call():
+    q, k, v, pe, off, koff, scale = _case(43, [5], [2000], 4, 2, "plain")
+    k[:] = 0
+    k[:, :, 0] = torch.linspace(0, 2000, 2000)[:, None].to(BF16)
+    q[:, :, 0] = 4.0
+    _run(q, k, v, pe, off, koff, scale, what="split, rising")
+    _run(q, k.flip(0), v, pe, off, koff, scale, what="split, falling")
+    d = [to_dev(t) for t in (q, k, v, off, koff)]
+    run = lambda: ops.packed_attention(d[0], d[1], d[2], d[3], scale, k_offsets=d[4], return_lse=True)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for keys in (2000, 300, 5, 1999):
+        d[4].copy_(_offsets([keys]))
+        want = run()
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1]), keys
+
+
 def test_many_sequences_and_blocks_of_queries():
     new = [(13 * i) % 40 for i in range(90)]
     _run(*_case(6, new, new, 2, 1, "plain"), what="90 sequences")
@@ -71,7 +109,8 @@ def test_scores_that_keep_rising():
     _run(q, k.flip(0), v, pe, off, koff, scale, causal=False, what="falling")
 
 
-@pytest.mark.parametrize("new,past,H,G,form", [([40], [0], 2, 1, "plain"), ([300, 70], [0, 90], 4, 4, "mla"), ([513], [100], 2, 2, "whole")])
+@pytest.mark.parametrize("new,past,H,G,form", [([40], [0], 2, 1, "plain"), ([300, 70], [0, 90], 4, 4, "mla"), ([513], [100], 2, 2, "whole"),
+                                              ([300, 70], [0, 90], 130, 130, "plain"), ([20], [1500], 2, 1, "mla")])
 def test_what_a_query_does_not_see_does_not_reach_it(new, past, H, G, form):
     """Infinities and NaN in a later key and in its values: the queries before it keep their bits, and the others the bits
     of every column without one."""

@@ -42,7 +42,7 @@ def _attend(L, c=None, q=P, seqs=2, S=1, H=16, ld=(16 * 576, 16 * 576, 576), len
 def _packed(L, **kw):
     a = dict(q=P, k=P, v=P, k_pe=None, out=P, lse=None, offsets=P, k_offsets=None, q_rows=10, k_rows=10, seqs=2, ldq=512,
              ldq_head=128, ldk=512, ldk_head=128, ldv=512, ldv_head=128, ld_pe=64, heads=4, kv_heads=4, dn=128, causal=1,
-             scale=0.1)
+             scale=0.1, workspace=P, workspace_bytes=BIG)
     a.update(kw)
     return L.amla_packed_attention(_lib.PackedArgs(*[a[f] for f, _ in _lib.PackedArgs._fields_]), None)
 
@@ -99,6 +99,13 @@ def test_packed(L):
                 dict(q=P + 8), dict(v=P + 8), dict(k_pe=P + 8), dict(seqs=65536), dict(k_rows=2 ** 31),
                 dict(q_rows=2 ** 31 - 1, heads=4)):
         assert _packed(L, **bad) == EUNSUPPORTED, bad
+    bytes_of = L.amla_packed_attention_workspace_bytes
+    need = bytes_of(10, 9000, 2, 4)
+    assert need > 0 and _packed(L, k_rows=9000, workspace_bytes=need - 1) == EWORKSPACE
+    assert _packed(L, k_rows=9000, workspace=None) == EWORKSPACE
+    assert _packed(L, k_rows=9000, workspace=P + 8) == EUNSUPPORTED
+    assert bytes_of(100000, 100000, 2, 128) == bytes_of(10, 10, 2, 4) == 0  # enough blocks, or few keys: nothing is split
+    assert bytes_of(0, 9000, 1, 1) == bytes_of(1, 9000, 1, 0) == bytes_of(1, -1, 1, 1) == 0
 
 
 @pytest.mark.parametrize("struct,name", [(_lib.LatentCache, "amla_latent_cache"), (_lib.PackedArgs, "amla_packed_args")])
