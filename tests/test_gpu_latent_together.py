@@ -247,3 +247,29 @@ def test_no_sequences_and_no_pages():
     q = torch.ones(2, 1, H, 576, dtype=BF16, device=DEV)
     o, lse = ops.latent_attention(q, s.cache, bare, two + 9, SCALE, return_lse=True)
     assert not o.any() and (lse == float("-inf")).all()
+
+
+@pytest.mark.parametrize("dtype", [FP8, BF16])
+def test_traced_and_in_inference_mode(dtype):
+    """A step that is compiled, with its writes as side effects, and one under inference mode give the eager step's bits."""
+    lens = [50, 9]
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def step(s, kv, q, n):
+        ops.latent_cache_write(kv, s.gamma, s.freqs, s.cache, s.dt, n)
+        return ops.latent_attention(q, s.cache, s.dt, n + 1, SCALE, return_lse=True)
+
+    def fresh():
+        s = _Server(9, dtype, lens, room=4)
+        ops.latent_cache_write(s.rows(sum(lens)), s.gamma, s.freqs, s.cache, s.dt, torch.zeros_like(n), offsets=_offsets(lens).to(DEV))
+        return s, s.rows(2, 1), (0.5 * torch.randn(2, 1, H, 576, generator=s.g)).to(BF16).to(DEV)
+
+    print(f"[case] {dtype} traced", flush=True)
+    s, kv, q = fresh()
+    want = step(s, kv, q, n)
+    for run in (torch.compile(step, backend="aot_eager"), torch.inference_mode()(step)):
+        t, kv, q = fresh()
+        got = run(t, kv, q, n)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for a, b in zip(s.cache, t.cache):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
