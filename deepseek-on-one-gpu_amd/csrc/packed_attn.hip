@@ -30,7 +30,6 @@ struct PackedParams {
   float *lse;
   const int32_t *offsets, *k_offsets;
   int q_rows, k_rows, seqs, heads, group, causal;
-  int tiles;                         // query blocks of all sequences, at most
   int splits;                        // workgroups of a block, at most
   int64_t ldq, ldq_head, ldk, ldk_head, ldv, ldv_head, ld_pe;
   float scale_log2;
@@ -635,7 +634,14 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
         for (int r = 0; r < 16; ++r) none[g] = __builtin_fmaf(w.o[g][cb][r], 0.f, none[g]);
     // the waves agree: their copies and barriers are common
     const bool low = __ballot(low0 || low1) != 0;
-    const bool strange = __ballot((w.l[0] != 0.f && none[0] != 0.f) || (w.l[1] != 0.f && none[1] != 0.f)) != 0;
+    // of queries that see a key: by either lane's keys, the other one may have the column
+    float seen[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(w.l[g]), __float_as_uint(w.l[g]), false, false);
+      seen[g] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    }
+    const bool strange = __ballot((seen[0] != 0.f && none[0] != 0.f) || (seen[1] != 0.f && none[1] != 0.f)) != 0;
     __syncthreads();
     uint32_t *vote = reinterpret_cast<uint32_t *>(sm);
     if (lane == 0) vote[wave] = (low ? 1 : 0) | (odd ? 2 : 0) | (strange ? 4 : 0);
@@ -828,7 +834,7 @@ extern "C" int amla_packed_attention(const amla_packed_args *a, void *stream) {
   p.out = static_cast<uint16_t *>(a->out); p.lse = a->lse;
   p.offsets = a->offsets; p.k_offsets = a->k_offsets ? a->k_offsets : a->offsets;
   p.q_rows = (int)a->q_rows; p.k_rows = (int)a->k_rows; p.seqs = (int)a->seqs;
-  p.heads = a->heads; p.group = a->heads / a->kv_heads; p.causal = a->causal != 0; p.tiles = (int)tiles;
+  p.heads = a->heads; p.group = a->heads / a->kv_heads; p.causal = a->causal != 0;
   p.ldq = a->ldq; p.ldq_head = a->ldq_head; p.ldk = a->ldk; p.ldk_head = a->ldk_head;
   p.ldv = a->ldv; p.ldv_head = a->ldv_head; p.ld_pe = a->ld_pe;
   p.scale_log2 = a->scale * 1.4426950408889634f;

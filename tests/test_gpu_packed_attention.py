@@ -139,6 +139,20 @@ def test_what_a_query_does_not_see_does_not_reach_it(new, past, H, G, form):
             assert torch.equal(got[~sees], want[~sees]) and torch.isnan(got[sees]).all(), (b, first)
 
 
+@pytest.mark.parametrize("col", [3, 77])
+def test_a_masked_nan_in_a_column_that_another_lane_holds(col):
+    """A lane holds every other four keys of its query, and other columns than theirs: three queries, all keys in one lane."""
+    q, k, v, pe, off, koff, scale = _case(22, [3], [3], 2, 2, "plain")
+    run = lambda v: ops.packed_attention(to_dev(q), to_dev(k), to_dev(v), to_dev(off), scale)  # noqa: E731
+    print(f"[case] column {col}", flush=True)
+    want = run(v)
+    v2 = v.clone()
+    v2[2, :, col] = float("nan")
+    got = run(v2)
+    rest = [c for c in range(128) if c != col]
+    assert torch.equal(got[:2], want[:2]) and torch.equal(got[..., rest], want[..., rest]) and torch.isnan(got[2, :, col]).all()
+
+
 def test_strides_alignment_and_no_lse():
     q, k, v, pe, off, koff, scale = _case(9, [50, 20], [50, 20], 4, 4, "mla")
     want, _ = _run(q, k, v, pe, off, koff, scale, what="views of kv_b")
