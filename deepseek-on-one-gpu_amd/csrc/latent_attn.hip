@@ -33,6 +33,7 @@ struct LatentAttnParams {
   // much error as the output's own; fp32 would be twice the bytes, a tenth of a long batch's time.
   uint16_t *part_o;
   float *part_lse, *part_scale;    // (slots, rows of a chunk), (slots, rows of a chunk, 4)
+  int2 *part_plan;                 // (first slot, splits) of each sequence that has rows: the join need not plan again
 };
 
 AMLA_DEV int lc_ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -103,13 +104,6 @@ struct SplitPlan {
       base += __builtin_amdgcn_readlane(incl, 63);
     }
     return int3{-1, 0, 0};
-  }
-  // (first slot, splits) of sequence b
-  AMLA_DEV int2 of(int b) const {
-    int before = 0;
-    for (int i = threadIdx.x & 63; i < b; i += 64) before += lc_ceil_div(tiles(i), len);
-    return int2{__builtin_amdgcn_readfirstlane(wave_isum(before)) * p.chunks,
-                __builtin_amdgcn_readfirstlane(lc_ceil_div(tiles(b), len))};
   }
 };
 
@@ -801,6 +795,7 @@ template <bool F8> AMLA_DEV SplitWork split_work(const LatentAttnParams &p) {
   const int per_xcd = lc_ceil_div(plan.used(plan.len), 8), slot = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
   const int3 at = plan.find(slot);
   if ((int)(blockIdx.x >> 3) >= per_xcd || at.x < 0) return SplitWork{-1, 0, 0, 0, 0, 0, 0};
+  if (slot == at.y && threadIdx.x == 0) p.part_plan[at.x] = int2{at.y, at.z};
   const int split = (slot - at.y) % at.z, held = __builtin_amdgcn_readfirstlane(min(max(p.lengths[at.x], 0), p.cap));
   const int n_tiles = lc_ceil_div(held, TILE);
   return SplitWork{at.x, (slot - at.y) / at.z, slot, at.z, held, (int)((int64_t)split * n_tiles / at.z),
@@ -1261,9 +1256,9 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
   __shared__ float part[3][64][9];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y, row = blockIdx.x;
-  const SplitPlan<Tile<F8>::ROWS> plan(p);
-  const int2 at = plan.of(b);
-  const int n = at.y;
+  const int held = min(max(p.lengths[b], 0), p.cap);
+  const int2 at = held ? p.part_plan[b] : int2{0, 0};
+  const int n = __builtin_amdgcn_readfirstlane(at.y);
   if (n == 1) return;
   const size_t dst = (size_t)b * p.rows + row;
   u32x4 *od = reinterpret_cast<u32x4 *>(p.out + dst * LC_LORA) + lane;
@@ -1377,7 +1372,7 @@ size_t amla_latent_attention_workspace_bytes(int64_t seqs, int64_t seq_len, int6
   if (seqs <= 0 || seq_len <= 0 || heads <= 0 || seqs > AMLA_MAX_SEQS || seq_len > INT32_MAX || heads > INT32_MAX / seq_len)
     return 0;
   const AttnSizes s = attn_sizes(seqs, seq_len * heads, max_rows);
-  return (size_t)s.slots * 32 * s.hg * (LC_LORA * 2 + 4 + 16);
+  return (size_t)s.slots * 32 * s.hg * (LC_LORA * 2 + 4 + 16) + (size_t)seqs * 8;
 }
 
 int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t seqs, int64_t seq_len, int64_t heads,
@@ -1413,6 +1408,7 @@ int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t
   p.part_o = static_cast<uint16_t *>(workspace);
   p.part_lse = reinterpret_cast<float *>(p.part_o + (size_t)s.slots * 32 * s.hg * LC_LORA);
   p.part_scale = p.part_lse + (size_t)s.slots * 32 * s.hg;
+  p.part_plan = reinterpret_cast<int2 *>(p.part_scale + (size_t)s.slots * 32 * s.hg * 4);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (p.pg.scales) {
     if (s.hg == 4) return launch_attn<true, 4>(p, st);
