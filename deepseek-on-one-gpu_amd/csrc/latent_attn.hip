@@ -166,18 +166,20 @@ template <typename T, typename... R> AMLA_DEV void lds_tie(T &v, R &...rest) {
   if constexpr (sizeof...(rest) > 0) lds_tie(rest...);
 }
 
-// Scores accumulate in vector registers (inline asm): the accumulator registers hold the outputs.  The
-// wait states cover a conversion that wrote the A operand just before.
-AMLA_DEV void mfma_score(f32x16 &c, bf16x8 a, bf16x8 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+// Scores accumulate in vector registers (inline asm): the accumulator registers hold the outputs.  WAIT: an operand may have
+// been written just before, which takes two wait states (8 cycles); where none can be, the test of the assembly holds it to that.
+template <bool WAIT> AMLA_DEV void mfma_score(f32x16 &c, bf16x8 a, bf16x8 b) {
+  if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
-AMLA_DEV void mfma_score0(f32x16 &c, bf16x8 a, bf16x8 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+template <bool WAIT> AMLA_DEV void mfma_score0(f32x16 &c, bf16x8 a, bf16x8 b) {
+  if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
 }
-// Outputs accumulate in accumulator registers that nothing else reads inside the loop.  The wait states
-// cover moves of the operands just before; settle() covers what follows outside the loop.
-AMLA_DEV void mfma_value(f32x16 &c, bf16x8 a, bf16x8 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+// Outputs accumulate in accumulator registers that nothing else reads inside the loop; settle() covers what follows outside it.
+template <bool WAIT> AMLA_DEV void mfma_value(f32x16 &c, bf16x8 a, bf16x8 b) {
+  if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 AMLA_DEV i32x8 join(u32x2 a, u32x2 b, u32x2 c, u32x2 d) {
   return i32x8{(int)a.x, (int)a.y, (int)b.x, (int)b.y, (int)c.x, (int)c.y, (int)d.x, (int)d.y};
@@ -185,9 +187,13 @@ AMLA_DEV i32x8 join(u32x2 a, u32x2 b, u32x2 c, u32x2 d) {
 // A (32 x 64) B (64 x 32) of e4m3 codes, lane l holding 32 codes of row (column) l % 32, B times
 // 2^(byte - 127) of the low byte of its scale: codes 0 - 15 of both lanes of a column are one block, scaled
 // by the byte of lane l % 32, codes 16 - 31 the other, by that of lane l % 32 + 32.  one: 127.
-AMLA_DEV void mfma_value(f32x16 &c, i32x8 a, int one, i32x8 b, int bs) {
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
-               : "+a"(c) : "v"(a), "v"(b), "v"(one), "v"(bs));
+template <bool WAIT> AMLA_DEV void mfma_value(f32x16 &c, i32x8 a, int one, i32x8 b, int bs) {
+  if constexpr (WAIT)
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "+a"(c) : "v"(a), "v"(b), "v"(one), "v"(bs));
+  else
+    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "+a"(c) : "v"(a), "v"(b), "v"(one), "v"(bs));
 }
 // Before vector code reads what the asm MFMAs above wrote, and before they read what it wrote.
 template <int N> AMLA_DEV void settle(f32x16 (&o)[N]) {
@@ -337,53 +343,61 @@ template <bool F8, int N, int I = 0> AMLA_DEV void score_reads_first(u32x4 (*ka)
   }
 }
 
-// x0: e4m3: the step's first fragment, converted in the step before (a conversion of four instructions fits
-// under each MFMA; all sixteen of a step in front of its four MFMAs cost 5900 cycles a tile, not 3900)
+// x0, y0: the step's first fragments; e4m3: converted in the step before (a conversion of four instructions fits under each
+// MFMA; all sixteen of a step in front of its four MFMAs cost 5900 cycles a tile, not 3900, and one right before the product
+// that takes it two wait states each time)
 template <bool F8, int HG, int I>
-AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, float f0,
-                         float f1, uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
+AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, bf16x8 y0,
+                         float f0, float f1, uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
   constexpr int N = 16 + (F8 ? 4 : 2);  // steps over the latent and the rope key
   if constexpr (I < N) {
-    constexpr int AHEAD = score_ahead<F8, HG>(), c = I % (AHEAD + 1);
+    constexpr int AHEAD = score_ahead<F8, HG>(), c = I % (AHEAD + 1), n = (I + 1) % (AHEAD + 1);
+    constexpr bool WAIT = HG < 4;  // (with fewer outputs some queries sit in accumulator registers, and are moved)
     if constexpr (I + AHEAD < N) score_read<F8, I + AHEAD>(ka[(I + AHEAD) % (AHEAD + 1)], kl, kr, w.qra);
     constexpr int r0q = q_reg<F8>(I < 16 ? 2 * I : 0), r1q = q_reg<F8>(I < 16 ? 2 * I + 1 : 0);
     const bf16x8 qa = w.q[r0q], qb = score_reads<F8>(I) == 3 ? as_bf16x8(ka[c][2]) : w.q[r1q];
-    bf16x8 xn = x0;
+    bf16x8 xn = x0, yn = y0;
     if constexpr (I >= 16) {
       constexpr int k0 = F8 ? I - 16 : 2 * (I - 16), k1 = F8 ? k0 : k0 + 1;
-      mfma_score(w.s[0], as_bf16x8(ka[c][0]), F8 ? qb : w.qr[F8 ? 0 : k0]);
-      mfma_score(w.s[1], as_bf16x8(ka[c][1]), F8 ? qb : w.qr[F8 ? 0 : k1]);
+      mfma_score<WAIT>(w.s[0], x0, F8 ? qb : w.qr[F8 ? 0 : k0]);
+      mfma_score<WAIT>(w.s[1], y0, F8 ? qb : w.qr[F8 ? 0 : k1]);
     } else if constexpr (F8) {
       const u32x4 x = ka[c][0], y = ka[c][1];
-      if constexpr (I == 0) mfma_score0(w.s[0], x0, qa);
-      else mfma_score(w.s[0], x0, qa);
-      const bf16x8 y0 = codes_to_bf16(y.x, y.y, f1);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (I == 0) mfma_score0(w.s[1], y0, qa);
-      else mfma_score(w.s[1], y0, qa);
+      if constexpr (I == 0) mfma_score0<true>(w.s[0], x0, qa);
+      else mfma_score<WAIT>(w.s[0], x0, qa);
       const bf16x8 x1 = codes_to_bf16(x.z, x.w, f0);
       __builtin_amdgcn_sched_barrier(0);
-      mfma_score(w.s[0], x1, qb);
+      if constexpr (I == 0) mfma_score0<true>(w.s[1], y0, qa);
+      else mfma_score<WAIT>(w.s[1], y0, qa);
       const bf16x8 y1 = codes_to_bf16(y.z, y.w, f1);
       __builtin_amdgcn_sched_barrier(0);
-      mfma_score(w.s[1], y1, qb);
+      mfma_score<WAIT>(w.s[0], x1, qb);
+      if constexpr (I + 1 < N) {
+        lds_wait<score_reads<F8>(I + 2, I + AHEAD)>();
+        lds_tie(ka[n][0], ka[n][1]);
+        if constexpr (score_reads<F8>(I + 1) == 3) lds_tie(ka[n][2]);
+        xn = I + 1 < 16 ? codes_to_bf16(ka[n][0].x, ka[n][0].y, f0) : as_bf16x8(ka[n][0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      mfma_score<WAIT>(w.s[1], y1, qb);
+      if constexpr (I + 1 < N) yn = I + 1 < 16 ? codes_to_bf16(ka[n][1].x, ka[n][1].y, f1) : as_bf16x8(ka[n][1]);
     } else if constexpr (I == 0) {
-      mfma_score0(w.s[0], as_bf16x8(ka[c][0]), qa);
-      mfma_score0(w.s[1], as_bf16x8(ka[c][1]), qb);
+      mfma_score0<true>(w.s[0], x0, qa);
+      mfma_score0<true>(w.s[1], y0, qb);
     } else {
-      mfma_score(w.s[0], as_bf16x8(ka[c][0]), qa);
-      mfma_score(w.s[1], as_bf16x8(ka[c][1]), qb);
+      mfma_score<WAIT>(w.s[0], x0, qa);
+      mfma_score<WAIT>(w.s[1], y0, qb);
     }
     if constexpr (I > 0 && I <= Rows<F8>::COPIES) next.template copy<I - 1>(pg, st_next, r0, lanes);
-    if constexpr (I + 1 < N) {
-      constexpr int n = (I + 1) % (AHEAD + 1);
+    if constexpr (I + 1 < N && (!F8 || I >= 16)) {
       lds_wait<score_reads<F8>(I + 2, I + AHEAD)>();
       lds_tie(ka[n][0], ka[n][1]);
       if constexpr (score_reads<F8>(I + 1) == 3) lds_tie(ka[n][2]);
-      if constexpr (F8 && I + 1 < 16) xn = codes_to_bf16(ka[n][0].x, ka[n][0].y, f0);
+      xn = as_bf16x8(ka[n][0]);
+      yn = as_bf16x8(ka[n][1]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    score_step<F8, HG, I + 1>(w, ka, kl, kr, xn, f0, f1, lanes, next, pg, st_next, r0);
+    score_step<F8, HG, I + 1>(w, ka, kl, kr, xn, yn, f0, f1, lanes, next, pg, st_next, r0);
   }
 }
 
@@ -409,10 +423,9 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
   lds_wait<score_reads<F8>(1, AHEAD - 1)>();
   lds_tie(f0, f1, ka[0][0], ka[0][1]);
   if constexpr (score_reads<F8>(0) == 3) lds_tie(ka[0][2]);
-  bf16x8 x0;
-  if constexpr (F8) x0 = codes_to_bf16(ka[0][0].x, ka[0][0].y, f0);
-  else x0 = as_bf16x8(ka[0][0]);
-  score_step<F8, HG, 0>(w, ka, kl, kr, x0, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
+  const bf16x8 x0 = F8 ? codes_to_bf16(ka[0][0].x, ka[0][0].y, f0) : as_bf16x8(ka[0][0]);
+  const bf16x8 y0 = F8 ? codes_to_bf16(ka[0][1].x, ka[0][1].y, f1) : as_bf16x8(ka[0][1]);
+  score_step<F8, HG, 0>(w, ka, kl, kr, x0, y0, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
   // the results are read by vector code that the compiler schedules: cover the asm's write-to-read wait states
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(w.s[0]), "+v"(w.s[1])::"memory");
 }
@@ -564,11 +577,11 @@ AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
     // apart that are still being loaded)
     u32x2 v0 = r.v[0], v1 = r.v[1], v2 = r.v[2], v3 = r.v[3];
     lds_tie(v0, v1, v2, v3);
-    if constexpr (F8) mfma_value(w.o[C], join(v0, v1, v2, v3), w.one, w.phi, w.ps);
-    else mfma_value(w.o[C], as_bf16x8(u32x4{v0.x, v0.y, v1.x, v1.y}), as_bf16x8(w.pb[0]));
+    if constexpr (F8) mfma_value<false>(w.o[C], join(v0, v1, v2, v3), w.one, w.phi, w.ps);
+    else mfma_value<false>(w.o[C], as_bf16x8(u32x4{v0.x, v0.y, v1.x, v1.y}), as_bf16x8(w.pb[0]));
     if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r);
-    if constexpr (F8) mfma_value(w.o[C], join(v0, v1, v2, v3), w.one, w.plo, w.ps_lo);
-    else mfma_value(w.o[C], as_bf16x8(u32x4{v2.x, v2.y, v3.x, v3.y}), as_bf16x8(w.pb[1]));
+    if constexpr (F8) mfma_value<false>(w.o[C], join(v0, v1, v2, v3), w.one, w.plo, w.ps_lo);
+    else mfma_value<false>(w.o[C], as_bf16x8(u32x4{v2.x, v2.y, v3.x, v3.y}), as_bf16x8(w.pb[1]));
     __builtin_amdgcn_sched_barrier(0);
     value_step<F8, HG, MASK, ZP, C + 1>(w, x);
   }
@@ -1137,11 +1150,11 @@ template <bool F8, int C> AMLA_DEV void few_value_step(FewWave<F8> &w, FewValues
     if constexpr (F8) {
       const i32x8 hi = {(int)x.p[0].x, (int)x.p[0].y, (int)x.p[0].z, (int)x.p[0].w, (int)x.p[1].x, (int)x.p[1].y, (int)x.p[1].z, (int)x.p[1].w};
       const i32x8 lo = {(int)x.p[2].x, (int)x.p[2].y, (int)x.p[2].z, (int)x.p[2].w, (int)x.p[3].x, (int)x.p[3].y, (int)x.p[3].z, (int)x.p[3].w};
-      mfma_value(w.o[C], join(a, b, d, e), 127, hi, x.ps);
-      mfma_value(w.o[C], join(a, b, d, e), 127, lo, x.ps - 4);
+      mfma_value<true>(w.o[C], join(a, b, d, e), 127, hi, x.ps);
+      mfma_value<true>(w.o[C], join(a, b, d, e), 127, lo, x.ps - 4);
     } else {
-      mfma_value(w.o[C], as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), as_bf16x8(x.p[0]));
-      mfma_value(w.o[C], as_bf16x8(u32x4{d.x, d.y, e.x, e.y}), as_bf16x8(x.p[1]));
+      mfma_value<true>(w.o[C], as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), as_bf16x8(x.p[0]));
+      mfma_value<true>(w.o[C], as_bf16x8(u32x4{d.x, d.y, e.x, e.y}), as_bf16x8(x.p[1]));
     }
     few_value_step<F8, C + 1>(w, x, v);
   }
