@@ -4,7 +4,7 @@
 // exact in it), probabilities are rounded once for the matrix units: to bf16, or to two e4m3 halves that hold eight bits
 // of them (inference/ops.py:179 rounds them to bf16).  Every row of the cache serves all heads, so it is read once from
 // memory per 128 query rows and split of the sequence.  Many query rows: latent_attn_kernel, bound by the matrix units
-// (8 x 32768 rows, 128 heads, e4m3: 91 us where 73 GFLOP at a large product's rate take 61; the units are busy 42 % of
+// (8 x 32768 rows, 128 heads, e4m3: 89 us where 73 GFLOP at a large product's rate take 61; the units are busy 42 % of
 // the cycles, conversions, softmax and barriers take the others).  Few: latent_attn_few_kernel, bound by the copies (40
 // ragged sequences, 16 heads, bf16: 64 us for 342 MB; the copies alone take nine tenths).  Then latent_join_kernel.
 #include <algorithm>
