@@ -330,7 +330,7 @@ template <bool F8> constexpr int score_reads(int i) {
 }
 // Steps that reads go out ahead: as many as the registers allow (an LDS read returns after 300 - 400 cycles with
 // four waves reading; two steps of bf16 are 128 cycles of products)
-template <bool F8, int HG> constexpr int score_ahead() { return F8 ? (HG == 4 ? 2 : 4) : (HG == 4 ? 3 : 6); }
+template <bool F8, int HG> constexpr int score_ahead() { return F8 ? 2 : 3; }
 template <bool F8> constexpr int score_reads(int first, int last) {
   int n = 0;
   for (int i = first; i <= last; ++i) n += score_reads<F8>(i);
@@ -352,26 +352,25 @@ AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1]
   constexpr int N = 16 + (F8 ? 4 : 2);  // steps over the latent and the rope key
   if constexpr (I < N) {
     constexpr int AHEAD = score_ahead<F8, HG>(), c = I % (AHEAD + 1), n = (I + 1) % (AHEAD + 1);
-    constexpr bool WAIT = HG < 4;  // (with fewer outputs some queries sit in accumulator registers, and are moved)
     if constexpr (I + AHEAD < N) score_read<F8, I + AHEAD>(ka[(I + AHEAD) % (AHEAD + 1)], kl, kr, w.qra);
     constexpr int r0q = q_reg<F8>(I < 16 ? 2 * I : 0), r1q = q_reg<F8>(I < 16 ? 2 * I + 1 : 0);
     const bf16x8 qa = w.q[r0q], qb = score_reads<F8>(I) == 3 ? as_bf16x8(ka[c][2]) : w.q[r1q];
     bf16x8 xn = x0, yn = y0;
     if constexpr (I >= 16) {
       constexpr int k0 = F8 ? I - 16 : 2 * (I - 16), k1 = F8 ? k0 : k0 + 1;
-      mfma_score<WAIT>(w.s[0], x0, F8 ? qb : w.qr[F8 ? 0 : k0]);
-      mfma_score<WAIT>(w.s[1], y0, F8 ? qb : w.qr[F8 ? 0 : k1]);
+      mfma_score<false>(w.s[0], x0, F8 ? qb : w.qr[F8 ? 0 : k0]);
+      mfma_score<false>(w.s[1], y0, F8 ? qb : w.qr[F8 ? 0 : k1]);
     } else if constexpr (F8) {
       const u32x4 x = ka[c][0], y = ka[c][1];
       if constexpr (I == 0) mfma_score0<true>(w.s[0], x0, qa);
-      else mfma_score<WAIT>(w.s[0], x0, qa);
+      else mfma_score<false>(w.s[0], x0, qa);
       const bf16x8 x1 = codes_to_bf16(x.z, x.w, f0);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (I == 0) mfma_score0<true>(w.s[1], y0, qa);
-      else mfma_score<WAIT>(w.s[1], y0, qa);
+      else mfma_score<false>(w.s[1], y0, qa);
       const bf16x8 y1 = codes_to_bf16(y.z, y.w, f1);
       __builtin_amdgcn_sched_barrier(0);
-      mfma_score<WAIT>(w.s[0], x1, qb);
+      mfma_score<false>(w.s[0], x1, qb);
       if constexpr (I + 1 < N) {
         lds_wait<score_reads<F8>(I + 2, I + AHEAD)>();
         lds_tie(ka[n][0], ka[n][1]);
@@ -379,14 +378,14 @@ AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1]
         xn = I + 1 < 16 ? codes_to_bf16(ka[n][0].x, ka[n][0].y, f0) : as_bf16x8(ka[n][0]);
       }
       __builtin_amdgcn_sched_barrier(0);
-      mfma_score<WAIT>(w.s[1], y1, qb);
+      mfma_score<false>(w.s[1], y1, qb);
       if constexpr (I + 1 < N) yn = I + 1 < 16 ? codes_to_bf16(ka[n][1].x, ka[n][1].y, f1) : as_bf16x8(ka[n][1]);
     } else if constexpr (I == 0) {
       mfma_score0<true>(w.s[0], x0, qa);
       mfma_score0<true>(w.s[1], y0, qb);
     } else {
-      mfma_score<WAIT>(w.s[0], x0, qa);
-      mfma_score<WAIT>(w.s[1], y0, qb);
+      mfma_score<false>(w.s[0], x0, qa);
+      mfma_score<false>(w.s[1], y0, qb);
     }
     if constexpr (I > 0 && I <= Rows<F8>::COPIES) next.template copy<I - 1>(pg, st_next, r0, lanes);
     if constexpr (I + 1 < N && (!F8 || I >= 16)) {
@@ -751,11 +750,12 @@ template <bool F16, int NCB> AMLA_DEV void turn_rows(uint8_t *turn, const f32x16
     }
 }
 // A split's sums, normalised: the output itself, or a partial one.  l, m: of the lane's query row.
-template <int HG, int NCB>
+// GROUPS: 32-row groups of a workgroup; hg: this one, cg: the wave's of 16 / NCB column groups.
+template <int GROUPS, int NCB>
 AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB], float l, float m, int b, int chunk, int slot,
-                          int splits, int wave) {
-  constexpr int CG = 4 / HG;
-  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5, hg = wave / CG, cg = wave % CG;
+                          int splits, int wave, int hg, int cg) {
+  constexpr int HG = GROUPS, CG = 16 / NCB;
+  const int lane = threadIdx.x & 63, j32 = lane & 31, hh = lane >> 5;
   const int row = (chunk * HG + hg) * 32 + j32;
   float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse2 = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
@@ -815,9 +815,8 @@ template <bool F8> AMLA_DEV SplitWork split_work(const LatentAttnParams &p) {
                    (int)((int64_t)(split + 1) * n_tiles / at.z)};
 }
 
-// One workgroup of four waves per (sequence, chunk of 32 HG rows, split).  HG (2 or 4) waves hold 32
-// query rows each; the 4 / HG waves of the same rows compute the same scores and
-// accumulate 512 HG / 4 columns each.  O^T fills half of a wave's 512 registers, the queries
+// One workgroup of four waves per (sequence, chunk of 32 HG rows, split), HG = 4: a wave holds 32
+// query rows, all of whose columns it sums up.  O^T fills half of its 512 registers, the queries
 // most of the others: one wave a SIMD, whose own products hide its conversions, copies, LDS
 // reads and softmax, each placed between two of them (one phase after the other took twice
 // as long).  What spills in the loop costs most: a reload waits behind all copies under way.
@@ -910,30 +909,34 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   float l = w.l;
   l += __shfl_xor(l, 32, 64);
   if constexpr (MASK) l = feed.odd < limit + 4 * hh ? __uint_as_float(0x7fc00000u) : l;
-  store_split<HG>(p, sm, w.o, l, w.m, b, chunk, slot, splits, wave);
+  store_split<HG>(p, sm, w.o, l, w.m, b, chunk, slot, splits, wave, hg, cg);
 }
 
 // ---------------------------------------------------------------- few query rows
 //
-// One workgroup per (sequence, 32 query rows, split).  Wave (r, q) scores one half of a tile's rows for 16 of the queries
-// with 16x16x32 products and writes its probabilities to LDS; a tile later, behind the barrier that the tiles have anyway,
-// each wave takes all of them for its 128 columns.  So a tile's keys are read, and e4m3 converted, twice and not once a
-// wave, which is what bounds the kernel above with one group of queries (LDS: 1700 of its cycles a bf16 tile).
-template <bool F8> struct FewStage {
+// One workgroup per (sequence, 32 or 64 query rows, split).  Wave (r, q) scores one half of a tile's rows for half of the
+// queries with 16x16x32 products and writes its probabilities to LDS; a tile later, behind the barrier that the tiles have
+// anyway, each wave takes all of them for its 128 columns.  So a tile's keys are read, and e4m3 converted, twice, and its
+// values once, where four waves that each hold the outputs of some queries and columns read them four times: with 16 heads
+// that took 90 us for 40 ragged sequences, not 69, with 32 heads and two tokens (8 x 17540 rows, bf16) 62, not 52.
+template <bool F8, int QG> struct FewStage {
   using G = Stage<F8>;
   // probabilities as the value products take them, 16 bytes a lane: bf16: rows 16 k ..; e4m3: high halves, low halves, the
   // scales of both blocks.  Two buffers: a tile's are read while the next one's are written.
-  static constexpr int LO = 2048, PS = 4096, PBUF = F8 ? 4352 : 2048, P = G::Q;
-  static constexpr int TOP = P + 2 * PBUF, M = TOP + 256, SUM = M + 128, ODD = SUM + 256, LIM = ODD + 16, LDS = LIM + 128;
+  static constexpr int LO = 2048, PS = 4096, PGRP = F8 ? 4352 : 2048, PBUF = QG * PGRP, P = G::Q;
+  static constexpr int TOP = P + 2 * PBUF, M = TOP + 256 * QG, SUM = M + 128 * QG, ODD = SUM + 256 * QG, LIM = ODD + 16,
+                       LDS = LIM + 128 * QG;
 };
-static_assert(FewStage<true>::LDS <= 160 * 1024 && FewStage<false>::LDS <= 160 * 1024);
+static_assert(FewStage<true, 2>::LDS <= 160 * 1024 && FewStage<false, 2>::LDS <= 160 * 1024);
 
-template <bool F8> struct FewWave {
+template <bool F8> struct FewSteps {
   static constexpr int N = F8 ? 10 : 18, READS = F8 ? 2 : 1, AHEAD = F8 ? 4 : 8;  // score steps, reads of one, steps ahead
-  bf16x8 q[18];   // the wave's 16 queries, in the order of the score steps
-  f32x16 o[4];    // O^T: the wave's 128 columns x 32 queries
-  f32x4 s[2];     // S^T: e4m3: rows 16 u .. of the wave's 32; bf16: two chains of its 16
-  float m, l, top;
+};
+template <bool F8, int QG> struct FewWave {  // QG groups of 32 queries: 16 of each are the wave's in the scores
+  bf16x8 q[QG][18];  // in the order of the score steps
+  f32x16 o[QG][4];   // O^T: the wave's 128 columns x 32 queries
+  f32x4 s[QG][2];    // S^T: e4m3: rows 16 u .. of the wave's 32; bf16: two chains of its 16
+  float m[QG], l[QG], top[QG];
 };
 // What a wave reads of a tile besides the keys: factors of the rows of its scores (4 (lane / 16) .. and, e4m3, 16 on)
 template <bool F8> struct FewFactors {
@@ -941,9 +944,9 @@ template <bool F8> struct FewFactors {
   float mul[2];
 };
 // What it needs for the values of the tile before: probabilities and the first columns
-template <bool F8> struct FewValues {
-  u32x4 p[4];
-  int ps;
+template <bool F8, int QG> struct FewValues {
+  u32x4 p[QG][4];
+  int ps[QG];
   u32x2 v[3][4];
 };
 
@@ -965,16 +968,16 @@ template <bool F8, int I> AMLA_DEV void few_read(u32x4 (&d)[2], uint32_t kl, uin
   }
 }
 template <bool F8, int I> AMLA_DEV void few_reads_first(u32x4 (*ka)[2], uint32_t kl, uint32_t kr) {
-  if constexpr (I < FewWave<F8>::AHEAD) {
+  if constexpr (I < FewSteps<F8>::AHEAD) {
     few_read<F8, I>(ka[I], kl, kr);
     few_reads_first<F8, I + 1>(ka, kl, kr);
   }
 }
 AMLA_DEV f32x4 mfma_few(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-template <bool F8, bool COPY, int I>
-AMLA_DEV void few_step(FewWave<F8> &w, u32x4 (&ka)[FewWave<F8>::AHEAD + 1][2], const float (&mul)[2], uint32_t kl, uint32_t kr,
+template <bool F8, int QG, bool COPY, int I>
+AMLA_DEV void few_step(FewWave<F8, QG> &w, u32x4 (&ka)[FewSteps<F8>::AHEAD + 1][2], const float (&mul)[2], uint32_t kl, uint32_t kr,
                        uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
-  using W = FewWave<F8>;
+  using W = FewSteps<F8>;
   if constexpr (I < W::N) {
     constexpr int A = W::AHEAD, c = I % (A + 1);
     if constexpr (I + A < W::N) few_read<F8, I + A>(ka[(I + A) % (A + 1)], kl, kr);
@@ -987,23 +990,35 @@ AMLA_DEV void few_step(FewWave<F8> &w, u32x4 (&ka)[FewWave<F8>::AHEAD + 1][2], c
       lds_tie(x);
     }
     if constexpr (!F8) {
-      w.s[I & 1] = mfma_few(as_bf16x8(x), w.q[I], w.s[I & 1]);
+#pragma unroll
+      for (int k = 0; k < QG; ++k) w.s[k][I & 1] = mfma_few(as_bf16x8(x), w.q[k][I], w.s[k][I & 1]);
     } else if constexpr (I < 8) {
-      w.s[0] = mfma_few(codes_to_bf16(x.x, x.y, mul[0]), w.q[2 * I], w.s[0]);
-      w.s[1] = mfma_few(codes_to_bf16(y.x, y.y, mul[1]), w.q[2 * I], w.s[1]);
-      w.s[0] = mfma_few(codes_to_bf16(x.z, x.w, mul[0]), w.q[2 * I + 1], w.s[0]);
-      w.s[1] = mfma_few(codes_to_bf16(y.z, y.w, mul[1]), w.q[2 * I + 1], w.s[1]);
+      const bf16x8 x0 = codes_to_bf16(x.x, x.y, mul[0]), y0 = codes_to_bf16(y.x, y.y, mul[1]);
+#pragma unroll
+      for (int k = 0; k < QG; ++k) {
+        w.s[k][0] = mfma_few(x0, w.q[k][2 * I], w.s[k][0]);
+        w.s[k][1] = mfma_few(y0, w.q[k][2 * I], w.s[k][1]);
+      }
+      const bf16x8 x1 = codes_to_bf16(x.z, x.w, mul[0]), y1 = codes_to_bf16(y.z, y.w, mul[1]);
+#pragma unroll
+      for (int k = 0; k < QG; ++k) {
+        w.s[k][0] = mfma_few(x1, w.q[k][2 * I + 1], w.s[k][0]);
+        w.s[k][1] = mfma_few(y1, w.q[k][2 * I + 1], w.s[k][1]);
+      }
     } else {
-      w.s[0] = mfma_few(as_bf16x8(x), w.q[16 + I - 8], w.s[0]);
-      w.s[1] = mfma_few(as_bf16x8(y), w.q[16 + I - 8], w.s[1]);
+#pragma unroll
+      for (int k = 0; k < QG; ++k) {
+        w.s[k][0] = mfma_few(as_bf16x8(x), w.q[k][16 + I - 8], w.s[k][0]);
+        w.s[k][1] = mfma_few(as_bf16x8(y), w.q[k][16 + I - 8], w.s[k][1]);
+      }
     }
     if constexpr (COPY && I < Rows<F8>::COPIES) next.template copy<I>(pg, st_next, r0, lanes);
-    few_step<F8, COPY, I + 1>(w, ka, mul, kl, kr, lanes, next, pg, st_next, r0);
+    few_step<F8, QG, COPY, I + 1>(w, ka, mul, kl, kr, lanes, next, pg, st_next, r0);
   }
 }
 // Scores of the tile at LDS address base; COPY: with the copies of a later one between
-template <bool F8, bool COPY>
-AMLA_DEV void few_scores(FewWave<F8> &w, FewFactors<F8> &f, uint32_t base, int half, const Rows<F8> &next, const LatentPages &pg,
+template <bool F8, int QG, bool COPY>
+AMLA_DEV void few_scores(FewWave<F8, QG> &w, FewFactors<F8> &f, uint32_t base, int half, const Rows<F8> &next, const LatentPages &pg,
                          uint8_t *st_next, int r0) {
   using G = Stage<F8>;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, row = half * (G::ROWS / 2) + l16;
@@ -1018,26 +1033,27 @@ AMLA_DEV void few_scores(FewWave<F8> &w, FewFactors<F8> &f, uint32_t base, int h
   }
   const uint32_t kl = base + row * Tile<F8>::RB + 16 * (few_chunk<F8>(g) ^ Tile<F8>::swz(row));
   const uint32_t kr = base + G::PE + row * 128 + 16 * (g ^ ((row >> 1) & 7));
-  u32x4 ka[FewWave<F8>::AHEAD + 1][2];
+  u32x4 ka[FewSteps<F8>::AHEAD + 1][2];
   few_reads_first<F8, 0>(ka, kl, kr);
-  lds_wait<FewWave<F8>::READS * FewWave<F8>::AHEAD>();
+  lds_wait<FewSteps<F8>::READS * FewSteps<F8>::AHEAD>();
   lds_tie(f.ex[0]);
   if constexpr (F8) lds_tie(f.ex[1], f.inv[0], f.inv[1], f.mul[0], f.mul[1]);
   else f.mul[0] = f.mul[1] = 1.f;
-  w.s[0] = w.s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  few_step<F8, COPY, 0>(w, ka, f.mul, kl, kr, Rows<F8>::lanes(r0), next, pg, st_next, r0);
+#pragma unroll
+  for (int k = 0; k < QG; ++k) w.s[k][0] = w.s[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  few_step<F8, QG, COPY, 0>(w, ka, f.mul, kl, kr, Rows<F8>::lanes(r0), next, pg, st_next, r0);
 }
 // z = s log2(e) scale + exponent of the row, in place; rows past lim are not seen
-template <bool F8, bool MASK> AMLA_DEV float few_scaled(FewWave<F8> &w, const FewFactors<F8> &f, float scale_log2, int lim) {
+template <bool F8, bool MASK> AMLA_DEV float few_scaled(f32x4 (&s)[2], const FewFactors<F8> &f, float scale_log2, int lim) {
   float top = -INFINITY;
-  if constexpr (!F8) w.s[0] += w.s[1];
+  if constexpr (!F8) s[0] += s[1];
 #pragma unroll
   for (int u = 0; u < (F8 ? 2 : 1); ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float z = __builtin_fmaf(w.s[u][i], scale_log2, __uint_as_float(f.ex[u][i]));
+      float z = __builtin_fmaf(s[u][i], scale_log2, __uint_as_float(f.ex[u][i]));
       if constexpr (MASK) z = 16 * u + i < lim ? z : -INFINITY;
-      w.s[u][i] = z;
+      s[u][i] = z;
       top = __builtin_fmaxf(top, z);
     }
   return top;
@@ -1052,38 +1068,40 @@ AMLA_DEV float few_max(float x) {
 AMLA_DEV void few_write(uint32_t addr, uint32_t v) { asm volatile("ds_write_b32 %0, %1" ::"v"(addr), "v"(v) : "memory"); }
 // Probabilities of the wave's scores, to LDS: rows 4 (g / 2 + 2 u) .. of query lane / 16 belong to lane query + 32 (g % 2)
 // of the value products
-template <bool F8> AMLA_DEV void few_probabilities(FewWave<F8> &w, const FewFactors<F8> &f, float top, uint32_t pbuf, int half, int qh) {
+template <bool F8>
+AMLA_DEV void few_probabilities(const f32x4 (&s)[2], float m, float &l, float &most, const FewFactors<F8> &f, float top, uint32_t pbuf,
+                                int half, int qh) {
   const int lane = threadIdx.x & 63, query = 16 * qh + (lane & 15), g = lane >> 4;
   const uint32_t to = pbuf + 1024 * half + 16 * (query + 32 * (g & 1));
-  w.top = __builtin_fmaxf(w.top, top);
+  most = __builtin_fmaxf(most, top);
   if constexpr (F8) {
-    const float ref = block_ref(few_max(top), w.m);  // of the 32 rows: a block of the matrix unit
+    const float ref = block_ref(few_max(top), m);  // of the 32 rows: a block of the matrix unit
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(w.s[u][i] - ref);
+        e[i] = __builtin_amdgcn_exp2f(s[u][i] - ref);
         sum = __builtin_fmaf(e[i], __uint_as_float(f.inv[u][i]), sum);
       }
       int hi, lo;
       split_fp8x4(e, 0.0625f, hi, lo);
       few_write(to + 4 * (g >> 1) + 8 * u, hi);
-      few_write(to + FewStage<F8>::LO + 4 * (g >> 1) + 8 * u, lo);
+      few_write(to + FewStage<F8, 1>::LO + 4 * (g >> 1) + 8 * u, lo);
     }
-    w.l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(ref - w.m), w.l);
-    few_write(pbuf + FewStage<F8>::PS + 4 * (32 * half + query), block_scale(ref, w.m));
+    l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(ref - m), l);
+    few_write(pbuf + FewStage<F8, 1>::PS + 4 * (32 * half + query), block_scale(ref, m));
   } else {
     float e[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(w.s[0][i] - w.m);
-    w.l += (e[0] + e[1]) + (e[2] + e[3]);
+    for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(s[0][i] - m);
+    l += (e[0] + e[1]) + (e[2] + e[3]);
     const u32x2 v = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
     asm volatile("ds_write_b64 %0, %1" ::"v"(to + 8 * (g >> 1)), "v"(v) : "memory");
   }
 }
-template <bool F8, int C> AMLA_DEV void few_value_read(FewValues<F8> &x, uint32_t v0, uint32_t v1) {
+template <bool F8, int QG, int C> AMLA_DEV void few_value_read(FewValues<F8, QG> &x, uint32_t v0, uint32_t v1) {
   if constexpr (C < 4) {
     u32x2(&v)[4] = x.v[C % 3];
     const uint32_t a = v0 ^ (F8 ? 32 * C : 64 * C), b = v1 ^ (64 * C);
@@ -1115,57 +1133,68 @@ template <bool F8> AMLA_DEV uint2 few_value_addr(uint32_t pv, int cg) {
   }
 }
 // The probabilities at pbuf and the first values
-template <bool F8> AMLA_DEV void few_values_first(FewValues<F8> &x, uint32_t pbuf, uint2 v) {
+template <bool F8, int QG> AMLA_DEV void few_values_first(FewValues<F8, QG> &x, uint32_t pbuf, uint2 v) {
   const int lane = threadIdx.x & 63;
-  x.p[0] = lds_read16<0>(pbuf + 16 * lane);
-  x.p[1] = lds_read16<1024>(pbuf + 16 * lane);
-  if constexpr (F8) {
-    x.p[2] = lds_read16<2048>(pbuf + 16 * lane);
-    x.p[3] = lds_read16<3 * 1024>(pbuf + 16 * lane);
-    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(x.ps) : "v"(pbuf + 4 * lane), "i"(FewStage<F8>::PS) : "memory");
+#pragma unroll
+  for (int k = 0; k < QG; ++k) {
+    const uint32_t pk = pbuf + k * FewStage<F8, QG>::PGRP;
+    x.p[k][0] = lds_read16<0>(pk + 16 * lane);
+    x.p[k][1] = lds_read16<1024>(pk + 16 * lane);
+    if constexpr (F8) {
+      x.p[k][2] = lds_read16<2048>(pk + 16 * lane);
+      x.p[k][3] = lds_read16<3 * 1024>(pk + 16 * lane);
+      asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(x.ps[k]) : "v"(pk + 4 * lane), "i"(FewStage<F8, QG>::PS) : "memory");
+    }
   }
-  few_value_read<F8, 0>(x, v.x, v.y);
-  few_value_read<F8, 1>(x, v.x, v.y);
+  few_value_read<F8, QG, 0>(x, v.x, v.y);
+  few_value_read<F8, QG, 1>(x, v.x, v.y);
 }
-template <bool F8, int C> AMLA_DEV void few_value_step(FewWave<F8> &w, FewValues<F8> &x, uint2 v) {
+template <bool F8, int QG, int C> AMLA_DEV void few_value_step(FewWave<F8, QG> &w, FewValues<F8, QG> &x, uint2 v) {
   if constexpr (C < 4) {
-    few_value_read<F8, C + 2>(x, v.x, v.y);
+    few_value_read<F8, QG, C + 2>(x, v.x, v.y);
     lds_wait<4 * ((C + 1 < 4) + (C + 2 < 4))>();
     if constexpr (C == 0) {
-      u32x4 a = x.p[0], b = x.p[1];
-      lds_tie(a, b);
-      x.p[0] = a;
-      x.p[1] = b;
-      if constexpr (F8) {
-        u32x4 d = x.p[2], e = x.p[3];
-        int ps = x.ps;
-        lds_tie(d, e, ps);
-        x.p[2] = d;
-        x.p[3] = e;
-        x.ps = ps;
+#pragma unroll
+      for (int k = 0; k < QG; ++k) {
+        u32x4 a = x.p[k][0], b = x.p[k][1];
+        lds_tie(a, b);
+        x.p[k][0] = a;
+        x.p[k][1] = b;
+        if constexpr (F8) {
+          u32x4 d = x.p[k][2], e = x.p[k][3];
+          int ps = x.ps[k];
+          lds_tie(d, e, ps);
+          x.p[k][2] = d;
+          x.p[k][3] = e;
+          x.ps[k] = ps;
+        }
       }
     }
     u32x2 a = x.v[C % 3][0], b = x.v[C % 3][1], d = x.v[C % 3][2], e = x.v[C % 3][3];
     lds_tie(a, b, d, e);
-    if constexpr (F8) {
-      const i32x8 hi = {(int)x.p[0].x, (int)x.p[0].y, (int)x.p[0].z, (int)x.p[0].w, (int)x.p[1].x, (int)x.p[1].y, (int)x.p[1].z, (int)x.p[1].w};
-      const i32x8 lo = {(int)x.p[2].x, (int)x.p[2].y, (int)x.p[2].z, (int)x.p[2].w, (int)x.p[3].x, (int)x.p[3].y, (int)x.p[3].z, (int)x.p[3].w};
-      mfma_value<true>(w.o[C], join(a, b, d, e), 127, hi, x.ps);
-      mfma_value<true>(w.o[C], join(a, b, d, e), 127, lo, x.ps - 4);
-    } else {
-      mfma_value<true>(w.o[C], as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), as_bf16x8(x.p[0]));
-      mfma_value<true>(w.o[C], as_bf16x8(u32x4{d.x, d.y, e.x, e.y}), as_bf16x8(x.p[1]));
+#pragma unroll
+    for (int k = 0; k < QG; ++k) {
+      const u32x4(&p)[4] = x.p[k];
+      if constexpr (F8) {
+        const i32x8 hi = {(int)p[0].x, (int)p[0].y, (int)p[0].z, (int)p[0].w, (int)p[1].x, (int)p[1].y, (int)p[1].z, (int)p[1].w};
+        const i32x8 lo = {(int)p[2].x, (int)p[2].y, (int)p[2].z, (int)p[2].w, (int)p[3].x, (int)p[3].y, (int)p[3].z, (int)p[3].w};
+        mfma_value<true>(w.o[k][C], join(a, b, d, e), 127, hi, x.ps[k]);
+        mfma_value<true>(w.o[k][C], join(a, b, d, e), 127, lo, x.ps[k] - 4);
+      } else {
+        mfma_value<true>(w.o[k][C], as_bf16x8(u32x4{a.x, a.y, b.x, b.y}), as_bf16x8(p[0]));
+        mfma_value<true>(w.o[k][C], as_bf16x8(u32x4{d.x, d.y, e.x, e.y}), as_bf16x8(p[1]));
+      }
     }
-    few_value_step<F8, C + 1>(w, x, v);
+    few_value_step<F8, QG, C + 1>(w, x, v);
   }
 }
 
-template <bool F8, bool MASK>
+template <bool F8, int QG, bool MASK>
 __global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParams p) {
   extern __shared__ __align__(1024) uint8_t sm[];
   using G = Stage<F8>;
-  using F = FewStage<F8>;
-  constexpr int TILE = Tile<F8>::ROWS;
+  using F = FewStage<F8, QG>;
+  constexpr int TILE = Tile<F8>::ROWS, NQ = 32 * QG;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = wave & 1, qh = wave >> 1, l16 = lane & 15, g = lane >> 4;
   const SplitWork at = split_work<F8>(p);
@@ -1176,95 +1205,123 @@ __global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParam
   if constexpr (MASK) feed.tail = p.seq_len - 1;
   feed.start(at.t_first);
 
-  FewWave<F8> w;
-  const int query = 16 * qh + l16, rq = min(at.chunk * 32 + query, p.rows - 1), tok = rq / p.heads;
-  // rows of a tile below lim - TILE tile are seen: of the lane's first, row TILE / 2 half + 4 g
-  const int limit = at.held - (p.seq_len - 1 - tok), lim = limit - TILE / 2 * half - 4 * g;
-  const uint16_t *qp = p.q + at.b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
+  FewWave<F8, QG> w;
+  const int query = 16 * qh + l16;  // of a group
+  int limit[QG], lim[QG];           // rows of a tile below lim - TILE tile are seen: of the lane's first, row TILE / 2 half + 4 g
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    w.q[i] = as_bf16x8(ldg16(qp + (F8 ? 64 * (i >> 1) + 16 * few_chunk<F8>(g) + 8 * (i & 1) : 32 * i + 8 * few_chunk<F8>(g))));
+  for (int k = 0; k < QG; ++k) {
+    const int rq = min(at.chunk * NQ + 32 * k + query, p.rows - 1), tok = rq / p.heads;
+    limit[k] = at.held - (p.seq_len - 1 - tok);
+    lim[k] = limit[k] - TILE / 2 * half - 4 * g;
+    const uint16_t *qp = p.q + at.b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) w.q[16 + i] = as_bf16x8(ldg16(qp + LC_LORA + 32 * i + 8 * g));
-  w.m = M_NONE;
+    for (int i = 0; i < 16; ++i)
+      w.q[k][i] = as_bf16x8(ldg16(qp + (F8 ? 64 * (i >> 1) + 16 * few_chunk<F8>(g) + 8 * (i & 1) : 32 * i + 8 * few_chunk<F8>(g))));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w.q[k][16 + i] = as_bf16x8(ldg16(qp + LC_LORA + 32 * i + 8 * g));
+    w.m[k] = M_NONE;
+  }
   float *const x_top = reinterpret_cast<float *>(sm + F::TOP), *const x_m = reinterpret_cast<float *>(sm + F::M);
   FewFactors<F8> f;
   for (int pass = 0;; ++pass) {  // once, or twice where m turned out too low
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int k = 0; k < QG; ++k) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w.o[c][i] = 0.f;
-    settle(w.o);
-    w.l = 0.f;
-    w.top = -INFINITY;
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w.o[k][c][i] = 0.f;
+      settle(w.o[k]);
+      w.l[k] = 0.f;
+      w.top[k] = -INFINITY;
+    }
     // nothing before the first tile: probabilities of 0 times its own values
     for (int o = threadIdx.x * 4; o < F::PBUF; o += 1024)
-      *reinterpret_cast<uint32_t *>(sm + F::P + F::PBUF + o) = o < F::PS ? 0u : 127u;
+      *reinterpret_cast<uint32_t *>(sm + F::P + F::PBUF + o) = o % F::PGRP < F::PS ? 0u : 127u;
     if (pass == 0) {  // the waves agree on m: the first tile's maxima, its scores made twice
       feed.template arrive<MASK>(at.t_first);
-      few_scores<F8, false>(w, f, lds0, half, feed.next, p.pg, sm, 0);
-      const float top = few_max(few_scaled<F8, MASK>(w, f, p.scale_log2, lim - at.t_first * TILE));
-      x_top[32 * half + query] = top;
+      few_scores<F8, QG, false>(w, f, lds0, half, feed.next, p.pg, sm, 0);
+#pragma unroll
+      for (int k = 0; k < QG; ++k)
+        x_top[NQ * half + 32 * k + query] = few_max(few_scaled<F8, MASK>(w.s[k], f, p.scale_log2, lim[k] - at.t_first * TILE));
       __syncthreads();
-      w.m = __builtin_fmaxf(__builtin_fmaxf(x_top[query], x_top[32 + query]), M_NONE);
+#pragma unroll
+      for (int k = 0; k < QG; ++k)
+        w.m[k] = __builtin_fmaxf(__builtin_fmaxf(x_top[32 * k + query], x_top[NQ + 32 * k + query]), M_NONE);
     }
     uint32_t base = lds0, pbuf = lds0 + F::P;
     for (int tile = at.t_first; tile < at.t_end; ++tile) {
       const uint32_t before = base, p_before = 2 * lds0 + 2 * F::P + F::PBUF - pbuf;
       feed.template arrive<MASK>(tile);
       base = lds0 + feed.cur * G::SIZE;
-      FewValues<F8> x;
+      FewValues<F8, QG> x;
       const uint2 v = few_value_addr<F8>(before, wave);
-      few_values_first<F8>(x, p_before, v);
-      few_scores<F8, true>(w, f, base, half, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
-      few_value_step<F8, 0>(w, x, v);
-      const float top = few_scaled<F8, MASK>(w, f, p.scale_log2, lim - tile * TILE);
-      few_probabilities<F8>(w, f, top, pbuf, half, qh);
+      few_values_first<F8, QG>(x, p_before, v);
+      few_scores<F8, QG, true>(w, f, base, half, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+      few_value_step<F8, QG, 0>(w, x, v);
+#pragma unroll
+      for (int k = 0; k < QG; ++k) {
+        const float top = few_scaled<F8, MASK>(w.s[k], f, p.scale_log2, lim[k] - tile * TILE);
+        few_probabilities<F8>(w.s[k], w.m[k], w.l[k], w.top[k], f, top, pbuf + k * F::PGRP, half, qh);
+      }
       pbuf = p_before;
       feed.advance(tile);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     {
-      FewValues<F8> x;
+      FewValues<F8, QG> x;
       const uint2 v = few_value_addr<F8>(base, wave);
-      few_values_first<F8>(x, 2 * lds0 + 2 * F::P + F::PBUF - pbuf, v);
-      few_value_step<F8, 0>(w, x, v);
+      few_values_first<F8, QG>(x, 2 * lds0 + 2 * F::P + F::PBUF - pbuf, v);
+      few_value_step<F8, QG, 0>(w, x, v);
     }
-    settle(w.o);
+#pragma unroll
+    for (int k = 0; k < QG; ++k) settle(w.o[k]);
     wait_vmcnt<0>();  // (copies past the last tile)
-    const float top = few_max(w.top);
-    x_top[32 * half + query] = top;
-    x_m[query] = w.m;
+#pragma unroll
+    for (int k = 0; k < QG; ++k) {
+      x_top[NQ * half + 32 * k + query] = few_max(w.top[k]);
+      x_m[32 * k + query] = w.m[k];
+    }
     if constexpr (MASK) reinterpret_cast<int *>(sm + F::ODD)[wave] = feed.odd;
     __syncthreads();
-    const float high = __builtin_fmaxf(x_top[query], x_top[32 + query]);
-    const bool again = __ballot(__builtin_fmaxf(x_top[lane & 31], x_top[32 + (lane & 31)]) > x_m[lane & 31] + LAG) != 0;
+    float high[QG];
+#pragma unroll
+    for (int k = 0; k < QG; ++k) high[k] = __builtin_fmaxf(x_top[32 * k + query], x_top[NQ + 32 * k + query]);
+    const int any = lane % NQ;
+    const bool again = __ballot(__builtin_fmaxf(x_top[any], x_top[NQ + any]) > x_m[any] + LAG) != 0;
     __syncthreads();
     if (!again) break;
-    w.m = high > w.m + LAG ? high : w.m;
+#pragma unroll
+    for (int k = 0; k < QG; ++k) w.m[k] = high[k] > w.m[k] + LAG ? high[k] : w.m[k];
     feed.start(at.t_first);
   }
   // sums over the four lanes and both halves of a query, handed to the lanes that hold its outputs
   float *const x_sum = reinterpret_cast<float *>(sm + F::SUM);
-  w.l += __shfl_xor(w.l, 16, 64);
-  w.l += __shfl_xor(w.l, 32, 64);
-  x_sum[32 * half + query] = w.l;
-  x_m[query] = w.m;
-  if constexpr (MASK) reinterpret_cast<int *>(sm + F::LIM)[query] = limit;
-  __syncthreads();
-  float l = x_sum[lane & 31] + x_sum[32 + (lane & 31)];
-  const float m = x_m[lane & 31];
-  if constexpr (MASK) {
-    const int *odd = reinterpret_cast<const int *>(sm + F::ODD);
-    const int first = min(min(odd[0], odd[1]), min(odd[2], odd[3]));
-    l = first < reinterpret_cast<const int *>(sm + F::LIM)[lane & 31] ? __uint_as_float(0x7fc00000u) : l;
+  int *const x_lim = reinterpret_cast<int *>(sm + F::LIM);
+#pragma unroll
+  for (int k = 0; k < QG; ++k) {
+    w.l[k] += __shfl_xor(w.l[k], 16, 64);
+    w.l[k] += __shfl_xor(w.l[k], 32, 64);
+    x_sum[NQ * half + 32 * k + query] = w.l[k];
+    x_m[32 * k + query] = w.m[k];
+    if constexpr (MASK) x_lim[32 * k + query] = limit[k];
   }
-  store_split<1>(p, sm, w.o, l, m, at.b, at.chunk, at.slot, at.splits, wave);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < QG; ++k) {
+    const int j = 32 * k + (lane & 31);
+    float l = x_sum[j] + x_sum[NQ + j];
+    if constexpr (MASK) {
+      const int *odd = reinterpret_cast<const int *>(sm + F::ODD);
+      const int first = min(min(odd[0], odd[1]), min(odd[2], odd[3]));
+      l = first < x_lim[j] ? __uint_as_float(0x7fc00000u) : l;
+    }
+    store_split<QG>(p, sm, w.o[k], l, x_m[j], at.b, at.chunk, at.slot, at.splits, wave, k, wave);
+  }
 }
 
 // Joins the splits of a query row: sum_j 2^(lse_j - max) O_j / sum_j 2^(lse_j - max).  One workgroup a row, wave k
 // taking splits k, k + 4, .., eight rows of 1 KB in flight; the waves' sums meet in LDS in wave order.
-template <bool F8, int HG>
+template <int HG, int CG>  // 32-row groups and column groups of the workgroups before
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
   __shared__ float part[3][64][9];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1288,7 +1345,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
   const float ref = top == -INFINITY ? 0.f : top;
   float total = 0.f, a[8] = {};
   const uint16_t *po = p.part_o + src * LC_LORA + 8 * lane;
-  const float *ps = p.part_scale + src * 4 + lane / (64 * HG / 4);
+  const float *ps = p.part_scale + src * 4 + lane / (64 / CG);
   for (int j0 = wave; j0 < n; j0 += 32) {
     float w[8], s[8];
     u32x4 v[8];
@@ -1333,11 +1390,11 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
 constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 
 // 32-row groups of a workgroup: as many as the rows of a sequence fill, since they share each tile's way through LDS, but
-// one (the kernel for few query rows) while the cached rows do not keep all CUs at work for long: then more, shorter
-// workgroups win.  Measured with 128 heads and one new token (1 / 2 / 4 groups, us), fp8: 1 x 257 rows 16 / 19 / 22,
-// 64 x 200 31 / 48 / 53, 8 x 4096 34 / 38 / 41, 8 x 6144 43 / 44 / 44, 32 x 2048 57 / 56 / 53, 32 x 4096 90 / 83 / 68,
-// 8 x 32768 149 / 128 / 92; bf16: 8 x 4096 34 / 40 / 41, 8 x 8192 50 / 54 / 49, 8 x 32768 148 / 145 / 104; 64 heads, 40 x
-// 4096: fp8 71 / 65, bf16 74 / 73.
+// one while the cached rows do not keep all CUs at work for long: then more, shorter workgroups win.  One or two: the kernel
+// for few query rows.  Measured with 128 heads and one new token (1 / 2 / 4 groups, us), fp8: 1 x 257 rows 16 / 21 / 22,
+// 64 x 512 31 / 43 / 52, 4 x 8192 34 / 39 / 42, 8 x 8192 50 / 49 / 50, 32 x 4096 85 / 74 / 67, 8 x 32768 146 / 115 / 96;
+// bf16: 4 x 8192 36 / 38 / 42, 8 x 8192 50 / 46 / 51, 32 x 4096 85 / 70 / 73, 8 x 32768 149 / 108 / 106; 64 heads: 64 x 1024
+// fp8 39 / 43, 40 x 4096 65 / 59, bf16 69 / 59 (four groups half empty there).
 static int attn_groups(int64_t seqs, int64_t rows, int64_t max_rows) {
   const double pairs = (double)seqs * rows * max_rows / LA_UNITS;  // query rows x cached rows of a CU
   return pairs < 32 * 1024 || rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
@@ -1360,9 +1417,9 @@ template <bool F8, int HG>
 static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
   void (*kernel)(LatentAttnParams);
   int lds;
-  if constexpr (HG == 1) {
-    kernel = p.seq_len > 1 ? latent_attn_few_kernel<F8, true> : latent_attn_few_kernel<F8, false>;
-    lds = FewStage<F8>::LDS;
+  if constexpr (HG <= 2) {
+    kernel = p.seq_len > 1 ? latent_attn_few_kernel<F8, HG, true> : latent_attn_few_kernel<F8, HG, false>;
+    lds = FewStage<F8, HG>::LDS;
   } else {
     kernel = p.seq_len > 1 ? latent_attn_kernel<F8, HG, true> : latent_attn_kernel<F8, HG, false>;
     lds = Stage<F8>::LDS;
@@ -1371,7 +1428,7 @@ static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
   if (rc) return rc;
   kernel<<<dim3((unsigned)(p.slots + 7) / 8 * 8), 256, lds, st>>>(p);  // whole runs of every XCD
   if ((rc = check_launch("latent_attention"))) return rc;
-  latent_join_kernel<F8, HG><<<dim3((unsigned)p.rows, (unsigned)p.seqs), 256, 0, st>>>(p);
+  latent_join_kernel<HG, HG <= 2 ? 4 : 1><<<dim3((unsigned)p.rows, (unsigned)p.seqs), 256, 0, st>>>(p);
   return check_launch("latent_attention join");
 }
 
