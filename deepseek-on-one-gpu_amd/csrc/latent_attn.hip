@@ -760,7 +760,9 @@ AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB
   float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse2 = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
   float scale = 1.f;
-  if (splits > 1) {  // the largest of the row's values in this wave to 2^14 .. 2^15
+  // The largest of the row's values in this wave to 2^14 .. 2^15, or as near as inv times that power stays finite: all of them
+  // may be 0 where l is far below 1 (it sums 2^(s - m), and m has the exponent of an e4m3 row in it: down to 2^-32).
+  if (splits > 1) {
     float top = 0.f;
 #pragma unroll
     for (int c = 0; c < NCB; ++c)
@@ -768,7 +770,8 @@ AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB
       for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(o[c][i]));
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
     top = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * inv;
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 240);  // biased; below 15: zeros nearly
+    const int least = max((int)(__float_as_uint(inv) >> 23) - 112, 15);                       // biased; below it: zeros nearly
+    const int e = min(max((int)(__float_as_uint(top) >> 23), least), 240);
     scale = __uint_as_float((uint32_t)(e - 14) << 23);                   // 2^(e - 127 - 14)
     inv *= __uint_as_float((uint32_t)(254 - (e - 14)) << 23);
   }
