@@ -749,7 +749,7 @@ template <bool F16, int NCB> AMLA_DEV void turn_rows(uint8_t *turn, const f32x16
           F16 ? u32x2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])} : u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
     }
 }
-// A split's sums, normalised: the output itself, or a partial one.  l, m: of the lane's query row.
+// A split's sums, normalised: the output itself, or a partial one.  l, m: of the lane's query row (l = 0: it sees no row).
 // GROUPS: 32-row groups of a workgroup; hg: this one, cg: the wave's of 16 / NCB column groups.
 template <int GROUPS, int NCB>
 AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB], float l, float m, int b, int chunk, int slot,
@@ -780,6 +780,9 @@ AMLA_DEV void store_split(LatentAttnParams p, uint8_t *sm, const f32x16 (&o)[NCB
   uint8_t *turn = sm + wave * 32 * RBYTES;
   if (splits > 1) turn_rows<true>(turn, o, inv);
   else turn_rows<false>(turn, o, inv);
+  if (l == 0.f) {  // no row is seen (sees_none)
+    for (int i = 0; i < RBYTES / 2; i += 8) *reinterpret_cast<u32x2 *>(turn + j32 * RBYTES + RBYTES / 2 * hh + i) = u32x2{0, 0};
+  }
   const int row0 = (chunk * HG + hg) * 32, held = min(32, p.rows - row0);
   const size_t dst0 = splits == 1 ? (size_t)b * p.rows + row0 : (size_t)slot * (32 * HG) + 32 * hg;
   uint16_t *to[2] = {p.part_o, p.out};
@@ -816,6 +819,18 @@ template <bool F8> AMLA_DEV SplitWork split_work(const LatentAttnParams &p) {
   const int n_tiles = lc_ceil_div(held, TILE);
   return SplitWork{at.x, (slot - at.y) / at.z, slot, at.z, held, (int)((int64_t)split * n_tiles / at.z),
                    (int)((int64_t)(split + 1) * n_tiles / at.z)};
+}
+// Whether a token of the split, which sees rows below lim, sees none.  Asked where its sum is NaN: a query that is no number
+// times the zeros of absent rows is NaN too (their scores have -inf added, not put in their place: that would be two
+// instructions more for each), but what has no rows gives zeros.
+template <int TILE> AMLA_DEV bool sees_none(const LatentPages &pg, const SplitWork &at, int lim) {
+  const int end = min(at.held, at.t_end * TILE);
+  for (int t = at.t_first * TILE; t < end; t += 64) {
+    const int r = t + (int)(threadIdx.x & 63);
+    const uint64_t there = __ballot(r < end && pg.slot(at.b, r) >= 0);
+    if (there) return t + __builtin_ctzll(there) >= lim;
+  }
+  return true;
 }
 
 // One workgroup of four waves per (sequence, chunk of 32 HG rows, split), HG = 4: a wave holds 32
@@ -912,6 +927,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   float l = w.l;
   l += __shfl_xor(l, 32, 64);
   if constexpr (MASK) l = feed.odd < limit + 4 * hh ? __uint_as_float(0x7fc00000u) : l;
+  if (__ballot(l != l)) l = sees_none<TILE>(p.pg, at, MASK ? limit + 4 * hh : INT32_MAX) ? 0.f : l;
   store_split<HG>(p, sm, w.o, l, w.m, b, chunk, slot, splits, wave, hg, cg);
 }
 
@@ -1318,6 +1334,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_few_kernel(LatentAttnParam
       const int first = min(min(odd[0], odd[1]), min(odd[2], odd[3]));
       l = first < x_lim[j] ? __uint_as_float(0x7fc00000u) : l;
     }
+    if (__ballot(l != l)) l = sees_none<TILE>(p.pg, at, MASK ? x_lim[j] : INT32_MAX) ? 0.f : l;
     store_split<QG>(p, sm, w.o[k], l, x_m[j], at.b, at.chunk, at.slot, at.splits, wave, k, wave);
   }
 }

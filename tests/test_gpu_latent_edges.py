@@ -3,8 +3,10 @@ references that are set anew, in every kernel that it has."""
 import pytest
 import torch
 
-from _latent import BF16, cache_of
-from test_gpu_latent_attention import _run, _wider
+from _latent import BF16, cache_of, check_attention, to_dev
+from amla import ops
+from oracle import ref_latent as L
+from test_gpu_latent_attention import SCALE, _case, _run, _weight, _wider
 
 pytestmark = pytest.mark.gpu
 
@@ -26,4 +28,25 @@ def test_columns_of_zeros_in_split_sequences(e, H, cols):
     q = (torch.randn(2, 1, H, 576, generator=g) * (3.2 / (448 * 2.0 ** e * 384 ** 0.5))).to(BF16)
     _run(q, cache, _wider(table, cols) if cols else table, torch.tensor(lens, dtype=torch.int32), scale=1.0,
          what=f"zero columns, e={e} H={H}")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", [(1, 16, 0), (1, 64, 450), (1, 128, 450), (2, 16, 0), (2, 32, 450), (2, 64, 450)])
+def test_no_rows_and_a_query_that_is_no_number(fp8, S, H, cols):
+    """A slot of the batch without a sequence: its pages are none, its query is whatever was there.  Zeros, like for any
+    token that sees no row, and nothing of it in the others."""
+    lens = [100, 70, 5000, 3, 17]
+    q, cache, table, lengths = _case(61 + S + H, lens, S, H, fp8, 16)
+    table[1], table[2], table[4, 0] = -1, -1, cache[0].shape[0]
+    clean = q.clone()
+    q[1] = float("nan")
+    q[2, ..., 5] = float("inf")
+    if S > 1:
+        q[4, 0] = float("nan")  # sees the absent page only, where the last token sees a row more
+    table = _wider(table, max(cols * 4, table.shape[1]))
+    print(f"[case] fp8={fp8} S={S} H={H}", flush=True)
+    got, lse = ops.latent_attention(to_dev(q), to_dev(cache), to_dev(table), to_dev(lengths), SCALE, return_lse=True)
+    want, want_lse = L.latent_attention(clean, cache, table, lengths, SCALE)
+    assert (want_lse[[1, 2]] == float("-inf")).all() and ((want_lse[4] == float("-inf")).sum() == (S - 1) * H)
+    check_attention(got, want, lse, want_lse, *_weight(clean, cache, table, lengths, SCALE), f"fp8={fp8} S={S} H={H} no rows")
 
