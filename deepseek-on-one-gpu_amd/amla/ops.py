@@ -946,6 +946,7 @@ def latent_cache_write(kv: torch.Tensor, kv_a_layernorm: torch.Tensor, rope_freq
         _need_i32(offsets, "offsets", what, dev, (B + 1,))
     pos = _positions(position, B, 1, dev, None)[0] if B else torch.empty(0, dtype=torch.int32, device=dev)
     _need_i32(pos, "position", what, dev, (B,))
+    rope_freqs = rope_freqs.resolve_conj()  # (conj() leaves the values as they are and sets a flag)
     torch_ops.call_latent("latent_cache_write", kv, kv_a_layernorm, rope_freqs, latent, k_pe, scales, block_table, pos,
                           offsets, float(eps))
 

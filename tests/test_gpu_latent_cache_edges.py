@@ -1,0 +1,31 @@
+"""Inputs of latent_cache_write that torch holds in an unusual way, and rows that are no numbers."""
+import pytest
+import torch
+
+from _latent import BF16, DEV, FP8
+from amla import ops
+from amla.config import DeepSeekConfig
+from test_gpu_latent_cache import _check_rows, _freqs, _gamma, _kv
+
+pytestmark = pytest.mark.gpu
+CFG = DeepSeekConfig()
+
+
+def _stored(kv, gamma, freqs, fp8, B, rows, **kw):
+    """Rows 0 .. rows - 1 of B sequences as they are read back after one write at position 0."""
+    cache = ops.latent_cache(B * 4, 8, CFG, DEV, FP8 if fp8 else BF16)
+    table = torch.arange(B * 4, dtype=torch.int32, device=DEV).view(B, 4)
+    ops.latent_cache_write(kv, gamma, freqs, cache, table, 0, **kw)
+    off = torch.arange(B + 1, dtype=torch.int32, device=DEV) * rows
+    return ops.latent_cache_read(cache, table, off, B * rows)
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+def test_conjugated_angles(fp8):
+    """``freqs.conj()`` is a view with a flag: the rotation is the other way round."""
+    g = torch.Generator().manual_seed(6)
+    kv, gamma, freqs = _kv(g, 2, 7), _gamma(g), _freqs(32)
+    print(f"[case] fp8={fp8} conjugated", flush=True)
+    lat, pe = _stored(kv.to(DEV), gamma.to(DEV), freqs.to(DEV).conj(), fp8, 2, 7)
+    turned = freqs.conj().resolve_conj()
+    _check_rows(lat, pe, kv.reshape(-1, 576), gamma, turned[:7].repeat(2, 1), 1e-6, fp8, "conjugated")
