@@ -1407,6 +1407,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentAttnParams p) {
   if (lane == 0 && p.lse) p.lse[dst] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
 }
 
+constexpr int LA_MAX_ROWS = INT32_MAX - 511;  // of a sequence: rows are counted in 32 bits up to three tiles past the last one
 constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 
 // 32-row groups of a workgroup: as many as the rows of a sequence fill, since they share each tile's way through LDS, but
@@ -1480,6 +1481,7 @@ int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t
   if (ldq_seq % 8 || ldq_token % 8 || ldq_head % 8 || !aligned16(q) || !aligned16(out))
     return fail(AMLA_EUNSUPPORTED, "%s: q rows and out must be 16-byte aligned", what);
   const int64_t cap = cache->cols * cache->page_size;
+  if (cap > LA_MAX_ROWS) return fail(AMLA_EUNSUPPORTED, "%s: sequences of at most %d rows in their table", what, LA_MAX_ROWS);
   const AttnSizes s = attn_sizes(seqs, seq_len * heads, cap);
   if (s.slots >= (1 << 24) - 8 || seq_len * heads >= 1 << 24)  // grids of fewer than 2^32 threads
     return fail(AMLA_EUNSUPPORTED, "%s: too many query rows", what);
