@@ -11,6 +11,7 @@
 #include <math.h>
 
 #include "latent.h"
+#include "latent_plan.h"
 
 namespace amla {
 
@@ -73,15 +74,17 @@ struct SplitPlan {
     return __builtin_amdgcn_readfirstlane(wave_isum(n)) * p.chunks;  // (scalar: what follows from it is uniform)
   }
   AMLA_DEV explicit SplitPlan(const LatentAttnParams &p_) : p(p_) {
-    int sum = 0, most = 0;
+    int64_t sum = 0;
+    int most = 0;
     for (int b = threadIdx.x & 63; b < p.seqs; b += 64) {
       const int n = tiles(b);
       sum += n;
       most = max(most, n);
     }
-    const int64_t total = (int64_t)__builtin_amdgcn_readfirstlane(wave_isum(sum)) * p.chunks;
-    int lo = max(1, (int)((total + p.slots - 1) / p.slots));
-    int hi = max(lo, min(__builtin_amdgcn_readfirstlane(wave_imax(most)), (int)(total / max(1, p.slots - p.chunks * p.seqs)) + 1));
+    const int low = __builtin_amdgcn_readfirstlane(wave_isum(plan_low(sum)));
+    const int high = __builtin_amdgcn_readfirstlane(wave_isum(plan_high(sum)));
+    const PlanRange r = plan_range(plan_total(low, high), __builtin_amdgcn_readfirstlane(wave_imax(most)), p.chunks, p.seqs, p.slots);
+    int lo = r.lo, hi = r.hi;
     for (int probe = lo; lo < hi; probe = (lo + hi) >> 1) {
       if (used(probe) <= p.slots) hi = probe;
       else lo = probe + 1;

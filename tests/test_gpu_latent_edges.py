@@ -50,3 +50,31 @@ def test_no_rows_and_a_query_that_is_no_number(fp8, S, H, cols):
     assert (want_lse[[1, 2]] == float("-inf")).all() and ((want_lse[4] == float("-inf")).sum() == (S - 1) * H)
     check_attention(got, want, lse, want_lse, *_weight(clean, cache, table, lengths, SCALE), f"fp8={fp8} S={S} H={H} no rows")
 
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("H", [8, 64, 128])
+def test_long_sequences_over_few_pages(fp8, H):
+    """More than 2^12 tiles in one lane's sum of the plan: tables that name three pages of 512 rows over and over."""
+    g = torch.Generator().manual_seed(27)
+    n = 1536
+    cache, once = cache_of([torch.randn(n, 512, generator=g, dtype=torch.float64)], [torch.randn(n, 64, generator=g, dtype=torch.float64)],
+                           fp8, 512, [n], g, junk=float("nan"))
+    lens = [270000, 5, 300007, 131073]
+    table = torch.stack([once[0, (torch.arange(600) + b) % 3] for b in range(4)])
+    q = (torch.randn(4, 1, H, 576, generator=g) * 0.5).to(BF16)
+    print(f"[case] fp8={fp8} H={H} long", flush=True)
+    got, lse = ops.latent_attention(to_dev(q), to_dev(cache), to_dev(table), to_dev(torch.tensor(lens, dtype=torch.int32)), SCALE,
+                                    return_lse=True)
+    lat, rope = L.pool_values(cache)
+    rows = torch.tensor([L.places(once, 0, t, 512, cache[0].shape[0]) for t in range(n)])
+    k = torch.cat([lat[rows], rope[rows]], -1)
+    want, weight = torch.zeros(2, 4, 1, H, 512, dtype=torch.float64)
+    want_lse = torch.zeros(4, 1, H, dtype=torch.float64)
+    for b, m in enumerate(lens):  # the rows as often as they are held
+        often = (m // n + (torch.arange(n) < m % n)).double().roll(512 * b)
+        s = q[b, 0].double() @ k.T * SCALE + often.log()
+        want_lse[b, 0] = s.logsumexp(-1)
+        p = (s - want_lse[b, 0, :, None]).exp()
+        want[b, 0], weight[b, 0] = p @ lat[rows], p @ lat[rows].abs()
+    size = SCALE * (q.double().abs().flatten(0, 2) @ k.abs().T).max().item()
+    check_attention(got, want, lse, want_lse, weight, size, f"fp8={fp8} H={H} long")
