@@ -22,6 +22,7 @@ constexpr int PA_KT = 64;                 // keys per tile
 constexpr int PA_QB = 256;                // queries per workgroup: four waves, two groups of 32 each
 constexpr int PA_NST = 3;                 // LDS stages: a tile, the one before it (values), the one to come
 constexpr int PA_VD = 128;
+constexpr int PA_MAX_ROWS = INT32_MAX - 511;  // of queries and of keys: counted in 32 bits up to a block past the last one
 constexpr int PA_HALF = PA_KT * 128;      // 64 rows of 128 bytes: 64 key or value columns of a tile
 
 struct PackedParams {
@@ -813,8 +814,8 @@ extern "C" int amla_packed_attention(const amla_packed_args *a, void *stream) {
   if ((a->dn != 128 && a->dn != 192) || (a->k_pe && a->dn != 128))
     return fail(AMLA_EUNSUPPORTED, "%s: keys of 128 values (with or without k_pe) or of 192 (dn=%d)", what, a->dn);
   if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(AMLA_EINVAL, "%s: scale must be positive", what);
-  if (a->q_rows > INT32_MAX || a->k_rows > INT32_MAX || a->seqs > AMLA_MAX_SEQS)
-    return fail(AMLA_EUNSUPPORTED, "%s: at most 2^31 - 1 rows and %d sequences", what, AMLA_MAX_SEQS);
+  if (a->q_rows > PA_MAX_ROWS || a->k_rows > PA_MAX_ROWS || a->seqs > AMLA_MAX_SEQS)
+    return fail(AMLA_EUNSUPPORTED, "%s: at most %d rows and %d sequences", what, PA_MAX_ROWS, AMLA_MAX_SEQS);
   const int64_t lds[] = {a->ldq, a->ldq_head, a->ldk, a->ldk_head, a->ldv, a->ldv_head, a->k_pe ? a->ld_pe : 0};
   for (int64_t ld : lds)
     if (ld % 8 || ld < 0 || ld > (1 << 27)) return fail(AMLA_EUNSUPPORTED, "%s: strides must be multiples of 8 values up to 2^27", what);

@@ -6,7 +6,7 @@ import subprocess
 import pytest
 
 from test_asm_waits import CSRC
-from test_latent_refusals import EUNSUPPORTED, EWORKSPACE, L, P, _attend, _cache  # noqa: F401  (L: a fixture)
+from test_latent_refusals import EUNSUPPORTED, EWORKSPACE, L, P, _attend, _cache, _packed  # noqa: F401  (L: a fixture)
 
 
 @pytest.mark.parametrize("scales", [P, None])
@@ -70,3 +70,13 @@ def test_sums_of_tiles_past_two_to_31(plan, tiles, chunks, slots):
     used = lambda n: chunks * sum(-(-t // n) * k for t, k in kinds.items())  # noqa: E731
     assert 1 <= lo <= hi and used(hi) <= slots and (lo == 1 or used(lo - 1) > slots)
     assert all(used(n) < 2 ** 31 for n in (lo, hi, (lo + hi) // 2))  # (counted in 32 bits)
+
+
+def test_rows_of_packed_prompts_end_below_two_to_31(L):  # noqa: F811
+    """Keys of one row for all (a stride of 0) can be that many; blocks of 256 queries and tiles of 64 keys are counted past the
+    last of them."""
+    for rows in (2 ** 31 - 512, 2 ** 31 - 511, 2 ** 31 - 256, 2 ** 31 - 63, 2 ** 31 - 1):
+        fits = rows + 256 + 64 < 2 ** 31 and rows <= 2 ** 31 - 512
+        # (what is taken goes on to ask for its workspace, or finds too many blocks)
+        assert _packed(L, k_rows=rows, ldk=0, ldv=0, workspace=None) == (EWORKSPACE if fits else EUNSUPPORTED), rows
+        assert _packed(L, q_rows=rows, heads=4) == EUNSUPPORTED
