@@ -990,7 +990,8 @@ def latent_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, l
     included; token s sees rows 0 .. lengths[b] - S + s.  ``scale``: ``softmax_scale(config)``.  Returns
     (B, S, H, 512) bf16, the softmax-weighted sums of latents (times W_UV: the heads' outputs), and with
     ``return_lse`` the log of the sum of exp(scores), (B, S, H) fp32.  A token that sees no row gives
-    zeros and -inf; pages outside the pool hold no rows.  A length past the table counts as its end."""
+    zeros and -inf; pages outside the pool hold no rows.  A length past the table counts as its end.  A finite
+    score below -2^126 log 2 counts as not seen."""
     what = "latent_attention"
     latent, k_pe, scales = _latent_parts(cache, what)
     dev = latent.device

@@ -141,7 +141,9 @@ template <bool F8> struct Stage {
 // row whose scores pass m by 2^LAG later on (or that saw nothing in the first tile) has the workgroup do
 // its split once more, with m from all of it.
 constexpr float LAG = 60.f;
-constexpr float M_NONE = -1e30f;  // no row seen yet (finite: 2^(-inf - M_NONE) is 0)
+// No row seen yet.  Finite, so that 2^(-inf - M_NONE) is 0, below the scores that are told from none, and their difference
+// from it is finite.
+constexpr float M_NONE = -0x1p126f;
 
 // The lane, opaque to the compiler: what is derived from it is formed anew instead of held in a register
 // throughout the loop (there are none to spare).

@@ -417,7 +417,9 @@ int amla_latent_cache_read(const amla_latent_cache *cache, int64_t rows, const i
  * q (seqs, seq_len, heads, 576) bf16, strides in elements, unit stride within a
  * head; token s of sequence b sees rows 0 .. lengths[b] - seq_len + s (lengths:
  * DEVICE int32, the rows held with the new tokens').  A token that sees no row
- * gives zeros and lse = -inf.  Tables of up to 2^31 - 512 rows a sequence.
+ * gives zeros and lse = -inf.  Finite scores in units of log 2, with the row's
+ * exponent added, are held within -2^126 .. 2^126: what is below counts as not
+ * seen.  Tables of up to 2^31 - 512 rows a sequence.
  * out (seqs, seq_len, heads, 512) bf16, lse (seqs,
  * seq_len, heads) fp32 or NULL.  Any heads; the rows of one sequence are split
  * over workgroups whose sums meet in the workspace (16-byte aligned, scratch

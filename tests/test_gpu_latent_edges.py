@@ -78,3 +78,32 @@ def test_long_sequences_over_few_pages(fp8, H):
         want[b, 0], weight[b, 0] = p @ lat[rows], p @ lat[rows].abs()
     size = SCALE * (q.double().abs().flatten(0, 2) @ k.abs().T).max().item()
     check_attention(got, want, lse, want_lse, weight, size, f"fp8={fp8} H={H} long")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("B,H,cols", [(2, 3, 0), (100, 33, 0), (100, 64, 30), (100, 128, 30)])
+def test_scores_far_below_zero(fp8, B, H, cols):
+    """Every score -1e33, of the last rows, which are alike, or -2e33, of those before.  At this size scores a unit in the last
+    place apart are worlds apart in probability, and alike ones may differ by one: any mean of the last rows is right, so
+    d out is 2^-8 of it and 2^-10 more for the sums in between (and 2^-100 of the largest value: an e4m3 block's probabilities
+    end at 2^-123), and d lse 2^-20 of it."""
+    g = torch.Generator().manual_seed(H)
+    n, first = 300, 260
+    lat = torch.randn(n, 512, generator=g, dtype=torch.float64) * (1e12 if fp8 else 2.0 ** 57)
+    lat[:, 0] = -448 * 2.0 ** 32 if fp8 else -2.0 ** 57
+    lat[:first, 0] *= 1.0 if fp8 else 2.0
+    lat[:first, 1] = lat[0, 0]
+    lat[first:, 1] = 0
+    lat[first:] = lat[first].clone()
+    cache, table = cache_of([lat], [torch.zeros(n, 64, dtype=torch.float64)], fp8, 64, [n], g)
+    last = L.pool_values(cache)[0][L.places(table, 0, n - 1, 64, cache[0].shape[0])]
+    q = torch.zeros(B, 1, H, 576)
+    q[..., 0] = 2.0 ** 72 if fp8 else 2.0 ** 56
+    q[..., 1] = 2.0 ** 72 if fp8 else 0.0
+    table = _wider(table, max(cols, table.shape[1])).repeat(B, 1)
+    lengths = torch.full((B,), n, dtype=torch.int32)
+    print(f"[case] fp8={fp8} B={B} H={H}", flush=True)
+    got, lse = ops.latent_attention(to_dev(q.to(BF16)), to_dev(cache), to_dev(table), to_dev(lengths), 0.1, return_lse=True)
+    assert ((got.double().cpu() - last).abs() <= (2.0 ** -8 + 2.0 ** -10) * last.abs() + 2.0 ** -100 * last.abs().max()).all()
+    z = 0.1 * (last[0] + last[1]) * q[0, 0, 0, 0]
+    assert -1e34 < z < -1e32 and ((lse.double().cpu() - z).abs() <= 2.0 ** -20 * z.abs()).all()
