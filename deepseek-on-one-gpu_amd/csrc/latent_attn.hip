@@ -494,8 +494,12 @@ template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F
 }
 
 // The reference of a block of e4m3 probabilities, whose largest score is mx: m plus a whole number, so that the block's scale
-// is a power of two, and 2^(mx - ref) in 128 .. 256 (m's own row: 128, without rounding)
-AMLA_DEV float block_ref(float mx, float m) { return m + (floorf(__builtin_fmaxf(mx, M_NONE) - m) - 7.f); }
+// is a power of two, and 2^(mx - ref) in 128 .. 256 (m's own row: 128, without rounding).  From mx, not m + floor(mx - m) - 7:
+// beyond 2^27 the rounding of that sum alone is more than e4m3 has room for, beyond 2^29 more than an exponential has.
+AMLA_DEV float block_ref(float mx, float m) {
+  mx = __builtin_fmaxf(mx, M_NONE);
+  return mx - (__builtin_amdgcn_fractf(mx - m) + 7.f);
+}
 // Its scale for the matrix unit: 2^(ref - m), whole but for the rounding of ref
 AMLA_DEV int block_scale(float ref, float m) { return (int)__builtin_rintf(__builtin_fmaxf(ref - m, -123.f)) + 127; }
 // Slice S of the softmax, its row factors in ex:

@@ -107,3 +107,31 @@ def test_scores_far_below_zero(fp8, B, H, cols):
     assert ((got.double().cpu() - last).abs() <= (2.0 ** -8 + 2.0 ** -10) * last.abs() + 2.0 ** -100 * last.abs().max()).all()
     z = 0.1 * (last[0] + last[1]) * q[0, 0, 0, 0]
     assert -1e34 < z < -1e32 and ((lse.double().cpu() - z).abs() <= 2.0 ** -20 * z.abs()).all()
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("H,cols", [(3, 0), (64, 30), (128, 30)])
+def test_scores_far_apart(fp8, H, cols):
+    """Blocks of 32 rows of score z, of -1.75 z and of -0.375 z, z from 2^24 to 2^100: the first, which are alike, and nothing of
+    the others."""
+    g = torch.Generator().manual_seed(3)
+    n, B = 500, 100
+    lat = torch.randn(n, 512, generator=g, dtype=torch.float64)
+    kind = (torch.arange(n) // 32) % 3
+    loud = kind == 1
+    lat[loud] = lat[40].clone()
+    lat[:, 0] = torch.tensor([-1.75, 1.0, -0.375])[kind].double()
+    cache, table = cache_of([lat], [torch.zeros(n, 64, dtype=torch.float64)], fp8, 64, [n], g)
+    row = L.pool_values(cache)[0][L.places(table, 0, 40, 64, cache[0].shape[0])]
+    table = _wider(table, max(cols, table.shape[1])).repeat(B, 1)
+    q = torch.zeros(B, 1, H, 576)
+    each = torch.arange(B * H).view(B, H)
+    powers = each % 76 + 24
+    q[:, 0, :, 0] = torch.exp2(powers.float()) * (1 + each * 37 % 128 / 128.0)
+    lengths = torch.full((B,), n, dtype=torch.int32)
+    print(f"[case] fp8={fp8} H={H} far apart", flush=True)
+    got, lse = ops.latent_attention(to_dev(q.to(BF16)), to_dev(cache), to_dev(table), to_dev(lengths), 0.7, return_lse=True)
+    far = ((got.double().cpu() - row).abs() / ((2.0 ** -8 + 2.0 ** -10) * row.abs() + 2.0 ** -100)).amax((1, 3))
+    assert (far <= 1).all(), f"2^{sorted({int(p) for p in powers[~(far <= 1)]})}: {far.max().item()}"
+    z = 0.7 * q[:, 0, :, 0].double()
+    assert ((lse[:, 0].double().cpu() - z).abs() <= 2.0 ** -20 * z).all()
