@@ -1019,7 +1019,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     ``k`` (N, G, 128): kv_b's output (N, G, 256) goes in as two views.  Queries are the last tokens of
     their sequence: with ``causal`` row i of n sees key j of m where j <= i + m - n.  Returns (T, H, 128)
     bf16, with ``return_lse`` also the log of the sum of exp(scores) (T, H) fp32.  A row that sees no
-    key gives zeros and -inf.  Offsets are not checked on the host; they are clamped to the rows, and
+    key gives zeros and -inf; scores are taken up to 2^28 in magnitude.  Offsets are not checked on the host; they are clamped to the rows, and
     the output of rows in no sequence is left unset."""
     what = "packed_attention"
     _need_cuda(q, "q")

@@ -124,7 +124,8 @@ template <bool ROPE> struct PackedWave {
 };
 // The reference m is the maximum of the first tile that shows a row any key (itself, not a whole number above it: the
 // probability of the largest score, all there is where few keys are seen, is not rounded): fp32 and bf16 have the range for
-// sums up to 2^PA_LAG above it.  A row that passes it has the workgroup start over with m from all keys.
+// sums up to 2^PA_LAG above it.  A row that passes it has the workgroup start over with m from all keys.  The rounding of m,
+// half a unit in its last place, is in every exponent of its row: no more than 16 up to scores of 2^28, where the range ends.
 constexpr float PA_LAG = 60.f, PA_NONE = -1e30f;
 
 template <int OFS> AMLA_DEV u32x4 pa_read16(uint32_t addr) {
@@ -669,7 +670,9 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
     float inv = l == 0.f ? 0.f : 1.f / l;
     const int r = 32 * g + j32;
     const float lse2 = l == 0.f ? -INFINITY : w.m[g] + __builtin_amdgcn_logf(l);
-    if (part) {  // the row's largest value to 2^14 .. 2^15
+    // the row's largest value to 2^14 .. 2^15, or as near as inv times that power stays finite: all of them may be 0 where l is
+    // below 1 (by the rounding of m: down to 2^-16 for scores of 2^28)
+    if (part) {
       float top = 0.f;
 #pragma unroll
       for (int cb = 0; cb < 4; ++cb)
@@ -687,7 +690,8 @@ __global__ __launch_bounds__(256, 1) void packed_attn_kernel(PackedParams p) {
       }
       const auto sx = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = __builtin_fmaxf(__uint_as_float(sx[0]), __uint_as_float(sx[1])) * inv;
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 240) - 14;
+      const int least = max((int)(__float_as_uint(inv) >> 23) - 112, 15);
+      const int e = min(max((int)(__float_as_uint(top) >> 23), least), 240) - 14;
       inv *= __uint_as_float((uint32_t)(254 - e) << 23);
       if (hh == 0) {
         float *ls = p.part_ls + 2 * (slot * PA_QB + 64 * wave + r);

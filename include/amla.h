@@ -440,7 +440,8 @@ size_t amla_latent_attention_workspace_bytes(int64_t seqs, int64_t seq_len, int6
  * unit stride within a head; heads / kv_heads heads share keys and values.
  * out (q_rows, heads, 128) bf16 and lse (q_rows, heads) fp32 or NULL, contiguous;
  * a row that sees no key gives zeros and -inf, rows of no sequence are not
- * written.  Up to 2^31 - 512 rows of q and of k. */
+ * written.  Up to 2^31 - 512 rows of q and of k; scores (scale times the product)
+ * of up to 2^28 in magnitude. */
 typedef struct amla_packed_args {
   const void *q, *k, *v, *k_pe;
   void *out;
