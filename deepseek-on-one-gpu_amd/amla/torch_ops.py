@@ -585,9 +585,11 @@ def _lc_rows(x: Tensor) -> Tensor:
         "Tensor block_table, Tensor position, Tensor? offsets, float eps) -> ()", lambda *args: None)
 def _latent_cache_write(kv, weight, freqs, latent, k_pe, scales, block_table, position, offsets, eps):
     kv, weight = _lc_rows(kv), _rows16(weight)
-    rows = kv.shape[0]
+    rows, width = kv.shape
+    if rows > 1 and kv.stride(0) < width:  # rows that share memory
+        kv = kv.clone(memory_format=torch.contiguous_format)
     check(lib().amla_latent_cache_write(_lc_cache(latent, k_pe, scales, block_table), kv.data_ptr(), rows,
-                                        kv.stride(0) if rows > 1 else kv.shape[1], weight.data_ptr(), eps,
+                                        kv.stride(0) if rows > 1 else width, weight.data_ptr(), eps,
                                         freqs.data_ptr(), freqs.shape[0], _ptr(offsets), block_table.shape[0],
                                         position.data_ptr(), _mx_stream(kv)), "latent_cache_write")
     for t in (latent, k_pe, scales):

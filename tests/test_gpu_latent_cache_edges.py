@@ -29,3 +29,21 @@ def test_conjugated_angles(fp8):
     lat, pe = _stored(kv.to(DEV), gamma.to(DEV), freqs.to(DEV).conj(), fp8, 2, 7)
     turned = freqs.conj().resolve_conj()
     _check_rows(lat, pe, kv.reshape(-1, 576), gamma, turned[:7].repeat(2, 1), 1e-6, fp8, "conjugated")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+def test_rows_that_share_memory(fp8):
+    """The same rows for every sequence (an expanded tensor), one row for all, and rows that overlap."""
+    g = torch.Generator().manual_seed(5)
+    gamma, freqs = _gamma(g).to(DEV), _freqs(32).to(DEV)
+    for kv in (_kv(g, 1, 5).to(DEV).expand(3, 5, 576), _kv(g, 1, 1).to(DEV).expand(3, 1, 576), _kv(g, 1, 1).to(DEV).expand(3, 5, 576),
+               _kv(g, 1, 3).to(DEV).flatten().as_strided((3, 1, 576), (64, 64, 1))):
+        rows = kv.shape[1]
+        print(f"[case] fp8={fp8} strides {kv.stride()}", flush=True)
+        lat, pe = _stored(kv, gamma, freqs, fp8, 3, rows)
+        want = _stored(kv.contiguous(), gamma, freqs, fp8, 3, rows)
+        assert torch.equal(lat, want[0]) and torch.equal(pe, want[1])
+        packed = kv.flatten(0, 1) if rows == 1 else kv.reshape(-1, 576)
+        off = torch.arange(4, dtype=torch.int32, device=DEV) * rows
+        lat, pe = _stored(packed, gamma, freqs, fp8, 3, rows, offsets=off)
+        assert torch.equal(lat, want[0]) and torch.equal(pe, want[1])
