@@ -570,11 +570,11 @@ def _lc_cache(latent, k_pe, scales, block_table) -> LatentCache:
                        cols, latent.shape[0], latent.shape[1])
 
 
-def _lc_rows(x: Tensor) -> Tensor:
-    """x itself when its rows are 16-byte aligned with unit stride, else a copy of such."""
+def _lc_rows(x: Tensor, most: int = 1 << 62) -> Tensor:
+    """x itself when its rows are 16-byte aligned with unit stride and at most ``most`` values apart, else a copy of such."""
     if x.stride(-1) == 1 and x.data_ptr() % 16 == 0:
         for s in x.stride()[:-1]:
-            if s % 8:
+            if s % 8 or s > most:
                 break
         else:
             return x
@@ -649,6 +649,9 @@ def _latent_attention(q, latent, k_pe, scales, block_table, lengths, scale, lse)
     return out, lse_out
 
 
+_PACKED_STRIDE = 1 << 27  # what the C entry takes
+
+
 def _packed_attention_fake(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse):
     rows, H, _ = q.shape
     return q.new_empty(rows, H, v.shape[2]), q.new_empty((rows, H) if lse else (0,), dtype=torch.float32)
@@ -657,8 +660,8 @@ def _packed_attention_fake(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse
 @_lc_op("packed_attention(Tensor q, Tensor k, Tensor v, Tensor? k_pe, Tensor offsets, Tensor? k_offsets, float scale, "
         "bool causal, bool lse) -> (Tensor, Tensor)", _packed_attention_fake)
 def _packed_attention(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse):
-    q, k, v = _lc_rows(q), _lc_rows(k), _lc_rows(v)
-    k_pe = None if k_pe is None else _lc_rows(k_pe)
+    q, k, v = _lc_rows(q, _PACKED_STRIDE), _lc_rows(k, _PACKED_STRIDE), _lc_rows(v, _PACKED_STRIDE)
+    k_pe = None if k_pe is None else _lc_rows(k_pe, _PACKED_STRIDE)
     out, lse_out = _packed_attention_fake(q, k, v, k_pe, offsets, k_offsets, scale, causal, lse)
     if not out.numel():
         return out, lse_out

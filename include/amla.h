@@ -436,8 +436,8 @@ size_t amla_latent_attention_workspace_bytes(int64_t seqs, int64_t seq_len, int6
  * key j of m where j <= i + m - n, else all m.
  * q (q_rows, heads, dk) with dk = dn + (k_pe ? 64 : 0), dn 128 or 192 (k_pe: 128
  * only), k (k_rows, kv_heads, dn), v (k_rows, kv_heads, 128), k_pe (k_rows, 64)
- * shared by all heads, all bf16 with strides in elements (multiples of 8) and
- * unit stride within a head; heads / kv_heads heads share keys and values.
+ * shared by all heads, all bf16 with strides in elements (multiples of 8, up to
+ * 2^27) and unit stride within a head; heads / kv_heads heads share keys and values.
  * out (q_rows, heads, 128) bf16 and lse (q_rows, heads) fp32 or NULL, contiguous;
  * a row that sees no key gives zeros and -inf, rows of no sequence are not
  * written.  Up to 2^31 - 512 rows of q and of k; scores (scale times the product)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from _latent import to_dev
+from _latent import BF16, DEV, to_dev
 from amla import ops
 from test_gpu_packed_attention import _case
 
@@ -46,3 +46,19 @@ def test_scores_far_from_zero(form, H, past, sign):
     assert z.abs().max() < 2.0 ** 28 and z.abs().min() >= 2.0 ** 19
     alike = torch.arange(2 * n) % n + past + 1 - torch.where(first, 0, low)
     assert ((lse.double().cpu() - z - alike.double().log()[:, None]).abs() <= 2.0 ** -20 * z.abs()).all()
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "pe"])
+def test_rows_further_apart_than_the_kernel_counts(which):
+    """Rows 2^27 + 8 values apart, like rows with any other stride that it does not take."""
+    q, k, v, pe, off, koff, scale = _case(12, [2, 1], [2, 1], 2, 2, "mla")
+    t = {n: to_dev(x) for n, x in zip(("q", "k", "v", "pe"), (q, k, v, pe))}
+    call = lambda: ops.packed_attention(t["q"], t["k"], t["v"], to_dev(off), scale, k_pe=t["pe"], k_offsets=to_dev(koff))  # noqa: E731
+    want = call()
+    rows, apart = t[which], 2 ** 27 + 8
+    store = torch.empty(2 * apart + rows[0].numel(), dtype=BF16, device=DEV)
+    far = store.as_strided(rows.shape, (apart, *rows[0].contiguous().stride()))
+    far.copy_(rows)
+    t[which] = far
+    print(f"[case] far {which}", flush=True)
+    assert torch.equal(call(), want)
