@@ -313,7 +313,7 @@ def call(name: str, t: Tensor, *args):
     return _on_device(_mx_impl[name], t, *args)
 
 
-_PLAIN_TYPES = frozenset((Tensor, torch.nn.Parameter, type(None), bool))  # of an operator's arguments
+_PLAIN_TYPES = frozenset((Tensor, torch.nn.Parameter, type(None), bool, int, float))  # of an operator's arguments
 
 
 def _intercepted(*args) -> bool:
