@@ -920,8 +920,8 @@ def latent_cache_write(kv: torch.Tensor, kv_a_layernorm: torch.Tensor, rope_freq
     sequence.  ``rope_freqs``: ``precompute_rope_freqs``.  ``cache``: ``latent_cache``; row i of
     sequence b is row i % page_size of page ``block_table[b, i // page_size]`` ((B, n) int32 on the
     device).  All in fp32 with one rounding, to bf16 or to e4m3 with the smallest power of two that
-    keeps the row within 448 times it (2^-32 .. 2^32); a row with an infinity or a NaN becomes one of
-    NaN.  Rows of no sequence, of a page outside the pool or past the rope table are not written;
+    keeps the row within 448 times it (2^-32 .. 2^32); an e4m3 row with an infinity or a NaN becomes one
+    of NaN (bf16: what the formula gives, zeros beside a NaN for an infinity).  Rows of no sequence, of a page outside the pool or past the rope table are not written;
     nothing of that is checked on the host.  Two rows of a call must not share a place."""
     what = "latent_cache_write"
     latent, k_pe, scales = _latent_parts(cache, what)

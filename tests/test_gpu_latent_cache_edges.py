@@ -47,3 +47,20 @@ def test_rows_that_share_memory(fp8):
         off = torch.arange(4, dtype=torch.int32, device=DEV) * rows
         lat, pe = _stored(packed, gamma, freqs, fp8, 3, rows, offsets=off)
         assert torch.equal(lat, want[0]) and torch.equal(pe, want[1])
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+def test_rows_with_values_that_are_no_numbers(fp8):
+    """e4m3: a row of NaN.  bf16: what the formula gives, 0 beside an infinity (1 / rms is 0) and NaN in its place, a row of
+    NaN for a NaN.  Rope keys: the pair of such a value only."""
+    g = torch.Generator().manual_seed(9)
+    kv, gamma, freqs = _kv(g, 1, 4), _gamma(g).to(DEV), _freqs(32).to(DEV)
+    clean = _stored(kv.to(DEV), gamma, freqs, fp8, 1, 4)
+    kv[0, 1, 77], kv[0, 2, 300], kv[0, 3, 520] = float("inf"), float("nan"), float("nan")
+    print(f"[case] fp8={fp8} no numbers", flush=True)
+    lat, pe = _stored(kv.to(DEV), gamma, freqs, fp8, 1, 4)
+    assert torch.equal(lat[[0, 3]], clean[0][[0, 3]]) and torch.equal(pe[:3], clean[1][:3])
+    assert torch.isnan(pe[3, 8:10]).all() and torch.equal(pe[3, 10:], clean[1][3, 10:]) and torch.equal(pe[3, :8], clean[1][3, :8])
+    assert torch.isnan(lat[2]).all() and torch.isnan(lat[1, 77])
+    rest = torch.arange(512, device=DEV) != 77
+    assert torch.isnan(lat[1, rest]).all() if fp8 else (lat[1, rest] == 0).all()
