@@ -135,3 +135,123 @@ def test_scores_far_apart(fp8, H, cols):
     assert (far <= 1).all(), f"2^{sorted({int(p) for p in powers[~(far <= 1)]})}: {far.max().item()}"
     z = 0.7 * q[:, 0, :, 0].double()
     assert ((lse[:, 0].double().cpu() - z).abs() <= 2.0 ** -20 * z).all()
+
+
+
+def _many(lat, pe, fp8, B, g, cols=0):
+    """(cache, table (B, .), lengths, the lengths there are): B sequences over the same pages, so that a workgroup's split has
+    several tiles; every third one is shorter by 37 rows, every third by 100."""
+    n = lat.shape[0]
+    cache, table = cache_of([lat], [pe], fp8, 64, [n], g, junk=float("nan"))
+    table = _wider(table, max(cols, table.shape[1]))
+    kinds = torch.tensor([n, n - 37, n - 100], dtype=torch.int32)
+    return cache, table.repeat(B, 1), kinds[torch.arange(B) % 3], kinds
+
+
+def _check_many(q, cache, table, lengths, scale, what):
+    """The same queries for every sequence: the first three against the definition, the others the same up to where their
+    splits begin."""
+    B = table.shape[0]
+    print(f"[case] {what}", flush=True)
+    qs = to_dev(q).expand(B, -1, -1, -1)
+    run = lambda: ops.latent_attention(qs, to_dev(cache), to_dev(table), to_dev(lengths), scale, return_lse=True)  # noqa: E731
+    got, lse = run()
+    few = q.expand(3, -1, -1, -1), cache, table[:3], lengths[:3], scale
+    want, want_lse = L.latent_attention(*few)
+    weight, size = _weight(*few)
+    for b in range(0, B, 90):
+        k = min(90, B - b)
+        some = torch.arange(k) % 3
+        check_attention(got[b:b + k], want[some], lse[b:b + k], want_lse[some], weight[some], size, f"{what}, from {b}")
+    again = run()
+    assert torch.equal(again[0], got) and torch.equal(again[1], lse), what
+    return got
+
+
+# query rows: one group of the kernel for few of them, several of those, two groups of it, four groups of the other one
+KERNELS = [(1, 32, 0), (1, 72, 0), (1, 64, 40), (1, 128, 40), (3, 8, 0), (3, 20, 40), (3, 43, 40)]
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", KERNELS)
+def test_a_reference_that_is_set_anew(fp8, S, H, cols):
+    """Scores that rise by up to 70 in log2 from one tile of a split to the next: sequences of five to 13 tiles, and so many of
+    them that a split has up to five."""
+    g = torch.Generator().manual_seed(H)
+    n = 400
+    for rising in (True, False):
+        ramp = torch.linspace(0, 60, n, dtype=torch.float64)
+        lat = 0.02 * torch.randn(n, 512, generator=g, dtype=torch.float64)
+        lat[:, 0] = ramp if rising else ramp.flip(0)
+        cache, table, lengths, _ = _many(lat, torch.zeros(n, 64, dtype=torch.float64), fp8, 270 * 64 // min(H * S, 64), g, cols)
+        q = torch.zeros(1, S, H, 576)
+        q[..., 0] = torch.linspace(0.1, 10, S * H).view(S, H)
+        _check_many(q.to(BF16), cache, table, lengths, 0.5, f"fp8={fp8} S={S} H={H} rising={rising}")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", [k for k in KERNELS if k[0] > 1])
+def test_a_masked_row_that_is_no_number_where_the_reference_is_set_anew(fp8, S, H, cols):
+    g = torch.Generator().manual_seed(5 * H)
+    n, B = 400, 270 * 64 // min(H * S, 64)
+    lat = 0.02 * torch.randn(n, 512, generator=g, dtype=torch.float64)
+    lat[:, 0] = torch.linspace(0, 60, n, dtype=torch.float64)
+    cache, table, _, _ = _many(lat, torch.zeros(n, 64, dtype=torch.float64), fp8, B, g, cols)
+    lengths = torch.full((B,), n, dtype=torch.int32)
+    q = torch.zeros(1, S, H, 576)
+    q[..., 0] = torch.linspace(0.1, 10, S * H).view(S, H)
+    want = _check_many(q.to(BF16), cache, table, lengths, 0.5, f"fp8={fp8} S={S} H={H}")
+    page, at = table[0, (n - 1) // 64], (n - 1) % 64
+    if fp8:
+        cache[0].view(torch.uint8)[page, at, 300] = 0x7F
+    else:
+        cache[0][page, at, 300] = float("inf")
+    qs = to_dev(q.to(BF16)).expand(B, -1, -1, -1)
+    got = ops.latent_attention(qs, to_dev(cache), to_dev(table), to_dev(lengths), 0.5)
+    assert torch.equal(got[:, :S - 1], want[:, :S - 1]) and torch.isnan(got[:, S - 1]).all()
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", [k for k in KERNELS if k[0] == 1])
+def test_rows_of_unlike_scales_in_splits_of_several_tiles(fp8, S, H, cols):
+    g = torch.Generator().manual_seed(4 + H)
+    n = 433
+    lat = torch.randn(n, 512, generator=g, dtype=torch.float64) * torch.exp2(torch.randint(-12, 13, (n, 1), generator=g).double())
+    lat[5] = 0
+    cache, table, lengths, _ = _many(lat, torch.randn(n, 64, generator=g, dtype=torch.float64), fp8, 270 * 64 // min(H, 64), g, cols)
+    q = (torch.randn(1, S, H, 576, generator=g) * 1e-3).to(BF16)
+    _check_many(q, cache, table, lengths, SCALE, f"fp8={fp8} H={H} unlike scales")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("H,cols", [(32, 0), (64, 200), (128, 200)])
+def test_many_faint_rows_outweigh_one_loud_in_splits_of_several_tiles(fp8, H, cols):
+    """One row 2^15 and 2^24 times as probable as each of 5000 others, 12 sequences: splits of four tiles and more."""
+    g = torch.Generator().manual_seed(18)
+    n, B = 5000, 12
+    for at in (0, 17, 4000):
+        lat = 0.2 * torch.randn(n, 512, generator=g, dtype=torch.float64)
+        lat[:, 1], lat[:, 0] = 1.0, 0.0
+        lat[at, 0], lat[at, 1] = 8.0, -1.0
+        cache, table, lengths, _ = _many(lat, torch.zeros(n, 64, dtype=torch.float64), fp8, B, g, cols)
+        q = torch.zeros(1, 1, H, 576)
+        q[..., 0] = torch.tensor([15.0, 24.0]).repeat(H // 2) * 0.6931 / 8.0
+        _check_many(q.to(BF16), cache, table, lengths, 1.0, f"fp8={fp8} H={H} loud row {at}")
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", KERNELS)
+def test_the_mean_error_is_that_of_two_roundings(fp8, S, H, cols):
+    """The output is rounded to 8 bits, and so is each probability, whose errors are independent of each other: an rms error of
+    at most 2^-8 / sqrt(3) of the values from either (half a step is 2^-8 of a power of two, and no value is below its own),
+    0.0032 together.  Of values spread evenly over an octave it is 0.0022; one bit less in either place makes that 0.0034."""
+    g = torch.Generator().manual_seed(H + S)
+    n = 700
+    cache, table, lengths, _ = _many(torch.randn(n, 512, generator=g, dtype=torch.float64), torch.randn(n, 64, generator=g, dtype=torch.float64),
+                                     fp8, 60, g, cols)
+    q = (torch.randn(1, S, H, 576, generator=g) * 0.6).to(BF16)
+    got = _check_many(q, cache, table, lengths, SCALE, f"fp8={fp8} S={S} H={H} rms")
+    want, _ = L.latent_attention(q.expand(3, -1, -1, -1), cache, table[:3], lengths[:3], SCALE)
+    for b in range(0, 60, 3):
+        rms = (got[b:b + 3].double().cpu() - want).square().mean().sqrt() / want.square().mean().sqrt()
+        assert rms <= 2.0 ** -8 * (2 / 3) ** 0.5, f"{b}: {rms.item():.5f}"

@@ -1,12 +1,76 @@
-"""packed_attention at its edges."""
+"""packed_attention at its edges: rows of no sequence, many sequences whose keys are split, far strides, scores far from zero."""
+import ctypes
+
 import pytest
 import torch
 
-from _latent import BF16, DEV, to_dev
-from amla import ops
-from test_gpu_packed_attention import _case
+from _latent import BF16, DEV, check_attention, to_dev
+from amla import _lib, ops
+from oracle import ref_latent as L
+from test_gpu_packed_attention import _case, _run
 
 pytestmark = pytest.mark.gpu
+
+
+def _split_keys(T, N, B, H):
+    return _lib.lib().amla_packed_attention_workspace_bytes(T, N, B, H) > 0
+
+
+def _entry(q, k, v, pe, off, koff, scale, out, lse):
+    """The C entry, with the caller's outputs."""
+    T, H, N, B = q.shape[0], q.shape[1], k.shape[0], off.shape[0] - 1
+    need = _lib.lib().amla_packed_attention_workspace_bytes(T, N, B, H)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    args = _lib.PackedArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), None if pe is None else pe.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                           off.data_ptr(), koff.data_ptr(), T, N, B, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
+                           v.stride(1), 0 if pe is None else pe.stride(0), H, k.shape[1], k.shape[2], 1, scale, ws.data_ptr(), need)
+    assert _lib.lib().amla_packed_attention(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("form,H,lens,split", [("mla", 4, [20, 300, 0, 5], False), ("plain", 130, [20, 300, 0, 5], False),
+                                               ("mla", 4, [20, 300, 0, 5], True), ("whole", 2, [1, 0, 70], True)])
+@pytest.mark.parametrize("before,behind", [(0, 9), (7, 0), (33, 300)])
+def test_rows_of_no_sequence_keep_their_bits(form, H, lens, split, before, behind):
+    """Rows before the first sequence and behind the last, and what lies around the outputs, are not written; the sequences'
+    own are what they are without such rows."""
+    past = [1500, 100, 800, 64][:len(lens)] if split else [0, 9, 0, 30]
+    held = [a + b for a, b in zip(lens, past)]
+    q, k, v, pe, off, koff, scale = _case(before + H, lens, held, H, H, form)
+    T = before + sum(lens) + behind
+    wide = torch.randn(T, H, q.shape[2]).to(BF16)
+    wide[before:before + sum(lens)] = q
+    assert _split_keys(T, sum(held), len(lens), H) == split
+    print(f"[case] {form} {before} + {lens} + {behind} split={split}", flush=True)
+    guard = 3 * H
+    out = torch.full((guard + T * H + guard, 128), 7.0, dtype=BF16, device=DEV)
+    lse = torch.full((guard + T * H + guard,), 7.0, device=DEV)
+    _entry(to_dev(wide), to_dev(k), to_dev(v), to_dev(pe), to_dev(off + before), to_dev(koff), scale, out[guard:], lse[guard:])
+    at = slice(guard + before * H, guard + (before + sum(lens)) * H)
+    outside = torch.ones(out.shape[0], dtype=torch.bool, device=DEV)
+    outside[at] = False
+    assert (out[outside] == 7.0).all() and (lse[outside] == 7.0).all()
+    want, want_lse = L.packed_attention(q, k, v, off, scale, koff, pe)
+    weight, _ = L.packed_attention(q, k, v.abs(), off, scale, koff, pe)
+    kk = k if pe is None else torch.cat([k, pe[:, None].expand(-1, H, -1)], -1)
+    size = scale * max((q[:, h].double().abs() @ kk[:, h].double().abs().T).max().item() for h in range(H))
+    check_attention(out[at].view(-1, H, 128), want, lse[at].view(-1, H), want_lse, weight, size, f"{form} {before} {behind}")
+
+
+@pytest.mark.parametrize("form,H", [("plain", 1), ("mla", 2)])
+def test_split_keys_of_more_sequences_than_a_wave_has_lanes(form, H):
+    """70 sequences, of one query but for four of none and two of 300, and up to 900 keys."""
+    n = 70 if H == 1 else 66
+    new = [0 if b in (3, 63, 64, n - 2) else 1 for b in range(n)]
+    if H == 1:
+        new[20], new[n - 1] = 300, 300
+    past = [(131 * b) % 900 for b in range(n)]
+    lens = [a + b for a, b in zip(new, past)]
+    if H == 2:
+        new, lens = new[2:], lens[2:]
+    assert len(new) >= 64 and _split_keys(sum(new), sum(lens), len(new), H)
+    _run(*_case(51, new, lens, H, H, form), what=f"{form} {len(new)} sequences, split")
+    _run(*_case(52, new, lens, H, H, form), causal=False, what=f"{form} {len(new)} sequences, split, not causal")
 
 
 @pytest.mark.parametrize("sign", [1, -1])
@@ -62,3 +126,15 @@ def test_rows_further_apart_than_the_kernel_counts(which):
     t[which] = far
     print(f"[case] far {which}", flush=True)
     assert torch.equal(call(), want)
+
+
+@pytest.mark.parametrize("form,H,new,past", [("mla", 4, [600], [0]), ("plain", 8, [300, 7], [0, 90]), ("whole", 2, [5], [4000])])
+def test_the_mean_error_is_that_of_two_roundings(form, H, new, past):
+    """Of the output and of the probabilities, 2^-8 / sqrt(3) of the values at most each (as in the cache's attention)."""
+    lens = [a + b for a, b in zip(new, past)]
+    case = _case(15, new, lens, H, H, form)
+    got, _ = _run(*case, what=f"{form} rms")
+    q, k, v, pe, off, koff, scale = case
+    want, _ = L.packed_attention(q, k, v, off, scale, koff, pe)
+    rms = (got.double().cpu() - want).square().mean().sqrt() / want.square().mean().sqrt()
+    assert rms <= 2.0 ** -8 * (2 / 3) ** 0.5, f"{rms.item():.5f}"
