@@ -299,9 +299,9 @@ template <bool F8> constexpr int q_reg(int f) {
 }
 static_assert(Stage<true>::LDS <= 160 * 1024 && Stage<false>::LDS <= 160 * 1024);
 
-template <bool F8, int HG> struct Wave {
+template <bool F8> struct Wave {
   static constexpr int KB = Tile<F8>::ROWS / 32;  // 32-row blocks of a tile
-  static constexpr int CG = 4 / HG, NCB = 16 / CG;
+  static constexpr int NCB = 16;                  // 32-column blocks of a row
   bf16x8 q[32 - Stage<F8>::QL], qr[F8 ? 1 : 4];  // the rest at qra in LDS, 1 KB a fragment
   uint32_t qra;
   f32x16 o[NCB];  // O^T: columns x queries
@@ -335,7 +335,7 @@ template <bool F8> constexpr int score_reads(int i) {
 }
 // Steps that reads go out ahead: as many as the registers allow (an LDS read returns after 300 - 400 cycles with
 // four waves reading; two steps of bf16 are 128 cycles of products)
-template <bool F8, int HG> constexpr int score_ahead() { return F8 ? 2 : 3; }
+template <bool F8> constexpr int score_ahead() { return F8 ? 2 : 3; }
 template <bool F8> constexpr int score_reads(int first, int last) {
   int n = 0;
   for (int i = first; i <= last; ++i) n += score_reads<F8>(i);
@@ -351,12 +351,12 @@ template <bool F8, int N, int I = 0> AMLA_DEV void score_reads_first(u32x4 (*ka)
 // x0, y0: the step's first fragments; e4m3: converted in the step before (a conversion of four instructions fits under each
 // MFMA; all sixteen of a step in front of its four MFMAs cost 5900 cycles a tile, not 3900, and one right before the product
 // that takes it two wait states each time)
-template <bool F8, int HG, int I>
-AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, bf16x8 y0,
+template <bool F8, int I>
+AMLA_DEV void score_step(Wave<F8> &w, u32x4 (&ka)[score_ahead<F8>() + 1][3], uint32_t kl, uint32_t kr, bf16x8 x0, bf16x8 y0,
                          float f0, float f1, uint2 lanes, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next, int r0) {
   constexpr int N = 16 + (F8 ? 4 : 2);  // steps over the latent and the rope key
   if constexpr (I < N) {
-    constexpr int AHEAD = score_ahead<F8, HG>(), c = I % (AHEAD + 1), n = (I + 1) % (AHEAD + 1);
+    constexpr int AHEAD = score_ahead<F8>(), c = I % (AHEAD + 1), n = (I + 1) % (AHEAD + 1);
     if constexpr (I + AHEAD < N) score_read<F8, I + AHEAD>(ka[(I + AHEAD) % (AHEAD + 1)], kl, kr, w.qra);
     constexpr int r0q = q_reg<F8>(I < 16 ? 2 * I : 0), r1q = q_reg<F8>(I < 16 ? 2 * I + 1 : 0);
     const bf16x8 qa = w.q[r0q], qb = score_reads<F8>(I) == 3 ? as_bf16x8(ka[c][2]) : w.q[r1q];
@@ -401,14 +401,14 @@ AMLA_DEV void score_step(Wave<F8, HG> &w, u32x4 (&ka)[score_ahead<F8, HG>() + 1]
       yn = as_bf16x8(ka[n][1]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    score_step<F8, HG, I + 1>(w, ka, kl, kr, xn, yn, f0, f1, lanes, next, pg, st_next, r0);
+    score_step<F8, I + 1>(w, ka, kl, kr, xn, yn, f0, f1, lanes, next, pg, st_next, r0);
   }
 }
 
 // S^T of the tile whose stage is at LDS address base, with the copies of a later tile spread between.
 // Two chains of MFMAs: one alone runs at two thirds of the rate.
-template <bool F8, int HG>
-AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next,
+template <bool F8>
+AMLA_DEV void score_phase(Wave<F8> &w, uint32_t base, const Rows<F8> &next, const LatentPages &pg, uint8_t *st_next,
                           int r0) {
   using T = Tile<F8>;
   using G = Stage<F8>;
@@ -421,7 +421,7 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f0) : "v"(base + 4 * j32), "i"(G::MUL) : "memory");
     asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(f1) : "v"(base + 4 * j32), "i"(G::MUL + 128) : "memory");
   }
-  constexpr int AHEAD = score_ahead<F8, HG>();
+  constexpr int AHEAD = score_ahead<F8>();
   u32x4 ka[AHEAD + 1][3];
   score_reads_first<F8, AHEAD>(ka, kl, kr, w.qra);
   lds_wait<score_reads<F8>(1, AHEAD - 1)>();
@@ -429,15 +429,15 @@ AMLA_DEV void score_phase(Wave<F8, HG> &w, uint32_t base, const Rows<F8> &next, 
   if constexpr (score_reads<F8>(0) == 3) lds_tie(ka[0][2]);
   const bf16x8 x0 = F8 ? codes_to_bf16(ka[0][0].x, ka[0][0].y, f0) : as_bf16x8(ka[0][0]);
   const bf16x8 y0 = F8 ? codes_to_bf16(ka[0][1].x, ka[0][1].y, f1) : as_bf16x8(ka[0][1]);
-  score_step<F8, HG, 0>(w, ka, kl, kr, x0, y0, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
+  score_step<F8, 0>(w, ka, kl, kr, x0, y0, f0, f1, Rows<F8>::lanes(r0), next, pg, st_next, r0);
   // the results are read by vector code that the compiler schedules: cover the asm's write-to-read wait states
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(w.s[0]), "+v"(w.s[1])::"memory");
 }
 
 // The second phase of a tile goes in steps of one 32-column block of the values; each carries some of the
 // slices (four rows) of the softmax: first all scaled scores and their maxima, then the probabilities.
-template <bool F8, int HG> struct Slices {
-  static constexpr int KB = Wave<F8, HG>::KB, NCB = Wave<F8, HG>::NCB, NZ = 4 * KB, NS = 8 * KB;
+template <bool F8> struct Slices {
+  static constexpr int KB = Wave<F8>::KB, NCB = Wave<F8>::NCB, NZ = 4 * KB, NS = 8 * KB;
   static constexpr int PER = (NS + NCB - 1) / NCB;  // slices of a step, at most
   static constexpr int first(int c) { return (c * NS + NCB - 1) / NCB; }
   static constexpr int reads(int c) {  // row factors read for step c: bf16's probabilities need none
@@ -447,35 +447,35 @@ template <bool F8, int HG> struct Slices {
     return n;
   }
 };
-template <bool F8, int HG> struct StepReads {
+template <bool F8> struct StepReads {
   u32x2 v[4];
-  u32x4 ex[Slices<F8, HG>::PER];
+  u32x4 ex[Slices<F8>::PER];
 };
 constexpr int VALUE_AHEAD = 2;
-template <bool F8, int HG> struct ValueState {
-  static constexpr int KB = Wave<F8, HG>::KB;
+template <bool F8> struct ValueState {
+  static constexpr int KB = Wave<F8>::KB;
   uint32_t v0, v1, eb;
   float scale_log2;
   int lim;  // MASK: rows of the tile below lim are seen by the lane's query
   float mx[KB], ref[KB], sum[KB];
   i32x8 phi, plo;
   u32x4 pb[2];
-  StepReads<F8, HG> rd[VALUE_AHEAD + 1];
+  StepReads<F8> rd[VALUE_AHEAD + 1];
 };
 
-template <bool F8, int HG, int S, int END, int K = 0> AMLA_DEV void slice_read(ValueState<F8, HG> &x, StepReads<F8, HG> &r) {
+template <bool F8, int S, int END, int K = 0> AMLA_DEV void slice_read(ValueState<F8> &x, StepReads<F8> &r) {
   using G = Stage<F8>;
-  using L = Slices<F8, HG>;
+  using L = Slices<F8>;
   if constexpr (S < END) {
     constexpr int t = S % L::NZ;
     if constexpr (S < L::NZ || F8) r.ex[K] = lds_read16<(S < L::NZ ? G::EXP : G::INV) + 4 * (32 * (t >> 2) + 8 * (t & 3))>(x.eb);
-    slice_read<F8, HG, S + 1, END, K + 1>(x, r);
+    slice_read<F8, S + 1, END, K + 1>(x, r);
   }
 }
-template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F8, HG> &x) {
-  using L = Slices<F8, HG>;
+template <bool F8, bool ZP, int C> AMLA_DEV void value_read(ValueState<F8> &x) {
+  using L = Slices<F8>;
   if constexpr (C < L::NCB) {
-    StepReads<F8, HG> &r = x.rd[C % (VALUE_AHEAD + 1)];
+    StepReads<F8> &r = x.rd[C % (VALUE_AHEAD + 1)];
     if constexpr (F8) {
       const uint32_t a = x.v0 ^ (32 * (C & 7));
       r.v[0] = lds_read_tr<F8, 256 * (C >> 3)>(a);
@@ -489,7 +489,7 @@ template <bool F8, int HG, bool ZP, int C> AMLA_DEV void value_read(ValueState<F
       r.v[2] = lds_read_tr<F8, 256 * (C >> 2) + 16384>(a);
       r.v[3] = lds_read_tr<F8, 256 * (C >> 2) + 16384>(b);
     }
-    if constexpr (ZP) slice_read<F8, HG, L::first(C), L::first(C + 1)>(x, r);
+    if constexpr (ZP) slice_read<F8, L::first(C), L::first(C + 1)>(x, r);
   }
 }
 
@@ -507,8 +507,8 @@ AMLA_DEV int block_scale(float ref, float m) { return (int)__builtin_rintf(__bui
 // e4m3: 32 rows are one block of the matrix unit with a scale of its own, 2^(ref - m), so that rows far
 // below the sequence's maximum keep their bits: a reference for all would drop those below 2^-22 of it,
 // and thousands of them can outweigh it.
-template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8, HG> &w, ValueState<F8, HG> &x, u32x4 ex) {
-  using L = Slices<F8, HG>;
+template <bool F8, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8> &w, ValueState<F8> &x, u32x4 ex) {
+  using L = Slices<F8>;
   constexpr int KB = L::KB, t = S % L::NZ, kb = t >> 2, q4 = t & 3;
   f32x16 &z = w.s[kb];
   if constexpr (S < L::NZ) {
@@ -560,25 +560,25 @@ template <bool F8, int HG, bool MASK, int S> AMLA_DEV void softmax_slice(Wave<F8
     }
   }
 }
-template <bool F8, int HG, bool MASK, int S, int END, int K = 0>
-AMLA_DEV void softmax_slices(Wave<F8, HG> &w, ValueState<F8, HG> &x, StepReads<F8, HG> &r) {
+template <bool F8, bool MASK, int S, int END, int K = 0>
+AMLA_DEV void softmax_slices(Wave<F8> &w, ValueState<F8> &x, StepReads<F8> &r) {
   if constexpr (S < END) {
     u32x4 ex = {0, 0, 0, 0};
-    if constexpr (S < Slices<F8, HG>::NZ || F8) {
+    if constexpr (S < Slices<F8>::NZ || F8) {
       ex = r.ex[K];
       lds_tie(ex);
     }
-    softmax_slice<F8, HG, MASK, S>(w, x, ex);
-    softmax_slices<F8, HG, MASK, S + 1, END, K + 1>(w, x, r);
+    softmax_slice<F8, MASK, S>(w, x, ex);
+    softmax_slices<F8, MASK, S + 1, END, K + 1>(w, x, r);
   }
 }
 
-template <bool F8, int HG, bool MASK, bool ZP, int C>
-AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
-  using L = Slices<F8, HG>;
+template <bool F8, bool MASK, bool ZP, int C>
+AMLA_DEV void value_step(Wave<F8> &w, ValueState<F8> &x) {
+  using L = Slices<F8>;
   if constexpr (C < L::NCB) {
-    StepReads<F8, HG> &r = x.rd[C % (VALUE_AHEAD + 1)];
-    value_read<F8, HG, ZP, C + VALUE_AHEAD>(x);
+    StepReads<F8> &r = x.rd[C % (VALUE_AHEAD + 1)];
+    value_read<F8, ZP, C + VALUE_AHEAD>(x);
     // this step's reads have landed: those of the next two steps may be in flight
     lds_wait<4 * ((C + 1 < L::NCB) + (C + 2 < L::NCB)) + (ZP ? L::reads(C + 1) + L::reads(C + 2) : 0)>();
     // (locals, not members: a pass that sees the members in memory loads several at once, and then takes registers
@@ -587,38 +587,37 @@ AMLA_DEV void value_step(Wave<F8, HG> &w, ValueState<F8, HG> &x) {
     lds_tie(v0, v1, v2, v3);
     if constexpr (F8) mfma_value<false>(w.o[C], join(v0, v1, v2, v3), w.one, w.phi, w.ps);
     else mfma_value<false>(w.o[C], as_bf16x8(u32x4{v0.x, v0.y, v1.x, v1.y}), as_bf16x8(w.pb[0]));
-    if constexpr (ZP) softmax_slices<F8, HG, MASK, L::first(C), L::first(C + 1)>(w, x, r);
+    if constexpr (ZP) softmax_slices<F8, MASK, L::first(C), L::first(C + 1)>(w, x, r);
     if constexpr (F8) mfma_value<false>(w.o[C], join(v0, v1, v2, v3), w.one, w.plo, w.ps_lo);
     else mfma_value<false>(w.o[C], as_bf16x8(u32x4{v2.x, v2.y, v3.x, v3.y}), as_bf16x8(w.pb[1]));
     __builtin_amdgcn_sched_barrier(0);
-    value_step<F8, HG, MASK, ZP, C + 1>(w, x);
+    value_step<F8, MASK, ZP, C + 1>(w, x);
   }
 }
 
 // O^T += C^T P^T of the tile before (its stage at pv) while the scores of this tile (stage at zb; ZP) become
 // probabilities.
-template <bool F8, int HG, bool MASK, bool ZP>
-AMLA_DEV void value_phase(Wave<F8, HG> &w, uint32_t pv, uint32_t zb, int cg, float scale_log2, int lim) {
+template <bool F8, bool MASK, bool ZP>
+AMLA_DEV void value_phase(Wave<F8> &w, uint32_t pv, uint32_t zb, float scale_log2, int lim) {
   using T = Tile<F8>;
-  using L = Slices<F8, HG>;
-  constexpr int KB = L::KB, NCB = L::NCB;
+  using L = Slices<F8>;
+  constexpr int KB = L::KB;
   const int lane = fresh_lane(), hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
-  ValueState<F8, HG> x;
+  ValueState<F8> x;
   if constexpr (F8) {  // rows 16 i + 4 hh + {0..3, 8..11} of 16 columns
     const int r = 8 * (L16 >> 3) + 4 * hh + ((L16 >> 1) & 3);
     x.v0 = pv + r * T::RB + 16 * ((g16 & 1) ^ T::swz(r)) + 8 * (L16 & 1);
-    x.v0 = (x.v0 ^ (32 * ((NCB * cg) & 7))) + 256 * ((NCB * cg) >> 3);
   } else {   // rows 16 kk + 8 i + 4 hh + 0..3
     const int r = 4 * hh + (L16 >> 2), ch = 2 * (g16 & 1) + ((L16 >> 1) & 1);
-    x.v0 = pv + r * T::RB + 16 * (ch ^ T::swz(r)) + 8 * (L16 & 1) + 256 * ((NCB * cg) >> 2);
-    x.v1 = pv + (r + 8) * T::RB + 16 * (ch ^ T::swz(r + 8)) + 8 * (L16 & 1) + 256 * ((NCB * cg) >> 2);
+    x.v0 = pv + r * T::RB + 16 * (ch ^ T::swz(r)) + 8 * (L16 & 1);
+    x.v1 = pv + (r + 8) * T::RB + 16 * (ch ^ T::swz(r + 8)) + 8 * (L16 & 1);
   }
   x.eb = zb + 16 * hh;
   x.scale_log2 = scale_log2;
   x.lim = lim;
-  value_read<F8, HG, ZP, 0>(x);
-  value_read<F8, HG, ZP, 1>(x);
-  value_step<F8, HG, MASK, ZP, 0>(w, x);
+  value_read<F8, ZP, 0>(x);
+  value_read<F8, ZP, 1>(x);
+  value_step<F8, MASK, ZP, 0>(w, x);
   if constexpr (ZP) {
 #pragma unroll
     for (int k = 0; k < KB; ++k) w.l += F8 ? x.sum[k] * __builtin_amdgcn_exp2f(x.ref[k] - w.m) : x.sum[k];
@@ -842,21 +841,20 @@ template <int TILE> AMLA_DEV bool sees_none(const LatentPages &pg, const SplitWo
   return true;
 }
 
-// One workgroup of four waves per (sequence, chunk of 32 HG rows, split), HG = 4: a wave holds 32
+// One workgroup of four waves per (sequence, chunk of 128 rows, split): a wave holds 32
 // query rows, all of whose columns it sums up.  O^T fills half of its 512 registers, the queries
 // most of the others: one wave a SIMD, whose own products hide its conversions, copies, LDS
 // reads and softmax, each placed between two of them (one phase after the other took twice
 // as long).  What spills in the loop costs most: a reload waits behind all copies under way.
-template <bool F8, int HG, bool MASK>
+template <bool F8, bool MASK>
 __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p) {
   extern __shared__ __align__(1024) uint8_t sm[];
   using T = Tile<F8>;
   using G = Stage<F8>;
-  using W = Wave<F8, HG>;
-  constexpr int TILE = T::ROWS, CG = W::CG, NCB = W::NCB;
+  using W = Wave<F8>;
+  constexpr int TILE = T::ROWS, NCB = W::NCB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j32 = lane & 31, hh = lane >> 5;
-  const int hg = wave / CG, cg = wave % CG;
 
   const SplitWork at = split_work<F8>(p);
   if (at.b < 0) return;
@@ -870,7 +868,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
 
   // queries: B fragments, lane = row of the chunk, in the order of the score steps' reads
   W w;
-  const int row = (chunk * HG + hg) * 32 + j32;
+  const int row = (chunk * 4 + wave) * 32 + j32;
   const int rq = min(row, p.rows - 1), tok = rq / p.heads;
   const int limit = rows_held - (p.seq_len - 1 - tok) - 4 * hh;  // rows [0, limit + 4 hh) are seen
   const uint16_t *qp = p.q + b * p.ldq_seq + tok * p.ldq_token + (rq - tok * p.heads) * p.ldq_head;
@@ -908,11 +906,11 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
       const uint32_t before = base;
       feed.template arrive<MASK>(tile);
       base = lds0 + feed.cur * G::SIZE;
-      score_phase<F8, HG>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
-      value_phase<F8, HG, MASK, true>(w, before, base, cg, p.scale_log2, limit - tile * TILE);
+      score_phase<F8>(w, base, feed.next, p.pg, feed.next_stage(), Rows<F8>::WR * wave);
+      value_phase<F8, MASK, true>(w, before, base, p.scale_log2, limit - tile * TILE);
       feed.advance(tile);
     }
-    value_phase<F8, HG, MASK, false>(w, base, base, cg, p.scale_log2, 0);
+    value_phase<F8, MASK, false>(w, base, base, p.scale_log2, 0);
     settle(w.o);
     wait_vmcnt<0>();  // (copies past the last tile)
     const bool low = w.top > w.m + LAG;
@@ -937,7 +935,7 @@ __global__ __launch_bounds__(256, 1) void latent_attn_kernel(LatentAttnParams p)
   l += __shfl_xor(l, 32, 64);
   if constexpr (MASK) l = feed.odd < limit + 4 * hh ? __uint_as_float(0x7fc00000u) : l;
   if (__ballot(l != l)) l = sees_none<TILE>(p.pg, at, MASK ? limit + 4 * hh : INT32_MAX) ? 0.f : l;
-  store_split<HG>(p, sm, w.o, l, w.m, b, chunk, slot, splits, wave, hg, cg);
+  store_split<4>(p, sm, w.o, l, w.m, b, chunk, slot, splits, wave, wave, 0);
 }
 
 // ---------------------------------------------------------------- few query rows
@@ -1146,7 +1144,7 @@ template <bool F8, int QG, int C> AMLA_DEV void few_value_read(FewValues<F8, QG>
     }
   }
 }
-// Where the wave's columns 128 c .. of the values at pv begin: like value_phase of four column groups
+// Where the wave's columns 128 cg .. of the values at pv begin: the addresses of value_phase, so far on
 template <bool F8> AMLA_DEV uint2 few_value_addr(uint32_t pv, int cg) {
   using T = Tile<F8>;
   const int lane = threadIdx.x & 63, hh = lane >> 5, L16 = lane & 15, g16 = lane >> 4;
@@ -1451,7 +1449,7 @@ static int launch_attn(const LatentAttnParams &p, hipStream_t st) {
     kernel = p.seq_len > 1 ? latent_attn_few_kernel<F8, HG, true> : latent_attn_few_kernel<F8, HG, false>;
     lds = FewStage<F8, HG>::LDS;
   } else {
-    kernel = p.seq_len > 1 ? latent_attn_kernel<F8, HG, true> : latent_attn_kernel<F8, HG, false>;
+    kernel = p.seq_len > 1 ? latent_attn_kernel<F8, true> : latent_attn_kernel<F8, false>;
     lds = Stage<F8>::LDS;
   }
   int rc = latent_lds(kernel, "latent_attention");
