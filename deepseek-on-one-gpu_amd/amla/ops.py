@@ -991,7 +991,9 @@ def latent_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, l
     (B, S, H, 512) bf16, the softmax-weighted sums of latents (times W_UV: the heads' outputs), and with
     ``return_lse`` the log of the sum of exp(scores), (B, S, H) fp32.  A token that sees no row gives
     zeros and -inf; pages outside the pool hold no rows.  A length past the table counts as its end.  A finite
-    score below -2^126 log 2 counts as not seen."""
+    score below -2^126 log 2 counts as not seen.  The table's width, not the lengths, chooses the kernel (the
+    host does not know them): a much wider one costs short sequences up to half as much time again, and the
+    last bits of the result go with it."""
     what = "latent_attention"
     latent, k_pe, scales = _latent_parts(cache, what)
     dev = latent.device

@@ -4,7 +4,7 @@
 // exact in it), probabilities are rounded once for the matrix units: to bf16, or to two e4m3 halves that hold eight bits
 // of them (inference/ops.py:179 rounds them to bf16).  Every row of the cache serves all heads, so it is read once from
 // memory per 128 query rows and split of the sequence.  Many query rows: latent_attn_kernel, bound by the matrix units
-// (8 x 32768 rows, 128 heads, e4m3: 89 us where 73 GFLOP at a large product's rate take 61; the units are busy 42 % of
+// (8 x 32768 rows, 128 heads, e4m3: 83 - 89 us where 73 GFLOP at a large product's rate take 61; the units are busy 43 % of
 // the cycles, conversions, softmax and barriers take the others).  Few: latent_attn_few_kernel, bound by the copies (40
 // ragged sequences, 16 heads, bf16: 64 us for 342 MB; the copies alone take nine tenths).  Then latent_join_kernel.
 #include <algorithm>
@@ -31,7 +31,8 @@ struct LatentAttnParams {
   float *lse;
   // Of each split: its sums, normalised, (slots, rows of a chunk, 512) in fp16 times part_scale, a power of two for each of
   // the up to four waves that hold a row's columns; log2 of its sum of 2^s.  fp16 and not bf16, whose rounding would add as
-  // much error as the output's own; fp32 would be twice the bytes, a tenth of a long batch's time.
+  // much error as the output's own; fp32 would be twice the bytes, a tenth of a long batch's time.  (Columns below 2^-38 of the
+  // row's largest are lost; a row of codes spans 2^18.)
   uint16_t *part_o;
   float *part_lse, *part_scale;    // (slots, rows of a chunk), (slots, rows of a chunk, 4)
   int2 *part_plan;                 // (first slot, splits) of each sequence that has rows: the join need not plan again
@@ -621,7 +622,8 @@ AMLA_DEV void value_phase(Wave<F8> &w, uint32_t pv, uint32_t zb, float scale_log
   if constexpr (ZP) {
 #pragma unroll
     for (int k = 0; k < KB; ++k) w.l += F8 ? x.sum[k] * __builtin_amdgcn_exp2f(x.ref[k] - w.m) : x.sum[k];
-    // the scale of block k comes from the lanes of half k; 4 .. 160, the low halves' 4 less
+    // the scale of block k comes from the lanes of half k; 4 .. 180 (more only in a pass that is made again), the low
+    // halves' 4 less
     if constexpr (F8) {
       w.ps = block_scale(hh ? x.ref[KB - 1] : x.ref[0], w.m);
       w.ps_lo = w.ps - 4;
@@ -1422,7 +1424,9 @@ constexpr int LA_UNITS = 256;  // workgroups that run at a time (one per CU)
 // for few query rows.  Measured with 128 heads and one new token (1 / 2 / 4 groups, us), fp8: 1 x 257 rows 16 / 21 / 22,
 // 64 x 512 31 / 43 / 52, 4 x 8192 34 / 39 / 42, 8 x 8192 50 / 49 / 50, 32 x 4096 85 / 74 / 67, 8 x 32768 146 / 115 / 96;
 // bf16: 4 x 8192 36 / 38 / 42, 8 x 8192 50 / 46 / 51, 32 x 4096 85 / 70 / 73, 8 x 32768 149 / 108 / 106; 64 heads: 64 x 1024
-// fp8 39 / 43, 40 x 4096 65 / 59, bf16 69 / 59 (four groups half empty there).
+// fp8 39 / 43, 40 x 4096 65 / 59, bf16 69 / 59 (four groups half empty there).  max_rows is what a table has room for, since
+// the lengths are on the device: of 64 x 512 rows 32 us with a table of their size, 47 - 50 with one of 2048 rows or more, of
+// 1 x 257 rows 16 up to 32768 and 22 with 163840 (captured; bf16 32, 48, 13.5 and 20).
 static int attn_groups(int64_t seqs, int64_t rows, int64_t max_rows) {
   const double pairs = (double)seqs * rows * max_rows / LA_UNITS;  // query rows x cached rows of a CU
   return pairs < 32 * 1024 || rows <= 32 ? 1 : rows <= 64 ? 2 : 4;

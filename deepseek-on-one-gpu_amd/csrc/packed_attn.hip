@@ -5,10 +5,9 @@
 // rounded to bf16 for the matrix units (as inference/ops.py:179 rounds it).
 //
 // Bound: the matrix units and their power.  Two prompts of 50 and 950 rows behind 562 and
-// 7438 cached ones, 128 heads with rope keys: 618 GFLOP in 617 - 640 us, 0.98 PFLOP/s at 1.8
-// GHz (an 8192^3 product of the library reaches 1.2 on this card), the units busy 54 % of the
-// cycles; what a wave issues besides is nearly as long as its products.  Five prompts of 4099
-// rows together: 338 - 355 us, where starting and ending a block (15000 cycles) and its last,
+// 7438 cached ones, 128 heads with rope keys: 618 GFLOP in 617 - 675 us by card, 0.92 - 1.0 PFLOP/s at
+// 1.8 GHz (an 8192^3 product of the library reaches 1.2), the units busy 54 % of the cycles; what a wave issues besides is nearly as long as its products.  Five prompts of 4099
+// rows together: 332 - 355 us, where starting and ending a block (15000 cycles) and its last,
 // masked tiles weigh as much as a third of the products.  64 queries a wave: with 32 each
 // fragment read from LDS fed one product and the same two cases took 858 and 413 us.
 #include <algorithm>
@@ -77,8 +76,9 @@ AMLA_DEV PackedBlock find_block(const PackedParams &p, int tile) {
   return PackedBlock{-1, 0, 0, 0, 0};
 }
 
-// Tiles of 64 keys that one workgroup takes of a block: with few blocks their keys are split, so that all CUs have work and
-// no block is much longer than the others: total / 256, but not below PA_LEAST (2 us each; starting and joining take 10).
+// Tiles of 64 keys that one workgroup takes of a block, at most: with few blocks their keys are split, so that all CUs have
+// work and no block is much longer than the others: total / 256, but not below PA_LEAST (2 us each; starting and joining take
+// 10).  A block of more is split evenly, seven tiles into three and four.
 constexpr int PA_LEAST = 6;
 AMLA_DEV int split_tiles(const PackedParams &p) {
   const int lane = threadIdx.x & 63;

@@ -423,7 +423,10 @@ int amla_latent_cache_read(const amla_latent_cache *cache, int64_t rows, const i
  * out (seqs, seq_len, heads, 512) bf16, lse (seqs,
  * seq_len, heads) fp32 or NULL.  Any heads; the rows of one sequence are split
  * over workgroups whose sums meet in the workspace (16-byte aligned, scratch
- * only).  The size depends on cols and page_size of the cache, on nothing else of it. */
+ * only).  The size depends on cols and page_size of the cache, on nothing else of it.
+ * So does the choice of the kernel, with the batch and the heads, since the lengths
+ * are not known to the host: a table much wider than its sequences costs short ones
+ * up to half as much time again, and the last bits of the result go with the width. */
 int amla_latent_attention(const amla_latent_cache *cache, const void *q, int64_t seqs, int64_t seq_len, int64_t heads,
                           int64_t ldq_seq, int64_t ldq_token, int64_t ldq_head, const int32_t *lengths, float scale,
                           void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
