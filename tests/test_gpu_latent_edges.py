@@ -255,3 +255,24 @@ def test_the_mean_error_is_that_of_two_roundings(fp8, S, H, cols):
     for b in range(0, 60, 3):
         rms = (got[b:b + 3].double().cpu() - want).square().mean().sqrt() / want.square().mean().sqrt()
         assert rms <= 2.0 ** -8 * (2 / 3) ** 0.5, f"{b}: {rms.item():.5f}"
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("S,H,cols", KERNELS)
+def test_a_query_that_is_no_number_stays_alone(fp8, S, H, cols):
+    """NaN for it, the bits of a call without it for all others; an infinite one has its workgroup start over."""
+    g = torch.Generator().manual_seed(H + 3)
+    n, B = 400, 270 * 64 // min(H * S, 64)
+    cache, table, lengths, _ = _many(torch.randn(n, 512, generator=g, dtype=torch.float64), torch.randn(n, 64, generator=g, dtype=torch.float64),
+                                     fp8, B, g, cols)
+    q = (torch.randn(B, S, H, 576, generator=g) * 0.5).to(BF16)
+    run = lambda q: ops.latent_attention(to_dev(q), to_dev(cache), to_dev(table), to_dev(lengths), SCALE, return_lse=True)  # noqa: E731
+    want, want_lse = run(q)
+    bad = torch.zeros(B, S, H, dtype=torch.bool)
+    bad[1, 0, 0], bad[2, S - 1, H // 2:], bad[B - 1, 0, H - 1] = True, True, True
+    q[bad] = float("nan")
+    q[1, 0, 0], q[1, 0, 0, 7] = 0.0, float("inf")
+    print(f"[case] fp8={fp8} S={S} H={H}", flush=True)
+    got, lse = run(q)
+    assert torch.isnan(got.cpu()[bad]).all() and torch.isnan(lse.cpu()[bad]).all()
+    assert torch.equal(got.cpu()[~bad], want.cpu()[~bad]) and torch.equal(lse.cpu()[~bad], want_lse.cpu()[~bad])

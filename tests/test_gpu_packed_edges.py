@@ -138,3 +138,36 @@ def test_the_mean_error_is_that_of_two_roundings(form, H, new, past):
     want, _ = L.packed_attention(q, k, v, off, scale, koff, pe)
     rms = (got.double().cpu() - want).square().mean().sqrt() / want.square().mean().sqrt()
     assert rms <= 2.0 ** -8 * (2 / 3) ** 0.5, f"{rms.item():.5f}"
+
+
+@pytest.mark.parametrize("form,H,new,held", [("plain", 2, [40, 9, 300], [25, 0, 90]), ("mla", 2, [600, 3], [450, 0]), ("whole", 130, [300], [90])])
+def test_a_query_that_sees_no_key_and_is_no_number(form, H, new, held):
+    """More queries than keys: the first of a causal sequence see none, and give zeros whatever they hold."""
+    q, k, v, pe, off, koff, scale = _case(17, new, held, H, H, form)
+    clean, blind = q.clone(), torch.cat([torch.arange(n) < n - m for n, m in zip(new, held)])
+    q[blind] = float("nan")
+    q[blind.nonzero()[::2, 0]] = 0.0
+    q[blind.nonzero()[::2, 0], :, 5] = float("inf")
+    call = lambda q: ops.packed_attention(to_dev(q), to_dev(k), to_dev(v), to_dev(off), scale, k_offsets=to_dev(koff), k_pe=to_dev(pe),  # noqa: E731
+                                          return_lse=True)
+    print(f"[case] {form} {new} over {held}", flush=True)
+    got, lse = call(q)
+    want, want_lse = call(clean)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    assert (got.cpu()[blind] == 0).all() and (lse.cpu()[blind] == float("-inf")).all() and torch.isfinite(lse.cpu()[~blind]).all()
+
+
+@pytest.mark.parametrize("form,H,new,past", [("plain", 2, [40, 300], [0, 90]), ("mla", 4, [600], [0]), ("mla", 4, [20], [2000]), ("whole", 130, [300], [70])])
+def test_a_query_that_is_no_number_stays_alone(form, H, new, past):
+    """NaN for it, the bits of a call without it for all others, also where its block is done again."""
+    q, k, v, pe, off, koff, scale = _case(18, new, [a + b for a, b in zip(new, past)], H, H, form)
+    call = lambda q: ops.packed_attention(to_dev(q), to_dev(k), to_dev(v), to_dev(off), scale, k_offsets=to_dev(koff), k_pe=to_dev(pe),  # noqa: E731
+                                          return_lse=True)
+    want, want_lse = call(q)
+    bad = torch.zeros(sum(new), H, dtype=torch.bool)
+    bad[3, 1], bad[sum(new) - 1, 0], bad[sum(new) // 2, :] = True, True, True
+    q[bad] = float("nan")
+    print(f"[case] {form} {new} behind {past}", flush=True)
+    got, lse = call(q)
+    assert torch.isnan(got.cpu()[bad]).all() and torch.isnan(lse.cpu()[bad]).all()
+    assert torch.equal(got.cpu()[~bad], want.cpu()[~bad]) and torch.equal(lse.cpu()[~bad], want_lse.cpu()[~bad])
